@@ -81,7 +81,7 @@ struct Entry<R (*)(A...)> {
 
 #define JL_ENTRIES(X)                                                                                                                    \
   X(jl_rmsnorm) X(jl_rope_kv_write) X(jl_gemv) X(jl_gemm) X(jl_gemm_2cta) X(jl_decode_attn) X(jl_decode_attn_fused) X(jl_flash_prefill)  \
-  X(jl_prefill_attn_mma) X(jl_sample_full) X(jl_swiglu) X(jl_argmax)                                                                     \
+  X(jl_prefill_attn_mma) X(jl_sample_full) X(jl_swiglu) X(jl_argmax) X(jl_decode_attn_prefix) X(jl_prefill_attn_prefix) X(jl_logit_rules) \
   X(jl_embed_f32) X(jl_norm_f32) X(jl_postnorm_add) X(jl_headnorm_gate) X(jl_act_cast) X(jl_act_inplace) X(jl_linear_any)                \
   X(jl_linear_resident) X(jl_linear_exact) X(jl_linear_f32_pair_ws) X(jl_linear_f32_pair) X(jl_attn_prep) X(jl_attn_prep_ex)             \
   X(jl_attn_step) X(jl_attn_generic) X(jl_attn_generic_splits) X(jl_head_gate) X(jl_gla_scan) X(jl_gla_scan_exact) X(jl_gla_step)           \

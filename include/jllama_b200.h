@@ -564,6 +564,33 @@ int jl_mlstm_scan(const float* y, int ldy, int q_off, int k_off, int v_off, cons
 int jl_mlstm_finish(const float* o, const float* aux, const void* w, const float* gate, int ldg, void* out, int M, int H, int V,
                     float eps, int gate_act, int dtype, void* stream);
 
+/* Attention of rows whose group shares keys (several answers to one prompt, many questions to one document).  Rows b of group b / (B / groups) attend the
+ * shared keys [prefix_pad[g], prefix_len[g]) of prefix_k / prefix_v [groups][nkv][P][hd] (prefix_len == NULL: all P, prefix_pad == NULL: from 0) and their own
+ * keys [pad_left[b], ..] of k_cache / v_cache [B][nkv][T][hd], softmax over both together.  hd 64 or 128, nh / nkv 1, 2, 4 or 8; all tensors start at 16-byte
+ * boundaries.  `scratch` holds jl_prefix_attn_scratch_bytes(..) bytes whose first B nkv 32-bit words are zero before the first call (every call leaves them so);
+ * calls that may run at the same time need one each.  Slots that hold no key may hold anything.
+ *
+ * jl_decode_attn_prefix: one new token per row.  qkv [B, (nh + 2 nkv) hd] not rotated; the token takes slot *cache_len of the row's own cache (nothing is stored at
+ * *cache_len >= T) at rotary position (prefix_len - prefix_pad)[g] + *cache_len - pad_left[b]; its k and v are appended, out [B, nh hd].
+ * jl_prefill_attn_prefix: S tokens per row in slots start..start+S, k and v appended and q [B, S, nh, hd] rotated by the caller; causal in the own keys; a query in
+ * front of its row's pad_left gives zeros. */
+size_t jl_prefix_attn_scratch_bytes(int B, int S, int groups, int nh, int nkv, int hd, int P);
+int jl_decode_attn_prefix(const void* qkv, const void* prefix_k, const void* prefix_v, void* k_cache, void* v_cache, const float* cos_t, const float* sin_t,
+                          const int* cache_len, const int* pad_left, const int* prefix_len, const int* prefix_pad, void* scratch, size_t scratch_bytes, void* out,
+                          int B, int groups, int nh, int nkv, int hd, int P, int T, int max_pos, float scale, void* stream);
+int jl_prefill_attn_prefix(const void* q, const void* prefix_k, const void* prefix_v, const void* k_cache, const void* v_cache, const int* pad_left,
+                           const int* prefix_len, const int* prefix_pad, void* scratch, size_t scratch_bytes, void* out, int B, int S, int groups, int nh, int nkv,
+                           int hd, int P, int T, int start, float scale, void* stream);
+
+/* The rules of a request on its logits, before selection: out[b, v] (fp32, pitch ldo; may be logits itself when that is fp32) from logits [B, V] (dtype 0 fp32, 1 bf16,
+ * 2 fp16; pitch ld).  Tokens that occur in tokens[b, starts[b] .. lengths[b]) (pitch ldt, T columns): x > 0 ? x / rep : x rep; n occurrences from position prompts[b]
+ * on: x - freq n - pres.  Then the biases of the entries (ids outside the vocabulary: unused; the same id twice: both, in order), then -infinity where bit v % 32 of
+ * word v / 32 of allowed[b] is zero.  starts / lengths / prompts: one number per row (.._n = B) or for all (1), NULL = 0 / T / 0; rep / freq / pres: [B], or
+ * NULL and the scalar beside; ldb / lda 0: one list / mask for all rows. */
+int jl_logit_rules(const void* logits, int dtype, int B, int V, int ld, float* out, int ldo, const int* tokens, int T, int ldt, const int* starts, int starts_n,
+                   const int* lengths, int lengths_n, const int* prompts, int prompts_n, const float* rep, float rep1, const float* freq, float freq1,
+                   const float* pres, float pres1, const int* bias_ids, const float* bias, int n_bias, int ldb, const void* allowed, int lda, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -52,6 +52,10 @@ _SIGNATURES = {
     "jl_argmax": (i32, [fp, i32, i32, i32, i32, fp, ip, vp]),
     "jl_topk": (i32, [fp, i32, i32, i32, i32, i32, fp, ip, vp]),
     "jl_sample": (i32, [fp, ip, i32, i32, sz, i32, i32, f32, f32, u64, ip, ip, vp]),
+    "jl_prefix_attn_scratch_bytes": (sz, [i32] * 7),
+    "jl_decode_attn_prefix": (i32, [vp, vp, vp, vp, vp, fp, fp, ip, ip, ip, ip, vp, sz, vp] + [i32] * 8 + [f32, vp]),
+    "jl_prefill_attn_prefix": (i32, [vp, vp, vp, vp, vp, ip, ip, ip, vp, sz, vp] + [i32] * 9 + [f32, vp]),
+    "jl_logit_rules": (i32, [vp, i32, i32, i32, i32, fp, i32, ip, i32, i32, ip, i32, ip, i32, ip, i32, fp, f32, fp, f32, fp, f32, ip, fp, i32, i32, vp, i32, vp]),
     "jl_decode_advance": (i32, [ip, ip, ip, ip, i32, i32, i32, i32, ip, ip, ip, ip, vp]),
 }
 

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import math
 import os
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
@@ -350,6 +350,268 @@ def prefill_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     _lib.check(_lib.lib().jl_flash_prefill(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _p(cache_len),
                                            _p(pad_left), out.data_ptr(), B, S, nh, nkv, hd, T, start,
                                            1.0 / math.sqrt(hd), _stream()), "jl_flash_prefill")
+    return out
+
+
+# --------------------------------------------------------------------------- attention over a prefix that the rows of a group share
+def _here(t: torch.Tensor, who: str) -> None:
+    """Launches go to the current device's stream: tensors of another device are refused."""
+    if _get_device is not None and t.device.index is not None and t.device.index != _get_device():
+        raise ValueError(f"{who}: tensors on {t.device}, current device cuda:{_get_device()}")
+
+
+def _index(t: Optional[torch.Tensor], n: Tuple[int, ...], name: str, device: torch.device) -> Optional[torch.Tensor]:
+    if t is not None and (t.dtype != torch.int32 or t.numel() not in n or not t.is_contiguous() or t.device != device):
+        raise ValueError(f"{name} must be int32, contiguous, on {device}, of {' or '.join(map(str, n))} elements (got {t.dtype}, {tuple(t.shape)}, {t.device})")
+    return t
+
+
+def _prefix_shapes(who: str, B: int, nkv: int, hd: int, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
+                   ) -> Tuple[int, int, int]:
+    """(groups, P, T) of the two caches, or a refusal."""
+    if prefix_k.dim() != 4 or k_cache.dim() != 4 or prefix_v.shape != prefix_k.shape or v_cache.shape != k_cache.shape:
+        raise ValueError(f"{who}: keys and values are [groups, nkv, P, hd] and [B, nkv, T, hd]")
+    groups, P, T = prefix_k.shape[0], prefix_k.shape[2], k_cache.shape[2]
+    if tuple(prefix_k.shape) != (groups, nkv, P, hd) or tuple(k_cache.shape) != (B, nkv, T, hd) or groups < 1 or B % groups or P < 1 or T < 1:
+        raise ValueError(f"{who}: prefix {tuple(prefix_k.shape)} and own keys {tuple(k_cache.shape)} for {B} rows, {nkv} key heads of {hd}")
+    if k_cache.is_cuda:
+        for name, t in (("prefix_k", prefix_k), ("prefix_v", prefix_v), ("k_cache", k_cache), ("v_cache", v_cache)):
+            _bf16c(t, name)
+            if t.device != k_cache.device:
+                raise ValueError(f"{who}: {name} on {t.device}, k_cache on {k_cache.device}")
+        _here(k_cache, who)
+    return groups, P, T
+
+
+def _prefix_counts(prefix_len: Optional[torch.Tensor], prefix_pad: Optional[torch.Tensor], groups: int, P: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """First and last + 1 shared key of every group (CPU path)."""
+    lo = prefix_pad.long().clamp(min=0) if prefix_pad is not None else torch.zeros(groups, dtype=torch.long)
+    hi = prefix_len.long().clamp(max=P) if prefix_len is not None else torch.full((groups,), P, dtype=torch.long)
+    return lo, hi
+
+
+def _prefix_attn_ref(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                     pad_left: Optional[torch.Tensor], lo: torch.Tensor, hi: torch.Tensor) -> torch.Tensor:
+    """q [B, S, nh, hd] of tokens in `slots` [S] of their rows' own caches -> [B, S, nh·hd] in q's type; one softmax over shared and own keys."""
+    B, S, nh, hd = q.shape
+    groups, nkv, P, _ = prefix_k.shape
+    T = k_cache.shape[2]
+    row_group = torch.arange(B) // (B // groups)
+    at = torch.arange(P)[None]
+    shared = ((at >= lo[:, None]) & (at < hi[:, None]))[row_group]                                          # [B, P]
+    own = torch.arange(T)[None, None] <= slots[None, :, None]
+    own = own.expand(B, S, T)
+    if pad_left is not None:
+        own = own & (torch.arange(T)[None, None] >= pad_left.long()[:, None, None])
+    seen = torch.cat([shared[:, None].expand(B, S, P), own], -1)
+    live = seen.any(1)                                                                                      # slots that hold no key may hold anything
+    k = torch.cat([prefix_k[row_group], k_cache], 2).float()
+    v = torch.cat([prefix_v[row_group], v_cache], 2).float().masked_fill(~live[:, None, :, None], 0.0)
+    k, v = k.repeat_interleave(nh // nkv, 1), v.repeat_interleave(nh // nkv, 1)
+    s = torch.einsum("bshd,bhkd->bhsk", q.float(), k) / math.sqrt(hd)
+    s = s.masked_fill(~seen[:, None], float("-inf"))
+    m = s.amax(-1, keepdim=True)
+    w = (s - torch.where(m == float("-inf"), torch.zeros_like(m), m)).exp()
+    total = w.sum(-1, keepdim=True)
+    o = torch.einsum("bhsk,bhkd->bshd", w / torch.where(total == 0, torch.ones_like(total), total), v)
+    return o.masked_fill(~own.any(-1)[..., None, None], 0.0).to(q.dtype).reshape(B, S, nh * hd)
+
+
+def prefix_attn_scratch(B: int, S: int, groups: int, nh: int, nkv: int, hd: int, prefix: int, device: torch.device) -> Optional[torch.Tensor]:
+    """Workspace of `decode_attn_prefix` (S = 1) or `prefill_attn_prefix` for B rows in `groups` groups over prefixes of up to `prefix` slots.  One may serve all
+    layers and steps of a stream of calls; calls that can run at the same time (two streams, two captured graphs) need one each."""
+    if torch.device(device).type != "cuda":
+        return None
+    n = int(_lib.lib().jl_prefix_attn_scratch_bytes(B, S, groups, nh, nkv, hd, prefix))
+    if n == 0:
+        raise ValueError(f"prefix_attn_scratch: {B} rows of {S} tokens in {groups} groups, {nh} / {nkv} heads of {hd}, prefix {prefix}")
+    t = torch.empty((n + 15) // 16 * 4, dtype=torch.int32, device=device)
+    t[:min(B * nkv, t.numel())].zero_()                       # tickets
+    return t
+
+
+def decode_attn_prefix(qkv: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cos: torch.Tensor,
+                       sin: torch.Tensor, cache_len: torch.Tensor, pad_left: Optional[torch.Tensor], prefix_len: Optional[torch.Tensor],
+                       prefix_pad: Optional[torch.Tensor], nh: int, nkv: int, hd: int, *, scratch: Optional[torch.Tensor] = None,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`decode_attn_fused` where the rows of a group share the keys in front of their own: RoPE + append to the row's own cache + attention over both.
+
+    qkv [B, (nh+2nkv)·hd] is the raw projection of the new token of every row; prefix_k / prefix_v [groups, nkv, P, hd] hold every group's shared keys in slots
+    [prefix_pad[g], prefix_len[g]) (int32 [groups]; None: all P, from 0), read once for the B / groups rows of the group (rows of a group are neighbours);
+    k_cache / v_cache [B, nkv, T, hd] the rows' own keys from pad_left[b] (int32 [B] or None) on.  The new token takes slot cache_len (int32 [1], device; nothing is
+    stored once the cache is full) at rotary position (prefix_len - prefix_pad)[g] + cache_len - pad_left[b].  -> [B, nh·hd]."""
+    who = "decode_attn_prefix"
+    B = qkv.shape[0]
+    if qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
+        raise ValueError(f"{who}: qkv {tuple(qkv.shape)} for {nh} + 2 x {nkv} heads of {hd}")
+    groups, P, T = _prefix_shapes(who, B, nkv, hd, prefix_k, prefix_v, k_cache, v_cache)
+    _index(cache_len, (1,), "cache_len", qkv.device); _index(pad_left, (B,), "pad_left", qkv.device)
+    _index(prefix_len, (groups,), "prefix_len", qkv.device); _index(prefix_pad, (groups,), "prefix_pad", qkv.device)
+    if not qkv.is_cuda:
+        lo, hi = _prefix_counts(prefix_len, prefix_pad, groups, P)
+        slot = min(int(cache_len.item()), T)
+        x = qkv.view(B, nh + 2 * nkv, hd)
+        pos = (hi - lo).clamp(min=0).repeat_interleave(B // groups) + slot
+        if pad_left is not None:
+            pos = pos - pad_left.long()
+        pos = pos.clamp(0, cos.shape[0] - 1)
+        c, s = cos[pos][:, None], sin[pos][:, None]
+        re, im = x[:, :nh + nkv, 0::2].float(), x[:, :nh + nkv, 1::2].float()
+        rot = torch.stack([re * c - im * s, re * s + im * c], -1).flatten(-2)
+        kn, vn = rot[:, nh:].to(k_cache.dtype)[:, :, None], x[:, nh + nkv:].to(v_cache.dtype)[:, :, None]
+        if slot < T:
+            k_cache[:, :, slot:slot + 1], v_cache[:, :, slot:slot + 1] = kn, vn
+        pad = torch.clamp(pad_left.long(), max=slot) if pad_left is not None else None        # the new token sees itself
+        o = _prefix_attn_ref(rot[:, None, :nh], prefix_k, prefix_v, torch.cat([k_cache[:, :, :slot], kn], 2), torch.cat([v_cache[:, :, :slot], vn], 2),
+                             torch.tensor([slot]), pad, lo, hi)
+        return o.view(B, nh * hd).to(qkv.dtype)
+    _bf16c(qkv, "qkv")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.shape[1] != hd // 2 or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError(f"{who}: cos/sin tables are fp32 [positions, {hd // 2}]")
+    if scratch is None:
+        scratch = prefix_attn_scratch(B, 1, groups, nh, nkv, hd, P, qkv.device)
+    if out is None:
+        out = qkv.new_empty((B, nh * hd))
+    else:
+        _bf16c(out, "out")
+        if out.numel() != B * nh * hd:
+            raise ValueError(f"{who}: out {tuple(out.shape)} for {B} x {nh * hd}")
+    _lib.check(_lib.lib().jl_decode_attn_prefix(qkv.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cos.data_ptr(),
+                                                sin.data_ptr(), cache_len.data_ptr(), _p(pad_left), _p(prefix_len), _p(prefix_pad), scratch.data_ptr(),
+                                                scratch.numel() * scratch.element_size(), out.data_ptr(), B, groups, nh, nkv, hd, P, T, cos.shape[0],
+                                                1.0 / math.sqrt(hd), _stream()), "jl_decode_attn_prefix")
+    return out
+
+
+def prefill_attn_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, start: int, S: int,
+                        pad_left: Optional[torch.Tensor], prefix_len: Optional[torch.Tensor], prefix_pad: Optional[torch.Tensor], *,
+                        scratch: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`prefill_attn` where the rows of a group share the keys in front of their own.  q [B, S, nh, hd] rotated, the S new tokens of every row appended to its own
+    cache in slots start..start+S; shared keys as in `decode_attn_prefix` (every query sees all of its group's), own keys [pad_left[b], slot of the query].  Queries
+    in front of pad_left give zeros.  -> [B, S, nh·hd]."""
+    who = "prefill_attn_prefix"
+    if q.dim() != 4 or q.shape[1] != S:
+        raise ValueError(f"{who}: q {tuple(q.shape)} is not [B, {S}, heads, head_dim]")
+    B, _, nh, hd = q.shape
+    nkv = k_cache.shape[1]
+    groups, P, T = _prefix_shapes(who, B, nkv, hd, prefix_k, prefix_v, k_cache, v_cache)
+    if start < 0 or start + S > T:
+        raise ValueError(f"{who}: slots {start}..{start + S} of a cache of {T}")
+    _index(pad_left, (B,), "pad_left", q.device); _index(prefix_len, (groups,), "prefix_len", q.device); _index(prefix_pad, (groups,), "prefix_pad", q.device)
+    if not q.is_cuda:
+        lo, hi = _prefix_counts(prefix_len, prefix_pad, groups, P)
+        return _prefix_attn_ref(q, prefix_k, prefix_v, k_cache[:, :, :start + S], v_cache[:, :, :start + S], start + torch.arange(S), pad_left, lo, hi)
+    _bf16c(q, "q")
+    if scratch is None:
+        scratch = prefix_attn_scratch(B, max(S, 1), groups, nh, nkv, hd, P, q.device)
+    if out is None:
+        out = q.new_empty((B, S, nh * hd))
+    else:
+        _bf16c(out, "out")
+        if out.numel() != B * S * nh * hd:
+            raise ValueError(f"{who}: out {tuple(out.shape)} for {B} x {S} x {nh * hd}")
+    _lib.check(_lib.lib().jl_prefill_attn_prefix(q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _p(pad_left),
+                                                 _p(prefix_len), _p(prefix_pad), scratch.data_ptr(), scratch.numel() * scratch.element_size(), out.data_ptr(), B, S,
+                                                 groups, nh, nkv, hd, P, T, start, 1.0 / math.sqrt(hd), _stream()), "jl_prefill_attn_prefix")
+    return out
+
+
+# --------------------------------------------------------------------------- the rules of a request on its logits
+def _constrain_ref(x: torch.Tensor, tokens: Optional[torch.Tensor], starts: torch.Tensor, lengths: torch.Tensor, prompts: torch.Tensor, rep: torch.Tensor,
+                   freq: torch.Tensor, pres: torch.Tensor, bias_ids: Optional[torch.Tensor], bias: Optional[torch.Tensor], allowed: Optional[torch.Tensor]) -> torch.Tensor:
+    x = x.float().clone()
+    B, V = x.shape
+    for b in range(B):
+        if tokens is not None:
+            lo, hi, cut = max(int(starts[b]), 0), min(int(lengths[b]), tokens.shape[1]), int(prompts[b])
+            said = tokens[b].long()
+            for first, part in ((True, said[lo:hi]), (False, said[max(lo, cut):hi])):
+                ids, n = torch.unique(part[(part >= 0) & (part < V)], return_counts=True)
+                if first:
+                    x[b, ids] = torch.where(x[b, ids] > 0, x[b, ids] / rep[b], x[b, ids] * rep[b])
+                else:
+                    x[b, ids] = x[b, ids] - freq[b] * n.float() - pres[b]
+        if bias_ids is not None:
+            ids, val = (t[b if t.shape[0] > 1 else 0] for t in (bias_ids, bias))
+            ok = (ids >= 0) & (ids < V)
+            x[b] += torch.zeros(V).index_add_(0, ids[ok].long(), val[ok])
+        if allowed is not None:
+            words = allowed[b if allowed.shape[0] > 1 else 0].long() & 0xFFFFFFFF
+            bits = (words[:, None] >> torch.arange(32)) & 1
+            x[b, bits.view(-1)[:V] == 0] = float("-inf")
+    return x
+
+
+_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                     prompt_lengths: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None, repetition: Union[float, torch.Tensor, None] = None,
+                     frequency: Union[float, torch.Tensor, None] = None, presence: Union[float, torch.Tensor, None] = None,
+                     bias_ids: Optional[torch.Tensor] = None, bias_values: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The rules of a request on the logits of a step, ahead of `argmax` / `sample_full`: fp32 [B, V] from logits [B, V] (fp32, bf16 or fp16; any row pitch).
+
+    tokens int32 [B, T]: row b has said tokens[b, starts[b] : lengths[b]] (int32 [B], or [1] for all rows; None: 0 and T), the part from prompt_lengths[b] on (None:
+    all of it) as its answer.  Ids outside the vocabulary are passed over.  For a token that occurs: x > 0 ? x / repetition : x · repetition; with n occurrences in
+    the answer, n > 0: x - frequency · n - presence.  (A number, or fp32 [B]; None: off.  repetition > 0.)  Then x + bias_values of the entries of bias_ids
+    (int32 / fp32 [B, n], or [1, n] for all rows; an id outside the vocabulary is no entry, the same id twice adds both), then -inf where bit v % 32 of word v // 32
+    of allowed (int32 [B, words] or [1, words]) is zero.  A row whose mask allows nothing is -inf throughout.  `out` may be `logits` itself when that is fp32."""
+    who = "constrain_logits"
+    if logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError(f"{who}: logits are [B, V], fp32, bf16 or fp16, with dense rows (got {logits.dtype}, {tuple(logits.shape)}, strides {logits.stride()})")
+    B, V = logits.shape
+    dev = logits.device
+    if tokens is None and any(t is not None for t in (lengths, prompt_lengths, starts)):
+        raise ValueError(f"{who}: row bounds without tokens")
+    T = 0
+    if tokens is not None:
+        if tokens.dim() != 2 or tokens.dtype != torch.int32 or tokens.shape[0] != B or (tokens.shape[1] > 1 and tokens.stride(1) != 1) or tokens.device != dev:
+            raise ValueError(f"{who}: tokens are int32 [{B}, T] with dense rows on {dev} (got {tokens.dtype}, {tuple(tokens.shape)}, {tokens.device})")
+        T = tokens.shape[1]
+        _index(lengths, (B, 1), "lengths", dev); _index(prompt_lengths, (B, 1), "prompt_lengths", dev); _index(starts, (B, 1), "starts", dev)
+    scalars, rows = [], []
+    for name, v, off in (("repetition", repetition, 1.0), ("frequency", frequency, 0.0), ("presence", presence, 0.0)):
+        if isinstance(v, torch.Tensor):
+            if v.dtype != torch.float32 or v.shape != (B,) or not v.is_contiguous() or v.device != dev:
+                raise ValueError(f"{who}: {name} is a number or fp32 [{B}] on {dev} (got {v.dtype}, {tuple(v.shape)}, {v.device})")
+            rows.append(v); scalars.append(off)
+        else:
+            rows.append(None); scalars.append(off if v is None else float(v))
+            if name == "repetition" and not scalars[-1] > 0.0:
+                raise ValueError(f"{who}: repetition {v} is not above zero")
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError(f"{who}: bias_ids and bias_values come together")
+    n_bias = 0
+    if bias_ids is not None:
+        if bias_ids.dtype != torch.int32 or bias_values.dtype != torch.float32 or bias_ids.dim() != 2 or bias_ids.shape != bias_values.shape \
+                or bias_ids.shape[0] not in (1, B) or not (bias_ids.is_contiguous() and bias_values.is_contiguous()) or bias_ids.device != dev or bias_values.device != dev:
+            raise ValueError(f"{who}: biases are int32 and fp32 [{B} or 1, n] on {dev} (got {tuple(bias_ids.shape)}, {tuple(bias_values.shape)})")
+        n_bias = bias_ids.shape[1]
+    if allowed is not None and (allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[0] not in (1, B) or allowed.shape[1] < (V + 31) // 32
+                                or not allowed.is_contiguous() or allowed.device != dev):
+        raise ValueError(f"{who}: allowed is int32 [{B} or 1, {(V + 31) // 32} or more words] on {dev} (got {allowed.dtype}, {tuple(allowed.shape)})")
+    if out is not None and (out.dtype != torch.float32 or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or out.device != dev):
+        raise ValueError(f"{who}: out is fp32 {tuple(logits.shape)} with dense rows on {dev} (got {out.dtype}, {tuple(out.shape)}, {out.device})")
+    if not logits.is_cuda:
+        def full(t: Optional[torch.Tensor], off: Union[int, float]) -> torch.Tensor:
+            return torch.full((B,), off) if t is None else t.reshape(-1).expand(B)
+        y = _constrain_ref(logits, tokens, full(starts, 0), full(lengths, T), full(prompt_lengths, 0), *(full(r, s) for r, s in zip(rows, scalars)),
+                           bias_ids if n_bias else None, bias_values, allowed)
+        return y if out is None else out.copy_(y)
+    _here(logits, who)
+    if out is None:
+        out = logits.new_empty((B, V), dtype=torch.float32)
+
+    def count(t: Optional[torch.Tensor]) -> int:
+        return 0 if t is None else t.numel()
+
+    _lib.check(_lib.lib().jl_logit_rules(
+        logits.data_ptr(), _LOGIT_TYPES[logits.dtype], B, V, logits.stride(0) if B > 1 else V, out.data_ptr(), out.stride(0) if B > 1 else V, _p(tokens), T,
+        tokens.stride(0) if tokens is not None and B > 1 else T, _p(starts), count(starts), _p(lengths), count(lengths), _p(prompt_lengths), count(prompt_lengths),
+        _p(rows[0]), scalars[0], _p(rows[1]), scalars[1], _p(rows[2]), scalars[2], _p(bias_ids), _p(bias_values), n_bias,
+        n_bias if n_bias and bias_ids.shape[0] > 1 else 0, _p(allowed), allowed.shape[1] if allowed is not None and allowed.shape[0] > 1 else 0, _stream()),
+        "jl_logit_rules")
     return out
 
 
