@@ -27,16 +27,51 @@
 
 namespace jl {
 
-constexpr int PX_BM = 128, PX_BN = 64, PX_THREADS = 192;
+constexpr int PX_BM = 128, PX_BN = 64, PX_THREADS = 352;
 constexpr float PX_RESCALE = 8.0f;                                 // log2 units
-constexpr uint32_t PX_BARS = 256;                                  // barriers and the address of the TMEM columns
 
-template <int HD> struct PxTile {
+// PAIR: two tiles of queries per CTA, each with its own softmax warps, over the same keys; else one tile whose keys the two sets of softmax warps take in turn.
+template <int HD, bool ROTATE, bool PAIR> struct PxTile {
   static constexpr int HALVES = HD / 64;
-  static constexpr uint32_t Q_HALF = PX_BM * 128, Q = HALVES * Q_HALF;       // bytes
-  static constexpr uint32_t KV_HALF = PX_BN * 128, SLOT = HALVES * KV_HALF;
-  static constexpr uint32_t TMEM_COLS = 256;
+  static constexpr uint32_t Q_HALF = PX_BM * 128, Q = HALVES * Q_HALF;       // bytes of a tile of queries (hi or lo)
+  static constexpr int NQ = ROTATE ? 2 : 1;                                  // hi, lo
+  static constexpr uint32_t QS = (PAIR ? 2 : 1) * NQ * Q;
+  static constexpr uint32_t KV_HALF = PX_BN * 128, SLOT = 2 * HALVES * KV_HALF;        // a tile of keys and its values
+  static constexpr uint32_t SMALL = 512 + (PAIR ? 0 : 2048);                 // barriers, the address of the TMEM columns; (m, l) of 2 x 128 rows
+  static constexpr int FIT = (int)((227 * 1024 - 1024 - SMALL - QS) / SLOT);
+  static constexpr int SLOTS = FIT < 8 ? FIT : 8;                            // tiles in flight (96 KB or more; a memory latency needs about 50 per SM)
+  static constexpr uint32_t SMEM = QS + SLOTS * SLOT + SMALL + 1024;         // (1024: alignment of the base)
+  static_assert(SLOTS >= 3 && SMEM <= 227 * 1024, "a tile ahead of the products");
 };
+
+// Two fp32 numbers at once (fma.rn.f32x2 and add.rn.f32x2: one issue slot for both).
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 f2(float a, float b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void f2_get(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+// the larger of three, NaN if one is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+
+// 2^a, 2^b without the special-function unit: x = n + f with n the nearest whole number (added to 1.5 2^23 it stands in the last bits of the sum), 2^f on
+// [-1/2, 1/2] by the cubic of least relative error among those with p(0) = 1 (1.0e-4; what it stands in for is rounded to 2^-9), n added to the exponent.  From
+// -127 down the result is 0 (p = 1 there, and its exponent 127); a, b below 2^22 and not NaN.
+__device__ __forceinline__ void exp2_pair(F2 x, float& a, float& b) {
+  f2_get(x, a, b);
+  x = f2(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
+  const F2 t = f2_add(x, f2(12582912.0f, 12582912.0f));
+  const F2 n = f2_add(t, f2(-12582912.0f, -12582912.0f));
+  const F2 f = f2_fma(n, f2(-1.0f, -1.0f), x);
+  F2 p = f2_fma(f, f2(0.05500906f, 0.05500906f), f2(0.24221097f, 0.24221097f));
+  p = f2_fma(p, f, f2(0.6932829f, 0.6932829f));
+  p = f2_fma(p, f, f2(1.0f, 1.0f));
+  float ta, tb;
+  f2_get(t, ta, tb);
+  f2_get(p, a, b);
+  a = __int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23));
+  b = __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23));
+}
+constexpr int PX_POLY = 4;          // of 16 pairs of exponentials, how many run on the FMA units
 
 struct PxParams {
   const __nv_bfloat16* q; int ldq;  // token t, head h at q + t · ldq + h · HD
@@ -44,61 +79,67 @@ struct PxParams {
   const int* prefix_len; const int* prefix_pad; const int* pad_left;
   __nv_bfloat16* out;
   float* o_part; float2* ml_part;   // [tokens · nh][splits]: written (partial) or joined (own keys behind a launch over the shared ones)
-  int S, rows, nh, nkv, P, T, start;
+  int S, rows, nh, nkv, gs, P, T, start;      // gs: log2 of the query heads per key head
   int shared, own, partial;         // which keys this launch visits; whether it leaves partial triples or the result
-  int smem;                         // bytes of dynamic shared memory
-  int splits, join, slots;          // splits of the shared keys in this launch; triples per (token, head) that the last step joins; tiles of the ring
+  int splits, join;                 // splits of the shared keys in this launch; triples per (token, head) that the last step joins
   float scale_log2;
 };
 
-template <int HD, bool ROTATE>
-__global__ void __launch_bounds__(256, 2)        // 256: caps registers at 128, so that two six-warp CTAs (allocated as eight) fit
+template <int HD, bool ROTATE, bool PAIR>
+__global__ void __launch_bounds__(PX_THREADS, 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv,
                    const __grid_constant__ CUtensorMap tm_ok, const __grid_constant__ CUtensorMap tm_ov, const PxParams p) {
-  using Tile = PxTile<HD>;
-  constexpr int HALVES = Tile::HALVES;
-  constexpr int NQ = ROTATE ? 2 : 1;             // hi, lo
+  using Tile = PxTile<HD, ROTATE, PAIR>;
+  constexpr int HALVES = Tile::HALVES, NQ = Tile::NQ, SLOTS = Tile::SLOTS;
   extern __shared__ __align__(1024) uint8_t px_smem[];
   const uint32_t raw = tc::smem_u32(px_smem);
   const uint32_t base = (raw + 1023u) & ~1023u;  // the 128-byte swizzle counts rows from 1024-byte boundaries
-  const uint32_t sQ = base, ring = base + NQ * Tile::Q;
-  const uint32_t bars = ring + p.slots * Tile::SLOT;
-  const uint32_t q_full = bars, p_full = bars + 8, o_full = bars + 16;
-  auto s_full = [&](int s) { return bars + 24 + 8u * s; };
-  auto slot_full = [&](int s) { return bars + 48 + 16u * s; };
-  auto slot_empty = [&](int s) { return bars + 56 + 16u * s; };
-  const uint32_t tmem_slot = bars + 40;
-  if (bars + PX_BARS > raw + p.smem) __trap();   // dynamic shared memory less aligned than budgeted
+  const uint32_t sQ = base, ring = base + Tile::QS, small = ring + SLOTS * Tile::SLOT;
+  const uint32_t q_full = small, tmem_slot = small + 8;
+  auto p_full = [&](int w, int i) { return small + 16 + 16u * w + 8u * (i & 1); };       // probabilities of a tile
+  auto o_last = [&](int w, int i) { return small + 80 + 16u * w + 8u * (i & 1); };       // the last product but one, the last (one phase each)
+  const uint32_t started = small + 120;                                // PAIR: the first set is through its first softmax
+  auto s_full = [&](int w, int i) { return small + 48 + 16u * w + 8u * (i & 1); };       // scores of a tile
+  auto slot_full = [&](int s) { return small + 128 + 16u * s; };
+  auto slot_empty = [&](int s) { return small + 136 + 16u * s; };
+  static_assert(128 + 16 * SLOTS <= 512, "barriers in front of the rows' statistics");
+  float2* s_ml = reinterpret_cast<float2*>(px_smem + (small + 512 - raw));       // [2][128]
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(px_smem + (tmem_slot - raw));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = p.nh / p.nkv;
-  // z: group (shared keys alone) or row; y: key head; x: query tile, and split for partial results
+  const int G = 1 << p.gs;
+  // z: group (shared keys alone) or row; y: key head; x: query tile (or pair), and split for partial results
   const int kvh = blockIdx.y, z = blockIdx.z;
   const int qt = (int)(gridDim.x / p.splits) - 1 - (int)blockIdx.x / p.splits;      // longest first
   const int split = blockIdx.x % p.splits;
   const int unit_tokens = p.own ? p.S : p.rows * p.S;             // tokens whose queries this launch packs together
   const int token0 = z * unit_tokens;
-  const int q0 = qt * PX_BM, n_rows = min(PX_BM, unit_tokens * G - q0);
+  const int q0 = qt * (PAIR ? 2 * PX_BM : PX_BM), n_rows = min(PAIR ? 2 * PX_BM : PX_BM, unit_tokens * G - q0);
   const int group = p.own ? z / p.rows : z;
+  const bool two = !PAIR || n_rows > PX_BM;                       // the second set of softmax warps has work
 
   if (warp == 0 && lane == 0) {
     if (p.shared) { tc::prefetch_tensormap(&tm_pk); tc::prefetch_tensormap(&tm_pv); }
     if (p.own) { tc::prefetch_tensormap(&tm_ok); tc::prefetch_tensormap(&tm_ov); }
   }
   if (warp == 1 && lane == 0) {
-    tc::mbar_init(q_full, 4); tc::mbar_init(p_full, 4); tc::mbar_init(o_full, 1);
-    tc::mbar_init(s_full(0), 1); tc::mbar_init(s_full(1), 1);
-    for (int s = 0; s < p.slots; ++s) { tc::mbar_init(slot_full(s), 1); tc::mbar_init(slot_empty(s), 1); }
+    tc::mbar_init(q_full, 8);
+    tc::mbar_init(started, 1);
+    const int users = PAIR && two ? 2 : 1;                        // products that read a tile
+    for (int w = 0; w < 2; ++w) {
+      tc::mbar_init(p_full(w, 0), 4); tc::mbar_init(p_full(w, 1), 4); tc::mbar_init(o_last(w, 0), 1); tc::mbar_init(o_last(w, 1), 1);
+      tc::mbar_init(s_full(w, 0), 1); tc::mbar_init(s_full(w, 1), 1);
+    }
+    for (int s = 0; s < SLOTS; ++s) { tc::mbar_init(slot_full(s), 1); tc::mbar_init(slot_empty(s), users); }
     tc::fence_barrier_init();
   }
-  if (warp == 0) tc::tmem_alloc(tmem_slot, Tile::TMEM_COLS);
+  if (warp == 0) tc::tmem_alloc(tmem_slot, 512);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot_ptr;
-  auto tS = [&](int j) { return tmem + (uint32_t)(j & 1) * 64u; };     // score tile j, afterwards its probabilities
-  const uint32_t tO = tmem + 128;
+  auto tS = [&](int w, int i) { return tmem + (uint32_t)w * 256u + (uint32_t)(i & 1) * 64u; };   // scores of tile i of set w, afterwards its probabilities
+  auto tO = [&](int w) { return tmem + (uint32_t)w * 256u + 128u; };
 
   pdl_wait();
   pdl_launch_dependents();
@@ -113,280 +154,360 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
     s_lo = g_lo + min(split * chunk, n);
     s_hi = g_lo + min((split + 1) * chunk, n);
   }
-  const int pad = p.pad_left ? max(p.pad_left[p.own ? z : 0], 0) : 0;  // (own keys only; the one-token form reads the rows' pads itself)
+  const int pad = p.own && p.pad_left ? max(p.pad_left[z], 0) : 0;
   if (p.own) {
     o_lo = pad;
-    o_hi = max(p.start + (q0 + n_rows - 1) / G + 1, o_lo);             // slot of the tile's last token: its last key
+    o_hi = max(p.start + ((q0 + n_rows - 1) >> p.gs) + 1, o_lo);             // slot of the tile's last token: its last key
   }
   const int n_shared = (s_hi - s_lo + PX_BN - 1) / PX_BN, n_tiles = n_shared + (o_hi - o_lo + PX_BN - 1) / PX_BN;
+  // set w's tile i is tile number i (PAIR) or 2 i + w of the keys
+  auto tiles_of = [&](int w) { return PAIR ? (w == 0 || two ? n_tiles : 0) : (n_tiles + 1 - w) / 2; };
+  auto tile_at = [&](int w, int i) { return PAIR ? i : 2 * i + w; };
 
   if (warp == 0) {
     if (lane == 0) {
       int sl = 0;
       uint32_t ph = 1;
-      for (int idx = 0; idx < 2 * n_tiles; ++idx) {                    // K_0, V_0, K_1, V_1, ...
-        const int j = idx >> 1;
+      for (int j = 0; j < n_tiles; ++j) {
         const bool mine = j >= n_shared;
-        const CUtensorMap* m = (idx & 1) ? (mine ? &tm_ov : &tm_pv) : (mine ? &tm_ok : &tm_pk);
         const int key0 = mine ? o_lo + (j - n_shared) * PX_BN : s_lo + j * PX_BN;
         const int head = (mine ? z : group) * p.nkv + kvh;
+        const CUtensorMap* mk = mine ? &tm_ok : &tm_pk;
+        const CUtensorMap* mv = mine ? &tm_ov : &tm_pv;
         tc::mbar_wait(slot_empty(sl), ph);
         tc::mbar_expect_tx(slot_full(sl), Tile::SLOT);
 #pragma unroll
+        for (int h = 0; h < HALVES; ++h) tc::tma_load_3d(ring + sl * Tile::SLOT + h * Tile::KV_HALF, mk, slot_full(sl), 64 * h, key0, head, tc::EVICT_NORMAL);
+#pragma unroll
         for (int h = 0; h < HALVES; ++h)
-          tc::tma_load_3d(ring + sl * Tile::SLOT + h * Tile::KV_HALF, m, slot_full(sl), 64 * h, key0, head, tc::EVICT_NORMAL);
-        if (++sl == p.slots) { sl = 0; ph ^= 1; }
+          tc::tma_load_3d(ring + sl * Tile::SLOT + (HALVES + h) * Tile::KV_HALF, mv, slot_full(sl), 64 * h, key0, head, tc::EVICT_NORMAL);
+        if (++sl == SLOTS) { sl = 0; ph ^= 1; }
       }
     }
-  } else if (warp == 1) {
-    // the whole warp walks the loop, one elected lane issues; descriptors are advanced by their address field (flash_prefill.cu)
+  } else if (warp == 1 || warp == 10) {
+    // a warp per set issues its products: the whole warp walks the loop, one elected lane issues; descriptors are advanced by their address field
+    // (flash_prefill.cu).  Two warps, so that neither set waits for the other's softmax, and as few waits as there are tiles: a wait costs this warp some
+    // 150 cycles even where nothing is left to wait for, and a loop with three of them and divisions took 1700 cycles per tile for 600 of products.
+    const int w = warp == 1 ? 0 : 1, mine = tiles_of(w);
     constexpr uint32_t IDESC_S = tc::idesc_bf16_f32(PX_BM, PX_BN, false, false);
     constexpr uint32_t IDESC_O = tc::idesc_bf16_f32(PX_BM, HD, false, true);        // B = V is MN-major
-    const uint64_t dQ = tc::smem_desc_kmajor_sw128(sQ);
+    constexpr int STEP = PAIR ? 1 : 2;                                 // tiles from one of this set's to the next
+    const uint64_t dQ = tc::smem_desc_kmajor_sw128(sQ + (PAIR ? w * NQ * Tile::Q : 0));
     const uint64_t dK0 = tc::smem_desc_kmajor_sw128(ring);
-    const uint64_t dV0 = tc::smem_desc_mnmajor_sw128(ring, Tile::KV_HALF, 1024);
-    int sl = 0;                                                        // slot of the next K or V tile in issue order K_0, K_1, V_0, K_2, V_1, ...
-    auto at = [&](int idx, uint32_t* phase) {                          // where tile number idx of the ring lies
-      const int use = idx / p.slots;
-      *phase = use & 1;
-      return idx - use * p.slots;
-    };
-    auto issue_s = [&](int j) {
-      uint32_t ph;
-      sl = at(2 * j, &ph);
-      tc::mbar_wait(slot_full(sl), ph);
+    const uint64_t dV0 = tc::smem_desc_mnmajor_sw128(ring + HALVES * Tile::KV_HALF, Tile::KV_HALF, 1024);
+    int k_sl = tile_at(w, 0), v_sl = k_sl;                             // slots of the next scores and of the next product
+    uint32_t k_ph = 0;
+    auto next_slot = [&](int& sl) { sl += STEP; if (sl >= SLOTS) { sl -= SLOTS; return 1u; } return 0u; };
+    auto issue_s = [&](int i) {
+      tc::mbar_wait(slot_full(k_sl), k_ph);
       tc::fence_after_sync();
       if (tc::elect_one()) {
-        const uint64_t dK = dK0 + (uint64_t)sl * (Tile::SLOT >> 4);
+        const uint64_t dK = dK0 + (uint64_t)k_sl * (Tile::SLOT >> 4);
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k)
-            tc::mma_ss(tS(j), dQ + (uint64_t)((n * Tile::Q + (k >> 2) * Tile::Q_HALF + (k & 3) * 32) >> 4),
+            tc::mma_ss(tS(w, i), dQ + (uint64_t)((n * Tile::Q + (k >> 2) * Tile::Q_HALF + (k & 3) * 32) >> 4),
                        dK + (uint64_t)(((k >> 2) * Tile::KV_HALF + (k & 3) * 32) >> 4), IDESC_S, n != 0 || k != 0);
-        tc::mma_commit(s_full(j & 1));
-        tc::mma_commit(slot_empty(sl));
+        tc::mma_commit(s_full(w, i));
       }
       __syncwarp();
+      k_ph ^= next_slot(k_sl);
     };
-    if (n_tiles > 0) {
+    if (mine > 0) {
       tc::mbar_wait(q_full, 0);
       tc::fence_after_sync();
+      // the sets run half a tile apart, so that one's exponentials fall into the other's loads and waits; started together they stay together
+      if (PAIR && w == 1) tc::mbar_wait(started, 0);
       issue_s(0);
     }
-    for (int j = 0; j < n_tiles; ++j) {
-      if (j + 1 < n_tiles) issue_s(j + 1);                             // the tensor core forms S_{j+1} during softmax_j
-      uint32_t ph;
-      sl = at(2 * j + 1, &ph);
-      tc::mbar_wait(slot_full(sl), ph);
+    for (int i = 0; i < mine; ++i) {
+      if (i + 1 < mine) issue_s(i + 1);                                // the tensor core forms the next scores during this tile's softmax
+      const int j = tile_at(w, i);
       const int left = j < n_shared ? s_hi - s_lo - j * PX_BN : o_hi - o_lo - (j - n_shared) * PX_BN;
-      if (left < PX_BN) {                                              // value rows that hold no key
-        for (int i = lane; i < (PX_BN - left) * 8 * HALVES; i += 32) {
-          const int r = left + i / (8 * HALVES), c = i % (8 * HALVES);
-          const uint32_t a = ring + sl * Tile::SLOT + (c >> 3) * Tile::KV_HALF + r * 128 + (c & 7) * 16;
+      if (left < PX_BN) {                                              // value rows that hold no key (both sets write the same zeros)
+        for (int e = lane; e < (PX_BN - left) * 8 * HALVES; e += 32) {
+          const int r = left + e / (8 * HALVES), c = e % (8 * HALVES);
+          const uint32_t a = ring + v_sl * Tile::SLOT + (HALVES + (c >> 3)) * Tile::KV_HALF + r * 128 + (c & 7) * 16;
           asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      tc::mbar_wait(p_full, j & 1);
+      tc::mbar_wait(p_full(w, i), (i >> 1) & 1);
       tc::fence_after_sync();
       if (tc::elect_one()) {
-        const uint64_t dV = dV0 + (uint64_t)sl * (Tile::SLOT >> 4);
+        const uint64_t dV = dV0 + (uint64_t)v_sl * (Tile::SLOT >> 4);
 #pragma unroll
-        for (int k = 0; k < PX_BN / 16; ++k)                           // A = P_j in TMEM: 16 keys = 8 columns of packed pairs
-          tc::mma_ts(tO, tS(j) + k * 8, dV + (uint64_t)((k * 2048) >> 4), IDESC_O, j != 0 || k != 0);
-        tc::mma_commit(o_full);
-        tc::mma_commit(slot_empty(sl));
+        for (int k = 0; k < (PAIR ? 1 : 2) * PX_BN / 16; ++k)          // A = P in TMEM: 16 keys = 8 columns of packed pairs; the low parts behind the high ones
+          tc::mma_ts(tO(w), tS(w, i) + k * 8, dV + (uint64_t)(((k & 3) * 2048) >> 4), IDESC_O, i != 0 || k != 0);
+        tc::mma_commit(slot_empty(v_sl));
+        if (i + 2 >= mine) tc::mma_commit(o_last(w, i + 2 - mine));
       }
       __syncwarp();
+      next_slot(v_sl);
     }
   } else {
+    const int w = warp >= 6 ? 1 : 0;                                   // set of softmax warps (2..5, 6..9)
     const int quarter = warp & 3;                                      // TMEM lane quadrant of this warp
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    // ---- queries: the warp's 32 rows, 16 bytes per lane and step
+    // ---- queries, 16 bytes per lane and step: a set's own tile, or half of the one tile
     constexpr int CH = HD / 8, RPS = 32 / CH;                          // 16-byte chunks of a row, rows of a step
     const int ch = lane % CH;
     if (n_tiles > 0) {
-#pragma unroll 4
-      for (int i = 0; i < CH; ++i) {
-        const int r = quarter * 32 + i * RPS + lane / CH;
-        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (r < n_rows) {
-          const int token = token0 + (q0 + r) / G, h = kvh * G + (q0 + r) % G;
-          hi = *reinterpret_cast<const uint4*>(p.q + (size_t)token * p.ldq + (size_t)h * HD + 8 * ch);
-          if constexpr (ROTATE) {
-            int pos = max(g_hi - g_lo, 0) + min(*p.cache_len, p.T) - (p.pad_left ? p.pad_left[token] : 0);
-            pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
-            const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t) + (size_t)pos * CH + ch);
-            const float4 s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t) + (size_t)pos * CH + ch);
-            const float cs[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
-            const uint32_t w[4] = {hi.x, hi.y, hi.z, hi.w};
-            uint32_t a[4], b[4];
+      constexpr int STEPS = (PAIR ? 32 : 16) / RPS, AHEAD = ROTATE ? 4 : 16;           // loads in flight
+      const int row0 = (PAIR ? quarter * 32 : (w * 4 + quarter) * 16) + lane / CH;       // (rows behind the last query: anything, they are never read)
+#pragma unroll 1
+      for (int i0 = 0; i0 < STEPS; i0 += AHEAD) {
+        uint4 x[AHEAD];
+        float4 c4[ROTATE ? AHEAD : 1], s4[ROTATE ? AHEAD : 1];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float re = bf16_lo(w[e]), im = bf16_hi(w[e]);
-              const float u = re * cs[e] - im * sn[e], v = re * sn[e] + im * cs[e];
-              a[e] = pack_bf16(u, v);
-              b[e] = pack_bf16(u - bf16_lo(a[e]), v - bf16_hi(a[e]));
+        for (int u = 0; u < AHEAD; ++u) {
+          const int qr = (PAIR ? w * PX_BM : 0) + row0 + (i0 + u) * RPS;
+          if (i0 + u < STEPS && qr < n_rows) {
+            const int token = token0 + ((q0 + qr) >> p.gs), h = kvh * G + ((q0 + qr) & (G - 1));
+            x[u] = *reinterpret_cast<const uint4*>(p.q + (size_t)token * p.ldq + (size_t)h * HD + 8 * ch);
+            if constexpr (ROTATE) {
+              int pos = max(g_hi - g_lo, 0) + min(*p.cache_len, p.T) - (p.pad_left ? p.pad_left[token] : 0);
+              pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
+              c4[u] = __ldg(reinterpret_cast<const float4*>(p.cos_t) + (size_t)pos * CH + ch);
+              s4[u] = __ldg(reinterpret_cast<const float4*>(p.sin_t) + (size_t)pos * CH + ch);
             }
-            hi = make_uint4(a[0], a[1], a[2], a[3]);
-            lo = make_uint4(b[0], b[1], b[2], b[3]);
           }
         }
-        const uint32_t dst = sQ + (ch >> 3) * Tile::Q_HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
-        if constexpr (ROTATE)
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + Tile::Q), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int r = row0 + (i0 + u) * RPS;
+          if (i0 + u < STEPS && (PAIR ? w * PX_BM : 0) + r < n_rows) {
+            const uint32_t dst = sQ + (PAIR ? w * NQ * Tile::Q : 0) + (ch >> 3) * Tile::Q_HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+            if constexpr (ROTATE) {
+              const float cs[4] = {c4[u].x, c4[u].y, c4[u].z, c4[u].w}, sn[4] = {s4[u].x, s4[u].y, s4[u].z, s4[u].w};
+              const uint32_t v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+              uint32_t a[4], b[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float re = bf16_lo(v[e]), im = bf16_hi(v[e]);
+                const float y = re * cs[e] - im * sn[e], z_ = re * sn[e] + im * cs[e];
+                a[e] = pack_bf16(y, z_);
+                b[e] = pack_bf16(y - bf16_lo(a[e]), z_ - bf16_hi(a[e]));
+              }
+              x[u] = make_uint4(a[0], a[1], a[2], a[3]);
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + Tile::Q), "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3]) : "memory");
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(x[u].x), "r"(x[u].y), "r"(x[u].z), "r"(x[u].w) : "memory");
+          }
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(q_full);
     }
 
-    const int r = quarter * 32 + lane;                                 // this thread's query
-    const bool row_on = r < n_rows;
-    const int slot = p.own ? p.start + (q0 + min(r, n_rows - 1)) / G : 0;             // of the query's own key
-    const int slot_warp = p.own ? p.start + (q0 + min(quarter * 32, n_rows - 1)) / G : 0;      // the smallest of the warp
+    const int r = quarter * 32 + lane, qr = (PAIR ? w * PX_BM : 0) + r;               // this thread's query
+    const int warp_row = (PAIR ? w * PX_BM : 0) + quarter * 32;                        // the warp's first
+    const bool row_on = qr < n_rows, warp_on = warp_row < n_rows;
+    const int at = q0 + min(qr, n_rows - 1);
+    const int slot = p.own ? p.start + (at >> p.gs) : 0;                                     // of the query's own key
+    const int slot_warp = p.own ? p.start + ((q0 + min(warp_row, n_rows - 1)) >> p.gs) : 0;  // the smallest of the warp
+    const int my_tiles = tiles_of(w);
     float m_ref = -INFINITY, l_run = 0.f;
-    for (int j = 0; j < n_tiles; ++j) {
+    for (int i = 0; i < my_tiles; ++i) {
+      const int j = tile_at(w, i);
       const bool mine = j >= n_shared;
       const int key0 = mine ? o_lo + (j - n_shared) * PX_BN : s_lo + j * PX_BN;
       const int end = mine ? slot + 1 : s_hi;                          // first key that this row does not see
-      const bool need_mask = key0 + PX_BN > (mine ? slot_warp + 1 : s_hi);       // warp-uniform
-      tc::mbar_wait(s_full(j & 1), (j >> 1) & 1);
+      const int end_warp = mine ? slot_warp + 1 : s_hi;                // the smallest of the warp
+      tc::mbar_wait(s_full(w, i), (i >> 1) & 1);
       tc::fence_after_sync();
-      uint32_t v0[32], v1[32];
-      tc::tmem_ld32(tS(j) + lane_off, v0);
-      tc::tmem_ld32(tS(j) + lane_off + 32, v1);
-      tc::tmem_ld_wait();
-      if (need_mask) {
+      if (warp_on) {
+        uint32_t v0[32], v1[32];
+        tc::tmem_ld32(tS(w, i) + lane_off, v0);
+        tc::tmem_ld32(tS(w, i) + lane_off + 32, v1);
+        tc::tmem_ld_wait();
+        if (key0 + PX_BN > end_warp) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (key0 + i >= end) v0[i] = 0xff800000u;                    // -inf
-          if (key0 + 32 + i >= end) v1[i] = 0xff800000u;
-        }
-      }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], fmaxf(__uint_as_float(v0[i]), __uint_as_float(v1[i])));
-      const float t = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-      const bool need = t > m_ref + PX_RESCALE || (m_ref == -INFINITY && t > -INFINITY);
-      if (j == 0) {
-        m_ref = t;
-      } else if (__any_sync(0xffffffffu, need)) {
-        const float factor = need ? exp2f(m_ref - t) : 1.0f;           // m_ref = -inf: 0 (O and l are 0 there)
-        tc::mbar_wait(o_full, (j - 1) & 1);                            // O at rest
-        tc::fence_after_sync();
-#pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t o[32];
-          tc::tmem_ld32(tO + lane_off + c * 32, o);
-          tc::tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-          tc::tmem_st32(tO + lane_off + c * 32, o);
-        }
-        tc::tmem_st_wait();
-        l_run *= factor;
-        if (need) m_ref = t;
-      }
-      const float m_safe = m_ref == -INFINITY ? 0.f : m_ref;
-      float psum = 0.f;
-      uint32_t w[32];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float a0 = exp2f(fmaf(__uint_as_float(v0[2 * i]), p.scale_log2, -m_safe));
-        const float a1 = exp2f(fmaf(__uint_as_float(v0[2 * i + 1]), p.scale_log2, -m_safe));
-        const float b0 = exp2f(fmaf(__uint_as_float(v1[2 * i]), p.scale_log2, -m_safe));
-        const float b1 = exp2f(fmaf(__uint_as_float(v1[2 * i + 1]), p.scale_log2, -m_safe));
-        psum += (a0 + a1) + (b0 + b1);
-        w[i] = pack_bf16(a0, a1);
-        w[16 + i] = pack_bf16(b0, b1);
-      }
-      tc::tmem_st32(tS(j) + lane_off, w);                              // keys 2c, 2c + 1 of this row: 32-bit column c
-      tc::tmem_st_wait();
-      l_run += psum;
-      // at most one phase of p_full outstanding: P·V_{j-1} done proves that the MMA warp has seen phase j - 1 (flash_prefill.cu)
-      if (j > 0) tc::mbar_wait(o_full, (j - 1) & 1);
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(p_full);
-    }
-    if (n_tiles > 0) {
-      tc::mbar_wait(o_full, (n_tiles - 1) & 1);
-      tc::fence_after_sync();
-    }
-    const int token = token0 + (q0 + min(r, n_rows - 1)) / G, h = kvh * G + (q0 + min(r, n_rows - 1)) % G;
-    const size_t th = (size_t)token * p.nh + h;
-    if (p.partial) {
-      const size_t part = th * p.splits + split;
-      if (row_on) p.ml_part[part] = make_float2(m_ref, l_run);
-      float4* dst = reinterpret_cast<float4*>(p.o_part + part * HD);
-      if (n_tiles > 0) {
-#pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t o[32];
-          tc::tmem_ld32(tO + lane_off + c * 32, o);
-          tc::tmem_ld_wait();
-          if (row_on) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dst[8 * c + i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          for (int e = 0; e < 32; ++e) {
+            if (key0 + e >= end) v0[e] = 0xff800000u;                  // -inf
+            if (key0 + 32 + e >= end) v1[e] = 0xff800000u;
           }
         }
-      }
-    } else {
-      // ---- join with the partial triples of the shared keys (none when this launch visited them), normalise, store the row
-      const int n_parts = p.join;
-      const bool seen = row_on && slot >= pad;                         // a query in front of its row's first token is padding: zeros
-      float M = l_run != 0.f ? m_ref : -INFINITY;                      // (a sum of zero: no keys; NaN stays NaN)
-      const float2* ml = p.ml_part + th * n_parts;
-      if (seen)
-        for (int s = 0; s < n_parts; ++s) {
-          const float2 v = __ldcg(ml + s);
-          if (v.y != 0.f) M = fmaxf(M, v.x);
-        }
-      const float Ms = M == -INFINITY ? 0.f : M;
-      const float f0 = l_run != 0.f ? exp2f(m_ref - Ms) : 0.f;
-      float L = l_run * f0;
-      if (seen)
-        for (int s = 0; s < n_parts; ++s) {
-          const float2 v = __ldcg(ml + s);
-          if (v.y != 0.f) L += v.y * exp2f(v.x - Ms);
-        }
-      const float inv = seen && L != 0.f ? 1.0f / L : 0.f;
-      uint4* dst = reinterpret_cast<uint4*>(p.out + th * HD);
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 32; ++e) mx4[e & 3] = max3_nan(mx4[e & 3], __uint_as_float(v0[e]), __uint_as_float(v1[e]));
+        const float t = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * p.scale_log2;
+        const bool need = t > m_ref + PX_RESCALE || (m_ref == -INFINITY && t > -INFINITY);
+        bool odd = !(t < INFINITY);                                    // NaN or infinite scores show in the result: no shortcuts
+        if (i == 0) m_ref = t;
+        if (__any_sync(0xffffffffu, odd || (i > 0 && need))) {
+          odd = __any_sync(0xffffffffu, odd);
+          if (i > 0 && __any_sync(0xffffffffu, need)) {
+            const float factor = need ? exp2f(m_ref - t) : 1.0f;       // m_ref = -inf: 0 (O and l are 0 there)
+            // O at rest: the next scores are issued behind product i - 1
+            if (i + 1 < my_tiles) tc::mbar_wait(s_full(w, i + 1), ((i + 1) >> 1) & 1);
+            else tc::mbar_wait(o_last(w, 0), 0);
+            tc::fence_after_sync();
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
-        if (n_tiles > 0) {
-          tc::tmem_ld32(tO + lane_off + c * 32, o);
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t o[32];
+              tc::tmem_ld32(tO(w) + lane_off + c * 32, o);
+              tc::tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+              tc::tmem_st32(tO(w) + lane_off + c * 32, o);
+            }
+            tc::tmem_st_wait();
+            l_run *= factor;
+            if (need) m_ref = t;
+          }
+        }
+        const float m_safe = m_ref == -INFINITY ? 0.f : m_ref;
+        F2 sum = f2(0.f, 0.f);
+        uint32_t hi[32], lo[PAIR ? 1 : 32];
+        const F2 scale2 = f2(p.scale_log2, p.scale_log2), minus_m = f2(-m_safe, -m_safe);
+        auto pair = [&](int e, bool poly) {                            // keys 2e, 2e + 1
+          const uint32_t* v = e < 16 ? v0 + 2 * e : v1 + 2 * e - 32;
+          const F2 x = f2_fma(f2(__uint_as_float(v[0]), __uint_as_float(v[1])), scale2, minus_m);
+          float a, b;
+          if (poly) {
+            exp2_pair(x, a, b);
+          } else {
+            f2_get(x, a, b);
+            a = exp2f(a); b = exp2f(b);
+          }
+          sum = f2_add(sum, f2(a, b));
+          hi[e] = pack_bf16(a, b);
+          if constexpr (!PAIR) lo[e] = pack_bf16(a - bf16_lo(hi[e]), b - bf16_hi(hi[e]));
+        };
+        if (PAIR && !odd) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) pair(e, (e * PX_POLY) % 16 < PX_POLY);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) pair(e, false);
+        }
+        float psum, psum2;
+        f2_get(sum, psum, psum2);
+        psum += psum2;
+        tc::tmem_st32(tS(w, i) + lane_off, hi);                        // keys 2c, 2c + 1 of this row: 32-bit column c
+        if constexpr (!PAIR) tc::tmem_st32(tS(w, i) + lane_off + 32, lo);
+        tc::tmem_st_wait();
+        l_run += psum;
+      }
+      // (two barriers in turn: this warp's next arrival at the same one comes after scores that the MMA warp forms behind its wait for this phase)
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(p_full(w, i));
+      if (PAIR && i == 0 && warp == 2 && lane == 0) tc::mbar_arrive(started);
+    }
+    if (my_tiles > 0) {
+      tc::mbar_wait(o_last(w, 1), 0);
+      tc::fence_after_sync();
+    }
+
+    // ---- one triple per row: o = f0 O_0 + f1 O_1 against M.  Without PAIR both sets of warps hold the same rows: each takes half of the columns
+    float M = l_run != 0.f ? m_ref : -INFINITY, L = l_run, f0 = l_run != 0.f ? 1.f : 0.f, f1 = 0.f;       // (a sum of zero: no keys; NaN stays NaN)
+    if constexpr (!PAIR) {
+      float2* other = s_ml + r + 128 * (1 - w);
+      s_ml[r + 128 * w] = make_float2(m_ref, l_run);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (tiles_of(1 - w) > 0) {
+        tc::mbar_wait(o_last(1 - w, 1), 0);
+        tc::fence_after_sync();
+      }
+      const float2 o = *other;
+      if (o.y != 0.f) M = fmaxf(M, o.x);
+      const float Ms = M == -INFINITY ? 0.f : M;
+      const float mine = l_run != 0.f ? exp2f(m_ref - Ms) : 0.f, theirs = o.y != 0.f ? exp2f(o.x - Ms) : 0.f;
+      L = l_run * mine + o.y * theirs;
+      f0 = w == 0 ? mine : theirs;
+      f1 = w == 0 ? theirs : mine;
+    }
+    if (warp_on) {
+      const int token = token0 + (at >> p.gs), h = kvh * G + (at & (G - 1));
+      const size_t th = (size_t)token * p.nh + h;
+      constexpr int CHUNKS = HD / 32 / (PAIR ? 1 : 2);
+      // columns [32 c, 32 c + 32) of the row's sum
+      auto columns = [&](int c, float (&o)[32]) {
+        uint32_t a[32];
+        if (__any_sync(0xffffffffu, f0 != 0.f)) {
+          tc::tmem_ld32(tO(PAIR ? w : 0) + lane_off + c * 32, a);
           tc::tmem_ld_wait();
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = f0 != 0.f ? __float_as_uint(__uint_as_float(o[i]) * f0) : 0u;
-        if (seen) {
-          for (int s = 0; s < n_parts; ++s) {
-            const float2 v = __ldcg(ml + s);
-            if (v.y == 0.f) continue;
-            const float f = exp2f(v.x - Ms);
-            const float4* src = reinterpret_cast<const float4*>(p.o_part + (th * n_parts + s) * HD + c * 32);
+        for (int e = 0; e < 32; ++e) o[e] = f0 != 0.f ? __uint_as_float(a[e]) * f0 : 0.f;
+        if constexpr (!PAIR) {
+          if (__any_sync(0xffffffffu, f1 != 0.f)) {
+            tc::tmem_ld32(tO(1) + lane_off + c * 32, a);
+            tc::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 x = __ldcg(src + i);
-              o[4 * i] = __float_as_uint(fmaf(x.x, f, __uint_as_float(o[4 * i])));
-              o[4 * i + 1] = __float_as_uint(fmaf(x.y, f, __uint_as_float(o[4 * i + 1])));
-              o[4 * i + 2] = __float_as_uint(fmaf(x.z, f, __uint_as_float(o[4 * i + 2])));
-              o[4 * i + 3] = __float_as_uint(fmaf(x.w, f, __uint_as_float(o[4 * i + 3])));
+            for (int e = 0; e < 32; ++e) o[e] += f1 != 0.f ? __uint_as_float(a[e]) * f1 : 0.f;
+          }
+        }
+      };
+      if (p.partial) {
+        const size_t part = th * p.splits + split;
+        if (row_on && (PAIR || w == 0)) p.ml_part[part] = make_float2(M, L);
+        float4* dst = reinterpret_cast<float4*>(p.o_part + part * HD);
+        if (n_tiles > 0) {
+#pragma unroll 1
+          for (int k = 0; k < CHUNKS; ++k) {
+            const int c = (PAIR ? 0 : w * CHUNKS) + k;
+            float o[32];
+            columns(c, o);
+            if (row_on) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) dst[8 * c + e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
           }
         }
-        if (row_on) {
+      } else {
+        // join with the partial triples of the shared keys (none when this launch visited them), normalise, store the row
+        const int n_parts = p.join;
+        const bool seen = row_on && slot >= pad;                       // a query in front of its row's first token is padding: zeros
+        const float2* ml = p.ml_part + th * n_parts;
+        float M2 = M;
+        if (seen)
+          for (int s = 0; s < n_parts; ++s) {
+            const float2 v = __ldcg(ml + s);
+            if (v.y != 0.f) M2 = fmaxf(M2, v.x);
+          }
+        const float Ms = M2 == -INFINITY ? 0.f : M2;
+        const float f = L != 0.f ? exp2f(M - Ms) : 0.f;
+        L *= f; f0 *= f; f1 *= f;
+        if (seen)
+          for (int s = 0; s < n_parts; ++s) {
+            const float2 v = __ldcg(ml + s);
+            if (v.y != 0.f) L += v.y * exp2f(v.x - Ms);
+          }
+        const float inv = seen && L != 0.f ? 1.0f / L : 0.f;
+        uint4* dst = reinterpret_cast<uint4*>(p.out + th * HD);
+#pragma unroll 1
+        for (int k = 0; k < CHUNKS; ++k) {
+          const int c = (PAIR ? 0 : w * CHUNKS) + k;
+          float o[32];
+          columns(c, o);
+          if (seen) {
+            for (int s = 0; s < n_parts; ++s) {
+              const float2 v = __ldcg(ml + s);
+              if (v.y == 0.f) continue;
+              const float g = exp2f(v.x - Ms);
+              const float4* src = reinterpret_cast<const float4*>(p.o_part + (th * n_parts + s) * HD + c * 32);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            auto v = [&](int e) { return seen ? __uint_as_float(o[8 * i + e]) * inv : 0.f; };
-            dst[c * 4 + i] = make_uint4(pack_bf16(v(0), v(1)), pack_bf16(v(2), v(3)), pack_bf16(v(4), v(5)), pack_bf16(v(6), v(7)));
+              for (int e = 0; e < 8; ++e) {
+                const float4 x = __ldcg(src + e);
+                o[4 * e] = fmaf(x.x, g, o[4 * e]);
+                o[4 * e + 1] = fmaf(x.y, g, o[4 * e + 1]);
+                o[4 * e + 2] = fmaf(x.z, g, o[4 * e + 2]);
+                o[4 * e + 3] = fmaf(x.w, g, o[4 * e + 3]);
+              }
+            }
+          }
+          if (row_on) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              auto v = [&](int i) { return seen ? o[8 * e + i] * inv : 0.f; };
+              dst[c * 4 + e] = make_uint4(pack_bf16(v(0), v(1)), pack_bf16(v(2), v(3)), pack_bf16(v(4), v(5)), pack_bf16(v(6), v(7)));
+            }
           }
         }
       }
@@ -396,50 +517,68 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
 
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == 0) tc::tmem_dealloc(tmem, Tile::TMEM_COLS);
+  if (warp == 0) tc::tmem_dealloc(tmem, 512);
 }
 
-template <int HD, bool ROTATE>
-static int px_launch(PxParams p, dim3 grid, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok, const CUtensorMap& ov, cudaStream_t st) {
-  using Tile = PxTile<HD>;
-  // slack for the alignment of the base; two rotated 128-wide CTAs fill an SM's 228 KB to the last byte with 768
-  const int smem = (int)((ROTATE ? 2 : 1) * Tile::Q + p.slots * Tile::SLOT + PX_BARS + (ROTATE && HD == 128 ? 768 : 1024));
-  p.smem = smem;
+template <int HD, bool ROTATE, bool PAIR>
+static int px_launch(const PxParams& p, dim3 grid, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok, const CUtensorMap& ov, cudaStream_t st) {
+  using Tile = PxTile<HD, ROTATE, PAIR>;
   // attributes belong to the device's context: set at the first call on each (bit per device; setting them twice is harmless)
   static std::atomic<uint64_t> set{0};
   int dev = 0;
   JL_CUDA(cudaGetDevice(&dev));
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (bit == 0 || !(set.load(std::memory_order_acquire) & bit)) {
-    JL_CUDA(cudaFuncSetAttribute(prefix_attn_kernel<HD, ROTATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    JL_CUDA(cudaFuncSetAttribute(prefix_attn_kernel<HD, ROTATE>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    JL_CUDA(cudaFuncSetAttribute(prefix_attn_kernel<HD, ROTATE, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile::SMEM));
     set.fetch_or(bit, std::memory_order_release);
   }
-  JL_CUDA(launch_pdl(prefix_attn_kernel<HD, ROTATE>, grid, dim3(PX_THREADS), (size_t)smem, st, pk, pv, ok, ov, p));
+  JL_CUDA(launch_pdl(prefix_attn_kernel<HD, ROTATE, PAIR>, grid, dim3(PX_THREADS), (size_t)Tile::SMEM, st, pk, pv, ok, ov, p));
   return JL_OK;
 }
 
-static int px_dispatch(const PxParams& p, dim3 grid, bool rotate, int hd, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok,
+// One launch over tiles of the queries of `units` groups or rows, `queries` of a key head each.
+static int px_dispatch(const PxParams& p, long queries, int units, bool rotate, int hd, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok,
                        const CUtensorMap& ov, cudaStream_t st) {
-  if (hd == 128) return rotate ? px_launch<128, true>(p, grid, pk, pv, ok, ov, st) : px_launch<128, false>(p, grid, pk, pv, ok, ov, st);
-  return rotate ? px_launch<64, true>(p, grid, pk, pv, ok, ov, st) : px_launch<64, false>(p, grid, pk, pv, ok, ov, st);
+  const bool pair = queries > PX_BM;
+  const int tile = pair ? 2 * PX_BM : PX_BM;
+  const dim3 grid((unsigned)((queries + tile - 1) / tile * p.splits), p.nkv, units);
+#define JL_PX(HD_, R_, P_) if (hd == HD_ && rotate == R_ && pair == P_) return px_launch<HD_, R_, P_>(p, grid, pk, pv, ok, ov, st);
+  JL_PX(128, true, true) JL_PX(128, true, false) JL_PX(128, false, true) JL_PX(128, false, false)
+  JL_PX(64, true, true) JL_PX(64, true, false) JL_PX(64, false, true) JL_PX(64, false, false)
+#undef JL_PX
+  return JL_ERR_UNSUPPORTED;
 }
 
-constexpr int PX_MAX_SPLITS = 64;
+constexpr int PX_MAX_SPLITS = 64, PX_SMS = 148;
 
-// Splits of the shared keys: as many CTAs as run at once (two per SM) when that leaves every CTA two tiles of keys or more.
-static int px_splits(long tokens_per_group, int groups, int nkv, int G, int prefix) {
-  const long items = (tokens_per_group * G + PX_BM - 1) / PX_BM * groups * nkv;
-  const long most = ((long)prefix + 2 * PX_BN - 1) / (2 * PX_BN);
-  long s = 2 * 148 / (items > 0 ? items : 1);
-  s = s < most ? s : most;
-  return (int)(s < 1 ? 1 : (s > PX_MAX_SPLITS ? PX_MAX_SPLITS : s));
+// Time of a launch in units of a tile of keys: rounds of CTAs (one per SM) times the tiles of one and its way in and out.
+static float px_rounds(long queries, long units, int nkv, int splits, float tiles) {
+  const long tile = queries > PX_BM ? 2 * PX_BM : PX_BM;
+  const long ctas = (queries + tile - 1) / tile * units * nkv * splits;
+  return (float)((ctas + PX_SMS - 1) / PX_SMS) * (tiles + 5.f);
 }
 
-// Whether a row's queries fill tiles by themselves: one launch over shared and own keys.
-static bool px_one_launch(int S, int G, int B, int nkv) {
-  const long tiles = ((long)S * G + PX_BM - 1) / PX_BM;
-  return 8l * S * G >= 7 * tiles * PX_BM && tiles * B * nkv >= 148;
+// Splits of the shared keys: the count with the least time, every one two tiles of keys or more; a split costs the triples' way to memory and back.
+static int px_splits(long queries, int groups, int nkv, int prefix, float* cost = nullptr) {
+  const int tiles = (prefix + PX_BN - 1) / PX_BN;
+  int best = 1;
+  float least = 0.f;
+  for (int s = 1; s <= PX_MAX_SPLITS && (s == 1 || 2 * s <= tiles); ++s) {
+    const float c = px_rounds(queries, groups, nkv, s, (float)((tiles + s - 1) / s)) + (float)(queries * groups * nkv) * s * 3e-4f;
+    if (s == 1 || c < least) { least = c; best = s; }
+  }
+  if (cost) *cost = least;
+  return best;
+}
+
+// Whether one launch over shared and own keys together, every row's queries in tiles of their own, is estimated to be no slower than shared keys for all rows of a
+// group together and then the own keys.
+static bool px_one_launch(int S, int G, int B, int groups, int nkv, int P, int start) {
+  float two;
+  px_splits((long)(B / groups) * S * G, groups, nkv, P, &two);
+  const float own = (float)(start + S) / PX_BN;
+  two += px_rounds((long)S * G, B, nkv, 1, own);
+  return px_rounds((long)S * G, B, nkv, 1, (float)P / PX_BN + own) <= two;
 }
 
 static size_t px_part_bytes(long tokens, int nh, int hd, int splits) { return (size_t)tokens * nh * splits * (hd + 2) * sizeof(float); }
@@ -451,8 +590,7 @@ using namespace jl;
 
 extern "C" JL_API size_t jl_prefix_attn_scratch_bytes(int B, int S, int groups, int nh, int nkv, int hd, int prefix) {
   if (B < 1 || S < 1 || groups < 1 || B % groups != 0 || nkv < 1 || nh % nkv != 0 || prefix < 0) return 0;
-  const int G = nh / nkv, splits = px_splits((long)(B / groups) * S, groups, nkv, G, prefix);
-  if (S > 1 && px_one_launch(S, G, B, nkv)) return 16;             // (no partial results; never nothing)
+  const int G = nh / nkv, splits = px_splits((long)(B / groups) * S * G, groups, nkv, prefix);
   return px_up(S == 1 ? prefix_step_scratch_bytes(B, nh, nkv, hd) : 0) + px_part_bytes((long)B * S, nh, hd, splits);
 }
 
@@ -488,15 +626,14 @@ extern "C" JL_API int jl_decode_attn_prefix(const void* qkv, const void* prefix_
   p.q = (const __nv_bfloat16*)qkv; p.ldq = (nh + 2 * nkv) * hd;
   p.cos_t = cos_t; p.sin_t = sin_t; p.max_pos = max_pos; p.cache_len = cache_len;
   p.prefix_len = prefix_len; p.prefix_pad = prefix_pad; p.pad_left = pad_left;
-  p.S = 1; p.rows = rows; p.nh = nh; p.nkv = nkv; p.P = P; p.T = T;
+  p.S = 1; p.rows = rows; p.nh = nh; p.nkv = nkv; p.gs = G == 1 ? 0 : (G == 2 ? 1 : (G == 4 ? 2 : 3)); p.P = P; p.T = T;
   p.shared = 1; p.partial = 1;
-  p.splits = px_splits(rows, groups, nkv, G, P);
-  p.slots = hd == 128 ? 3 : 6;
+  p.splits = px_splits((long)rows * G, groups, nkv, P);
   p.scale_log2 = scale * 1.4426950408889634f;
   char* parts = (char*)scratch + px_up(prefix_step_scratch_bytes(B, nh, nkv, hd));
   p.o_part = (float*)parts;
   p.ml_part = (float2*)(p.o_part + (size_t)B * nh * p.splits * hd);
-  rc = px_dispatch(p, dim3((rows * G + PX_BM - 1) / PX_BM * p.splits, nkv, groups), true, hd, pk, pv, pk, pv, (cudaStream_t)stream);
+  rc = px_dispatch(p, (long)rows * G, groups, true, hd, pk, pv, pk, pv, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;
   const PrefixStep step{(const __nv_bfloat16*)qkv, (__nv_bfloat16*)k_cache, (__nv_bfloat16*)v_cache, cos_t, sin_t, cache_len, pad_left, prefix_len, prefix_pad,
                         (__nv_bfloat16*)out, scratch, B, rows, nh, nkv, hd, P, T, max_pos, scale, {p.o_part, p.ml_part, p.splits}};
@@ -523,21 +660,19 @@ extern "C" JL_API int jl_prefill_attn_prefix(const void* q, const void* prefix_k
   p.q = (const __nv_bfloat16*)q; p.ldq = nh * hd;
   p.prefix_len = prefix_len; p.prefix_pad = prefix_pad; p.pad_left = pad_left;
   p.out = (__nv_bfloat16*)out;
-  p.S = S; p.rows = rows; p.nh = nh; p.nkv = nkv; p.P = P; p.T = T; p.start = start;
-  p.slots = hd == 128 ? 4 : 8;
+  p.S = S; p.rows = rows; p.nh = nh; p.nkv = nkv; p.gs = G == 1 ? 0 : (G == 2 ? 1 : (G == 4 ? 2 : 3)); p.P = P; p.T = T; p.start = start;
   p.scale_log2 = scale * 1.4426950408889634f;
-  const dim3 own_grid((S * G + PX_BM - 1) / PX_BM, nkv, B);
   p.splits = 1;
-  if (px_one_launch(S, G, B, nkv)) {
+  if (px_one_launch(S, G, B, groups, nkv, P, start)) {
     p.shared = p.own = 1;
-    return px_dispatch(p, own_grid, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
+    return px_dispatch(p, (long)S * G, B, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   }
-  const int splits = px_splits((long)rows * S, groups, nkv, G, P);
+  const int splits = px_splits((long)rows * S * G, groups, nkv, P);
   p.o_part = (float*)((char*)scratch + px_up(S == 1 ? prefix_step_scratch_bytes(B, nh, nkv, hd) : 0));
   p.ml_part = (float2*)(p.o_part + (size_t)B * S * nh * splits * hd);
   p.shared = p.partial = 1; p.splits = splits;
-  rc = px_dispatch(p, dim3((rows * S * G + PX_BM - 1) / PX_BM * splits, nkv, groups), false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
+  rc = px_dispatch(p, (long)rows * S * G, groups, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;
   p.shared = p.partial = 0; p.own = 1; p.splits = 1; p.join = splits;
-  return px_dispatch(p, own_grid, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
+  return px_dispatch(p, (long)S * G, B, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
 }
