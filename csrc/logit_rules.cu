@@ -6,10 +6,11 @@
 //   every entry i with bias_ids[b, i] == v:                x = x + bias[b, i]                             (in the order of the entries)
 //   bit v of allowed[b] is zero:                           x = -infinity
 //
-// A CTA owns a slice of one row's vocabulary and keeps, per token of the slice, a count in shared memory: bit 31 = occurred, the rest = occurrences behind the
-// prompt (whole numbers: the order of the atomics does not show), and beside it the sum of the biases when there are any.  It walks the row's
-// history, counts what falls into its slice, then passes over the slice once.  No state is kept between calls: the history is the sequence
-// buffer that the decode loop writes anyway, so forks, restarts and replayed graphs need nothing.
+// A CTA owns a slice of one row's vocabulary and keeps one word per token of the slice in shared memory: occurrences behind the prompt in the low bits, and bits
+// for "occurred", "has a bias", "has several" (whole numbers and bits: the order of the atomics does not show).  Everything it reads is asked for at once, the slice's
+// logits, the row's bounds, the first tokens of its history, its first biases: a CTA's way is a chain of memory latencies, and a batch of 96 rows is seven rounds of
+// CTAs.  Then one pass writes the slice, and the threads that were first to mark a token's bias add it, all entries of a token in their order.  No state
+// is kept between calls: the history is the sequence buffer that the decode loop writes anyway, so forks, restarts and replayed graphs need nothing.
 #include "common.cuh"
 #include "jllama_b200.h"
 
@@ -17,12 +18,12 @@
 
 namespace jl {
 
-constexpr int LR_THREADS = 512;
+constexpr unsigned LR_SAID = 1u << 31, LR_BIAS = 1u << 30, LR_MORE = 1u << 29, LR_COUNT = LR_MORE - 1u;
 
 struct RulesParams {
   const void* logits; int ld;
   float* out; int ldo;
-  int V, slice;
+  int V;
   const int* tokens; int ldt, T;
   const int* starts; int starts_n;                  // [B] or one for all rows (n = 1), or nullptr
   const int* lengths; int lengths_n;
@@ -33,72 +34,162 @@ struct RulesParams {
   const unsigned* allowed; int lda;
 };
 
-template <typename T> __device__ __forceinline__ float lr_load(const T* p) { return (float)*p; }
-
-template <typename T>
-__global__ void __launch_bounds__(LR_THREADS) logit_rules_kernel(const RulesParams p) {
-  extern __shared__ unsigned lr_count[];
-  float* s_bias = reinterpret_cast<float*>(lr_count + p.slice);
-  const int b = blockIdx.y, lo = blockIdx.x * p.slice, n = min(p.slice, p.V - lo);
+// TH threads with N groups of four tokens each.  Rows whose logits and results lie alike on 16-byte boundaries (8-byte ones for 16-bit logits)
+// start their groups there, others load and store token by token.
+template <typename T, int TH, int N>
+__global__ void __launch_bounds__(TH, 4) logit_rules_kernel(const RulesParams p) {
+  constexpr int SLICE = 4 * N * TH;
+  extern __shared__ __align__(16) unsigned lr_count[];
+  const int b = blockIdx.y, t = threadIdx.x;
+  const T* x = static_cast<const T*>(p.logits) + (size_t)b * p.ld;
+  float* y = p.out + (size_t)b * p.ldo;
+  const int off = (int)(((uintptr_t)y >> 2) & 3);                       // tokens past a boundary at the row's start
+  const bool wide = ((uintptr_t)y & 3) == 0 && ((uintptr_t)x / sizeof(T) & 3) == (unsigned)off;
+  const int lo = (int)blockIdx.x * SLICE - (wide ? off : 0);            // (the first slice starts up to three tokens in front of the row)
   const bool history = p.tokens != nullptr;
-  if (history)
-    for (int i = threadIdx.x; i < n; i += LR_THREADS) lr_count[i] = 0;
-  if (p.n_bias)
-    for (int i = threadIdx.x; i < n; i += LR_THREADS) s_bias[i] = 0.f;
-  __syncthreads();
+  const bool table = history || p.n_bias;
+#pragma unroll
+  for (int k = 0; k < N; ++k) if (table) reinterpret_cast<uint4*>(lr_count)[k * TH + t] = make_uint4(0, 0, 0, 0);
   pdl_wait();
   pdl_launch_dependents();
-  if (history) {
-    const int len = p.lengths ? min(p.lengths[p.lengths_n > 1 ? b : 0], p.T) : p.T;
-    const int start = p.starts ? max(p.starts[p.starts_n > 1 ? b : 0], 0) : 0;
-    const int prompt = p.prompts ? p.prompts[p.prompts_n > 1 ? b : 0] : 0;
-    const int* row = p.tokens + (size_t)b * p.ldt;
-    for (int i = start + threadIdx.x; i < len; i += LR_THREADS) {
-      const unsigned v = (unsigned)row[i] - (unsigned)lo;
-      if (v < (unsigned)n) {
-        if (i < prompt) atomicOr(&lr_count[v], 0x80000000u);
-        else atomicAdd(&lr_count[v], 1u);
+  // ---- all that is read, on its way together
+  const int len = p.lengths ? min(p.lengths[p.lengths_n > 1 ? b : 0], p.T) : p.T;
+  const int start = p.starts ? max(p.starts[p.starts_n > 1 ? b : 0], 0) : 0;
+  const int prompt = p.prompts ? p.prompts[p.prompts_n > 1 ? b : 0] : 0;
+  const float r = p.rep ? p.rep[b] : p.rep1, f = p.freq ? p.freq[b] : p.freq1, pr = p.pres ? p.pres[b] : p.pres1;
+  const float inv_r = __fdividef(1.0f, r);
+  const int* row = p.tokens + (size_t)b * p.ldt;
+  constexpr int AHEAD = 8;                                              // tokens of the history per thread before its length is known
+  int said[AHEAD];
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) said[u] = history && u * TH + t < p.T ? row[u * TH + t] : -1;
+  const int* ids = p.bias_ids + (size_t)b * p.ldb;
+  const float* bias = p.bias + (size_t)b * p.ldb;
+  const int id0 = t < p.n_bias ? ids[t] : -1;
+  const float bias0 = t < p.n_bias ? bias[t] : 0.f;
+  float v[N][4];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = lo + 4 * (k * TH + t);
+    if (wide && i >= 0 && i + 4 <= p.V) {
+      if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4*>(x + i);
+        v[k][0] = a.x; v[k][1] = a.y; v[k][2] = a.z; v[k][3] = a.w;
+      } else {
+        T a[4];
+        *reinterpret_cast<uint2*>(a) = *reinterpret_cast<const uint2*>(x + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[k][e] = (float)a[e];
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[k][e] = i + e >= 0 && i + e < p.V ? (float)x[i + e] : 0.f;
     }
   }
-  if (p.n_bias && threadIdx.x < 32) {
-    // one warp, the entries in order: those of a token that stand in one load are added one after the other
-    const int* ids = p.bias_ids + (size_t)b * p.ldb;
-    const float* val = p.bias + (size_t)b * p.ldb;
-    for (int i0 = 0; i0 < p.n_bias; i0 += 32) {
-      const int i = i0 + (int)threadIdx.x;
-      const int id = i < p.n_bias ? (int)((unsigned)ids[i] - (unsigned)lo) : -1;
-      const float x = i < p.n_bias ? val[i] : 0.f;
-      const bool mine = (unsigned)id < (unsigned)n;
-      const unsigned same = __match_any_sync(0xffffffffu, mine ? id : -1 - (int)threadIdx.x);
-      const int before = __popc(same & ((1u << threadIdx.x) - 1u));
-      int most = mine ? __popc(same) : 0;
-      most = __reduce_max_sync(0xffffffffu, most);
-      for (int k = 0; k < most; ++k) {
-        if (mine && before == k) s_bias[id] += x;
-        __syncwarp();
-      }
+  unsigned bits[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    bits[k] = 0xfu;
+    const int i = lo + 4 * (k * TH + t);
+    if (p.allowed && i + 3 >= 0 && i < p.V) {
+      const unsigned* row = p.allowed + (size_t)b * p.lda;
+      const int w = i >> 5;                                             // (-1 in front of the row)
+      const unsigned a = w >= 0 ? __ldg(row + w) : 0u;
+      const unsigned c = (i & 31) > 28 && (w + 1) * 32 < p.V ? __ldg(row + w + 1) : 0u;
+      bits[k] = __funnelshift_r(a, c, i & 31);
     }
   }
   __syncthreads();
-  const float r = p.rep ? p.rep[b] : p.rep1, f = p.freq ? p.freq[b] : p.freq1, pr = p.pres ? p.pres[b] : p.pres1;
-  const T* x = static_cast<const T*>(p.logits) + (size_t)b * p.ld + lo;
-  float* y = p.out + (size_t)b * p.ldo + lo;
-  const unsigned* bits = p.allowed ? p.allowed + (size_t)b * p.lda : nullptr;
-  for (int i = threadIdx.x; i < n; i += LR_THREADS) {
-    float v = lr_load(x + i);
-    if (history) {
-      const unsigned c = lr_count[i];
-      if (c) {
-        v = v > 0.f ? __fdiv_rn(v, r) : v * r;
-        const unsigned k = c & 0x7fffffffu;
-        if (k) v = v - f * (float)k - pr;
+  if (history) {
+    // (ids outside the vocabulary: beyond the slice, or words of it that stand for no token)
+    const unsigned span = (unsigned)max(len - start, 0);
+    auto count = [&](int i, int id) {
+      const unsigned at = (unsigned)id - (unsigned)lo;
+      if (at < (unsigned)SLICE && (unsigned)(i - start) < span) {
+        if (i < prompt) atomicOr(&lr_count[at], LR_SAID);
+        else atomicAdd(&lr_count[at], 1u);
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) count(u * TH + t, said[u]);
+    for (int i0 = AHEAD * TH + t; i0 < len; i0 += AHEAD * TH) {         // AHEAD loads in flight
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) said[u] = i0 + u * TH < len ? row[i0 + u * TH] : -1;
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) count(i0 + u * TH, said[u]);
+    }
+  }
+  // ---- biases: whoever marks a token first adds them at the end, the others say that there are more
+  unsigned mine = 0;                                                    // bit k: this thread was first with entry t + k TH
+  for (int i = t, k = 0; i < p.n_bias; i += TH, ++k) {
+    const int id = k == 0 ? id0 : ids[i];
+    const unsigned at = (unsigned)id - (unsigned)lo;
+    if (at < (unsigned)SLICE && id >= 0 && id < p.V) {
+      if (atomicOr(&lr_count[at], LR_BIAS) & LR_BIAS) atomicOr(&lr_count[at], LR_MORE);
+      else mine |= 1u << k;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = lo + 4 * (k * TH + t);
+    if (table) {
+      const uint4 c4 = reinterpret_cast<const uint4*>(lr_count)[k * TH + t];
+      const unsigned c[4] = {c4.x, c4.y, c4.z, c4.w};
+      if (c4.x | c4.y | c4.z | c4.w) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned n = c[e] & LR_COUNT;
+          // v / r as q = v (1 / r), a few last bits off, and one step with the remainder v - q r, which a fused product gives exactly; infinite quotients have none
+          const float a = v[k][e], q = a * inv_r;
+          const float pen = a > 0.f ? (q < INFINITY ? fmaf(fmaf(-q, r, a), inv_r, q) : q) : a * r;
+          if (c[e] & (LR_COUNT | LR_SAID)) v[k][e] = pen;
+          if (n) v[k][e] = v[k][e] - f * (float)n - pr;
+          if ((c[e] & LR_BIAS) && !((bits[k] >> e) & 1u)) lr_count[4 * (k * TH + t) + e] = 0;       // masked: no bias is added
+        }
       }
     }
-    if (p.n_bias) v += s_bias[i];
-    if (bits && !((bits[(lo + i) >> 5] >> ((lo + i) & 31)) & 1u)) v = -INFINITY;
-    y[i] = v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (!((bits[k] >> e) & 1u)) v[k][e] = -INFINITY;
+    if (wide && i >= 0 && i + 4 <= p.V) {
+      *reinterpret_cast<float4*>(y + i) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (i + e >= 0 && i + e < p.V) y[i + e] = v[k][e];
+    }
   }
+  if (!p.n_bias || !__syncthreads_or(mine)) return;                     // the slice is written
+  for (int k = 0; k < 32 && mine >> k; ++k) {
+    if (!((mine >> k) & 1u)) continue;
+    const int i = t + k * TH, id = k == 0 ? id0 : ids[i];
+    const unsigned c = lr_count[id - lo];
+    if (!(c & LR_BIAS)) continue;                                       // masked
+    float v0 = y[id];
+    if (c & LR_MORE) {
+      float sum = 0.f;
+      for (int j = 0; j < p.n_bias; ++j) if (ids[j] == id) sum += bias[j];
+      v0 += sum;
+    } else {
+      v0 += k == 0 ? bias0 : bias[i];
+    }
+    y[id] = v0;
+  }
+}
+
+template <typename T, int TH, int N>
+static cudaError_t lr_launch(const RulesParams& p, int B, cudaStream_t st) {
+  constexpr int SLICE = 4 * N * TH;
+  const size_t smem = p.tokens || p.n_bias ? (size_t)SLICE * 4 : 0;
+  return launch_pdl(logit_rules_kernel<T, TH, N>, dim3((p.V + 3 + SLICE - 1) / SLICE, B), dim3(TH), smem, st, p);
+}
+template <typename T>
+static cudaError_t lr_dispatch(const RulesParams& p, int B, cudaStream_t st) {
+  // Few rows: the smallest slices, for more SMs; many: the largest that keep four CTAs per SM, because every slice's CTA walks the row's whole history.  us in a graph,
+  // 1, 2, 4 groups per thread: 1 x 32000 2.0, 2.8, 3.2; 17 x 128259 8.9, 6.9, 5.5; 96 x 128256 50, 47, 40.  (512 threads with 4: 4.3, 9.1, 41.)
+  const long groups = ((long)p.V + 3) / 4 * B / 256;                   // CTAs of 256 threads with one group each
+  if (groups <= 2 * 148) return lr_launch<T, 256, 1>(p, B, st);
+  if (groups <= 6 * 148) return lr_launch<T, 256, 2>(p, B, st);
+  return lr_launch<T, 256, 4>(p, B, st);
 }
 
 }  // namespace jl
@@ -111,11 +202,12 @@ extern "C" JL_API int jl_logit_rules(const void* logits, int dtype, int B, int V
                                      const void* allowed, int lda, void* stream) {
   if (B == 0 || V == 0) return JL_OK;
   JL_CHECK_ARG(logits && out && B > 0 && V > 0 && B <= 65535 && ld >= V && ldo >= V, "jl_logit_rules: %d rows of %d logits, pitches %d and %d", B, V, ld, ldo);
+  JL_CHECK_ARG(V <= (1 << 30) && (uintptr_t)logits % (dtype == 0 ? 4 : 2) == 0 && (uintptr_t)out % 4 == 0, "jl_logit_rules: vocabulary of %d, or misplaced logits", V);
   JL_CHECK_ARG(dtype >= 0 && dtype <= 2, "jl_logit_rules: dtype %d (0 fp32, 1 bf16, 2 fp16)", dtype);
   JL_CHECK_ARG(tokens == nullptr || (T >= 0 && ldt >= T), "jl_logit_rules: history of %d tokens, pitch %d", T, ldt);
   for (int n : {starts ? starts_n : 1, lengths ? lengths_n : 1, prompts ? prompts_n : 1})
     JL_CHECK_ARG(n == 1 || n == B, "jl_logit_rules: %d row bounds for %d rows", n, B);
-  JL_CHECK_ARG(n_bias >= 0 && (n_bias == 0 || (bias_ids && bias && (ldb == 0 || ldb >= n_bias))), "jl_logit_rules: %d biases, pitch %d", n_bias, ldb);
+  JL_CHECK_ARG(n_bias >= 0 && n_bias <= 8192 && (n_bias == 0 || (bias_ids && bias && (ldb == 0 || ldb >= n_bias))), "jl_logit_rules: %d biases, pitch %d", n_bias, ldb);
   JL_CHECK_ARG(allowed == nullptr || lda == 0 || lda >= (V + 31) / 32, "jl_logit_rules: mask rows of %d words for %d tokens", lda, V);
   RulesParams p{};
   p.logits = logits; p.ld = ld; p.out = out; p.ldo = ldo; p.V = V;
@@ -124,13 +216,8 @@ extern "C" JL_API int jl_logit_rules(const void* logits, int dtype, int B, int V
   p.rep = rep; p.rep1 = rep1; p.freq = freq; p.freq1 = freq1; p.pres = pres; p.pres1 = pres1;
   p.bias_ids = bias_ids; p.bias = bias; p.n_bias = n_bias; p.ldb = ldb;
   p.allowed = (const unsigned*)allowed; p.lda = lda;
-  p.slice = 4096;
-  const dim3 grid((V + p.slice - 1) / p.slice, B);
-  const size_t smem = (size_t)p.slice * 4 * (n_bias ? 2 : 1);
-  cudaError_t e;
-  if (dtype == 0) e = launch_pdl(logit_rules_kernel<float>, grid, dim3(LR_THREADS), smem, (cudaStream_t)stream, p);
-  else if (dtype == 1) e = launch_pdl(logit_rules_kernel<__nv_bfloat16>, grid, dim3(LR_THREADS), smem, (cudaStream_t)stream, p);
-  else e = launch_pdl(logit_rules_kernel<__half>, grid, dim3(LR_THREADS), smem, (cudaStream_t)stream, p);
+  cudaError_t e = dtype == 0 ? lr_dispatch<float>(p, B, (cudaStream_t)stream)
+                             : (dtype == 1 ? lr_dispatch<__nv_bfloat16>(p, B, (cudaStream_t)stream) : lr_dispatch<__half>(p, B, (cudaStream_t)stream));
   JL_CUDA(e);
   return JL_OK;
 }

@@ -555,7 +555,7 @@ def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = N
     tokens int32 [B, T]: row b has said tokens[b, starts[b] : lengths[b]] (int32 [B], or [1] for all rows; None: 0 and T), the part from prompt_lengths[b] on (None:
     all of it) as its answer.  Ids outside the vocabulary are passed over.  For a token that occurs: x > 0 ? x / repetition : x · repetition; with n occurrences in
     the answer, n > 0: x - frequency · n - presence.  (A number, or fp32 [B]; None: off.  repetition > 0.)  Then x + bias_values of the entries of bias_ids
-    (int32 / fp32 [B, n], or [1, n] for all rows; an id outside the vocabulary is no entry, the same id twice adds both), then -inf where bit v % 32 of word v // 32
+    (int32 / fp32 [B, n], or [1, n] for all rows, n <= 8192; an id outside the vocabulary is no entry, the same id twice adds both), then -inf where bit v % 32 of word v // 32
     of allowed (int32 [B, words] or [1, words]) is zero.  A row whose mask allows nothing is -inf throughout.  `out` may be `logits` itself when that is fp32."""
     who = "constrain_logits"
     if logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES or (logits.shape[1] > 1 and logits.stride(1) != 1):
@@ -588,6 +588,8 @@ def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = N
                 or bias_ids.shape[0] not in (1, B) or not (bias_ids.is_contiguous() and bias_values.is_contiguous()) or bias_ids.device != dev or bias_values.device != dev:
             raise ValueError(f"{who}: biases are int32 and fp32 [{B} or 1, n] on {dev} (got {tuple(bias_ids.shape)}, {tuple(bias_values.shape)})")
         n_bias = bias_ids.shape[1]
+        if n_bias > 8192:
+            raise ValueError(f"{who}: {n_bias} biases per row (at most 8192)")
     if allowed is not None and (allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[0] not in (1, B) or allowed.shape[1] < (V + 31) // 32
                                 or not allowed.is_contiguous() or allowed.device != dev):
         raise ValueError(f"{who}: allowed is int32 [{B} or 1, {(V + 31) // 32} or more words] on {dev} (got {allowed.dtype}, {tuple(allowed.shape)})")

@@ -96,7 +96,7 @@ def test_refusals():
     bad = [dict(tokens=torch.zeros(2, 4)), dict(tokens=i(3, 4)), dict(tokens=i(2, 8)[:, ::2]), dict(lengths=i(2)), dict(tokens=i(2, 4), lengths=i(3)),
            dict(tokens=i(2, 4), starts=torch.zeros(2)), dict(repetition=0.0), dict(repetition=-1.0), dict(repetition=math.nan), dict(repetition=torch.ones(3)),
            dict(frequency=torch.ones(2, dtype=torch.float64)), dict(bias_ids=i(2, 3)), dict(bias_ids=i(2, 3), bias_values=torch.zeros(2, 4)),
-           dict(bias_ids=i(3, 3), bias_values=torch.zeros(3, 3)), dict(allowed=i(2, 1)), dict(allowed=i(2, 2).float()), dict(allowed=i(3, 2)), dict(out=torch.zeros(2, 41)),
+           dict(bias_ids=i(3, 3), bias_values=torch.zeros(3, 3)), dict(bias_ids=i(1, 8193), bias_values=torch.zeros(1, 8193)), dict(allowed=i(2, 1)), dict(allowed=i(2, 2).float()), dict(allowed=i(3, 2)), dict(out=torch.zeros(2, 41)),
            dict(out=torch.zeros(2, 40, dtype=torch.bfloat16))]
     for kw in bad:
         with pytest.raises(ValueError):
