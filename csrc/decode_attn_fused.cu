@@ -16,7 +16,6 @@
 #include "common.cuh"
 #include "tcgen05.cuh"
 #include "jllama_b200.h"
-#include "prefix_attn.cuh"
 
 namespace jl {
 
@@ -38,11 +37,6 @@ struct FusedAttnParams {
   int nkv, T, max_pos, splits;
   float scale_log2;
   int vec;                       // o_part on 16-byte and out on 8-byte boundaries
-  // rows whose group shares keys in front of their own (decode_attn_mma_kernel<.., true>): what positions count, and the shared keys' partial results
-  const int* prefix_len;
-  const int* prefix_pad;
-  int rows, P;
-  PrefixParts parts;
 };
 
 // Shared tail of both kernels: s_o / s_ml hold the (m, l, o) triples of the CTA's NG independent streams.  Folds them,
@@ -145,104 +139,6 @@ __device__ __forceinline__ void df_fold_and_merge(const FusedAttnParams& p, floa
       }
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;
-    *reinterpret_cast<uint2*>(p.out + bh * HD + d) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
-  }
-}
-
-// The same where the row's group shares keys: the fold of this CTA's streams, then the join of the own keys' splits with the partial triples of the
-// shared keys, in order, by the last CTA of this (batch, kv-head).
-constexpr int DF_OWN_MAX = 32, DF_PARTS_MAX = 64;
-template <int NG, int G, int HD>
-__device__ __forceinline__ void df_fold_and_join(const FusedAttnParams& p, float (*s_o)[G][HD], float (*s_ml)[G][2], int* s_last_p, const int b,
-                                                 const int kvh, const int split, const int active) {
-  constexpr int N = DF_OWN_MAX + DF_PARTS_MAX;
-  static_assert((NG - 1) * HD >= 2 * N, "weights of all triples behind the folded output");
-  __shared__ float s_own[G][2];
-  const int nh = p.nkv * G;
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < G * HD; idx += (int)blockDim.x) {
-    const int g = idx / HD, d = idx - g * HD;
-    float M = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < NG; ++j) M = fmaxf(M, s_ml[j][g][0]);
-    const float Ms = M == -INFINITY ? 0.f : M;
-    float acc = 0.f, L = 0.f;
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      const float w = exp2f(s_ml[j][g][0] - Ms);
-      acc += w * s_o[j][g][d];
-      L += w * s_ml[j][g][1];
-    }
-    if (active == 1) {
-      s_o[0][g][d] = acc;                                // (read by this thread alone)
-      if (d == 0) { s_own[g][0] = M; s_own[g][1] = L; }
-    } else {
-      const size_t pi = ((size_t)b * nh + kvh * G + g) * p.splits + split;
-      p.o_part[pi * HD + d] = acc;
-      if (d == 0) { p.ml_part[pi * 2] = M; p.ml_part[pi * 2 + 1] = L; }
-    }
-  }
-  if (active > 1) {
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int* t = p.tickets + b * p.nkv + kvh;
-      *s_last_p = atomicAdd(t, 1) == active - 1;
-      if (*s_last_p) *t = 0;                             // everyone has arrived: re-armed for the next launch
-    }
-    __syncthreads();
-    if (!*s_last_p) return;
-    __threadfence();
-  }
-  pdl_wait();                                            // the shared keys' triples
-  __syncthreads();
-  float* s_m = &s_o[1][0][0];
-  float* s_l = s_m + G * N;
-  const int parts = p.parts.splits, n = active + parts;
-  for (int i = threadIdx.x; i < G * n; i += (int)blockDim.x) {
-    const int g = i / n, e = i - g * n;
-    const size_t bh = (size_t)b * nh + kvh * G + g;
-    float m, l;
-    if (e >= active) {
-      const float2 v = __ldcg(p.parts.ml + bh * parts + (e - active));
-      m = v.x; l = v.y;
-    } else if (active == 1) {
-      m = s_own[g][0]; l = s_own[g][1];
-    } else {
-      m = __ldcg(p.ml_part + (bh * p.splits + e) * 2); l = __ldcg(p.ml_part + (bh * p.splits + e) * 2 + 1);
-    }
-    s_m[g * N + e] = m; s_l[g * N + e] = l;
-  }
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < G * (HD / 4); idx += (int)blockDim.x) {
-    const int g = idx / (HD / 4), d = 4 * (idx - g * (HD / 4));
-    const size_t bh = (size_t)b * nh + kvh * G + g;
-    float M = -INFINITY;
-    for (int e = 0; e < n; ++e) if (s_l[g * N + e] != 0.f) M = fmaxf(M, s_m[g * N + e]);     // (a sum of zero: no keys, and no o was written)
-    const float Ms = M == -INFINITY ? 0.f : M;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, L = 0.f;
-    const float* own = p.o_part + bh * p.splits * HD + d;
-    const float* shared = p.parts.o + bh * parts * HD + d;
-    for (int e0 = 0; e0 < n; e0 += 16) {                 // 16 rows requested before the first is used
-      float4 ov[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int e = e0 + i;
-        if (e < n && s_l[g * N + e] != 0.f)
-          ov[i] = e >= active ? __ldcg(reinterpret_cast<const float4*>(shared + (size_t)(e - active) * HD))
-                              : (active == 1 ? *reinterpret_cast<const float4*>(&s_o[0][g][d]) : __ldcg(reinterpret_cast<const float4*>(own + (size_t)e * HD)));
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int e = e0 + i;
-        if (e < n && s_l[g * N + e] != 0.f) {
-          const float w = exp2f(s_m[g * N + e] - Ms);
-          acc[0] += w * ov[i].x; acc[1] += w * ov[i].y; acc[2] += w * ov[i].z; acc[3] += w * ov[i].w;
-          L += w * s_l[g * N + e];
-        }
-      }
-    }
-    const float inv = 1.f / L;                           // the new token is always seen: L > 0
     *reinterpret_cast<uint2*>(p.out + bh * HD + d) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
   }
 }
@@ -495,9 +391,7 @@ __device__ __forceinline__ uint4 rope_chunk(const uint4 a, const float4 cs, cons
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// PREFIX: the row's own keys behind keys that its group shares.  Positions count those too, the rotated query keeps 16 bits (its low part in the rows
-// 8..15 that the scores' product leaves free), and the fold joins the partial triples of the shared keys.
-template <int G, int HD, bool PREFIX = false>
+template <int G, int HD>
 __global__ void __launch_bounds__(DM_WARPS * 32, 2)
     decode_attn_mma_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const FusedAttnParams p) {
   using Tile = DmTile<HD>;
@@ -535,11 +429,6 @@ __global__ void __launch_bounds__(DM_WARPS * 32, 2)
   const int first = p.pad_left ? p.pad_left[b] : 0;
   const int valid = len - first > 0 ? len - first : 0;
   int pos = len - first;
-  if constexpr (PREFIX) {
-    const int group = b / p.rows;
-    const int lo_g = p.prefix_pad ? max(p.prefix_pad[group], 0) : 0, hi_g = p.prefix_len ? min(p.prefix_len[group], p.P) : p.P;
-    pos += max(hi_g - lo_g, 0);
-  }
   pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
   int chunk = (valid + p.splits - 1) / p.splits;
   chunk = ((chunk + DM_WARPS * KPI - 1) / (DM_WARPS * KPI)) * (DM_WARPS * KPI);
@@ -578,19 +467,17 @@ __global__ void __launch_bounds__(DM_WARPS * 32, 2)
   const float* sin_p = p.sin_t + (size_t)pos * (HD / 2);
 
   // Q of head kvh·G + g, rotated and rounded to bf16 (as the unfused path does): qa[s] = (a0, a2) of k-step s
-  uint32_t qa[KS][2], ql[PREFIX ? KS : 1][2];
+  uint32_t qa[KS][2];
 #pragma unroll
   for (int s = 0; s < KS; ++s)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       qa[s][i] = 0;
-      if constexpr (PREFIX) ql[s][i] = 0;
       if (g < G) {
         const int pair = 8 * s + 4 * i + t;
         const uint32_t w = *reinterpret_cast<const uint32_t*>(row + (size_t)(kvh * G + g) * HD + 2 * pair);
         const float c = __ldg(cos_p + pair), sn = __ldg(sin_p + pair), re = bf16_lo(w), im = bf16_hi(w);
         qa[s][i] = pack_bf16(re * c - im * sn, re * sn + im * c);
-        if constexpr (PREFIX) ql[s][i] = pack_bf16(re * c - im * sn - bf16_lo(qa[s][i]), re * sn + im * c - bf16_hi(qa[s][i]));
       }
     }
 
@@ -620,17 +507,11 @@ __global__ void __launch_bounds__(DM_WARPS * 32, 2)
       for (int i = 0; i < KS / 2; ++i) {
         uint32_t r[4];
         dm_ldsm(ks + (i >> 1) * Tile::BOX + j * 1024 + koff[i & 1], r);
-        if constexpr (PREFIX) {
-          mma_16816(d[0], qa[2 * i][0], ql[2 * i][0], qa[2 * i][1], ql[2 * i][1], r[0], r[1]);
-          mma_16816(d[1], qa[2 * i + 1][0], ql[2 * i + 1][0], qa[2 * i + 1][1], ql[2 * i + 1][1], r[2], r[3]);
-        } else {
-          mma_16816(d[0], qa[2 * i][0], 0u, qa[2 * i][1], 0u, r[0], r[1]);
-          mma_16816(d[1], qa[2 * i + 1][0], 0u, qa[2 * i + 1][1], 0u, r[2], r[3]);
-        }
+        mma_16816(d[0], qa[2 * i][0], 0u, qa[2 * i][1], 0u, r[0], r[1]);
+        mma_16816(d[1], qa[2 * i + 1][0], 0u, qa[2 * i + 1][1], 0u, r[2], r[3]);
       }
       c[j][0] = d[0][0] + d[1][0];
       c[j][1] = d[0][1] + d[1][1];
-      if constexpr (PREFIX) { c[j][0] += d[0][2] + d[1][2]; c[j][1] += d[0][3] + d[1][3]; }
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -726,35 +607,10 @@ __global__ void __launch_bounds__(DM_WARPS * 32, 2)
       *reinterpret_cast<float2*>(&s_o[warp][g][8 * e + 2 * t]) = make_float2(o[e][0] + o[e][2], o[e][1] + o[e][3]);
     if (t == 0) { s_ml[warp][g][0] = m; s_ml[warp][g][1] = l; }
   }
-  if constexpr (PREFIX) df_fold_and_join<DM_WARPS, G, HD>(p, s_o, s_ml, &s_last, b, kvh, split, active);
-  else df_fold_and_merge<DM_WARPS, G, HD>(p, s_o, s_ml, &s_last, b, kvh, split, active);
+  df_fold_and_merge<DM_WARPS, G, HD>(p, s_o, s_ml, &s_last, b, kvh, split, active);
 }
 
-// Splits by estimate, `most` being the most there may be.  A call costs the
-// larger of its bytes and of the waves of CTAs (2 per SM) times the keys of one CTA at the pace of its dependent
-// blocks; each wave adds the way from the position to the first block, splitting adds the merge.  The five constants are
-// fits to 31 shapes swept over 1 to 32 splits; the choice was within 5 % of the best count in all but two of them (8 %).
-static int dm_splits(int pairs, int T, int hd, int most) {
-  static int sms = 0;
-  if (sms == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-      sms = 148;
-  }
-  const int slots = 2 * sms, step = hd == 128 ? 64 : 128;
-  const float key_us = hd == 128 ? 0.0091f : 0.0039f, bw_us = (float)pairs * (float)T * (float)hd * 4.f / 6.0e6f;
-  int ms = 1;
-  float best = 0.f;
-  for (int c = 1; c <= most && c <= 32; ++c) {
-    const float waves = (float)((pairs * c + slots - 1) / slots);
-    const float chunk = (float)(((T + c - 1) / c + step - 1) / step * step);
-    const float us = fmaxf(bw_us, waves * chunk * key_us) + 3.4f * waves + (c > 1 ? 2.5f + 0.12f * c : 0.f);
-    if (c == 1 || us < best) { best = us; ms = c; }
-  }
-  return ms;
-}
-
-template <int G, int HD, bool PREFIX = false>
+template <int G, int HD>
 static int launch_decode_mma(const FusedAttnParams& p, int B, cudaStream_t s) {
   CUtensorMap tk, tv;
   const uint64_t rows = (uint64_t)B * p.nkv * p.T;
@@ -767,38 +623,12 @@ static int launch_decode_mma(const FusedAttnParams& p, int B, cudaStream_t s) {
   JL_CUDA(cudaGetDevice(&dev));
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (bit == 0 || !(set.load(std::memory_order_acquire) & bit)) {
-    JL_CUDA(cudaFuncSetAttribute(decode_attn_mma_kernel<G, HD, PREFIX>, cudaFuncAttributeMaxDynamicSharedMemorySize, DmTile<HD>::SMEM));
-    JL_CUDA(cudaFuncSetAttribute(decode_attn_mma_kernel<G, HD, PREFIX>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    JL_CUDA(cudaFuncSetAttribute(decode_attn_mma_kernel<G, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, DmTile<HD>::SMEM));
+    JL_CUDA(cudaFuncSetAttribute(decode_attn_mma_kernel<G, HD>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     set.fetch_or(bit, std::memory_order_release);
   }
-  JL_CUDA(launch_pdl(decode_attn_mma_kernel<G, HD, PREFIX>, dim3(p.splits, p.nkv, B), dim3(DM_WARPS * 32), DmTile<HD>::SMEM, s, tk, tv, p));
+  JL_CUDA(launch_pdl(decode_attn_mma_kernel<G, HD>, dim3(p.splits, p.nkv, B), dim3(DM_WARPS * 32), DmTile<HD>::SMEM, s, tk, tv, p));
   return JL_OK;
-}
-
-// ---- the own keys of a step behind shared ones (prefix_attn.cuh)
-size_t prefix_step_scratch_bytes(int B, int nh, int nkv, int hd) {
-  // tickets (zero before the first call, left zero), then the triples of the most splits that dm_splits chooses for this many pairs at any capacity
-  const int most = B * nkv >= 148 ? 8 : DF_OWN_MAX;
-  return ((size_t)B * nkv * sizeof(int) + 15) / 16 * 16 + (size_t)B * nh * most * (hd + 2) * sizeof(float);
-}
-
-int prefix_step_launch(const PrefixStep& a, cudaStream_t st) {
-  const int G = a.nh / a.nkv, pairs = a.B * a.nkv;
-  FusedAttnParams p{};
-  p.qkv = a.qkv; p.kc = a.k_cache; p.vc = a.v_cache; p.cos_t = a.cos_t; p.sin_t = a.sin_t;
-  p.cache_len_ptr = a.cache_len; p.pad_left = a.pad_left; p.out = a.out;
-  p.nkv = a.nkv; p.T = a.T; p.max_pos = a.max_pos; p.scale_log2 = a.scale * 1.4426950408889634f;
-  p.prefix_len = a.prefix_len; p.prefix_pad = a.prefix_pad; p.rows = a.rows; p.P = a.P; p.parts = a.parts;
-  p.splits = dm_splits(pairs, a.T, a.hd, pairs >= 148 ? 8 : DF_OWN_MAX);
-  p.tickets = (int*)a.scratch;
-  p.o_part = (float*)((char*)a.scratch + ((size_t)pairs * sizeof(int) + 15) / 16 * 16);
-  p.ml_part = p.o_part + (size_t)a.B * a.nh * p.splits * a.hd;
-#define JL_DP(G_, HD_) if (G == G_ && a.hd == HD_) return launch_decode_mma<G_, HD_, true>(p, a.B, st);
-  JL_DP(1, 128) JL_DP(2, 128) JL_DP(4, 128) JL_DP(8, 128)
-  JL_DP(1, 64) JL_DP(2, 64) JL_DP(4, 64) JL_DP(8, 64)
-#undef JL_DP
-  set_error("attention over a shared prefix: unsupported GQA group %d / head_dim %d (groups 1,2,4,8; head_dim 64,128)", G, a.hd);
-  return JL_ERR_UNSUPPORTED;
 }
 
 }  // namespace jl
@@ -856,7 +686,26 @@ extern "C" JL_API int jl_decode_attn_fused(const void* qkv, void* k_cache, void*
   // and 64.
   const bool use_mma = (hd == 128 || hd == 64) && (g_attn_variant == 2 || (g_attn_variant == 0 && !(G == 1 && T <= 128)));
   if (use_mma) {
-    const int ms = dm_splits(B * nkv, T, hd, splits);
+    static int sms = 0;
+    if (sms == 0) {
+      int dev = 0;
+      if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        sms = 148;
+    }
+    // Splits by estimate, the caller's count (which sizes the scratch) being the most there may be.  A call costs the
+    // larger of its bytes and of the waves of CTAs (2 per SM) times the keys of one CTA at the pace of its dependent
+    // blocks; each wave adds the way from the position to the first block, splitting adds the merge.  The five constants are
+    // fits to 31 shapes swept over 1 to 32 splits; the choice was within 5 % of the best count in all but two of them (8 %).
+    const int slots = 2 * sms, pairs = B * nkv, step = hd == 128 ? 64 : 128;
+    const float key_us = hd == 128 ? 0.0091f : 0.0039f, bw_us = (float)pairs * (float)T * (float)hd * 4.f / 6.0e6f;
+    int ms = 1;
+    float best = 0.f;
+    for (int c = 1; c <= splits && c <= 32; ++c) {
+      const float waves = (float)((pairs * c + slots - 1) / slots);
+      const float chunk = (float)(((T + c - 1) / c + step - 1) / step * step);
+      const float us = fmaxf(bw_us, waves * chunk * key_us) + 3.4f * waves + (c > 1 ? 2.5f + 0.12f * c : 0.f);
+      if (c == 1 || us < best) { best = us; ms = c; }
+    }
     p.splits = ms;
 #define JL_DM(G_, HD_) if (G == G_ && hd == HD_) return launch_decode_mma<G_, HD_>(p, B, s);
     JL_DM(1, 128) JL_DM(2, 128) JL_DM(4, 128) JL_DM(8, 128)

@@ -6,8 +6,8 @@
 // The shared keys are read once for all rows: the queries of a group, every row's tokens and the G query heads of a key head, are the rows of one
 // matrix [rows · S · G, d] per (group, key head), cut into tiles of 128 for tcgen05.  With running statistics a softmax over two sets of keys
 // is a join of two triples (reference exponent m, sum l, weighted values o):  M = max(m1, m2),  o = o1 2^(m1 - M) + o2 2^(m2 - M),  l likewise.
-//   * one token per row (jl_decode_attn_prefix): shared keys in tiles of queries here, cut into splits over the SMs, partial triples in fp32; then the
-//     rows' own keys in the one-token kernel (decode_attn_fused.cu), which appends the new key and joins;
+//   * one token per row (jl_decode_attn_prefix): one launch in which some CTAs take the shared keys, tiles of queries by splits of the keys, and others the
+//     rows' own keys, a warp per (row, key head), appending the new one; all leave partial triples in fp32, and a second, small launch joins them;
 //   * S tokens per row (jl_prefill_attn_prefix): the same for the shared keys, then a second launch of this kernel over every row's own keys, causal, that
 //     joins in its last step; or one launch over both sets, tile after tile, where a row's queries fill tiles by themselves.
 //
@@ -22,13 +22,20 @@
 #include <atomic>
 
 #include "jllama_b200.h"
-#include "prefix_attn.cuh"
 #include "tcgen05.cuh"
 
 namespace jl {
 
 constexpr int PX_BM = 128, PX_BN = 64, PX_THREADS = 352;
 constexpr float PX_RESCALE = 8.0f;                                 // log2 units
+
+// The CTAs of a step that take the rows' own keys: WARPS independent warps with a ring of STAGES blocks of KPI keys and values each.
+template <int HD> struct PxOwn {
+  static constexpr int WARPS = 8, STAGES = 3, HALVES = HD / 64;
+  static constexpr int KPI = HD == 128 ? 16 : 32;                  // 8 KB of keys and values at either width
+  static constexpr uint32_t BOX = KPI * 128, STAGE = 2 * HALVES * BOX, RING = STAGES * STAGE;
+  static constexpr uint32_t SMEM = WARPS * RING + WARPS * STAGES * 8 + 1024;
+};
 
 // PAIR: two tiles of queries per CTA, each with its own softmax warps, over the same keys; else one tile whose keys the two sets of softmax warps take in turn.
 template <int HD, bool ROTATE, bool PAIR> struct PxTile {
@@ -40,7 +47,8 @@ template <int HD, bool ROTATE, bool PAIR> struct PxTile {
   static constexpr uint32_t SMALL = 512 + (PAIR ? 0 : 2048);                 // barriers, the address of the TMEM columns; (m, l) of 2 x 128 rows
   static constexpr int FIT = (int)((227 * 1024 - 1024 - SMALL - QS) / SLOT);
   static constexpr int SLOTS = FIT < 8 ? FIT : 8;                            // tiles in flight (96 KB or more; a memory latency needs about 50 per SM)
-  static constexpr uint32_t SMEM = QS + SLOTS * SLOT + SMALL + 1024;         // (1024: alignment of the base)
+  static constexpr uint32_t NEED = QS + SLOTS * SLOT + SMALL + 1024;         // (1024: alignment of the base)
+  static constexpr uint32_t SMEM = ROTATE && NEED < PxOwn<HD>::SMEM ? PxOwn<HD>::SMEM : NEED;
   static_assert(SLOTS >= 3 && SMEM <= 227 * 1024, "a tile ahead of the products");
 };
 
@@ -78,12 +86,237 @@ struct PxParams {
   const float* cos_t; const float* sin_t; int max_pos; const int* cache_len;     // ROTATE: tables and the slot of the new token
   const int* prefix_len; const int* prefix_pad; const int* pad_left;
   __nv_bfloat16* out;
-  float* o_part; float2* ml_part;   // [tokens · nh][splits]: written (partial) or joined (own keys behind a launch over the shared ones)
+  float* o_part; float2* ml_part;   // [tokens · nh][parts]: written (partial) or joined (own keys behind a launch over the shared ones)
   int S, rows, nh, nkv, gs, P, T, start;      // gs: log2 of the query heads per key head
   int shared, own, partial;         // which keys this launch visits; whether it leaves partial triples or the result
-  int splits, join;                 // splits of the shared keys in this launch; triples per (token, head) that the last step joins
+  int splits, parts;                // splits of the shared keys in this launch; triples per (token, head)
+  // ROTATE: the CTAs in front take the own keys, `own_splits` parts of every (row, key head)
+  const __nv_bfloat16* qkv; __nv_bfloat16* k_cache; __nv_bfloat16* v_cache;
+  int own_ctas, own_splits, B, tiles_q;
   float scale_log2;
 };
+
+__device__ __forceinline__ void px_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void px_ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void px_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+// The own keys of a step.  A warp takes units, a part of the keys of one (row, key head), one after the other; its ring holds the next blocks of the same or the
+// following unit.  As in decode_attn_fused.cu the G query heads are rows 0..G-1 of mma.sync operands of 16 rows, which leaves rows 8..15 for the low parts
+// of the queries (scores) and of the probabilities (values): both keep 16 bits at no cost.  The new token of a unit's row, in the last part, is folded in from
+// registers.  Bound by the cache's bytes; a block's chain of dependent steps takes about 0.6 us, so that a warp moves 13 GB/s and eight of them an SM's share
+// of the bandwidth twice over.
+template <int HD>
+__device__ __forceinline__ void px_own_keys(const PxParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint8_t* smem) {
+  using Own = PxOwn<HD>;
+  constexpr int KPI = Own::KPI, HALVES = Own::HALVES, STAGES = Own::STAGES;
+  constexpr int NT = KPI / 8, NB = KPI / 16, KS = HD / 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (warp >= Own::WARPS) return;
+  const uint32_t raw = tc::smem_u32(smem), base0 = (raw + 1023u) & ~1023u;
+  const uint32_t ring = base0 + warp * Own::RING, bar0 = base0 + Own::WARPS * Own::RING + warp * STAGES * 8;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) tc::mbar_init(bar0 + 8 * i, 1);
+    tc::fence_barrier_init();
+  }
+  __syncwarp();
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const int G = 1 << p.gs, units = p.B * p.nkv * p.own_splits, step = p.own_ctas * Own::WARPS;
+  const int len = min(*p.cache_len, p.T);                  // keys in front of the new token
+  // first and last + 1 key of unit u
+  auto range = [&](int u, int& lo, int& hi) {
+    const int item = u / p.own_splits, part = u - item * p.own_splits, b = item / p.nkv;
+    const int first = p.pad_left ? max(p.pad_left[b], 0) : 0, valid = max(len - first, 0);
+    const int chunk = ((valid + p.own_splits - 1) / p.own_splits + KPI - 1) / KPI * KPI;
+    lo = first + min(part * chunk, valid);
+    hi = first + min((part + 1) * chunk, valid);
+  };
+  // what is asked for next: block [r_base, r_base + KPI) of unit r_u
+  int r_u = blockIdx.x * Own::WARPS + warp, r_base = 0, r_hi = 0, r_st = 0;
+  if (r_u < units) range(r_u, r_base, r_hi);
+  auto request = [&]() {
+    while (r_u < units && r_base >= r_hi) {
+      r_u += step;
+      if (r_u < units) range(r_u, r_base, r_hi);
+    }
+    if (r_u >= units) return;
+    if (lane == 0) {
+      const uint32_t dst = ring + r_st * Own::STAGE, bar = bar0 + 8 * r_st;
+      const int head = r_u / p.own_splits;                 // b · nkv + key head
+      tc::mbar_expect_tx(bar, Own::STAGE);
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        tc::tma_load_3d(dst + h * Own::BOX, &tm_k, bar, 64 * h, r_base, head, tc::EVICT_FIRST);
+        tc::tma_load_3d(dst + (HALVES + h) * Own::BOX, &tm_v, bar, 64 * h, r_base, head, tc::EVICT_FIRST);
+      }
+    }
+    r_base += KPI;
+    if (++r_st == STAGES) r_st = 0;
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) request();
+
+  // ldmatrix addresses within a 64-column box: row r's 16-byte chunk c lies at r * 128 + ((c ^ (r & 7)) << 4)
+  const int l7 = lane & 7, q8 = lane >> 3;
+  uint32_t koff[2], voff[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) koff[i] = l7 * 128 + (((4 * i + q8) ^ l7) << 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) voff[i] = ((q8 & 1) * 8 + l7) * 128 + (((2 * i + (q8 >> 1)) ^ l7) << 4);
+
+  int st = 0;
+  uint32_t phase = 0;
+#pragma unroll 1
+  for (int u = blockIdx.x * Own::WARPS + warp; u < units; u += step) {
+    int lo, hi;
+    range(u, lo, hi);
+    const int item = u / p.own_splits, part = u - item * p.own_splits, b = item / p.nkv, kvh = item - b * p.nkv;
+    const int group = b / p.rows;
+    const int g_lo = p.prefix_pad ? max(p.prefix_pad[group], 0) : 0, g_hi = p.prefix_len ? min(p.prefix_len[group], p.P) : p.P;
+    int pos = max(g_hi - g_lo, 0) + len - (p.pad_left ? p.pad_left[b] : 0);
+    pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
+    const float* cos_p = p.cos_t + (size_t)pos * (HD / 2);
+    const float* sin_p = p.sin_t + (size_t)pos * (HD / 2);
+    const __nv_bfloat16* row = p.qkv + (size_t)b * (p.nh + 2 * p.nkv) * HD;
+    const bool newest = part == p.own_splits - 1;
+
+    // query of head kvh · G + g, rotated: qa = high parts (a0, a2) of the k-steps, ql = low parts; and, in the newest part, its product with the new key
+    uint32_t qa[KS][2], ql[KS][2];
+    float s_new = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int pair = 8 * s + 4 * i + t;
+        const float c = __ldg(cos_p + pair), sn = __ldg(sin_p + pair);
+        float qr = 0.f, qi = 0.f;
+        if (g < G) {
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(row + (size_t)(kvh * G + g) * HD + 2 * pair);
+          const float re = bf16_lo(x), im = bf16_hi(x);
+          qr = re * c - im * sn; qi = re * sn + im * c;
+        }
+        qa[s][i] = pack_bf16(qr, qi);
+        ql[s][i] = pack_bf16(qr - bf16_lo(qa[s][i]), qi - bf16_hi(qa[s][i]));
+        if (newest) {
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(row + (size_t)(p.nh + kvh) * HD + 2 * pair);
+          const float re = bf16_lo(x), im = bf16_hi(x);
+          const uint32_t kx = pack_bf16(re * c - im * sn, re * sn + im * c);
+          s_new = fmaf(qr, bf16_lo(kx), fmaf(qi, bf16_hi(kx), s_new));
+          if (g == 0 && len < p.T) *reinterpret_cast<uint32_t*>(p.k_cache + ((size_t)item * p.T + len) * HD + 2 * pair) = kx;
+        }
+      }
+
+    float m = -INFINITY, l = 0.f;                // row g: m is quad-uniform, l is this thread's share of the sum
+    float o[HD / 8][4];                          // [0..1]: row g against P's high parts, [2..3]: against the low parts
+#pragma unroll
+    for (int e = 0; e < HD / 8; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[e][i] = 0.f;
+#pragma unroll 1
+    for (int base = lo; base < hi; base += KPI) {
+      tc::mbar_wait(bar0 + 8 * st, phase);
+      const uint32_t ks = ring + st * Own::STAGE, vs = ks + HALVES * Own::BOX;
+      if (base + KPI > hi) {                     // value rows that hold no key: a weight of zero times a NaN is a NaN
+        for (int i = lane; i < (KPI - (hi - base)) * 8 * HALVES; i += 32) {
+          const int r = hi - base + i / (8 * HALVES), c = i % (8 * HALVES);
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vs + (c >> 3) * Own::BOX + r * 128 + (c & 7) * 16), "r"(0) : "memory");
+        }
+        __syncwarp();
+      }
+      float c[NT][2];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float d[2][4] = {};                      // two chains: half the latency of the dependent products
+#pragma unroll
+        for (int i = 0; i < KS / 2; ++i) {
+          uint32_t r[4];
+          px_ldsm(ks + (i >> 1) * Own::BOX + j * 1024 + koff[i & 1], r);
+          px_mma(d[0], qa[2 * i][0], ql[2 * i][0], qa[2 * i][1], ql[2 * i][1], r[0], r[1]);
+          px_mma(d[1], qa[2 * i + 1][0], ql[2 * i + 1][0], qa[2 * i + 1][1], ql[2 * i + 1][1], r[2], r[3]);
+        }
+        const int key = base + 8 * j + 2 * t;
+        c[j][0] = key < hi ? ((d[0][0] + d[1][0]) + (d[0][2] + d[1][2])) * p.scale_log2 : -INFINITY;
+        c[j][1] = key + 1 < hi ? ((d[0][1] + d[1][1]) + (d[0][3] + d[1][3])) * p.scale_log2 : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) mx = fmaxf(mx, fmaxf(c[j][0], c[j][1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float m_new = fmaxf(m, mx), m_safe = m_new == -INFINITY ? 0.f : m_new;
+      const float corr = exp2f(m - m_safe);
+      m = m_new;
+      float psum = 0.f;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        c[j][0] = exp2f(c[j][0] - m_safe);
+        c[j][1] = exp2f(c[j][1] - m_safe);
+        psum += c[j][0] + c[j][1];
+      }
+      l = l * corr + psum;
+      if (__any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll
+        for (int e = 0; e < HD / 8; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[e][i] *= corr;
+      }
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) {
+        const float(&c0)[2] = c[2 * kb];
+        const float(&c1)[2] = c[2 * kb + 1];
+        const uint32_t h0 = pack_bf16(c0[0], c0[1]), h2 = pack_bf16(c1[0], c1[1]);
+        const uint32_t l0 = pack_bf16(c0[0] - bf16_lo(h0), c0[1] - bf16_hi(h0));
+        const uint32_t l2 = pack_bf16(c1[0] - bf16_lo(h2), c1[1] - bf16_hi(h2));
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e) {
+          uint32_t r[4];
+          px_ldsm_t(vs + (e >> 2) * Own::BOX + kb * 2048 + voff[e & 3], r);
+          px_mma(o[2 * e], h0, l0, h2, l2, r[0], r[1]);
+          px_mma(o[2 * e + 1], h0, l0, h2, l2, r[2], r[3]);
+        }
+      }
+      __syncwarp();                              // every lane has read the stage: it may be filled again
+      request();
+      if (++st == STAGES) { st = 0; phase ^= 1; }
+    }
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    const size_t th = (size_t)b * p.nh + kvh * G + (g < G ? g : 0), at = th * p.parts + p.splits + part;
+    float w_old = 1.f, w_new = 0.f;
+    if (newest) {                                // one more key
+      s_new += __shfl_xor_sync(0xffffffffu, s_new, 1);
+      s_new += __shfl_xor_sync(0xffffffffu, s_new, 2);
+      s_new *= p.scale_log2;
+      const float m_new = fmaxf(m, s_new), m_safe = m_new == -INFINITY ? 0.f : m_new;
+      w_old = exp2f(m - m_safe);
+      w_new = exp2f(s_new - m_safe);
+      l = l * w_old + w_new;
+      m = m_new;
+    }
+    float* dst = p.o_part + at * HD;
+#pragma unroll
+    for (int e = 0; e < HD / 8; ++e) {
+      float x = o[e][0] + o[e][2], y = o[e][1] + o[e][3];
+      if (newest) {
+        const uint32_t v = *reinterpret_cast<const uint32_t*>(row + (size_t)(p.nh + p.nkv + kvh) * HD + 8 * e + 2 * t);
+        x = fmaf(w_new, bf16_lo(v), x * w_old);
+        y = fmaf(w_new, bf16_hi(v), y * w_old);
+        if (g == 0 && len < p.T) *reinterpret_cast<uint32_t*>(p.v_cache + ((size_t)item * p.T + len) * HD + 8 * e + 2 * t) = v;
+      }
+      if (g < G && l != 0.f) *reinterpret_cast<float2*>(dst + 8 * e + 2 * t) = make_float2(x, y);
+    }
+    if (g < G && t == 0) p.ml_part[at] = make_float2(m, l);
+  }
+}
 
 template <int HD, bool ROTATE, bool PAIR>
 __global__ void __launch_bounds__(PX_THREADS, 1)
@@ -108,10 +341,19 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = 1 << p.gs;
-  // z: group (shared keys alone) or row; y: key head; x: query tile (or pair), and split for partial results
-  const int kvh = blockIdx.y, z = blockIdx.z;
-  const int qt = (int)(gridDim.x / p.splits) - 1 - (int)blockIdx.x / p.splits;      // longest first
-  const int split = blockIdx.x % p.splits;
+  if constexpr (ROTATE) {
+    if ((int)blockIdx.x < p.own_ctas) {
+      px_own_keys<HD>(p, tm_ok, tm_ov, px_smem);
+      return;
+    }
+  }
+  // z: group (shared keys alone) or row; kvh: key head; qt: query tile (or pair), longest first; split of the shared keys
+  int idx = (int)blockIdx.x - p.own_ctas;
+  const int split = idx % p.splits;
+  idx /= p.splits;
+  const int qt = p.tiles_q - 1 - idx % p.tiles_q;
+  idx /= p.tiles_q;
+  const int kvh = idx % p.nkv, z = idx / p.nkv;
   const int unit_tokens = p.own ? p.S : p.rows * p.S;             // tokens whose queries this launch packs together
   const int token0 = z * unit_tokens;
   const int q0 = qt * (PAIR ? 2 * PX_BM : PX_BM), n_rows = min(PAIR ? 2 * PX_BM : PX_BM, unit_tokens * G - q0);
@@ -445,7 +687,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
         }
       };
       if (p.partial) {
-        const size_t part = th * p.splits + split;
+        const size_t part = th * p.parts + split;
         if (row_on && (PAIR || w == 0)) p.ml_part[part] = make_float2(M, L);
         float4* dst = reinterpret_cast<float4*>(p.o_part + part * HD);
         if (n_tiles > 0) {
@@ -462,7 +704,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
         }
       } else {
         // join with the partial triples of the shared keys (none when this launch visited them), normalise, store the row
-        const int n_parts = p.join;
+        const int n_parts = p.shared ? 0 : p.parts;
         const bool seen = row_on && slot >= pad;                       // a query in front of its row's first token is padding: zeros
         const float2* ml = p.ml_part + th * n_parts;
         float M2 = M;
@@ -520,8 +762,66 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
   if (warp == 0) tc::tmem_dealloc(tmem, 512);
 }
 
+// Joins the triples of a step: a warp per (token, head).
+template <int HD>
+__global__ void __launch_bounds__(256) prefix_join_kernel(const float* __restrict__ o_part, const float2* __restrict__ ml_part, __nv_bfloat16* out, int rows, int parts) {
+  constexpr int V = HD / 32;                                           // columns of a lane
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (row >= rows) return;
+  const float2* ml = ml_part + (size_t)row * parts;
+  float m[3], w[3], M = -INFINITY, L = 0.f;                            // parts i, i + 32, i + 64
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const float2 v = lane + 32 * k < parts ? __ldcg(ml + lane + 32 * k) : make_float2(-INFINITY, 0.f);
+    m[k] = v.x; w[k] = v.y;
+    if (w[k] != 0.f) M = fmaxf(M, m[k]);                               // (a sum of zero: no keys, and no o was written; NaN stays NaN)
+  }
+  M = warp_max(M);
+  if (M == -INFINITY) M = 0.f;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const float f = w[k] != 0.f ? exp2f(m[k] - M) : 0.f;
+    L += f * w[k];
+    w[k] = f;
+  }
+  L = warp_sum(L);
+  const float* src = o_part + (size_t)row * parts * HD + V * lane;
+  float acc[V] = {};
+#pragma unroll 1
+  for (int i0 = 0; i0 < parts; i0 += 8) {                              // eight rows requested before the first is used
+    float x[8][V], f[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u, k = i >> 5;
+      f[u] = __shfl_sync(0xffffffffu, k == 0 ? w[0] : (k == 1 ? w[1] : w[2]), i & 31);
+      if (i >= parts) f[u] = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[u][e] = 0.f;
+      if (f[u] != 0.f) {
+        if constexpr (V == 4) {
+          const float4 a = __ldcg(reinterpret_cast<const float4*>(src + (size_t)i * HD));
+          x[u][0] = a.x; x[u][1] = a.y; x[u][2] = a.z; x[u][3] = a.w;
+        } else {
+          const float2 a = __ldcg(reinterpret_cast<const float2*>(src + (size_t)i * HD));
+          x[u][0] = a.x; x[u][1] = a.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = fmaf(f[u], x[u][e], acc[e]);
+  }
+  const float inv = 1.f / L;                                           // the new token is always seen: L > 0
+  uint32_t* dst = reinterpret_cast<uint32_t*>(out + (size_t)row * HD + V * lane);
+  if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+  else *dst = pack_bf16(acc[0] * inv, acc[1] * inv);
+}
+
 template <int HD, bool ROTATE, bool PAIR>
-static int px_launch(const PxParams& p, dim3 grid, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok, const CUtensorMap& ov, cudaStream_t st) {
+static int px_launch(const PxParams& p, unsigned ctas, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok, const CUtensorMap& ov, cudaStream_t st) {
   using Tile = PxTile<HD, ROTATE, PAIR>;
   // attributes belong to the device's context: set at the first call on each (bit per device; setting them twice is harmless)
   static std::atomic<uint64_t> set{0};
@@ -532,57 +832,83 @@ static int px_launch(const PxParams& p, dim3 grid, const CUtensorMap& pk, const 
     JL_CUDA(cudaFuncSetAttribute(prefix_attn_kernel<HD, ROTATE, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile::SMEM));
     set.fetch_or(bit, std::memory_order_release);
   }
-  JL_CUDA(launch_pdl(prefix_attn_kernel<HD, ROTATE, PAIR>, grid, dim3(PX_THREADS), (size_t)Tile::SMEM, st, pk, pv, ok, ov, p));
+  JL_CUDA(launch_pdl(prefix_attn_kernel<HD, ROTATE, PAIR>, dim3(ctas), dim3(PX_THREADS), (size_t)Tile::SMEM, st, pk, pv, ok, ov, p));
   return JL_OK;
 }
 
+static long px_tiles(long queries) { return queries > PX_BM ? (queries + 2 * PX_BM - 1) / (2 * PX_BM) : 1; }
+
 // One launch over tiles of the queries of `units` groups or rows, `queries` of a key head each.
-static int px_dispatch(const PxParams& p, long queries, int units, bool rotate, int hd, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok,
+static int px_dispatch(PxParams p, long queries, int units, bool rotate, int hd, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok,
                        const CUtensorMap& ov, cudaStream_t st) {
   const bool pair = queries > PX_BM;
-  const int tile = pair ? 2 * PX_BM : PX_BM;
-  const dim3 grid((unsigned)((queries + tile - 1) / tile * p.splits), p.nkv, units);
-#define JL_PX(HD_, R_, P_) if (hd == HD_ && rotate == R_ && pair == P_) return px_launch<HD_, R_, P_>(p, grid, pk, pv, ok, ov, st);
+  p.tiles_q = (int)px_tiles(queries);
+  const long ctas = p.own_ctas + (long)p.tiles_q * p.splits * p.nkv * units;
+  JL_CHECK_ARG(ctas < (1l << 31), "attention over a shared prefix: %ld tiles", ctas);
+#define JL_PX(HD_, R_, P_) if (hd == HD_ && rotate == R_ && pair == P_) return px_launch<HD_, R_, P_>(p, (unsigned)ctas, pk, pv, ok, ov, st);
   JL_PX(128, true, true) JL_PX(128, true, false) JL_PX(128, false, true) JL_PX(128, false, false)
   JL_PX(64, true, true) JL_PX(64, true, false) JL_PX(64, false, true) JL_PX(64, false, false)
 #undef JL_PX
   return JL_ERR_UNSUPPORTED;
 }
 
-constexpr int PX_MAX_SPLITS = 64, PX_SMS = 148;
+constexpr int PX_MAX_SPLITS = 64, PX_MAX_OWN = 16, PX_SMS = 148;
 
 // Time of a launch in units of a tile of keys: rounds of CTAs (one per SM) times the tiles of one and its way in and out.
-static float px_rounds(long queries, long units, int nkv, int splits, float tiles) {
-  const long tile = queries > PX_BM ? 2 * PX_BM : PX_BM;
-  const long ctas = (queries + tile - 1) / tile * units * nkv * splits;
-  return (float)((ctas + PX_SMS - 1) / PX_SMS) * (tiles + 5.f);
+static float px_rounds(long queries, long units, int nkv, int splits, float tiles, int sms = PX_SMS) {
+  const long ctas = px_tiles(queries) * units * nkv * splits;
+  return (float)((ctas + sms - 1) / sms) * (tiles + 5.f);
 }
 
-// Splits of the shared keys: the count with the least time, every one two tiles of keys or more; a split costs the triples' way to memory and back.
-static int px_splits(long queries, int groups, int nkv, int prefix, float* cost = nullptr) {
+// Splits of the shared keys over `sms` SMs: the count with the least time, every one two tiles of keys or more; a split costs the triples' way to memory and back.
+static int px_splits(long queries, int groups, int nkv, int prefix, int sms = PX_SMS, float* cost = nullptr) {
   const int tiles = (prefix + PX_BN - 1) / PX_BN;
   int best = 1;
   float least = 0.f;
   for (int s = 1; s <= PX_MAX_SPLITS && (s == 1 || 2 * s <= tiles); ++s) {
-    const float c = px_rounds(queries, groups, nkv, s, (float)((tiles + s - 1) / s)) + (float)(queries * groups * nkv) * s * 3e-4f;
+    const float c = px_rounds(queries, groups, nkv, s, (float)((tiles + s - 1) / s), sms) + (float)(queries * groups * nkv) * s * 3e-4f;
     if (s == 1 || c < least) { least = c; best = s; }
   }
   if (cost) *cost = least;
   return best;
 }
 
+// A step: CTAs and parts for the own keys (of caches of T slots, taken to be half full), splits for the shared keys on the other SMs.
+struct PxStep { int own_ctas, own_splits, splits; };
+static int px_own_splits(long items) {                                 // parts that give every warp of all SMs one
+  const long s = (8l * PX_SMS + items - 1) / items;
+  return (int)(s < 1 ? 1 : (s > PX_MAX_OWN ? PX_MAX_OWN : s));
+}
+static PxStep px_step(int B, int groups, int nkv, int G, int hd, int P, int T) {
+  PxStep r;
+  const long items = (long)B * nkv, queries = (long)(B / groups) * G;
+  const int most = px_own_splits(items), by_keys = (T + 127) / 128;
+  r.own_splits = most < by_keys ? most : by_keys;
+  const long full = (items * r.own_splits + 7) / 8;                    // CTAs with a unit for every warp
+  // SM time of both sides in us: 64 KB/us of own keys per SM and a way in and out per unit; a tile of shared keys
+  const float own = (float)items * ((float)T * 0.5f * (float)hd * 4.f / 64e3f + (float)r.own_splits * 0.5f);
+  const float tile = queries > PX_BM ? 1.1f : 0.65f;
+  const float shared = (float)(px_tiles(queries) * groups * nkv) * ((float)P / PX_BN * tile + 5.f);
+  long n = (long)(PX_SMS * own / (own + shared) + 0.5f);
+  n = n < 1 ? 1 : (n > PX_SMS - 8 ? PX_SMS - 8 : n);
+  r.own_ctas = (int)(n < full ? n : full);
+  r.splits = px_splits(queries, groups, nkv, P, PX_SMS - r.own_ctas);
+  const int cap = px_splits(queries, groups, nkv, P);                  // (what the scratch is sized for)
+  if (r.splits > cap) r.splits = cap;
+  return r;
+}
+
 // Whether one launch over shared and own keys together, every row's queries in tiles of their own, is estimated to be no slower than shared keys for all rows of a
 // group together and then the own keys.
 static bool px_one_launch(int S, int G, int B, int groups, int nkv, int P, int start) {
   float two;
-  px_splits((long)(B / groups) * S * G, groups, nkv, P, &two);
+  px_splits((long)(B / groups) * S * G, groups, nkv, P, PX_SMS, &two);
   const float own = (float)(start + S) / PX_BN;
   two += px_rounds((long)S * G, B, nkv, 1, own);
   return px_rounds((long)S * G, B, nkv, 1, (float)P / PX_BN + own) <= two;
 }
 
 static size_t px_part_bytes(long tokens, int nh, int hd, int splits) { return (size_t)tokens * nh * splits * (hd + 2) * sizeof(float); }
-static size_t px_up(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace jl
 
@@ -590,8 +916,10 @@ using namespace jl;
 
 extern "C" JL_API size_t jl_prefix_attn_scratch_bytes(int B, int S, int groups, int nh, int nkv, int hd, int prefix) {
   if (B < 1 || S < 1 || groups < 1 || B % groups != 0 || nkv < 1 || nh % nkv != 0 || prefix < 0) return 0;
-  const int G = nh / nkv, splits = px_splits((long)(B / groups) * S * G, groups, nkv, prefix);
-  return px_up(S == 1 ? prefix_step_scratch_bytes(B, nh, nkv, hd) : 0) + px_part_bytes((long)B * S, nh, hd, splits);
+  const int G = nh / nkv;
+  int parts = px_splits((long)(B / groups) * S * G, groups, nkv, prefix);
+  if (S == 1) parts += px_own_splits((long)B * nkv);
+  return px_part_bytes((long)B * S, nh, hd, parts);
 }
 
 static int px_check(const char* who, int B, int S, int groups, int nh, int nkv, int hd, int P, int T, const void* scratch, size_t scratch_bytes, const void* const* aligned,
@@ -618,26 +946,32 @@ extern "C" JL_API int jl_decode_attn_prefix(const void* qkv, const void* prefix_
   if (rc0) return rc0;
   JL_CHECK_ARG(cache_len != nullptr && max_pos >= 1, "jl_decode_attn_prefix: the slot of the new token and its tables are required");
   const int G = nh / nkv, rows = B / groups;
-  CUtensorMap pk, pv;
+  JL_CHECK_ARG((long)B * nkv <= (1l << 26), "jl_decode_attn_prefix: %d rows of %d key heads", B, nkv);
+  CUtensorMap pk, pv, ok, ov;
+  const int kpi = hd == 128 ? PxOwn<128>::KPI : PxOwn<64>::KPI;
   int rc = make_tmap_3d_bf16(&pk, prefix_k, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
   if (rc == JL_OK) rc = make_tmap_3d_bf16(&pv, prefix_v, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
+  if (rc == JL_OK) rc = make_tmap_3d_bf16(&ok, k_cache, (uint64_t)B * nkv, T, hd, (uint64_t)T * hd, hd, kpi);
+  if (rc == JL_OK) rc = make_tmap_3d_bf16(&ov, v_cache, (uint64_t)B * nkv, T, hd, (uint64_t)T * hd, hd, kpi);
   if (rc != JL_OK) return rc;
+  const PxStep plan = px_step(B, groups, nkv, G, hd, P, T);
   PxParams p{};
-  p.q = (const __nv_bfloat16*)qkv; p.ldq = (nh + 2 * nkv) * hd;
+  p.q = p.qkv = (const __nv_bfloat16*)qkv; p.ldq = (nh + 2 * nkv) * hd;
+  p.k_cache = (__nv_bfloat16*)k_cache; p.v_cache = (__nv_bfloat16*)v_cache;
   p.cos_t = cos_t; p.sin_t = sin_t; p.max_pos = max_pos; p.cache_len = cache_len;
   p.prefix_len = prefix_len; p.prefix_pad = prefix_pad; p.pad_left = pad_left;
-  p.S = 1; p.rows = rows; p.nh = nh; p.nkv = nkv; p.gs = G == 1 ? 0 : (G == 2 ? 1 : (G == 4 ? 2 : 3)); p.P = P; p.T = T;
+  p.S = 1; p.B = B; p.rows = rows; p.nh = nh; p.nkv = nkv; p.gs = G == 1 ? 0 : (G == 2 ? 1 : (G == 4 ? 2 : 3)); p.P = P; p.T = T;
   p.shared = 1; p.partial = 1;
-  p.splits = px_splits((long)rows * G, groups, nkv, P);
+  p.own_ctas = plan.own_ctas; p.own_splits = plan.own_splits; p.splits = plan.splits; p.parts = plan.splits + plan.own_splits;
   p.scale_log2 = scale * 1.4426950408889634f;
-  char* parts = (char*)scratch + px_up(prefix_step_scratch_bytes(B, nh, nkv, hd));
-  p.o_part = (float*)parts;
-  p.ml_part = (float2*)(p.o_part + (size_t)B * nh * p.splits * hd);
-  rc = px_dispatch(p, (long)rows * G, groups, true, hd, pk, pv, pk, pv, (cudaStream_t)stream);
+  p.o_part = (float*)scratch;
+  p.ml_part = (float2*)(p.o_part + (size_t)B * nh * p.parts * hd);
+  rc = px_dispatch(p, (long)rows * G, groups, true, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;
-  const PrefixStep step{(const __nv_bfloat16*)qkv, (__nv_bfloat16*)k_cache, (__nv_bfloat16*)v_cache, cos_t, sin_t, cache_len, pad_left, prefix_len, prefix_pad,
-                        (__nv_bfloat16*)out, scratch, B, rows, nh, nkv, hd, P, T, max_pos, scale, {p.o_part, p.ml_part, p.splits}};
-  return prefix_step_launch(step, (cudaStream_t)stream);
+  const dim3 grid((unsigned)(((long)B * nh + 7) / 8));
+  if (hd == 128) JL_CUDA(launch_pdl(prefix_join_kernel<128>, grid, dim3(256), 0, (cudaStream_t)stream, p.o_part, p.ml_part, (__nv_bfloat16*)out, B * nh, p.parts));
+  else JL_CUDA(launch_pdl(prefix_join_kernel<64>, grid, dim3(256), 0, (cudaStream_t)stream, p.o_part, p.ml_part, (__nv_bfloat16*)out, B * nh, p.parts));
+  return JL_OK;
 }
 
 extern "C" JL_API int jl_prefill_attn_prefix(const void* q, const void* prefix_k, const void* prefix_v, const void* k_cache, const void* v_cache,
@@ -668,11 +1002,11 @@ extern "C" JL_API int jl_prefill_attn_prefix(const void* q, const void* prefix_k
     return px_dispatch(p, (long)S * G, B, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   }
   const int splits = px_splits((long)rows * S * G, groups, nkv, P);
-  p.o_part = (float*)((char*)scratch + px_up(S == 1 ? prefix_step_scratch_bytes(B, nh, nkv, hd) : 0));
+  p.o_part = (float*)scratch;
   p.ml_part = (float2*)(p.o_part + (size_t)B * S * nh * splits * hd);
-  p.shared = p.partial = 1; p.splits = splits;
+  p.shared = p.partial = 1; p.splits = p.parts = splits;
   rc = px_dispatch(p, (long)rows * S * G, groups, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;
-  p.shared = p.partial = 0; p.own = 1; p.splits = 1; p.join = splits;
+  p.shared = p.partial = 0; p.own = 1; p.splits = 1;
   return px_dispatch(p, (long)S * G, B, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
 }

@@ -567,8 +567,8 @@ int jl_mlstm_finish(const float* o, const float* aux, const void* w, const float
 /* Attention of rows whose group shares keys (several answers to one prompt, many questions to one document).  Rows b of group b / (B / groups) attend the
  * shared keys [prefix_pad[g], prefix_len[g]) of prefix_k / prefix_v [groups][nkv][P][hd] (prefix_len == NULL: all P, prefix_pad == NULL: from 0) and their own
  * keys [pad_left[b], ..] of k_cache / v_cache [B][nkv][T][hd], softmax over both together.  hd 64 or 128, nh / nkv 1, 2, 4 or 8; all tensors start at 16-byte
- * boundaries.  `scratch` holds jl_prefix_attn_scratch_bytes(..) bytes whose first B nkv 32-bit words are zero before the first call (every call leaves them so);
- * calls that may run at the same time need one each.  Slots that hold no key may hold anything.
+ * boundaries.  `scratch` holds jl_prefix_attn_scratch_bytes(..) bytes of any content; calls that may run at the same time
+ * need one each.  Slots that hold no key may hold anything.
  *
  * jl_decode_attn_prefix: one new token per row.  qkv [B, (nh + 2 nkv) hd] not rotated; the token takes slot *cache_len of the row's own cache (nothing is stored at
  * *cache_len >= T) at rotary position (prefix_len - prefix_pad)[g] + *cache_len - pad_left[b]; its k and v are appended, out [B, nh hd].

@@ -425,9 +425,7 @@ def prefix_attn_scratch(B: int, S: int, groups: int, nh: int, nkv: int, hd: int,
     n = int(_lib.lib().jl_prefix_attn_scratch_bytes(B, S, groups, nh, nkv, hd, prefix))
     if n == 0:
         raise ValueError(f"prefix_attn_scratch: {B} rows of {S} tokens in {groups} groups, {nh} / {nkv} heads of {hd}, prefix {prefix}")
-    t = torch.empty((n + 15) // 16 * 4, dtype=torch.int32, device=device)
-    t[:min(B * nkv, t.numel())].zero_()                       # tickets
-    return t
+    return torch.empty((n + 15) // 16 * 4, dtype=torch.float32, device=device)
 
 
 def decode_attn_prefix(qkv: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cos: torch.Tensor,
