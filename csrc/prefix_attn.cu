@@ -34,7 +34,8 @@ template <int HD> struct PxOwn {
   static constexpr int WARPS = 8, STAGES = 3, HALVES = HD / 64;
   static constexpr int KPI = HD == 128 ? 16 : 32;                  // 8 KB of keys and values at either width
   static constexpr uint32_t BOX = KPI * 128, STAGE = 2 * HALVES * BOX, RING = STAGES * STAGE;
-  static constexpr uint32_t SMEM = WARPS * RING + WARPS * STAGES * 8 + 1024;
+  static constexpr uint32_t QT = 16 * HD * 2;                      // a unit's queries: 8 rows of high parts, 8 of low ones
+  static constexpr uint32_t SMEM = WARPS * (RING + QT) + 1024;
 };
 
 // PAIR: two tiles of queries per CTA, each with its own softmax warps, over the same keys; else one tile whose keys the two sets of softmax warps take in turn.
@@ -97,7 +98,7 @@ struct PxParams {
 };
 
 __device__ __forceinline__ void px_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void px_ldsm(uint32_t addr, uint32_t (&r)[4]) {
@@ -113,19 +114,17 @@ __device__ __forceinline__ void px_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
 // registers.  Bound by the cache's bytes; a block's chain of dependent steps takes about 0.6 us, so that a warp moves 13 GB/s and eight of them an SM's share
 // of the bandwidth twice over.
 template <int HD>
-__device__ __forceinline__ void px_own_keys(const PxParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint8_t* smem) {
+__device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
   using Own = PxOwn<HD>;
   constexpr int KPI = Own::KPI, HALVES = Own::HALVES, STAGES = Own::STAGES;
   constexpr int NT = KPI / 8, NB = KPI / 16, KS = HD / 16;
+  constexpr int CH = HD / 8, RPS = 32 / CH, PASSES = 8 / RPS;       // 16-byte chunks of a row, rows that a warp holds at once
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (warp >= Own::WARPS) return;
   const uint32_t raw = tc::smem_u32(smem), base0 = (raw + 1023u) & ~1023u;
-  const uint32_t ring = base0 + warp * Own::RING, bar0 = base0 + Own::WARPS * Own::RING + warp * STAGES * 8;
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < STAGES; ++i) tc::mbar_init(bar0 + 8 * i, 1);
-    tc::fence_barrier_init();
-  }
+  const uint32_t ring = base0 + warp * Own::RING, qt = base0 + Own::WARPS * Own::RING + warp * Own::QT;
+  for (int i = lane; i < (int)Own::QT / 16; i += 32)                  // rows without a head stay zero
+    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(qt + 16 * i), "r"(0) : "memory");
   __syncwarp();
   pdl_wait();
   pdl_launch_dependents();
@@ -143,24 +142,30 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, const CUtensorMap
   // what is asked for next: block [r_base, r_base + KPI) of unit r_u
   int r_u = blockIdx.x * Own::WARPS + warp, r_base = 0, r_hi = 0, r_st = 0;
   if (r_u < units) range(r_u, r_base, r_hi);
+  // 16-byte copies into the swizzled layout, eight 512-byte rows of requests each for keys and values; keys behind the last one become zeros (a weight of
+  // zero times a NaN is a NaN).  By TMA, whose boxes of 16 rows leave the SM at 28 bytes a cycle, the warps waited for its queue a third of their time.
+  const int r_ch = lane % CH, r_key = lane / CH;
   auto request = [&]() {
     while (r_u < units && r_base >= r_hi) {
       r_u += step;
       if (r_u < units) range(r_u, r_base, r_hi);
     }
-    if (r_u >= units) return;
-    if (lane == 0) {
-      const uint32_t dst = ring + r_st * Own::STAGE, bar = bar0 + 8 * r_st;
-      const int head = r_u / p.own_splits;                 // b · nkv + key head
-      tc::mbar_expect_tx(bar, Own::STAGE);
+    if (r_u < units) {
+      const uint32_t dst = ring + r_st * Own::STAGE + (r_ch >> 3) * Own::BOX;
+      const size_t src = ((size_t)(r_u / p.own_splits) * p.T + r_base + r_key) * HD + 8 * r_ch;
 #pragma unroll
-      for (int h = 0; h < HALVES; ++h) {
-        tc::tma_load_3d(dst + h * Own::BOX, &tm_k, bar, 64 * h, r_base, head, tc::EVICT_FIRST);
-        tc::tma_load_3d(dst + (HALVES + h) * Own::BOX, &tm_v, bar, 64 * h, r_base, head, tc::EVICT_FIRST);
+      for (int i = 0; i < KPI / RPS; ++i) {
+        const int key = i * RPS + r_key;
+        const uint32_t at = dst + key * 128 + (((r_ch & 7) ^ (key & 7)) << 4);
+        const bool on = r_base + key < r_hi;
+        const size_t from = on ? src + (size_t)(i * RPS) * HD : 0;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(p.k_cache + from), "r"(on ? 16 : 0) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + HALVES * Own::BOX), "l"(p.v_cache + from), "r"(on ? 16 : 0) : "memory");
       }
+      r_base += KPI;
+      if (++r_st == STAGES) r_st = 0;
     }
-    r_base += KPI;
-    if (++r_st == STAGES) r_st = 0;
+    asm volatile("cp.async.commit_group;" ::: "memory");       // (a group per block or an empty one: the count of groups behind a block stays the same)
   };
 #pragma unroll
   for (int i = 0; i < STAGES; ++i) request();
@@ -174,7 +179,6 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, const CUtensorMap
   for (int i = 0; i < 4; ++i) voff[i] = ((q8 & 1) * 8 + l7) * 128 + (((2 * i + (q8 >> 1)) ^ l7) << 4);
 
   int st = 0;
-  uint32_t phase = 0;
 #pragma unroll 1
   for (int u = blockIdx.x * Own::WARPS + warp; u < units; u += step) {
     int lo, hi;
@@ -182,38 +186,76 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, const CUtensorMap
     const int item = u / p.own_splits, part = u - item * p.own_splits, b = item / p.nkv, kvh = item - b * p.nkv;
     const int group = b / p.rows;
     const int g_lo = p.prefix_pad ? max(p.prefix_pad[group], 0) : 0, g_hi = p.prefix_len ? min(p.prefix_len[group], p.P) : p.P;
-    int pos = max(g_hi - g_lo, 0) + len - (p.pad_left ? p.pad_left[b] : 0);
-    pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
-    const float* cos_p = p.cos_t + (size_t)pos * (HD / 2);
-    const float* sin_p = p.sin_t + (size_t)pos * (HD / 2);
     const __nv_bfloat16* row = p.qkv + (size_t)b * (p.nh + 2 * p.nkv) * HD;
     const bool newest = part == p.own_splits - 1;
-
-    // query of head kvh · G + g, rotated: qa = high parts (a0, a2) of the k-steps, ql = low parts; and, in the newest part, its product with the new key
-    uint32_t qa[KS][2], ql[KS][2];
-    float s_new = 0.f;
+    // ---- the new token: chunk `ch` of query rows pass · RPS + lane / CH, and of its key and value
+    const int ch = lane % CH, rr = lane / CH;
+    uint4 qx[PASSES], kx = make_uint4(0, 0, 0, 0), vx = kx;
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int i = 0; i < PASSES; ++i)
+      if (i * RPS + rr < G) qx[i] = *reinterpret_cast<const uint4*>(row + (size_t)(kvh * G + i * RPS + rr) * HD + 8 * ch);
+    if (newest) {
+      kx = *reinterpret_cast<const uint4*>(row + (size_t)(p.nh + kvh) * HD + 8 * ch);
+      vx = *reinterpret_cast<const uint4*>(row + (size_t)(p.nh + p.nkv + kvh) * HD + 8 * ch);
+    }
+    int pos = max(g_hi - g_lo, 0) + len - (p.pad_left ? p.pad_left[b] : 0);
+    pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
+    const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t) + (size_t)pos * CH + ch);
+    const float4 s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t) + (size_t)pos * CH + ch);
+    const float cs[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
+    float kf[8];                                 // the new key, rotated and rounded as the cache holds it
+    {
+      const uint32_t x[4] = {kx.x, kx.y, kx.z, kx.w};
+      uint32_t a[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int pair = 8 * s + 4 * i + t;
-        const float c = __ldg(cos_p + pair), sn = __ldg(sin_p + pair);
-        float qr = 0.f, qi = 0.f;
-        if (g < G) {
-          const uint32_t x = *reinterpret_cast<const uint32_t*>(row + (size_t)(kvh * G + g) * HD + 2 * pair);
-          const float re = bf16_lo(x), im = bf16_hi(x);
-          qr = re * c - im * sn; qi = re * sn + im * c;
-        }
-        qa[s][i] = pack_bf16(qr, qi);
-        ql[s][i] = pack_bf16(qr - bf16_lo(qa[s][i]), qi - bf16_hi(qa[s][i]));
-        if (newest) {
-          const uint32_t x = *reinterpret_cast<const uint32_t*>(row + (size_t)(p.nh + kvh) * HD + 2 * pair);
-          const float re = bf16_lo(x), im = bf16_hi(x);
-          const uint32_t kx = pack_bf16(re * c - im * sn, re * sn + im * c);
-          s_new = fmaf(qr, bf16_lo(kx), fmaf(qi, bf16_hi(kx), s_new));
-          if (g == 0 && len < p.T) *reinterpret_cast<uint32_t*>(p.k_cache + ((size_t)item * p.T + len) * HD + 2 * pair) = kx;
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float re = bf16_lo(x[e]), im = bf16_hi(x[e]);
+        a[e] = pack_bf16(re * cs[e] - im * sn[e], re * sn[e] + im * cs[e]);
+        kf[2 * e] = bf16_lo(a[e]); kf[2 * e + 1] = bf16_hi(a[e]);
       }
+      if (newest && rr == 0 && len < p.T) {
+        const size_t slot = ((size_t)item * p.T + len) * HD + 8 * ch;
+        *reinterpret_cast<uint4*>(p.k_cache + slot) = make_uint4(a[0], a[1], a[2], a[3]);
+        *reinterpret_cast<uint4*>(p.v_cache + slot) = vx;
+      }
+    }
+    float s_new = 0.f;                           // of row g
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      if (i * RPS >= G) continue;                // warp-uniform
+      const int r = i * RPS + rr;
+      float dot = 0.f;
+      if (r < G) {
+        const uint32_t x[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
+        uint32_t a[4], c[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float re = bf16_lo(x[e]), im = bf16_hi(x[e]);
+          const float y = re * cs[e] - im * sn[e], z = re * sn[e] + im * cs[e];
+          a[e] = pack_bf16(y, z);
+          c[e] = pack_bf16(y - bf16_lo(a[e]), z - bf16_hi(a[e]));
+          dot = fmaf(y, kf[2 * e], fmaf(z, kf[2 * e + 1], dot));
+        }
+        const uint32_t at = qt + r * (HD * 2) + ((ch ^ r) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + 8 * HD * 2), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]) : "memory");
+      }
+      if (newest) {
+#pragma unroll
+        for (int d = CH / 2; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+        const float mine = __shfl_sync(0xffffffffu, dot, (g % RPS) * CH);
+        if (g / RPS == i) s_new = mine;
+      }
+    }
+    __syncwarp();
+    uint32_t qa[KS][4];                          // k-steps of the 16 rows
+#pragma unroll
+    for (int s = 0; s < KS; ++s) px_ldsm(qt + ((q8 & 1) * 8 + l7) * (HD * 2) + (((2 * s + (q8 >> 1)) ^ l7) << 4), qa[s]);
+    if (newest) {                                // the new values wait where the queries were
+      __syncwarp();
+      if (rr == 0) asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(qt + 16 * ch), "r"(vx.x), "r"(vx.y), "r"(vx.z), "r"(vx.w) : "memory");
+      __syncwarp();
+    }
 
     float m = -INFINITY, l = 0.f;                // row g: m is quad-uniform, l is this thread's share of the sum
     float o[HD / 8][4];                          // [0..1]: row g against P's high parts, [2..3]: against the low parts
@@ -223,29 +265,37 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, const CUtensorMap
       for (int i = 0; i < 4; ++i) o[e][i] = 0.f;
 #pragma unroll 1
     for (int base = lo; base < hi; base += KPI) {
-      tc::mbar_wait(bar0 + 8 * st, phase);
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      __syncwarp();
       const uint32_t ks = ring + st * Own::STAGE, vs = ks + HALVES * Own::BOX;
-      if (base + KPI > hi) {                     // value rows that hold no key: a weight of zero times a NaN is a NaN
-        for (int i = lane; i < (KPI - (hi - base)) * 8 * HALVES; i += 32) {
-          const int r = hi - base + i / (8 * HALVES), c = i % (8 * HALVES);
-          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vs + (c >> 3) * Own::BOX + r * 128 + (c & 7) * 16), "r"(0) : "memory");
+      // operands ahead of the products that take them: a load in front of each is 30 cycles apiece
+      uint32_t kr[NT][KS / 2][4];
+#pragma unroll
+      for (int i = 0; i < KS / 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) px_ldsm(ks + (i >> 1) * Own::BOX + j * 1024 + koff[i & 1], kr[j][i]);
+      float d[NT][2][4] = {};                    // two chains per 8 keys: half the latency of the dependent products
+#pragma unroll
+      for (int i = 0; i < KS / 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          px_mma(d[j][0], qa[2 * i][0], qa[2 * i][1], qa[2 * i][2], qa[2 * i][3], kr[j][i][0], kr[j][i][1]);
+          px_mma(d[j][1], qa[2 * i + 1][0], qa[2 * i + 1][1], qa[2 * i + 1][2], qa[2 * i + 1][3], kr[j][i][2], kr[j][i][3]);
         }
-        __syncwarp();
-      }
+      uint32_t vr[NB][HD / 16][4];
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e) px_ldsm_t(vs + (e >> 2) * Own::BOX + kb * 2048 + voff[e & 3], vr[kb][e]);
+      __syncwarp();                              // every lane has read the stage: it may be filled again
+      request();
+      if (++st == STAGES) st = 0;
       float c[NT][2];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        float d[2][4] = {};                      // two chains: half the latency of the dependent products
-#pragma unroll
-        for (int i = 0; i < KS / 2; ++i) {
-          uint32_t r[4];
-          px_ldsm(ks + (i >> 1) * Own::BOX + j * 1024 + koff[i & 1], r);
-          px_mma(d[0], qa[2 * i][0], ql[2 * i][0], qa[2 * i][1], ql[2 * i][1], r[0], r[1]);
-          px_mma(d[1], qa[2 * i + 1][0], ql[2 * i + 1][0], qa[2 * i + 1][1], ql[2 * i + 1][1], r[2], r[3]);
-        }
         const int key = base + 8 * j + 2 * t;
-        c[j][0] = key < hi ? ((d[0][0] + d[1][0]) + (d[0][2] + d[1][2])) * p.scale_log2 : -INFINITY;
-        c[j][1] = key + 1 < hi ? ((d[0][1] + d[1][1]) + (d[0][3] + d[1][3])) * p.scale_log2 : -INFINITY;
+        c[j][0] = key < hi ? ((d[j][0][0] + d[j][1][0]) + (d[j][0][2] + d[j][1][2])) * p.scale_log2 : -INFINITY;
+        c[j][1] = key + 1 < hi ? ((d[j][0][1] + d[j][1][1]) + (d[j][0][3] + d[j][1][3])) * p.scale_log2 : -INFINITY;
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -278,23 +328,16 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, const CUtensorMap
         const uint32_t l2 = pack_bf16(c1[0] - bf16_lo(h2), c1[1] - bf16_hi(h2));
 #pragma unroll
         for (int e = 0; e < HD / 16; ++e) {
-          uint32_t r[4];
-          px_ldsm_t(vs + (e >> 2) * Own::BOX + kb * 2048 + voff[e & 3], r);
-          px_mma(o[2 * e], h0, l0, h2, l2, r[0], r[1]);
-          px_mma(o[2 * e + 1], h0, l0, h2, l2, r[2], r[3]);
+          px_mma(o[2 * e], h0, l0, h2, l2, vr[kb][e][0], vr[kb][e][1]);
+          px_mma(o[2 * e + 1], h0, l0, h2, l2, vr[kb][e][2], vr[kb][e][3]);
         }
       }
-      __syncwarp();                              // every lane has read the stage: it may be filled again
-      request();
-      if (++st == STAGES) { st = 0; phase ^= 1; }
     }
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     const size_t th = (size_t)b * p.nh + kvh * G + (g < G ? g : 0), at = th * p.parts + p.splits + part;
     float w_old = 1.f, w_new = 0.f;
     if (newest) {                                // one more key
-      s_new += __shfl_xor_sync(0xffffffffu, s_new, 1);
-      s_new += __shfl_xor_sync(0xffffffffu, s_new, 2);
       s_new *= p.scale_log2;
       const float m_new = fmaxf(m, s_new), m_safe = m_new == -INFINITY ? 0.f : m_new;
       w_old = exp2f(m - m_safe);
@@ -307,14 +350,15 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, const CUtensorMap
     for (int e = 0; e < HD / 8; ++e) {
       float x = o[e][0] + o[e][2], y = o[e][1] + o[e][3];
       if (newest) {
-        const uint32_t v = *reinterpret_cast<const uint32_t*>(row + (size_t)(p.nh + p.nkv + kvh) * HD + 8 * e + 2 * t);
+        uint32_t v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(qt + 16 * e + 4 * t) : "memory");
         x = fmaf(w_new, bf16_lo(v), x * w_old);
         y = fmaf(w_new, bf16_hi(v), y * w_old);
-        if (g == 0 && len < p.T) *reinterpret_cast<uint32_t*>(p.v_cache + ((size_t)item * p.T + len) * HD + 8 * e + 2 * t) = v;
       }
       if (g < G && l != 0.f) *reinterpret_cast<float2*>(dst + 8 * e + 2 * t) = make_float2(x, y);
     }
     if (g < G && t == 0) p.ml_part[at] = make_float2(m, l);
+    __syncwarp();                                // the next unit's queries take the place of the new values
   }
 }
 
@@ -343,7 +387,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
   const int G = 1 << p.gs;
   if constexpr (ROTATE) {
     if ((int)blockIdx.x < p.own_ctas) {
-      px_own_keys<HD>(p, tm_ok, tm_ov, px_smem);
+      px_own_keys<HD>(p, px_smem);
       return;
     }
   }
@@ -947,12 +991,9 @@ extern "C" JL_API int jl_decode_attn_prefix(const void* qkv, const void* prefix_
   JL_CHECK_ARG(cache_len != nullptr && max_pos >= 1, "jl_decode_attn_prefix: the slot of the new token and its tables are required");
   const int G = nh / nkv, rows = B / groups;
   JL_CHECK_ARG((long)B * nkv <= (1l << 26), "jl_decode_attn_prefix: %d rows of %d key heads", B, nkv);
-  CUtensorMap pk, pv, ok, ov;
-  const int kpi = hd == 128 ? PxOwn<128>::KPI : PxOwn<64>::KPI;
+  CUtensorMap pk, pv;
   int rc = make_tmap_3d_bf16(&pk, prefix_k, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
   if (rc == JL_OK) rc = make_tmap_3d_bf16(&pv, prefix_v, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
-  if (rc == JL_OK) rc = make_tmap_3d_bf16(&ok, k_cache, (uint64_t)B * nkv, T, hd, (uint64_t)T * hd, hd, kpi);
-  if (rc == JL_OK) rc = make_tmap_3d_bf16(&ov, v_cache, (uint64_t)B * nkv, T, hd, (uint64_t)T * hd, hd, kpi);
   if (rc != JL_OK) return rc;
   const PxStep plan = px_step(B, groups, nkv, G, hd, P, T);
   PxParams p{};
@@ -966,7 +1007,7 @@ extern "C" JL_API int jl_decode_attn_prefix(const void* qkv, const void* prefix_
   p.scale_log2 = scale * 1.4426950408889634f;
   p.o_part = (float*)scratch;
   p.ml_part = (float2*)(p.o_part + (size_t)B * nh * p.parts * hd);
-  rc = px_dispatch(p, (long)rows * G, groups, true, hd, pk, pv, ok, ov, (cudaStream_t)stream);
+  rc = px_dispatch(p, (long)rows * G, groups, true, hd, pk, pv, pk, pv, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;
   const dim3 grid((unsigned)(((long)B * nh + 7) / 8));
   if (hd == 128) JL_CUDA(launch_pdl(prefix_join_kernel<128>, grid, dim3(256), 0, (cudaStream_t)stream, p.o_part, p.ml_part, (__nv_bfloat16*)out, B * nh, p.parts));
