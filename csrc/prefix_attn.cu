@@ -44,13 +44,17 @@ template <int HD, bool ROTATE, bool PAIR> struct PxTile {
   static constexpr uint32_t Q_HALF = PX_BM * 128, Q = HALVES * Q_HALF;       // bytes of a tile of queries (hi or lo)
   static constexpr int NQ = ROTATE ? 2 : 1;                                  // hi, lo
   static constexpr uint32_t QS = (PAIR ? 2 : 1) * NQ * Q;
-  static constexpr uint32_t KV_HALF = PX_BN * 128, SLOT = 2 * HALVES * KV_HALF;        // a tile of keys and its values
+  static constexpr uint32_t KV_HALF = PX_BN * 128, KV = HALVES * KV_HALF;    // 64 columns of a tile of keys or values, all of them
+  // A slot of the ring holds both (PAIR: one wait and one release per tile, the warps that issue products have none to spare), or keys and values in turn (the keys'
+  // place is free again as soon as their scores are there: with both in one slot the four tiles that the two sets work on held the whole ring, and the keys of 48
+  // rows x 32 heads came in at 29 GB/s per SM)
+  static constexpr uint32_t SLOT = (PAIR ? 2 : 1) * KV;
   static constexpr uint32_t SMALL = 512 + (PAIR ? 0 : 2048);                 // barriers, the address of the TMEM columns; (m, l) of 2 x 128 rows
   static constexpr int FIT = (int)((227 * 1024 - 1024 - SMALL - QS) / SLOT);
-  static constexpr int SLOTS = FIT < 8 ? FIT : 8;                            // tiles in flight (96 KB or more; a memory latency needs about 50 per SM)
+  static constexpr int SLOTS = FIT < 16 ? FIT : 16;
   static constexpr uint32_t NEED = QS + SLOTS * SLOT + SMALL + 1024;         // (1024: alignment of the base)
   static constexpr uint32_t SMEM = ROTATE && NEED < PxOwn<HD>::SMEM ? PxOwn<HD>::SMEM : NEED;
-  static_assert(SLOTS >= 3 && SMEM <= 227 * 1024, "a tile ahead of the products");
+  static_assert(SLOTS >= (PAIR ? 3 : 8) && SMEM <= 227 * 1024, "a tile ahead of the products");
 };
 
 // Two fp32 numbers at once (fma.rn.f32x2 and add.rn.f32x2: one issue slot for both).
@@ -94,6 +98,7 @@ struct PxParams {
   // ROTATE: the CTAs in front take the own keys, `own_splits` parts of every (row, key head)
   const __nv_bfloat16* qkv; __nv_bfloat16* k_cache; __nv_bfloat16* v_cache;
   int own_ctas, own_splits, B, tiles_q;
+  int p_low;                        // one tile of queries: probabilities as two bfloat16 numbers
   float scale_log2;
 };
 
@@ -454,7 +459,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
     if (lane == 0) {
       int sl = 0;
       uint32_t ph = 1;
-      for (int j = 0; j < n_tiles; ++j) {
+      for (int idx = 0; idx < (PAIR ? 1 : 2) * n_tiles; ++idx) {       // tiles, or K_0, V_0, K_1, V_1, ...
+        const int j = PAIR ? idx : idx >> 1;
         const bool mine = j >= n_shared;
         const int key0 = mine ? o_lo + (j - n_shared) * PX_BN : s_lo + j * PX_BN;
         const int head = (mine ? z : group) * p.nkv + kvh;
@@ -462,11 +468,14 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
         const CUtensorMap* mv = mine ? &tm_ov : &tm_pv;
         tc::mbar_wait(slot_empty(sl), ph);
         tc::mbar_expect_tx(slot_full(sl), Tile::SLOT);
+        const CUtensorMap* m0 = !PAIR && (idx & 1) ? mv : mk;
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) tc::tma_load_3d(ring + sl * Tile::SLOT + h * Tile::KV_HALF, mk, slot_full(sl), 64 * h, key0, head, tc::EVICT_NORMAL);
+        for (int h = 0; h < HALVES; ++h) tc::tma_load_3d(ring + sl * Tile::SLOT + h * Tile::KV_HALF, m0, slot_full(sl), 64 * h, key0, head, tc::EVICT_NORMAL);
+        if constexpr (PAIR) {
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h)
-          tc::tma_load_3d(ring + sl * Tile::SLOT + (HALVES + h) * Tile::KV_HALF, mv, slot_full(sl), 64 * h, key0, head, tc::EVICT_NORMAL);
+          for (int h = 0; h < HALVES; ++h)
+            tc::tma_load_3d(ring + sl * Tile::SLOT + Tile::KV + h * Tile::KV_HALF, mv, slot_full(sl), 64 * h, key0, head, tc::EVICT_NORMAL);
+        }
         if (++sl == SLOTS) { sl = 0; ph ^= 1; }
       }
     }
@@ -477,12 +486,12 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
     const int w = warp == 1 ? 0 : 1, mine = tiles_of(w);
     constexpr uint32_t IDESC_S = tc::idesc_bf16_f32(PX_BM, PX_BN, false, false);
     constexpr uint32_t IDESC_O = tc::idesc_bf16_f32(PX_BM, HD, false, true);        // B = V is MN-major
-    constexpr int STEP = PAIR ? 1 : 2;                                 // tiles from one of this set's to the next
+    constexpr int STEP = PAIR ? 1 : 4;                                 // slots from one of this set's tiles to the next
     const uint64_t dQ = tc::smem_desc_kmajor_sw128(sQ + (PAIR ? w * NQ * Tile::Q : 0));
     const uint64_t dK0 = tc::smem_desc_kmajor_sw128(ring);
-    const uint64_t dV0 = tc::smem_desc_mnmajor_sw128(ring + HALVES * Tile::KV_HALF, Tile::KV_HALF, 1024);
-    int k_sl = tile_at(w, 0), v_sl = k_sl;                             // slots of the next scores and of the next product
-    uint32_t k_ph = 0;
+    const uint64_t dV0 = tc::smem_desc_mnmajor_sw128(ring + (PAIR ? Tile::KV : 0), Tile::KV_HALF, 1024);
+    int k_sl = PAIR ? 0 : 2 * w, v_sl = PAIR ? 0 : 2 * w + 1;          // slots of the next scores and of the next product
+    uint32_t k_ph = 0, v_ph = 0;
     auto next_slot = [&](int& sl) { sl += STEP; if (sl >= SLOTS) { sl -= SLOTS; return 1u; } return 0u; };
     auto issue_s = [&](int i) {
       tc::mbar_wait(slot_full(k_sl), k_ph);
@@ -496,6 +505,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
             tc::mma_ss(tS(w, i), dQ + (uint64_t)((n * Tile::Q + (k >> 2) * Tile::Q_HALF + (k & 3) * 32) >> 4),
                        dK + (uint64_t)(((k >> 2) * Tile::KV_HALF + (k & 3) * 32) >> 4), IDESC_S, n != 0 || k != 0);
         tc::mma_commit(s_full(w, i));
+        if (!PAIR) tc::mma_commit(slot_empty(k_sl));
       }
       __syncwarp();
       k_ph ^= next_slot(k_sl);
@@ -509,12 +519,13 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
     }
     for (int i = 0; i < mine; ++i) {
       if (i + 1 < mine) issue_s(i + 1);                                // the tensor core forms the next scores during this tile's softmax
+      if (!PAIR) tc::mbar_wait(slot_full(v_sl), v_ph);
       const int j = tile_at(w, i);
       const int left = j < n_shared ? s_hi - s_lo - j * PX_BN : o_hi - o_lo - (j - n_shared) * PX_BN;
       if (left < PX_BN) {                                              // value rows that hold no key (both sets write the same zeros)
         for (int e = lane; e < (PX_BN - left) * 8 * HALVES; e += 32) {
           const int r = left + e / (8 * HALVES), c = e % (8 * HALVES);
-          const uint32_t a = ring + v_sl * Tile::SLOT + (HALVES + (c >> 3)) * Tile::KV_HALF + r * 128 + (c & 7) * 16;
+          const uint32_t a = ring + v_sl * Tile::SLOT + (PAIR ? Tile::KV : 0) + (c >> 3) * Tile::KV_HALF + r * 128 + (c & 7) * 16;
           asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -526,12 +537,12 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
         const uint64_t dV = dV0 + (uint64_t)v_sl * (Tile::SLOT >> 4);
 #pragma unroll
         for (int k = 0; k < (PAIR ? 1 : 2) * PX_BN / 16; ++k)          // A = P in TMEM: 16 keys = 8 columns of packed pairs; the low parts behind the high ones
-          tc::mma_ts(tO(w), tS(w, i) + k * 8, dV + (uint64_t)(((k & 3) * 2048) >> 4), IDESC_O, i != 0 || k != 0);
+          if (k < 4 || p.p_low) tc::mma_ts(tO(w), tS(w, i) + k * 8, dV + (uint64_t)(((k & 3) * 2048) >> 4), IDESC_O, i != 0 || k != 0);
         tc::mma_commit(slot_empty(v_sl));
         if (i + 2 >= mine) tc::mma_commit(o_last(w, i + 2 - mine));
       }
       __syncwarp();
-      next_slot(v_sl);
+      v_ph ^= next_slot(v_sl);
     }
   } else {
     const int w = warp >= 6 ? 1 : 0;                                   // set of softmax warps (2..5, 6..9)
@@ -662,9 +673,9 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
           }
           sum = f2_add(sum, f2(a, b));
           hi[e] = pack_bf16(a, b);
-          if constexpr (!PAIR) lo[e] = pack_bf16(a - bf16_lo(hi[e]), b - bf16_hi(hi[e]));
+          if (!PAIR && p.p_low) lo[PAIR ? 0 : e] = pack_bf16(a - bf16_lo(hi[e]), b - bf16_hi(hi[e]));
         };
-        if (PAIR && !odd) {
+        if (!odd && (PAIR || !p.p_low)) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) pair(e, (e * PX_POLY) % 16 < PX_POLY);
         } else {
@@ -675,7 +686,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
         f2_get(sum, psum, psum2);
         psum += psum2;
         tc::tmem_st32(tS(w, i) + lane_off, hi);                        // keys 2c, 2c + 1 of this row: 32-bit column c
-        if constexpr (!PAIR) tc::tmem_st32(tS(w, i) + lane_off + 32, lo);
+        if constexpr (!PAIR) if (p.p_low) tc::tmem_st32(tS(w, i) + lane_off + 32, lo);
         tc::tmem_st_wait();
         l_run += psum;
       }
@@ -887,6 +898,7 @@ static int px_dispatch(PxParams p, long queries, int units, bool rotate, int hd,
                        const CUtensorMap& ov, cudaStream_t st) {
   const bool pair = queries > PX_BM;
   p.tiles_q = (int)px_tiles(queries);
+  p.p_low = queries <= PX_BM;
   const long ctas = p.own_ctas + (long)p.tiles_q * p.splits * p.nkv * units;
   JL_CHECK_ARG(ctas < (1l << 31), "attention over a shared prefix: %ld tiles", ctas);
 #define JL_PX(HD_, R_, P_) if (hd == HD_ && rotate == R_ && pair == P_) return px_launch<HD_, R_, P_>(p, (unsigned)ctas, pk, pv, ok, ov, st);
@@ -900,8 +912,11 @@ constexpr int PX_MAX_SPLITS = 64, PX_MAX_OWN = 16, PX_SMS = 148;
 
 // Time of a launch in units of a tile of keys: rounds of CTAs (one per SM) times the tiles of one and its way in and out.
 static float px_rounds(long queries, long units, int nkv, int splits, float tiles, int sms = PX_SMS) {
-  const long ctas = px_tiles(queries) * units * nkv * splits;
-  return (float)((ctas + sms - 1) / sms) * (tiles + 5.f);
+  const long full = queries > PX_BM ? queries / (2 * PX_BM) : 1, rest = px_tiles(queries) - full;      // whole pairs, one that may be half a pair
+  const long ctas = (full + rest) * units * nkv * splits;
+  const float whole = tiles + 5.f, part = rest && queries % (2 * PX_BM) <= PX_BM ? 0.78f * tiles + 5.f : whole;
+  if (part == whole || ctas <= sms) return (float)((ctas + sms - 1) / sms) * (full ? whole : part);
+  return (float)(units * nkv * splits) * (full * whole + rest * part) / sms + 0.5f * whole;
 }
 
 // Splits of the shared keys over `sms` SMs: the count with the least time, every one two tiles of keys or more; a split costs the triples' way to memory and back.
@@ -935,7 +950,9 @@ static PxStep px_step(int B, int groups, int nkv, int G, int hd, int P, int T) {
   const float shared = (float)(px_tiles(queries) * groups * nkv) * ((float)P / PX_BN * tile + 5.f);
   long n = (long)(PX_SMS * own / (own + shared) + 0.5f);
   n = n < 1 ? 1 : (n > PX_SMS - 8 ? PX_SMS - 8 : n);
-  r.own_ctas = (int)(n < full ? n : full);
+  // the same number of units for every warp, or one less
+  const long rounds = (2 * full + n) / (2 * n);
+  r.own_ctas = (int)((full + (rounds > 0 ? rounds : 1) - 1) / (rounds > 0 ? rounds : 1));
   r.splits = px_splits(queries, groups, nkv, P, PX_SMS - r.own_ctas);
   const int cap = px_splits(queries, groups, nkv, P);                  // (what the scratch is sized for)
   if (r.splits > cap) r.splits = cap;
