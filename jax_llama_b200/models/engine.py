@@ -27,7 +27,8 @@ import torch
 from ..config import LLaMAConfig
 from ..ops import _lib
 from ..ops import kernels as K
-from .reference import KVCache, ModelOutput, rope_cos_sin
+from ..ops.rules import BoundRules, LogitRules
+from .reference import KVCache, ModelOutput, join_prefix, rope_cos_sin
 
 logger = logging.getLogger(__name__)
 
@@ -35,10 +36,26 @@ Tree = Dict[str, Any]
 
 
 @dataclass
+class SharedPrefix:
+    """Keys and values in front of the rows of a batch, held once per group of neighbouring rows."""
+
+    k: torch.Tensor                             # [L, groups, nkv, P, hd]
+    v: torch.Tensor
+    length: torch.Tensor                        # int32 [groups]: shared keys lie in slots [pad, length)
+    pad: torch.Tensor                           # int32 [groups]
+    scratch: Optional[torch.Tensor] = None      # of the one-token attention: one per cache, its steps follow each other on one stream
+
+    def counts(self, rows: int) -> torch.Tensor:
+        """Shared keys in front of every row, int32 [rows]."""
+        return (self.length - self.pad).repeat_interleave(rows // self.length.shape[0])
+
+
+@dataclass
 class DeviceKVCache(KVCache):
-    """KV cache whose fill level also lives on the device (read by kernels, advanced by kernels)."""
+    """KV cache whose fill level also lives on the device (read by kernels, advanced by kernels).  With `prefix` it holds the rows' own keys only."""
 
     len_dev: Optional[torch.Tensor] = None      # int32 [1]
+    prefix: Optional[SharedPrefix] = None
 
     def set_index(self, value: int) -> None:
         self.index = int(value)
@@ -87,6 +104,12 @@ class DecodeState:
     splits: int
     scratch: Optional[torch.Tensor]
     graphs: Dict[Tuple, torch.cuda.CUDAGraph] = field(default_factory=dict)
+    # what a request asks of its tokens: the rules in force, their result [B, V], where the answer begins in `sequences` and where its rows do
+    rules: Optional[BoundRules] = None
+    rule_sets: Dict[Tuple, BoundRules] = field(default_factory=dict)
+    ruled: Optional[torch.Tensor] = None
+    prompt_len: Optional[torch.Tensor] = None
+    seq_pad: Optional[torch.Tensor] = None
 
 
 class B200Engine:
@@ -324,14 +347,28 @@ class B200Engine:
         # (see below) only the graph-replayed batched decode of a TP engine takes the fused all-reduce + norm form
         fuse_norm = (self.tp > 1 and S == 1 and positions is None and ws is not None and 4 < B <= 128
                      and os.environ.get("JLLAMA_TP_FUSE_NORM", "1") != "0")
-        xn = None
+        xn = prefix_ws = None
+        if cache.prefix is not None and not (S == 1 and positions is None):
+            groups, P = cache.prefix.k.shape[1], cache.prefix.k.shape[3]
+            prefix_ws = K.prefix_attn_scratch(B, S, groups, nh, nkv, hd, P, self.device)      # one for all layers
         for i, l in enumerate(self.layers):
             kc, vc = cache.k[i], cache.v[i]
             if xn is None:
                 qkv = K.linear(x, l.wqkv, norm_w=l.attn_norm, eps=eps, out=ws.qkv if ws else None)
             else:
                 qkv = K.linear(xn, l.wqkv, out=ws.qkv if ws else None)      # normalised by the previous layer's all-reduce
-            if S == 1 and positions is None:
+            pre = cache.prefix
+            if pre is not None and S == 1 and positions is None:
+                attn = K.decode_attn_prefix(qkv, pre.k[i], pre.v[i], kc, vc, self.cos, self.sin, cache.len_dev, cache.pad_left, pre.length, pre.pad,
+                                            nh, nkv, hd, scratch=pre.scratch, out=ws.attn if ws else None)
+            elif pre is not None:
+                # positions count the shared keys too (`forward` passes them)
+                q_rot = torch.empty((B * S, nh * hd), dtype=qkv.dtype, device=qkv.device)
+                K.rope_kv_write(qkv, kc, vc, self.cos, self.sin, B, S, nh, nkv, hd, cache_len=cache.len_dev, pad_left=cache.pad_left,
+                                positions=positions, q_out=q_rot)
+                attn = K.prefill_attn_prefix(q_rot.view(B, S, nh, hd), pre.k[i], pre.v[i], kc, vc, start, S, cache.pad_left, pre.length, pre.pad,
+                                             scratch=prefix_ws).view(B * S, nh * hd)
+            elif S == 1 and positions is None:
                 # decode: RoPE + KV append + split-KV attention + merge in one launch
                 attn = K.decode_attn_fused(qkv, kc, vc, self.cos, self.sin, cache.len_dev, cache.pad_left, nh, nkv,
                                            hd, ws.splits if ws else 1, ws.scratch if ws else None,
@@ -520,6 +557,9 @@ class B200Engine:
         positions = None
         if position_ids is not None:
             positions = position_ids.to(torch.int32).reshape(-1).contiguous()
+        elif cache.prefix is not None and S > 1:
+            slots = cache.index + torch.arange(S, dtype=torch.int32, device=self.device)
+            positions = (cache.prefix.counts(B)[:, None] + slots[None] - cache.pad_left[:, None]).clamp(min=0).reshape(-1).contiguous()
         if (self.tp > 1 and S > 1 and last_only and with_head and positions is None and self.hd == 128
                 and (B * S) % (128 * self.tp) == 0 and self.sequence_parallel_prefill):
             # sequence-parallel prefill: all-gather→GEMM and GEMM→reduce-scatter fused over NVLink peer memory
@@ -591,11 +631,12 @@ class B200Engine:
             if val is st:
                 del self._decode_states[key]
         st.graphs.clear()
-        st._cache = None
+        st._cache = st._front_cache = None
 
     # ------------------------------------------------------------------ decode state + graph
-    def _decode_state(self, B: int, max_len: int) -> DecodeState:
-        key = (B, max_len)
+    def _decode_state(self, B: int, max_len: int, shared: Tuple[int, ...] = ()) -> DecodeState:
+        """`shared`: (groups, P) of a batch behind shared prefixes."""
+        key = (B, max_len, *shared)
         if key in self._decode_states:
             return self._decode_states[key]
         c, dev = self.config, self.device
@@ -667,14 +708,35 @@ class B200Engine:
         counters, on device: one launch of the exact full-vocabulary kernel (csrc/sample_full.cu), at tp > 1 after an
         NVLS gather of the shards so that every rank selects from identical logits."""
         full = st.logits if self.tp == 1 else self._gather_logits(st)
-        self._sample_full(st, cache, sampling, eos, pad, full, wait_mega=False)
+        self._sample_full(st, cache, sampling, eos, pad, self._ruled(st, cache, full), wait_mega=False)
+
+    def _ruled(self, st: DecodeState, cache: DeviceKVCache, logits: torch.Tensor) -> torch.Tensor:
+        """The logits under the request's rules (`st.logits` stays what the model said)."""
+        if st.rules is None:
+            return logits
+        return st.rules.apply(logits, st.sequences, st.cur_len, st.prompt_len, cache.pad_left if cache.prefix is None else st.seq_pad, out=st.ruled)
+
+    def _set_rules(self, st: DecodeState, rules: Optional[LogitRules], prompt: int, rows: int, repeat: int) -> None:
+        """The rules of a new request batch: `rows` prompts of `prompt` tokens with `repeat` answers each.  Their tensors stay where a captured step of rules of
+        the same form expects them."""
+        st.rules = None
+        if rules is None or not rules.active:
+            return
+        bound = rules.bind(rows, self.config.vocab_size, self.device, repeat)
+        key = bound.structure()
+        st.rules = st.rule_sets[key].copy_(bound) if key in st.rule_sets else st.rule_sets.setdefault(key, bound)
+        if st.ruled is None:
+            st.ruled = torch.empty(st.B, self.config.vocab_size, dtype=torch.float32, device=self.device)
+            st.prompt_len = torch.zeros(1, dtype=torch.int32, device=self.device)
+        st.prompt_len.fill_(int(prompt))
 
     def _decode_step(self, st: DecodeState, cache: DeviceKVCache, sampling: Tuple, eos: int, pad: int) -> None:
         """One token for every row: ids → logits → next ids.  All state on device; capturable."""
         c = self.config
         if self.comm is not None:
             self.comm.begin_sequence()
-        if self._mega_fits(st.B):
+        # (rules under tensor parallelism read the gathered logits, which the whole-step kernel's selection waits for itself)
+        if self._mega_fits(st.B) and cache.prefix is None and not (st.rules is not None and self.tp > 1):
             # whole model in one persistent kernel: embedding → L layers → final norm → LM head (+ running arg-max)
             L = _lib.lib()
             sms = K.num_sms(self.device)
@@ -688,7 +750,7 @@ class B200Engine:
             if do_sample and self.tp > 1:
                 # sampling under tensor parallelism: every rank's shard goes into every rank's [B, V] buffer (multimem.st)
                 logits_args = (self._logits_full_mc, c.vocab_size, self.rank * self.v_local, 1)
-            elif do_sample or self.mega_write_logits:
+            elif do_sample or self.mega_write_logits or st.rules is not None:
                 logits_args = (st.logits.data_ptr(), self.v_local, 0, 0)
             else:
                 logits_args = (None, 0, 0, 0)
@@ -703,7 +765,7 @@ class B200Engine:
                 len(self.layers), c.hidden_size, c.intermediate_size // self.tp, self.v_local, c.vocab_size,
                 self.nh, self.nkv, self.hd, cache.capacity, self.cos.shape[0], float(c.rms_norm_eps),
                 1.0 / (self.hd ** 0.5), sms, *tp_args, K._stream()), "jl_decode_mega")
-            if not do_sample:
+            if not do_sample and st.rules is None:
                 # greedy: the kernel left one candidate per CTA (and rank); merge + bookkeeping in one launch
                 cand = st.mega_cand if self.tp == 1 else self._mega_peer[5]
                 _lib.check(L.jl_mega_select(
@@ -716,7 +778,7 @@ class B200Engine:
                 return
             # sampling: exact full-vocabulary kernel on the logits the decode kernel just wrote (second and last launch)
             full = st.logits if self.tp == 1 else self._logits_full[:st.B]
-            self._sample_full(st, cache, sampling, eos, pad, full, wait_mega=True)
+            self._sample_full(st, cache, sampling, eos, pad, self._ruled(st, cache, full), wait_mega=True)
             if self.comm is not None:
                 self.comm.end_sequence()
             return
@@ -737,12 +799,13 @@ class B200Engine:
                    ) -> Optional[torch.cuda.CUDAGraph]:
         if not self.use_cuda_graph:
             return None
-        key = (cache.k.data_ptr(), sampling, eos, pad)
+        key = (cache.k.data_ptr(), sampling, eos, pad, st.rules.structure() if st.rules is not None else None)
         if key in st.graphs:
             return st.graphs[key]
         # warm up outside capture on a side stream (first-use initialisation, cudaFuncSetAttribute, …);
         # the step is re-playable because a snapshot of the mutable state is restored afterwards
-        mutable = (st.ids, st.finished, st.sequences, st.cur_len, st.step, st.n_unfinished, st.logits, *cache.mutable_state())
+        mutable = (st.ids, st.finished, st.sequences, st.cur_len, st.step, st.n_unfinished, st.logits, *([] if st.rules is None else [st.ruled]),
+                   *cache.mutable_state())
         snap = [t.clone() for t in mutable]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
@@ -770,15 +833,20 @@ class B200Engine:
     def generate(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None, *,
                  max_length: int, do_sample: bool = False, temperature: float = 1.0,
                  top_k: Optional[int] = 50, top_p: float = 1.0, pad_token_id: int = 0, eos_token_id: int = -1,
-                 seed: int = 0, check_every: int = 16) -> torch.Tensor:
-        """Prefill + graph-replayed decode.  Returns [B, max_length] int64 (pad-filled), like HF generate."""
-        B, S = input_ids.shape
+                 seed: int = 0, check_every: int = 16, rules: Optional[LogitRules] = None, num_return_sequences: int = 1,
+                 prefix_ids: Optional[torch.Tensor] = None, prefix_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Prefill + graph-replayed decode.  Returns [B, max_length] int64 (pad-filled), like HF generate.
+
+        `rules`: penalties, biases and allowed tokens of the request.  `num_return_sequences` n: n answers to every prompt, neighbouring rows of the result.
+        `prefix_ids` [G, P]: what the prompts have in front of them, B / G neighbouring prompts each; the result's rows begin with it and max_length counts
+        it.  A prompt with several answers, and a prefix, run through the model once and their keys are held and read once (`SharedPrefix`), where the engine's
+        attention knows that form; other engines run the rows as if they had been written out."""
         self._check_max_length(max_length)
         from ..utils.stats import CudaTimer, GenerationStats, nvtx_range
-        st = self._decode_state(B, max_length)
-        stats = GenerationStats(batch=B, prompt_len=S, weight_bytes_per_step=self.weight_bytes_per_step())
         with nvtx_range("prefill"), CudaTimer() as t_prefill:
-            cache = self.prepare(st, input_ids, attention_mask, pad_token_id)
+            st, cache, S = self._begin(input_ids, attention_mask, max_length, pad_token_id, rules, int(num_return_sequences), prefix_ids, prefix_mask)
+        B = st.B
+        stats = GenerationStats(batch=B, prompt_len=S, weight_bytes_per_step=self.weight_bytes_per_step())
         sampling = (bool(do_sample), float(temperature), int(top_k or 0), float(top_p), int(seed))
         # first new token comes from the prefill logits
         self._select_and_advance_after_prefill(st, cache, sampling, eos_token_id, pad_token_id)
@@ -806,6 +874,87 @@ class B200Engine:
         self.last_stats = stats
         return st.sequences.to(torch.long)
 
+    def _shares(self, rows: int, groups: int) -> bool:
+        """Whether `rows` rows behind `groups` shared prefixes take the attention over shared keys (head sizes and groups that it is built for)."""
+        return self.shares_prefixes and self.hd in (64, 128) and self.nh // self.nkv in (1, 2, 4, 8) and rows > groups
+
+    shares_prefixes = True                       # engines whose layers hold anything else per row say no
+
+    def _begin(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], max_length: int, pad: int, rules: Optional[LogitRules], repeat: int,
+               prefix_ids: Optional[torch.Tensor], prefix_mask: Optional[torch.Tensor], logit_rows: Optional[torch.Tensor] = None
+               ) -> Tuple[DecodeState, DeviceKVCache, int]:
+        """Prefill of a new request batch in whichever form it takes: (decode state, cache, tokens per row so far)."""
+        rows, S = input_ids.shape
+        if repeat < 1:
+            raise ValueError(f"num_return_sequences {repeat}")
+        if prefix_ids is None and repeat == 1:
+            st = self._decode_state(rows, max_length)
+            cache = self.prepare(st, input_ids, attention_mask, pad, logit_rows=logit_rows)
+            self._set_rules(st, rules, S, rows, 1)
+            return st, cache, S
+        if logit_rows is not None:
+            raise NotImplementedError("logits of prompt rows go with one answer per prompt and no prefix")
+        B = rows * repeat
+        if prefix_ids is not None:
+            prefix_ids = prefix_ids.to(self.device)
+            if prefix_ids.dim() != 2 or prefix_ids.shape[0] < 1 or rows % prefix_ids.shape[0]:
+                raise ValueError(f"prefix_ids {tuple(prefix_ids.shape)} in front of {rows} prompts")
+        groups, P = (rows, S) if prefix_ids is None else prefix_ids.shape
+        total = S if prefix_ids is None else P + S
+        if max_length < total:
+            raise ValueError(f"max_length {max_length} is shorter than the prompt ({total})")
+        # (a prompt without a token of its own ends with its prefix: its answer begins at the prefix's last position, not behind padding)
+        empty = S == 0 or (prefix_ids is not None and attention_mask is not None and bool((attention_mask[:, S - 1] == 0).any()))
+        if P == 0 or empty or not self._shares(B, groups):
+            ids, mask = (input_ids, attention_mask) if prefix_ids is None else join_prefix(prefix_ids, input_ids, prefix_mask, attention_mask, pad)
+            st = self._decode_state(B, max_length)
+            cache = self.prepare(st, ids.repeat_interleave(repeat, 0), None if mask is None else mask.repeat_interleave(repeat, 0), pad)
+        else:
+            st = self._decode_state(B, max_length, (int(groups), int(P)))
+            cache = self._prepare_shared(st, input_ids, attention_mask, pad, repeat, prefix_ids, prefix_mask)
+        self._set_rules(st, rules, total, rows, repeat)
+        return st, cache, total
+
+    def _prepare_shared(self, st: DecodeState, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], pad: int, repeat: int,
+                        prefix_ids: Optional[torch.Tensor], prefix_mask: Optional[torch.Tensor]) -> DeviceKVCache:
+        """`prepare` for rows that share keys: the prefixes' prefill into a cache of their own, then the prompts' (when they are not the prefixes
+        themselves) behind it."""
+        rows, S = input_ids.shape
+        whole = prefix_ids is None                                             # several answers: the prompts are what is shared
+        front, front_mask = (input_ids, attention_mask) if whole else (prefix_ids, prefix_mask)
+        groups, P = front.shape
+        front_cache, cache = getattr(st, "_front_cache", None), getattr(st, "_cache", None)
+        if cache is None:
+            front_cache, cache = self.new_cache(groups, P), self.new_cache(st.B, max(st.max_len - P, 1))
+            cache.prefix = SharedPrefix(front_cache.k, front_cache.v, torch.full((groups,), P, dtype=torch.int32, device=self.device), front_cache.pad_left,
+                                        K.prefix_attn_scratch(st.B, 1, groups, self.nh, self.nkv, self.hd, P, self.device))
+            st._front_cache, st._cache = front_cache, cache
+            st.seq_pad = torch.zeros(st.B, dtype=torch.int32, device=self.device)
+        front_cache.set_index(0)
+        cache.set_index(0)
+        out = self.forward(front, attention_mask=front_mask, cache=front_cache, last_only=True, gather_logits=False)
+        ids, mask = front, front_mask
+        cache.pad_left.zero_()
+        if not whole:
+            ids, mask = join_prefix(front, input_ids, front_mask, attention_mask, pad)
+            if repeat > 1:
+                input_ids = input_ids.repeat_interleave(repeat, 0)
+                attention_mask = None if attention_mask is None else attention_mask.repeat_interleave(repeat, 0)
+            out = self.forward(input_ids, attention_mask=attention_mask, cache=cache, last_only=True, gather_logits=False)
+        total = ids.shape[1]
+        times = st.B // ids.shape[0]
+        st.sequences.fill_(int(pad))
+        st.sequences[:, :total] = ids.to(torch.int32).repeat_interleave(times, 0)
+        st.seq_pad.copy_(self.pad_left_from_mask(mask, ids.shape[0], total, self.device).repeat_interleave(times, 0))
+        st.finished.zero_()
+        st.cur_len.fill_(total)
+        st.step.zero_()
+        st.n_unfinished.fill_(st.B)
+        st.prompt_logits = None
+        logits = out.logits.view(-1, out.logits.shape[-1])
+        st.logits.copy_(logits.repeat_interleave(st.B // logits.shape[0], 0))
+        return cache
+
     def weight_bytes_per_step(self) -> int:
         """Bytes of weights one decode step streams on this rank (the HBM-roofline numerator)."""
         return sum(t.numel() * 2 for t in (self.wqkv_all, self.wo_all, self.w13_all, self.w2_all, self.lm_head))
@@ -820,6 +969,7 @@ class B200Engine:
             cache = self.new_cache(B, st.max_len)
             st._cache = cache
         cache.set_index(0)
+        st.rules = None                          # (`_begin` sets those of the new batch)
         st.sequences.fill_(int(pad))
         st.sequences[:, :S] = input_ids.to(torch.int32)
         st.finished.zero_()
@@ -854,13 +1004,12 @@ class B200Engine:
     def begin_stream(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None, *,
                      max_length: int, do_sample: bool = False, temperature: float = 1.0,
                      top_k: Optional[int] = 50, top_p: float = 1.0, pad_token_id: int = 0,
-                     eos_token_id: int = -1, seed: int = 0, logit_rows: Optional[torch.Tensor] = None) -> "EngineStream":
+                     eos_token_id: int = -1, seed: int = 0, logit_rows: Optional[torch.Tensor] = None, rules: Optional[LogitRules] = None,
+                     num_return_sequences: int = 1, prefix_ids: Optional[torch.Tensor] = None, prefix_mask: Optional[torch.Tensor] = None) -> "EngineStream":
         """Prefill and select the first new token; subsequent tokens come from `EngineStream.step`.  `logit_rows`:
-        prompt rows whose logits the caller wants to read back (`EngineStream.prompt_logits`)."""
-        B, S = input_ids.shape
+        prompt rows whose logits the caller wants to read back (`EngineStream.prompt_logits`).  The others as in `generate`."""
         self._check_max_length(max_length)
-        st = self._decode_state(B, max_length)
-        cache = self.prepare(st, input_ids, attention_mask, pad_token_id, logit_rows=logit_rows)
+        st, cache, S = self._begin(input_ids, attention_mask, max_length, pad_token_id, rules, int(num_return_sequences), prefix_ids, prefix_mask, logit_rows)
         sampling = (bool(do_sample), float(temperature), int(top_k or 0), float(top_p), int(seed))
         self._select_and_advance_after_prefill(st, cache, sampling, eos_token_id, pad_token_id)
         graph = self._graph_for(st, cache, sampling, eos_token_id, pad_token_id)
@@ -883,14 +1032,24 @@ class EngineStream:
     def last_tokens(self) -> torch.Tensor:
         return self.host_tok
 
-    def step(self, feed: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def step(self, feed: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Advance every row by one token.  `feed` (pinned int32 [B] on the host) overrides the input
         token of this step — the interactive case where the host owns the sequence; otherwise the token
-        selected on the device in the previous step is used.  Returns the new tokens in pinned memory."""
+        selected on the device in the previous step is used.  `allowed` (int32 masks of the rules' shape, [1 or B, words]) are the tokens that this step
+        may choose, for a grammar that follows the text; the stream's rules then have `allowed_tokens` from the start, for its first token.  Returns the
+        new tokens in pinned memory."""
         if self.length >= self.st.max_len:
             raise RuntimeError("stream is at max_length")
+        rules = self.st.rules
+        if allowed is not None:
+            if rules is None or rules.allowed is None or allowed.dtype != torch.int32 or allowed.shape != rules.allowed.shape:
+                want = None if rules is None or rules.allowed is None else tuple(rules.allowed.shape)
+                raise ValueError(f"masks {allowed.dtype} {tuple(allowed.shape)} for a stream whose rules have masks of shape {want}")
+            rules.allowed.copy_(allowed, non_blocking=True)
         if feed is not None:
             self.st.ids.copy_(feed, non_blocking=True)
+            if rules is not None:                         # what was said is what was fed
+                self.st.sequences[:, self.length - 1].copy_(feed, non_blocking=True)
         if self.graph is not None:
             self.graph.replay()
         else:

@@ -14,6 +14,7 @@ from typing import Any, Dict, Optional, Tuple
 import torch
 
 from ..config import HybridConfig
+from ..ops.rules import LogitRules
 from .hybrid_engine import HybridEngine, random_tensors
 from .llama import WEIGHTS_NAME, GenerateOutput
 from .reference import ModelOutput
@@ -100,16 +101,20 @@ class HybridForCausalLM:
                  params: Optional[Params] = None, max_length: Optional[int] = None,
                  max_new_tokens: Optional[int] = None, do_sample: bool = False, temperature: float = 1.0,
                  top_k: Optional[int] = 50, top_p: float = 1.0, pad_token_id: Optional[int] = None,
-                 eos_token_id: Optional[int] = None, seed: int = 0) -> GenerateOutput:
+                 eos_token_id: Optional[int] = None, seed: int = 0, rules: Optional[LogitRules] = None, num_return_sequences: int = 1,
+                 prefix_ids: Optional[torch.Tensor] = None, prefix_mask: Optional[torch.Tensor] = None) -> GenerateOutput:
+        """`rules`, `num_return_sequences`, `prefix_ids`, `prefix_mask`: as in `LLaMAForCausalLM.generate`; the rows of this family are written out."""
         eng = self._engine_for(params)
         ids = torch.as_tensor(input_ids).to(eng.device)
         if max_length is None:
             if max_new_tokens is None:
                 raise ValueError("give max_length or max_new_tokens")
-            max_length = ids.shape[1] + max_new_tokens
+            max_length = ids.shape[1] + max_new_tokens + (0 if prefix_ids is None else torch.as_tensor(prefix_ids).shape[1])
         eos = self.config.eos_token_id if eos_token_id is None else eos_token_id
         pad = self.config.pad_token_id if pad_token_id is None else pad_token_id
         mask = None if attention_mask is None else torch.as_tensor(attention_mask).to(eng.device)
         seqs = eng.generate(ids, mask, max_length=max_length, do_sample=do_sample, temperature=temperature, top_k=top_k,
-                            top_p=top_p, pad_token_id=pad, eos_token_id=eos, seed=seed)
+                            top_p=top_p, pad_token_id=pad, eos_token_id=eos, seed=seed, rules=rules, num_return_sequences=num_return_sequences,
+                            prefix_ids=None if prefix_ids is None else torch.as_tensor(prefix_ids).to(eng.device),
+                            prefix_mask=None if prefix_mask is None else torch.as_tensor(prefix_mask).to(eng.device))
         return GenerateOutput(sequences=seqs)

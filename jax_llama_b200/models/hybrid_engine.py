@@ -179,6 +179,8 @@ def tensor_shapes(config: Any, decay_rank: int = 16, present: Optional[Dict[str,
 
 class HybridEngine(B200Engine):
 
+    shares_prefixes = False                      # per-layer caches of unequal shapes and recurrent states: rows are written out
+
     def __init__(self, config: Any, tensors: Dict[str, torch.Tensor], *, dtype: torch.dtype = torch.bfloat16,
                  device: Any = "cuda", use_cuda_graph: bool = True):
         """`tensors`: checkpoint names → tensors (any float dtype, any device); they are cast to `dtype` and moved."""
@@ -485,8 +487,8 @@ class HybridEngine(B200Engine):
         return (self._branch_stream, *self._branch_events[layer])
 
     # ------------------------------------------------------------------ decode state
-    def _decode_state(self, B: int, max_len: int) -> DecodeState:
-        key = (B, max_len)
+    def _decode_state(self, B: int, max_len: int, shared: Tuple[int, ...] = ()) -> DecodeState:
+        key = (B, max_len, *shared)
         if key in self._decode_states:
             return self._decode_states[key]
         c, dev = self.config, self.device

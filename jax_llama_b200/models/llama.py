@@ -21,10 +21,11 @@ from typing import Any, Dict, Optional, Tuple, Union
 import torch
 
 from ..config import LLaMAConfig
+from ..ops.rules import LogitRules
 from ..ops.sampling import sample
 from . import reference as ref
 from .modules import LLaMAForCausalLMModule, LLaMAModule
-from .reference import KVCache, ModelOutput
+from .reference import KVCache, ModelOutput, join_prefix
 
 logger = logging.getLogger(__name__)
 
@@ -252,8 +253,9 @@ class LLaMAForCausalLM(LLaMAPreTrainedModel):
                  params: Optional[Tree] = None, max_length: Optional[int] = None,
                  max_new_tokens: Optional[int] = None, do_sample: bool = False, temperature: float = 1.0,
                  top_k: Optional[int] = 50, top_p: float = 1.0, pad_token_id: Optional[int] = None,
-                 eos_token_id: Optional[int] = None, seed: int = 0, generation_config: Any = None
-                 ) -> GenerateOutput:
+                 eos_token_id: Optional[int] = None, seed: int = 0, generation_config: Any = None,
+                 rules: Optional[LogitRules] = None, num_return_sequences: int = 1, prefix_ids: Optional[torch.Tensor] = None,
+                 prefix_mask: Optional[torch.Tensor] = None) -> GenerateOutput:
         """Greedy / sampling decode with a KV cache.
 
         Semantics of HF's Flax ``_greedy_search`` / ``_sample`` that the reference inherits
@@ -261,6 +263,11 @@ class LLaMAForCausalLM(LLaMAPreTrainedModel):
         already produced EOS keep emitting ``pad``; the loop ends at ``max_length`` or when every row has
         finished; `sequences` is ``[B, max_length]`` padded with ``pad``.  A fixed `seed` makes sampling
         repeatable per call (the reference always used PRNGKey(0)).
+
+        `rules` (`LogitRules`): penalties for tokens that occurred, biases, allowed tokens, ahead of the sampling.  `num_return_sequences` n: n answers to every
+        prompt, neighbouring rows of the result.  `prefix_ids` [G, P] (and `prefix_mask`, left-padded): what the prompts, B / G neighbours each, have
+        in front of them, a system prompt or a document; the result's rows begin with it, `max_length` counts it.  On the GPU the prefix, or a prompt with
+        several answers, runs through the model once, and its keys are held once and read once per token for all its rows.
         """
         if generation_config is not None:
             g = generation_config
@@ -275,6 +282,15 @@ class LLaMAForCausalLM(LLaMAPreTrainedModel):
         dev = _tree_device(params)
         input_ids = torch.as_tensor(input_ids).to(dev)
         b, s = input_ids.shape
+        if prefix_ids is not None:
+            prefix_ids = torch.as_tensor(prefix_ids).to(dev)
+            if prefix_ids.dim() != 2:
+                raise ValueError("prefix_ids must be [groups, tokens]")
+            s += prefix_ids.shape[1]
+            if prefix_mask is not None:
+                prefix_mask = torch.as_tensor(prefix_mask).to(dev)
+        if num_return_sequences < 1:
+            raise ValueError(f"num_return_sequences {num_return_sequences}")
         if max_length is None:
             if max_new_tokens is None:
                 raise ValueError("give max_length or max_new_tokens")
@@ -290,8 +306,18 @@ class LLaMAForCausalLM(LLaMAPreTrainedModel):
             seqs = self._engine_for(params).generate(
                 input_ids, attention_mask, max_length=max_length, do_sample=do_sample,
                 temperature=temperature, top_k=top_k, top_p=top_p, pad_token_id=pad,
-                eos_token_id=eos, seed=seed)
+                eos_token_id=eos, seed=seed, rules=rules, num_return_sequences=num_return_sequences,
+                prefix_ids=prefix_ids, prefix_mask=prefix_mask)
             return GenerateOutput(sequences=seqs)
+
+        bound = rules.bind(b, self.config.vocab_size, dev, num_return_sequences) if rules is not None and rules.active else None
+        if prefix_ids is not None:
+            input_ids, attention_mask = join_prefix(prefix_ids, input_ids, prefix_mask, attention_mask, pad)
+        if num_return_sequences > 1:
+            input_ids = input_ids.repeat_interleave(num_return_sequences, 0)
+            attention_mask = None if attention_mask is None else attention_mask.repeat_interleave(num_return_sequences, 0)
+            b = input_ids.shape[0]
+        starts = None if attention_mask is None else (attention_mask[:, :s] == 0).sum(-1).to(torch.int32)
 
         gen = torch.Generator(device="cpu").manual_seed(seed)
         sequences = torch.full((b, max_length), pad, dtype=torch.long, device=dev)
@@ -303,6 +329,8 @@ class LLaMAForCausalLM(LLaMAPreTrainedModel):
         while cur < max_length and not bool(finished.all()):
             out = self(running, params=params, last_only=True, **kwargs)
             logits = out.logits[:, -1].float()
+            if bound is not None:
+                logits = bound.apply(logits, sequences.to(torch.int32), torch.tensor([cur], dtype=torch.int32), torch.tensor([s], dtype=torch.int32), starts)
             nxt = sample(logits, temperature if do_sample else 0.0, top_k, top_p, gen)
             nxt = torch.where(finished, torch.full_like(nxt, pad), nxt)
             finished = finished | (nxt == eos)

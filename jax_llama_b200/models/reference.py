@@ -19,6 +19,28 @@ from ..config import LLaMAConfig
 Tree = Dict[str, Any]
 
 
+# --------------------------------------------------------------------------- prompts behind a common prefix
+def join_prefix(prefix_ids: torch.Tensor, input_ids: torch.Tensor, prefix_mask: Optional[torch.Tensor] = None,
+                attention_mask: Optional[torch.Tensor] = None, pad: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Prefixes [G, P] and prompts [B, S], both left-padded, B a multiple of G (the prompts of a prefix are neighbours) -> joined prompts [B, P + S], padded
+    on the left, and their mask.  The prompts keep their places at the end of the rows."""
+    (G, P), (B, S) = prefix_ids.shape, input_ids.shape
+    if G < 1 or B % G:
+        raise ValueError(f"{B} prompts behind {G} prefixes")
+    dev = input_ids.device
+    pm = torch.ones(G, P, dtype=torch.int32, device=dev) if prefix_mask is None else prefix_mask.to(device=dev, dtype=torch.int32)
+    m = torch.ones(B, S, dtype=torch.int32, device=dev) if attention_mask is None else attention_mask[:, :S].to(device=dev, dtype=torch.int32)
+    ids, pm = prefix_ids.to(device=dev, dtype=input_ids.dtype).repeat_interleave(B // G, 0), pm.repeat_interleave(B // G, 0)
+    shift = (m == 0).sum(-1, keepdim=True)                                     # the prefix moves up to the prompt's first token
+    at = torch.arange(P + S, device=dev)[None] - shift
+    whole = torch.cat([ids, input_ids], 1), torch.cat([pm, m], 1)
+    joined = torch.gather(whole[0], 1, at.clamp(min=0)), torch.gather(whole[1], 1, at.clamp(min=0))
+    tail = torch.arange(P + S, device=dev)[None] >= P + shift                  # the prompt itself stays
+    out_ids, out_mask = torch.where(tail, whole[0], joined[0]), torch.where(tail, whole[1], joined[1])
+    out_mask = torch.where(at >= 0, out_mask, torch.zeros_like(out_mask))
+    return torch.where(out_mask > 0, out_ids, torch.full_like(out_ids, int(pad))), out_mask
+
+
 # --------------------------------------------------------------------------- building blocks
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
     """x · rsqrt(mean(x²) + eps) · w, statistics in fp32 (model.py:42-48)."""
