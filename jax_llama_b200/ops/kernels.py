@@ -354,32 +354,40 @@ def prefill_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 
 
 # --------------------------------------------------------------------------- attention over a prefix that the rows of a group share
-def _here(t: torch.Tensor, who: str) -> None:
+# (The checks below run on every call of a decode step: identities and whole numbers, a message is put together only for what fails.)
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+
+
+def _here(dev: int, who: str) -> None:
     """Launches go to the current device's stream: tensors of another device are refused."""
-    if _get_device is not None and t.device.index is not None and t.device.index != _get_device():
-        raise ValueError(f"{who}: tensors on {t.device}, current device cuda:{_get_device()}")
+    if _get_device is not None and dev != _get_device():
+        raise ValueError(f"{who}: tensors on cuda:{dev}, current device cuda:{_get_device()}")
 
 
-def _index(t: Optional[torch.Tensor], n: Tuple[int, ...], name: str, device: torch.device) -> Optional[torch.Tensor]:
-    if t is not None and (t.dtype != torch.int32 or t.numel() not in n or not t.is_contiguous() or t.device != device):
-        raise ValueError(f"{name} must be int32, contiguous, on {device}, of {' or '.join(map(str, n))} elements (got {t.dtype}, {tuple(t.shape)}, {t.device})")
-    return t
+def _rows(t: Optional[torch.Tensor], n: int, dev: int, name: str, or_one: bool = False) -> None:
+    """`t`, if given, is int32 [n] (or [1]) on device number `dev` (-1: the CPU)."""
+    if t is None:
+        return
+    m = t.numel()
+    if t.dtype is not _I32 or (m != n and not (or_one and m == 1)) or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be int32, contiguous, of {n}{' or 1' if or_one else ''} elements, on the other tensors' device (got {t.dtype}, {tuple(t.shape)}, {t.device})")
 
 
-def _prefix_shapes(who: str, B: int, nkv: int, hd: int, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
-                   ) -> Tuple[int, int, int]:
+def _prefix_shapes(who: str, B: int, nkv: int, hd: int, dev: int, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k_cache: torch.Tensor,
+                   v_cache: torch.Tensor) -> Tuple[int, int, int]:
     """(groups, P, T) of the two caches, or a refusal."""
-    if prefix_k.dim() != 4 or k_cache.dim() != 4 or prefix_v.shape != prefix_k.shape or v_cache.shape != k_cache.shape:
+    ps, cs = prefix_k.shape, k_cache.shape
+    if len(ps) != 4 or len(cs) != 4 or prefix_v.shape != ps or v_cache.shape != cs:
         raise ValueError(f"{who}: keys and values are [groups, nkv, P, hd] and [B, nkv, T, hd]")
-    groups, P, T = prefix_k.shape[0], prefix_k.shape[2], k_cache.shape[2]
-    if tuple(prefix_k.shape) != (groups, nkv, P, hd) or tuple(k_cache.shape) != (B, nkv, T, hd) or groups < 1 or B % groups or P < 1 or T < 1:
-        raise ValueError(f"{who}: prefix {tuple(prefix_k.shape)} and own keys {tuple(k_cache.shape)} for {B} rows, {nkv} key heads of {hd}")
-    if k_cache.is_cuda:
-        for name, t in (("prefix_k", prefix_k), ("prefix_v", prefix_v), ("k_cache", k_cache), ("v_cache", v_cache)):
-            _bf16c(t, name)
-            if t.device != k_cache.device:
-                raise ValueError(f"{who}: {name} on {t.device}, k_cache on {k_cache.device}")
-        _here(k_cache, who)
+    groups, pn, P, ph = ps
+    rows, cn, T, ch = cs
+    if pn != nkv or cn != nkv or ph != hd or ch != hd or rows != B or groups < 1 or B % groups or P < 1 or T < 1:
+        raise ValueError(f"{who}: prefix {tuple(ps)} and own keys {tuple(cs)} for {B} rows, {nkv} key heads of {hd}")
+    for t in (prefix_k, prefix_v, k_cache, v_cache):
+        if t.get_device() != dev or (dev >= 0 and (t.dtype is not _BF16 or not t.is_contiguous())):
+            raise ValueError(f"{who}: keys and values are contiguous bf16 tensors on the queries' device (got {t.dtype}, contiguous={t.is_contiguous()}, {t.device})")
+    if dev >= 0:
+        _here(dev, who)
     return groups, P, T
 
 
@@ -439,13 +447,14 @@ def decode_attn_prefix(qkv: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torc
     k_cache / v_cache [B, nkv, T, hd] the rows' own keys from pad_left[b] (int32 [B] or None) on.  The new token takes slot cache_len (int32 [1], device; nothing is
     stored once the cache is full) at rotary position (prefix_len - prefix_pad)[g] + cache_len - pad_left[b].  -> [B, nh·hd]."""
     who = "decode_attn_prefix"
-    B = qkv.shape[0]
-    if qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
+    B, width = qkv.shape if qkv.dim() == 2 else (-1, -1)
+    if width != (nh + 2 * nkv) * hd:
         raise ValueError(f"{who}: qkv {tuple(qkv.shape)} for {nh} + 2 x {nkv} heads of {hd}")
-    groups, P, T = _prefix_shapes(who, B, nkv, hd, prefix_k, prefix_v, k_cache, v_cache)
-    _index(cache_len, (1,), "cache_len", qkv.device); _index(pad_left, (B,), "pad_left", qkv.device)
-    _index(prefix_len, (groups,), "prefix_len", qkv.device); _index(prefix_pad, (groups,), "prefix_pad", qkv.device)
-    if not qkv.is_cuda:
+    dev = qkv.get_device()
+    groups, P, T = _prefix_shapes(who, B, nkv, hd, dev, prefix_k, prefix_v, k_cache, v_cache)
+    _rows(cache_len, 1, dev, "cache_len"); _rows(pad_left, B, dev, "pad_left")
+    _rows(prefix_len, groups, dev, "prefix_len"); _rows(prefix_pad, groups, dev, "prefix_pad")
+    if dev < 0:
         lo, hi = _prefix_counts(prefix_len, prefix_pad, groups, P)
         slot = min(int(cache_len.item()), T)
         x = qkv.view(B, nh + 2 * nkv, hd)
@@ -464,8 +473,10 @@ def decode_attn_prefix(qkv: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torc
                              torch.tensor([slot]), pad, lo, hi)
         return o.view(B, nh * hd).to(qkv.dtype)
     _bf16c(qkv, "qkv")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.shape[1] != hd // 2 or not (cos.is_contiguous() and sin.is_contiguous()):
-        raise ValueError(f"{who}: cos/sin tables are fp32 [positions, {hd // 2}]")
+    table = cos.shape
+    if cos.dtype is not _F32 or sin.dtype is not _F32 or sin.shape != table or table[1] != hd // 2 or not (cos.is_contiguous() and sin.is_contiguous()) \
+            or cos.get_device() != dev or sin.get_device() != dev:
+        raise ValueError(f"{who}: cos/sin tables are fp32 [positions, {hd // 2}] on {qkv.device}")
     if scratch is None:
         scratch = prefix_attn_scratch(B, 1, groups, nh, nkv, hd, P, qkv.device)
     if out is None:
@@ -474,10 +485,11 @@ def decode_attn_prefix(qkv: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torc
         _bf16c(out, "out")
         if out.numel() != B * nh * hd:
             raise ValueError(f"{who}: out {tuple(out.shape)} for {B} x {nh * hd}")
-    _lib.check(_lib.lib().jl_decode_attn_prefix(qkv.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cos.data_ptr(),
-                                                sin.data_ptr(), cache_len.data_ptr(), _p(pad_left), _p(prefix_len), _p(prefix_pad), scratch.data_ptr(),
-                                                scratch.numel() * scratch.element_size(), out.data_ptr(), B, groups, nh, nkv, hd, P, T, cos.shape[0],
-                                                1.0 / math.sqrt(hd), _stream()), "jl_decode_attn_prefix")
+    rc = _lib.lib().jl_decode_attn_prefix(qkv.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cos.data_ptr(),
+                                          sin.data_ptr(), cache_len.data_ptr(), _p(pad_left), _p(prefix_len), _p(prefix_pad), scratch.data_ptr(), scratch.nbytes,
+                                          out.data_ptr(), B, groups, nh, nkv, hd, P, T, table[0], hd ** -0.5, _stream())
+    if rc:
+        _lib.check(rc, "jl_decode_attn_prefix")
     return out
 
 
@@ -488,15 +500,15 @@ def prefill_attn_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch
     cache in slots start..start+S; shared keys as in `decode_attn_prefix` (every query sees all of its group's), own keys [pad_left[b], slot of the query].  Queries
     in front of pad_left give zeros.  -> [B, S, nh·hd]."""
     who = "prefill_attn_prefix"
-    if q.dim() != 4 or q.shape[1] != S:
+    B, s_q, nh, hd = q.shape if q.dim() == 4 else (0, -1, 0, 0)
+    if s_q != S:
         raise ValueError(f"{who}: q {tuple(q.shape)} is not [B, {S}, heads, head_dim]")
-    B, _, nh, hd = q.shape
-    nkv = k_cache.shape[1]
-    groups, P, T = _prefix_shapes(who, B, nkv, hd, prefix_k, prefix_v, k_cache, v_cache)
+    nkv, dev = k_cache.shape[1] if k_cache.dim() == 4 else 0, q.get_device()
+    groups, P, T = _prefix_shapes(who, B, nkv, hd, dev, prefix_k, prefix_v, k_cache, v_cache)
     if start < 0 or start + S > T:
         raise ValueError(f"{who}: slots {start}..{start + S} of a cache of {T}")
-    _index(pad_left, (B,), "pad_left", q.device); _index(prefix_len, (groups,), "prefix_len", q.device); _index(prefix_pad, (groups,), "prefix_pad", q.device)
-    if not q.is_cuda:
+    _rows(pad_left, B, dev, "pad_left"); _rows(prefix_len, groups, dev, "prefix_len"); _rows(prefix_pad, groups, dev, "prefix_pad")
+    if dev < 0:
         lo, hi = _prefix_counts(prefix_len, prefix_pad, groups, P)
         return _prefix_attn_ref(q, prefix_k, prefix_v, k_cache[:, :, :start + S], v_cache[:, :, :start + S], start + torch.arange(S), pad_left, lo, hi)
     _bf16c(q, "q")
@@ -508,9 +520,11 @@ def prefill_attn_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch
         _bf16c(out, "out")
         if out.numel() != B * S * nh * hd:
             raise ValueError(f"{who}: out {tuple(out.shape)} for {B} x {S} x {nh * hd}")
-    _lib.check(_lib.lib().jl_prefill_attn_prefix(q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _p(pad_left),
-                                                 _p(prefix_len), _p(prefix_pad), scratch.data_ptr(), scratch.numel() * scratch.element_size(), out.data_ptr(), B, S,
-                                                 groups, nh, nkv, hd, P, T, start, 1.0 / math.sqrt(hd), _stream()), "jl_prefill_attn_prefix")
+    rc = _lib.lib().jl_prefill_attn_prefix(q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _p(pad_left), _p(prefix_len),
+                                           _p(prefix_pad), scratch.data_ptr(), scratch.nbytes, out.data_ptr(), B, S, groups, nh, nkv, hd, P, T, start, hd ** -0.5,
+                                           _stream())
+    if rc:
+        _lib.check(rc, "jl_prefill_attn_prefix")
     return out
 
 
@@ -543,6 +557,17 @@ def _constrain_ref(x: torch.Tensor, tokens: Optional[torch.Tensor], starts: torc
 _LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+def _coefficient(v: Union[float, torch.Tensor, None], off: float, B: int, dev: int, name: str) -> Tuple[Optional[torch.Tensor], float]:
+    """(fp32 [B], off) or (None, the number)."""
+    if v is None:
+        return None, off
+    if isinstance(v, torch.Tensor):
+        if v.dtype is not _F32 or v.dim() != 1 or v.shape[0] != B or not v.is_contiguous() or v.get_device() != dev:
+            raise ValueError(f"constrain_logits: {name} is a number or fp32 [{B}] on the logits' device (got {v.dtype}, {tuple(v.shape)}, {v.device})")
+        return v, off
+    return None, float(v)
+
+
 def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
                      prompt_lengths: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None, repetition: Union[float, torch.Tensor, None] = None,
                      frequency: Union[float, torch.Tensor, None] = None, presence: Union[float, torch.Tensor, None] = None,
@@ -556,62 +581,64 @@ def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = N
     (int32 / fp32 [B, n], or [1, n] for all rows, n <= 8192; an id outside the vocabulary is no entry, the same id twice adds both), then -inf where bit v % 32 of word v // 32
     of allowed (int32 [B, words] or [1, words]) is zero.  A row whose mask allows nothing is -inf throughout.  `out` may be `logits` itself when that is fp32."""
     who = "constrain_logits"
-    if logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    kind = _LOGIT_TYPES.get(logits.dtype)
+    B, V = logits.shape if logits.dim() == 2 else (-1, -1)
+    if kind is None or B < 0 or (V > 1 and logits.stride(1) != 1):
         raise ValueError(f"{who}: logits are [B, V], fp32, bf16 or fp16, with dense rows (got {logits.dtype}, {tuple(logits.shape)}, strides {logits.stride()})")
-    B, V = logits.shape
-    dev = logits.device
-    if tokens is None and any(t is not None for t in (lengths, prompt_lengths, starts)):
-        raise ValueError(f"{who}: row bounds without tokens")
-    T = 0
+    dev = logits.get_device()
+    T = ldt = n_start = n_len = n_prompt = 0
     if tokens is not None:
-        if tokens.dim() != 2 or tokens.dtype != torch.int32 or tokens.shape[0] != B or (tokens.shape[1] > 1 and tokens.stride(1) != 1) or tokens.device != dev:
-            raise ValueError(f"{who}: tokens are int32 [{B}, T] with dense rows on {dev} (got {tokens.dtype}, {tuple(tokens.shape)}, {tokens.device})")
-        T = tokens.shape[1]
-        _index(lengths, (B, 1), "lengths", dev); _index(prompt_lengths, (B, 1), "prompt_lengths", dev); _index(starts, (B, 1), "starts", dev)
-    scalars, rows = [], []
-    for name, v, off in (("repetition", repetition, 1.0), ("frequency", frequency, 0.0), ("presence", presence, 0.0)):
-        if isinstance(v, torch.Tensor):
-            if v.dtype != torch.float32 or v.shape != (B,) or not v.is_contiguous() or v.device != dev:
-                raise ValueError(f"{who}: {name} is a number or fp32 [{B}] on {dev} (got {v.dtype}, {tuple(v.shape)}, {v.device})")
-            rows.append(v); scalars.append(off)
-        else:
-            rows.append(None); scalars.append(off if v is None else float(v))
-            if name == "repetition" and not scalars[-1] > 0.0:
-                raise ValueError(f"{who}: repetition {v} is not above zero")
-    if (bias_ids is None) != (bias_values is None):
-        raise ValueError(f"{who}: bias_ids and bias_values come together")
-    n_bias = 0
-    if bias_ids is not None:
-        if bias_ids.dtype != torch.int32 or bias_values.dtype != torch.float32 or bias_ids.dim() != 2 or bias_ids.shape != bias_values.shape \
-                or bias_ids.shape[0] not in (1, B) or not (bias_ids.is_contiguous() and bias_values.is_contiguous()) or bias_ids.device != dev or bias_values.device != dev:
-            raise ValueError(f"{who}: biases are int32 and fp32 [{B} or 1, n] on {dev} (got {tuple(bias_ids.shape)}, {tuple(bias_values.shape)})")
-        n_bias = bias_ids.shape[1]
+        T = tokens.shape[1] if tokens.dim() == 2 else -1
+        if T < 0 or tokens.dtype is not _I32 or tokens.shape[0] != B or (T > 1 and tokens.stride(1) != 1) or tokens.get_device() != dev:
+            raise ValueError(f"{who}: tokens are int32 [{B}, T] with dense rows on {logits.device} (got {tokens.dtype}, {tuple(tokens.shape)}, {tokens.device})")
+        ldt = tokens.stride(0) if B > 1 else T
+        if lengths is not None:
+            _rows(lengths, B, dev, "lengths", True); n_len = lengths.numel()
+        if prompt_lengths is not None:
+            _rows(prompt_lengths, B, dev, "prompt_lengths", True); n_prompt = prompt_lengths.numel()
+        if starts is not None:
+            _rows(starts, B, dev, "starts", True); n_start = starts.numel()
+    elif lengths is not None or prompt_lengths is not None or starts is not None:
+        raise ValueError(f"{who}: row bounds without tokens")
+    rep_t, rep = _coefficient(repetition, 1.0, B, dev, "repetition")
+    freq_t, freq = _coefficient(frequency, 0.0, B, dev, "frequency")
+    pres_t, pres = _coefficient(presence, 0.0, B, dev, "presence")
+    if not rep > 0.0:
+        raise ValueError(f"{who}: repetition {repetition} is not above zero")
+    n_bias = ldb = 0
+    if bias_ids is not None and bias_values is not None:
+        shape = bias_ids.shape
+        if len(shape) != 2 or bias_values.shape != shape or shape[0] not in (1, B) or bias_ids.dtype is not _I32 or bias_values.dtype is not _F32 \
+                or not (bias_ids.is_contiguous() and bias_values.is_contiguous()) or bias_ids.get_device() != dev or bias_values.get_device() != dev:
+            raise ValueError(f"{who}: biases are int32 and fp32 [{B} or 1, n] on {logits.device} (got {tuple(shape)}, {tuple(bias_values.shape)})")
+        n_bias = shape[1]
+        ldb = n_bias if shape[0] > 1 else 0
         if n_bias > 8192:
             raise ValueError(f"{who}: {n_bias} biases per row (at most 8192)")
-    if allowed is not None and (allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[0] not in (1, B) or allowed.shape[1] < (V + 31) // 32
-                                or not allowed.is_contiguous() or allowed.device != dev):
-        raise ValueError(f"{who}: allowed is int32 [{B} or 1, {(V + 31) // 32} or more words] on {dev} (got {allowed.dtype}, {tuple(allowed.shape)})")
-    if out is not None and (out.dtype != torch.float32 or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or out.device != dev):
-        raise ValueError(f"{who}: out is fp32 {tuple(logits.shape)} with dense rows on {dev} (got {out.dtype}, {tuple(out.shape)}, {out.device})")
-    if not logits.is_cuda:
+    elif bias_ids is not None or bias_values is not None:
+        raise ValueError(f"{who}: bias_ids and bias_values come together")
+    lda = 0
+    if allowed is not None:
+        shape = allowed.shape
+        if len(shape) != 2 or allowed.dtype is not _I32 or shape[0] not in (1, B) or shape[1] < (V + 31) // 32 or not allowed.is_contiguous() or allowed.get_device() != dev:
+            raise ValueError(f"{who}: allowed is int32 [{B} or 1, {(V + 31) // 32} or more words] on {logits.device} (got {allowed.dtype}, {tuple(shape)})")
+        lda = shape[1] if shape[0] > 1 else 0
+    if out is not None and (out.dtype is not _F32 or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or out.get_device() != dev):
+        raise ValueError(f"{who}: out is fp32 {tuple(logits.shape)} with dense rows on {logits.device} (got {out.dtype}, {tuple(out.shape)}, {out.device})")
+    if dev < 0:
         def full(t: Optional[torch.Tensor], off: Union[int, float]) -> torch.Tensor:
             return torch.full((B,), off) if t is None else t.reshape(-1).expand(B)
-        y = _constrain_ref(logits, tokens, full(starts, 0), full(lengths, T), full(prompt_lengths, 0), *(full(r, s) for r, s in zip(rows, scalars)),
+        y = _constrain_ref(logits, tokens, full(starts, 0), full(lengths, T), full(prompt_lengths, 0), full(rep_t, rep), full(freq_t, freq), full(pres_t, pres),
                            bias_ids if n_bias else None, bias_values, allowed)
         return y if out is None else out.copy_(y)
-    _here(logits, who)
+    _here(dev, who)
     if out is None:
         out = logits.new_empty((B, V), dtype=torch.float32)
-
-    def count(t: Optional[torch.Tensor]) -> int:
-        return 0 if t is None else t.numel()
-
-    _lib.check(_lib.lib().jl_logit_rules(
-        logits.data_ptr(), _LOGIT_TYPES[logits.dtype], B, V, logits.stride(0) if B > 1 else V, out.data_ptr(), out.stride(0) if B > 1 else V, _p(tokens), T,
-        tokens.stride(0) if tokens is not None and B > 1 else T, _p(starts), count(starts), _p(lengths), count(lengths), _p(prompt_lengths), count(prompt_lengths),
-        _p(rows[0]), scalars[0], _p(rows[1]), scalars[1], _p(rows[2]), scalars[2], _p(bias_ids), _p(bias_values), n_bias,
-        n_bias if n_bias and bias_ids.shape[0] > 1 else 0, _p(allowed), allowed.shape[1] if allowed is not None and allowed.shape[0] > 1 else 0, _stream()),
-        "jl_logit_rules")
+    rc = _lib.lib().jl_logit_rules(logits.data_ptr(), kind, B, V, logits.stride(0) if B > 1 else V, out.data_ptr(), out.stride(0) if B > 1 else V, _p(tokens), T, ldt,
+                                   _p(starts), n_start, _p(lengths), n_len, _p(prompt_lengths), n_prompt, _p(rep_t), rep, _p(freq_t), freq, _p(pres_t), pres,
+                                   _p(bias_ids), _p(bias_values), n_bias, ldb, _p(allowed), lda, _stream())
+    if rc:
+        _lib.check(rc, "jl_logit_rules")
     return out
 
 
