@@ -8,8 +8,8 @@
 // is a join of two triples (reference exponent m, sum l, weighted values o):  M = max(m1, m2),  o = o1 2^(m1 - M) + o2 2^(m2 - M),  l likewise.
 //   * one token per row (jl_decode_attn_prefix): one launch in which some CTAs take the shared keys, tiles of queries by splits of the keys, and others the
 //     rows' own keys, a warp per (row, key head), appending the new one; all leave partial triples in fp32, and a second, small launch joins them;
-//   * S tokens per row (jl_prefill_attn_prefix): the same for the shared keys, then a second launch of this kernel over every row's own keys, causal, that
-//     joins in its last step; or one launch over both sets, tile after tile, where a row's queries fill tiles by themselves.
+//   * S tokens per row (jl_prefill_attn_prefix): the same for the shared keys, then a second launch over every row's own keys, causal, and the join; or
+//     one launch over both sets, tile after tile, where a row's queries fill tiles by themselves.
 //
 // One CTA owns a tile of 128 queries of one key head, as in flash_prefill.cu: a warp asks for K and V tiles of 64 keys (TMA, 128-byte swizzle), a warp
 // issues S = Q·Kᵀ into one of two score tiles in TMEM and O += P·V with P read from TMEM, four warps hold one query row per thread: one pass over 64
@@ -91,10 +91,10 @@ struct PxParams {
   const float* cos_t; const float* sin_t; int max_pos; const int* cache_len;     // ROTATE: tables and the slot of the new token
   const int* prefix_len; const int* prefix_pad; const int* pad_left;
   __nv_bfloat16* out;
-  float* o_part; float2* ml_part;   // [tokens · nh][parts]: written (partial) or joined (own keys behind a launch over the shared ones)
+  float* o_part; float2* ml_part;   // partial triples [tokens · nh][parts]
   int S, rows, nh, nkv, gs, P, T, start;      // gs: log2 of the query heads per key head
   int shared, own, partial;         // which keys this launch visits; whether it leaves partial triples or the result
-  int splits, parts;                // splits of the shared keys in this launch; triples per (token, head)
+  int splits, parts, part0;         // splits of the shared keys in this launch; triples per (token, head), the first that this launch writes
   // ROTATE: the CTAs in front take the own keys, `own_splits` parts of every (row, key head)
   const __nv_bfloat16* qkv; __nv_bfloat16* k_cache; __nv_bfloat16* v_cache;
   int own_ctas, own_splits, B, tiles_q;
@@ -720,93 +720,65 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
       f1 = w == 0 ? theirs : mine;
     }
     if (warp_on) {
-      const int token = token0 + (at >> p.gs), h = kvh * G + (at & (G - 1));
-      const size_t th = (size_t)token * p.nh + h;
+      const int th = (token0 + (at >> p.gs)) * p.nh + kvh * G + (at & (G - 1));       // (token, head) of this row
       constexpr int CHUNKS = HD / 32 / (PAIR ? 1 : 2);
-      // columns [32 c, 32 c + 32) of the row's sum
-      auto columns = [&](int c, float (&o)[32]) {
-        uint32_t a[32];
-        if (__any_sync(0xffffffffu, f0 != 0.f)) {
-          tc::tmem_ld32(tO(PAIR ? w : 0) + lane_off + c * 32, a);
-          tc::tmem_ld_wait();
-        }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = f0 != 0.f ? __uint_as_float(a[e]) * f0 : 0.f;
-        if constexpr (!PAIR) {
-          if (__any_sync(0xffffffffu, f1 != 0.f)) {
-            tc::tmem_ld32(tO(1) + lane_off + c * 32, a);
+      // a row is a thread here and a run of memory there: 32 x 32 values change hands in shared memory that no product reads any more (the set's own queries, or the
+      // ring when both sets are through), so that a store covers whole rows of 128 or 64 bytes
+      const uint32_t stage = PAIR ? sQ + w * NQ * Tile::Q + quarter * 4096 : ring + (w * 4 + quarter) * 4096;
+      const float inv = !p.partial && row_on && slot >= pad && L != 0.f ? 1.0f / L : 0.f;       // a query in front of its row's first token is padding: zeros
+      const size_t part = (size_t)p.part0 + split;
+      if (p.partial && row_on && (PAIR || w == 0)) p.ml_part[(size_t)th * p.parts + part] = make_float2(M, slot >= pad ? L : 0.f);
+#pragma unroll 1
+      for (int k = 0; k < CHUNKS; ++k) {
+        const int c = (PAIR ? 0 : w * CHUNKS) + k;                     // columns [32 c, 32 c + 32)
+        float o[32];
+        {
+          uint32_t a[32];
+          if (__any_sync(0xffffffffu, f0 != 0.f)) {
+            tc::tmem_ld32(tO(PAIR ? w : 0) + lane_off + c * 32, a);
             tc::tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] += f1 != 0.f ? __uint_as_float(a[e]) * f1 : 0.f;
           }
-        }
-      };
-      if (p.partial) {
-        const size_t part = th * p.parts + split;
-        if (row_on && (PAIR || w == 0)) p.ml_part[part] = make_float2(M, L);
-        float4* dst = reinterpret_cast<float4*>(p.o_part + part * HD);
-        if (n_tiles > 0) {
-#pragma unroll 1
-          for (int k = 0; k < CHUNKS; ++k) {
-            const int c = (PAIR ? 0 : w * CHUNKS) + k;
-            float o[32];
-            columns(c, o);
-            if (row_on) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) dst[8 * c + e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          for (int e = 0; e < 32; ++e) o[e] = f0 != 0.f ? __uint_as_float(a[e]) * f0 : 0.f;
+          if constexpr (!PAIR) {
+            if (__any_sync(0xffffffffu, f1 != 0.f)) {
+              tc::tmem_ld32(tO(1) + lane_off + c * 32, a);
+              tc::tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] += f1 != 0.f ? __uint_as_float(a[e]) * f1 : 0.f;
             }
           }
         }
-      } else {
-        // join with the partial triples of the shared keys (none when this launch visited them), normalise, store the row
-        const int n_parts = p.shared ? 0 : p.parts;
-        const bool seen = row_on && slot >= pad;                       // a query in front of its row's first token is padding: zeros
-        const float2* ml = p.ml_part + th * n_parts;
-        float M2 = M;
-        if (seen)
-          for (int s = 0; s < n_parts; ++s) {
-            const float2 v = __ldcg(ml + s);
-            if (v.y != 0.f) M2 = fmaxf(M2, v.x);
-          }
-        const float Ms = M2 == -INFINITY ? 0.f : M2;
-        const float f = L != 0.f ? exp2f(M - Ms) : 0.f;
-        L *= f; f0 *= f; f1 *= f;
-        if (seen)
-          for (int s = 0; s < n_parts; ++s) {
-            const float2 v = __ldcg(ml + s);
-            if (v.y != 0.f) L += v.y * exp2f(v.x - Ms);
-          }
-        const float inv = seen && L != 0.f ? 1.0f / L : 0.f;
-        uint4* dst = reinterpret_cast<uint4*>(p.out + th * HD);
-#pragma unroll 1
-        for (int k = 0; k < CHUNKS; ++k) {
-          const int c = (PAIR ? 0 : w * CHUNKS) + k;
-          float o[32];
-          columns(c, o);
-          if (seen) {
-            for (int s = 0; s < n_parts; ++s) {
-              const float2 v = __ldcg(ml + s);
-              if (v.y == 0.f) continue;
-              const float g = exp2f(v.x - Ms);
-              const float4* src = reinterpret_cast<const float4*>(p.o_part + (th * n_parts + s) * HD + c * 32);
+        if (p.partial) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float4 x = __ldcg(src + e);
-                o[4 * e] = fmaf(x.x, g, o[4 * e]);
-                o[4 * e + 1] = fmaf(x.y, g, o[4 * e + 1]);
-                o[4 * e + 2] = fmaf(x.z, g, o[4 * e + 2]);
-                o[4 * e + 3] = fmaf(x.w, g, o[4 * e + 3]);
-              }
-            }
-          }
-          if (row_on) {
+          for (int e = 0; e < 8; ++e)
+            asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128 + ((e ^ (lane & 7)) << 4)), "f"(o[4 * e]), "f"(o[4 * e + 1]), "f"(o[4 * e + 2]),
+                         "f"(o[4 * e + 3]) : "memory");
+          __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              auto v = [&](int i) { return seen ? o[8 * e + i] * inv : 0.f; };
-              dst[c * 4 + e] = make_uint4(pack_bf16(v(0), v(1)), pack_bf16(v(2), v(3)), pack_bf16(v(4), v(5)), pack_bf16(v(6), v(7)));
-            }
+          for (int i = 0; i < 8; ++i) {
+            const int r2 = 4 * i + (lane >> 3), th2 = __shfl_sync(0xffffffffu, th, r2);
+            float4 v;
+            asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(stage + r2 * 128 + (((lane ^ r2) & 7) << 4)) : "memory");
+            if (warp_row + r2 < n_rows) *reinterpret_cast<float4*>(p.o_part + ((size_t)th2 * p.parts + part) * HD + 32 * c + 4 * (lane & 7)) = v;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            auto v = [&](int i) { return inv != 0.f ? o[8 * e + i] * inv : 0.f; };
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)), "r"(pack_bf16(v(0), v(1))),
+                         "r"(pack_bf16(v(2), v(3))), "r"(pack_bf16(v(4), v(5))), "r"(pack_bf16(v(6), v(7))) : "memory");
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r2 = 8 * i + (lane >> 2), th2 = __shfl_sync(0xffffffffu, th, r2);
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(stage + r2 * 64 + (((lane ^ (r2 >> 1)) & 3) << 4)) : "memory");
+            if (warp_row + r2 < n_rows) *reinterpret_cast<uint4*>(p.out + (size_t)th2 * HD + 32 * c + 8 * (lane & 3)) = v;
           }
         }
+        __syncwarp();
       }
     }
     tc::fence_before_sync();
@@ -817,9 +789,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
   if (warp == 0) tc::tmem_dealloc(tmem, 512);
 }
 
-// Joins the triples of a step: a warp per (token, head).
+// Joins the triples of a (token, head), a warp each.  `own`: the part of the own keys of a prompt; a query without any is padding and gives zeros (-1: one token,
+// which sees itself).
 template <int HD>
-__global__ void __launch_bounds__(256) prefix_join_kernel(const float* __restrict__ o_part, const float2* __restrict__ ml_part, __nv_bfloat16* out, int rows, int parts) {
+__global__ void __launch_bounds__(256) prefix_join_kernel(const float* __restrict__ o_part, const float2* __restrict__ ml_part, __nv_bfloat16* out, int rows, int parts, int own) {
   constexpr int V = HD / 32;                                           // columns of a lane
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   pdl_wait();
@@ -869,8 +842,12 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const float* __restric
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] = fmaf(f[u], x[u][e], acc[e]);
   }
-  const float inv = 1.f / L;                                           // the new token is always seen: L > 0
+  const bool seen = own < 0 || ml[own].y != 0.f;                       // (the same address for the warp)
+  const float inv = seen ? 1.f / L : 0.f;
   uint32_t* dst = reinterpret_cast<uint32_t*>(out + (size_t)row * HD + V * lane);
+  if (!seen)
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
   if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
   else *dst = pack_bf16(acc[0] * inv, acc[1] * inv);
 }
@@ -888,6 +865,13 @@ static int px_launch(const PxParams& p, unsigned ctas, const CUtensorMap& pk, co
     set.fetch_or(bit, std::memory_order_release);
   }
   JL_CUDA(launch_pdl(prefix_attn_kernel<HD, ROTATE, PAIR>, dim3(ctas), dim3(PX_THREADS), (size_t)Tile::SMEM, st, pk, pv, ok, ov, p));
+  return JL_OK;
+}
+
+static int px_join(const PxParams& p, __nv_bfloat16* out, int rows, int hd, int own, cudaStream_t st) {
+  const dim3 grid((unsigned)((rows + 7) / 8));
+  if (hd == 128) JL_CUDA(launch_pdl(prefix_join_kernel<128>, grid, dim3(256), 0, st, (const float*)p.o_part, (const float2*)p.ml_part, out, rows, p.parts, own));
+  else JL_CUDA(launch_pdl(prefix_join_kernel<64>, grid, dim3(256), 0, st, (const float*)p.o_part, (const float2*)p.ml_part, out, rows, p.parts, own));
   return JL_OK;
 }
 
@@ -979,7 +963,7 @@ extern "C" JL_API size_t jl_prefix_attn_scratch_bytes(int B, int S, int groups, 
   if (B < 1 || S < 1 || groups < 1 || B % groups != 0 || nkv < 1 || nh % nkv != 0 || prefix < 0) return 0;
   const int G = nh / nkv;
   int parts = px_splits((long)(B / groups) * S * G, groups, nkv, prefix);
-  if (S == 1) parts += px_own_splits((long)B * nkv);
+  parts += S == 1 ? px_own_splits((long)B * nkv) : 1;
   return px_part_bytes((long)B * S, nh, hd, parts);
 }
 
@@ -1007,7 +991,7 @@ extern "C" JL_API int jl_decode_attn_prefix(const void* qkv, const void* prefix_
   if (rc0) return rc0;
   JL_CHECK_ARG(cache_len != nullptr && max_pos >= 1, "jl_decode_attn_prefix: the slot of the new token and its tables are required");
   const int G = nh / nkv, rows = B / groups;
-  JL_CHECK_ARG((long)B * nkv <= (1l << 26), "jl_decode_attn_prefix: %d rows of %d key heads", B, nkv);
+  JL_CHECK_ARG((long)B * nh < (1l << 26), "jl_decode_attn_prefix: %d rows of %d heads", B, nh);
   CUtensorMap pk, pv;
   int rc = make_tmap_3d_bf16(&pk, prefix_k, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
   if (rc == JL_OK) rc = make_tmap_3d_bf16(&pv, prefix_v, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
@@ -1026,10 +1010,7 @@ extern "C" JL_API int jl_decode_attn_prefix(const void* qkv, const void* prefix_
   p.ml_part = (float2*)(p.o_part + (size_t)B * nh * p.parts * hd);
   rc = px_dispatch(p, (long)rows * G, groups, true, hd, pk, pv, pk, pv, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;
-  const dim3 grid((unsigned)(((long)B * nh + 7) / 8));
-  if (hd == 128) JL_CUDA(launch_pdl(prefix_join_kernel<128>, grid, dim3(256), 0, (cudaStream_t)stream, p.o_part, p.ml_part, (__nv_bfloat16*)out, B * nh, p.parts));
-  else JL_CUDA(launch_pdl(prefix_join_kernel<64>, grid, dim3(256), 0, (cudaStream_t)stream, p.o_part, p.ml_part, (__nv_bfloat16*)out, B * nh, p.parts));
-  return JL_OK;
+  return px_join(p, (__nv_bfloat16*)out, B * nh, hd, -1, (cudaStream_t)stream);
 }
 
 extern "C" JL_API int jl_prefill_attn_prefix(const void* q, const void* prefix_k, const void* prefix_v, const void* k_cache, const void* v_cache,
@@ -1041,7 +1022,7 @@ extern "C" JL_API int jl_prefill_attn_prefix(const void* q, const void* prefix_k
   if (rc) return rc;
   JL_CHECK_ARG(start >= 0 && start <= T - S, "jl_prefill_attn_prefix: start=%d + S=%d exceeds cache capacity %d", start, S, T);
   const int G = nh / nkv, rows = B / groups;
-  JL_CHECK_ARG((long)rows * S * G <= (1l << 30), "jl_prefill_attn_prefix: %d rows of %d tokens share one prefix", rows, S);
+  JL_CHECK_ARG((long)B * S * nh < (1l << 31), "jl_prefill_attn_prefix: %d rows of %d tokens of %d heads", B, S, nh);
   CUtensorMap pk, pv, ok, ov;
   rc = make_tmap_3d_bf16(&pk, prefix_k, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
   if (rc == JL_OK) rc = make_tmap_3d_bf16(&pv, prefix_v, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
@@ -1059,12 +1040,15 @@ extern "C" JL_API int jl_prefill_attn_prefix(const void* q, const void* prefix_k
     p.shared = p.own = 1;
     return px_dispatch(p, (long)S * G, B, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   }
-  const int splits = px_splits((long)rows * S * G, groups, nkv, P);
+  p.splits = px_splits((long)rows * S * G, groups, nkv, P);
+  p.parts = p.splits + 1;
   p.o_part = (float*)scratch;
-  p.ml_part = (float2*)(p.o_part + (size_t)B * S * nh * splits * hd);
-  p.shared = p.partial = 1; p.splits = p.parts = splits;
+  p.ml_part = (float2*)(p.o_part + (size_t)B * S * nh * p.parts * hd);
+  p.shared = p.partial = 1;
   rc = px_dispatch(p, (long)rows * S * G, groups, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;
-  p.shared = p.partial = 0; p.own = 1; p.splits = 1;
-  return px_dispatch(p, (long)S * G, B, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
+  p.shared = 0; p.own = 1; p.part0 = p.splits; p.splits = 1;
+  rc = px_dispatch(p, (long)S * G, B, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
+  if (rc != JL_OK) return rc;
+  return px_join(p, (__nv_bfloat16*)out, B * S * nh, hd, p.part0, (cudaStream_t)stream);
 }
