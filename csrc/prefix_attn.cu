@@ -8,8 +8,8 @@
 // is a join of two triples (reference exponent m, sum l, weighted values o):  M = max(m1, m2),  o = o1 2^(m1 - M) + o2 2^(m2 - M),  l likewise.
 //   * one token per row (jl_decode_attn_prefix): one launch in which some CTAs take the shared keys, tiles of queries by splits of the keys, and others the
 //     rows' own keys, a warp per (row, key head), appending the new one; all leave partial triples in fp32, and a second, small launch joins them;
-//   * S tokens per row (jl_prefill_attn_prefix): the same for the shared keys, then a second launch over every row's own keys, causal, and the join; or
-//     one launch over both sets, tile after tile, where a row's queries fill tiles by themselves.
+//   * S tokens per row (jl_prefill_attn_prefix): the same for the shared keys, then a second launch over every row's own keys, causal, and the join; or, where
+//     a row's queries fill tiles by themselves, one launch over both sets of keys, tile after tile, whole or in splits that the join puts together.
 //
 // One CTA owns a tile of 128 queries of one key head, as in flash_prefill.cu: a warp asks for K and V tiles of 64 keys (TMA, 128-byte swizzle), a warp
 // issues S = Q·Kᵀ into one of two score tiles in TMEM and O += P·V with P read from TMEM, four warps hold one query row per thread: one pass over 64
@@ -439,16 +439,17 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
   int s_lo = 0, s_hi = 0, o_lo = 0, o_hi = 0;
   const int g_lo = p.prefix_pad ? max(p.prefix_pad[group], 0) : 0;
   const int g_hi = p.prefix_len ? min(p.prefix_len[group], p.P) : p.P;
-  if (p.shared) {
-    const int n = max(g_hi - g_lo, 0);
-    const int chunk = ((n + p.splits - 1) / p.splits + PX_BN - 1) / PX_BN * PX_BN;
-    s_lo = g_lo + min(split * chunk, n);
-    s_hi = g_lo + min((split + 1) * chunk, n);
-  }
   const int pad = p.own && p.pad_left ? max(p.pad_left[z], 0) : 0;
-  if (p.own) {
-    o_lo = pad;
-    o_hi = max(p.start + ((q0 + n_rows - 1) >> p.gs) + 1, o_lo);             // slot of the tile's last token: its last key
+  {
+    const int n_sh = p.shared ? max(g_hi - g_lo, 0) : 0, sh_tiles = (n_sh + PX_BN - 1) / PX_BN;
+    const int own_end = p.own ? max(p.start + ((q0 + n_rows - 1) >> p.gs) + 1, pad) : pad;       // slot of the tile's last token: its last key
+    // this split's tiles [j0, j1) of the shared keys' and then the own keys'
+    const int all = sh_tiles + (own_end - pad + PX_BN - 1) / PX_BN, per = (all + p.splits - 1) / p.splits;
+    const int j0 = min(split * per, all), j1 = min(j0 + per, all);
+    s_lo = g_lo + min(min(j0, sh_tiles) * PX_BN, n_sh);
+    s_hi = g_lo + min(min(j1, sh_tiles) * PX_BN, n_sh);
+    o_lo = min(pad + max(j0 - sh_tiles, 0) * PX_BN, own_end);
+    o_hi = min(pad + max(j1 - sh_tiles, 0) * PX_BN, own_end);
   }
   const int n_shared = (s_hi - s_lo + PX_BN - 1) / PX_BN, n_tiles = n_shared + (o_hi - o_lo + PX_BN - 1) / PX_BN;
   // set w's tile i is tile number i (PAIR) or 2 i + w of the keys
@@ -789,8 +790,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
   if (warp == 0) tc::tmem_dealloc(tmem, 512);
 }
 
-// Joins the triples of a (token, head), a warp each.  `own`: the part of the own keys of a prompt; a query without any is padding and gives zeros (-1: one token,
-// which sees itself).
+// Joins the triples of a (token, head), a warp each.  `own`: the part of the own keys of a prompt, -1 where every part says itself that a query
+// is padding: without own keys, or without any, it gives zeros.
 template <int HD>
 __global__ void __launch_bounds__(256) prefix_join_kernel(const float* __restrict__ o_part, const float2* __restrict__ ml_part, __nv_bfloat16* out, int rows, int parts, int own) {
   constexpr int V = HD / 32;                                           // columns of a lane
@@ -842,7 +843,7 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const float* __restric
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] = fmaf(f[u], x[u][e], acc[e]);
   }
-  const bool seen = own < 0 || ml[own].y != 0.f;                       // (the same address for the warp)
+  const bool seen = L != 0.f && (own < 0 || ml[own].y != 0.f);         // (the same address for the warp)
   const float inv = seen ? 1.f / L : 0.f;
   uint32_t* dst = reinterpret_cast<uint32_t*>(out + (size_t)row * HD + V * lane);
   if (!seen)
@@ -943,14 +944,21 @@ static PxStep px_step(int B, int groups, int nkv, int G, int hd, int P, int T) {
   return r;
 }
 
-// Whether one launch over shared and own keys together, every row's queries in tiles of their own, is estimated to be no slower than shared keys for all rows of a
-// group together and then the own keys.
-static bool px_one_launch(int S, int G, int B, int groups, int nkv, int P, int start) {
-  float two;
-  px_splits((long)(B / groups) * S * G, groups, nkv, P, PX_SMS, &two);
-  const float own = (float)(start + S) / PX_BN;
-  two += px_rounds((long)S * G, B, nkv, 1, own);
-  return px_rounds((long)S * G, B, nkv, 1, (float)P / PX_BN + own) <= two;
+// S tokens per row.  Both sets of keys in one launch, every row's queries in tiles of their own, in `splits`; or the shared keys for all rows of a group together, in
+// `splits`, and then the own keys (taken to be the call's own tokens).
+struct PxPrompt { bool both; int splits; };
+static PxPrompt px_prompt(int B, int S, int groups, int nkv, int G, int P) {
+  const long queries = (long)(B / groups) * S * G, rows = (long)B * S * G * nkv;
+  const float own = (float)S / PX_BN, shared = (float)P / PX_BN, join = 4e-4f * (float)rows;
+  PxPrompt r{false, 1};
+  float least;
+  r.splits = px_splits(queries, groups, nkv, P, PX_SMS, &least);
+  least += px_rounds((long)S * G, B, nkv, 1, own) + join + 3.f;
+  for (int s = 1; s <= 4; ++s) {
+    const float c = px_rounds((long)S * G, B, nkv, s, (shared + own) / s) + (s > 1 ? s * join + 3.f : 0.f);
+    if (c < least) { least = c; r = PxPrompt{true, s}; }
+  }
+  return r;
 }
 
 static size_t px_part_bytes(long tokens, int nh, int hd, int splits) { return (size_t)tokens * nh * splits * (hd + 2) * sizeof(float); }
@@ -962,8 +970,13 @@ using namespace jl;
 extern "C" JL_API size_t jl_prefix_attn_scratch_bytes(int B, int S, int groups, int nh, int nkv, int hd, int prefix) {
   if (B < 1 || S < 1 || groups < 1 || B % groups != 0 || nkv < 1 || nh % nkv != 0 || prefix < 0) return 0;
   const int G = nh / nkv;
-  int parts = px_splits((long)(B / groups) * S * G, groups, nkv, prefix);
-  parts += S == 1 ? px_own_splits((long)B * nkv) : 1;
+  const PxPrompt plan = px_prompt(B, S, groups, nkv, G, prefix);
+  int parts = plan.both ? (plan.splits > 1 ? plan.splits : 0) : plan.splits + 1;
+  if (S == 1) {                                                        // either form of one token
+    const int step = px_splits((long)(B / groups) * G, groups, nkv, prefix) + px_own_splits((long)B * nkv);
+    parts = parts > step ? parts : step;
+  }
+  if (parts == 0) return 16;                                           // (nothing is left in between; never nothing)
   return px_part_bytes((long)B * S, nh, hd, parts);
 }
 
@@ -1035,15 +1048,18 @@ extern "C" JL_API int jl_prefill_attn_prefix(const void* q, const void* prefix_k
   p.out = (__nv_bfloat16*)out;
   p.S = S; p.rows = rows; p.nh = nh; p.nkv = nkv; p.gs = G == 1 ? 0 : (G == 2 ? 1 : (G == 4 ? 2 : 3)); p.P = P; p.T = T; p.start = start;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.splits = 1;
-  if (px_one_launch(S, G, B, groups, nkv, P, start)) {
-    p.shared = p.own = 1;
-    return px_dispatch(p, (long)S * G, B, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
-  }
-  p.splits = px_splits((long)rows * S * G, groups, nkv, P);
-  p.parts = p.splits + 1;
+  const PxPrompt plan = px_prompt(B, S, groups, nkv, G, P);
+  p.splits = plan.splits;
+  p.parts = plan.both ? plan.splits : plan.splits + 1;
   p.o_part = (float*)scratch;
   p.ml_part = (float2*)(p.o_part + (size_t)B * S * nh * p.parts * hd);
+  if (plan.both) {
+    p.shared = p.own = 1;
+    p.partial = p.splits > 1;
+    rc = px_dispatch(p, (long)S * G, B, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
+    if (rc != JL_OK || !p.partial) return rc;
+    return px_join(p, (__nv_bfloat16*)out, B * S * nh, hd, -1, (cudaStream_t)stream);
+  }
   p.shared = p.partial = 1;
   rc = px_dispatch(p, (long)rows * S * G, groups, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;
