@@ -145,7 +145,8 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
     hi = first + min((part + 1) * chunk, valid);
   };
   // what is asked for next: block [r_base, r_base + KPI) of unit r_u
-  int r_u = blockIdx.x * Own::WARPS + warp, r_base = 0, r_hi = 0, r_st = 0;
+  const int first_unit = ((int)blockIdx.x - ((int)gridDim.x - p.own_ctas)) * Own::WARPS + warp;
+  int r_u = first_unit, r_base = 0, r_hi = 0, r_st = 0;
   if (r_u < units) range(r_u, r_base, r_hi);
   // 16-byte copies into the swizzled layout, eight 512-byte rows of requests each for keys and values; keys behind the last one become zeros (a weight of
   // zero times a NaN is a NaN).  By TMA, whose boxes of 16 rows leave the SM at 28 bytes a cycle, the warps waited for its queue a third of their time.
@@ -185,7 +186,7 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
 
   int st = 0;
 #pragma unroll 1
-  for (int u = blockIdx.x * Own::WARPS + warp; u < units; u += step) {
+  for (int u = first_unit; u < units; u += step) {
     int lo, hi;
     range(u, lo, hi);
     const int item = u / p.own_splits, part = u - item * p.own_splits, b = item / p.nkv, kvh = item - b * p.nkv;
@@ -391,13 +392,13 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = 1 << p.gs;
   if constexpr (ROTATE) {
-    if ((int)blockIdx.x < p.own_ctas) {
+    if ((int)blockIdx.x >= (int)gridDim.x - p.own_ctas) {
       px_own_keys<HD>(p, px_smem);
       return;
     }
   }
   // z: group (shared keys alone) or row; kvh: key head; qt: query tile (or pair), longest first; split of the shared keys
-  int idx = (int)blockIdx.x - p.own_ctas;
+  int idx = (int)blockIdx.x;
   const int split = idx % p.splits;
   idx /= p.splits;
   const int qt = p.tiles_q - 1 - idx % p.tiles_q;
@@ -917,7 +918,10 @@ static int px_splits(long queries, int groups, int nkv, int prefix, int sms = PX
   return best;
 }
 
-// A step: CTAs and parts for the own keys (of caches of T slots, taken to be half full), splits for the shared keys on the other SMs.
+// A step: CTAs and parts for the own keys, splits for the shared keys.  The shared keys' CTAs come first in the grid and the own keys', a unit for every warp, take the
+// SMs that are left and those that get free: how full the caches are is known on the device alone, and an order that is right at any fill beats a division of the
+// SMs between the two (us on one B200, a division by estimate, the best of all divisions, this: 96 rows over 32768 shared 118, 118, 106; 48 rows x 32 heads, a
+// quarter full, 55, 41, 44; 4 x 16 rows over 3501 42, 42, 45; own keys first 135, 50, 42).  What is estimated is the count of splits alone, at half full caches.
 struct PxStep { int own_ctas, own_splits, splits; };
 static int px_own_splits(long items) {                                 // parts that give every warp of all SMs one
   const long s = (8l * PX_SMS + items - 1) / items;
@@ -928,19 +932,20 @@ static PxStep px_step(int B, int groups, int nkv, int G, int hd, int P, int T) {
   const long items = (long)B * nkv, queries = (long)(B / groups) * G;
   const int most = px_own_splits(items), by_keys = (T + 127) / 128;
   r.own_splits = most < by_keys ? most : by_keys;
-  const long full = (items * r.own_splits + 7) / 8;                    // CTAs with a unit for every warp
-  // SM time of both sides in us: 64 KB/us of own keys per SM and a way in and out per unit; a tile of shared keys
-  const float own = (float)items * ((float)T * 0.5f * (float)hd * 4.f / 64e3f + (float)r.own_splits * 0.5f);
-  const float tile = queries > PX_BM ? 1.1f : 0.65f;
-  const float shared = (float)(px_tiles(queries) * groups * nkv) * ((float)P / PX_BN * tile + 5.f);
-  long n = (long)(PX_SMS * own / (own + shared) + 0.5f);
-  n = n < 1 ? 1 : (n > PX_SMS - 8 ? PX_SMS - 8 : n);
-  // the same number of units for every warp, or one less
-  const long rounds = (2 * full + n) / (2 * n);
-  r.own_ctas = (int)((full + (rounds > 0 ? rounds : 1) - 1) / (rounds > 0 ? rounds : 1));
-  r.splits = px_splits(queries, groups, nkv, P, PX_SMS - r.own_ctas);
-  const int cap = px_splits(queries, groups, nkv, P);                  // (what the scratch is sized for)
-  if (r.splits > cap) r.splits = cap;
+  r.own_ctas = (int)((items * r.own_splits + 7) / 8);
+  // us: 3 in and out of a unit, 55 KB/us of own keys for the 8 warps of an SM (what one SM draws under load); 0.9 a tile of shared keys and 1.25 for two tiles of
+  // queries, 8 in and out of a CTA
+  const float unit = 3.f + (float)T * 0.5f / (float)r.own_splits * (float)hd * 4.f * 8.f / 55e3f, tile = queries > PX_BM ? 1.25f : 0.9f;
+  const int tiles = (P + PX_BN - 1) / PX_BN, cap = px_splits(queries, groups, nkv, P);       // (what the scratch is sized for)
+  const bool half = queries > PX_BM && (queries % (2 * PX_BM) <= PX_BM && queries % (2 * PX_BM) != 0);
+  const float heads = (float)(groups * nkv), work = heads * ((float)px_tiles(queries) - (half ? 0.22f : 0.f)) * (float)tiles * tile + (float)r.own_ctas * unit;
+  float best = 0.f;
+  r.splits = 1;
+  for (int s = 1; s <= cap && (s == 1 || 2 * s <= tiles); ++s) {
+    const float ctas = heads * (float)px_tiles(queries) * s, cta = (float)((tiles + s - 1) / s) * tile + 8.f;
+    const float us = fmaxf(cta, (work + 8.f * ctas) / PX_SMS + (ctas <= PX_SMS ? 0.5f * unit : 0.4f * cta)) + (float)queries * heads * s * 3e-4f;
+    if (best == 0.f || us < best) { best = us; r.splits = s; }
+  }
   return r;
 }
 
