@@ -135,7 +135,7 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
   pdl_launch_dependents();
 
   const int G = 1 << p.gs, units = p.B * p.nkv * p.own_splits, step = p.own_ctas * Own::WARPS;
-  const int len = min(*p.cache_len, p.T);                  // keys in front of the new token
+  const int len = min(max(*p.cache_len, 0), p.T);                // keys in front of the new token
   // first and last + 1 key of unit u
   auto range = [&](int u, int& lo, int& hi) {
     const int item = u / p.own_splits, part = u - item * p.own_splits, b = item / p.nkv;
@@ -567,7 +567,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
             const int token = token0 + ((q0 + qr) >> p.gs), h = kvh * G + ((q0 + qr) & (G - 1));
             x[u] = *reinterpret_cast<const uint4*>(p.q + (size_t)token * p.ldq + (size_t)h * HD + 8 * ch);
             if constexpr (ROTATE) {
-              int pos = max(g_hi - g_lo, 0) + min(*p.cache_len, p.T) - (p.pad_left ? p.pad_left[token] : 0);
+              int pos = max(g_hi - g_lo, 0) + min(max(*p.cache_len, 0), p.T) - (p.pad_left ? p.pad_left[token] : 0);
               pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
               c4[u] = __ldg(reinterpret_cast<const float4*>(p.cos_t) + (size_t)pos * CH + ch);
               s4[u] = __ldg(reinterpret_cast<const float4*>(p.sin_t) + (size_t)pos * CH + ch);
@@ -634,8 +634,9 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
 #pragma unroll
         for (int e = 0; e < 32; ++e) mx4[e & 3] = max3_nan(mx4[e & 3], __uint_as_float(v0[e]), __uint_as_float(v1[e]));
         const float t = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * p.scale_log2;
-        const bool need = t > m_ref + PX_RESCALE || (m_ref == -INFINITY && t > -INFINITY);
-        bool odd = !(t < INFINITY);                                    // NaN or infinite scores show in the result: no shortcuts
+        // (rows behind the last query hold what the memory held before: they have no say in the way that the warp takes)
+        const bool need = row_on && (t > m_ref + PX_RESCALE || (m_ref == -INFINITY && t > -INFINITY));
+        bool odd = row_on && !(t < INFINITY);                                    // NaN or infinite scores show in the result: no shortcuts
         if (i == 0) m_ref = t;
         if (__any_sync(0xffffffffu, odd || (i > 0 && need))) {
           odd = __any_sync(0xffffffffu, odd);

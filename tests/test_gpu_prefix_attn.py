@@ -60,6 +60,9 @@ STEPS = [  # rows, groups, nh, nkv, hd, P, T, own keys, ragged
     (70, 2, 8, 4, 128, 300, 20, 5, True),
     (3, 1, 4, 4, 128, 1500, 700, 650, True),     # splits of both kinds
     (2, 1, 2, 1, 64, 3000, 1400, 1300, True),
+    (75, 1, 4, 1, 64, 1000, 12, 5, True),        # 300 queries of a key head: a pair of tiles and one tile that is not full
+    (100, 1, 4, 1, 128, 700, 20, 11, False),     # 400: two pairs, the last tile with 16 queries
+    (66, 2, 16, 2, 128, 520, 9, 0, True),        # 264: the second pair has eight queries
 ]
 
 
@@ -103,6 +106,10 @@ PROMPTS = [  # rows, groups, nh, nkv, hd, P, start, S, T, ragged
     (4, 1, 32, 32, 64, 100, 0, 130, 130, True),      # one key head per query head: a row's queries fill two tiles, 256 of them
     (2, 1, 32, 32, 128, 200, 11, 256, 300, False),   # whole tiles, enough of them: one launch over both sets of keys
     (3, 3, 32, 32, 64, 70, 2, 256, 258, True),
+    (2, 2, 16, 2, 64, 600, 4, 70, 80, True),         # both sets of keys in three splits, 560 queries of a key head
+    (1, 1, 8, 2, 128, 2500, 0, 300, 300, False),     # in four
+    (40, 1, 16, 2, 64, 1000, 7, 3, 16, True),        # the shared keys for all rows together, in splits, then the own keys
+    (1, 1, 8, 2, 128, 2500, 9, 1, 12, True),         # one token
 ]
 
 
@@ -124,3 +131,104 @@ def test_prompt(B, groups, nh, nkv, hd, P, start, S, T, ragged):
     assert (err <= bound(want, mag)).all(), float((err / bound(want, mag)).max())
     for b in range(B):                                                       # padding: exact zeros
         assert (out[b, :max(0, c["pad"][b] - start)] == 0).all()
+
+
+def small(dev, B=3, groups=1, nh=4, nkv=2, hd=64, P=90, T=20, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16).to(dev)
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    cos, sin = oracle.tables(hd, P + T + 1)
+    return dict(qkv=rnd(B, (nh + 2 * nkv) * hd), pk=rnd(groups, nkv, P, hd), pv=rnd(groups, nkv, P, hd), kc=rnd(B, nkv, T, hd), vc=rnd(B, nkv, T, hd), cos=cos.to(dev), sin=sin.to(dev),
+                cache_len=i([7]), pad_left=i([2] * B), prefix_len=i([P - 3] * groups), prefix_pad=i([1] * groups), nh=nh, nkv=nkv, hd=hd)
+
+
+def call(c, **kw):
+    c = dict(c, **kw)
+    return K.decode_attn_prefix(c["qkv"], c["pk"], c["pv"], c["kc"], c["vc"], c["cos"], c["sin"], c["cache_len"], c["pad_left"], c["prefix_len"], c["prefix_pad"],
+                                c["nh"], c["nkv"], c["hd"], scratch=c.get("scratch"))
+
+
+def agree(got, want):
+    """Two results of the same sum, each within the bound of their definition: 2 (2^-8 |out| + 2^-7 mean |v|), with mean |v| below 5 for values of a normal draw."""
+    assert ((got.cpu().float() - want.float()).abs() <= 2 * (2 ** -8 * want.float().abs() + 2 ** -7 * 5)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("full", [20, 25])
+def test_full_cache_stores_nothing(full):
+    """From slot T on the new token sees every key and itself, and the cache stays as it is."""
+    c, d = small("cpu"), small(DEV)
+    kc, vc = d["kc"].clone(), d["vc"].clone()
+    got = call(d, cache_len=i32([full]))
+    assert torch.equal(d["kc"], kc) and torch.equal(d["vc"], vc)
+    agree(got, call(c, cache_len=torch.tensor([full], dtype=torch.int32)))
+
+
+@pytest.mark.gpu
+def test_row_bounds_outside_the_caches():
+    """Bounds that no cache has are taken as the nearest that it has: the calls of the two sides agree, and nothing outside is touched."""
+    for kw in (dict(pad_left=[50, 0, 7]), dict(prefix_len=[500]), dict(prefix_pad=[80]), dict(prefix_len=[0]), dict(prefix_len=[5], prefix_pad=[9])):
+        c, d = small("cpu"), small(DEV)
+        host = {k: torch.tensor(v, dtype=torch.int32) for k, v in kw.items()}
+        agree(call(d, **{k: v.to(DEV) for k, v in host.items()}), call(c, **host))
+    d = small(DEV)
+    assert torch.isfinite(call(d, cache_len=i32([-4])).float()).all()        # slot 0
+
+
+@pytest.mark.gpu
+def test_a_nan_reaches_the_rows_that_see_it():
+    d = small(DEV, B=4, groups=2)
+    d["pk"][1, 0, 40, 3] = NAN
+    out = torch.isnan(call(d).float()).view(2, 2, 2, 2, 64)                  # [group, row, key head, query head, :]
+    assert out[1, :, 0].all() and not out[0].any() and not out[1, :, 1].any()
+    d = small(DEV)
+    d["vc"][1, 1, 4, 9] = NAN
+    out = torch.isnan(call(d).float()).view(3, 2, 2, 64)
+    assert out[1, 1, :, 9].all() and int(out.sum()) == 2
+
+
+@pytest.mark.gpu
+def test_graphs_on_two_streams():
+    """Two captured steps with workspaces of their own, replayed at the same time on streams of their own, and again after the token count moved on."""
+    made, want = [], []
+    for seed in (3, 4):
+        d = small(DEV, B=40, T=300, seed=seed)
+        d["cache_len"].fill_(200)
+        d["scratch"] = K.prefix_attn_scratch(40, 1, 1, 4, 2, 64, 90, torch.device(DEV))
+        want.append([call(dict(d, kc=d["kc"].clone(), vc=d["vc"].clone()), cache_len=i32([n])).clone() for n in (200, 260)])
+        g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(g, stream=s):
+            out = call(d)
+        made.append((d, g, s, out))
+    torch.cuda.synchronize()
+    for at, n in enumerate((200, 260)):
+        for d, *_ in made:
+            d["cache_len"].fill_(n)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for _, g, s, _ in made:
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        if at == 0:
+            for (_, _, _, out), w in zip(made, want):
+                assert torch.equal(out, w[0])
+        else:                                                                # slot 200 holds the first step's token now
+            for d, _, _, out in made:
+                assert torch.equal(out, call(dict(d, kc=d["kc"].clone(), vc=d["vc"].clone())))
+
+
+@pytest.mark.gpu
+def test_workspaces_and_devices_are_refused(monkeypatch):
+    d = small(DEV)
+    need = K.prefix_attn_scratch(3, 1, 1, 4, 2, 64, 90, torch.device(DEV))
+    with pytest.raises(Exception, match="scratch"):
+        call(d, scratch=need[:need.numel() // 2])
+    with pytest.raises(Exception, match="16-byte"):
+        call(d, scratch=torch.empty(need.numel() + 8, device=DEV)[1:])
+    with pytest.raises(ValueError):
+        K.prefix_attn_scratch(3, 1, 2, 4, 2, 64, 90, torch.device(DEV))
+    monkeypatch.setattr(K, "_get_device", lambda: 1)
+    for f in (lambda: call(d), lambda: K.constrain_logits(torch.zeros(1, 8, device=DEV))):
+        with pytest.raises(ValueError, match="current device"):
+            f()
