@@ -9,7 +9,7 @@
 // A CTA owns a slice of one row's vocabulary and keeps one word per token of the slice in shared memory: occurrences behind the prompt in the low bits, and bits
 // for "occurred", "has a bias", "has several" (whole numbers and bits: the order of the atomics does not show).  Everything it reads is asked for at once, the slice's
 // logits, the row's bounds, the first tokens of its history, its first biases: a CTA's way is a chain of memory latencies, and a batch of 96 rows is seven rounds of
-// CTAs.  Then one pass writes the slice, and the threads that were first to mark a token's bias add it, all entries of a token in their order.  No state
+// CTAs.  A second table has the bias of a token; where there are several, the thread that was first to mark it goes through all of them in their order.  No state
 // is kept between calls: the history is the sequence buffer that the decode loop writes anyway, so forks, restarts and replayed graphs need nothing.
 #include "common.cuh"
 #include "jllama_b200.h"
@@ -37,9 +37,10 @@ struct RulesParams {
 // TH threads with N groups of four tokens each.  Rows whose logits and results lie alike on 16-byte boundaries (8-byte ones for 16-bit logits)
 // start their groups there, others load and store token by token.
 template <typename T, int TH, int N>
-__global__ void __launch_bounds__(TH, 4) logit_rules_kernel(const RulesParams p) {
+__global__ void __launch_bounds__(TH, 1024 / TH) logit_rules_kernel(const RulesParams p) {
   constexpr int SLICE = 4 * N * TH;
   extern __shared__ __align__(16) unsigned lr_count[];
+  float* lr_value = reinterpret_cast<float*>(lr_count + SLICE);         // of the tokens with a bias
   const int b = blockIdx.y, t = threadIdx.x;
   const T* x = static_cast<const T*>(p.logits) + (size_t)b * p.ld;
   float* y = p.out + (size_t)b * p.ldo;
@@ -59,14 +60,27 @@ __global__ void __launch_bounds__(TH, 4) logit_rules_kernel(const RulesParams p)
   const float r = p.rep ? p.rep[b] : p.rep1, f = p.freq ? p.freq[b] : p.freq1, pr = p.pres ? p.pres[b] : p.pres1;
   const float inv_r = __fdividef(1.0f, r);
   const int* row = p.tokens + (size_t)b * p.ldt;
-  constexpr int AHEAD = 8;                                              // tokens of the history per thread before its length is known
-  int said[AHEAD];
+  // history: AHEAD groups of four tokens per thread before its length is known, each on a 16-byte boundary (the first up to three tokens in front of the row)
+  constexpr int AHEAD = 2;
+  const int past = (int)(((uintptr_t)row >> 2) & 3);
+  const int limit = history ? p.T : 0;
+  auto group = [&](int i, int end) {
+    if (i >= 0 && i + 4 <= end) return *reinterpret_cast<const int4*>(row + i);
+    int4 a = make_int4(-1, -1, -1, -1);
+    if (i >= end) return a;
+    a.x = i >= 0 && i < end ? row[i] : -1;
+    a.y = i + 1 >= 0 && i + 1 < end ? row[i + 1] : -1;
+    a.z = i + 2 >= 0 && i + 2 < end ? row[i + 2] : -1;
+    a.w = i + 3 < end ? row[i + 3] : -1;                                // (never in front of the row)
+    return a;
+  };
+  int4 said[AHEAD];
 #pragma unroll
-  for (int u = 0; u < AHEAD; ++u) said[u] = history && u * TH + t < p.T ? row[u * TH + t] : -1;
+  for (int u = 0; u < AHEAD; ++u) said[u] = group(4 * (u * TH + t) - past, limit);
   const int* ids = p.bias_ids + (size_t)b * p.ldb;
   const float* bias = p.bias + (size_t)b * p.ldb;
-  const int id0 = t < p.n_bias ? ids[t] : -1;
-  const float bias0 = t < p.n_bias ? bias[t] : 0.f;
+  const int id0 = t < p.n_bias ? ids[t] : -1, id1 = t + TH < p.n_bias ? ids[t + TH] : -1;
+  const float bias0 = t < p.n_bias ? bias[t] : 0.f, bias1 = t + TH < p.n_bias ? bias[t + TH] : 0.f;
   float v[N][4];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
@@ -86,17 +100,16 @@ __global__ void __launch_bounds__(TH, 4) logit_rules_kernel(const RulesParams p)
       for (int e = 0; e < 4; ++e) v[k][e] = i + e >= 0 && i + e < p.V ? (float)x[i + e] : 0.f;
     }
   }
-  unsigned bits[N];
+  unsigned word[N], next[N];                                            // the mask's word with a group's first token, and the one behind it where the group ends there
+  const int words = (p.V + 31) >> 5;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    bits[k] = 0xfu;
-    const int i = lo + 4 * (k * TH + t);
-    if (p.allowed && i + 3 >= 0 && i < p.V) {
-      const unsigned* row = p.allowed + (size_t)b * p.lda;
-      const int w = i >> 5;                                             // (-1 in front of the row)
-      const unsigned a = w >= 0 ? __ldg(row + w) : 0u;
-      const unsigned c = (i & 31) > 28 && (w + 1) * 32 < p.V ? __ldg(row + w + 1) : 0u;
-      bits[k] = __funnelshift_r(a, c, i & 31);
+    const int i = lo + 4 * (k * TH + t), w = i >> 5;                    // (-1 in front of the row)
+    word[k] = next[k] = ~0u;
+    if (p.allowed) {
+      const unsigned* mask = p.allowed + (size_t)b * p.lda;
+      if (w >= 0 && w < words) word[k] = __ldg(mask + w);
+      if (off && (i & 31) > 28 && w + 1 < words) next[k] = __ldg(mask + w + 1);
     }
   }
   __syncthreads();
@@ -110,29 +123,44 @@ __global__ void __launch_bounds__(TH, 4) logit_rules_kernel(const RulesParams p)
         else atomicAdd(&lr_count[at], 1u);
       }
     };
+    auto count4 = [&](int i, int4 a) {                                  // (few groups have a token of the slice)
+      if (min(min((unsigned)(a.x - lo), (unsigned)(a.y - lo)), min((unsigned)(a.z - lo), (unsigned)(a.w - lo))) >= (unsigned)SLICE) return;
+      count(i, a.x); count(i + 1, a.y); count(i + 2, a.z); count(i + 3, a.w);
+    };
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) count(u * TH + t, said[u]);
-    for (int i0 = AHEAD * TH + t; i0 < len; i0 += AHEAD * TH) {         // AHEAD loads in flight
+    for (int u = 0; u < AHEAD; ++u) count4(4 * (u * TH + t) - past, said[u]);
+    for (int i0 = 4 * (AHEAD * TH + t) - past; i0 < len; i0 += 4 * AHEAD * TH) {        // AHEAD loads in flight
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) said[u] = i0 + u * TH < len ? row[i0 + u * TH] : -1;
+      for (int u = 0; u < AHEAD; ++u) said[u] = group(i0 + 4 * u * TH, len);
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) count(i0 + u * TH, said[u]);
+      for (int u = 0; u < AHEAD; ++u) count4(i0 + 4 * u * TH, said[u]);
     }
   }
-  // ---- biases: whoever marks a token first adds them at the end, the others say that there are more
+  // ---- biases: whoever marks a token first leaves the value, the others say that there are more: then it is the sum
   unsigned mine = 0;                                                    // bit k: this thread was first with entry t + k TH
   for (int i = t, k = 0; i < p.n_bias; i += TH, ++k) {
-    const int id = k == 0 ? id0 : ids[i];
+    const int id = k == 0 ? id0 : (k == 1 ? id1 : ids[i]);
     const unsigned at = (unsigned)id - (unsigned)lo;
     if (at < (unsigned)SLICE && id >= 0 && id < p.V) {
       if (atomicOr(&lr_count[at], LR_BIAS) & LR_BIAS) atomicOr(&lr_count[at], LR_MORE);
-      else mine |= 1u << k;
+      else { lr_value[at] = k == 0 ? bias0 : (k == 1 ? bias1 : bias[i]); mine |= 1u << k; }
+    }
+  }
+  if (p.n_bias) {
+    __syncthreads();
+    for (unsigned left = mine; left; left &= left - 1) {
+      const int id = ids[t + (__ffs(left) - 1) * TH];
+      if (!(lr_count[id - lo] & LR_MORE)) continue;
+      float sum = 0.f;
+      for (int j = 0; j < p.n_bias; ++j) if (ids[j] == id) sum += bias[j];
+      lr_value[id - lo] = sum;
     }
   }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int i = lo + 4 * (k * TH + t);
+    const unsigned bits = __funnelshift_r(word[k], next[k], i & 31);
     if (table) {
       const uint4 c4 = reinterpret_cast<const uint4*>(lr_count)[k * TH + t];
       const unsigned c[4] = {c4.x, c4.y, c4.z, c4.w};
@@ -145,12 +173,12 @@ __global__ void __launch_bounds__(TH, 4) logit_rules_kernel(const RulesParams p)
           const float pen = a > 0.f ? (q < INFINITY ? fmaf(fmaf(-q, r, a), inv_r, q) : q) : a * r;
           if (c[e] & (LR_COUNT | LR_SAID)) v[k][e] = pen;
           if (n) v[k][e] = v[k][e] - f * (float)n - pr;
-          if ((c[e] & LR_BIAS) && !((bits[k] >> e) & 1u)) lr_count[4 * (k * TH + t) + e] = 0;       // masked: no bias is added
+          if (c[e] & LR_BIAS) v[k][e] += lr_value[4 * (k * TH + t) + e];
         }
       }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) if (!((bits[k] >> e) & 1u)) v[k][e] = -INFINITY;
+    for (int e = 0; e < 4; ++e) if (!((bits >> e) & 1u)) v[k][e] = -INFINITY;
     if (wide && i >= 0 && i + 4 <= p.V) {
       *reinterpret_cast<float4*>(y + i) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
     } else {
@@ -158,38 +186,26 @@ __global__ void __launch_bounds__(TH, 4) logit_rules_kernel(const RulesParams p)
       for (int e = 0; e < 4; ++e) if (i + e >= 0 && i + e < p.V) y[i + e] = v[k][e];
     }
   }
-  if (!p.n_bias || !__syncthreads_or(mine)) return;                     // the slice is written
-  for (int k = 0; k < 32 && mine >> k; ++k) {
-    if (!((mine >> k) & 1u)) continue;
-    const int i = t + k * TH, id = k == 0 ? id0 : ids[i];
-    const unsigned c = lr_count[id - lo];
-    if (!(c & LR_BIAS)) continue;                                       // masked
-    float v0 = y[id];
-    if (c & LR_MORE) {
-      float sum = 0.f;
-      for (int j = 0; j < p.n_bias; ++j) if (ids[j] == id) sum += bias[j];
-      v0 += sum;
-    } else {
-      v0 += k == 0 ? bias0 : bias[i];
-    }
-    y[id] = v0;
-  }
 }
 
 template <typename T, int TH, int N>
 static cudaError_t lr_launch(const RulesParams& p, int B, cudaStream_t st) {
   constexpr int SLICE = 4 * N * TH;
-  const size_t smem = p.tokens || p.n_bias ? (size_t)SLICE * 4 : 0;
+  const size_t smem = (size_t)SLICE * 4 * (p.n_bias ? 2 : (p.tokens ? 1 : 0));
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(logit_rules_kernel<T, TH, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
   return launch_pdl(logit_rules_kernel<T, TH, N>, dim3((p.V + 3 + SLICE - 1) / SLICE, B), dim3(TH), smem, st, p);
 }
 template <typename T>
 static cudaError_t lr_dispatch(const RulesParams& p, int B, cudaStream_t st) {
-  // Few rows: the smallest slices, for more SMs; many: the largest that keep four CTAs per SM, because every slice's CTA walks the row's whole history.  us in a graph,
-  // 1, 2, 4 groups per thread: 1 x 32000 2.0, 2.8, 3.2; 17 x 128259 8.9, 6.9, 5.5; 96 x 128256 50, 47, 40.  (512 threads with 4: 4.3, 9.1, 41.)
+  // Few rows: the smallest slices, for more SMs; many: large ones, because every slice's CTA walks the row's whole history.  us in a graph on one B200, 17 x 128259
+  // with 2049 tokens of history and 96 x 128256 with 4000: four groups for each of 128, 256, 512 threads 6.0, 5.8, 5.4 and 38, 32, 30; two for 512 7.4 and 40.
   const long groups = ((long)p.V + 3) / 4 * B / 256;                   // CTAs of 256 threads with one group each
   if (groups <= 2 * 148) return lr_launch<T, 256, 1>(p, B, st);
   if (groups <= 6 * 148) return lr_launch<T, 256, 2>(p, B, st);
-  return lr_launch<T, 256, 4>(p, B, st);
+  return lr_launch<T, 512, 4>(p, B, st);
 }
 
 }  // namespace jl

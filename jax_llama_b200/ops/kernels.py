@@ -568,6 +568,18 @@ def _coefficient(v: Union[float, torch.Tensor, None], off: float, B: int, dev: i
     return None, float(v)
 
 
+def _same_or_apart(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether y [B, V] is x, or has no byte of x: rows beside one another of one buffer are apart."""
+    a, b, (B, V), n, m = x.data_ptr(), y.data_ptr(), x.shape, x.element_size(), y.element_size()
+    p, q = (x.stride(0) * n, y.stride(0) * m) if B > 1 else (V * n, V * m)
+    if a + (B - 1) * p + V * n <= b or b + (B - 1) * q + V * m <= a or B * V == 0:
+        return True
+    if p != q:
+        return False
+    gap = (b - a) % p
+    return (a == b and x.dtype is y.dtype) or (gap >= V * n and p - gap >= V * m)
+
+
 def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
                      prompt_lengths: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None, repetition: Union[float, torch.Tensor, None] = None,
                      frequency: Union[float, torch.Tensor, None] = None, presence: Union[float, torch.Tensor, None] = None,
@@ -579,7 +591,8 @@ def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = N
     all of it) as its answer.  Ids outside the vocabulary are passed over.  For a token that occurs: x > 0 ? x / repetition : x · repetition; with n occurrences in
     the answer, n > 0: x - frequency · n - presence.  (A number, or fp32 [B]; None: off.  repetition > 0.)  Then x + bias_values of the entries of bias_ids
     (int32 / fp32 [B, n], or [1, n] for all rows, n <= 8192; an id outside the vocabulary is no entry, the same id twice adds both), then -inf where bit v % 32 of word v // 32
-    of allowed (int32 [B, words] or [1, words]) is zero.  A row whose mask allows nothing is -inf throughout.  `out` may be `logits` itself when that is fp32."""
+    of allowed (int32 [B, words] or [1, words]) is zero.  A row whose mask allows nothing is -inf throughout.  `out` may be `logits` itself when that is fp32; any
+    other overlap is refused."""
     who = "constrain_logits"
     kind = _LOGIT_TYPES.get(logits.dtype)
     B, V = logits.shape if logits.dim() == 2 else (-1, -1)
@@ -625,6 +638,8 @@ def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = N
         lda = shape[1] if shape[0] > 1 else 0
     if out is not None and (out.dtype is not _F32 or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or out.get_device() != dev):
         raise ValueError(f"{who}: out is fp32 {tuple(logits.shape)} with dense rows on {logits.device} (got {out.dtype}, {tuple(out.shape)}, {out.device})")
+    if out is not None and out is not logits and not _same_or_apart(logits, out):
+        raise ValueError(f"{who}: out overlaps logits that it is not the same as")
     if dev < 0:
         def full(t: Optional[torch.Tensor], off: Union[int, float]) -> torch.Tensor:
             return torch.full((B,), off) if t is None else t.reshape(-1).expand(B)

@@ -104,3 +104,63 @@ def test_refusals():
     for logits in (torch.zeros(40), torch.zeros(2, 40, dtype=torch.float64), torch.zeros(40, 2).t()):
         with pytest.raises(ValueError):
             K.constrain_logits(logits)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_out_may_be_the_logits_or_apart(dev):
+    buf = torch.randn(3, 100, generator=torch.Generator().manual_seed(1)).to(dev)
+    want = buf[:, :40] - 0.0
+    for bad in (buf[:, 1:41], buf[:, 39:79], buf[:, 20:60]):
+        with pytest.raises(ValueError):
+            K.constrain_logits(buf[:, :40], out=bad)
+    half = buf.view(-1).view(torch.bfloat16)[:120].view(3, 40)
+    with pytest.raises(ValueError):
+        K.constrain_logits(half, out=buf.view(-1)[:120].view(3, 40))
+    assert torch.equal(K.constrain_logits(buf[:, :40], out=buf[:, 40:80]), want) and torch.equal(buf[:, 40:80], want)
+    assert torch.equal(K.constrain_logits(buf[:, :40], out=buf[:, :40]), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,V,T,dtype,n_bias,seed", [(8, 128000, 5001, torch.float32, 1200, 0), (9, 128259, 4100, torch.bfloat16, 0, 1), (4, 100003, 2500, torch.bfloat16, 600, 2),
+                                                     (3, 40001, 1030, torch.float16, 300, 3), (1, 3001, 9, torch.float32, 8192, 4)])
+def test_long_histories_and_many_biases(B, V, T, dtype, n_bias, seed):
+    """Every width of slice, history and entries beyond what is asked for ahead, rows of tokens at any 4-byte boundary."""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(B, V, generator=g) * 4).to(dtype)
+    tokens = (torch.rand(B, T + 4, generator=g) ** 2 * V).to(torch.int32).clamp(max=V - 1)[:, 1:T + 1]
+    rnd = lambda lo, hi: torch.randint(lo, hi + 1, (B,), generator=g, dtype=torch.int32)
+    starts, lengths, prompts = rnd(0, 50), rnd(T - 9, T), rnd(0, T)
+    rep, freq, pres = 0.7 + torch.rand(B, generator=g), torch.randn(B, generator=g), torch.randn(B, generator=g)
+    ids = torch.randint(0, V, (B, n_bias), generator=g, dtype=torch.int32)
+    if n_bias:
+        ids[:, 5:n_bias:n_bias // 20] = ids[:, :1]                           # an id up to 23 times, from every round of entries
+    bias = torch.randn(B, n_bias, generator=g)
+    allowed = mask_of(1, V, 0.9, g)
+    wanted = [oracle.rules(x[b:b + 1], tokens[b:b + 1], [int(starts[b])], [int(lengths[b])], [int(prompts[b])], [float(rep[b])], [float(freq[b])], [float(pres[b])],
+                           ids[b:b + 1], bias[b:b + 1]) for b in range(B)]
+    want = torch.cat(wanted)
+    bits = (allowed.long()[:, torch.arange(V) // 32] >> (torch.arange(V) % 32)) & 1
+    want = want.masked_fill(bits == 0, -math.inf)
+    scale = x.double().abs() * 2 + (T * 4.0 + 4) * freq.abs().max() + pres.abs().max() + 5.0 * bias.abs().sum(1, keepdim=True)
+    d = lambda t: t.to("cuda")
+    buf = torch.full((B, T + 6), 7, dtype=torch.int32, device="cuda")
+    buf[:, 1:T + 1] = d(tokens)
+    got = K.constrain_logits(d(x), tokens=buf[:, 1:T + 1], starts=d(starts), lengths=d(lengths), prompt_lengths=d(prompts), repetition=d(rep), frequency=d(freq),
+                             presence=d(pres), bias_ids=d(ids) if n_bias else None, bias_values=d(bias) if n_bias else None, allowed=d(allowed))
+    close(got, want, x, scale)
+
+
+@pytest.mark.gpu
+def test_a_captured_call_follows_the_text():
+    """The history is read at replay: tokens and lengths that changed in between count."""
+    x, tokens, n = torch.randn(2, 900, device="cuda"), torch.zeros(2, 30, dtype=torch.int32, device="cuda"), torch.tensor([0], dtype=torch.int32, device="cuda")
+    out, g = torch.empty_like(x), torch.cuda.CUDAGraph()
+    kw = dict(tokens=tokens, lengths=n, repetition=1.5, frequency=0.25)
+    with torch.cuda.graph(g):
+        K.constrain_logits(x, out=out, **kw)
+    for k in (0, 3, 30):
+        tokens.copy_(torch.randint(0, 900, (2, 30), generator=torch.Generator().manual_seed(k)))
+        n.fill_(k)
+        g.replay()
+        assert torch.equal(out, K.constrain_logits(x, **kw))
+        assert (out != x).any().item() == (k > 0)
