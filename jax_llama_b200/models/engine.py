@@ -874,11 +874,21 @@ class B200Engine:
         self.last_stats = stats
         return st.sequences.to(torch.long)
 
-    def _shares(self, rows: int, groups: int) -> bool:
-        """Whether `rows` rows behind `groups` shared prefixes take the attention over shared keys (head sizes and groups that it is built for)."""
-        return self.shares_prefixes and self.hd in (64, 128) and self.nh // self.nkv in (1, 2, 4, 8) and rows > groups
-
+    # Own copies of shared keys, in bytes that a step of a layer reads for them, from which on they are held once for all rows; with the whole-step kernel for up to
+    # four rows, which reads own keys alone.  ms a token behind one prompt on one B200, keys of copies -> together: 8 layers 4096 wide (8 key heads of 128), 16 answers to
+    # 128 tokens (8 MB) 0.78 -> 0.83, to 1024 (63 MB) 1.16 -> 0.86; 4 answers by the whole-step kernel to 1024 (13 MB) 0.84 -> 1.24, to 4096 (50 MB) 1.14 -> 1.22; 8 layers
+    # 2048 wide (4 of 64), 8 answers to 1024 (7 MB) 0.377 -> 0.387, to 4096 (29 MB) 0.424 -> 0.411, 16 to 1024 (16 MB) 0.393 -> 0.406, to 4096 (63 MB) 0.492 -> 0.432.
+    share_above, share_above_whole_step = 20 << 20, 56 << 20
     shares_prefixes = True                       # engines whose layers hold anything else per row say no
+
+    def _together(self, rows: int, groups: int, P: int) -> bool:
+        """Whether `rows` rows behind `groups` prefixes of P tokens take the attention over shared keys, not copies of them."""
+        whole_step = rows <= 4 and self._mega_fits(rows)
+        copies = (rows - groups) * P * self.nkv * self.hd * 4
+        return self._shared_attention() and copies >= (self.share_above_whole_step if whole_step else self.share_above)
+
+    def _shared_attention(self) -> bool:
+        return self.hd in (64, 128) and self.nh // self.nkv in (1, 2, 4, 8)
 
     def _begin(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], max_length: int, pad: int, rules: Optional[LogitRules], repeat: int,
                prefix_ids: Optional[torch.Tensor], prefix_mask: Optional[torch.Tensor], logit_rows: Optional[torch.Tensor] = None
@@ -905,36 +915,48 @@ class B200Engine:
             raise ValueError(f"max_length {max_length} is shorter than the prompt ({total})")
         # (a prompt without a token of its own ends with its prefix: its answer begins at the prefix's last position, not behind padding)
         empty = S == 0 or (prefix_ids is not None and attention_mask is not None and bool((attention_mask[:, S - 1] == 0).any()))
-        if P == 0 or empty or not self._shares(B, groups):
+        # copies need prompts without padding between them and their prefix
+        dense = prefix_ids is None or attention_mask is None or bool((attention_mask != 0).all())
+        if P == 0 or empty or not self.shares_prefixes or B == groups or not (dense or self._shared_attention()):
             ids, mask = (input_ids, attention_mask) if prefix_ids is None else join_prefix(prefix_ids, input_ids, prefix_mask, attention_mask, pad)
             st = self._decode_state(B, max_length)
             cache = self.prepare(st, ids.repeat_interleave(repeat, 0), None if mask is None else mask.repeat_interleave(repeat, 0), pad)
         else:
-            st = self._decode_state(B, max_length, (int(groups), int(P)))
-            cache = self._prepare_shared(st, input_ids, attention_mask, pad, repeat, prefix_ids, prefix_mask)
+            together = not dense or self._together(B, groups, P)
+            st = self._decode_state(B, max_length, (int(groups), int(P)) if together else ())
+            cache = self._prepare_shared(st, input_ids, attention_mask, pad, repeat, prefix_ids, prefix_mask, together)
         self._set_rules(st, rules, total, rows, repeat)
         return st, cache, total
 
     def _prepare_shared(self, st: DecodeState, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], pad: int, repeat: int,
-                        prefix_ids: Optional[torch.Tensor], prefix_mask: Optional[torch.Tensor]) -> DeviceKVCache:
-        """`prepare` for rows that share keys: the prefixes' prefill into a cache of their own, then the prompts' (when they are not the prefixes
-        themselves) behind it."""
+                        prefix_ids: Optional[torch.Tensor], prefix_mask: Optional[torch.Tensor], together: bool) -> DeviceKVCache:
+        """`prepare` for rows that share keys: the prefixes' prefill into a cache of their own, which the rows' caches refer to or (not `together`) get copies of, then
+        the prompts' (when they are not the prefixes themselves) behind it."""
         rows, S = input_ids.shape
         whole = prefix_ids is None                                             # several answers: the prompts are what is shared
         front, front_mask = (input_ids, attention_mask) if whole else (prefix_ids, prefix_mask)
         groups, P = front.shape
         front_cache, cache = getattr(st, "_front_cache", None), getattr(st, "_cache", None)
+        if front_cache is None or front_cache.k.shape[1] != groups or front_cache.k.shape[3] != P:
+            front_cache = st._front_cache = self.new_cache(groups, P)
         if cache is None:
-            front_cache, cache = self.new_cache(groups, P), self.new_cache(st.B, max(st.max_len - P, 1))
-            cache.prefix = SharedPrefix(front_cache.k, front_cache.v, torch.full((groups,), P, dtype=torch.int32, device=self.device), front_cache.pad_left,
-                                        K.prefix_attn_scratch(st.B, 1, groups, self.nh, self.nkv, self.hd, P, self.device))
-            st._front_cache, st._cache = front_cache, cache
-            st.seq_pad = torch.zeros(st.B, dtype=torch.int32, device=self.device)
+            cache = st._cache = self.new_cache(st.B, max(st.max_len - P, 1) if together else st.max_len)
+            if together:
+                cache.prefix = SharedPrefix(front_cache.k, front_cache.v, torch.full((groups,), P, dtype=torch.int32, device=self.device), front_cache.pad_left,
+                                            K.prefix_attn_scratch(st.B, 1, groups, self.nh, self.nkv, self.hd, P, self.device))
+                st.seq_pad = torch.zeros(st.B, dtype=torch.int32, device=self.device)
+        st.rules = None
         front_cache.set_index(0)
-        cache.set_index(0)
         out = self.forward(front, attention_mask=front_mask, cache=front_cache, last_only=True, gather_logits=False)
         ids, mask = front, front_mask
-        cache.pad_left.zero_()
+        if together:
+            cache.set_index(0)
+            cache.pad_left.zero_()
+        else:
+            for own, shared in ((cache.k, front_cache.k), (cache.v, front_cache.v)):
+                own.unflatten(1, (groups, -1))[..., :P, :].copy_(shared[:, :, None])
+            cache.pad_left.copy_(front_cache.pad_left.repeat_interleave(st.B // groups))
+            cache.set_index(P)
         if not whole:
             ids, mask = join_prefix(front, input_ids, front_mask, attention_mask, pad)
             if repeat > 1:
@@ -945,7 +967,8 @@ class B200Engine:
         times = st.B // ids.shape[0]
         st.sequences.fill_(int(pad))
         st.sequences[:, :total] = ids.to(torch.int32).repeat_interleave(times, 0)
-        st.seq_pad.copy_(self.pad_left_from_mask(mask, ids.shape[0], total, self.device).repeat_interleave(times, 0))
+        if together:
+            st.seq_pad.copy_(self.pad_left_from_mask(mask, ids.shape[0], total, self.device).repeat_interleave(times, 0))
         st.finished.zero_()
         st.cur_len.fill_(total)
         st.step.zero_()

@@ -23,7 +23,13 @@ CFGS = {
 def make(name, **kw):
     cfg = CFGS[name]
     tree = tree_to(ref.init_params(cfg, seed=1), dtype=torch.bfloat16)
-    return cfg, tree_to(tree, dtype=torch.float32), B200Engine.from_tree(cfg, tree_to(tree, device="cuda"), **kw)
+    eng = B200Engine.from_tree(cfg, tree_to(tree, device="cuda"), **kw)
+    eng.share_above = eng.share_above_whole_step = 0         # keys held once however few they are
+    return cfg, tree_to(tree, dtype=torch.float32), eng
+
+
+def eng_tree(cfg):
+    return tree_to(ref.init_params(cfg, seed=1), dtype=torch.bfloat16, device="cuda")
 
 
 def rel(a, b):
@@ -41,15 +47,16 @@ def padded(pads, n):
 
 @pytest.mark.parametrize("name", list(CFGS))
 @pytest.mark.parametrize("graph", [True, False])
-@pytest.mark.parametrize("groups,rows,repeat,P,S", [(1, 3, 1, 70, 9), (2, 4, 3, 33, 5), (1, 1, 6, 40, 0), (3, 3, 2, 65, 0)])
-def test_logits_behind_a_prefix_match_the_written_out_rows(name, graph, groups, rows, repeat, P, S):
+@pytest.mark.parametrize("groups,rows,repeat,P,S,together", [(1, 3, 1, 70, 9, True), (2, 4, 3, 33, 5, True), (1, 1, 6, 40, 0, True), (3, 3, 2, 65, 0, True),
+                                                             (1, 3, 1, 70, 9, False), (2, 4, 3, 33, 5, False), (1, 1, 6, 40, 0, False), (3, 3, 1, 20, 7, False)])
+def test_logits_behind_a_prefix_match_the_written_out_rows(name, graph, groups, rows, repeat, P, S, together):
     """Prefix prefill, prompts behind it, steps: the logits of every fed token against the fp32 model on the joined rows (bf16 weights and activations on one
     side: the 3e-2 of the other engine tests).  S = 0: several answers to the prompts themselves."""
     cfg, tree32, eng = make(name, use_cuda_graph=graph)
     front, fpads = ids_of(groups, P, 1), [(3 * g) % 5 for g in range(groups)]
     fmask = padded(fpads, P)
     if S:
-        ids, mask = ids_of(rows, S, 2), padded([(2 * b) % S for b in range(rows)], S)
+        ids, mask = ids_of(rows, S, 2), padded([(2 * b) % S if together else 0 for b in range(rows)], S)
         joined, jmask = join_prefix(front, ids, fmask, mask, 0)
         kw = dict(prefix_ids=front.cuda(), prefix_mask=fmask.cuda())
     else:
@@ -57,9 +64,12 @@ def test_logits_behind_a_prefix_match_the_written_out_rows(name, graph, groups, 
     full, fullm = joined.repeat_interleave(repeat, 0), jmask.repeat_interleave(repeat, 0)
     B, total = full.shape
     feed = ids_of(B, 4, 3)
+    if not together:
+        eng.mega_write_logits = True
+        eng.share_above = eng.share_above_whole_step = 1 << 40
     for _ in range(2):                                       # the second time on the same caches and captured step
         stream = eng.begin_stream(ids.cuda(), mask.cuda(), max_length=total + 6, num_return_sequences=repeat, pad_token_id=0, **kw)
-        assert stream.cache.prefix is not None and stream.st.B == B
+        assert (stream.cache.prefix is not None) == together and stream.st.B == B
         seen = [stream.logits().clone()]
         for t in range(4):
             stream.step(feed[:, t].to(torch.int32).pin_memory())
@@ -76,6 +86,7 @@ def test_logits_behind_a_prefix_match_the_written_out_rows(name, graph, groups, 
 def test_greedy_behind_a_prefix_agrees_with_the_model():
     """Every token that generate() takes is the fp32 model's best one, or within the engine's rounding of it."""
     cfg, tree32, eng = make("gqa128")
+    assert eng._together(5, 1, 1) and not B200Engine.from_tree(cfg, eng_tree(cfg))._together(5, 1, 1)
     front, ids = ids_of(1, 50, 5), ids_of(6, 7, 6)
     seqs = eng.generate(ids.cuda(), None, max_length=50 + 7 + 12, prefix_ids=front.cuda(), eos_token_id=-1).cpu()
     assert torch.equal(seqs[:, :57], torch.cat([front.expand(6, 50), ids], 1))
@@ -193,3 +204,15 @@ def test_text_front_end_on_the_gpu(spm_model):
     tokens, mask, _ = gen.encode_prompts(["hello"])
     h = gen.stream(tokens, mask, 8, temperature=0.0, num_return_sequences=2, rules=LogitRules(logit_bias={5: 1e4}))
     assert h.last_tokens().tolist() == [5, 5] and h.step().tolist() == [5, 5]
+
+
+def test_copies_of_another_length_take_their_own_keys():
+    """The same captured step and caches serve prompts of other lengths and counts, with and without copies."""
+    cfg, tree32, eng = make("gqa128")
+    eng.share_above = eng.share_above_whole_step = 1 << 40
+    for rows, n, seed in ((1, 40, 1), (2, 23, 2), (4, 31, 3), (1, 40, 4)):
+        ids = ids_of(rows, n, seed)
+        got = eng.generate(ids.cuda(), None, max_length=60, num_return_sequences=4 // rows, eos_token_id=-1).cpu()
+        logits = ref.forward(tree32, cfg, got).logits[:, n - 1:-1]
+        gap = logits.amax(-1) - logits.gather(-1, got[:, n:, None])[..., 0]
+        assert torch.equal(got[:, :n], ids.repeat_interleave(4 // rows, 0)) and (gap <= 6e-2 * logits.abs().amax()).all()
