@@ -555,7 +555,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
     const int ch = lane % CH;
     if (n_tiles > 0) {
       constexpr int STEPS = (PAIR ? 32 : 16) / RPS, AHEAD = ROTATE ? 4 : 16;           // loads in flight
-      const int row0 = (PAIR ? quarter * 32 : (w * 4 + quarter) * 16) + lane / CH;       // (rows behind the last query: anything, they are never read)
+      const int row0 = (PAIR ? quarter * 32 : (w * 4 + quarter) * 16) + lane / CH;       // (rows behind the last query: zeros; their scores have a say in the way that a warp takes)
 #pragma unroll 1
       for (int i0 = 0; i0 < STEPS; i0 += AHEAD) {
         uint4 x[AHEAD];
@@ -577,8 +577,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
           const int r = row0 + (i0 + u) * RPS;
-          if (i0 + u < STEPS && (PAIR ? w * PX_BM : 0) + r < n_rows) {
+          if (i0 + u < STEPS) {
+            const bool on = (PAIR ? w * PX_BM : 0) + r < n_rows;
             const uint32_t dst = sQ + (PAIR ? w * NQ * Tile::Q : 0) + (ch >> 3) * Tile::Q_HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+            if (!on) x[u] = make_uint4(0, 0, 0, 0);
             if constexpr (ROTATE) {
               const float cs[4] = {c4[u].x, c4[u].y, c4[u].z, c4[u].w}, sn[4] = {s4[u].x, s4[u].y, s4[u].z, s4[u].w};
               const uint32_t v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
@@ -590,7 +592,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
                 a[e] = pack_bf16(y, z_);
                 b[e] = pack_bf16(y - bf16_lo(a[e]), z_ - bf16_hi(a[e]));
               }
-              x[u] = make_uint4(a[0], a[1], a[2], a[3]);
+              if (on) x[u] = make_uint4(a[0], a[1], a[2], a[3]);
+              else b[0] = b[1] = b[2] = b[3] = 0;
               asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + Tile::Q), "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3]) : "memory");
             }
             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(x[u].x), "r"(x[u].y), "r"(x[u].z), "r"(x[u].w) : "memory");
@@ -634,9 +637,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
 #pragma unroll
         for (int e = 0; e < 32; ++e) mx4[e & 3] = max3_nan(mx4[e & 3], __uint_as_float(v0[e]), __uint_as_float(v1[e]));
         const float t = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * p.scale_log2;
-        // (rows behind the last query hold what the memory held before: they have no say in the way that the warp takes)
-        const bool need = row_on && (t > m_ref + PX_RESCALE || (m_ref == -INFINITY && t > -INFINITY));
-        bool odd = row_on && !(t < INFINITY);                                    // NaN or infinite scores show in the result: no shortcuts
+        const bool need = t > m_ref + PX_RESCALE || (m_ref == -INFINITY && t > -INFINITY);
+        bool odd = !(t < INFINITY);                                    // NaN or infinite scores show in the result: no shortcuts
         if (i == 0) m_ref = t;
         if (__any_sync(0xffffffffu, odd || (i > 0 && need))) {
           odd = __any_sync(0xffffffffu, odd);

@@ -123,6 +123,8 @@ def test_prompt(B, groups, nh, nkv, hd, P, start, S, T, ragged):
     pk, pv, kc, vc = dirty(c, start + S)
     got = K.prefill_attn_prefix(q.to(DEV), pk, pv, kc, vc, start, S, i32(c["pad"]) if ragged else None, i32(c["plen"]) if ragged else None,
                                 i32(c["ppad"]) if ragged else None)
+    assert torch.equal(got, K.prefill_attn_prefix(q.to(DEV), pk, pv, kc, vc, start, S, i32(c["pad"]) if ragged else None, i32(c["plen"]) if ragged else None,
+                                                  i32(c["ppad"]) if ragged else None))          # sums in a fixed order
     some = torch.arange(0, S, max(1, S // 24)).tolist() + [S - 1]            # queries that the slow oracle answers
     want, mag = oracle.attention(q[:, some].double(), c["pk"], c["pv"], c["kc"], c["vc"], [start + i for i in some], c["pad"], c["plen"], c["ppad"])
     out = got.cpu().double().view(B, S, nh, hd)
