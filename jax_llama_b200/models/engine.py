@@ -839,8 +839,8 @@ class B200Engine:
 
         `rules`: penalties, biases and allowed tokens of the request.  `num_return_sequences` n: n answers to every prompt, neighbouring rows of the result.
         `prefix_ids` [G, P]: what the prompts have in front of them, B / G neighbouring prompts each; the result's rows begin with it and max_length counts
-        it.  A prompt with several answers, and a prefix, run through the model once and their keys are held and read once (`SharedPrefix`), where the engine's
-        attention knows that form; other engines run the rows as if they had been written out."""
+        it.  A prompt with several answers, and a prefix, run through the model once; their keys are held and read once for all rows (`SharedPrefix`), or copied
+        behind every row's own where they are few.  Engines that cannot share run the rows as if they had been written out."""
         self._check_max_length(max_length)
         from ..utils.stats import CudaTimer, GenerationStats, nvtx_range
         with nvtx_range("prefill"), CudaTimer() as t_prefill:

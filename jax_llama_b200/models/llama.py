@@ -267,7 +267,7 @@ class LLaMAForCausalLM(LLaMAPreTrainedModel):
         `rules` (`LogitRules`): penalties for tokens that occurred, biases, allowed tokens, ahead of the sampling.  `num_return_sequences` n: n answers to every
         prompt, neighbouring rows of the result.  `prefix_ids` [G, P] (and `prefix_mask`, left-padded): what the prompts, B / G neighbours each, have
         in front of them, a system prompt or a document; the result's rows begin with it, `max_length` counts it.  On the GPU the prefix, or a prompt with
-        several answers, runs through the model once, and its keys are held once and read once per token for all its rows.
+        several answers, runs through the model once, and its keys, where they are many, are held once and read once per token for all its rows.
         """
         if generation_config is not None:
             g = generation_config

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from numbers import Integral
 from typing import Any, Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -91,7 +92,7 @@ class LogitRules:
             m = a.view(-1, words)
         else:
             a = list(a)
-            nested = len(a) > 0 and not isinstance(a[0], int)
+            nested = len(a) > 0 and not isinstance(a[0], Integral)
             if nested and len(a) != rows:
                 raise ValueError(f"allowed_tokens: token ids, or one list of them per row ({rows}), got {len(a)} lists")
             m = torch.stack([allowed_mask(r if r is not None else range(vocab_size), vocab_size) for r in (a if nested else [a])])

@@ -35,6 +35,8 @@ def test_bind_lays_out_rows_and_answers():
     same = LogitRules(logit_bias={9: 1.0}, allowed_tokens=allowed_mask([1, 2], 40)).bind(3, 40, "cpu")
     assert one.structure() == same.structure() and one.copy_(same).bias_ids.tolist() == [[9]] and one.allowed[0, 0] == 6
     assert isinstance(one, BoundRules)
+    some = torch.tensor([1, 2]).numpy()                                      # ids of any whole type
+    assert LogitRules(allowed_tokens=list(some)).bind(3, 40, "cpu").allowed[0, 0] == 6 and LogitRules(allowed_tokens=some).bind(3, 40, "cpu").allowed[0, 0] == 6
 
 
 @pytest.mark.parametrize("kw", [dict(repetition_penalty=0.0), dict(repetition_penalty=math.inf), dict(repetition_penalty=[1.0, 1.0, 1.0]), dict(frequency_penalty=math.nan),
