@@ -8,9 +8,12 @@
 //
 // A CTA owns a slice of one row's vocabulary and keeps one word per token of the slice in shared memory: occurrences behind the prompt in the low bits, and bits
 // for "occurred", "has a bias", "has several" (whole numbers and bits: the order of the atomics does not show).  Everything it reads is asked for at once, the slice's
-// logits, the row's bounds, the first tokens of its history, its first biases: a CTA's way is a chain of memory latencies, and a batch of 96 rows is seven rounds of
-// CTAs.  A second table has the bias of a token; where there are several, the thread that was first to mark it goes through all of them in their order.  No state
-// is kept between calls: the history is the sequence buffer that the decode loop writes anyway, so forks, restarts and replayed graphs need nothing.
+// logits, the row's bounds, the first tokens of its history, its first biases: a CTA's way is a chain of memory latencies.  A second table has the bias of a
+// token; where there are several, the thread that was first to mark it goes through all of them in their order.  No state is kept between calls: the history is the
+// sequence buffer that the decode loop writes anyway, so forks, restarts and replayed graphs need nothing.
+//
+// One B200, us in a graph: 96 x 128256 with 4000 tokens, 300 biases and masks 30 (3.4 TB/s; logits alone 16, the history 8, the biases 4), bound by the instructions
+// issued, 69 % of the slots, some 50 a token; 17 x 128259 5.4, 1 x 32000 2.1, a launch and a chain of loads.
 #include "common.cuh"
 #include "jllama_b200.h"
 

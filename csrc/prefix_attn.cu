@@ -16,9 +16,16 @@
 // scores in registers, exponentials in base 2 against a reference that is raised only when it has grown by 2^8.
 // Queries go to shared memory by hand: rows of different tokens and heads follow each other in a tile, and the one-token form rotates them on the way.
 // A rotated query is kept as two bfloat16 numbers, hi + lo (two products into the same scores): rounded to one, a score of size s would be off by
-// s 2^-9 and the result by as much again as its own rounding.  Probabilities are rounded to bfloat16 (2^-9 of each weight, sums in fp32).
+// s 2^-8 and the result by as much again as its own rounding.  Probabilities are rounded to bfloat16 (2^-8 of each weight, sums in fp32) where a launch has
+// more than one tile of queries; with one tile, where the products have time to spare, they are hi + lo too.
 // Slots that hold no key may hold anything: their scores are masked, and their value rows are cleared in shared memory, because a weight of zero
 // times a NaN is a NaN.
+//
+// One B200, us a call in a graph: one token, 16 rows x 32 heads over 8 of keys, 2048 shared 13; 96 rows, 32768 shared and 500 own each 106 (790 TFLOP/s with the
+// second products of the queries, 3.1 TB/s beside them); 4 x 16 rows, 3501 shared and 701 own 45 (5.4 TB/s).  Prompts: 2 x 2048 tokens over 16384 1065 (1080 TFLOP/s; a
+// single launch of its own 906 and 1290: the power cap), 8 x 333 over 1500 68 (1110), 16 x 48 over 8192 111 (920).  What bounds them: products of small width
+// (a 128 x 64 tile of scores reads its queries from shared memory, 384 cycles for 256 of products) and the exponentials, half of the special-function
+// unit's rate with a quarter of them on the FMA units; in short calls the chain launch, queries, scores, last rows, join.
 #include <atomic>
 
 #include "jllama_b200.h"
@@ -67,7 +74,7 @@ __device__ __forceinline__ F2 f2_add(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %
 __device__ __forceinline__ float max3_nan(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 
 // 2^a, 2^b without the special-function unit: x = n + f with n the nearest whole number (added to 1.5 2^23 it stands in the last bits of the sum), 2^f on
-// [-1/2, 1/2] by the cubic of least relative error among those with p(0) = 1 (1.0e-4; what it stands in for is rounded to 2^-9), n added to the exponent.  From
+// [-1/2, 1/2] by the cubic of least relative error among those with p(0) = 1 (1.0e-4; what it stands in for is rounded by up to 2^-8), n added to the exponent.  From
 // -127 down the result is 0 (p = 1 there, and its exponent 127); a, b below 2^22 and not NaN.
 __device__ __forceinline__ void exp2_pair(F2 x, float& a, float& b) {
   f2_get(x, a, b);
