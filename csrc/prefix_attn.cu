@@ -102,7 +102,7 @@ struct PxParams {
   int S, rows, nh, nkv, gs, P, T, start;      // gs: log2 of the query heads per key head
   int shared, own, partial;         // which keys this launch visits; whether it leaves partial triples or the result
   int splits, parts, part0;         // splits of the shared keys in this launch; triples per (token, head), the first that this launch writes
-  // ROTATE: the CTAs in front take the own keys, `own_splits` parts of every (row, key head)
+  // the last `own_ctas` CTAs of a step, or a launch of their own, take the own keys, `own_splits` parts of every (token, key head)
   const __nv_bfloat16* qkv; __nv_bfloat16* k_cache; __nv_bfloat16* v_cache;
   int own_ctas, own_splits, B, tiles_q;
   int p_low;                        // one tile of queries: probabilities as two bfloat16 numbers
@@ -120,12 +120,12 @@ __device__ __forceinline__ void px_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
-// The own keys of a step.  A warp takes units, a part of the keys of one (row, key head), one after the other; its ring holds the next blocks of the same or the
+// The own keys of a step (ROTATE), or of prompts of a few tokens, whose tiles would be all but empty.  A warp takes units, a part of the keys of one (token, key head), one after the other; its ring holds the next blocks of the same or the
 // following unit.  As in decode_attn_fused.cu the G query heads are rows 0..G-1 of mma.sync operands of 16 rows, which leaves rows 8..15 for the low parts
-// of the queries (scores) and of the probabilities (values): both keep 16 bits at no cost.  The new token of a unit's row, in the last part, is folded in from
-// registers.  Bound by the cache's bytes; a block's chain of dependent steps takes about 0.6 us, so that a warp moves 13 GB/s and eight of them an SM's share
+// of the queries (scores) and of the probabilities (values): both keep 16 bits at no cost.  The new token of a step's row, in the last part, is folded in from
+// registers; a prompt's tokens are in the cache.  Bound by the cache's bytes; a block's chain of dependent steps takes about 0.6 us, so that a warp moves 13 GB/s and eight of them an SM's share
 // of the bandwidth twice over.
-template <int HD>
+template <int HD, bool ROTATE>
 __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
   using Own = PxOwn<HD>;
   constexpr int KPI = Own::KPI, HALVES = Own::HALVES, STAGES = Own::STAGES;
@@ -138,19 +138,21 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
   for (int i = lane; i < (int)Own::QT / 16; i += 32)                  // rows without a head stay zero
     asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(qt + 16 * i), "r"(0) : "memory");
   __syncwarp();
-  pdl_wait();
+  if constexpr (ROTATE) pdl_wait();
   pdl_launch_dependents();
 
-  const int G = 1 << p.gs, units = p.B * p.nkv * p.own_splits, step = p.own_ctas * Own::WARPS;
-  const int len = min(max(*p.cache_len, 0), p.T);                // keys in front of the new token
+  const int G = 1 << p.gs, units = p.B * p.S * p.nkv * p.own_splits, step = p.own_ctas * Own::WARPS;
+  const int len = ROTATE ? min(max(*p.cache_len, 0), p.T) : 0;           // a step: keys in front of the new token
   // first and last + 1 key of unit u
   auto range = [&](int u, int& lo, int& hi) {
-    const int item = u / p.own_splits, part = u - item * p.own_splits, b = item / p.nkv;
-    const int first = p.pad_left ? max(p.pad_left[b], 0) : 0, valid = max(len - first, 0);
+    const int item = u / p.own_splits, part = u - item * p.own_splits, token = item / p.nkv, b = ROTATE ? token : token / p.S;
+    const int first = p.pad_left ? max(p.pad_left[b], 0) : 0, valid = max((ROTATE ? len : p.start + token - b * p.S + 1) - first, 0);
     const int chunk = ((valid + p.own_splits - 1) / p.own_splits + KPI - 1) / KPI * KPI;
     lo = first + min(part * chunk, valid);
     hi = first + min((part + 1) * chunk, valid);
   };
+  // (row, key head) of unit u in the caches
+  auto cache_row = [&](int u) { const int item = u / p.own_splits; return ROTATE ? item : item / p.nkv / p.S * p.nkv + item % p.nkv; };
   // what is asked for next: block [r_base, r_base + KPI) of unit r_u
   const int first_unit = ((int)blockIdx.x - ((int)gridDim.x - p.own_ctas)) * Own::WARPS + warp;
   int r_u = first_unit, r_base = 0, r_hi = 0, r_st = 0;
@@ -165,7 +167,7 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
     }
     if (r_u < units) {
       const uint32_t dst = ring + r_st * Own::STAGE + (r_ch >> 3) * Own::BOX;
-      const size_t src = ((size_t)(r_u / p.own_splits) * p.T + r_base + r_key) * HD + 8 * r_ch;
+      const size_t src = ((size_t)cache_row(r_u) * p.T + r_base + r_key) * HD + 8 * r_ch;
 #pragma unroll
       for (int i = 0; i < KPI / RPS; ++i) {
         const int key = i * RPS + r_key;
@@ -196,28 +198,32 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
   for (int u = first_unit; u < units; u += step) {
     int lo, hi;
     range(u, lo, hi);
-    const int item = u / p.own_splits, part = u - item * p.own_splits, b = item / p.nkv, kvh = item - b * p.nkv;
-    const int group = b / p.rows;
-    const int g_lo = p.prefix_pad ? max(p.prefix_pad[group], 0) : 0, g_hi = p.prefix_len ? min(p.prefix_len[group], p.P) : p.P;
-    const __nv_bfloat16* row = p.qkv + (size_t)b * (p.nh + 2 * p.nkv) * HD;
-    const bool newest = part == p.own_splits - 1;
-    // ---- the new token: chunk `ch` of query rows pass · RPS + lane / CH, and of its key and value
+    const int item = u / p.own_splits, part = u - item * p.own_splits, b = item / p.nkv, kvh = item - b * p.nkv;      // (b: the token)
+    const __nv_bfloat16* row = p.q + (size_t)b * p.ldq;
+    const bool newest = ROTATE && part == p.own_splits - 1;
+    // ---- queries: chunk `ch` of rows pass · RPS + lane / CH; and of the new token's key and value
     const int ch = lane % CH, rr = lane / CH;
     uint4 qx[PASSES], kx = make_uint4(0, 0, 0, 0), vx = kx;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i)
       if (i * RPS + rr < G) qx[i] = *reinterpret_cast<const uint4*>(row + (size_t)(kvh * G + i * RPS + rr) * HD + 8 * ch);
-    if (newest) {
-      kx = *reinterpret_cast<const uint4*>(row + (size_t)(p.nh + kvh) * HD + 8 * ch);
-      vx = *reinterpret_cast<const uint4*>(row + (size_t)(p.nh + p.nkv + kvh) * HD + 8 * ch);
+    float cs[4], sn[4];
+    if constexpr (ROTATE) {
+      const int group = b / p.rows;
+      const int g_lo = p.prefix_pad ? max(p.prefix_pad[group], 0) : 0, g_hi = p.prefix_len ? min(p.prefix_len[group], p.P) : p.P;
+      if (newest) {
+        kx = *reinterpret_cast<const uint4*>(row + (size_t)(p.nh + kvh) * HD + 8 * ch);
+        vx = *reinterpret_cast<const uint4*>(row + (size_t)(p.nh + p.nkv + kvh) * HD + 8 * ch);
+      }
+      int pos = max(g_hi - g_lo, 0) + len - (p.pad_left ? p.pad_left[b] : 0);
+      pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
+      const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t) + (size_t)pos * CH + ch);
+      const float4 s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t) + (size_t)pos * CH + ch);
+      cs[0] = c4.x; cs[1] = c4.y; cs[2] = c4.z; cs[3] = c4.w;
+      sn[0] = s4.x; sn[1] = s4.y; sn[2] = s4.z; sn[3] = s4.w;
     }
-    int pos = max(g_hi - g_lo, 0) + len - (p.pad_left ? p.pad_left[b] : 0);
-    pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
-    const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t) + (size_t)pos * CH + ch);
-    const float4 s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t) + (size_t)pos * CH + ch);
-    const float cs[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
     float kf[8];                                 // the new key, rotated and rounded as the cache holds it
-    {
+    if constexpr (ROTATE) {
       const uint32_t x[4] = {kx.x, kx.y, kx.z, kx.w};
       uint32_t a[4];
 #pragma unroll
@@ -239,19 +245,22 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
       const int r = i * RPS + rr;
       float dot = 0.f;
       if (r < G) {
-        const uint32_t x[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
-        uint32_t a[4], c[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float re = bf16_lo(x[e]), im = bf16_hi(x[e]);
-          const float y = re * cs[e] - im * sn[e], z = re * sn[e] + im * cs[e];
-          a[e] = pack_bf16(y, z);
-          c[e] = pack_bf16(y - bf16_lo(a[e]), z - bf16_hi(a[e]));
-          dot = fmaf(y, kf[2 * e], fmaf(z, kf[2 * e + 1], dot));
-        }
         const uint32_t at = qt + r * (HD * 2) + ((ch ^ r) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]) : "memory");
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + 8 * HD * 2), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]) : "memory");
+        if constexpr (ROTATE) {
+          const uint32_t x[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
+          uint32_t a[4], c[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float re = bf16_lo(x[e]), im = bf16_hi(x[e]);
+            const float y = re * cs[e] - im * sn[e], z = re * sn[e] + im * cs[e];
+            a[e] = pack_bf16(y, z);
+            c[e] = pack_bf16(y - bf16_lo(a[e]), z - bf16_hi(a[e]));
+            dot = fmaf(y, kf[2 * e], fmaf(z, kf[2 * e + 1], dot));
+          }
+          qx[i] = make_uint4(a[0], a[1], a[2], a[3]);
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + 8 * HD * 2), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]) : "memory");
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(qx[i].x), "r"(qx[i].y), "r"(qx[i].z), "r"(qx[i].w) : "memory");
       }
       if (newest) {
 #pragma unroll
@@ -375,6 +384,15 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
   }
 }
 
+// The own keys of prompts of a few tokens, behind the launch over the shared ones.  It starts on SMs that this one leaves: every CTA there has waited for what ran
+// before it lets a launch behind it begin, so nothing that is read here is still being written, and the wait is at the end, for the launch that joins both.
+template <int HD>
+__global__ void __launch_bounds__(256, 1) prefix_own_kernel(const PxParams p) {
+  extern __shared__ __align__(1024) uint8_t px_smem[];
+  px_own_keys<HD, false>(p, px_smem);
+  pdl_wait();
+}
+
 template <int HD, bool ROTATE, bool PAIR>
 __global__ void __launch_bounds__(PX_THREADS, 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv,
@@ -400,7 +418,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
   const int G = 1 << p.gs;
   if constexpr (ROTATE) {
     if ((int)blockIdx.x >= (int)gridDim.x - p.own_ctas) {
-      px_own_keys<HD>(p, px_smem);
+      px_own_keys<HD, true>(p, px_smem);
       return;
     }
   }
@@ -864,19 +882,34 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const float* __restric
   else *dst = pack_bf16(acc[0] * inv, acc[1] * inv);
 }
 
-template <int HD, bool ROTATE, bool PAIR>
-static int px_launch(const PxParams& p, unsigned ctas, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok, const CUtensorMap& ov, cudaStream_t st) {
-  using Tile = PxTile<HD, ROTATE, PAIR>;
-  // attributes belong to the device's context: set at the first call on each (bit per device; setting them twice is harmless)
-  static std::atomic<uint64_t> set{0};
+// (attributes belong to the device's context: set at the first call on each, a bit per device; setting them twice is harmless)
+static int px_smem_set(std::atomic<uint64_t>& set, const void* kernel, uint32_t smem) {
   int dev = 0;
   JL_CUDA(cudaGetDevice(&dev));
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (bit == 0 || !(set.load(std::memory_order_acquire) & bit)) {
-    JL_CUDA(cudaFuncSetAttribute(prefix_attn_kernel<HD, ROTATE, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile::SMEM));
+    JL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     set.fetch_or(bit, std::memory_order_release);
   }
+  return JL_OK;
+}
+
+template <int HD, bool ROTATE, bool PAIR>
+static int px_launch(const PxParams& p, unsigned ctas, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok, const CUtensorMap& ov, cudaStream_t st) {
+  using Tile = PxTile<HD, ROTATE, PAIR>;
+  static std::atomic<uint64_t> set{0};
+  const int rc = px_smem_set(set, (const void*)prefix_attn_kernel<HD, ROTATE, PAIR>, Tile::SMEM);
+  if (rc != JL_OK) return rc;
   JL_CUDA(launch_pdl(prefix_attn_kernel<HD, ROTATE, PAIR>, dim3(ctas), dim3(PX_THREADS), (size_t)Tile::SMEM, st, pk, pv, ok, ov, p));
+  return JL_OK;
+}
+
+template <int HD>
+static int px_own_launch(const PxParams& p, cudaStream_t st) {
+  static std::atomic<uint64_t> set{0};
+  const int rc = px_smem_set(set, (const void*)prefix_own_kernel<HD>, PxOwn<HD>::SMEM);
+  if (rc != JL_OK) return rc;
+  JL_CUDA(launch_pdl(prefix_own_kernel<HD>, dim3((unsigned)p.own_ctas), dim3(256), (size_t)PxOwn<HD>::SMEM, st, p));
   return JL_OK;
 }
 
@@ -959,8 +992,11 @@ static PxStep px_step(int B, int groups, int nkv, int G, int hd, int P, int T) {
   return r;
 }
 
+// Prompts of few tokens, own keys by a warp per (token, key head): their time in tiles of keys, 5 us in and out of 8 units.
+static float px_few(int B, int S, int nkv, float keys) { return (float)B * S * nkv / (8.f * PX_SMS) * (5.6f + keys / 12.f) + 1.f; }
+
 // S tokens per row.  Both sets of keys in one launch, every row's queries in tiles of their own, in `splits`; or the shared keys for all rows of a group together, in
-// `splits`, and then the own keys (taken to be the call's own tokens).
+// `splits`, and the own keys (taken to be the call's own tokens) in a second launch, in tiles or by warps.
 struct PxPrompt { bool both; int splits; };
 static PxPrompt px_prompt(int B, int S, int groups, int nkv, int G, int P) {
   const long queries = (long)(B / groups) * S * G, rows = (long)B * S * G * nkv;
@@ -968,7 +1004,7 @@ static PxPrompt px_prompt(int B, int S, int groups, int nkv, int G, int P) {
   PxPrompt r{false, 1};
   float least;
   r.splits = px_splits(queries, groups, nkv, P, PX_SMS, &least);
-  least += px_rounds((long)S * G, B, nkv, 1, own) + join + 3.f;
+  least += fminf(px_rounds((long)S * G, B, nkv, 1, own), px_few(B, S, nkv, (float)S)) + join + 3.f;
   for (int s = 1; s <= 4; ++s) {
     const float c = px_rounds((long)S * G, B, nkv, s, (shared + own) / s) + (s > 1 ? s * join + 3.f : 0.f);
     if (c < least) { least = c; r = PxPrompt{true, s}; }
@@ -1076,8 +1112,16 @@ extern "C" JL_API int jl_prefill_attn_prefix(const void* q, const void* prefix_k
     return px_join(p, (__nv_bfloat16*)out, B * S * nh, hd, -1, (cudaStream_t)stream);
   }
   p.shared = p.partial = 1;
+  const long units = (long)B * S * nkv;
+  const bool few = units < (1l << 30) && px_few(B, S, nkv, (float)(start + S)) < px_rounds((long)S * G, B, nkv, 1, (float)(start + S) / PX_BN);
   rc = px_dispatch(p, (long)rows * S * G, groups, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;
+  if (few) {
+    p.k_cache = (__nv_bfloat16*)k_cache; p.v_cache = (__nv_bfloat16*)v_cache;            // (read only)
+    p.B = B; p.own_splits = 1; p.own_ctas = (int)((units + 7) / 8);
+    rc = hd == 128 ? px_own_launch<128>(p, (cudaStream_t)stream) : px_own_launch<64>(p, (cudaStream_t)stream);
+    return rc != JL_OK ? rc : px_join(p, (__nv_bfloat16*)out, B * S * nh, hd, p.splits, (cudaStream_t)stream);
+  }
   p.shared = 0; p.own = 1; p.part0 = p.splits; p.splits = 1;
   rc = px_dispatch(p, (long)S * G, B, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;

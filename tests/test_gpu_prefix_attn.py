@@ -110,6 +110,9 @@ PROMPTS = [  # rows, groups, nh, nkv, hd, P, start, S, T, ragged
     (1, 1, 8, 2, 128, 2500, 0, 300, 300, False),     # in four
     (40, 1, 16, 2, 64, 1000, 7, 3, 16, True),        # the shared keys for all rows together, in splits, then the own keys
     (1, 1, 8, 2, 128, 2500, 9, 1, 12, True),         # one token
+    (15, 3, 32, 32, 64, 300, 0, 3, 20, True),        # a few tokens: own keys by a warp each
+    (12, 2, 16, 8, 128, 130, 70, 5, 90, True),
+    (6, 1, 8, 1, 128, 2000, 100, 2, 102, False),
 ]
 
 
