@@ -45,23 +45,29 @@ template <int HD> struct PxOwn {
   static constexpr uint32_t SMEM = WARPS * (RING + QT) + 1024;
 };
 
-// PAIR: two tiles of queries per CTA, each with its own softmax warps, over the same keys; else one tile whose keys the two sets of softmax warps take in turn.
-template <int HD, bool ROTATE, bool PAIR> struct PxTile {
+// How a CTA works.  PX_PAIR: two tiles of queries, each with its own softmax warps, over the same keys.  PX_TURNS: one tile whose keys the two sets of softmax warps
+// take in turn.  PX_SOLO: one tile, one set, half an SM (its way in and out falls into the other half's work).
+constexpr int PX_TURNS = 0, PX_PAIR = 1, PX_SOLO = 2;
+
+template <int HD, bool ROTATE, int MODE> struct PxTile {
+  static constexpr bool PAIR = MODE != PX_TURNS, SOLO = MODE == PX_SOLO, JOINT = MODE == PX_PAIR;        // PAIR: a set walks all tiles with queries of its own
   static constexpr int HALVES = HD / 64;
   static constexpr uint32_t Q_HALF = PX_BM * 128, Q = HALVES * Q_HALF;       // bytes of a tile of queries (hi or lo)
   static constexpr int NQ = ROTATE ? 2 : 1;                                  // hi, lo
-  static constexpr uint32_t QS = (PAIR ? 2 : 1) * NQ * Q;
+  static constexpr uint32_t QS = (JOINT ? 2 : 1) * NQ * Q;
+  static constexpr int ROWS = (JOINT ? 2 : 1) * PX_BM, SETS = SOLO ? 1 : 2, THREADS = SOLO ? 192 : PX_THREADS;      // (two warps and four for each set; one more for two)
   static constexpr uint32_t KV_HALF = PX_BN * 128, KV = HALVES * KV_HALF;    // 64 columns of a tile of keys or values, all of them
-  // A slot of the ring holds both (PAIR: one wait and one release per tile, the warps that issue products have none to spare), or keys and values in turn (the keys'
+  // A slot of the ring holds both (JOINT: one wait and one release per tile, the warps that issue products have none to spare), or keys and values in turn (the keys'
   // place is free again as soon as their scores are there: with both in one slot the four tiles that the two sets work on held the whole ring, and the keys of 48
   // rows x 32 heads came in at 29 GB/s per SM)
-  static constexpr uint32_t SLOT = (PAIR ? 2 : 1) * KV;
+  static constexpr uint32_t SLOT = (JOINT ? 2 : 1) * KV;
   static constexpr uint32_t SMALL = 512 + (PAIR ? 0 : 2048);                 // barriers, the address of the TMEM columns; (m, l) of 2 x 128 rows
-  static constexpr int FIT = (int)((227 * 1024 - 1024 - SMALL - QS) / SLOT);
+  static constexpr uint32_t MOST = (SOLO ? 113 : 227) * 1024;
+  static constexpr int FIT = (int)((MOST - 1024 - SMALL - QS) / SLOT);
   static constexpr int SLOTS = FIT < 16 ? FIT : 16;
   static constexpr uint32_t NEED = QS + SLOTS * SLOT + SMALL + 1024;         // (1024: alignment of the base)
   static constexpr uint32_t SMEM = ROTATE && NEED < PxOwn<HD>::SMEM ? PxOwn<HD>::SMEM : NEED;
-  static_assert(SLOTS >= (PAIR ? 3 : 8) && SMEM <= 227 * 1024, "a tile ahead of the products");
+  static_assert(SLOTS >= (SOLO ? 4 : (JOINT ? 3 : 8)) && SMEM <= MOST, "a tile ahead of the products");
 };
 
 // Two fp32 numbers at once (fma.rn.f32x2 and add.rn.f32x2: one issue slot for both).
@@ -393,11 +399,12 @@ __global__ void __launch_bounds__(256, 1) prefix_own_kernel(const PxParams p) {
   pdl_wait();
 }
 
-template <int HD, bool ROTATE, bool PAIR>
-__global__ void __launch_bounds__(PX_THREADS, 1)
+template <int HD, bool ROTATE, int MODE>
+__global__ void __launch_bounds__(PxTile<HD, ROTATE, MODE>::THREADS, MODE == PX_SOLO ? 2 : 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv,
                    const __grid_constant__ CUtensorMap tm_ok, const __grid_constant__ CUtensorMap tm_ov, const PxParams p) {
-  using Tile = PxTile<HD, ROTATE, PAIR>;
+  using Tile = PxTile<HD, ROTATE, MODE>;
+  constexpr bool PAIR = Tile::PAIR, SOLO = Tile::SOLO, JOINT = Tile::JOINT, LOW = !JOINT;      // LOW: probabilities may have low parts
   constexpr int HALVES = Tile::HALVES, NQ = Tile::NQ, SLOTS = Tile::SLOTS;
   extern __shared__ __align__(1024) uint8_t px_smem[];
   const uint32_t raw = tc::smem_u32(px_smem);
@@ -431,18 +438,18 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
   const int kvh = idx % p.nkv, z = idx / p.nkv;
   const int unit_tokens = p.own ? p.S : p.rows * p.S;             // tokens whose queries this launch packs together
   const int token0 = z * unit_tokens;
-  const int q0 = qt * (PAIR ? 2 * PX_BM : PX_BM), n_rows = min(PAIR ? 2 * PX_BM : PX_BM, unit_tokens * G - q0);
+  const int q0 = qt * Tile::ROWS, n_rows = min(Tile::ROWS, unit_tokens * G - q0);
   const int group = p.own ? z / p.rows : z;
-  const bool two = !PAIR || n_rows > PX_BM;                       // the second set of softmax warps has work
+  const bool two = !SOLO && (!PAIR || n_rows > PX_BM);                       // the second set of softmax warps has work
 
   if (warp == 0 && lane == 0) {
     if (p.shared) { tc::prefetch_tensormap(&tm_pk); tc::prefetch_tensormap(&tm_pv); }
     if (p.own) { tc::prefetch_tensormap(&tm_ok); tc::prefetch_tensormap(&tm_ov); }
   }
   if (warp == 1 && lane == 0) {
-    tc::mbar_init(q_full, 8);
+    tc::mbar_init(q_full, 4 * Tile::SETS);
     tc::mbar_init(started, 1);
-    const int users = PAIR && two ? 2 : 1;                        // products that read a tile
+    const int users = JOINT && two ? 2 : 1;                        // products that read a tile
     for (int w = 0; w < 2; ++w) {
       tc::mbar_init(p_full(w, 0), 4); tc::mbar_init(p_full(w, 1), 4); tc::mbar_init(o_last(w, 0), 1); tc::mbar_init(o_last(w, 1), 1);
       tc::mbar_init(s_full(w, 0), 1); tc::mbar_init(s_full(w, 1), 1);
@@ -450,7 +457,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
     for (int s = 0; s < SLOTS; ++s) { tc::mbar_init(slot_full(s), 1); tc::mbar_init(slot_empty(s), users); }
     tc::fence_barrier_init();
   }
-  if (warp == 0) tc::tmem_alloc(tmem_slot, 512);
+  if (warp == 0) tc::tmem_alloc(tmem_slot, 256 * Tile::SETS);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -486,8 +493,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
     if (lane == 0) {
       int sl = 0;
       uint32_t ph = 1;
-      for (int idx = 0; idx < (PAIR ? 1 : 2) * n_tiles; ++idx) {       // tiles, or K_0, V_0, K_1, V_1, ...
-        const int j = PAIR ? idx : idx >> 1;
+      for (int idx = 0; idx < (JOINT ? 1 : 2) * n_tiles; ++idx) {       // tiles, or K_0, V_0, K_1, V_1, ...
+        const int j = JOINT ? idx : idx >> 1;
         const bool mine = j >= n_shared;
         const int key0 = mine ? o_lo + (j - n_shared) * PX_BN : s_lo + j * PX_BN;
         const int head = (mine ? z : group) * p.nkv + kvh;
@@ -495,10 +502,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
         const CUtensorMap* mv = mine ? &tm_ov : &tm_pv;
         tc::mbar_wait(slot_empty(sl), ph);
         tc::mbar_expect_tx(slot_full(sl), Tile::SLOT);
-        const CUtensorMap* m0 = !PAIR && (idx & 1) ? mv : mk;
+        const CUtensorMap* m0 = !JOINT && (idx & 1) ? mv : mk;
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) tc::tma_load_3d(ring + sl * Tile::SLOT + h * Tile::KV_HALF, m0, slot_full(sl), 64 * h, key0, head, tc::EVICT_NORMAL);
-        if constexpr (PAIR) {
+        if constexpr (JOINT) {
 #pragma unroll
           for (int h = 0; h < HALVES; ++h)
             tc::tma_load_3d(ring + sl * Tile::SLOT + Tile::KV + h * Tile::KV_HALF, mv, slot_full(sl), 64 * h, key0, head, tc::EVICT_NORMAL);
@@ -513,11 +520,11 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
     const int w = warp == 1 ? 0 : 1, mine = tiles_of(w);
     constexpr uint32_t IDESC_S = tc::idesc_bf16_f32(PX_BM, PX_BN, false, false);
     constexpr uint32_t IDESC_O = tc::idesc_bf16_f32(PX_BM, HD, false, true);        // B = V is MN-major
-    constexpr int STEP = PAIR ? 1 : 4;                                 // slots from one of this set's tiles to the next
+    constexpr int STEP = JOINT ? 1 : 2 * Tile::SETS;                                 // slots from one of this set's tiles to the next
     const uint64_t dQ = tc::smem_desc_kmajor_sw128(sQ + (PAIR ? w * NQ * Tile::Q : 0));
     const uint64_t dK0 = tc::smem_desc_kmajor_sw128(ring);
-    const uint64_t dV0 = tc::smem_desc_mnmajor_sw128(ring + (PAIR ? Tile::KV : 0), Tile::KV_HALF, 1024);
-    int k_sl = PAIR ? 0 : 2 * w, v_sl = PAIR ? 0 : 2 * w + 1;          // slots of the next scores and of the next product
+    const uint64_t dV0 = tc::smem_desc_mnmajor_sw128(ring + (JOINT ? Tile::KV : 0), Tile::KV_HALF, 1024);
+    int k_sl = JOINT ? 0 : 2 * w, v_sl = JOINT ? 0 : 2 * w + 1;          // slots of the next scores and of the next product
     uint32_t k_ph = 0, v_ph = 0;
     auto next_slot = [&](int& sl) { sl += STEP; if (sl >= SLOTS) { sl -= SLOTS; return 1u; } return 0u; };
     auto issue_s = [&](int i) {
@@ -532,7 +539,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
             tc::mma_ss(tS(w, i), dQ + (uint64_t)((n * Tile::Q + (k >> 2) * Tile::Q_HALF + (k & 3) * 32) >> 4),
                        dK + (uint64_t)(((k >> 2) * Tile::KV_HALF + (k & 3) * 32) >> 4), IDESC_S, n != 0 || k != 0);
         tc::mma_commit(s_full(w, i));
-        if (!PAIR) tc::mma_commit(slot_empty(k_sl));
+        if (!JOINT) tc::mma_commit(slot_empty(k_sl));
       }
       __syncwarp();
       k_ph ^= next_slot(k_sl);
@@ -541,18 +548,18 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
       tc::mbar_wait(q_full, 0);
       tc::fence_after_sync();
       // the sets run half a tile apart, so that one's exponentials fall into the other's loads and waits; started together they stay together
-      if (PAIR && w == 1) tc::mbar_wait(started, 0);
+      if (JOINT && w == 1) tc::mbar_wait(started, 0);
       issue_s(0);
     }
     for (int i = 0; i < mine; ++i) {
       if (i + 1 < mine) issue_s(i + 1);                                // the tensor core forms the next scores during this tile's softmax
-      if (!PAIR) tc::mbar_wait(slot_full(v_sl), v_ph);
+      if (!JOINT) tc::mbar_wait(slot_full(v_sl), v_ph);
       const int j = tile_at(w, i);
       const int left = j < n_shared ? s_hi - s_lo - j * PX_BN : o_hi - o_lo - (j - n_shared) * PX_BN;
       if (left < PX_BN) {                                              // value rows that hold no key (both sets write the same zeros)
         for (int e = lane; e < (PX_BN - left) * 8 * HALVES; e += 32) {
           const int r = left + e / (8 * HALVES), c = e % (8 * HALVES);
-          const uint32_t a = ring + v_sl * Tile::SLOT + (PAIR ? Tile::KV : 0) + (c >> 3) * Tile::KV_HALF + r * 128 + (c & 7) * 16;
+          const uint32_t a = ring + v_sl * Tile::SLOT + (JOINT ? Tile::KV : 0) + (c >> 3) * Tile::KV_HALF + r * 128 + (c & 7) * 16;
           asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -563,7 +570,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
       if (tc::elect_one()) {
         const uint64_t dV = dV0 + (uint64_t)v_sl * (Tile::SLOT >> 4);
 #pragma unroll
-        for (int k = 0; k < (PAIR ? 1 : 2) * PX_BN / 16; ++k)          // A = P in TMEM: 16 keys = 8 columns of packed pairs; the low parts behind the high ones
+        for (int k = 0; k < (LOW ? 2 : 1) * PX_BN / 16; ++k)          // A = P in TMEM: 16 keys = 8 columns of packed pairs; the low parts behind the high ones
           if (k < 4 || p.p_low) tc::mma_ts(tO(w), tS(w, i) + k * 8, dV + (uint64_t)(((k & 3) * 2048) >> 4), IDESC_O, i != 0 || k != 0);
         tc::mma_commit(slot_empty(v_sl));
         if (i + 2 >= mine) tc::mma_commit(o_last(w, i + 2 - mine));
@@ -572,7 +579,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
       v_ph ^= next_slot(v_sl);
     }
   } else {
-    const int w = warp >= 6 ? 1 : 0;                                   // set of softmax warps (2..5, 6..9)
+    const int w = !SOLO && warp >= 6 ? 1 : 0;                                   // set of softmax warps (2..5, 6..9)
     const int quarter = warp & 3;                                      // TMEM lane quadrant of this warp
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     // ---- queries, 16 bytes per lane and step: a set's own tile, or half of the one tile
@@ -689,7 +696,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
         }
         const float m_safe = m_ref == -INFINITY ? 0.f : m_ref;
         F2 sum = f2(0.f, 0.f);
-        uint32_t hi[32], lo[PAIR ? 1 : 32];
+        uint32_t hi[32], lo[LOW ? 32 : 1];
         const F2 scale2 = f2(p.scale_log2, p.scale_log2), minus_m = f2(-m_safe, -m_safe);
         auto pair = [&](int e, bool poly) {                            // keys 2e, 2e + 1
           const uint32_t* v = e < 16 ? v0 + 2 * e : v1 + 2 * e - 32;
@@ -703,9 +710,9 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
           }
           sum = f2_add(sum, f2(a, b));
           hi[e] = pack_bf16(a, b);
-          if (!PAIR && p.p_low) lo[PAIR ? 0 : e] = pack_bf16(a - bf16_lo(hi[e]), b - bf16_hi(hi[e]));
+          if (LOW && p.p_low) lo[LOW ? e : 0] = pack_bf16(a - bf16_lo(hi[e]), b - bf16_hi(hi[e]));
         };
-        if (!odd && (PAIR || !p.p_low)) {
+        if (!odd && (!LOW || !p.p_low)) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) pair(e, (e * PX_POLY) % 16 < PX_POLY);
         } else {
@@ -716,7 +723,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
         f2_get(sum, psum, psum2);
         psum += psum2;
         tc::tmem_st32(tS(w, i) + lane_off, hi);                        // keys 2c, 2c + 1 of this row: 32-bit column c
-        if constexpr (!PAIR) if (p.p_low) tc::tmem_st32(tS(w, i) + lane_off + 32, lo);
+        if constexpr (LOW) if (p.p_low) tc::tmem_st32(tS(w, i) + lane_off + 32, lo);
         tc::tmem_st_wait();
         l_run += psum;
       }
@@ -724,7 +731,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(p_full(w, i));
-      if (PAIR && i == 0 && warp == 2 && lane == 0) tc::mbar_arrive(started);
+      if (JOINT && i == 0 && warp == 2 && lane == 0) tc::mbar_arrive(started);
     }
     if (my_tiles > 0) {
       tc::mbar_wait(o_last(w, 1), 0);
@@ -816,7 +823,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
 
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == 0) tc::tmem_dealloc(tmem, 512);
+  if (warp == 0) tc::tmem_dealloc(tmem, 256 * Tile::SETS);
 }
 
 // Joins the triples of a (token, head), a warp each.  `own`: the part of the own keys of a prompt, -1 where every part says itself that a query
@@ -894,13 +901,13 @@ static int px_smem_set(std::atomic<uint64_t>& set, const void* kernel, uint32_t 
   return JL_OK;
 }
 
-template <int HD, bool ROTATE, bool PAIR>
+template <int HD, bool ROTATE, int MODE>
 static int px_launch(const PxParams& p, unsigned ctas, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok, const CUtensorMap& ov, cudaStream_t st) {
-  using Tile = PxTile<HD, ROTATE, PAIR>;
+  using Tile = PxTile<HD, ROTATE, MODE>;
   static std::atomic<uint64_t> set{0};
-  const int rc = px_smem_set(set, (const void*)prefix_attn_kernel<HD, ROTATE, PAIR>, Tile::SMEM);
+  const int rc = px_smem_set(set, (const void*)prefix_attn_kernel<HD, ROTATE, MODE>, Tile::SMEM);
   if (rc != JL_OK) return rc;
-  JL_CUDA(launch_pdl(prefix_attn_kernel<HD, ROTATE, PAIR>, dim3(ctas), dim3(PX_THREADS), (size_t)Tile::SMEM, st, pk, pv, ok, ov, p));
+  JL_CUDA(launch_pdl(prefix_attn_kernel<HD, ROTATE, MODE>, dim3(ctas), dim3(Tile::THREADS), (size_t)Tile::SMEM, st, pk, pv, ok, ov, p));
   return JL_OK;
 }
 
@@ -925,14 +932,14 @@ static long px_tiles(long queries) { return queries > PX_BM ? (queries + 2 * PX_
 // One launch over tiles of the queries of `units` groups or rows, `queries` of a key head each.
 static int px_dispatch(PxParams p, long queries, int units, bool rotate, int hd, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok,
                        const CUtensorMap& ov, cudaStream_t st) {
-  const bool pair = queries > PX_BM;
   p.tiles_q = (int)px_tiles(queries);
   p.p_low = queries <= PX_BM;
   const long ctas = p.own_ctas + (long)p.tiles_q * p.splits * p.nkv * units;
   JL_CHECK_ARG(ctas < (1l << 31), "attention over a shared prefix: %ld tiles", ctas);
-#define JL_PX(HD_, R_, P_) if (hd == HD_ && rotate == R_ && pair == P_) return px_launch<HD_, R_, P_>(p, (unsigned)ctas, pk, pv, ok, ov, st);
-  JL_PX(128, true, true) JL_PX(128, true, false) JL_PX(128, false, true) JL_PX(128, false, false)
-  JL_PX(64, true, true) JL_PX(64, true, false) JL_PX(64, false, true) JL_PX(64, false, false)
+  const int mode = queries > PX_BM ? PX_PAIR : (!rotate && ctas > 148 ? PX_SOLO : PX_TURNS);
+#define JL_PX(HD_, R_, M_) if (hd == HD_ && rotate == R_ && mode == M_) return px_launch<HD_, R_, M_>(p, (unsigned)ctas, pk, pv, ok, ov, st);
+  JL_PX(128, true, PX_PAIR) JL_PX(128, true, PX_TURNS) JL_PX(128, false, PX_PAIR) JL_PX(128, false, PX_TURNS) JL_PX(128, false, PX_SOLO)
+  JL_PX(64, true, PX_PAIR) JL_PX(64, true, PX_TURNS) JL_PX(64, false, PX_PAIR) JL_PX(64, false, PX_TURNS) JL_PX(64, false, PX_SOLO)
 #undef JL_PX
   return JL_ERR_UNSUPPORTED;
 }

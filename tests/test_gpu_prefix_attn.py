@@ -113,6 +113,10 @@ PROMPTS = [  # rows, groups, nh, nkv, hd, P, start, S, T, ragged
     (15, 3, 32, 32, 64, 300, 0, 3, 20, True),        # a few tokens: own keys by a warp each
     (12, 2, 16, 8, 128, 130, 70, 5, 90, True),
     (6, 1, 8, 1, 128, 2000, 100, 2, 102, False),
+    (40, 4, 32, 8, 128, 300, 0, 7, 20, True),        # more tiles than SMs, two to an SM: one launch
+    (20, 2, 8, 8, 64, 500, 30, 100, 140, True),
+    (24, 1, 16, 8, 128, 3000, 3, 40, 50, False),     # and the own keys behind the shared ones
+    (60, 1, 32, 4, 64, 1500, 0, 12, 12, True),
 ]
 
 
