@@ -927,16 +927,24 @@ static int px_join(const PxParams& p, __nv_bfloat16* out, int rows, int hd, int 
   return JL_OK;
 }
 
+constexpr int PX_MAX_SPLITS = 64, PX_MAX_OWN = 16, PX_SMS = 148;
+
 static long px_tiles(long queries) { return queries > PX_BM ? (queries + 2 * PX_BM - 1) / (2 * PX_BM) : 1; }
 
 // One launch over tiles of the queries of `units` groups or rows, `queries` of a key head each.
 static int px_dispatch(PxParams p, long queries, int units, bool rotate, int hd, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& ok,
                        const CUtensorMap& ov, cudaStream_t st) {
-  p.tiles_q = (int)px_tiles(queries);
+  // Two CTAs to an SM where tiles outnumber the SMs, and for larger prompts over few keys, where what a CTA does beside its tiles counts most: us in a graph, pairs and
+  // this, 26 x 146 tokens x 32 key heads over 35 keys 76, 59; 10 x 403 over 47 54, 46; 8 x 64 x 4 over 500 (64 pairs) 14.8, 12.2, over 1000 22, 18; 16 x 128 x 4 over 100 21.6, 20.4; and over
+  // 1000 44, 47, 4000 120, 135: every CTA then asks L2 for keys of its own.
+  const float keys = (p.shared ? (float)p.P : 0.f) + (p.own ? (float)p.start + 0.5f * (float)p.S : 0.f), tiles = keys / (float)(PX_BN * p.splits);
+  const long pairs = px_tiles(queries) * p.splits * p.nkv * units;
+  const bool solo = !rotate && (queries <= PX_BM ? pairs > PX_SMS : tiles <= (2 * pairs <= PX_SMS ? 20.f : 8.f));
+  const int mode = solo ? PX_SOLO : (queries > PX_BM ? PX_PAIR : PX_TURNS);
+  p.tiles_q = solo ? (int)((queries + PX_BM - 1) / PX_BM) : (int)px_tiles(queries);
   p.p_low = queries <= PX_BM;
   const long ctas = p.own_ctas + (long)p.tiles_q * p.splits * p.nkv * units;
   JL_CHECK_ARG(ctas < (1l << 31), "attention over a shared prefix: %ld tiles", ctas);
-  const int mode = queries > PX_BM ? PX_PAIR : (!rotate && ctas > 148 ? PX_SOLO : PX_TURNS);
 #define JL_PX(HD_, R_, M_) if (hd == HD_ && rotate == R_ && mode == M_) return px_launch<HD_, R_, M_>(p, (unsigned)ctas, pk, pv, ok, ov, st);
   JL_PX(128, true, PX_PAIR) JL_PX(128, true, PX_TURNS) JL_PX(128, false, PX_PAIR) JL_PX(128, false, PX_TURNS) JL_PX(128, false, PX_SOLO)
   JL_PX(64, true, PX_PAIR) JL_PX(64, true, PX_TURNS) JL_PX(64, false, PX_PAIR) JL_PX(64, false, PX_TURNS) JL_PX(64, false, PX_SOLO)
@@ -944,24 +952,25 @@ static int px_dispatch(PxParams p, long queries, int units, bool rotate, int hd,
   return JL_ERR_UNSUPPORTED;
 }
 
-constexpr int PX_MAX_SPLITS = 64, PX_MAX_OWN = 16, PX_SMS = 148;
 
-// Time of a launch in units of a tile of keys: rounds of CTAs (one per SM) times the tiles of one and its way in and out.
-static float px_rounds(long queries, long units, int nkv, int splits, float tiles, int sms = PX_SMS) {
+// Time of a launch in units of a tile of keys: rounds of CTAs (one per SM; `solo`: two where one tile of queries has more of them) times the tiles of one and its
+// way in and out.
+static float px_rounds(long queries, long units, int nkv, int splits, float tiles, bool solo) {
   const long full = queries > PX_BM ? queries / (2 * PX_BM) : 1, rest = px_tiles(queries) - full;      // whole pairs, one that may be half a pair
   const long ctas = (full + rest) * units * nkv * splits;
+  if (solo && queries <= PX_BM && ctas > PX_SMS) return (float)((ctas + 2 * PX_SMS - 1) / (2 * PX_SMS)) * (1.35f * tiles + 8.f);
   const float whole = tiles + 5.f, part = rest && queries % (2 * PX_BM) <= PX_BM ? 0.78f * tiles + 5.f : whole;
-  if (part == whole || ctas <= sms) return (float)((ctas + sms - 1) / sms) * (full ? whole : part);
-  return (float)(units * nkv * splits) * (full * whole + rest * part) / sms + 0.5f * whole;
+  if (part == whole || ctas <= PX_SMS) return (float)((ctas + PX_SMS - 1) / PX_SMS) * (full ? whole : part);
+  return (float)(units * nkv * splits) * (full * whole + rest * part) / PX_SMS + 0.5f * whole;
 }
 
-// Splits of the shared keys over `sms` SMs: the count with the least time, every one two tiles of keys or more; a split costs the triples' way to memory and back.
-static int px_splits(long queries, int groups, int nkv, int prefix, int sms = PX_SMS, float* cost = nullptr) {
+// Splits of the shared keys: the count with the least time, every one two tiles of keys or more; a split costs the triples' way to memory and back.
+static int px_splits(long queries, int groups, int nkv, int prefix, bool solo = false, float* cost = nullptr) {
   const int tiles = (prefix + PX_BN - 1) / PX_BN;
   int best = 1;
   float least = 0.f;
   for (int s = 1; s <= PX_MAX_SPLITS && (s == 1 || 2 * s <= tiles); ++s) {
-    const float c = px_rounds(queries, groups, nkv, s, (float)((tiles + s - 1) / s), sms) + (float)(queries * groups * nkv) * s * 3e-4f;
+    const float c = px_rounds(queries, groups, nkv, s, (float)((tiles + s - 1) / s), solo) + (float)(queries * groups * nkv) * s * 3e-4f;
     if (s == 1 || c < least) { least = c; best = s; }
   }
   if (cost) *cost = least;
@@ -1010,10 +1019,10 @@ static PxPrompt px_prompt(int B, int S, int groups, int nkv, int G, int P) {
   const float own = (float)S / PX_BN, shared = (float)P / PX_BN, join = 4e-4f * (float)rows;
   PxPrompt r{false, 1};
   float least;
-  r.splits = px_splits(queries, groups, nkv, P, PX_SMS, &least);
-  least += fminf(px_rounds((long)S * G, B, nkv, 1, own), px_few(B, S, nkv, (float)S)) + join + 3.f;
+  r.splits = px_splits(queries, groups, nkv, P, true, &least);
+  least += fminf(px_rounds((long)S * G, B, nkv, 1, own, true), px_few(B, S, nkv, (float)S)) + join + 3.f;
   for (int s = 1; s <= 4; ++s) {
-    const float c = px_rounds((long)S * G, B, nkv, s, (shared + own) / s) + (s > 1 ? s * join + 3.f : 0.f);
+    const float c = px_rounds((long)S * G, B, nkv, s, (shared + own) / s, true) + (s > 1 ? s * join + 3.f : 0.f);
     if (c < least) { least = c; r = PxPrompt{true, s}; }
   }
   return r;
@@ -1120,7 +1129,7 @@ extern "C" JL_API int jl_prefill_attn_prefix(const void* q, const void* prefix_k
   }
   p.shared = p.partial = 1;
   const long units = (long)B * S * nkv;
-  const bool few = units < (1l << 30) && px_few(B, S, nkv, (float)(start + S)) < px_rounds((long)S * G, B, nkv, 1, (float)(start + S) / PX_BN);
+  const bool few = units < (1l << 30) && px_few(B, S, nkv, (float)(start + S)) < px_rounds((long)S * G, B, nkv, 1, (float)(start + S) / PX_BN, true);
   rc = px_dispatch(p, (long)rows * S * G, groups, false, hd, pk, pv, ok, ov, (cudaStream_t)stream);
   if (rc != JL_OK) return rc;
   if (few) {
