@@ -7,9 +7,11 @@
 // matrix [rows · S · G, d] per (group, key head), cut into tiles of 128 for tcgen05.  With running statistics a softmax over two sets of keys
 // is a join of two triples (reference exponent m, sum l, weighted values o):  M = max(m1, m2),  o = o1 2^(m1 - M) + o2 2^(m2 - M),  l likewise.
 //   * one token per row (jl_decode_attn_prefix): one launch in which some CTAs take the shared keys, tiles of queries by splits of the keys, and others the
-//     rows' own keys, a warp per (row, key head), appending the new one; all leave partial triples in fp32, and a second, small launch joins them;
-//   * S tokens per row (jl_prefill_attn_prefix): the same for the shared keys, then a second launch over every row's own keys, causal, and the join; or, where
-//     a row's queries fill tiles by themselves, one launch over both sets of keys, tile after tile, whole or in splits that the join puts together.
+//     rows' own keys, a warp per (row, key head), appending the new one; all leave partial triples in fp32, and a second, small launch joins them; with up to
+//     eight queries of a (group, key head), warps take the shared keys too;
+//   * S tokens per row (jl_prefill_attn_prefix): the same for the shared keys, then a second launch over every row's own keys, causal, in tiles or, a few tokens, by
+//     warps, and the join; or, where a row's queries fill tiles by themselves, one launch over both sets of keys, tile after tile, whole or in splits that the join
+//     puts together.
 //
 // One CTA owns a tile of 128 queries of one key head, as in flash_prefill.cu: a warp asks for K and V tiles of 64 keys (TMA, 128-byte swizzle), a warp
 // issues S = Q·Kᵀ into one of two score tiles in TMEM and O += P·V with P read from TMEM, four warps hold one query row per thread: one pass over 64
@@ -21,8 +23,8 @@
 // Slots that hold no key may hold anything: their scores are masked, and their value rows are cleared in shared memory, because a weight of zero
 // times a NaN is a NaN.
 //
-// One B200, us a call in a graph: one token, 16 rows x 32 heads over 8 of keys, 2048 shared 13; 96 rows, 32768 shared and 500 own each 106 (790 TFLOP/s with the
-// second products of the queries, 3.1 TB/s beside them); 4 x 16 rows, 3501 shared and 701 own 45 (5.4 TB/s).  Prompts: 2 x 2048 tokens over 16384 1065 (1080 TFLOP/s; a
+// One B200, us a call in a graph: one token, 16 rows x 32 heads over 8 of keys, 2048 shared 12.7; 96 rows, 32768 shared and 500 own each 106 (790 TFLOP/s with the
+// second products of the queries, 3.1 TB/s beside them); 4 x 16 rows, 3501 shared and 701 own 44 (5.5 TB/s).  Prompts: 2 x 2048 tokens over 16384 1065 (1080 TFLOP/s; a
 // single launch of its own 906 and 1290: the power cap), 8 x 333 over 1500 68 (1110), 16 x 48 over 8192 111 (920).  What bounds them: products of small width
 // (a 128 x 64 tile of scores reads its queries from shared memory, 384 cycles for 256 of products) and the exponentials, half of the special-function
 // unit's rate with a quarter of them on the FMA units; in short calls the chain launch, queries, scores, last rows, join.
@@ -109,7 +111,7 @@ struct PxParams {
   int shared, own, partial;         // which keys this launch visits; whether it leaves partial triples or the result
   int splits, parts, part0;         // splits of the shared keys in this launch; triples per (token, head), the first that this launch writes
   // the last `own_ctas` CTAs of a step, or a launch of their own, take the own keys, `own_splits` parts of every (token, key head)
-  const __nv_bfloat16* qkv; __nv_bfloat16* k_cache; __nv_bfloat16* v_cache;
+  const __nv_bfloat16* prefix_k; const __nv_bfloat16* prefix_v; __nv_bfloat16* k_cache; __nv_bfloat16* v_cache;
   int own_ctas, own_splits, B, tiles_q;
   int p_low;                        // one tile of queries: probabilities as two bfloat16 numbers
   float scale_log2;
@@ -131,9 +133,12 @@ __device__ __forceinline__ void px_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
 // of the queries (scores) and of the probabilities (values): both keep 16 bits at no cost.  The new token of a step's row, in the last part, is folded in from
 // registers; a prompt's tokens are in the cache.  Bound by the cache's bytes; a block's chain of dependent steps takes about 0.6 us, so that a warp moves 13 GB/s and eight of them an SM's share
 // of the bandwidth twice over.
-template <int HD, bool ROTATE>
+// KIND: what the units are.
+constexpr int PX_PROMPT_OWN = 0, PX_STEP_OWN = 1, PX_STEP_ALL = 2;    // ALL: parts of the shared keys too, for the up to eight queries of a (group, key head)
+template <int HD, int KIND>
 __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
   using Own = PxOwn<HD>;
+  constexpr bool ROTATE = KIND != PX_PROMPT_OWN, ALL = KIND == PX_STEP_ALL;
   constexpr int KPI = Own::KPI, HALVES = Own::HALVES, STAGES = Own::STAGES;
   constexpr int NT = KPI / 8, NB = KPI / 16, KS = HD / 16;
   constexpr int CH = HD / 8, RPS = 32 / CH, PASSES = 8 / RPS;       // 16-byte chunks of a row, rows that a warp holds at once
@@ -141,47 +146,65 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
   if (warp >= Own::WARPS) return;
   const uint32_t raw = tc::smem_u32(smem), base0 = (raw + 1023u) & ~1023u;
   const uint32_t ring = base0 + warp * Own::RING, qt = base0 + Own::WARPS * Own::RING + warp * Own::QT;
-  for (int i = lane; i < (int)Own::QT / 16; i += 32)                  // rows without a head stay zero
+  for (int i = lane; i < (int)Own::QT / 16; i += 32)                  // rows without a head: zero, or what a unit before had there
     asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(qt + 16 * i), "r"(0) : "memory");
   __syncwarp();
   if constexpr (ROTATE) pdl_wait();
   pdl_launch_dependents();
 
-  const int G = 1 << p.gs, units = p.B * p.S * p.nkv * p.own_splits, step = p.own_ctas * Own::WARPS;
+  const int G = 1 << p.gs, shared_units = ALL ? p.B / p.rows * p.nkv * p.splits : 0;
+  const int units = shared_units + p.B * p.S * p.nkv * p.own_splits, step = p.own_ctas * Own::WARPS;
   const int len = ROTATE ? min(max(*p.cache_len, 0), p.T) : 0;           // a step: keys in front of the new token
-  // first and last + 1 key of unit u
-  auto range = [&](int u, int& lo, int& hi) {
-    const int item = u / p.own_splits, part = u - item * p.own_splits, token = item / p.nkv, b = ROTATE ? token : token / p.S;
-    const int first = p.pad_left ? max(p.pad_left[b], 0) : 0, valid = max((ROTATE ? len : p.start + token - b * p.S + 1) - first, 0);
-    const int chunk = ((valid + p.own_splits - 1) / p.own_splits + KPI - 1) / KPI * KPI;
-    lo = first + min(part * chunk, valid);
-    hi = first + min((part + 1) * chunk, valid);
+  auto shared_range = [&](int group, int& lo, int& hi) {
+    lo = p.prefix_pad ? max(p.prefix_pad[group], 0) : 0;
+    hi = max(p.prefix_len ? min(p.prefix_len[group], p.P) : p.P, lo);
   };
-  // (row, key head) of unit u in the caches
-  auto cache_row = [&](int u) { const int item = u / p.own_splits; return ROTATE ? item : item / p.nkv / p.S * p.nkv + item % p.nkv; };
+  // first and last + 1 key of unit u, and its (row or group, key head) in the caches
+  auto range = [&](int u, int& lo, int& hi, int& at) {
+    int parts = p.own_splits, part, n;
+    if (ALL && u < shared_units) {
+      parts = p.splits;
+      at = u / parts; part = u - at * parts;
+      shared_range(at / p.nkv, lo, hi);
+      n = hi - lo;
+    } else {
+      if (ALL) u -= shared_units;
+      const int item = u / parts, token = item / p.nkv, b = ROTATE ? token : token / p.S;
+      part = u - item * parts;
+      at = ROTATE ? item : b * p.nkv + item - token * p.nkv;
+      lo = p.pad_left ? max(p.pad_left[b], 0) : 0;
+      n = max((ROTATE ? len : p.start + token - b * p.S + 1) - lo, 0);
+    }
+    const int chunk = ((n + parts - 1) / parts + KPI - 1) / KPI * KPI;
+    hi = lo + min((part + 1) * chunk, n);
+    lo += min(part * chunk, n);
+  };
   // what is asked for next: block [r_base, r_base + KPI) of unit r_u
   const int first_unit = ((int)blockIdx.x - ((int)gridDim.x - p.own_ctas)) * Own::WARPS + warp;
-  int r_u = first_unit, r_base = 0, r_hi = 0, r_st = 0;
-  if (r_u < units) range(r_u, r_base, r_hi);
+  int r_u = first_unit, r_base = 0, r_hi = 0, r_at = 0, r_st = 0;
+  if (r_u < units) range(r_u, r_base, r_hi, r_at);
   // 16-byte copies into the swizzled layout, eight 512-byte rows of requests each for keys and values; keys behind the last one become zeros (a weight of
   // zero times a NaN is a NaN).  By TMA, whose boxes of 16 rows leave the SM at 28 bytes a cycle, the warps waited for its queue a third of their time.
   const int r_ch = lane % CH, r_key = lane / CH;
   auto request = [&]() {
     while (r_u < units && r_base >= r_hi) {
       r_u += step;
-      if (r_u < units) range(r_u, r_base, r_hi);
+      if (r_u < units) range(r_u, r_base, r_hi, r_at);
     }
     if (r_u < units) {
+      const bool sh = ALL && r_u < shared_units;
+      const __nv_bfloat16* from_k = sh ? p.prefix_k : p.k_cache;
+      const __nv_bfloat16* from_v = sh ? p.prefix_v : p.v_cache;
       const uint32_t dst = ring + r_st * Own::STAGE + (r_ch >> 3) * Own::BOX;
-      const size_t src = ((size_t)cache_row(r_u) * p.T + r_base + r_key) * HD + 8 * r_ch;
+      const size_t src = ((size_t)r_at * (sh ? p.P : p.T) + r_base + r_key) * HD + 8 * r_ch;
 #pragma unroll
       for (int i = 0; i < KPI / RPS; ++i) {
         const int key = i * RPS + r_key;
         const uint32_t at = dst + key * 128 + (((r_ch & 7) ^ (key & 7)) << 4);
         const bool on = r_base + key < r_hi;
         const size_t from = on ? src + (size_t)(i * RPS) * HD : 0;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(p.k_cache + from), "r"(on ? 16 : 0) : "memory");
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + HALVES * Own::BOX), "l"(p.v_cache + from), "r"(on ? 16 : 0) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from_k + from), "r"(on ? 16 : 0) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + HALVES * Own::BOX), "l"(from_v + from), "r"(on ? 16 : 0) : "memory");
       }
       r_base += KPI;
       if (++r_st == STAGES) r_st = 0;
@@ -202,31 +225,40 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
   int st = 0;
 #pragma unroll 1
   for (int u = first_unit; u < units; u += step) {
-    int lo, hi;
-    range(u, lo, hi);
-    const int item = u / p.own_splits, part = u - item * p.own_splits, b = item / p.nkv, kvh = item - b * p.nkv;      // (b: the token)
-    const __nv_bfloat16* row = p.q + (size_t)b * p.ldq;
-    const bool newest = ROTATE && part == p.own_splits - 1;
+    int lo, hi, at_row;
+    range(u, lo, hi, at_row);
+    // queries of the unit: n of them, number r of token b + r / G and head r % G of the key head
+    const bool sh = ALL && u < shared_units;
+    const int parts = sh ? p.splits : p.own_splits, own_u = sh ? u : u - shared_units, item = own_u / parts, part = own_u - item * parts;
+    const int kvh = item % p.nkv, b = sh ? item / p.nkv * p.rows : item / p.nkv, n = sh ? p.rows * G : G;
+    auto row_of = [&](int r) { return p.q + (size_t)(b + (r >> p.gs)) * p.ldq + (size_t)(kvh * G + (r & (G - 1))) * HD; };
+    const bool newest = ROTATE && !sh && part == p.own_splits - 1;
     // ---- queries: chunk `ch` of rows pass · RPS + lane / CH; and of the new token's key and value
     const int ch = lane % CH, rr = lane / CH;
     uint4 qx[PASSES], kx = make_uint4(0, 0, 0, 0), vx = kx;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i)
-      if (i * RPS + rr < G) qx[i] = *reinterpret_cast<const uint4*>(row + (size_t)(kvh * G + i * RPS + rr) * HD + 8 * ch);
-    float cs[4], sn[4];
+      if (i * RPS + rr < n) qx[i] = *reinterpret_cast<const uint4*>(row_of(i * RPS + rr) + 8 * ch);
+    constexpr int NP = ALL ? PASSES : 1;         // rows of several tokens have angles of their own
+    float cs[NP][4], sn[NP][4];
     if constexpr (ROTATE) {
-      const int group = b / p.rows;
-      const int g_lo = p.prefix_pad ? max(p.prefix_pad[group], 0) : 0, g_hi = p.prefix_len ? min(p.prefix_len[group], p.P) : p.P;
       if (newest) {
+        const __nv_bfloat16* row = p.q + (size_t)b * p.ldq;
         kx = *reinterpret_cast<const uint4*>(row + (size_t)(p.nh + kvh) * HD + 8 * ch);
         vx = *reinterpret_cast<const uint4*>(row + (size_t)(p.nh + p.nkv + kvh) * HD + 8 * ch);
       }
-      int pos = max(g_hi - g_lo, 0) + len - (p.pad_left ? p.pad_left[b] : 0);
-      pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
-      const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t) + (size_t)pos * CH + ch);
-      const float4 s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t) + (size_t)pos * CH + ch);
-      cs[0] = c4.x; cs[1] = c4.y; cs[2] = c4.z; cs[3] = c4.w;
-      sn[0] = s4.x; sn[1] = s4.y; sn[2] = s4.z; sn[3] = s4.w;
+      int g_lo, g_hi;
+      shared_range(b / p.rows, g_lo, g_hi);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int token = ALL ? b + (min(i * RPS + rr, n - 1) >> p.gs) : b;
+        int pos = g_hi - g_lo + len - (p.pad_left ? p.pad_left[token] : 0);
+        pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
+        const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t) + (size_t)pos * CH + ch);
+        const float4 s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t) + (size_t)pos * CH + ch);
+        cs[i][0] = c4.x; cs[i][1] = c4.y; cs[i][2] = c4.z; cs[i][3] = c4.w;
+        sn[i][0] = s4.x; sn[i][1] = s4.y; sn[i][2] = s4.z; sn[i][3] = s4.w;
+      }
     }
     float kf[8];                                 // the new key, rotated and rounded as the cache holds it
     if constexpr (ROTATE) {
@@ -235,11 +267,11 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float re = bf16_lo(x[e]), im = bf16_hi(x[e]);
-        a[e] = pack_bf16(re * cs[e] - im * sn[e], re * sn[e] + im * cs[e]);
+        a[e] = pack_bf16(re * cs[0][e] - im * sn[0][e], re * sn[0][e] + im * cs[0][e]);
         kf[2 * e] = bf16_lo(a[e]); kf[2 * e + 1] = bf16_hi(a[e]);
       }
       if (newest && rr == 0 && len < p.T) {
-        const size_t slot = ((size_t)item * p.T + len) * HD + 8 * ch;
+        const size_t slot = ((size_t)at_row * p.T + len) * HD + 8 * ch;
         *reinterpret_cast<uint4*>(p.k_cache + slot) = make_uint4(a[0], a[1], a[2], a[3]);
         *reinterpret_cast<uint4*>(p.v_cache + slot) = vx;
       }
@@ -247,10 +279,10 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
     float s_new = 0.f;                           // of row g
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      if (i * RPS >= G) continue;                // warp-uniform
+      if (i * RPS >= n) continue;                // warp-uniform
       const int r = i * RPS + rr;
       float dot = 0.f;
-      if (r < G) {
+      if (r < n) {
         const uint32_t at = qt + r * (HD * 2) + ((ch ^ r) << 4);
         if constexpr (ROTATE) {
           const uint32_t x[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
@@ -258,7 +290,7 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float re = bf16_lo(x[e]), im = bf16_hi(x[e]);
-            const float y = re * cs[e] - im * sn[e], z = re * sn[e] + im * cs[e];
+            const float y = re * cs[i % NP][e] - im * sn[i % NP][e], z = re * sn[i % NP][e] + im * cs[i % NP][e];
             a[e] = pack_bf16(y, z);
             c[e] = pack_bf16(y - bf16_lo(a[e]), z - bf16_hi(a[e]));
             dot = fmaf(y, kf[2 * e], fmaf(z, kf[2 * e + 1], dot));
@@ -363,7 +395,8 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
     }
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    const size_t th = (size_t)b * p.nh + kvh * G + (g < G ? g : 0), at = th * p.parts + p.splits + part;
+    const int row = g < n ? g : 0;
+    const size_t th = (size_t)(b + (row >> p.gs)) * p.nh + kvh * G + (row & (G - 1)), at = th * p.parts + (sh ? 0 : p.splits) + part;
     float w_old = 1.f, w_new = 0.f;
     if (newest) {                                // one more key
       s_new *= p.scale_log2;
@@ -383,9 +416,9 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
         x = fmaf(w_new, bf16_lo(v), x * w_old);
         y = fmaf(w_new, bf16_hi(v), y * w_old);
       }
-      if (g < G && l != 0.f) *reinterpret_cast<float2*>(dst + 8 * e + 2 * t) = make_float2(x, y);
+      if (g < n && l != 0.f) *reinterpret_cast<float2*>(dst + 8 * e + 2 * t) = make_float2(x, y);
     }
-    if (g < G && t == 0) p.ml_part[at] = make_float2(m, l);
+    if (g < n && t == 0) p.ml_part[at] = make_float2(m, l);
     __syncwarp();                                // the next unit's queries take the place of the new values
   }
 }
@@ -395,8 +428,15 @@ __device__ __forceinline__ void px_own_keys(const PxParams& p, uint8_t* smem) {
 template <int HD>
 __global__ void __launch_bounds__(256, 1) prefix_own_kernel(const PxParams p) {
   extern __shared__ __align__(1024) uint8_t px_smem[];
-  px_own_keys<HD, false>(p, px_smem);
+  px_own_keys<HD, PX_PROMPT_OWN>(p, px_smem);
   pdl_wait();
+}
+
+// A step whose groups have up to eight queries of a key head: both sets of keys by warps.
+template <int HD>
+__global__ void __launch_bounds__(256, 1) prefix_rows_kernel(const PxParams p) {
+  extern __shared__ __align__(1024) uint8_t px_smem[];
+  px_own_keys<HD, PX_STEP_ALL>(p, px_smem);
 }
 
 template <int HD, bool ROTATE, int MODE>
@@ -425,7 +465,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
   const int G = 1 << p.gs;
   if constexpr (ROTATE) {
     if ((int)blockIdx.x >= (int)gridDim.x - p.own_ctas) {
-      px_own_keys<HD, true>(p, px_smem);
+      px_own_keys<HD, PX_STEP_OWN>(p, px_smem);
       return;
     }
   }
@@ -830,7 +870,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_const
 // is padding: without own keys, or without any, it gives zeros.
 template <int HD>
 __global__ void __launch_bounds__(256) prefix_join_kernel(const float* __restrict__ o_part, const float2* __restrict__ ml_part, __nv_bfloat16* out, int rows, int parts, int own) {
-  constexpr int V = HD / 32;                                           // columns of a lane
+  constexpr int V = HD / 32, AT_ONCE = 16;                             // columns of a lane, rows in flight
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
@@ -855,10 +895,10 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const float* __restric
   const float* src = o_part + (size_t)row * parts * HD + V * lane;
   float acc[V] = {};
 #pragma unroll 1
-  for (int i0 = 0; i0 < parts; i0 += 8) {                              // eight rows requested before the first is used
-    float x[8][V], f[8];
+  for (int i0 = 0; i0 < parts; i0 += AT_ONCE) {                        // that many rows requested before the first is used
+    float x[AT_ONCE][V], f[AT_ONCE];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < AT_ONCE; ++u) {
       const int i = i0 + u, k = i >> 5;
       f[u] = __shfl_sync(0xffffffffu, k == 0 ? w[0] : (k == 1 ? w[1] : w[2]), i & 31);
       if (i >= parts) f[u] = 0.f;
@@ -875,7 +915,7 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const float* __restric
       }
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
+    for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] = fmaf(f[u], x[u][e], acc[e]);
   }
@@ -911,12 +951,13 @@ static int px_launch(const PxParams& p, unsigned ctas, const CUtensorMap& pk, co
   return JL_OK;
 }
 
-template <int HD>
-static int px_own_launch(const PxParams& p, cudaStream_t st) {
+template <int HD, bool STEP>
+static int px_warps_launch(const PxParams& p, cudaStream_t st) {
   static std::atomic<uint64_t> set{0};
-  const int rc = px_smem_set(set, (const void*)prefix_own_kernel<HD>, PxOwn<HD>::SMEM);
+  void (*const kernel)(const PxParams) = STEP ? prefix_rows_kernel<HD> : prefix_own_kernel<HD>;
+  const int rc = px_smem_set(set, (const void*)kernel, PxOwn<HD>::SMEM);
   if (rc != JL_OK) return rc;
-  JL_CUDA(launch_pdl(prefix_own_kernel<HD>, dim3((unsigned)p.own_ctas), dim3(256), (size_t)PxOwn<HD>::SMEM, st, p));
+  JL_CUDA(launch_pdl(kernel, dim3((unsigned)p.own_ctas), dim3(256), (size_t)PxOwn<HD>::SMEM, st, p));
   return JL_OK;
 }
 
@@ -980,11 +1021,22 @@ static int px_splits(long queries, int groups, int nkv, int prefix, bool solo = 
 // A step: CTAs and parts for the own keys, splits for the shared keys.  The shared keys' CTAs come first in the grid and the own keys', a unit for every warp, take the
 // SMs that are left and those that get free: how full the caches are is known on the device alone, and an order that is right at any fill beats a division of the
 // SMs between the two (us on one B200, a division by estimate, the best of all divisions, this: 96 rows over 32768 shared 118, 118, 106; 48 rows x 32 heads, a
-// quarter full, 55, 41, 44; 4 x 16 rows over 3501 42, 42, 45; own keys first 135, 50, 42).  What is estimated is the count of splits alone, at half full caches.
+// quarter full, 55, 41, 44; 4 x 16 rows over 3501 42, 42, 45; own keys first 135, 50, 42; with two units a warp 124, 41, 55).  What is estimated is the count of splits alone, at half full caches.
 struct PxStep { int own_ctas, own_splits, splits; };
 static int px_own_splits(long items) {                                 // parts that give every warp of all SMs one
   const long s = (8l * PX_SMS + items - 1) / items;
   return (int)(s < 1 ? 1 : (s > PX_MAX_OWN ? PX_MAX_OWN : s));
+}
+// Up to eight queries of a (group, key head): they are rows of one mma.sync operand, and a warp per part of the keys moves them as fast as an SM can take them, where a tile
+// of 128 rows for tcgen05 would be all but empty.  Not where a few heads have long prefixes: one warp's part is then long, or the parts many.  us in a graph, tiles and
+// this: 8 rows x 32 heads with keys of their own over 1000 17.2, 11.8, over 4000 27, 18; 5 groups of 2 over 6070 132, 100; 8 groups of 2 rows, 8 key heads, over 1000 19.6, 13.0; one
+// such group over 100 10.0, 9.5, over 4000 13.2, 14.1; one key head over 19074 13, 17.
+static bool px_rows(int B, int groups, int nkv, int G, int P) { return B / groups * G <= 8 && (groups * nkv >= 16 || P <= 512); }
+// parts of 64 keys or more, at most one for every warp of the SMs
+static int px_rows_splits(int groups, int nkv, int P) {
+  const int most = (8 * PX_SMS + groups * nkv - 1) / (groups * nkv), by_keys = (P + 63) / 64;
+  const int s = most < by_keys ? most : by_keys;
+  return s > PX_MAX_SPLITS ? PX_MAX_SPLITS : s;
 }
 static PxStep px_step(int B, int groups, int nkv, int G, int hd, int P, int T) {
   PxStep r;
@@ -992,6 +1044,20 @@ static PxStep px_step(int B, int groups, int nkv, int G, int hd, int P, int T) {
   const int most = px_own_splits(items), by_keys = (T + 127) / 128;
   r.own_splits = most < by_keys ? most : by_keys;
   r.own_ctas = (int)((items * r.own_splits + 7) / 8);
+  if (px_rows(B, groups, nkv, G, P)) {
+    // us: 3 in and out of a unit, 13 KB/us of keys for a warp; the rounds of CTAs that all units make, half of the longest unit, the parts to join
+    const float heads = (float)groups * nkv, own = (float)items * r.own_splits, warps = 8.f * PX_SMS, key = (float)hd * 4.f / 13e3f;
+    const float own_us = 3.f + (float)T * 0.5f / (float)r.own_splits * key;
+    const int most = px_rows_splits(groups, nkv, P);
+    float best = 0.f;
+    for (int n = 1; n <= most; ++n) {
+      const float us = 3.f + (float)P / (float)n * key, units = heads * n + own;
+      const float c = (own * own_us + heads * n * us) / warps + 0.6f * fmaxf(us, own_us) + 1.3f * ceilf(units / warps) + 0.06f * n;
+      if (best == 0.f || c < best) { best = c; r.splits = n; }
+    }
+    r.own_ctas = (int)((items * r.own_splits + (long)groups * nkv * r.splits + 7) / 8);
+    return r;
+  }
   // us: 3 in and out of a unit, 55 KB/us of own keys for the 8 warps of an SM (what one SM draws under load); 0.9 a tile of shared keys and 1.25 for two tiles of
   // queries, 8 in and out of a CTA
   const float unit = 3.f + (float)T * 0.5f / (float)r.own_splits * (float)hd * 4.f * 8.f / 55e3f, tile = queries > PX_BM ? 1.25f : 0.9f;
@@ -1040,7 +1106,7 @@ extern "C" JL_API size_t jl_prefix_attn_scratch_bytes(int B, int S, int groups, 
   const PxPrompt plan = px_prompt(B, S, groups, nkv, G, prefix);
   int parts = plan.both ? (plan.splits > 1 ? plan.splits : 0) : plan.splits + 1;
   if (S == 1) {                                                        // either form of one token
-    const int step = px_splits((long)(B / groups) * G, groups, nkv, prefix) + px_own_splits((long)B * nkv);
+    const int step = (px_rows(B, groups, nkv, G, prefix) ? px_rows_splits(groups, nkv, prefix) : px_splits((long)(B / groups) * G, groups, nkv, prefix)) + px_own_splits((long)B * nkv);
     parts = parts > step ? parts : step;
   }
   if (parts == 0) return 16;                                           // (nothing is left in between; never nothing)
@@ -1078,7 +1144,7 @@ extern "C" JL_API int jl_decode_attn_prefix(const void* qkv, const void* prefix_
   if (rc != JL_OK) return rc;
   const PxStep plan = px_step(B, groups, nkv, G, hd, P, T);
   PxParams p{};
-  p.q = p.qkv = (const __nv_bfloat16*)qkv; p.ldq = (nh + 2 * nkv) * hd;
+  p.q = (const __nv_bfloat16*)qkv; p.ldq = (nh + 2 * nkv) * hd;
   p.k_cache = (__nv_bfloat16*)k_cache; p.v_cache = (__nv_bfloat16*)v_cache;
   p.cos_t = cos_t; p.sin_t = sin_t; p.max_pos = max_pos; p.cache_len = cache_len;
   p.prefix_len = prefix_len; p.prefix_pad = prefix_pad; p.pad_left = pad_left;
@@ -1088,7 +1154,12 @@ extern "C" JL_API int jl_decode_attn_prefix(const void* qkv, const void* prefix_
   p.scale_log2 = scale * 1.4426950408889634f;
   p.o_part = (float*)scratch;
   p.ml_part = (float2*)(p.o_part + (size_t)B * nh * p.parts * hd);
-  rc = px_dispatch(p, (long)rows * G, groups, true, hd, pk, pv, pk, pv, (cudaStream_t)stream);
+  if (px_rows(B, groups, nkv, G, P)) {
+    p.prefix_k = (const __nv_bfloat16*)prefix_k; p.prefix_v = (const __nv_bfloat16*)prefix_v;
+    rc = hd == 128 ? px_warps_launch<128, true>(p, (cudaStream_t)stream) : px_warps_launch<64, true>(p, (cudaStream_t)stream);
+  } else {
+    rc = px_dispatch(p, (long)rows * G, groups, true, hd, pk, pv, pk, pv, (cudaStream_t)stream);
+  }
   if (rc != JL_OK) return rc;
   return px_join(p, (__nv_bfloat16*)out, B * nh, hd, -1, (cudaStream_t)stream);
 }
@@ -1135,7 +1206,7 @@ extern "C" JL_API int jl_prefill_attn_prefix(const void* q, const void* prefix_k
   if (few) {
     p.k_cache = (__nv_bfloat16*)k_cache; p.v_cache = (__nv_bfloat16*)v_cache;            // (read only)
     p.B = B; p.own_splits = 1; p.own_ctas = (int)((units + 7) / 8);
-    rc = hd == 128 ? px_own_launch<128>(p, (cudaStream_t)stream) : px_own_launch<64>(p, (cudaStream_t)stream);
+    rc = hd == 128 ? px_warps_launch<128, false>(p, (cudaStream_t)stream) : px_warps_launch<64, false>(p, (cudaStream_t)stream);
     return rc != JL_OK ? rc : px_join(p, (__nv_bfloat16*)out, B * S * nh, hd, p.splits, (cudaStream_t)stream);
   }
   p.shared = 0; p.own = 1; p.part0 = p.splits; p.splits = 1;

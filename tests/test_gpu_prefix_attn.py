@@ -60,6 +60,13 @@ STEPS = [  # rows, groups, nh, nkv, hd, P, T, own keys, ragged
     (70, 2, 8, 4, 128, 300, 20, 5, True),
     (3, 1, 4, 4, 128, 1500, 700, 650, True),     # splits of both kinds
     (2, 1, 2, 1, 64, 3000, 1400, 1300, True),
+    (12, 1, 8, 4, 128, 1500, 700, 650, True),    # 24 queries of a key head, splits of both kinds
+    (30, 3, 4, 4, 64, 900, 200, 130, True),
+    (8, 1, 8, 8, 64, 2000, 30, 20, True),        # up to eight queries: rows of several tokens, angles of their own
+    (4, 2, 16, 4, 128, 700, 300, 250, True),
+    (6, 3, 8, 2, 64, 40, 500, 480, True),
+    (8, 4, 16, 4, 128, 600, 60, 50, True),
+    (10, 5, 16, 16, 64, 1300, 9, 0, True),
     (75, 1, 4, 1, 64, 1000, 12, 5, True),        # 300 queries of a key head: a pair of tiles and one tile that is not full
     (100, 1, 4, 1, 128, 700, 20, 11, False),     # 400: two pairs, the last tile with 16 queries
     (66, 2, 16, 2, 128, 520, 9, 0, True),        # 264: the second pair has eight queries
