@@ -875,17 +875,20 @@ class B200Engine:
         return st.sequences.to(torch.long)
 
     # Own copies of shared keys, in bytes that a step of a layer reads for them, from which on they are held once for all rows; with the whole-step kernel for up to
-    # four rows, which reads own keys alone.  ms a token behind one prompt on one B200, keys of copies -> together: 8 layers 4096 wide (8 key heads of 128), 16 answers to
-    # 128 tokens (8 MB) 0.78 -> 0.83, to 1024 (63 MB) 1.16 -> 0.86; 4 answers by the whole-step kernel to 1024 (13 MB) 0.84 -> 1.24, to 4096 (50 MB) 1.14 -> 1.22; 8 layers
-    # 2048 wide (4 of 64), 8 answers to 1024 (7 MB) 0.377 -> 0.387, to 4096 (29 MB) 0.424 -> 0.411, 16 to 1024 (16 MB) 0.393 -> 0.406, to 4096 (63 MB) 0.492 -> 0.432.
-    share_above, share_above_whole_step = 20 << 20, 56 << 20
+    # four rows, which reads own keys alone, by the length of the prefix.  ms a token behind one prompt on one B200, copies and together: 8 layers 4096 wide (8 key heads
+    # of 128), 16 answers to 128 tokens (8 MB) 0.79, 0.85, to 1024 (63 MB) 0.87, 0.86, to 4096 1.13, 0.89; 4 answers by the whole-step kernel to 1024 0.84, 1.19, to 4096
+    # 0.97, 1.25; 8 layers 2048 wide (4 of 64), 16 answers to 1024 (16 MB) 0.398, 0.410, to 4096 0.468, 0.428, 8 to 4096 (29 MB) 0.422, 0.409, 4 to 1024 0.563, 0.584, to 4096
+    # 0.597, 0.606 (the lines cross at 5000 to 11000 tokens).
+    share_above, share_above_whole_step = 28 << 20, 8192
     shares_prefixes = True                       # engines whose layers hold anything else per row say no
 
     def _together(self, rows: int, groups: int, P: int) -> bool:
         """Whether `rows` rows behind `groups` prefixes of P tokens take the attention over shared keys, not copies of them."""
-        whole_step = rows <= 4 and self._mega_fits(rows)
-        copies = (rows - groups) * P * self.nkv * self.hd * 4
-        return self._shared_attention() and copies >= (self.share_above_whole_step if whole_step else self.share_above)
+        if not self._shared_attention():
+            return False
+        if rows <= 4 and self._mega_fits(rows):
+            return P >= self.share_above_whole_step
+        return (rows - groups) * P * self.nkv * self.hd * 4 >= self.share_above
 
     def _shared_attention(self) -> bool:
         return self.hd in (64, 128) and self.nh // self.nkv in (1, 2, 4, 8)
