@@ -1138,10 +1138,6 @@ extern "C" JL_API int jl_decode_attn_prefix(const void* qkv, const void* prefix_
   JL_CHECK_ARG(cache_len != nullptr && max_pos >= 1, "jl_decode_attn_prefix: the slot of the new token and its tables are required");
   const int G = nh / nkv, rows = B / groups;
   JL_CHECK_ARG((long)B * nh < (1l << 26), "jl_decode_attn_prefix: %d rows of %d heads", B, nh);
-  CUtensorMap pk, pv;
-  int rc = make_tmap_3d_bf16(&pk, prefix_k, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
-  if (rc == JL_OK) rc = make_tmap_3d_bf16(&pv, prefix_v, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
-  if (rc != JL_OK) return rc;
   const PxStep plan = px_step(B, groups, nkv, G, hd, P, T);
   PxParams p{};
   p.q = (const __nv_bfloat16*)qkv; p.ldq = (nh + 2 * nkv) * hd;
@@ -1154,11 +1150,15 @@ extern "C" JL_API int jl_decode_attn_prefix(const void* qkv, const void* prefix_
   p.scale_log2 = scale * 1.4426950408889634f;
   p.o_part = (float*)scratch;
   p.ml_part = (float2*)(p.o_part + (size_t)B * nh * p.parts * hd);
+  int rc;
   if (px_rows(B, groups, nkv, G, P)) {
     p.prefix_k = (const __nv_bfloat16*)prefix_k; p.prefix_v = (const __nv_bfloat16*)prefix_v;
     rc = hd == 128 ? px_warps_launch<128, true>(p, (cudaStream_t)stream) : px_warps_launch<64, true>(p, (cudaStream_t)stream);
   } else {
-    rc = px_dispatch(p, (long)rows * G, groups, true, hd, pk, pv, pk, pv, (cudaStream_t)stream);
+    CUtensorMap pk, pv;
+    rc = make_tmap_3d_bf16(&pk, prefix_k, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
+    if (rc == JL_OK) rc = make_tmap_3d_bf16(&pv, prefix_v, (uint64_t)groups * nkv, P, hd, (uint64_t)P * hd, hd, PX_BN);
+    if (rc == JL_OK) rc = px_dispatch(p, (long)rows * G, groups, true, hd, pk, pv, pk, pv, (cudaStream_t)stream);
   }
   if (rc != JL_OK) return rc;
   return px_join(p, (__nv_bfloat16*)out, B * nh, hd, -1, (cudaStream_t)stream);
