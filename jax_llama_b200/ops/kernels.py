@@ -478,7 +478,7 @@ def decode_attn_prefix(qkv: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torc
             or cos.get_device() != dev or sin.get_device() != dev:
         raise ValueError(f"{who}: cos/sin tables are fp32 [positions, {hd // 2}] on {qkv.device}")
     if scratch is None:
-        scratch = prefix_attn_scratch(B, 1, groups, nh, nkv, hd, P, qkv.device)
+        scratch = prefix_attn_scratch(max(B, groups), 1, groups, nh, nkv, hd, P, qkv.device)
     if out is None:
         out = qkv.new_empty((B, nh * hd))
     else:
@@ -513,7 +513,7 @@ def prefill_attn_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch
         return _prefix_attn_ref(q, prefix_k, prefix_v, k_cache[:, :, :start + S], v_cache[:, :, :start + S], start + torch.arange(S), pad_left, lo, hi)
     _bf16c(q, "q")
     if scratch is None:
-        scratch = prefix_attn_scratch(B, max(S, 1), groups, nh, nkv, hd, P, q.device)
+        scratch = prefix_attn_scratch(max(B, groups), max(S, 1), groups, nh, nkv, hd, P, q.device)
     if out is None:
         out = q.new_empty((B, S, nh * hd))
     else:

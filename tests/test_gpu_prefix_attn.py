@@ -248,3 +248,31 @@ def test_workspaces_and_devices_are_refused(monkeypatch):
     for f in (lambda: call(d), lambda: K.constrain_logits(torch.zeros(1, 8, device=DEV))):
         with pytest.raises(ValueError, match="current device"):
             f()
+
+
+@pytest.mark.gpu
+def test_no_rows_and_no_tokens():
+    d = small(DEV)
+    none = dict(d, qkv=d["qkv"][:0], kc=d["kc"][:0].contiguous(), vc=d["vc"][:0].contiguous(), pad_left=None)
+    assert call(none).shape == (0, 256)
+    q = torch.empty(3, 0, 4, 64, dtype=torch.bfloat16, device=DEV)
+    assert K.prefill_attn_prefix(q, d["pk"], d["pv"], d["kc"], d["vc"], 0, 0, None, None, None).shape == (3, 0, 256)
+
+
+@pytest.mark.gpu
+def test_another_stream_than_the_tensors_own():
+    """Work queued on a stream of its own behind the copies that fill its inputs."""
+    d = small(DEV, B=40, T=300)
+    want = call(dict(d, kc=d["kc"].clone(), vc=d["vc"].clone()))
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        late = {k: (v.clone() if torch.is_tensor(v) else v) for k, v in d.items()}
+        late["qkv"].zero_()
+        late["qkv"].copy_(d["qkv"])
+        got = call(late)
+        q = torch.randn(40, 6, 4, 64, device=DEV).to(torch.bfloat16)
+        one = K.prefill_attn_prefix(q, d["pk"], d["pv"], d["kc"], d["vc"], 3, 6, d["pad_left"], None, None)
+    s.synchronize()
+    assert torch.equal(got, want)
+    assert torch.equal(one, K.prefill_attn_prefix(q, d["pk"], d["pv"], d["kc"], d["vc"], 3, 6, d["pad_left"], None, None))
