@@ -18,13 +18,14 @@
 // scores in registers, exponentials in base 2 against a reference that is raised only when it has grown by 2^8.
 // Queries go to shared memory by hand: rows of different tokens and heads follow each other in a tile, and the one-token form rotates them on the way.
 // A rotated query is kept as two bfloat16 numbers, hi + lo (two products into the same scores): rounded to one, a score of size s would be off by
-// s 2^-8 and the result by as much again as its own rounding.  Probabilities are rounded to bfloat16 (2^-8 of each weight, sums in fp32) where a launch has
-// more than one tile of queries; with one tile, where the products have time to spare, they are hi + lo too.
+// s 2^-8 and the result by as much again as its own rounding.  Probabilities of a step are hi + lo too, as in decode_attn_fused.cu, so that a row's result
+// has the same bits however many rows share the keys.  Those of prompts are where a launch has one tile of queries and the products have time to spare; with
+// more they are rounded to bfloat16 (2^-8 of each weight, sums in fp32), as flash_prefill.cu rounds those of the same rows written out.
 // Slots that hold no key may hold anything: their scores are masked, and their value rows are cleared in shared memory, because a weight of zero
 // times a NaN is a NaN.
 //
-// One B200, us a call in a graph: one token, 16 rows x 32 heads over 8 of keys, 2048 shared 12.7; 96 rows, 32768 shared and 500 own each 106 (790 TFLOP/s with the
-// second products of the queries, 3.1 TB/s beside them); 4 x 16 rows, 3501 shared and 701 own 44 (5.5 TB/s).  Prompts: 2 x 2048 tokens over 16384 1065 (1080 TFLOP/s; a
+// One B200, us a call in a graph: one token, 16 rows x 32 heads over 8 of keys, 2048 shared 12.7; 96 rows, 32768 shared and 500 own each 122 (860 TFLOP/s with the
+// second products of queries and probabilities, 2.7 TB/s beside them); 4 x 16 rows, 3501 shared and 701 own 44 (5.5 TB/s).  Prompts: 2 x 2048 tokens over 16384 1065 (1080 TFLOP/s; a
 // single launch of its own 906 and 1290: the power cap), 8 x 333 over 1500 68 (1110), 16 x 48 over 8192 111 (920).  What bounds them: products of small width
 // (a 128 x 64 tile of scores reads its queries from shared memory, 384 cycles for 256 of products) and the exponentials, half of the special-function
 // unit's rate with a quarter of them on the FMA units; in short calls the chain launch, queries, scores, last rows, join.
@@ -113,7 +114,7 @@ struct PxParams {
   // the last `own_ctas` CTAs of a step, or a launch of their own, take the own keys, `own_splits` parts of every (token, key head)
   const __nv_bfloat16* prefix_k; const __nv_bfloat16* prefix_v; __nv_bfloat16* k_cache; __nv_bfloat16* v_cache;
   int own_ctas, own_splits, B, tiles_q;
-  int p_low;                        // one tile of queries: probabilities as two bfloat16 numbers
+  int p_low;                        // a step, or one tile of queries: probabilities as two bfloat16 numbers
   float scale_log2;
 };
 
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(PxTile<HD, ROTATE, MODE>::THREADS, MODE == PX_
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv,
                    const __grid_constant__ CUtensorMap tm_ok, const __grid_constant__ CUtensorMap tm_ov, const PxParams p) {
   using Tile = PxTile<HD, ROTATE, MODE>;
-  constexpr bool PAIR = Tile::PAIR, SOLO = Tile::SOLO, JOINT = Tile::JOINT, LOW = !JOINT;      // LOW: probabilities may have low parts
+  constexpr bool PAIR = Tile::PAIR, SOLO = Tile::SOLO, JOINT = Tile::JOINT, LOW = !JOINT || ROTATE;      // LOW: probabilities may have low parts
   constexpr int HALVES = Tile::HALVES, NQ = Tile::NQ, SLOTS = Tile::SLOTS;
   extern __shared__ __align__(1024) uint8_t px_smem[];
   const uint32_t raw = tc::smem_u32(px_smem);
@@ -983,7 +984,7 @@ static int px_dispatch(PxParams p, long queries, int units, bool rotate, int hd,
   const bool solo = !rotate && (queries <= PX_BM ? pairs > PX_SMS : tiles <= (2 * pairs <= PX_SMS ? 20.f : 8.f));
   const int mode = solo ? PX_SOLO : (queries > PX_BM ? PX_PAIR : PX_TURNS);
   p.tiles_q = solo ? (int)((queries + PX_BM - 1) / PX_BM) : (int)px_tiles(queries);
-  p.p_low = queries <= PX_BM;
+  p.p_low = rotate || queries <= PX_BM;
   const long ctas = p.own_ctas + (long)p.tiles_q * p.splits * p.nkv * units;
   JL_CHECK_ARG(ctas < (1l << 31), "attention over a shared prefix: %ld tiles", ctas);
 #define JL_PX(HD_, R_, M_) if (hd == HD_ && rotate == R_ && mode == M_) return px_launch<HD_, R_, M_>(p, (unsigned)ctas, pk, pv, ok, ov, st);
@@ -1020,7 +1021,7 @@ static int px_splits(long queries, int groups, int nkv, int prefix, bool solo = 
 
 // A step: CTAs and parts for the own keys, splits for the shared keys.  The shared keys' CTAs come first in the grid and the own keys', a unit for every warp, take the
 // SMs that are left and those that get free: how full the caches are is known on the device alone, and an order that is right at any fill beats a division of the
-// SMs between the two (us on one B200, a division by estimate, the best of all divisions, this: 96 rows over 32768 shared 118, 118, 106; 48 rows x 32 heads, a
+// SMs between the two (us on one B200, a division by estimate, the best of all divisions, this: 96 rows over 32768 shared, with probabilities of one number, 118, 118, 106; 48 rows x 32 heads, a
 // quarter full, 55, 41, 44; 4 x 16 rows over 3501 42, 42, 45; own keys first 135, 50, 42; with two units a warp 124, 41, 55).  What is estimated is the count of splits alone, at half full caches.
 struct PxStep { int own_ctas, own_splits, splits; };
 static int px_own_splits(long items) {                                 // parts that give every warp of all SMs one
@@ -1058,9 +1059,9 @@ static PxStep px_step(int B, int groups, int nkv, int G, int hd, int P, int T) {
     r.own_ctas = (int)((items * r.own_splits + (long)groups * nkv * r.splits + 7) / 8);
     return r;
   }
-  // us: 3 in and out of a unit, 55 KB/us of own keys for the 8 warps of an SM (what one SM draws under load); 0.9 a tile of shared keys and 1.25 for two tiles of
-  // queries, 8 in and out of a CTA
-  const float unit = 3.f + (float)T * 0.5f / (float)r.own_splits * (float)hd * 4.f * 8.f / 55e3f, tile = queries > PX_BM ? 1.25f : 0.9f;
+  // us: 3 in and out of a unit, 55 KB/us of own keys for the 8 warps of an SM (what one SM draws under load); 0.9 a tile of shared keys and 1.45 for two tiles of
+  // queries (64 rows x 32 heads over 4096 by splits for 1.25: 32, for this 29.5), 8 in and out of a CTA
+  const float unit = 3.f + (float)T * 0.5f / (float)r.own_splits * (float)hd * 4.f * 8.f / 55e3f, tile = queries > PX_BM ? 1.45f : 0.9f;
   const int tiles = (P + PX_BN - 1) / PX_BN, cap = px_splits(queries, groups, nkv, P);       // (what the scratch is sized for)
   const bool half = queries > PX_BM && (queries % (2 * PX_BM) <= PX_BM && queries % (2 * PX_BM) != 0);
   const float heads = (float)(groups * nkv), work = heads * ((float)px_tiles(queries) - (half ? 0.22f : 0.f)) * (float)tiles * tile + (float)r.own_ctas * unit;
