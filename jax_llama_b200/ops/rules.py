@@ -89,7 +89,7 @@ class LogitRules:
         if torch.is_tensor(a):
             if a.dtype != torch.int32 or a.dim() not in (1, 2) or a.shape[-1] != words or (a.dim() == 2 and a.shape[0] not in (1, rows)):
                 raise ValueError(f"allowed_tokens: masks are int32 [{words}] or [{rows}, {words}] (got {a.dtype}, {tuple(a.shape)})")
-            m = a.view(-1, words)
+            m = a.reshape(-1, words).clone()                 # the caller's stays the caller's: later batches and steps write into what is bound
         else:
             a = list(a)
             nested = len(a) > 0 and not isinstance(a[0], Integral)

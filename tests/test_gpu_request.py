@@ -216,3 +216,21 @@ def test_copies_of_another_length_take_their_own_keys():
         logits = ref.forward(tree32, cfg, got).logits[:, n - 1:-1]
         gap = logits.amax(-1) - logits.gather(-1, got[:, n:, None])[..., 0]
         assert torch.equal(got[:, :n], ids.repeat_interleave(4 // rows, 0)) and (gap <= 6e-2 * logits.abs().amax()).all()
+
+
+@pytest.mark.parametrize("graph", [True, False])
+@pytest.mark.parametrize("shape", [(32,), (1, 32), (3, 32)])
+def test_masks_on_the_device_stay_the_callers(graph, shape):
+    """Batches of the same form with masks that lie on the engine's device: each chooses from its own, and no mask is written over."""
+    cfg, _, eng = make("gqa128", use_cuda_graph=graph)
+    sets = [set(range(100, 120)), set(range(500, 520)), {7}]
+    a, b, c = (allowed_mask(s, 1000).expand(shape).clone().cuda() for s in sets)
+    was = [t.clone() for t in (a, b, c)]
+    run = lambda m, seed: eng.generate(ids_of(3, 6, 2).cuda(), None, max_length=14, do_sample=True, top_k=0, eos_token_id=-1, seed=seed, rules=LogitRules(allowed_tokens=m))  # noqa: E731
+    first = run(a, 1)
+    for mask, allowed in ((b, sets[1]), (a, sets[0])):
+        assert set(run(mask, 1)[:, 6:].flatten().tolist()) <= allowed
+    assert torch.equal(run(a, 1), first)
+    stream = eng.begin_stream(ids_of(3, 6, 2).cuda(), None, max_length=14, rules=LogitRules(allowed_tokens=b))
+    assert stream.step(allowed=c.view(-1, 32)).tolist() == [7, 7, 7]
+    assert all(torch.equal(t, w) for t, w in zip((a, b, c), was))

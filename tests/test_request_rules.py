@@ -163,3 +163,15 @@ def test_attention_on_the_cpu_path(full):
     want, _ = oracle.attention(turned[:, None, :nh], pk, pv, k2, v2, [own], pad, plen, ppad)
     assert (got.double().view_as(want) - want).abs().max() < 1e-5
     assert torch.equal(kc, was) if full else not torch.equal(kc, was)
+
+
+@pytest.mark.parametrize("shape", [(2,), (1, 2), (3, 2)])
+def test_bound_masks_are_not_the_callers(shape):
+    """What a request brings stays what it is: neither a later batch of the same form nor a mask of a step is written into it, and its own changes do not reach a batch at work."""
+    mask = allowed_mask([1, 39], 40).expand(shape).clone()
+    was, bound = mask.clone(), LogitRules(allowed_tokens=mask).bind(3, 40, "cpu")
+    bound.copy_(LogitRules(allowed_tokens=torch.zeros_like(mask)).bind(3, 40, "cpu"))
+    assert torch.equal(mask, was) and not bound.allowed.any()
+    bound = LogitRules(allowed_tokens=mask).bind(3, 40, "cpu")
+    mask.zero_()
+    assert torch.equal(bound.allowed, was.view(-1, 2))
