@@ -61,7 +61,11 @@ __global__ void __launch_bounds__(TH, 1024 / TH) logit_rules_kernel(const RulesP
   const int start = p.starts ? max(p.starts[p.starts_n > 1 ? b : 0], 0) : 0;
   const int prompt = p.prompts ? p.prompts[p.prompts_n > 1 ? b : 0] : 0;
   const float r = p.rep ? p.rep[b] : p.rep1, f = p.freq ? p.freq[b] : p.freq1, pr = p.pres ? p.pres[b] : p.pres1;
-  const float inv_r = __fdividef(1.0f, r);
+  // v / r as v (1 / r) in 64 bits, rounded once to 32, over the whole range of r.  It is v / r rounded: with v = m 2^i, r = n 2^j (m, n < 2^24 whole) a midpoint M 2^l of two fp32
+  // numbers (M < 2^25, odd) is v / r only if M divides m, which is smaller; otherwise |m 2^.. - M n 2^..| >= 1 keeps v / r 2^-49 of its size away, and the two roundings
+  // in 64 bits are 2^-52 together.  (Below 2^-126 midpoints are shorter, and the last bit may be the other one.)  us of the calls above, 1, 17, 96 rows, on one box: a division in fp32
+  // 2.55, 5.9, 30.1; this 2.24, 5.45, 29.7.
+  const double inv_r = 1.0 / (double)r;
   const int* row = p.tokens + (size_t)b * p.ldt;
   // history: AHEAD groups of four tokens per thread before its length is known, each on a 16-byte boundary (the first up to three tokens in front of the row)
   constexpr int AHEAD = 2;
@@ -171,9 +175,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) logit_rules_kernel(const RulesP
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned n = c[e] & LR_COUNT;
-          // v / r as q = v (1 / r), a few last bits off, and one step with the remainder v - q r, which a fused product gives exactly; infinite quotients have none
-          const float a = v[k][e], q = a * inv_r;
-          const float pen = a > 0.f ? (q < INFINITY ? fmaf(fmaf(-q, r, a), inv_r, q) : q) : a * r;
+          const float quo = (float)((double)v[k][e] * inv_r), pen = v[k][e] > 0.f ? quo : v[k][e] * r;
           if (c[e] & (LR_COUNT | LR_SAID)) v[k][e] = pen;
           if (n) v[k][e] = v[k][e] - f * (float)n - pr;
           if (c[e] & LR_BIAS) v[k][e] += lr_value[4 * (k * TH + t) + e];

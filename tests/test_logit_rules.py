@@ -164,3 +164,16 @@ def test_a_captured_call_follows_the_text():
         g.replay()
         assert torch.equal(out, K.constrain_logits(x, **kw))
         assert (out != x).any().item() == (k > 0)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("r", [1e-45, 1e-40, 2.0 ** -127, 0.3, 1.7, 2.0 ** 126, 2.0 ** 127, 3.4e38, math.inf])
+def test_a_penalty_divides(r, dev):
+    """x / r and x r as fp32 has them, each rounded once, over the whole range of penalties and logits."""
+    x = torch.cat([torch.randn(200, generator=torch.Generator().manual_seed(5)) * 10.0 ** torch.arange(-40, 40).repeat_interleave(5)[:200].float(),
+                   torch.tensor([1.0, 7.5, 3e38, 1e-45, math.inf, -1.0, -7.5, -3e38, -1e-45])])[None].float()
+    want = torch.where(x > 0, x / torch.tensor(r), x * torch.tensor(r))
+    tokens = torch.arange(x.shape[1], dtype=torch.int32)[None]
+    for rep in (r, torch.tensor([r], device=dev)):
+        got = K.constrain_logits(x.to(dev), tokens=tokens.to(dev), prompt_lengths=torch.tensor([x.shape[1]], dtype=torch.int32, device=dev), repetition=rep).cpu()
+        assert torch.equal(got.nan_to_num(nan=123.0, posinf=math.inf, neginf=-math.inf), want.nan_to_num(nan=123.0, posinf=math.inf, neginf=-math.inf))
