@@ -39,5 +39,9 @@ def sample(logits: torch.Tensor, temperature: float = 1.0, top_k: Optional[int] 
     """[B, V] logits → [B] token ids.  temperature == 0 selects greedy argmax (generation.py:34)."""
     if temperature == 0.0:
         return logits.float().argmax(dim=-1)
-    probs = torch.softmax(filter_logits(logits, temperature, top_k, top_p), dim=-1)
+    x = filter_logits(logits, temperature, top_k, top_p)
+    # nothing is left of a row: token 0, as with the arg-max and in csrc/sample_full.cu
+    none = torch.isneginf(x.amax(dim=-1, keepdim=True)) & (torch.arange(x.shape[-1], device=x.device) == 0)
+    x = x.masked_fill(none, 0.0)
+    probs = torch.softmax(x, dim=-1)
     return torch.multinomial(probs, 1, generator=generator).squeeze(-1)

@@ -234,3 +234,19 @@ def test_masks_on_the_device_stay_the_callers(graph, shape):
     stream = eng.begin_stream(ids_of(3, 6, 2).cuda(), None, max_length=14, rules=LogitRules(allowed_tokens=b))
     assert stream.step(allowed=c.view(-1, 32)).tolist() == [7, 7, 7]
     assert all(torch.equal(t, w) for t, w in zip((a, b, c), was))
+
+
+@pytest.mark.parametrize("top_k,top_p", [(0, 1.0), (50, 1.0), (0, 0.9), (49, 0.9)])
+def test_a_row_without_a_token_left_takes_the_first(top_k, top_p):
+    """Sampling from masks that leave nothing: token 0, as on the CPU, and the other rows as they would be."""
+    from jax_llama_b200.ops import kernels as K
+    cfg, _, eng = make("gqa128")
+    kw = dict(max_length=10, do_sample=True, top_k=top_k, top_p=top_p, eos_token_id=-1, seed=2)
+    ids = ids_of(2, 5, 1).cuda()
+    assert not eng.generate(ids, None, rules=LogitRules(allowed_tokens=[]), **kw)[:, 5:].any()
+    one = eng.generate(ids, None, rules=LogitRules(allowed_tokens=[[], range(400, 600)]), **kw)[:, 5:].tolist()
+    assert one[0] == [0] * 5 and all(400 <= t < 600 for t in one[1])
+    assert one[1] == eng.generate(ids, None, rules=LogitRules(allowed_tokens=[range(1000), range(400, 600)]), **kw)[1, 5:].tolist()
+    for vocab in (1, 33, 1000, 20001, 128256):
+        x = torch.full((2, vocab), -float("inf"), device="cuda")
+        assert K.sample_full(x, temperature=0.7, top_k=top_k, top_p=top_p, seed=5).tolist() == [0, 0]

@@ -175,3 +175,13 @@ def test_bound_masks_are_not_the_callers(shape):
     bound = LogitRules(allowed_tokens=mask).bind(3, 40, "cpu")
     mask.zero_()
     assert torch.equal(bound.allowed, was.view(-1, 2))
+
+
+@pytest.mark.parametrize("top_k,top_p", [(0, 1.0), (50, 1.0), (0, 0.9), (50, 0.9)])
+def test_a_row_without_a_token_left_takes_the_first(model, top_k, top_p):
+    """Sampling from masks that leave nothing, or nothing in one row: token 0 as with the arg-max and on the GPU, the other rows as they would be."""
+    ids, kw = prompts(2, 5, 1), dict(max_new_tokens=4, do_sample=True, top_k=top_k, top_p=top_p, eos_token_id=-5, seed=2)
+    assert not model.generate(ids, rules=LogitRules(allowed_tokens=[]), **kw).sequences[:, 5:].any()
+    one = model.generate(ids, rules=LogitRules(allowed_tokens=[[], range(40, 60)]), **kw).sequences[:, 5:]
+    assert not one[0].any() and set(one[1].tolist()) <= set(range(40, 60))
+    assert torch.equal(one[1], model.generate(ids, rules=LogitRules(allowed_tokens=[range(300), range(40, 60)]), **kw).sequences[1, 5:])
