@@ -456,7 +456,7 @@ def decode_attn_prefix(qkv: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torc
     _rows(prefix_len, groups, dev, "prefix_len"); _rows(prefix_pad, groups, dev, "prefix_pad")
     if dev < 0:
         lo, hi = _prefix_counts(prefix_len, prefix_pad, groups, P)
-        slot = min(int(cache_len.item()), T)
+        slot = min(max(int(cache_len.item()), 0), T)
         x = qkv.view(B, nh + 2 * nkv, hd)
         pos = (hi - lo).clamp(min=0).repeat_interleave(B // groups) + slot
         if pad_left is not None:

@@ -276,3 +276,12 @@ def test_another_stream_than_the_tensors_own():
     s.synchronize()
     assert torch.equal(got, want)
     assert torch.equal(one, K.prefill_attn_prefix(q, d["pk"], d["pv"], d["kc"], d["vc"], 3, 6, d["pad_left"], None, None))
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(DEV, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("count", [-4, -1, -1000])
+def test_a_negative_count_is_slot_0(count, dev):
+    """On either side: the result and both caches are those of a call at slot 0."""
+    c, d = small(dev), small(dev)
+    got, want = (call(t, cache_len=torch.tensor([n], dtype=torch.int32, device=dev)) for t, n in ((c, count), (d, 0)))
+    assert torch.equal(got, want) and torch.equal(c["kc"], d["kc"]) and torch.equal(c["vc"], d["vc"])
