@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import logging
 import os
+import weakref
 from dataclasses import dataclass, field
 from typing import Any, Dict, List, Optional, Tuple
 
@@ -39,7 +40,7 @@ Tree = Dict[str, Any]
 class SharedPrefix:
     """Keys and values in front of the rows of a batch, held once per group of neighbouring rows."""
 
-    k: torch.Tensor                             # [L, groups, nkv, P, hd]
+    k: torch.Tensor                             # [L, groups, nkv, slots, hd]
     v: torch.Tensor
     length: torch.Tensor                        # int32 [groups]: shared keys lie in slots [pad, length)
     pad: torch.Tensor                           # int32 [groups]
@@ -110,6 +111,9 @@ class DecodeState:
     ruled: Optional[torch.Tensor] = None
     prompt_len: Optional[torch.Tensor] = None
     seq_pad: Optional[torch.Tensor] = None
+    # behind shared prefixes: their length in the batch at work, and the stream that works on it
+    prefix_len: int = 0
+    stream: Optional["weakref.ref[EngineStream]"] = None
 
 
 class B200Engine:
@@ -144,7 +148,7 @@ class B200Engine:
         self.v_local = lm_head.shape[0]
         cos, sin = rope_cos_sin(self.hd, 2 * config.max_sequence_length, config.rope_theta)
         self.cos, self.sin = cos.to(self.device), sin.to(self.device)
-        self._decode_states: Dict[Tuple[int, int], DecodeState] = {}
+        self._decode_states: Dict[Tuple[int, ...], DecodeState] = {}
         self.warned_slow_prefill = False
         self._mega_fit_cache: Dict[int, bool] = {}
         # step counter of the whole-step decode kernel: the base of its packet tags (never reset, see decode_mega.cu)
@@ -483,7 +487,8 @@ class B200Engine:
         graphs = self.__dict__.setdefault("_sp_graphs", {})
         # the graph bakes the addresses of the cache tensors: all of them are part of the key, so a later cache object
         # that happens to reuse one address can never pick up a graph that points at freed memory
-        key = (cache.k.data_ptr(), cache.v.data_ptr(), cache.len_dev.data_ptr(), cache.pad_left.data_ptr(), B, S, cache.index)
+        # (and their slots per row, which the strides come from)
+        key = (cache.k.data_ptr(), cache.v.data_ptr(), cache.len_dev.data_ptr(), cache.pad_left.data_ptr(), B, S, cache.index, cache.capacity)
         ent = graphs.get(key)
         if ent is None:
             while len(graphs) >= 4:                # each graph owns its activations: keep a handful
@@ -635,10 +640,14 @@ class B200Engine:
 
     # ------------------------------------------------------------------ decode state + graph
     def _decode_state(self, B: int, max_len: int, shared: Tuple[int, ...] = ()) -> DecodeState:
-        """`shared`: (groups, P) of a batch behind shared prefixes."""
+        """`shared`: (groups, slots) of a batch behind shared prefixes."""
         key = (B, max_len, *shared)
         if key in self._decode_states:
+            if shared:
+                self._decode_states[key] = self._decode_states.pop(key)          # used last
             return self._decode_states[key]
+        if shared:
+            self._make_room(B, max_len, *shared)
         c, dev = self.config, self.device
         i32 = dict(dtype=torch.int32, device=dev)
         bf = dict(dtype=torch.bfloat16, device=dev)
@@ -893,6 +902,41 @@ class B200Engine:
     def _shared_attention(self) -> bool:
         return self.hd in (64, 128) and self.nh // self.nkv in (1, 2, 4, 8)
 
+    # Decode states behind shared prefixes are kept for the next batch of their sizes: this many, and with this part of the device's memory in keys and values.
+    kept_shared, kept_shared_part = 4, 0.125
+
+    @staticmethod
+    def _shared_slots(P: int) -> Tuple[int, int]:
+        """(slots for P shared keys, the smallest P with as many): steps of 64, of an eighth of P's power of two from 1024 on.  The number of keys is read from the device, so lengths
+        up to a step apart take the same caches and captured step."""
+        step = max(64, 1 << max((P - 1).bit_length() - 4, 0))
+        slots = (P + step - 1) // step * step
+        return slots, slots - step + 1
+
+    def _own_slots(self, max_len: int, slots: int) -> int:
+        """Slots for the own keys of rows behind any prefix that takes `slots`."""
+        return max(max_len - self._shared_slots(slots)[1], 1)
+
+    def _make_room(self, B: int, max_len: int, groups: int, slots: int) -> None:
+        """States of other shared prefixes go, the one unused for longest first, until a new one finds room.  (A stream at work holds its own and goes on.)"""
+        per_slot = 4 * self.config.num_hidden_layers * self.nkv * self.hd
+        held = {key: per_slot * (key[0] * self._own_slots(key[1], key[3]) + key[2] * key[3]) for key in (*self._decode_states, (B, max_len, groups, slots)) if len(key) > 2}
+        room = self.kept_shared_part * torch.cuda.get_device_properties(self.device).total_memory
+        for key in list(held)[:-1]:
+            if len(held) <= self.kept_shared and sum(held.values()) <= room:
+                break
+            del held[key], self._decode_states[key]
+
+    def _shared_state(self, B: int, max_len: int, groups: int, P: int) -> DecodeState:
+        """The decode state of a batch behind prefixes of P tokens.  One on which a stream behind prefixes of another length is at work stays that stream's."""
+        shared = (groups, self._shared_slots(P)[0])
+        st = self._decode_states.get((B, max_len, *shared))
+        if st is not None and st.prefix_len != P and st.stream is not None and st.stream() is not None:
+            del self._decode_states[(B, max_len, *shared)]
+        st = self._decode_state(B, max_len, shared)
+        st.prefix_len = P
+        return st
+
     def _begin(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], max_length: int, pad: int, rules: Optional[LogitRules], repeat: int,
                prefix_ids: Optional[torch.Tensor], prefix_mask: Optional[torch.Tensor], logit_rows: Optional[torch.Tensor] = None
                ) -> Tuple[DecodeState, DeviceKVCache, int]:
@@ -926,27 +970,30 @@ class B200Engine:
             cache = self.prepare(st, ids.repeat_interleave(repeat, 0), None if mask is None else mask.repeat_interleave(repeat, 0), pad)
         else:
             together = not dense or self._together(B, groups, P)
-            st = self._decode_state(B, max_length, (int(groups), int(P)) if together else ())
+            st = self._shared_state(B, max_length, int(groups), int(P)) if together else self._decode_state(B, max_length)
             cache = self._prepare_shared(st, input_ids, attention_mask, pad, repeat, prefix_ids, prefix_mask, together)
         self._set_rules(st, rules, total, rows, repeat)
         return st, cache, total
 
     def _prepare_shared(self, st: DecodeState, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor], pad: int, repeat: int,
                         prefix_ids: Optional[torch.Tensor], prefix_mask: Optional[torch.Tensor], together: bool) -> DeviceKVCache:
-        """`prepare` for rows that share keys: the prefixes' prefill into a cache of their own, which the rows' caches refer to or (not `together`) get copies of, then
-        the prompts' (when they are not the prefixes themselves) behind it."""
+        """`prepare` for rows that share keys: the prefixes' prefill into a cache of their own, which the rows' caches refer to or (not `together`) get copies of, with
+        nothing left of it then, and the prompts' (when they are not the prefixes themselves) behind it."""
         rows, S = input_ids.shape
         whole = prefix_ids is None                                             # several answers: the prompts are what is shared
         front, front_mask = (input_ids, attention_mask) if whole else (prefix_ids, prefix_mask)
         groups, P = front.shape
+        slots = self._shared_slots(P)[0]
         front_cache, cache = getattr(st, "_front_cache", None), getattr(st, "_cache", None)
-        if front_cache is None or front_cache.k.shape[1] != groups or front_cache.k.shape[3] != P:
-            front_cache = st._front_cache = self.new_cache(groups, P)
+        if not together:
+            front_cache = self.new_cache(groups, P)
+        elif front_cache is None:
+            front_cache = st._front_cache = self.new_cache(groups, slots)
         if cache is None:
-            cache = st._cache = self.new_cache(st.B, max(st.max_len - P, 1) if together else st.max_len)
+            cache = st._cache = self.new_cache(st.B, self._own_slots(st.max_len, slots) if together else st.max_len)
             if together:
-                cache.prefix = SharedPrefix(front_cache.k, front_cache.v, torch.full((groups,), P, dtype=torch.int32, device=self.device), front_cache.pad_left,
-                                            K.prefix_attn_scratch(st.B, 1, groups, self.nh, self.nkv, self.hd, P, self.device))
+                cache.prefix = SharedPrefix(front_cache.k, front_cache.v, torch.zeros(groups, dtype=torch.int32, device=self.device), front_cache.pad_left,
+                                            K.prefix_attn_scratch(st.B, 1, groups, self.nh, self.nkv, self.hd, slots, self.device))
                 st.seq_pad = torch.zeros(st.B, dtype=torch.int32, device=self.device)
         st.rules = None
         front_cache.set_index(0)
@@ -955,6 +1002,7 @@ class B200Engine:
         if together:
             cache.set_index(0)
             cache.pad_left.zero_()
+            cache.prefix.length.fill_(P)
         else:
             for own, shared in ((cache.k, front_cache.k), (cache.v, front_cache.v)):
                 own.unflatten(1, (groups, -1))[..., :P, :].copy_(shared[:, :, None])
@@ -1048,6 +1096,7 @@ class EngineStream:
     def __init__(self, engine: B200Engine, st: DecodeState, cache: DeviceKVCache, sampling: Tuple, eos: int,
                  pad: int, graph: Optional[torch.cuda.CUDAGraph], produced_upto: int):
         self.engine, self.st, self.cache = engine, st, cache
+        st.stream = weakref.ref(self)
         self.sampling, self.eos, self.pad, self.graph = sampling, eos, pad, graph
         self.length = produced_upto
         self.host_tok = torch.empty(st.B, dtype=torch.int32).pin_memory()
