@@ -956,18 +956,18 @@ class B200Engine:
             prefix_ids = prefix_ids.to(self.device)
             if prefix_ids.dim() != 2 or prefix_ids.shape[0] < 1 or rows % prefix_ids.shape[0]:
                 raise ValueError(f"prefix_ids {tuple(prefix_ids.shape)} in front of {rows} prompts")
-        groups, P = (rows, S) if prefix_ids is None else prefix_ids.shape
-        total = S if prefix_ids is None else P + S
+            if S == 0:                           # nothing behind the prefixes: they are the prompts
+                input_ids, attention_mask, prefix_ids, prefix_mask = prefix_ids, prefix_mask, None, None
+        groups, P = (input_ids if prefix_ids is None else prefix_ids).shape
+        total = P if prefix_ids is None else P + S
         if max_length < total:
             raise ValueError(f"max_length {max_length} is shorter than the prompt ({total})")
-        # (a prompt without a token of its own ends with its prefix: its answer begins at the prefix's last position, not behind padding)
-        empty = S == 0 or (prefix_ids is not None and attention_mask is not None and bool((attention_mask[:, S - 1] == 0).any()))
         # copies need prompts without padding between them and their prefix
-        dense = prefix_ids is None or attention_mask is None or bool((attention_mask != 0).all())
-        if P == 0 or empty or not self.shares_prefixes or B == groups or not (dense or self._shared_attention()):
+        dense = prefix_ids is None or attention_mask is None or bool((attention_mask[:, :S] != 0).all())
+        if P == 0 or not self.shares_prefixes or B == groups or not (dense or self._shared_attention()):
             ids, mask = (input_ids, attention_mask) if prefix_ids is None else join_prefix(prefix_ids, input_ids, prefix_mask, attention_mask, pad)
-            st = self._decode_state(B, max_length)
-            cache = self.prepare(st, ids.repeat_interleave(repeat, 0), None if mask is None else mask.repeat_interleave(repeat, 0), pad)
+            st, times = self._decode_state(B, max_length), B // ids.shape[0]
+            cache = self.prepare(st, ids.repeat_interleave(times, 0), None if mask is None else mask.repeat_interleave(times, 0), pad)
         else:
             together = not dense or self._together(B, groups, P)
             st = self._shared_state(B, max_length, int(groups), int(P)) if together else self._decode_state(B, max_length)
@@ -997,7 +997,8 @@ class B200Engine:
                 st.seq_pad = torch.zeros(st.B, dtype=torch.int32, device=self.device)
         st.rules = None
         front_cache.set_index(0)
-        out = self.forward(front, attention_mask=front_mask, cache=front_cache, last_only=True, gather_logits=False)
+        logits = self.forward(front, attention_mask=front_mask, cache=front_cache, last_only=True, gather_logits=False).logits
+        logits = logits.view(groups, -1).repeat_interleave(st.B // groups, 0)
         ids, mask = front, front_mask
         if together:
             cache.set_index(0)
@@ -1013,7 +1014,10 @@ class B200Engine:
             if repeat > 1:
                 input_ids = input_ids.repeat_interleave(repeat, 0)
                 attention_mask = None if attention_mask is None else attention_mask.repeat_interleave(repeat, 0)
-            out = self.forward(input_ids, attention_mask=attention_mask, cache=cache, last_only=True, gather_logits=False)
+            behind = self.forward(input_ids, attention_mask=attention_mask, cache=cache, last_only=True, gather_logits=False).logits.view(st.B, -1)
+            # a prompt without a token of its own ends with its prefix: its answer begins there, not behind padding
+            empty = None if attention_mask is None else (attention_mask[:, S - 1:S] == 0).to(self.device)
+            logits = behind if empty is None else torch.where(empty, logits, behind)
         total = ids.shape[1]
         times = st.B // ids.shape[0]
         st.sequences.fill_(int(pad))
@@ -1025,8 +1029,7 @@ class B200Engine:
         st.step.zero_()
         st.n_unfinished.fill_(st.B)
         st.prompt_logits = None
-        logits = out.logits.view(-1, out.logits.shape[-1])
-        st.logits.copy_(logits.repeat_interleave(st.B // logits.shape[0], 0))
+        st.logits.copy_(logits)
         return cache
 
     def weight_bytes_per_step(self) -> int:

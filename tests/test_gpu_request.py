@@ -250,3 +250,32 @@ def test_a_row_without_a_token_left_takes_the_first(top_k, top_p):
     for vocab in (1, 33, 1000, 20001, 128256):
         x = torch.full((2, vocab), -float("inf"), device="cuda")
         assert K.sample_full(x, temperature=0.7, top_k=top_k, top_p=top_p, seed=5).tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("groups,pads,S,repeat", [(1, [9, 0, 4], 9, 1), (2, [0, 5, 5, 2], 5, 2), (1, [1, 0, 1, 1, 0], 1, 1), (2, [3, 3, 3, 3], 3, 1), (2, [0] * 4, 0, 3), (1, [0], 0, 6)])
+@pytest.mark.parametrize("name", list(CFGS))
+def test_prompts_without_a_token_of_their_own(name, groups, pads, S, repeat):
+    """Rows that are their prefix alone, among others or all of them: the prefix is still held once, and logits and tokens are those of the joined rows."""
+    cfg, tree32, eng = make(name)
+    rows, P = len(pads), 70
+    front, fmask, ids, mask = ids_of(groups, P, 1), padded([(3 * g) % 5 for g in range(groups)], P), ids_of(rows, S, 2), padded(pads, S)
+    joined, jmask = (t.repeat_interleave(repeat, 0) for t in join_prefix(front, ids, fmask, mask, 0))
+    B, total = joined.shape
+    feed, rules = ids_of(B, 4, 3), LogitRules(presence_penalty=0.5)
+    for _ in range(2):
+        stream = eng.begin_stream(ids.cuda(), mask.cuda(), max_length=total + 6, num_return_sequences=repeat, prefix_ids=front.cuda(), prefix_mask=fmask.cuda(), rules=rules)
+        assert stream.cache.prefix is not None and stream.st.B == B
+        seen = [stream.logits().clone()]
+        for t in range(4):
+            stream.step(feed[:, t].to(torch.int32).pin_memory())
+            seen.append(stream.logits().clone())
+        whole, m = torch.cat([joined, feed], 1), torch.cat([jmask, torch.ones(B, 4, dtype=torch.int32)], 1)
+        want = ref.forward(tree32, cfg, whole, m, ref.default_position_ids(m, B, total + 4, "cpu")).logits[:, total - 1:]
+        for t in range(5):
+            assert rel(seen[t], want[:, t]) < 3e-2, t
+        got = stream.sequences().cpu()
+        assert torch.equal(got[:, :total][jmask > 0], joined[jmask > 0]) and torch.equal(got[:, total:total + 4], feed)
+    seqs = eng.generate(ids.cuda(), mask.cuda(), max_length=total + 6, num_return_sequences=repeat, prefix_ids=front.cuda(), prefix_mask=fmask.cuda(), eos_token_id=-1).cpu()
+    m = torch.cat([jmask, torch.ones(B, 6, dtype=torch.int32)], 1)
+    logits = ref.forward(tree32, cfg, seqs, m, ref.default_position_ids(m, B, total + 6, "cpu")).logits[:, total - 1:-1]
+    assert (logits.amax(-1) - logits.gather(-1, seqs[:, total:, None])[..., 0] <= 6e-2 * logits.abs().amax()).all()
