@@ -1,4 +1,5 @@
-"""What attention over shared keys keeps beyond the 8 bits of one bfloat16 number: queries and probabilities of a step are two of them, at any count of rows."""
+"""What attention over shared keys keeps beyond the 8 bits of one bfloat16 number: queries and probabilities of a step are two of them, at any count of rows, and so are the
+probabilities of prompts with up to 128 queries of a key head."""
 import math
 
 import pytest
@@ -81,3 +82,27 @@ def test_a_step_has_sixteen_bits(B, groups, nh, nkv, hd, size):
                                nh, nkv, hd)
     err = (got.cpu().double().view(B, nh, hd) - want).abs()
     assert (err <= bound(want, mag, s)).all(), float((err / bound(want, mag, s)).max())
+
+
+PROMPTS = [(1, 1, 8, 8, 128, 40), (1, 1, 8, 8, 64, 128), (4, 1, 32, 8, 64, 4), (8, 2, 8, 2, 128, 3), (3, 1, 16, 2, 64, 5), (16, 1, 32, 4, 128, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,groups,nh,nkv,hd,S", PROMPTS)
+def test_a_prompt_of_one_tile_has_sixteen_bits(B, groups, nh, nkv, hd, S):
+    """The same two keys in front of tokens without key or value; queries come rotated, in one number each."""
+    qkv, pk, pv = case(B * S, groups, nh, nkv, hd, 0.25, B + S)
+    q = qkv[:, :nh * hd].view(B, S, nh, hd)
+    kc = torch.zeros(B, nkv, S, hd, dtype=torch.bfloat16, device=DEV)
+    got = K.prefill_attn_prefix(q.to(DEV), pk.to(DEV), pv.to(DEV), kc, kc.clone(), 0, S, None, None, None).cpu().double().view(B, S, nh, hd)
+    head, row = torch.arange(nh) // (nh // nkv), torch.arange(B) // (B // groups)
+    k, v = (t.double()[row][:, head] for t in (pk, pv))                      # [B, nh, 2, hd]
+    s = torch.einsum("bshd,bhkd->bshk", q.double(), k) / math.sqrt(hd)
+    size = (torch.einsum("bshd,bhkd->bshk", q.double().abs(), k.abs()) / math.sqrt(hd)).amax(-1, keepdim=True)
+    own = torch.zeros(B, S, nh, 1, dtype=torch.float64) + torch.log(torch.arange(1.0, S + 1, dtype=torch.float64))[:, None, None]      # s + 1 keys of score 0
+    w = torch.softmax(torch.cat([s, own], -1), -1)[..., :2]
+    want, mag = torch.einsum("bshk,bhkd->bshd", w, v), torch.einsum("bshk,bhkd->bshd", w, v.abs())
+    err, most = (got - want).abs(), bound(want, mag, size)
+    assert (err <= most).all(), float((err / most).max())
+    one_number = one(torch.einsum("bshk,bhkd->bshd", one(w / w.amax(-1, keepdim=True)) * w.amax(-1, keepdim=True), v))
+    assert ((one_number - want).abs() > most).any()                          # (what the bound is for)
