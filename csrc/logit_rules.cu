@@ -3,7 +3,7 @@
 //   x = logits[b, v]
 //   v occurs in tokens[b, start_b .. len_b):               x = x > 0 ? x / r_b : x r_b                    (repetition)
 //   n = occurrences in tokens[b, prompt_b .. len_b), n > 0: x = x - f_b n - p_b                           (frequency, presence)
-//   every entry i with bias_ids[b, i] == v:                x = x + bias[b, i]                             (in the order of the entries)
+//   entries i with bias_ids[b, i] == v:                    x = x + sum of bias[b, i]                      (summed in the order of the entries, added once)
 //   bit v of allowed[b] is zero:                           x = -infinity
 //
 // A CTA owns a slice of one row's vocabulary and keeps one word per token of the slice in shared memory: occurrences behind the prompt in the low bits, and bits

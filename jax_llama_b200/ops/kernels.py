@@ -590,7 +590,7 @@ def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = N
     tokens int32 [B, T]: row b has said tokens[b, starts[b] : lengths[b]] (int32 [B], or [1] for all rows; None: 0 and T), the part from prompt_lengths[b] on (None:
     all of it) as its answer.  Ids outside the vocabulary are passed over.  For a token that occurs: x > 0 ? x / repetition : x · repetition; with n occurrences in
     the answer, n > 0: x - frequency · n - presence.  (A number, or fp32 [B]; None: off.  repetition > 0.)  Then x + bias_values of the entries of bias_ids
-    (int32 / fp32 [B, n], or [1, n] for all rows, n <= 8192; an id outside the vocabulary is no entry, the same id twice adds both), then -inf where bit v % 32 of word v // 32
+    (int32 / fp32 [B, n], or [1, n] for all rows, n <= 8192; an id outside the vocabulary is no entry, the same id twice adds the sum of both), then -inf where bit v % 32 of word v // 32
     of allowed (int32 [B, words] or [1, words]) is zero.  A row whose mask allows nothing is -inf throughout.  `out` may be `logits` itself when that is fp32; any
     other overlap is refused."""
     who = "constrain_logits"

@@ -177,3 +177,13 @@ def test_a_penalty_divides(r, dev):
     for rep in (r, torch.tensor([r], device=dev)):
         got = K.constrain_logits(x.to(dev), tokens=tokens.to(dev), prompt_lengths=torch.tensor([x.shape[1]], dtype=torch.int32, device=dev), repetition=rep).cpu()
         assert torch.equal(got.nan_to_num(nan=123.0, posinf=math.inf, neginf=-math.inf), want.nan_to_num(nan=123.0, posinf=math.inf, neginf=-math.inf))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_biases_of_one_token_are_summed_and_added_once(dev):
+    """In the order of the entries: 1e8 and -1e8 leave a logit its bits, and 1 is lost behind 1e8, not in front of its opposite."""
+    x = torch.tensor([[0.1, 0.2, 0.3]])
+    ids = torch.tensor([[0, 1, 0, 1, 1]], dtype=torch.int32)
+    bias = torch.tensor([[1e8, 1e8, -1e8, 1.0, -1e8]])
+    got = K.constrain_logits(x.to(dev), bias_ids=ids.to(dev), bias_values=bias.to(dev)).cpu()
+    assert torch.equal(got, x)
