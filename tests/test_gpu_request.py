@@ -279,3 +279,16 @@ def test_prompts_without_a_token_of_their_own(name, groups, pads, S, repeat):
     m = torch.cat([jmask, torch.ones(B, 6, dtype=torch.int32)], 1)
     logits = ref.forward(tree32, cfg, seqs, m, ref.default_position_ids(m, B, total + 6, "cpu")).logits[:, total - 1:-1]
     assert (logits.amax(-1) - logits.gather(-1, seqs[:, total:, None])[..., 0] <= 6e-2 * logits.abs().amax()).all()
+
+
+@pytest.mark.parametrize("rules", [None, LogitRules(presence_penalty=0.1)])
+def test_sequences_of_a_fed_stream(rules):
+    """With rules the fed tokens, which are their history; without them the selected ones, as the documentation says."""
+    cfg, _, eng = make("gqa128")
+    stream = eng.begin_stream(ids_of(2, 6, 3).cuda(), None, max_length=16, rules=rules)
+    chosen = [stream.last_tokens().clone()]
+    feed = ids_of(2, 4, 9).to(torch.int32)
+    for t in range(4):
+        chosen.append(stream.step(feed[:, t].contiguous().pin_memory()).clone())
+    said = torch.stack(chosen, 1) if rules is None else torch.cat([feed, chosen[-1][:, None]], 1)
+    assert torch.equal(stream.sequences()[:, 6:].cpu(), said.long())
