@@ -1113,7 +1113,8 @@ class EngineStream:
     def step(self, feed: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Advance every row by one token.  `feed` (pinned int32 [B] on the host) overrides the input
         token of this step — the interactive case where the host owns the sequence; otherwise the token
-        selected on the device in the previous step is used.  `allowed` (int32 masks of the rules' shape, [1 or B, words]) are the tokens that this step
+        selected on the device in the previous step is used.  A batch with rules takes fed tokens as what was said: they count for its
+        penalties and stand in `sequences`.  `allowed` (int32 masks of the rules' shape, [1 or B, words]) are the tokens that this step
         may choose, for a grammar that follows the text; the stream's rules then have `allowed_tokens` from the start, for its first token.  Returns the
         new tokens in pinned memory."""
         if self.length >= self.st.max_len:
@@ -1138,6 +1139,8 @@ class EngineStream:
         return self.host_tok
 
     def sequences(self) -> torch.Tensor:
+        """[B, tokens so far]: the prompt and the tokens selected on the device.  Where a step was fed others, these stand here with rules, whose history this is, and
+        the selected ones without (the host that feeds has its own)."""
         return self.st.sequences[:, :self.length].to(torch.long)
 
     def logits(self) -> torch.Tensor:
