@@ -222,7 +222,7 @@ extern "C" JL_API int jl_logit_rules(const void* logits, int dtype, int B, int V
                                      const float* freq, float freq1, const float* pres, float pres1, const int* bias_ids, const float* bias, int n_bias, int ldb,
                                      const void* allowed, int lda, void* stream) {
   if (B == 0 || V == 0) return JL_OK;
-  JL_CHECK_ARG(logits && out && B > 0 && V > 0 && B <= 65535 && ld >= V && ldo >= V, "jl_logit_rules: %d rows of %d logits, pitches %d and %d", B, V, ld, ldo);
+  JL_CHECK_ARG(logits && out && B > 0 && V > 0 && B <= 65535 && (ld >= V || ld == 0) && ldo >= V, "jl_logit_rules: %d rows of %d logits, pitches %d and %d", B, V, ld, ldo);
   JL_CHECK_ARG(V <= (1 << 30) && (uintptr_t)logits % (dtype == 0 ? 4 : 2) == 0 && (uintptr_t)out % 4 == 0, "jl_logit_rules: vocabulary of %d, or misplaced logits", V);
   JL_CHECK_ARG(dtype >= 0 && dtype <= 2, "jl_logit_rules: dtype %d (0 fp32, 1 bf16, 2 fp16)", dtype);
   JL_CHECK_ARG(tokens == nullptr || (T >= 0 && ldt >= T), "jl_logit_rules: history of %d tokens, pitch %d", T, ldt);

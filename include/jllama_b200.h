@@ -583,7 +583,7 @@ int jl_prefill_attn_prefix(const void* q, const void* prefix_k, const void* pref
                            int hd, int P, int T, int start, float scale, void* stream);
 
 /* The rules of a request on its logits, before selection: out[b, v] (fp32, pitch ldo; may be logits itself when that is fp32) from logits [B, V] (dtype 0 fp32, 1 bf16,
- * 2 fp16; pitch ld).  Tokens that occur in tokens[b, starts[b] .. lengths[b]) (pitch ldt, T columns): x > 0 ? x / rep : x rep; n occurrences from position prompts[b]
+ * 2 fp16; pitch ld, 0 = one row for all).  Tokens that occur in tokens[b, starts[b] .. lengths[b]) (pitch ldt, T columns): x > 0 ? x / rep : x rep; n occurrences from position prompts[b]
  * on: x - freq n - pres.  Then the biases of the entries (n_bias <= 8192; ids outside the vocabulary: unused; the same id twice: the sum of both, formed
  * in the order of the entries), then -infinity where bit v % 32 of
  * word v / 32 of allowed[b] is zero.  starts / lengths / prompts: one number per row (.._n = B) or for all (1), NULL = 0 / T / 0; rep / freq / pres: [B], or

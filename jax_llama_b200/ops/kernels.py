@@ -574,7 +574,7 @@ def _same_or_apart(x: torch.Tensor, y: torch.Tensor) -> bool:
     p, q = (x.stride(0) * n, y.stride(0) * m) if B > 1 else (V * n, V * m)
     if a + (B - 1) * p + V * n <= b or b + (B - 1) * q + V * m <= a or B * V == 0:
         return True
-    if p != q:
+    if p != q or p == 0:
         return False
     gap = (b - a) % p
     return (a == b and x.dtype is y.dtype) or (gap >= V * n and p - gap >= V * m)

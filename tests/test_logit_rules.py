@@ -187,3 +187,17 @@ def test_biases_of_one_token_are_summed_and_added_once(dev):
     bias = torch.tensor([[1e8, 1e8, -1e8, 1.0, -1e8]])
     got = K.constrain_logits(x.to(dev), bias_ids=ids.to(dev), bias_values=bias.to(dev)).cpu()
     assert torch.equal(got, x)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("V", [40, 5003])
+def test_one_row_of_logits_for_all(V, dev):
+    """Rows that are one another's memory are read, each under its own rules; as a place for results they are refused, and so is one that overlaps the row."""
+    g = torch.Generator().manual_seed(V)
+    row, tokens = torch.randn(1, V, generator=g).to(dev), torch.randint(0, V, (3, 20), generator=g, dtype=torch.int32).to(dev)
+    kw = dict(tokens=tokens, repetition=1.5, presence=0.25)
+    assert torch.equal(K.constrain_logits(row.expand(3, V), **kw), K.constrain_logits(row.repeat(3, 1), **kw))
+    half = V // 2
+    for logits, out in ((row.expand(3, V), row.expand(3, V)), (row[:, :half].expand(2, half), row.view(-1)[:2 * half].view(2, half))):
+        with pytest.raises(ValueError, match="overlaps"):
+            K.constrain_logits(logits, tokens=tokens[:len(out)], out=out)
