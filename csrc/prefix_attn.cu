@@ -1059,9 +1059,10 @@ static PxStep px_step(int B, int groups, int nkv, int G, int hd, int P, int T) {
     r.own_ctas = (int)((items * r.own_splits + (long)groups * nkv * r.splits + 7) / 8);
     return r;
   }
-  // us: 3 in and out of a unit, 55 KB/us of own keys for the 8 warps of an SM (what one SM draws under load); 0.9 a tile of shared keys and 1.45 for two tiles of
-  // queries (64 rows x 32 heads over 4096 by splits for 1.25: 32, for this 29.5), 8 in and out of a CTA
-  const float unit = 3.f + (float)T * 0.5f / (float)r.own_splits * (float)hd * 4.f * 8.f / 55e3f, tile = queries > PX_BM ? 1.45f : 0.9f;
+  // us: 3 in and out of a unit, 55 KB/us of own keys for the 8 warps of an SM (what one SM draws under load); 0.9 a tile of shared keys and 2 for two tiles of
+  // queries (1.8 in 96 rows over 32768; splits by 1.25, 1.45, 1.7, this, 2.4: 64 rows x 32 heads over 4096 32, 30.5, 29, 26.4, 26.4; 40 over 16000 -, 42.7, 42.6, 40.6, 44.5; 2 x 48 over 8192 -, 51,
+  // 51, 49, 49.3), 8 in and out of a CTA
+  const float unit = 3.f + (float)T * 0.5f / (float)r.own_splits * (float)hd * 4.f * 8.f / 55e3f, tile = queries > PX_BM ? 2.0f : 0.9f;
   const int tiles = (P + PX_BN - 1) / PX_BN, cap = px_splits(queries, groups, nkv, P);       // (what the scratch is sized for)
   const bool half = queries > PX_BM && (queries % (2 * PX_BM) <= PX_BM && queries % (2 * PX_BM) != 0);
   const float heads = (float)(groups * nkv), work = heads * ((float)px_tiles(queries) - (half ? 0.22f : 0.f)) * (float)tiles * tile + (float)r.own_ctas * unit;
