@@ -24,7 +24,7 @@
 // Slots that hold no key may hold anything: their scores are masked, and their value rows are cleared in shared memory, because a weight of zero
 // times a NaN is a NaN.
 //
-// One B200, us a call in a graph: one token, 16 rows x 32 heads over 8 of keys, 2048 shared 12.7; 96 rows, 32768 shared and 500 own each 122 (860 TFLOP/s with the
+// One B200, us a call in a graph of ten, by itself: one token, 16 rows x 32 heads over 8 of keys, 2048 shared 12.7; 96 rows, 32768 shared and 500 own each 122 (860 TFLOP/s with the
 // second products of queries and probabilities, 2.7 TB/s beside them); 4 x 16 rows, 3501 shared and 701 own 44 (5.5 TB/s).  Prompts: 2 x 2048 tokens over 16384 1065 (1080 TFLOP/s; a
 // single launch of its own 906 and 1290: the power cap), 8 x 333 over 1500 68 (1110), 16 x 48 over 8192 111 (920).  What bounds them: products of small width
 // (a 128 x 64 tile of scores reads its queries from shared memory, 384 cycles for 256 of products) and the exponentials, half of the special-function
