@@ -1,0 +1,363 @@
+// Products of 8-bit integers on tcgen05 (kind::i8), weights as the MMA's rows: out[row, feature] = sx[row] sw[feature] qx[row] · qw[feature].
+//
+// 128 weight rows fill the MMA's lanes, up to 256 rows of activations its N; a TMA ring of 128-byte k-blocks (128 values), one thread issues the MMAs, int32 sums in
+// TMEM, two accumulators.  Sums leave through shared memory as [row][feature], so that a thread finishes four neighbouring features of a row: both scales, the
+// residual or the gate, one rounding.  One matrix, or one per expert: rows come ordered by expert, at any row, no padding between experts; a tile of rows that runs
+// past its expert's end computes rows of the next one and does not store them.
+// Few tiles of one matrix: the CTAs of a cluster share one and take a part of K each; the partials meet in distributed shared memory, whole numbers, so their order
+// changes nothing.
+#include "int8.cuh"
+#include "jllama_b200.h"
+#include "tcgen05.cuh"
+
+namespace jl {
+
+constexpr int I8S_BM = 128, I8S_BK = 128, I8S_THREADS = 256;      // warp 0: TMA, warp 1: MMA, warp 2: TMEM; 4-7 (split: all): results
+constexpr uint32_t I8S_A_BYTES = I8S_BM * I8S_BK, I8S_STAGING = 16 * I8S_BM * 4;
+
+struct Int8Swap {
+  Int8Out o;
+  Int8Work work;
+  int K, nb, stages, ksplit;        // rows of a tile: nb, a multiple of 16
+  uint32_t cols, idesc;
+  int early;                        // weights may be read ahead of the wait for the kernels before
+};
+
+__device__ __forceinline__ uint32_t i8s_mapa(uint32_t local_addr, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local_addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ int4 i8s_ld_cluster(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int MODE, bool SPLIT>
+__global__ void __launch_bounds__(I8S_THREADS, 2)
+int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Int8Swap p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int stages = p.stages, ksplit = SPLIT ? p.ksplit : 1;
+  const uint32_t b_bytes = (uint32_t)p.nb * I8S_BK, stage_bytes = I8S_A_BYTES + b_bytes;
+  const uint32_t staging = smem_base + stages * stage_bytes;    // !SPLIT: 16 rows x 32 features for each epilogue warp
+  const uint32_t bars = staging + (SPLIT ? 0u : I8S_STAGING);   // full[stages] | empty[stages] | tfull[2] | tempty[2]
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (stages + s); };
+  auto tfull_bar = [&](int s) { return bars + 8u * (2 * stages + s); };
+  auto tempty_bar = [&](int s) { return bars + 8u * (2 * stages + 2 + s); };
+  const uint32_t tmem_slot = bars + 8u * (2 * stages + 4);
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - tc::smem_u32(smem_raw)));
+  int* table = reinterpret_cast<int*>(smem_raw + (tmem_slot + 16 - tc::smem_u32(smem_raw)));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_kb = (p.K + I8S_BK - 1) / I8S_BK;
+  const int tile0 = (int)blockIdx.x / ksplit, tstep = (int)gridDim.x / ksplit;      // SPLIT: one tile, its parts are the CTAs of a cluster
+  const int rank = (int)blockIdx.x % ksplit, kb0 = rank * num_kb / ksplit, kb1 = (rank + 1) * num_kb / ksplit;
+
+  if (warp == 0 && lane == 0) {
+    tc::prefetch_tensormap(&tmap_w);
+    tc::prefetch_tensormap(&tmap_x);
+  }
+  if (warp == 1 && lane == 0) {
+    for (int s = 0; s < stages; ++s) { tc::mbar_init(full_bar(s), 1); tc::mbar_init(empty_bar(s), 1); }
+    for (int s = 0; s < 2; ++s) { tc::mbar_init(tfull_bar(s), 1); tc::mbar_init(tempty_bar(s), 4); }
+    tc::fence_barrier_init();
+  }
+  if (warp == 2) tc::tmem_alloc(tmem_slot, SPLIT ? p.cols : 2 * p.cols);
+  if (warp == 3) {
+    if (p.work.offsets != nullptr) pdl_wait();
+    i8_list(p.work, table);
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot_ptr;
+  pdl_launch_dependents();
+  const int tiles = table[p.work.experts];
+
+  if (warp == 0) {
+    // ===================================================== TMA producer
+    if (lane == 0) {
+      int pre = 0;
+      if (p.early && tile0 < tiles) {                           // (one matrix: the first tile's weights are known)
+        Int8Walk walk;
+        const Int8Tile t = walk.at(p.work, table, tile0);
+        pre = kb1 - kb0 < stages ? kb1 - kb0 : stages;
+        for (int i = 0; i < pre; ++i) {
+          tc::mbar_expect_tx(full_bar(i), stage_bytes);
+          tc::tma_load_2d(smem_base + i * stage_bytes, &tmap_w, full_bar(i), (kb0 + i) * I8S_BK, t.col * I8S_BM, tc::EVICT_FIRST);
+        }
+      }
+      pdl_wait();
+      Int8Walk walk;
+      int stage = 0; uint32_t phase = 0;
+      for (int tile = tile0; tile < tiles; tile += tstep) {
+        const Int8Tile t = walk.at(p.work, table, tile);
+        const int w_row = t.expert * p.o.N + t.col * I8S_BM;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          const uint32_t sa = smem_base + stage * stage_bytes;
+          if (pre > 0) {
+            --pre;
+          } else {
+            tc::mbar_wait(empty_bar(stage), phase ^ 1);
+            tc::mbar_expect_tx(full_bar(stage), stage_bytes);
+            tc::tma_load_2d(sa, &tmap_w, full_bar(stage), kb * I8S_BK, w_row, tc::EVICT_FIRST);
+          }
+          tc::tma_load_2d(sa + I8S_A_BYTES, &tmap_x, full_bar(stage), kb * I8S_BK, t.row0, tc::EVICT_LAST);
+          if (++stage == stages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ===================================================== MMA issuer (single thread)
+    if (lane == 0) {
+      int stage = 0, it = 0; uint32_t phase = 0;
+      for (int tile = tile0; tile < tiles; tile += tstep, ++it) {
+        const int as = it & 1;
+        if constexpr (!SPLIT) {
+          tc::mbar_wait(tempty_bar(as), ((it >> 1) & 1) ^ 1);      // the epilogue has drained this accumulator
+          tc::fence_after_sync();
+        }
+        const uint32_t d = tmem_base + as * p.cols;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          tc::mbar_wait(full_bar(stage), phase);
+          tc::fence_after_sync();
+          const uint32_t sa = smem_base + stage * stage_bytes;
+          const uint64_t da = tc::smem_desc_kmajor_sw128(sa), db = tc::smem_desc_kmajor_sw128(sa + I8S_A_BYTES);
+#pragma unroll
+          for (int k = 0; k < I8S_BK / 32; ++k)             // +32 bytes per UMMA_K inside the swizzle span
+            tc::mma_ss_i8(d, da + 2 * k, db + 2 * k, p.idesc, kb != kb0 || k != 0);
+          tc::mma_commit(empty_bar(stage));                 // frees the smem slot when these MMAs retire
+          if (++stage == stages) { stage = 0; phase ^= 1; }
+        }
+        tc::mma_commit(tfull_bar(as));
+      }
+    }
+    __syncwarp();
+  }
+
+  // TMEM lane = weight row, column = row of activations
+  const uint32_t t_lane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+  auto to_shared = [&](uint32_t t_col, uint32_t at, int pitch) {      // 16 rows
+    uint32_t v[16];
+    tc::tmem_ld16(t_col, v);
+    tc::tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + j * pitch), "r"(v[j]) : "memory");
+  };
+  auto feature_scales = [&](int expert, int f0, float (&sw)[4]) {
+    const float* s = p.o.ws + (size_t)expert * p.o.N + f0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sw[i] = f0 + i < p.o.N ? s[i] : 0.0f;
+  };
+  if constexpr (!SPLIT) {
+    // ===================================================== epilogue of a persistent CTA: warps 4-7, 16 rows at a time
+    if (warp >= 4) {
+      pdl_wait();                                           // scales, residual, output: after the previous kernel
+      const uint32_t st = staging + (warp & 3) * (I8S_STAGING / 4);
+      Int8Walk walk;
+      int it = 0;
+      for (int tile = tile0; tile < tiles; tile += tstep, ++it) {
+        const Int8Tile t = walk.at(p.work, table, tile);
+        const int as = it & 1, f0 = t.col * I8S_BM + (warp & 3) * 32 + 4 * (lane & 7);
+        float sw[4];
+        feature_scales(t.expert, f0, sw);
+        tc::mbar_wait(tfull_bar(as), (it >> 1) & 1);
+        tc::fence_after_sync();
+        const int used = (t.rows + 15) / 16 * 16;
+        for (int c0 = 0; c0 < used; c0 += 16) {
+          to_shared(t_lane + as * p.cols + c0, st + lane * 4, 128);
+          tc::fence_before_sync();
+          __syncwarp();
+          if (c0 + 16 >= used && lane == 0) tc::mbar_arrive(tempty_bar(as));      // read: the sums of the tile after next may begin
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int r = (lane >> 3) + 4 * u, row = c0 + r;
+            if (f0 >= p.o.N || row >= t.rows) continue;
+            int x[4];
+            asm volatile("ld.shared.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(st + r * 128 + (lane & 7) * 16) : "memory");
+            i8_finish4<MODE>(p.o, t.row0 + row, f0, x, p.o.xs[t.row0 + row], sw);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    // ===================================================== all warps: partial sums meet in the cluster (one matrix, one tile)
+    pdl_wait();
+    Int8Walk walk;
+    const Int8Tile t = walk.at(p.work, table, tile0);
+    const int f0 = t.col * I8S_BM + 4 * lane, row = I8S_BM * 4;
+    const uint32_t put = smem_base + ((warp & 3) * 32 + lane) * 4, get = smem_base + lane * 16;
+    float sw[4];
+    feature_scales(t.expert, f0, sw);
+    tc::mbar_wait(tfull_bar(0), 0);
+    tc::fence_after_sync();
+    // the ring is free (all MMAs done) and takes the partial
+    for (int c0 = (warp >> 2) * 16; c0 < t.rows; c0 += 32) to_shared(t_lane + c0, put + c0 * row, row);
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    const int per = (t.rows + ksplit - 1) / ksplit, t_lo = rank * per, t_hi = min(t_lo + per, t.rows);
+    for (int r0 = t_lo + warp; r0 < t_hi; r0 += 8) {
+      int x[4] = {0, 0, 0, 0};
+      int4 part[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < ksplit) part[r] = i8s_ld_cluster(i8s_mapa(get, r) + r0 * row);
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < ksplit) { x[0] += part[r].x; x[1] += part[r].y; x[2] += part[r].z; x[3] += part[r].w; }
+      if (f0 < p.o.N) i8_finish4<MODE>(p.o, t.row0 + r0, f0, x, p.o.xs[t.row0 + r0], sw);
+    }
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");      // no CTA leaves while its partial may still be read
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 2) tc::tmem_dealloc(tmem_base, SPLIT ? p.cols : 2 * p.cols);
+}
+
+static size_t i8s_smem(int stages, int nb, bool split, int experts) {
+  return (size_t)stages * (I8S_A_BYTES + nb * I8S_BK) + (split ? 0 : I8S_STAGING) + 8 * (2 * stages + 4) + 16 + 4 * i8_table_ints(experts) + 1024;
+}
+
+// Parts of K, a cluster's CTAs: enough to fill both slots of every SM, at least four k-blocks each
+static int i8s_parts(int nb, int tiles, int num_kb, int num_sms) {
+  const int slots = nb > 128 ? num_sms : 2 * num_sms - 32;
+  int ks = slots / tiles;
+  if (ks > 8) ks = 8;
+  if (nb > 128 && ks > 4) ks = 4;
+  if (ks > num_kb / 4) ks = num_kb / 4;
+  return ks > 1 ? ks : 1;
+}
+
+template <int MODE>
+static int swap_launch(const void* xq, const void* wq, Int8Swap p, int ldx, int ldw, int num_sms, cudaStream_t stream) {
+  const int E = p.work.experts;
+  p.work.cols = (p.o.N + I8S_BM - 1) / I8S_BM;
+  p.work.chunk = p.nb;
+  const bool grouped = p.work.offsets != nullptr;
+  const int num_kb = (p.K + I8S_BK - 1) / I8S_BK;
+  const long long most = (long long)p.work.cols * ((p.work.rows + p.nb - 1) / p.nb + (grouped ? (E < p.work.rows ? E : p.work.rows) : 0));      // tiles, at most
+  JL_CHECK_ARG(most < (1ll << 30), "int8 product: %lld tiles", most);
+  p.ksplit = grouped || p.work.rows > p.nb ? 1 : i8s_parts(p.nb, (int)most, num_kb, num_sms);
+  const bool split = p.ksplit > 1;
+  p.cols = p.nb <= 32 ? 32 : p.nb <= 64 ? 64 : p.nb <= 128 ? 128 : 256;
+  p.idesc = tc::idesc_s8_s32(I8S_BM, p.nb);
+  const int stage = (int)I8S_A_BYTES + p.nb * I8S_BK, room = 4 * i8_table_ints(E) + (split ? 0 : (int)I8S_STAGING);
+  int stages = ((p.nb > 128 ? 200 * 1024 : 110 * 1024) - room) / stage;
+  if (stages > 10) stages = 10;
+  const int slots = p.nb <= 128 ? 2 * num_sms : num_sms;
+  const long long blocks = split ? (num_kb + p.ksplit - 1) / p.ksplit : (most + slots - 1) / slots * num_kb;
+  const int tile = split ? (p.nb * I8S_BM * 4 + stage - 1) / stage : 2;                    // a split's partial fits the ring
+  if (stages > blocks) stages = (int)blocks;
+  if (stages < tile) stages = tile;
+  p.stages = stages;
+  CUtensorMap tw, tx;
+  int rc;
+  if ((rc = make_tmap_2d_i8(&tw, wq, (uint64_t)p.o.N * E, p.K, ldw, I8S_BM))) return rc;
+  if ((rc = make_tmap_2d_i8(&tx, xq, p.work.rows, p.K, ldx, p.nb))) return rc;
+  const size_t smem = i8s_smem(stages, p.nb, split, E);
+  auto kern = split ? int8_swap_kernel<MODE, true> : int8_swap_kernel<MODE, false>;
+  JL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(split ? most * p.ksplit : most < slots ? most : slots));
+  cfg.blockDim = dim3(I8S_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  if (pdl_enabled()) {
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (split) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = p.ksplit;
+    attr[na].val.clusterDim.y = 1;
+    attr[na++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = na;
+  count_launch();
+  JL_CUDA(cudaLaunchKernelEx(&cfg, kern, tw, tx, p));
+  return JL_OK;
+}
+
+int int8_rows(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int n, const void* gain, float eps, void* q, int ldq, float* s, bool early,
+              cudaStream_t stream);
+
+static int product(const void* xq, int ldx, const void* wq, int ldw, Int8Swap p, int mode, int num_sms, cudaStream_t stream) {
+  if (mode == I8_PLAIN) return swap_launch<I8_PLAIN>(xq, wq, p, ldx, ldw, num_sms, stream);
+  if (mode == I8_RESIDUAL) return swap_launch<I8_RESIDUAL>(xq, wq, p, ldx, ldw, num_sms, stream);
+  return swap_launch<I8_GATED>(xq, wq, p, ldx, ldw, num_sms, stream);
+}
+
+static int up16(int k) { return (k + 15) / 16 * 16; }
+
+// result, residual and scales; rows of four features in one access where the row pitch and both addresses allow it
+static Int8Out out_of(void* out, const void* residual, const float* xs, const float* ws, int kind, int N, int mode) {
+  Int8Out o{out, residual, xs, ws, kind, N, mode == I8_GATED ? N / 2 : N, 0};
+  const uintptr_t step = (kind == DT_F32 ? 4 : 2) * (mode == I8_GATED ? 2 : 4);
+  o.wide = N % 4 == 0 && (((uintptr_t)out | (uintptr_t)residual) & (step - 1)) == 0;
+  return o;
+}
+
+}  // namespace jl
+
+using namespace jl;
+
+// bytes that jl_linear_int8 (rows = M) and jl_experts_int8 need beside their operands: the activations' values (rows on 16 bytes) and scales
+extern "C" JL_API size_t jl_int8_scratch_bytes(int rows, int K) { return rows < 0 || K < 1 ? 0 : ((size_t)rows * up16(K) + 255) / 256 * 256 + (size_t)rows * 4; }
+
+extern "C" JL_API int jl_linear_int8(const void* x, int dtype, int M, int K, long long ldx, const void* wq, int ldw, const float* ws, int N, const void* gain, float eps,
+                                     const void* residual, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int resident, int num_sms, void* stream) {
+  JL_CHECK_ARG(dtype >= DT_BF16 && dtype <= DT_F16 && out_dtype >= DT_BF16 && out_dtype <= DT_F16, "jl_linear_int8: element types %d, %d", dtype, out_dtype);
+  JL_CHECK_ARG(M >= 0 && N >= 1 && K >= 1 && K <= I8_MAX_K && (ldx >= K || M <= 1), "jl_linear_int8: M=%d N=%d K=%d (at most %d), pitch %lld", M, N, K, I8_MAX_K, ldx);
+  JL_CHECK_ARG(ldw >= K && ldw % 16 == 0 && ((uintptr_t)wq & 15) == 0, "jl_linear_int8: weights on 16-byte rows (pitch %d)", ldw);
+  JL_CHECK_ARG(mode >= I8_PLAIN && mode <= I8_GATED && (mode == I8_RESIDUAL) == (residual != nullptr) && (mode != I8_GATED || N % 2 == 0),
+               "jl_linear_int8: mode %d with%s residual, N=%d", mode, residual != nullptr ? "" : "out", N);
+  if (M == 0) return JL_OK;
+  JL_CHECK_ARG(scratch != nullptr && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= jl_int8_scratch_bytes(M, K), "jl_linear_int8: scratch of %zu bytes", scratch_bytes);
+  if (num_sms <= 0) num_sms = SMS;
+  const int ldq = up16(K);
+  float* xs = reinterpret_cast<float*>((uint8_t*)scratch + ((size_t)M * ldq + 255) / 256 * 256);
+  int rc;
+  if ((rc = int8_rows(x, dtype, M, K, ldx, nullptr, M, gain, eps, scratch, ldq, xs, true, (cudaStream_t)stream))) return rc;
+  Int8Swap p{};
+  p.o = out_of(out, residual, xs, ws, out_dtype, N, mode);
+  p.work = Int8Work{nullptr, 1, M, 0, 0};
+  p.K = K;
+  p.nb = M >= 256 ? 256 : (M + 15) / 16 * 16;
+  p.early = 1;                      // the kernel ahead is the one above, and it began when those before it were done
+  return product(scratch, ldq, wq, ldw, p, mode, num_sms, (cudaStream_t)stream);
+}
+
+extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int T, const int* offsets, int experts, const void* wq, int ldw,
+                                      const float* ws, int N, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int num_sms, void* stream) {
+  JL_CHECK_ARG(dtype >= DT_BF16 && dtype <= DT_F16 && out_dtype >= DT_BF16 && out_dtype <= DT_F16, "jl_experts_int8: element types %d, %d", dtype, out_dtype);
+  JL_CHECK_ARG(M >= 0 && T >= 0 && N >= 1 && K >= 1 && K <= I8_MAX_K && (ldx >= K || M <= 1) && (rows != nullptr || T <= M),
+               "jl_experts_int8: M=%d T=%d N=%d K=%d (at most %d), pitch %lld", M, T, N, K, I8_MAX_K, ldx);
+  JL_CHECK_ARG(experts >= 1 && experts <= I8_MAX_EXPERTS && offsets != nullptr, "jl_experts_int8: %d experts (at most %d)", experts, I8_MAX_EXPERTS);
+  JL_CHECK_ARG((long long)N * experts < (1ll << 31), "jl_experts_int8: %d x %d weight rows", experts, N);
+  JL_CHECK_ARG(ldw >= K && ldw % 16 == 0 && ((uintptr_t)wq & 15) == 0, "jl_experts_int8: weights on 16-byte rows (pitch %d)", ldw);
+  JL_CHECK_ARG(mode == I8_PLAIN || (mode == I8_GATED && N % 2 == 0), "jl_experts_int8: mode %d, N=%d", mode, N);
+  if (T == 0) return JL_OK;
+  JL_CHECK_ARG(scratch != nullptr && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= jl_int8_scratch_bytes(T, K), "jl_experts_int8: scratch of %zu bytes", scratch_bytes);
+  if (num_sms <= 0) num_sms = SMS;
+  const int ldq = up16(K);
+  float* xs = reinterpret_cast<float*>((uint8_t*)scratch + ((size_t)T * ldq + 255) / 256 * 256);
+  int rc;
+  if ((rc = int8_rows(x, dtype, M, K, ldx, rows, T, nullptr, 0.0f, scratch, ldq, xs, true, (cudaStream_t)stream))) return rc;
+  Int8Swap p{};
+  p.o = out_of(out, nullptr, xs, ws, out_dtype, N, mode);
+  p.work = Int8Work{offsets, experts, T, 0, 0};
+  p.K = K;
+  const int even = (T + experts - 1) / experts;                 // rows of an expert if all have the same
+  p.nb = even <= 8 ? 16 : even <= 32 ? 64 : even <= 64 ? 128 : 256;
+  p.early = 0;
+  return product(scratch, ldq, wq, ldw, p, mode, num_sms, (cudaStream_t)stream);
+}

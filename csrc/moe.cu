@@ -130,7 +130,7 @@ constexpr int MS_KEEP = 16;
 template <int KEEP>
 __global__ void __launch_bounds__(1024) moe_sort_kernel(const int* __restrict__ idx, int n, int top, int E, int tile, int cap,
                                                         int* __restrict__ pos, int* __restrict__ row_src,
-                                                        int* __restrict__ tile_group, int* __restrict__ tiles_used) {
+                                                        int* __restrict__ tile_group, int* __restrict__ tiles_used, int* __restrict__ offsets) {
   pdl_wait();                      // programmatic dependent launch: nothing is read before the predecessor is done
   pdl_launch_dependents();
   extern __shared__ int si[];
@@ -140,23 +140,28 @@ __global__ void __launch_bounds__(1024) moe_sort_kernel(const int* __restrict__ 
   // asked for at once), a warp adds up the counts.  2048 tokens x 4 of 32 experts: 11.4 -> 8.7 us.  KEEP is the smallest of 1, 4 and MS_KEEP that holds the
   // pairs: sixteen steps of which fifteen have nothing to do are a us (200 tokens x 2 of 8 experts: 2.8 us with pairs in memory, 3.8 with MS_KEEP, 2.6 with 1).
   const bool keep = n <= KEEP * (int)blockDim.x;
+  auto expert = [&](int i) { const int e = idx[i]; return e < E ? e : -1; };      // (one that there is not runs nothing)
   int ex[KEEP], rank[KEEP];
   if (keep) {
 #pragma unroll
     for (int u = 0; u < KEEP; ++u) {
       const int i = threadIdx.x + u * blockDim.x;
-      ex[u] = i < n ? idx[i] : -1;
+      ex[u] = i < n ? expert(i) : -1;
     }
   }
   for (int e = threadIdx.x; e < E; e += blockDim.x) count[e] = 0;
   for (int i = threadIdx.x; i < cap; i += blockDim.x) row_src[i] = -1;
-  for (int i = threadIdx.x; i < cap / tile; i += blockDim.x) tile_group[i] = -1;
+  if (tile_group != nullptr)
+    for (int i = threadIdx.x; i < cap / tile; i += blockDim.x) tile_group[i] = -1;
   __syncthreads();
   if (keep) {                                                      // rank within its expert (expert < 0: a pair that runs no expert)
 #pragma unroll
     for (int u = 0; u < KEEP; ++u) rank[u] = ex[u] >= 0 ? atomicAdd(&count[ex[u]], 1) : -1;
   } else {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) pos[i] = idx[i] >= 0 ? atomicAdd(&count[idx[i]], 1) : -1;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int e = expert(i);
+      pos[i] = e >= 0 ? atomicAdd(&count[e], 1) : -1;
+    }
   }
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -177,8 +182,11 @@ __global__ void __launch_bounds__(1024) moe_sort_kernel(const int* __restrict__ 
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += blockDim.x)
-    for (int t = start[e] / tile; t < start[e + 1] / tile; ++t) tile_group[t] = e;
+  if (offsets != nullptr)
+    for (int e = threadIdx.x; e <= E; e += blockDim.x) offsets[e] = start[e];
+  if (tile_group != nullptr)
+    for (int e = threadIdx.x; e < E; e += blockDim.x)
+      for (int t = start[e] / tile; t < start[e + 1] / tile; ++t) tile_group[t] = e;
   if (keep) {
 #pragma unroll
     for (int u = 0; u < KEEP; ++u) {
@@ -191,8 +199,9 @@ __global__ void __launch_bounds__(1024) moe_sort_kernel(const int* __restrict__ 
     return;
   }
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    if (idx[i] < 0) continue;                                      // pos stays -1: the combine pass skips the pair
-    const int at = start[idx[i]] + pos[i];
+    const int e = expert(i);
+    if (e < 0) continue;                                           // pos stays -1: the combine pass skips the pair
+    const int at = start[e] + pos[i];
     pos[i] = at;
     row_src[at] = i / top;
   }
@@ -342,17 +351,25 @@ extern "C" JL_API int jl_moe_route_ex(const float* z, int ldz, int M, int E, int
 // Rows of the sorted layout for n pairs over E experts with row tiles of `tile`: every expert's segment is rounded up.
 extern "C" JL_API int jl_moe_sorted_rows(int n, int E, int tile) { return (n + E * (tile - 1) + tile - 1) / tile * tile; }
 
-extern "C" JL_API int jl_moe_sort(const int* idx, int M, int top, int E, int tile, int cap, int* pos, int* row_src, int* tile_group,
-                                  int* tiles_used, void* stream) {
-  JL_CHECK_ARG(M >= 1 && top >= 1 && E >= 1 && tile >= 1, "jl_moe_sort: bad shape");
-  JL_CHECK_ARG(cap % tile == 0 && cap >= jl_moe_sorted_rows(M * top, E, tile), "jl_moe_sort: %d rows are too few", cap);
+static int moe_sort_launch(const int* idx, int M, int top, int E, int tile, int cap, int* pos, int* row_src, int* tile_group, int* tiles_used, int* offsets,
+                           void* stream) {
   const size_t smem = (size_t)(2 * E + 1) * sizeof(int);
   JL_CHECK_ARG(smem <= 48 * 1024, "jl_moe_sort: %d experts do not fit shared memory", E);
   const int n = M * top;
   auto* kernel = n <= 1024 ? moe_sort_kernel<1> : n <= 4096 ? moe_sort_kernel<4> : moe_sort_kernel<MS_KEEP>;
-  JL_LAUNCH_PDL(kernel, dim3(1), dim3(1024), smem, stream, idx, n, top, E, tile, cap, pos, row_src, tile_group, tiles_used);
+  JL_LAUNCH_PDL(kernel, dim3(1), dim3(1024), smem, stream, idx, n, top, E, tile, cap, pos, row_src, tile_group, tiles_used, offsets);
   JL_CUDA(cudaGetLastError());
   return JL_OK;
+}
+extern "C" JL_API int jl_moe_sort(const int* idx, int M, int top, int E, int tile, int cap, int* pos, int* row_src, int* tile_group,
+                                  int* tiles_used, void* stream) {
+  JL_CHECK_ARG(M >= 1 && top >= 1 && E >= 1 && tile >= 1, "jl_moe_sort: bad shape");
+  JL_CHECK_ARG(cap % tile == 0 && cap >= jl_moe_sorted_rows(M * top, E, tile), "jl_moe_sort: %d rows are too few", cap);
+  return moe_sort_launch(idx, M, top, E, tile, cap, pos, row_src, tile_group, tiles_used, nullptr, stream);
+}
+extern "C" JL_API int jl_moe_order(const int* idx, int M, int top, int E, int* pos, int* row_src, int* offsets, void* stream) {
+  JL_CHECK_ARG(M >= 0 && top >= 1 && E >= 1 && (long long)M * top < (1ll << 31), "jl_moe_order: bad shape M=%d top=%d E=%d", M, top, E);
+  return moe_sort_launch(idx, M, top, E, 1, M * top, pos, row_src, nullptr, nullptr, offsets, stream);
 }
 
 extern "C" JL_API int jl_moe_combine(const float* z, int ldz, const int* pos, const float* wt, int top, const float* shared, int lds,

@@ -592,6 +592,26 @@ int jl_logit_rules(const void* logits, int dtype, int B, int V, int ld, float* o
                    const int* lengths, int lengths_n, const int* prompts, int prompts_n, const float* rep, float rep1, const float* freq, float freq1,
                    const float* pres, float pres1, const int* bias_ids, const float* bias, int n_bias, int ldb, const void* allowed, int lda, void* stream);
 
+/* Layers in 8-bit integers: a row is int8 values q and one fp32 scale s = amax / 127, q = 127 x / amax to the nearest whole number (ties to even), both as 64 bits would
+ * give them; a row of zeros has s = 0, one with an infinity or a NaN s = NaN and q = 0.  Element types 0 bf16, 1 fp32, 2 fp16.
+ *
+ * jl_int8_rows: n rows of x [M, K] (row pitch ldx): row rows[i] (NULL: row i; one that x does not have: zeros), normed first where gain [K] (x's type) is given; q with row
+ * pitch ldq, columns behind K zero.
+ * jl_linear_int8: out [M, N] (gated: [M, N / 2]) = sx sw (qx qw^T) of the rows of x [M, K] and weights wq [N, ldw] / ws [N]; ldw a multiple of 16, the columns behind K not
+ * used.  mode 0 plain, 1 + residual (out's type and size, may be out), 2 silu(y[2j]) y[2j+1].  K <= 131072.  resident: no kernel directly before the call writes the weights.
+ * jl_experts_int8: out[t], offsets[e] <= t < offsets[e + 1], of row rows[t] of x against expert e's weights wq [experts][N][ldw], ws [experts][N]; offsets [experts + 1] on
+ * the device; other rows of out are left as they were.  mode 0 or 2; experts <= 1024.
+ * scratch: jl_int8_scratch_bytes(M, K) (experts: (T, K)) bytes of any content on a 16-byte boundary; calls that may run at the same time need one each. */
+int jl_int8_rows(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int n, const void* gain, float eps, void* q, int ldq, float* s, void* stream);
+size_t jl_int8_scratch_bytes(int rows, int K);
+int jl_linear_int8(const void* x, int dtype, int M, int K, long long ldx, const void* wq, int ldw, const float* ws, int N, const void* gain, float eps,
+                   const void* residual, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int resident, int num_sms, void* stream);
+int jl_experts_int8(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int T, const int* offsets, int experts, const void* wq, int ldw,
+                    const float* ws, int N, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int num_sms, void* stream);
+/* The M * top (token, choice) pairs ordered by expert with nothing between experts: pos [M * top]: row of each pair (-1 where idx < 0); row_src [M * top]: token of each row
+ * (-1 behind the last); offsets [E + 1]: first row of every expert, and behind the last. */
+int jl_moe_order(const int* idx, int M, int top, int E, int* pos, int* row_src, int* offsets, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,10 @@ i32, f32, u64, sz, i64 = C.c_int, C.c_float, C.c_ulonglong, C.c_size_t, C.c_long
 
 _SIGNATURES = {
     "jl_last_error": (C.c_char_p, []),
+    "jl_int8_rows": (i32, [vp, i32, i32, i32, i64, ip, i32, vp, f32, vp, i32, fp, vp]),
+    "jl_int8_scratch_bytes": (sz, [i32, i32]),
+    "jl_linear_int8": (i32, [vp, i32, i32, i32, i64, vp, i32, fp, i32, vp, f32, vp, vp, i32, i32, vp, sz, i32, i32, vp]),
+    "jl_experts_int8": (i32, [vp, i32, i32, i32, i64, ip, i32, ip, i32, vp, i32, fp, i32, vp, i32, i32, vp, sz, i32, vp]),
     "jl_version": (i32, []),
     "jl_launch_count": (u64, []),
     "jl_embed": (i32, [ip, vp, vp, i32, i32, i32, vp]),
@@ -127,6 +131,7 @@ _HYBRID = {
     "jl_mlstm_scan": (i32, [fp, i32, i32, i32, i32, fp, i32, f32, fp, fp, ip, ip] + [i32] * 5 + [fp, vp]),
     "jl_mlstm_finish": (i32, [fp, fp, vp, fp, i32, vp, i32, i32, i32, f32, i32, i32, vp]),
     "jl_delta_scan": (i32, [fp, i32, i32, i32, i32, i32, fp, i32, i32, i32, vp, vp, vp, fp, fp, ip, ip] + [i32] * 6 + [fp, i32, vp]),
+    "jl_moe_order": (i32, [ip, i32, i32, i32, ip, ip, ip, vp]),
     "jl_delta_head_scan_ws_floats": (sz, [i32] * 6),
     "jl_delta_head_scan": (i32, [fp, i32, i32, i32, i32, i32, fp, i32, i32, i32, vp, vp, fp, fp, ip, ip] + [i32] * 5 + [fp, i32, vp]),
 }

@@ -183,7 +183,13 @@ def linear(x: torch.Tensor, w: torch.Tensor, *, norm_w: Optional[torch.Tensor] =
     by token count: M ≤ 4 → register-streaming GEMV with RMSNorm fused (JLLAMA_SMALL_M=gemv_tma selects the
     TMA-ring GEMV, which falls back when the activations do not fit next to its ring), otherwise the tcgen05
     GEMM (swap-AB up to M = 128, and to 256 with few features).  `force` ∈ {"gemv_tma", "gemv", "gemm"} pins the kernel.  Up to 128
-    rows w is a parameter: it is read ahead of this library's kernels directly before the call, which must not write it."""
+    rows w is a parameter: it is read ahead of this library's kernels directly before the call, which must not write it.
+    An `int8.Int8Weight` for w makes it a layer in 8-bit integers (`int8.linear_int8`, with the same contract; no `force`)."""
+    if not isinstance(w, torch.Tensor):
+        from .int8 import linear_int8
+        if force is not None:
+            raise ValueError(f"linear: no path {force!r} for 8-bit weights")
+        return linear_int8(x, w, norm_w=norm_w, eps=eps, residual=residual, mode=mode, out_f32=out_f32, out=out, resident=True)
     if not x.is_cuda:
         return _linear_ref(x, w, norm_w, eps, residual, mode, out_f32)
     _bf16c(x, "x"); _bf16c(w, "w")
