@@ -290,7 +290,11 @@ static int swap_launch(const void* xq, const void* wq, Int8Swap p, int ldx, int 
 int int8_rows(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int n, const void* gain, float eps, void* q, int ldq, float* s, bool early,
               cudaStream_t stream);
 
+int int8_pair(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8Work work, int K, int mode, int num_sms, cudaStream_t stream);
+
 static int product(const void* xq, int ldx, const void* wq, int ldw, Int8Swap p, int mode, int num_sms, cudaStream_t stream) {
+  static const int pair_from = getenv("I8_PAIR") ? atoi(getenv("I8_PAIR")) : 257;
+  if (p.work.offsets == nullptr ? p.work.rows >= pair_from : p.nb == 256) return int8_pair(xq, ldx, wq, ldw, p.o, p.work, p.K, mode, num_sms, stream);
   if (mode == I8_PLAIN) return swap_launch<I8_PLAIN>(xq, wq, p, ldx, ldw, num_sms, stream);
   if (mode == I8_RESIDUAL) return swap_launch<I8_RESIDUAL>(xq, wq, p, ldx, ldw, num_sms, stream);
   return swap_launch<I8_GATED>(xq, wq, p, ldx, ldw, num_sms, stream);
