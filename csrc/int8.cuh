@@ -6,6 +6,9 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "seq_types.cuh"
 
 namespace jl {
@@ -24,6 +27,142 @@ template <> __device__ __forceinline__ __half from_f<__half>(float v) { return _
     else if ((dt) == jl::DT_F32) { using T = float; __VA_ARGS__; }       \
     else { using T = __half; __VA_ARGS__; }                              \
   } while (0)
+
+// the magnitude's bits (for 16-bit types the larger of two, in the upper or lower half)
+template <typename T> __device__ __forceinline__ uint32_t i8r_bits(T v);
+template <> __device__ __forceinline__ uint32_t i8r_bits<float>(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+template <> __device__ __forceinline__ uint32_t i8r_bits<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat16_as_ushort(v) & 0x7fffu; }
+template <> __device__ __forceinline__ uint32_t i8r_bits<__half>(__half v) { return __half_as_ushort(v) & 0x7fffu; }
+template <typename T> __device__ __forceinline__ float i8r_value(uint32_t bits);
+template <> __device__ __forceinline__ float i8r_value<float>(uint32_t b) { return __uint_as_float(b); }
+template <> __device__ __forceinline__ float i8r_value<__nv_bfloat16>(uint32_t b) { return __uint_as_float(b << 16); }
+template <> __device__ __forceinline__ float i8r_value<__half>(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)b)); }
+
+template <typename T>
+__device__ __forceinline__ void i8r_unpack(const uint4& w, float (&v)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 4) {
+    v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+  } else {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __half>) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = bf16_lo(u[i]); v[2 * i + 1] = bf16_hi(u[i]);
+      }
+    }
+  }
+}
+
+// what a row's elements are multiplied with: x * pre * inv = 127 x / amax.  pre lifts rows so small that 127 / amax would overflow.
+struct Int8Quotient {
+  float pre, inv, amax;
+  __device__ __forceinline__ explicit Int8Quotient(float a) {
+    amax = a;
+    pre = a < 0x1p-60f ? 0x1p64f : 1.0f;
+    inv = a > 0.0f && a <= 3.402823466e38f ? __fdiv_rn(127.0f, a * pre) : 0.0f;
+  }
+  __device__ __forceinline__ bool ordinary() const { return amax >= 0x1p-60f && amax <= 3.402823466e38f; }      // (not zero, not tiny, all of them numbers)
+  __device__ __forceinline__ float scale() const { return amax <= 3.402823466e38f ? __fdiv_rn(amax, 127.0f) : __int_as_float(0x7fc00000); }
+  // any row: the value as the low byte of the result
+  __device__ __forceinline__ uint32_t operator()(float x) const {
+    const float t = x * pre * inv;
+    const float magic = t + 12582912.0f;                         // 1.5 * 2^23: the nearest whole number, ties to even, in the low bits
+    uint32_t q = __float_as_uint(magic);
+    if (fabsf(t - (magic - 12582912.0f)) > 0.49997f) {      // (off by at most 1.6e-5)
+      const int k = (int)fabsf(t);                               // between k and k + 1, near the middle
+      const double a = 254.0 * (double)fabsf(x), b = (2.0 * k + 1.0) * (double)amax;
+      const int r = a > b ? k + 1 : a < b ? k : k + (k & 1);
+      q = (uint32_t)(x < 0.0f ? -r : r);
+    }
+    return inv == 0.0f ? 0u : q;                                 // (inf * 0 and NaN go nowhere)
+  }
+};
+
+// Ordinary rows, two elements at a time (packed fp32).  With X = 127 x and a = amax (both by 2^-8, which keeps X finite) the quotient is t0 = X * (1 / a), corrected once by what
+// it leaves: t = t0 + (X - t0 a) (1 / a).  t0 is off by a share d of a few 2^-24, the remainder is taken with one rounding, so t before its own rounding is off by d 2^-24 or so:
+//   * a quotient on the middle k + 1/2, which fp32 holds, comes out as that, and the sum with 1.5 * 2^23 rounds it to the even side;
+//   * rounding t does not carry it over a middle, and onto one only from less than 2^-24 t away.  With x and amax of p bits, exponents e apart, the nearest quotient beside a
+//     middle is 2^(e - p - 1) away, and 2^-24 t is at most 2^(e - 16): never for the 16-bit types (p = 8, 11).
+// fp32 rows can come that near: quotients within I8R_NEAR of a middle are settled.  (16-bit rows meet middles often, amax / 2 is one at every scale: a quarter of all groups
+// of 256 elements.  Settling those too took 313 us for 8192 x 14336, most of it for instructions that were not in the cache.)
+constexpr float I8R_NEAR = 0.49999f;      // (a step of fp32 below 128 is 7.6e-6)
+struct Int8Pairs {
+  uint64_t a, inv;
+  __device__ __forceinline__ explicit Int8Pairs(float amax) {
+    const float lo = amax * 0x1p-8f, r = __fdiv_rn(1.0f, lo);
+    asm("mov.b64 %0, {%1, %1};" : "=l"(a) : "f"(-lo));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(inv) : "f"(r));
+  }
+  // the whole numbers in the low bytes; `off`: how far the worst quotient so far lies from a whole number
+  template <bool OFF>
+  __device__ __forceinline__ void get(float x0, float x1, uint32_t& q0, uint32_t& q1, float& off) const {
+    uint64_t x, t, e, m;
+    const uint64_t c = 0x3efe00003efe0000ull, magic = 0x4b4000004b400000ull;      // 127 / 256 and 1.5 * 2^23, twice
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(x0), "f"(x1));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(x), "l"(c));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x), "l"(inv));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e) : "l"(t), "l"(a), "l"(x));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t) : "l"(e), "l"(inv), "l"(t));
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(m) : "l"(t), "l"(magic));
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(q0), "=r"(q1) : "l"(m));
+    if constexpr (OFF) {
+      float t0, t1;
+      asm("mov.b64 {%0, %1}, %2;" : "=f"(t0), "=f"(t1) : "l"(t));
+      off = fmaxf(off, fmaxf(fabsf(t0 - (__uint_as_float(q0) - 12582912.0f)), fabsf(t1 - (__uint_as_float(q1) - 12582912.0f))));
+    }
+  }
+};
+// The whole number that a rounded quotient of x gave, or the one beside it, exactly: r against 127 x - r amax.  Both products are taken with what their rounding
+// left; near a middle the differences of the large parts are exact, so is that of the small ones, and the last sum has the right sign.
+static __device__ __noinline__ uint4 i8r_settle4(float4 v, uint4 bits, float amax) {
+  const float a = amax * 0x1p-8f, h = 0.5f * a;
+  const float x[4] = {v.x, v.y, v.z, v.w};
+  uint32_t b[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    float r = __uint_as_float(b[i]) - 12582912.0f;
+    const float X = x[i] * 0x1p-8f, hi = 127.0f * X, lo = fmaf(127.0f, X, -hi), hi2 = r * a, lo2 = fmaf(r, a, -hi2);
+    const float d = hi - hi2, e = lo - lo2, over = (d - h) + e, under = (d + h) + e;
+    const bool odd = b[i] & 1;
+    r += over > 0.0f || (over == 0.0f && odd) ? 1.0f : under < 0.0f || (under == 0.0f && odd) ? -1.0f : 0.0f;
+    b[i] = __float_as_uint(r + 12582912.0f);
+  }
+  return make_uint4(b[0], b[1], b[2], b[3]);
+}
+// a piece of an ordinary row.  EXACT: x is what the row holds (rows behind a norm are rounded already)
+template <typename T, bool EXACT>
+__device__ __forceinline__ void i8r_piece(const Int8Pairs& pairs, float amax, const float (&f)[16 / sizeof(T)], uint32_t (&b)[16 / sizeof(T)]) {
+  constexpr int VE = 16 / sizeof(T);
+  float off = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VE; i += 2) pairs.get<EXACT && VE == 4>(f[i], f[i + 1], b[i], b[i + 1], off);
+  if constexpr (EXACT && VE == 4) {
+    if (off > I8R_NEAR) {
+      const uint4 s = i8r_settle4(make_float4(f[0], f[1], f[2], f[3]), make_uint4(b[0], b[1], b[2], b[3]), amax);
+      b[0] = s.x; b[1] = s.y; b[2] = s.z; b[3] = s.w;
+    }
+  }
+}
+__device__ __forceinline__ uint32_t i8r_pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// All of an SM's shared memory for a kernel (asked for once per device)
+template <auto KERNEL>
+static cudaError_t i8_room() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (bit & done.load(std::memory_order_relaxed)) return cudaSuccess;
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // Result, residual and scales of a product
 struct Int8Out {
@@ -53,7 +192,8 @@ __device__ __forceinline__ float2 i8_unpack(int kind, uint32_t w) {
   if (kind == DT_BF16) return make_float2(bf16_lo(w), bf16_hi(w));
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
-__device__ __forceinline__ float i8_gate(float g, float u) { return g * sigmoid_f(g) * u; }
+// silu(g) u.  The quotient is the product with an approximate reciprocal (two units in the last place): a true one branches, and values then wait for one another
+__device__ __forceinline__ float i8_gate(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
 // four neighbouring residuals (index of the first one: a multiple of four where `wide`)
 __device__ __forceinline__ void i8_residual4(const Int8Out& o, size_t at, int f0, float (&r)[4]) {
@@ -114,8 +254,9 @@ struct Int8Work {
 };
 struct Int8Tile { int expert, col, row0, rows; };
 
-// first row of expert e, whatever the offsets say: never outside the rows there are
-__device__ __forceinline__ int i8_offset(const Int8Work& w, int e) { return min(max(w.offsets[e], 0), w.rows); }
+// first row of expert e, whatever the offsets say: never outside the rows there are.  (Read from L2: the caller may not have waited for the kernel ahead, which began
+// when those before it were done.)
+__device__ __forceinline__ int i8_offset(const Int8Work& w, int e) { return min(max(__ldcg(w.offsets + e), 0), w.rows); }
 
 // table[e]: tiles ahead of expert e (experts + 1 of them), table[experts + 1 + e]: its first row (experts + 1).  By one warp.
 __device__ __forceinline__ void i8_list(const Int8Work& w, int* table) {

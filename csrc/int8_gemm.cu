@@ -4,8 +4,12 @@
 // TMEM, two accumulators.  Sums leave through shared memory as [row][feature], so that a thread finishes four neighbouring features of a row: both scales, the
 // residual or the gate, one rounding.  One matrix, or one per expert: rows come ordered by expert, at any row, no padding between experts; a tile of rows that runs
 // past its expert's end computes rows of the next one and does not store them.
-// Few tiles of one matrix: the CTAs of a cluster share one and take a part of K each; the partials meet in distributed shared memory, whole numbers, so their order
+// The launch ahead is always the one that brings the activations to 8 bits, which lets this one start when the kernels before it are done (or, with resident weights, at
+// once): offsets and weights are read without waiting for it.
+// Few tiles: the CTAs of a cluster share one and take a part of K each; the partials meet in distributed shared memory, whole numbers, so their order
 // changes nothing.
+#include <type_traits>
+
 #include "int8.cuh"
 #include "jllama_b200.h"
 #include "tcgen05.cuh"
@@ -14,13 +18,14 @@ namespace jl {
 
 constexpr int I8S_BM = 128, I8S_BK = 128, I8S_THREADS = 256;      // warp 0: TMA, warp 1: MMA, warp 2: TMEM; 4-7 (split: all): results
 constexpr uint32_t I8S_A_BYTES = I8S_BM * I8S_BK, I8S_STAGING = 16 * I8S_BM * 4;
+constexpr int I8S_PARTS = 8;                                      // of K, at most
+constexpr int I8S_HALF = 112 * 1024, I8S_WIDE = 201 * 1024;       // shared memory of a CTA of two an SM, of one
 
 struct Int8Swap {
   Int8Out o;
   Int8Work work;
   int K, nb, stages, ksplit;        // rows of a tile: nb, a multiple of 16
   uint32_t cols, idesc;
-  int early;                        // weights may be read ahead of the wait for the kernels before
 };
 
 __device__ __forceinline__ uint32_t i8s_mapa(uint32_t local_addr, int rank) {
@@ -67,7 +72,6 @@ int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   }
   if (warp == 2) tc::tmem_alloc(tmem_slot, SPLIT ? p.cols : 2 * p.cols);
   if (warp == 3) {
-    if (p.work.offsets != nullptr) pdl_wait();
     i8_list(p.work, table);
   }
   tc::fence_before_sync();
@@ -81,13 +85,13 @@ int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     // ===================================================== TMA producer
     if (lane == 0) {
       int pre = 0;
-      if (p.early && tile0 < tiles) {                           // (one matrix: the first tile's weights are known)
+      if (tile0 < tiles) {                                      // weights do not wait for the activations
         Int8Walk walk;
         const Int8Tile t = walk.at(p.work, table, tile0);
         pre = kb1 - kb0 < stages ? kb1 - kb0 : stages;
         for (int i = 0; i < pre; ++i) {
           tc::mbar_expect_tx(full_bar(i), stage_bytes);
-          tc::tma_load_2d(smem_base + i * stage_bytes, &tmap_w, full_bar(i), (kb0 + i) * I8S_BK, t.col * I8S_BM, tc::EVICT_FIRST);
+          tc::tma_load_2d(smem_base + i * stage_bytes, &tmap_w, full_bar(i), (kb0 + i) * I8S_BK, t.expert * p.o.N + t.col * I8S_BM, tc::EVICT_FIRST);
         }
       }
       pdl_wait();
@@ -186,32 +190,51 @@ int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       }
     }
   } else {
-    // ===================================================== all warps: partial sums meet in the cluster (one matrix, one tile)
+    // ===================================================== all warps: partial sums meet in the cluster (one tile, or none)
     pdl_wait();
     Int8Walk walk;
-    const Int8Tile t = walk.at(p.work, table, tile0);
+    Int8Tile t{0, 0, 0, 0};
+    if (tile0 < tiles) t = walk.at(p.work, table, tile0);
     const int f0 = t.col * I8S_BM + 4 * lane, row = I8S_BM * 4;
     const uint32_t put = smem_base + ((warp & 3) * 32 + lane) * 4, get = smem_base + lane * 16;
     float sw[4];
     feature_scales(t.expert, f0, sw);
-    tc::mbar_wait(tfull_bar(0), 0);
+    if (tile0 < tiles) tc::mbar_wait(tfull_bar(0), 0);
     tc::fence_after_sync();
     // the ring is free (all MMAs done) and takes the partial
     for (int c0 = (warp >> 2) * 16; c0 < t.rows; c0 += 32) to_shared(t_lane + c0, put + c0 * row, row);
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     const int per = (t.rows + ksplit - 1) / ksplit, t_lo = rank * per, t_hi = min(t_lo + per, t.rows);
-    for (int r0 = t_lo + warp; r0 < t_hi; r0 += 8) {
-      int x[4] = {0, 0, 0, 0};
-      int4 part[8];
+    // a warp takes U rows at a time, all ranks' parts of them on their way together
+    auto meet = [&](auto ranks, auto many) {
+      constexpr int R = decltype(ranks)::value, U = decltype(many)::value;
+      for (int r0 = t_lo + warp; r0 < t_hi; r0 += 8 * U) {
+        int4 part[U][R];
+        float sx[U];
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < ksplit) part[r] = i8s_ld_cluster(i8s_mapa(get, r) + r0 * row);
+        for (int u = 0; u < U; ++u) {
+          const int at = r0 + 8 * u;
+          if (at >= t_hi) continue;
+          sx[u] = p.o.xs[t.row0 + at];
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < ksplit) { x[0] += part[r].x; x[1] += part[r].y; x[2] += part[r].z; x[3] += part[r].w; }
-      if (f0 < p.o.N) i8_finish4<MODE>(p.o, t.row0 + r0, f0, x, p.o.xs[t.row0 + r0], sw);
-    }
+          for (int r = 0; r < R; ++r)
+            if (r < ksplit) part[u][r] = i8s_ld_cluster(i8s_mapa(get, r) + at * row);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int at = r0 + 8 * u;
+          if (at >= t_hi) continue;
+          int x[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (r < ksplit) { x[0] += part[u][r].x; x[1] += part[u][r].y; x[2] += part[u][r].z; x[3] += part[u][r].w; }
+          if (f0 < p.o.N) i8_finish4<MODE>(p.o, t.row0 + at, f0, x, sx[u], sw);
+        }
+      }
+    };
+    if (ksplit <= 4) meet(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+    else meet(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");      // no CTA leaves while its partial may still be read
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   }
@@ -224,14 +247,15 @@ static size_t i8s_smem(int stages, int nb, bool split, int experts) {
   return (size_t)stages * (I8S_A_BYTES + nb * I8S_BK) + (split ? 0 : I8S_STAGING) + 8 * (2 * stages + 4) + 16 + 4 * i8_table_ints(experts) + 1024;
 }
 
-// Parts of K, a cluster's CTAs: enough to fill both slots of every SM, at least four k-blocks each
-static int i8s_parts(int nb, int tiles, int num_kb, int num_sms) {
-  const int slots = nb > 128 ? num_sms : 2 * num_sms - 32;
-  int ks = slots / tiles;
-  if (ks > 8) ks = 8;
-  if (nb > 128 && ks > 4) ks = 4;
+// Parts of K, a cluster's CTAs: up to eight of at least four k-blocks that fill both slots of nearly every SM; clusters find place for about 264 CTAs (48 tiles of 100 rows, K 4096: 5
+// parts 12.6 us, 6 parts 18.5; 32 tiles of 6 rows, K 14336: 2 parts 20.7, 4 15.2, 8 13.1).  Above 128 rows a CTA fills an SM: up to four, for about 128.
+static int i8s_parts(int nb, long long tiles, int num_kb, int num_sms) {
+  const int slots = nb > 128 ? num_sms - 20 : 2 * num_sms - 32;
+  long long ks = slots / tiles;
+  const int most = nb > 128 ? 4 : I8S_PARTS;
+  if (ks > most) ks = most;
   if (ks > num_kb / 4) ks = num_kb / 4;
-  return ks > 1 ? ks : 1;
+  return ks > 1 ? (int)ks : 1;
 }
 
 template <int MODE>
@@ -243,12 +267,12 @@ static int swap_launch(const void* xq, const void* wq, Int8Swap p, int ldx, int 
   const int num_kb = (p.K + I8S_BK - 1) / I8S_BK;
   const long long most = (long long)p.work.cols * ((p.work.rows + p.nb - 1) / p.nb + (grouped ? (E < p.work.rows ? E : p.work.rows) : 0));      // tiles, at most
   JL_CHECK_ARG(most < (1ll << 30), "int8 product: %lld tiles", most);
-  p.ksplit = grouped || p.work.rows > p.nb ? 1 : i8s_parts(p.nb, (int)most, num_kb, num_sms);
+  p.ksplit = i8s_parts(p.nb, most, num_kb, num_sms);
   const bool split = p.ksplit > 1;
   p.cols = p.nb <= 32 ? 32 : p.nb <= 64 ? 64 : p.nb <= 128 ? 128 : 256;
   p.idesc = tc::idesc_s8_s32(I8S_BM, p.nb);
   const int stage = (int)I8S_A_BYTES + p.nb * I8S_BK, room = 4 * i8_table_ints(E) + (split ? 0 : (int)I8S_STAGING);
-  int stages = ((p.nb > 128 ? 200 * 1024 : 110 * 1024) - room) / stage;
+  int stages = ((p.nb > 128 ? I8S_WIDE : I8S_HALF) - 2048 - room) / stage;      // (2 KB: barriers, alignment)
   if (stages > 10) stages = 10;
   const int slots = p.nb <= 128 ? 2 * num_sms : num_sms;
   const long long blocks = split ? (num_kb + p.ksplit - 1) / p.ksplit : (most + slots - 1) / slots * num_kb;
@@ -262,7 +286,7 @@ static int swap_launch(const void* xq, const void* wq, Int8Swap p, int ldx, int 
   if ((rc = make_tmap_2d_i8(&tx, xq, p.work.rows, p.K, ldx, p.nb))) return rc;
   const size_t smem = i8s_smem(stages, p.nb, split, E);
   auto kern = split ? int8_swap_kernel<MODE, true> : int8_swap_kernel<MODE, false>;
-  JL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  JL_CUDA(split ? (i8_room<int8_swap_kernel<MODE, true>>()) : (i8_room<int8_swap_kernel<MODE, false>>()));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(split ? most * p.ksplit : most < slots ? most : slots));
   cfg.blockDim = dim3(I8S_THREADS);
@@ -287,14 +311,17 @@ static int swap_launch(const void* xq, const void* wq, Int8Swap p, int ldx, int 
   return JL_OK;
 }
 
-int int8_rows(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int n, const void* gain, float eps, void* q, int ldq, float* s, bool early,
+int int8_rows(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int n, const void* gain, float eps, void* q, int ldq, float* s, int early,
               cudaStream_t stream);
 
+bool int8_vec_takes(int rows, int N, int K);
+int int8_vec(const void* x, int dtype, long long ldx, const void* gain, float eps, const void* wq, int ldw, Int8Out o, int rows, int K, int mode, bool early, int num_sms,
+             cudaStream_t stream);
 int int8_pair(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8Work work, int K, int mode, int num_sms, cudaStream_t stream);
 
-static int product(const void* xq, int ldx, const void* wq, int ldw, Int8Swap p, int mode, int num_sms, cudaStream_t stream) {
-  static const int pair_from = getenv("I8_PAIR") ? atoi(getenv("I8_PAIR")) : 257;
-  if (p.work.offsets == nullptr ? p.work.rows >= pair_from : p.nb == 256) return int8_pair(xq, ldx, wq, ldw, p.o, p.work, p.K, mode, num_sms, stream);
+static int int8_swap(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8Work work, int K, int nb, int mode, int num_sms, cudaStream_t stream) {
+  Int8Swap p{};
+  p.o = o; p.work = work; p.K = K; p.nb = nb;
   if (mode == I8_PLAIN) return swap_launch<I8_PLAIN>(xq, wq, p, ldx, ldw, num_sms, stream);
   if (mode == I8_RESIDUAL) return swap_launch<I8_RESIDUAL>(xq, wq, p, ldx, ldw, num_sms, stream);
   return swap_launch<I8_GATED>(xq, wq, p, ldx, ldw, num_sms, stream);
@@ -314,8 +341,9 @@ static Int8Out out_of(void* out, const void* residual, const float* xs, const fl
 
 using namespace jl;
 
-// bytes that jl_linear_int8 (rows = M) and jl_experts_int8 need beside their operands: the activations' values (rows on 16 bytes) and scales
+// bytes that jl_linear_int8 and jl_experts_int8 need beside their operands: the activations' values (rows on 16 bytes) and scales
 extern "C" JL_API size_t jl_int8_scratch_bytes(int rows, int K) { return rows < 0 || K < 1 ? 0 : ((size_t)rows * up16(K) + 255) / 256 * 256 + (size_t)rows * 4; }
+extern "C" JL_API size_t jl_linear_int8_scratch_bytes(int M, int N, int K) { return int8_vec_takes(M, N, K) ? 0 : jl_int8_scratch_bytes(M, K); }
 
 extern "C" JL_API int jl_linear_int8(const void* x, int dtype, int M, int K, long long ldx, const void* wq, int ldw, const float* ws, int N, const void* gain, float eps,
                                      const void* residual, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int resident, int num_sms, void* stream) {
@@ -325,19 +353,26 @@ extern "C" JL_API int jl_linear_int8(const void* x, int dtype, int M, int K, lon
   JL_CHECK_ARG(mode >= I8_PLAIN && mode <= I8_GATED && (mode == I8_RESIDUAL) == (residual != nullptr) && (mode != I8_GATED || N % 2 == 0),
                "jl_linear_int8: mode %d with%s residual, N=%d", mode, residual != nullptr ? "" : "out", N);
   if (M == 0) return JL_OK;
-  JL_CHECK_ARG(scratch != nullptr && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= jl_int8_scratch_bytes(M, K), "jl_linear_int8: scratch of %zu bytes", scratch_bytes);
   if (num_sms <= 0) num_sms = SMS;
+  if (int8_vec_takes(M, N, K)) {
+    const Int8Out o = out_of(out, residual, nullptr, ws, out_dtype, N, mode);
+    return int8_vec(x, dtype, M > 1 ? ldx : K, gain, eps, wq, ldw, o, M, K, mode, resident != 0, num_sms, (cudaStream_t)stream);
+  }
+  JL_CHECK_ARG(scratch != nullptr && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= jl_linear_int8_scratch_bytes(M, N, K), "jl_linear_int8: scratch of %zu bytes", scratch_bytes);
   const int ldq = up16(K);
   float* xs = reinterpret_cast<float*>((uint8_t*)scratch + ((size_t)M * ldq + 255) / 256 * 256);
   int rc;
-  if ((rc = int8_rows(x, dtype, M, K, ldx, nullptr, M, gain, eps, scratch, ldq, xs, true, (cudaStream_t)stream))) return rc;
-  Int8Swap p{};
-  p.o = out_of(out, residual, xs, ws, out_dtype, N, mode);
-  p.work = Int8Work{nullptr, 1, M, 0, 0};
-  p.K = K;
-  p.nb = M >= 256 ? 256 : (M + 15) / 16 * 16;
-  p.early = 1;                      // the kernel ahead is the one above, and it began when those before it were done
-  return product(scratch, ldq, wq, ldw, p, mode, num_sms, (cudaStream_t)stream);
+  if ((rc = int8_rows(x, dtype, M, K, ldx, nullptr, M, gain, eps, scratch, ldq, xs, resident ? 2 : 1, (cudaStream_t)stream))) return rc;
+  const Int8Out o = out_of(out, residual, xs, ws, out_dtype, N, mode);
+  const Int8Work work{nullptr, 1, M, 0, 0};
+  const int chunks = (M + 255) / 256, nb = ((M + chunks - 1) / chunks + 15) / 16 * 16;
+  // Up to 128 rows weights fill the MMA's rows; up to 512 where K, split over clusters, then gives every SM work and is long enough to pay for the meeting; pairs above (us,
+  // weights as rows | pairs: 130 x 4096 x 4096 10.7 | 16.9; 256 x 4096 x 4096 14.5 | 17.3; 512 x 4096 x 4096 17.2 | 18.4; 400 x 2048 x 2048 11.0 | 12.0; 200 x 1024 x 1024
+  // 9.2 | 7.2; 333 x 1000 x 960 8.9 | 7.5; no parts: 256 x 28672 x 4096 46 | 34; 333 x 6144 x 4096 21.0 | 19.3).
+  const long long tiles = (long long)((N + I8S_BM - 1) / I8S_BM) * chunks;
+  if (M <= 128 || (M <= 512 && K >= 2048 && i8s_parts(nb, tiles, 16, num_sms) > 1))
+    return int8_swap(scratch, ldq, wq, ldw, o, work, K, nb, mode, num_sms, (cudaStream_t)stream);
+  return int8_pair(scratch, ldq, wq, ldw, o, work, K, mode, num_sms, (cudaStream_t)stream);
 }
 
 extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int T, const int* offsets, int experts, const void* wq, int ldw,
@@ -355,13 +390,14 @@ extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, lo
   const int ldq = up16(K);
   float* xs = reinterpret_cast<float*>((uint8_t*)scratch + ((size_t)T * ldq + 255) / 256 * 256);
   int rc;
-  if ((rc = int8_rows(x, dtype, M, K, ldx, rows, T, nullptr, 0.0f, scratch, ldq, xs, true, (cudaStream_t)stream))) return rc;
-  Int8Swap p{};
-  p.o = out_of(out, nullptr, xs, ws, out_dtype, N, mode);
-  p.work = Int8Work{offsets, experts, T, 0, 0};
-  p.K = K;
-  const int even = (T + experts - 1) / experts;                 // rows of an expert if all have the same
-  p.nb = even <= 8 ? 16 : even <= 32 ? 64 : even <= 64 ? 128 : 256;
-  p.early = 0;
-  return product(scratch, ldq, wq, ldw, p, mode, num_sms, (cudaStream_t)stream);
+  if ((rc = int8_rows(x, dtype, M, K, ldx, rows, T, nullptr, 0.0f, scratch, ldq, xs, 1, (cudaStream_t)stream))) return rc;
+  const Int8Out o = out_of(out, nullptr, xs, ws, out_dtype, N, mode);
+  const Int8Work work{offsets, experts, T, 0, 0};
+  // Rows of a tile by the rows that an expert has if all have the same (us with 16, 32, 64, 128 rows | pairs, 32 experts of 2048 x 2048: 2 rows 18.6, 17.9, 16.9, 16.9 | 25.8; 32
+  // rows 29.6, 25.9, 26.7, 28.0 | 40.6; 64 rows 43.6, 32.1, 29.1, 33.5 | 38.4; 128 rows 77.6, 48.1, 38.2, 41.8 | 42.9; 256 rows 145, 83, 60.4, 63.5 | 56.9); 16 wherever that
+  // gives no more tiles than there are slots (8 experts of 1024 x 512, 50 rows: 7.2, 7.5, 9.2, 12.7 | 13.8).
+  const int even = (T + experts - 1) / experts;
+  const long long tiles = (long long)((N + I8S_BM - 1) / I8S_BM) * ((T + 15) / 16 + (experts < T ? experts : T));
+  if (even > 160 && tiles > 2 * num_sms) return int8_pair(scratch, ldq, wq, ldw, o, work, K, mode, num_sms, (cudaStream_t)stream);
+  return int8_swap(scratch, ldq, wq, ldw, o, work, K, tiles <= 2 * num_sms || even <= 1 ? 16 : even <= 24 ? 32 : 64, mode, num_sms, (cudaStream_t)stream);
 }

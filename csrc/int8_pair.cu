@@ -13,15 +13,17 @@
 namespace jl {
 
 constexpr int I8P_BM = 128, I8P_BN = 256, I8P_BK = 128, I8P_THREADS = 384;      // rows per CTA; features per pair; warps: 0 TMA, 1 MMA (leader), 2 TMEM, 3 the list, 4-11 results
-constexpr uint32_t I8P_A_BYTES = I8P_BM * I8P_BK, I8P_B_BYTES = I8P_BN / 2 * I8P_BK, I8P_STAGE = I8P_A_BYTES + I8P_B_BYTES;
-constexpr uint32_t I8P_EPI = 8 * (4096 + 512);             // of each warp: 32 rows of 128 bytes, the scales of 128 features
-constexpr int I8P_STAGES = 5;
+constexpr uint32_t I8P_A_BYTES = I8P_BM * I8P_BK;
+constexpr uint32_t I8P_EPI = 8 * 4096;                     // of each warp: 32 rows of 128 bytes
+constexpr int I8P_STAGES = 8;                              // at most
+constexpr size_t I8P_SMEM = 227 * 1024;
 constexpr uint32_t I8P_LEADER = 0xFEFFFFFFu;               // shared::cluster address of the same offset in CTA 0
 
 struct Int8Pair {
   Int8Out o;
   Int8Work work;
-  int K, stages;
+  int K, stages, bn;              // bn: features of a tile, a multiple of 32
+  uint32_t idesc;
 };
 
 __device__ __forceinline__ uint32_t i8p_mapa(uint32_t local_smem_addr, uint32_t rank) {
@@ -69,10 +71,9 @@ template <typename T, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
 int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Int8Pair p) {
   extern __shared__ uint8_t smem_raw[];
-  constexpr uint32_t IDESC = tc::idesc_s8_s32(2 * I8P_BM, I8P_BN);
   const uint32_t smem_base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
   const int stages = p.stages;
-  const uint32_t epi_smem = smem_base + stages * I8P_STAGE, bars = epi_smem + I8P_EPI;       // full[stages] | empty[stages] | tfull[2] | tempty[2]
+  const uint32_t stage_bytes = I8P_A_BYTES + (uint32_t)p.bn / 2 * I8P_BK, epi_smem = smem_base + stages * stage_bytes, bars = epi_smem + I8P_EPI;       // full[stages] | empty[stages] | tfull[2] | tempty[2]
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (stages + s); };
   auto tfull_bar = [&](int s) { return bars + 8u * (2 * stages + s); };
@@ -108,7 +109,6 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   if (warp == 3) {
-    if (p.work.offsets != nullptr) pdl_wait();
     i8_list(p.work, table);
   }
   tc::fence_before_sync();
@@ -126,11 +126,11 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
       int stage = 0; uint32_t phase = 0;
       for (int t = pair; t < tiles; t += n_pairs) {
         const Int8Tile tile = walk.at(p.work, table, t);
-        const int x_row = tile.row0 + (int)rank * I8P_BM, w_row = tile.expert * p.o.N + tile.col * I8P_BN + (int)rank * (I8P_BN / 2);
+        const int x_row = tile.row0 + (int)rank * I8P_BM, w_row = tile.expert * p.o.N + tile.col * p.bn + (int)rank * (p.bn / 2);
         for (int kb = 0; kb < num_kb; ++kb) {
           tc::mbar_wait(empty_bar(stage), phase ^ 1);
-          const uint32_t sa = smem_base + stage * I8P_STAGE, sb = sa + I8P_A_BYTES;
-          if (rank == 0) tc::mbar_expect_tx(full_bar(stage), 2 * I8P_STAGE);      // both CTAs' bytes
+          const uint32_t sa = smem_base + stage * stage_bytes, sb = sa + I8P_A_BYTES;
+          if (rank == 0) tc::mbar_expect_tx(full_bar(stage), 2 * stage_bytes);      // both CTAs' bytes
           else i8p_remote_arrive(i8p_mapa(full_bar(stage), 0));
           i8p_load(sa, &tmap_x, full_bar(stage), kb * I8P_BK, x_row, tc::EVICT_NORMAL);
           i8p_load(sb, &tmap_w, full_bar(stage), kb * I8P_BK, w_row, tc::EVICT_LAST);
@@ -150,10 +150,10 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
         for (int kb = 0; kb < num_kb; ++kb) {
           tc::mbar_wait(full_bar(stage), phase);
           tc::fence_after_sync();
-          const uint32_t sa = smem_base + stage * I8P_STAGE;
+          const uint32_t sa = smem_base + stage * stage_bytes;
           const uint64_t da = tc::smem_desc_kmajor_sw128(sa), db = tc::smem_desc_kmajor_sw128(sa + I8P_A_BYTES);
 #pragma unroll
-          for (int k = 0; k < I8P_BK / 32; ++k) i8p_mma(d, da + 2 * k, db + 2 * k, IDESC, kb != 0 || k != 0);
+          for (int k = 0; k < I8P_BK / 32; ++k) i8p_mma(d, da + 2 * k, db + 2 * k, p.idesc, kb != 0 || k != 0);
           i8p_commit_both(empty_bar(stage));                // frees the slot in both CTAs when these MMAs retire
           if (++stage == stages) { stage = 0; phase ^= 1; }
         }
@@ -163,84 +163,106 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   } else if (warp >= 4) {
     // ===================================================== results: TMEM -> registers -> shared memory -> whole lines; four warps a half of the features
     const int quarter = warp & 3, part = (warp >> 2) - 1;   // TMEM lanes [32 quarter, 32 quarter + 32)
-    uint8_t* const mine = smem + (epi_smem - smem_base) + (warp - 4) * (4096 + 512);
-    float* const scales = reinterpret_cast<float*>(mine + 4096);
+    uint8_t* const mine = smem + (epi_smem - smem_base) + (warp - 4) * 4096;
     const uint32_t tempty_leader = i8p_mapa(tempty_bar(0), 0);
     constexpr int PER = 128 / sizeof(T);                    // results of a 128-byte row
     constexpr int STEP = MODE == I8_GATED ? 2 * PER : PER;  // accumulator columns for them
+    constexpr int AT = MODE == I8_PLAIN && STEP >= 64 ? 2 : 1;      // reads of 32 columns under way at once (two with the rest spill)
     const T* const residual = reinterpret_cast<const T*>(p.o.residual);
     T* const out = reinterpret_cast<T*>(p.o.out);
-    const int out_n = MODE == I8_GATED ? p.o.N / 2 : p.o.N;
     Int8Walk walk;
     int it = 0;
     for (int t = pair; t < tiles; t += n_pairs, ++it) {
       const Int8Tile tile = walk.at(p.work, table, t);
       const int as = it & 1;
       const int first = (int)rank * I8P_BM + quarter * 32;               // of the tile's rows, this warp's first
-      const int n0 = tile.col * I8P_BN + part * 128;                     // and its first feature
+      const int n0 = tile.col * p.bn, n_end = min(n0 + p.bn, p.o.N);      // the tile's features
       const int rows = tile.rows - first;                                // how many of its 32 there are
       const size_t row0 = (size_t)tile.row0 + first;
-      __syncwarp();
-      {
-        const float* s = p.o.ws + (size_t)tile.expert * p.o.N;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) scales[lane + 32 * i] = n0 + lane + 32 * i < p.o.N ? s[n0 + lane + 32 * i] : 0.0f;
-      }
+      const float* const ws = p.o.ws + (size_t)tile.expert * p.o.N;
+      const bool four = (((uintptr_t)(ws + n0)) & 15) == 0;              // scales of four features in one access
       const float sx = lane < rows ? p.o.xs[row0 + lane] : 0.0f;
-      __syncwarp();
       tc::mbar_wait(tfull_bar(as), (it >> 1) & 1);
       tc::fence_after_sync();
-      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + as * I8P_BN + part * 128;
-      if (rows > 0 && n0 < p.o.N) {
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + as * I8P_BN;
+      if (rows > 0) {
 #pragma unroll 1
-        for (int c0 = 0; c0 < 128; c0 += STEP) {
-          if (n0 + c0 >= p.o.N) break;
-          uint32_t w[32];
+        for (int c0 = part * STEP; n0 + c0 < n_end; c0 += 2 * STEP) {     // the two halves of the warps take turns
+          uint32_t w[32], own[MODE == I8_RESIDUAL ? 32 : 1];
+          if constexpr (MODE == I8_RESIDUAL) {
+            if (p.o.wide && lane < rows) {                  // the line of the lane's row, all of it at once
+              const T* r = residual + (row0 + lane) * p.o.ldo + n0 + c0;
 #pragma unroll
-          for (int h = 0; h < STEP / 32; ++h) {
-            uint32_t v[32];
-            float y[32];
-            uint4 res[MODE == I8_RESIDUAL ? (int)sizeof(T) * 2 : 1];
-            const int col = n0 + c0 + h * 32;
-            if constexpr (MODE == I8_RESIDUAL) {
-              if (p.o.wide && lane < rows) {
-#pragma unroll
-                for (int j = 0; j < (int)sizeof(T) * 2; ++j)
-                  if (col + j * (16 / (int)sizeof(T)) < p.o.N) res[j] = *reinterpret_cast<const uint4*>(residual + (row0 + lane) * p.o.ldo + col + j * (16 / (int)sizeof(T)));
+              for (int j = 0; j < 8; ++j) {
+                const uint4 q = n0 + c0 + j * (16 / (int)sizeof(T)) < n_end ? reinterpret_cast<const uint4*>(r)[j] : make_uint4(0, 0, 0, 0);
+                own[4 * j] = q.x; own[4 * j + 1] = q.y; own[4 * j + 2] = q.z; own[4 * j + 3] = q.w;
               }
             }
-            tc::tmem_ld32(t_row + c0 + h * 32, v);
+          }
+#pragma unroll
+          for (int h0 = 0; h0 < STEP / 32; h0 += AT) {
+            uint32_t v[AT][32];
+#pragma unroll
+            for (int a = 0; a < AT; ++a) tc::tmem_ld32(t_row + c0 + (h0 + a) * 32, v[a]);
+            float4 sw[AT][8];
+#pragma unroll
+            for (int a = 0; a < AT; ++a) {
+              const int col = n0 + c0 + (h0 + a) * 32;
+              if (four && col + 31 < n_end) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sw[a][j] = *reinterpret_cast<const float4*>(ws + col + 4 * j);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  sw[a][j].x = col + 4 * j < n_end ? ws[col + 4 * j] : 0.0f;
+                  sw[a][j].y = col + 4 * j + 1 < n_end ? ws[col + 4 * j + 1] : 0.0f;
+                  sw[a][j].z = col + 4 * j + 2 < n_end ? ws[col + 4 * j + 2] : 0.0f;
+                  sw[a][j].w = col + 4 * j + 3 < n_end ? ws[col + 4 * j + 3] : 0.0f;
+                }
+              }
+            }
             tc::tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 sw = *reinterpret_cast<const float4*>(scales + c0 + h * 32 + j);
-              y[j] = __int2float_rn((int)v[j]) * sx * sw.x;
-              y[j + 1] = __int2float_rn((int)v[j + 1]) * sx * sw.y;
-              y[j + 2] = __int2float_rn((int)v[j + 2]) * sx * sw.z;
-              y[j + 3] = __int2float_rn((int)v[j + 3]) * sx * sw.w;
-            }
-            if constexpr (MODE == I8_RESIDUAL) {
-              if (p.o.wide) {
-                const T* r = reinterpret_cast<const T*>(res);
+            for (int a = 0; a < AT; ++a) {
+              const int h = h0 + a, col = n0 + c0 + h * 32;
+              float y[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) y[j] += to_f(r[j]);
-              } else if (lane < rows) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (col + j < p.o.N) y[j] += to_f(residual[(row0 + lane) * p.o.ldo + col + j]);
+              for (int j = 0; j < 32; j += 4) {
+                y[j] = __int2float_rn((int)v[a][j]) * sx * sw[a][j / 4].x;
+                y[j + 1] = __int2float_rn((int)v[a][j + 1]) * sx * sw[a][j / 4].y;
+                y[j + 2] = __int2float_rn((int)v[a][j + 2]) * sx * sw[a][j / 4].z;
+                y[j + 3] = __int2float_rn((int)v[a][j + 3]) * sx * sw[a][j / 4].w;
               }
-            }
-            if constexpr (MODE == I8_GATED) {
+              if constexpr (MODE == I8_RESIDUAL) {
+                if (p.o.wide) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) y[j] = i8_gate(y[2 * j], y[2 * j + 1]);
-            }
-            constexpr int Y = MODE == I8_GATED ? 16 : 32;     // results of these 32 columns
-            if constexpr (sizeof(T) == 4) {
+                  for (int j = 0; j < 32; ++j) {
+                    if constexpr (sizeof(T) == 4) {
+                      y[j] += __uint_as_float(own[j]);
+                    } else {
+                      const uint32_t q = own[h * 16 + j / 2];
+                      if constexpr (std::is_same_v<T, __half>) y[j] += __half2float(__ushort_as_half((unsigned short)(j & 1 ? q >> 16 : q)));
+                      else y[j] += j & 1 ? bf16_hi(q) : bf16_lo(q);
+                    }
+                  }
+                } else if (lane < rows) {
 #pragma unroll
-              for (int j = 0; j < Y; ++j) w[h * Y + j] = __float_as_uint(y[j]);
-            } else {
+                  for (int j = 0; j < 32; ++j)
+                    if (col + j < n_end) y[j] += to_f(residual[(row0 + lane) * p.o.ldo + col + j]);
+                }
+              }
+              if constexpr (MODE == I8_GATED) {
 #pragma unroll
-              for (int j = 0; j < Y / 2; ++j) w[h * Y / 2 + j] = i8p_pack<T>(y[2 * j], y[2 * j + 1]);
+                for (int j = 0; j < 16; ++j) y[j] = i8_gate(y[2 * j], y[2 * j + 1]);
+              }
+              constexpr int Y = MODE == I8_GATED ? 16 : 32;     // results of these 32 columns
+              if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int j = 0; j < Y; ++j) w[h * Y + j] = __float_as_uint(y[j]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < Y / 2; ++j) w[h * Y / 2 + j] = i8p_pack<T>(y[2 * j], y[2 * j + 1]);
+              }
             }
           }
           __syncwarp();                                     // what was in the buffer has been read
@@ -248,14 +270,14 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
           for (int j = 0; j < 8; ++j)                       // 16-byte chunks, turned by the row so that a warp's accesses meet all banks
             *reinterpret_cast<uint4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
           __syncwarp();
-          const int o0 = MODE == I8_GATED ? (n0 + c0) / 2 : n0 + c0;     // first result column of the 128 bytes
+          const int o0 = MODE == I8_GATED ? (n0 + c0) / 2 : n0 + c0, o_end = MODE == I8_GATED ? n_end / 2 : n_end;      // result columns of the 128 bytes
           if (p.o.wide) {
             const int j = lane & 7, col = o0 + j * (16 / (int)sizeof(T));
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int r = i * 4 + (lane >> 3);
               const uint4 q = *reinterpret_cast<const uint4*>(mine + r * 128 + ((j ^ (r & 7)) << 4));
-              if (r < rows && col < out_n) *reinterpret_cast<uint4*>(out + (row0 + r) * p.o.ldo + col) = q;
+              if (r < rows && col < o_end) *reinterpret_cast<uint4*>(out + (row0 + r) * p.o.ldo + col) = q;
             }
           } else {
             for (int r = 0; r < 32 && r < rows; ++r) {
@@ -263,7 +285,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
               for (int c = lane; c < PER; c += 32) {
                 const int byte = c * (int)sizeof(T);
                 const T q = *reinterpret_cast<const T*>(mine + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
-                if (o0 + c < out_n) out[(row0 + r) * p.o.ldo + o0 + c] = q;
+                if (o0 + c < o_end) out[(row0 + r) * p.o.ldo + o0 + c] = q;
               }
             }
           }
@@ -281,16 +303,19 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
 }
 
-static size_t i8p_smem(int stages, int experts) { return (size_t)stages * I8P_STAGE + I8P_EPI + 8 * (2 * stages + 4) + 16 + 4 * i8_table_ints(experts) + 1024; }
+static size_t i8p_smem(int stages, int bn, int experts) { return (size_t)stages * (I8P_A_BYTES + bn / 2 * I8P_BK) + I8P_EPI + 8 * (2 * stages + 4) + 16 + 4 * i8_table_ints(experts) + 1024; }
 
 using Int8PairKernel = void (*)(const CUtensorMap, const CUtensorMap, const Int8Pair);
 template <typename T>
-static Int8PairKernel pair_kernel(int mode) {
-  return mode == I8_PLAIN ? int8_pair_kernel<T, I8_PLAIN> : mode == I8_RESIDUAL ? int8_pair_kernel<T, I8_RESIDUAL> : int8_pair_kernel<T, I8_GATED>;
+static cudaError_t pair_kernel(int mode, Int8PairKernel* k) {
+  if (mode == I8_PLAIN) { *k = int8_pair_kernel<T, I8_PLAIN>; return i8_room<int8_pair_kernel<T, I8_PLAIN>>(); }
+  if (mode == I8_RESIDUAL) { *k = int8_pair_kernel<T, I8_RESIDUAL>; return i8_room<int8_pair_kernel<T, I8_RESIDUAL>>(); }
+  *k = int8_pair_kernel<T, I8_GATED>;
+  return i8_room<int8_pair_kernel<T, I8_GATED>>();
 }
 
 // Clusters that can be resident at once: the tile loop is persistent, a pair that starts when another one is done doubles the time.  Asked once per device.
-static int i8p_resident(Int8PairKernel kern, size_t smem, int num_sms) {
+static int i8p_resident(Int8PairKernel kern, int num_sms) {
   constexpr int DEVICES = 16;
   static std::atomic<int> known[DEVICES];
   int dev = 0, n = 0;
@@ -299,7 +324,7 @@ static int i8p_resident(Int8PairKernel kern, size_t smem, int num_sms) {
   if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(I8P_THREADS);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = I8P_SMEM;
     cfg.gridDim = dim3((num_sms / 2) * 2);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -311,28 +336,41 @@ static int i8p_resident(Int8PairKernel kern, size_t smem, int num_sms) {
   return n < num_sms / 2 ? n : num_sms / 2;
 }
 
+// Features of a tile: 256, or fewer where that saves more than it costs in rounds of tiles over the pairs.  A k-block takes 406 ns with 256 features, 375 with 192, 345 with
+// 128 (2048 x 6144 x 4096): what does not shrink with the features is worth 600 of them.
+static int i8p_features(const Int8Out& o, const Int8Work& work, int pairs) {
+  const long long pieces = (work.rows + work.chunk - 1) / work.chunk + (work.offsets != nullptr ? work.experts / 2 : 0);
+  int best = I8P_BN;
+  long long least = 0;
+  for (int bn = I8P_BN; bn >= 64; bn -= 32) {
+    const long long rounds = (pieces * ((o.N + bn - 1) / bn) + pairs - 1) / pairs, cost = rounds * (bn + 600);
+    if (bn == I8P_BN || cost < least) { best = bn; least = cost; }
+  }
+  return best;
+}
+
 int int8_pair(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8Work work, int K, int mode, int num_sms, cudaStream_t stream) {
   Int8Pair p{};
   // 16-byte pieces of rows of results (and residuals)
   const int size = o.kind == DT_F32 ? 4 : 2, out_n = mode == I8_GATED ? o.N / 2 : o.N;
   o.wide = (out_n * size) % 16 == 0 && (((uintptr_t)o.out | (uintptr_t)o.residual) & 15) == 0;
   work.chunk = 2 * I8P_BM;
-  work.cols = (o.N + I8P_BN - 1) / I8P_BN;
+  Int8PairKernel kern = nullptr;
+  JL_DISPATCH_INT8(o.kind, JL_CUDA(pair_kernel<T>(mode, &kern)));
+  const int pairs = i8p_resident(kern, num_sms), E = work.experts;
+  p.bn = i8p_features(o, work, pairs);
+  work.cols = (o.N + p.bn - 1) / p.bn;
   p.o = o; p.work = work; p.K = K;
-  const int E = work.experts;
+  p.idesc = tc::idesc_s8_s32(2 * I8P_BM, p.bn);
   const long long most = (long long)work.cols * ((work.rows + work.chunk - 1) / work.chunk + (work.offsets != nullptr ? (E < work.rows ? E : work.rows) : 0));
   JL_CHECK_ARG(most < (1ll << 30), "int8 product: %lld tiles", most);
   CUtensorMap tx, tw;
   int rc;
   if ((rc = make_tmap_2d_i8(&tx, xq, work.rows, K, ldx, I8P_BM))) return rc;
-  if ((rc = make_tmap_2d_i8(&tw, wq, (uint64_t)o.N * E, K, ldw, I8P_BN / 2))) return rc;
+  if ((rc = make_tmap_2d_i8(&tw, wq, (uint64_t)o.N * E, K, ldw, p.bn / 2))) return rc;
   p.stages = I8P_STAGES;
-  const size_t smem = i8p_smem(p.stages, E);
-  Int8PairKernel kern;
-  JL_DISPATCH_INT8(o.kind, kern = pair_kernel<T>(mode));
-  JL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  const int pairs = i8p_resident(kern, smem, num_sms);
-  JL_CUDA(launch_pdl(kern, dim3(2 * (unsigned)(most < pairs ? most : pairs)), dim3(I8P_THREADS), smem, stream, tx, tw, p));
+  while (i8p_smem(p.stages, p.bn, E) > I8P_SMEM) --p.stages;
+  JL_CUDA(launch_pdl(kern, dim3(2 * (unsigned)(most < pairs ? most : pairs)), dim3(I8P_THREADS), i8p_smem(p.stages, p.bn, E), stream, tx, tw, p));
   return JL_OK;
 }
 

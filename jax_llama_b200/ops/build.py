@@ -27,7 +27,7 @@ STAMP = OUT_DIR / "build.stamp"
 
 # Sources whose arithmetic has to be exact float32 (true division, expf, tanhf, sqrtf): built without --use_fast_math.
 PRECISE_SOURCES = {"gemm_group.cu", "seq_norm.cu", "seq_linear.cu", "linear_f32.cu", "linear_f32_pair.cu", "attn_generic.cu", "flash_wide.cu", "gla_scan.cu", "gla_chunk.cu", "moe.cu", "seq_mix.cu",
-                   "delta_scan.cu", "delta_chunk.cu", "seq_token.cu", "logit_rules.cu", "int8_rows.cu", "int8_gemm.cu", "int8_pair.cu"}
+                   "delta_scan.cu", "delta_chunk.cu", "seq_token.cu", "logit_rules.cu", "int8_rows.cu", "int8_gemm.cu", "int8_pair.cu", "int8_gemv.cu"}
 
 # Named subsets of the library: a model family that needs only some kernels gets a small library of its own at the
 # first use in a fresh tree (seconds instead of the minutes of the whole-step decode kernels).  The full library

@@ -16,7 +16,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .kernels import PLAIN, RESIDUAL, SWIGLU, _here, _p, _stream, num_sms
+from .kernels import PLAIN, RESIDUAL, SWIGLU, _here, _stream, num_sms
 
 TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 MAX_K = 131072                 # inputs of a layer: 127 * 127 * K stays below 2^31
@@ -41,21 +41,24 @@ def _norm_ref(x: torch.Tensor, norm_w: Optional[torch.Tensor], eps: float) -> to
     return xf / (xf.pow(2).mean(-1, keepdim=True) + eps).sqrt() * norm_w.float()
 
 
-def _dense_rows(who: str, x: torch.Tensor, K: int) -> torch.Tensor:
-    """x as [rows, K] with dense rows (any row pitch), or a refusal."""
-    if x.dtype not in TYPES or x.dim() < 1 or x.shape[-1] != K or K < 1:
-        raise ValueError(f"{who}: rows of {K} numbers in bf16, fp16 or fp32 (got {x.dtype}, {tuple(x.shape)})")
-    if x.dim() != 2:
-        if not x.is_contiguous():
-            raise ValueError(f"{who}: x is [rows, {K}], or contiguous (got {tuple(x.shape)}, strides {x.stride()})")
-        return x.view(-1, K)
-    if (K > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < K):
-        raise ValueError(f"{who}: x has dense rows that do not overlap (got {tuple(x.shape)}, strides {x.stride()})")
-    return x
+def _take(who: str, x: torch.Tensor, K: int) -> Tuple[torch.Tensor, int, int]:
+    """x as rows [M, K] with dense rows, M and the row pitch, or a refusal.  (On every call of a decode step: a message is put together only for what fails.)"""
+    shape = x.shape
+    if len(shape) == 2 and shape[1] == K and K > 0 and x.dtype in TYPES:
+        M = shape[0]
+        if x.is_contiguous():
+            return x, M, K
+        pitch = x.stride(0) if M > 1 else K
+        if (K == 1 or x.stride(1) == 1) and pitch >= K:
+            return x, M, pitch
+    elif len(shape) >= 1 and shape[-1] == K and K > 0 and x.dtype in TYPES and x.is_contiguous():
+        return x.view(-1, K), x.numel() // K, K
+    raise ValueError(f"{who}: x is rows of {K} numbers in bf16, fp16 or fp32: [M, {K}] with dense rows that do not overlap, or contiguous (got {x.dtype}, {tuple(shape)}, "
+                     f"strides {x.stride()})")
 
 
-def _gain(who: str, norm_w: Optional[torch.Tensor], x: torch.Tensor, K: int) -> None:
-    if norm_w is not None and (norm_w.dtype is not x.dtype or norm_w.numel() != K or not norm_w.is_contiguous() or norm_w.get_device() != x.get_device()):
+def _gain(who: str, norm_w: torch.Tensor, x: torch.Tensor, K: int) -> None:
+    if (norm_w.dtype is not x.dtype or norm_w.numel() != K or not norm_w.is_contiguous() or norm_w.get_device() != x.get_device()):
         raise ValueError(f"{who}: norm_w is {x.dtype} [{K}], contiguous, on {x.device} (got {norm_w.dtype}, {tuple(norm_w.shape)}, {norm_w.device})")
 
 
@@ -68,9 +71,10 @@ def quantize_rows(x: torch.Tensor, *, norm_w: Optional[torch.Tensor] = None, eps
     if x.dim() < 1:
         raise ValueError(f"{who}: x has no rows")
     K = x.shape[-1]
-    x2 = _dense_rows(who, x, K)
-    _gain(who, norm_w, x2, K)
-    M, shape = x2.shape[0], x.shape
+    x2, M, pitch = _take(who, x, K)
+    if norm_w is not None:
+        _gain(who, norm_w, x2, K)
+    shape = x.shape
     if out is None:
         q, s = x.new_empty(shape, dtype=_I8), x.new_empty(shape[:-1], dtype=_F32)
     else:
@@ -85,7 +89,7 @@ def quantize_rows(x: torch.Tensor, *, norm_w: Optional[torch.Tensor] = None, eps
         return q, s
     _here(x.get_device(), who)
     if M:
-        rc = _lib.lib().jl_int8_rows(x2.data_ptr(), TYPES[x.dtype], M, K, x2.stride(0) if M > 1 else K, None, M, _p(norm_w), float(eps), q.data_ptr(), K, s.data_ptr(), _stream())
+        rc = _lib.lib().jl_int8_rows(x2.data_ptr(), TYPES[x.dtype], M, K, pitch, 0, M, 0 if norm_w is None else norm_w.data_ptr(), eps, q.data_ptr(), K, s.data_ptr(), _stream())
         if rc:
             _lib.check(rc, "jl_int8_rows")
     return q, s
@@ -96,7 +100,7 @@ class Int8Weight:
     """Weights [N, K], or [E, N, K] of E experts, as int8 values and fp32 scales [N] / [E, N].  Rows lie on 16-byte boundaries (a copy is made where K is not a multiple
     of 16).  A SWIGLU layer's rows are interleaved: row 2j is the gate of result j, row 2j + 1 its up part (`models.engine.interleave_rows`)."""
 
-    __slots__ = ("values", "scales", "experts", "n", "k", "pitch", "device", "dev")
+    __slots__ = ("values", "scales", "experts", "n", "k", "pitch", "device", "dev", "_held")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         if values.dtype is not _I8 or values.dim() not in (2, 3) or scales.dtype is not _F32 or scales.shape != values.shape[:-1] or scales.get_device() != values.get_device():
@@ -114,6 +118,8 @@ class Int8Weight:
         self.experts = values.shape[0] if values.dim() == 3 else 0
         self.n, self.k, self.pitch = values.shape[-2], k, pitch
         self.device, self.dev = values.device, values.get_device()
+        # what a call hands to the library: (values, row pitch, scales, features), and the SMs there are (asked once: a layer is called for every token)
+        self._held = (values.data_ptr(), pitch, self.scales.data_ptr(), self.n), num_sms(self.device) if self.dev >= 0 else 0
 
     @classmethod
     def of(cls, w: torch.Tensor) -> "Int8Weight":
@@ -144,14 +150,15 @@ def _finish_ref(y: torch.Tensor, residual: Optional[torch.Tensor], mode: int, dt
 
 
 def _result(who: str, x: torch.Tensor, rows: int, n: int, mode: int, out_f32: bool, out: Optional[torch.Tensor]) -> torch.Tensor:
-    if mode == SWIGLU and n % 2:
-        raise ValueError(f"{who}: gate and up rows are interleaved, {n} rows are no pairs")
-    cols = n // 2 if mode == SWIGLU else n
-    dtype = _F32 if out_f32 else x.dtype
+    if mode == SWIGLU:
+        if n % 2:
+            raise ValueError(f"{who}: gate and up rows are interleaved, {n} rows are no pairs")
+        n //= 2
     if out is None:
-        return x.new_empty((rows, cols), dtype=dtype)
-    if out.dtype is not dtype or out.numel() != rows * cols or not out.is_contiguous() or out.get_device() != x.get_device():
-        raise ValueError(f"{who}: out is {dtype} with {rows} x {cols} elements, contiguous, on {x.device} (got {out.dtype}, {tuple(out.shape)}, {out.device})")
+        return x.new_empty((rows, n), dtype=_F32) if out_f32 else x.new_empty((rows, n))
+    dtype = _F32 if out_f32 else x.dtype
+    if out.dtype is not dtype or out.numel() != rows * n or not out.is_contiguous() or out.get_device() != x.get_device():
+        raise ValueError(f"{who}: out is {dtype} with {rows} x {n} elements, contiguous, on {x.device} (got {out.dtype}, {tuple(out.shape)}, {out.device})")
     if out.data_ptr() == x.data_ptr() and rows:
         raise ValueError(f"{who}: out is x, which is read while results are written")
     return out
@@ -165,30 +172,34 @@ def linear_int8(x: torch.Tensor, w: Int8Weight, *, norm_w: Optional[torch.Tensor
     `residual` (of the result's type and size; `out` may be it); SWIGLU gives silu(y[2j]) · y[2j + 1] of interleaved rows.  `resident`: w is a parameter that no kernel
     directly before the call writes; it may then be read ahead of those."""
     who = "linear_int8"
-    if not isinstance(w, Int8Weight) or w.experts:
+    if w.__class__ is not Int8Weight or w.experts:
         raise ValueError(f"{who}: w is an Int8Weight of one matrix")
-    x2 = _dense_rows(who, x, w.k)
-    M, dev = x2.shape[0], x.get_device()
+    dev, k, n = x.get_device(), w.k, w.n
+    x, M, pitch = _take(who, x, k)
     if dev != w.dev:
         raise ValueError(f"{who}: x on {x.device}, weights on {w.device}")
     if norm_w is not None:
-        _gain(who, norm_w, x2, w.k)
-    out = _result(who, x2, M, w.n, mode, out_f32, out)
-    if (mode == RESIDUAL) != (residual is not None) or mode not in (PLAIN, RESIDUAL, SWIGLU):
-        raise ValueError(f"{who}: mode {mode} with{'' if residual is not None else 'out'} a residual")
-    if residual is not None and (residual.dtype is not out.dtype or residual.numel() != M * w.n or not residual.is_contiguous() or residual.get_device() != dev):
-        raise ValueError(f"{who}: residual is {out.dtype} with {M} x {w.n} elements, contiguous, on {x.device} (got {residual.dtype}, {tuple(residual.shape)}, {residual.device})")
+        _gain(who, norm_w, x, k)
+    out = _result(who, x, M, n, mode, out_f32, out)
+    if residual is not None:
+        if mode != RESIDUAL:
+            raise ValueError(f"{who}: a residual in mode {mode}")
+        if residual.dtype is not out.dtype or residual.numel() != M * n or not residual.is_contiguous() or residual.get_device() != dev:
+            raise ValueError(f"{who}: residual is {out.dtype} with {M} x {n} elements, contiguous, on {x.device} (got {residual.dtype}, {tuple(residual.shape)}, {residual.device})")
+    elif mode != PLAIN and mode != SWIGLU:
+        raise ValueError(f"{who}: mode {mode} without a residual")
     if dev < 0:
-        q, s = _rows_ref(_norm_ref(x2, norm_w, eps))
+        q, s = _rows_ref(_norm_ref(x, norm_w, eps))
         y = (q.double() @ w.values.double().t()).float() * s[:, None] * w.scales
         return out.copy_(_finish_ref(y, residual, mode, out.dtype).view(out.shape))
     _here(dev, who)
     if M:
+        held, sms = w._held
         L = _lib.lib()
-        need = L.jl_int8_scratch_bytes(M, w.k)
-        scratch = x.new_empty(need, dtype=torch.uint8)
-        rc = L.jl_linear_int8(x2.data_ptr(), TYPES[x.dtype], M, w.k, x2.stride(0) if M > 1 else w.k, w.values.data_ptr(), w.pitch, w.scales.data_ptr(), w.n, _p(norm_w), float(eps),
-                              _p(residual), out.data_ptr(), TYPES[out.dtype], mode, scratch.data_ptr(), need, int(resident), num_sms(x.device), _stream())
+        need = L.jl_linear_int8_scratch_bytes(M, n, k)
+        scratch = x.new_empty(need, dtype=torch.uint8).data_ptr() if need else 0
+        rc = L.jl_linear_int8(x.data_ptr(), TYPES[x.dtype], M, k, pitch, *held, 0 if norm_w is None else norm_w.data_ptr(), eps, 0 if residual is None else residual.data_ptr(),
+                              out.data_ptr(), TYPES[out.dtype], mode, scratch, need, resident, sms, _stream())
         if rc:
             _lib.check(rc, "jl_linear_int8")
     return out
@@ -228,12 +239,12 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
     that x does not have is a row of zeros), without `rows` with row t (T = M): [T, N] (SWIGLU: [T, N / 2]) in x's type, or fp32.  Rows in front of offsets[0] and from
     offsets[E] on are left as they were.  `expert_order` gives rows and offsets of a router's choice.  Scales, sums and modes (PLAIN, SWIGLU) as in `linear_int8`."""
     who = "expert_linear_int8"
-    if not isinstance(w, Int8Weight) or not 1 <= w.experts <= MAX_EXPERTS:
+    if w.__class__ is not Int8Weight or not 1 <= w.experts <= MAX_EXPERTS:
         raise ValueError(f"{who}: w is an Int8Weight of 1 to {MAX_EXPERTS} experts")
     if mode not in (PLAIN, SWIGLU):
         raise ValueError(f"{who}: mode {mode}")
-    x2 = _dense_rows(who, x, w.k)
-    M, dev = x2.shape[0], x.get_device()
+    dev, k = x.get_device(), w.k
+    x, M, pitch = _take(who, x, k)
     if dev != w.dev:
         raise ValueError(f"{who}: x on {x.device}, weights on {w.device}")
     for t, name in ((offsets, "offsets"), (rows, "rows")):
@@ -242,10 +253,10 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
     if offsets.numel() != w.experts + 1:
         raise ValueError(f"{who}: {offsets.numel()} offsets for {w.experts} experts")
     T = M if rows is None else rows.numel()
-    out = _result(who, x2, T, w.n, mode, out_f32, out)
+    out = _result(who, x, T, w.n, mode, out_f32, out)
     if dev < 0:
         flat = out.view(T, -1)
-        q, s = _rows_ref(x2)
+        q, s = _rows_ref(x)
         if rows is not None:
             there = ((rows >= 0) & (rows < M))
             at = rows.long().clamp(0, max(M - 1, 0))
@@ -260,11 +271,11 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
         return out
     _here(dev, who)
     if T:
+        held, sms = w._held
         L = _lib.lib()
-        need = L.jl_int8_scratch_bytes(T, w.k)
-        scratch = x.new_empty(need, dtype=torch.uint8)
-        rc = L.jl_experts_int8(x2.data_ptr(), TYPES[x.dtype], M, w.k, x2.stride(0) if M > 1 else w.k, _p(rows), T, offsets.data_ptr(), w.experts, w.values.data_ptr(), w.pitch,
-                               w.scales.data_ptr(), w.n, out.data_ptr(), TYPES[out.dtype], mode, scratch.data_ptr(), need, num_sms(x.device), _stream())
+        need = L.jl_int8_scratch_bytes(T, k)
+        rc = L.jl_experts_int8(x.data_ptr(), TYPES[x.dtype], M, k, pitch, 0 if rows is None else rows.data_ptr(), T, offsets.data_ptr(), w.experts, *held, out.data_ptr(),
+                               TYPES[out.dtype], mode, x.new_empty(need, dtype=torch.uint8).data_ptr(), need, sms, _stream())
         if rc:
             _lib.check(rc, "jl_experts_int8")
     return out

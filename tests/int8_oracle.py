@@ -45,8 +45,8 @@ def bound(y, dtype, residual=None, extra=None):
 
 
 def bound_gated(y, dtype, extra=None):
-    """silu(g) u: g and u are off by 3 roundings (and `extra`); the exponential by two steps of its own and |g| times what g is off; a sum, a quotient and two products
-    add a rounding each.  |d silu / dg| <= 1.1."""
+    """silu(g) u: g and u are off by 3 roundings (and `extra`); the exponential by two steps (four roundings) of its own and |g| times what g is off; the
+    sum adds a rounding, the quotient at most two steps (four).  |d silu / dg| <= 1.1."""
     g, u = y[:, 0::2], y[:, 1::2]
     r = gated(y)
     eg = 3.1 * U * g.abs() + (extra[:, 0::2] if extra is not None else 0.0)
@@ -54,6 +54,7 @@ def bound_gated(y, dtype, extra=None):
     silu = g * torch.sigmoid(g)
     # d silu / silu = dg / g + (1 - sigmoid) dg, and 9 roundings of the chain
     es = 9.0 * U * silu.abs() + eg * (torch.sigmoid(g) + silu.abs() * (1 - torch.sigmoid(g))) * 1.01
-    # below g = -88.72 the exponential of -g passes fp32's largest number, 2^128, and the sigmoid becomes 0 where it is less than 2^-128: g u times that is lost
-    off = es * u.abs() + silu.abs() * eu + es * eu + 1.1 * U * r.abs() + 2.0 ** -128 * (g * u).abs()
+    # a reciprocal of 2^126 and more may be taken as 0 (fp32's smallest normal number is 2^-126): from 1 + exp(-g) = 2^126 on, the sigmoid is less than 2^-126, and g u times
+    # that is lost
+    off = es * u.abs() + silu.abs() * eu + es * eu + 1.1 * U * r.abs() + 2.0 ** -126 * (g * u).abs()
     return off + half_step(dtype) * (r.abs() + off) + smallest(dtype), r
