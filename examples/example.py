@@ -71,6 +71,7 @@ def main() -> None:
     ap.add_argument("--ckpt_dir", help="Meta-format LLaMA checkpoint directory")
     ap.add_argument("--model_dir", help="config.json + model.safetensors of any registered design (LLaMA, Folirax, Nikonex)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"], help="compute type with --model_dir")
+    ap.add_argument("--weights", default="bf16", choices=["bf16", "int8"], help="how layers are held on the GPU with --ckpt_dir (int8: one GPU)")
     ap.add_argument("--tokenizer_path", default="")
     ap.add_argument("--is_llama3", type=lambda s: str(s).lower() in ("1", "true", "yes"), default=False)
     ap.add_argument("--max_gen_len", type=int, default=256)
@@ -87,8 +88,10 @@ def main() -> None:
         ap.error("give exactly one of --ckpt_dir and --model_dir")
     if a.ckpt_dir and not a.tokenizer_path:
         ap.error("--ckpt_dir needs --tokenizer_path")
+    if a.model_dir and a.weights != "bf16":
+        ap.error("--weights goes with --ckpt_dir")
     generator = load_model_dir(a.model_dir, a.tokenizer_path, a.is_llama3, a.dtype) if a.model_dir else \
-        load(a.ckpt_dir, a.tokenizer_path, a.is_llama3, device=a.device)
+        load(a.ckpt_dir, a.tokenizer_path, a.is_llama3, device=a.device, weights=a.weights)
     if a.model_dir and not a.tokenizer_path and not a.prompt:
         a.prompt = ["7 8 9 10", "40 41"]
     prompts = a.prompt or ["The capital of Germany is the city of",

@@ -28,6 +28,7 @@ import torch
 from ..config import LLaMAConfig
 from ..ops import _lib
 from ..ops import kernels as K
+from ..ops.int8 import Int8Weight
 from ..ops.rules import BoundRules, LogitRules
 from .reference import KVCache, ModelOutput, join_prefix, rope_cos_sin
 
@@ -70,6 +71,8 @@ class DeviceKVCache(KVCache):
 
 @dataclass
 class LayerWeights:
+    """The matrices are bf16 [N, K]; an engine with weights="int8" holds `Int8Weight`s in their places."""
+
     attn_norm: torch.Tensor
     wqkv: torch.Tensor
     wo: torch.Tensor
@@ -120,11 +123,20 @@ class B200Engine:
     def __init__(self, config: LLaMAConfig, embedding: torch.Tensor, layers: List[LayerWeights],
                  final_norm: torch.Tensor, lm_head: torch.Tensor, *, use_cuda_graph: bool = True,
                  use_megakernel: bool = True,
-                 tp: int = 1, rank: int = 0, comm: Any = None):
+                 tp: int = 1, rank: int = 0, comm: Any = None, weights: str = "bf16"):
         """`layers` / `lm_head` hold this rank's tensor-parallel slice (Megatron layout of
         parallel/layout.py: wqkv/w13 cut on output rows, wo/w2 on the reduction dim, lm_head on vocab);
-        the embedding table and the norm scales are replicated."""
+        the embedding table and the norm scales are replicated.
+
+        weights="int8": the layers and the head are held in 8 bits with a scale per output feature, and every token's activations are brought to 8 bits in front
+        of each product (ops/int8.py): half the bytes in memory and per decoded token, twice the tensor-core rate for prompts.  One GPU (tp = 1); decoding runs the
+        per-op step (the whole-step kernel streams bf16)."""
+        if weights not in ("bf16", "int8"):
+            raise ValueError(f"weights are 'bf16' or 'int8', not {weights!r}")
+        if weights == "int8" and int(tp) > 1:
+            raise NotImplementedError("weights='int8' runs on one GPU (tp = 1)")
         self.config = config
+        self.weights = weights
         self.tp, self.rank = int(tp), int(rank)
         if self.tp > 1:
             from ..parallel.layout import check_tp_divisibility
@@ -140,6 +152,11 @@ class B200Engine:
         self.embedding = embedding
         self.layers = layers
         self.final_norm = final_norm
+        if weights == "int8":
+            lm_head = Int8Weight.of(lm_head)
+            for l in layers:
+                for name in ("wqkv", "wo", "w13", "w2"):
+                    setattr(l, name, Int8Weight.of(getattr(l, name)))          # (one matrix at a time: its bf16 form is dropped)
         self.lm_head = lm_head
         self.use_cuda_graph = use_cuda_graph
         self.nh = config.num_attention_heads // self.tp          # local (per-rank) head counts
@@ -160,10 +177,11 @@ class B200Engine:
         # Prefill at tp > 1 runs over NVLS (parallel/comm.py `NvlsPrefill`): sequence-parallel when the token count is a
         # multiple of 128·tp, otherwise tcgen05 GEMM + in-switch all-reduce kernel.  JLLAMA_SP=0 forces the latter.
         self.sequence_parallel_prefill = os.environ.get("JLLAMA_SP", "1") != "0"
-        self.use_megakernel = use_megakernel and self.hd == 128 \
+        self.use_megakernel = use_megakernel and weights == "bf16" and self.hd == 128 \
             and config.hidden_size % 256 == 0 and (config.intermediate_size // self.tp) % 256 == 0 \
             and (self.nh * self.hd) % 256 == 0 and (self.nh // self.nkv) in (1, 2, 4, 8)
-        self._stack_weights()
+        if weights == "bf16":
+            self._stack_weights()
         # Largest batch the whole-step kernel takes (it can hold 8 rows).  From batch 5 up the per-op path (tcgen05
         # swap-AB GEMMs + tensor-core decode attention, under TP with the fused exchange / all-reduce / norm kernel) is
         # faster whenever a rank streams a lot of weights per step; the whole-step kernel keeps all 8 rows only where
@@ -296,24 +314,29 @@ class B200Engine:
         return cls(config, emb, layers, ones(), head, **kw)
 
     def to_tree(self) -> Tree:
-        """Inverse of `from_tree` (canonical names / ``[in, out]`` layout) for export and tests."""
+        """Inverse of `from_tree` (canonical names / ``[in, out]`` layout) for export and tests.  8-bit weights come back as the numbers they stand for."""
         c = self.config
+
+        def numbers(w: Any) -> torch.Tensor:
+            return w.float().to(torch.bfloat16) if isinstance(w, Int8Weight) else w
+
         q, kv = self.nh * self.hd, self.nkv * self.hd
         layers = {}
         for i, l in enumerate(self.layers):
+            wqkv, wo, w13, w2 = (numbers(w) for w in (l.wqkv, l.wo, l.w13, l.w2))
             layers[str(i)] = {
-                "attention": {"wq": {"kernel": l.wqkv[:q].t().contiguous()},
-                              "wk": {"kernel": l.wqkv[q:q + kv].t().contiguous()},
-                              "wv": {"kernel": l.wqkv[q + kv:].t().contiguous()},
-                              "wo": {"kernel": l.wo.t().contiguous()}},
-                "feed_forward": {"w1": {"kernel": l.w13[0::2].t().contiguous()},
-                                 "w3": {"kernel": l.w13[1::2].t().contiguous()},
-                                 "w2": {"kernel": l.w2.t().contiguous()}},
+                "attention": {"wq": {"kernel": wqkv[:q].t().contiguous()},
+                              "wk": {"kernel": wqkv[q:q + kv].t().contiguous()},
+                              "wv": {"kernel": wqkv[q + kv:].t().contiguous()},
+                              "wo": {"kernel": wo.t().contiguous()}},
+                "feed_forward": {"w1": {"kernel": w13[0::2].t().contiguous()},
+                                 "w3": {"kernel": w13[1::2].t().contiguous()},
+                                 "w2": {"kernel": w2.t().contiguous()}},
                 "attention_norm": {"kernel": l.attn_norm}, "ffn_norm": {"kernel": l.ffn_norm}}
         tree: Tree = {"transformer": {"wte": {"embedding": self.embedding}, "ln_f": {"kernel": self.final_norm},
                                       "h": layers}}
         if not c.tie_word_embeddings:
-            tree["lm_head"] = {"kernel": self.lm_head.t().contiguous()}
+            tree["lm_head"] = {"kernel": numbers(self.lm_head).t().contiguous()}
         return tree
 
     # ------------------------------------------------------------------ cache
@@ -1034,6 +1057,8 @@ class B200Engine:
 
     def weight_bytes_per_step(self) -> int:
         """Bytes of weights one decode step streams on this rank (the HBM-roofline numerator)."""
+        if self.weights == "int8":
+            return self.lm_head.nbytes + sum(w.nbytes for l in self.layers for w in (l.wqkv, l.wo, l.w13, l.w2))
         return sum(t.numel() * 2 for t in (self.wqkv_all, self.wo_all, self.w13_all, self.w2_all, self.lm_head))
 
     def prepare(self, st: DecodeState, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor],

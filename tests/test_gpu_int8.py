@@ -459,3 +459,19 @@ def test_repeated_calls_give_the_same_bits():
         first = I.linear_int8(x, w, mode=K_.SWIGLU)
         for _ in range(3):
             assert torch.equal(I.linear_int8(x, w, mode=K_.SWIGLU), first)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N,K", [(256, 512), (1000, 2048), (130, 72)])
+def test_every_kernel_gives_a_row_the_same_bits(N, K, dtype):
+    """Sums are exact and what follows them is one chain of fp32 operations: the rows beside it, and with them the kernel, change nothing."""
+    I, K_ = _ops()
+    x, w = _randn(700, K, seed=1, dtype=dtype), _weight(N, K)
+    for mode in (K_.PLAIN, K_.SWIGLU):
+        full = I.linear_int8(x, w, mode=mode)
+        for M in (1, 2, 4, 8, 9, 16, 40, 64, 128, 130, 256, 300, 512, 600):
+            assert torch.equal(I.linear_int8(x[:M], w, mode=mode), full[:M])
+        e = I.Int8Weight(w.values[None], w.scales[None])
+        for M in (1, 30, 700):
+            off = torch.tensor([0, M], dtype=torch.int32, device=DEV)
+            assert torch.equal(I.expert_linear_int8(x[:M], e, off, mode=mode), full[:M])
