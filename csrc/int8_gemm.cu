@@ -341,9 +341,11 @@ static Int8Out out_of(void* out, const void* residual, const float* xs, const fl
 
 using namespace jl;
 
-// bytes that jl_linear_int8 and jl_experts_int8 need beside their operands: the activations' values (rows on 16 bytes) and scales
-extern "C" JL_API size_t jl_int8_scratch_bytes(int rows, int K) { return rows < 0 || K < 1 ? 0 : ((size_t)rows * up16(K) + 255) / 256 * 256 + (size_t)rows * 4; }
-extern "C" JL_API size_t jl_linear_int8_scratch_bytes(int M, int N, int K) { return int8_vec_takes(M, N, K) ? 0 : jl_int8_scratch_bytes(M, K); }
+// the activations' values (rows on 16 bytes) and scales
+static size_t values_bytes(int rows, int K) { return rows < 0 || K < 1 ? 0 : ((size_t)rows * up16(K) + 255) / 256 * 256 + (size_t)rows * 4; }
+extern "C" JL_API size_t jl_linear_int8_scratch_bytes(int M, int N, int K) { return int8_vec_takes(M, N, K) ? 0 : values_bytes(M, K); }
+
+extern "C" JL_API size_t jl_experts_int8_scratch_bytes(int T, int K) { return values_bytes(T, K); }
 
 extern "C" JL_API int jl_linear_int8(const void* x, int dtype, int M, int K, long long ldx, const void* wq, int ldw, const float* ws, int N, const void* gain, float eps,
                                      const void* residual, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int resident, int num_sms, void* stream) {
@@ -385,8 +387,9 @@ extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, lo
   JL_CHECK_ARG(ldw >= K && ldw % 16 == 0 && ((uintptr_t)wq & 15) == 0, "jl_experts_int8: weights on 16-byte rows (pitch %d)", ldw);
   JL_CHECK_ARG(mode == I8_PLAIN || (mode == I8_GATED && N % 2 == 0), "jl_experts_int8: mode %d, N=%d", mode, N);
   if (T == 0) return JL_OK;
-  JL_CHECK_ARG(scratch != nullptr && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= jl_int8_scratch_bytes(T, K), "jl_experts_int8: scratch of %zu bytes", scratch_bytes);
   if (num_sms <= 0) num_sms = SMS;
+  JL_CHECK_ARG(scratch != nullptr && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= values_bytes(T, K),
+               "jl_experts_int8: scratch of %zu bytes", scratch_bytes);
   const int ldq = up16(K);
   float* xs = reinterpret_cast<float*>((uint8_t*)scratch + ((size_t)T * ldq + 255) / 256 * 256);
   int rc;

@@ -2,8 +2,11 @@
 //
 // Two CTAs of a cluster are one MMA engine: each stages its 128 rows of activations and its 128 rows of weights (32 KB a k-block of 128 bytes), the leader's one thread
 // issues for both, each keeps the int32 sums of its own 128 rows in its own TMEM, two accumulators of 256 columns.  A lane of the epilogue holds a row, a column a feature:
-// the row's scale is a register, the features' scales come from shared memory; finished rows of 128 bytes go through shared memory, so that a warp's stores are whole lines.
-// One matrix, or one per expert (rows ordered by expert, at any row): what a tile holds of the next expert's rows is computed and not stored.
+// the row's scale is a register, the features' scales come from shared memory (a warp of its own brings both ahead of the tile); finished rows of 128 bytes go through shared
+// memory, so that a warp's stores are whole lines.
+// One matrix, or one per expert (rows ordered by expert, at any row): what a tile holds of the next expert's rows is computed and not stored.  (Rows of
+// several experts held once and gathered by the loads, `tile::gather4`: 8192 tokens x 4 of 32 experts of 2048 x 2048 410 us, with the rows written out by the kernel that
+// brings them to 8 bits 145.)
 #include <atomic>
 
 #include "int8.cuh"
@@ -12,9 +15,10 @@
 
 namespace jl {
 
-constexpr int I8P_BM = 128, I8P_BN = 256, I8P_BK = 128, I8P_THREADS = 384;      // rows per CTA; features per pair; warps: 0 TMA, 1 MMA (leader), 2 TMEM, 3 the list, 4-11 results
+constexpr int I8P_BM = 128, I8P_BN = 256, I8P_BK = 128, I8P_THREADS = 384;      // rows per CTA; features per pair; warps: 0 TMA, 1 MMA (leader), 2 TMEM, 3 list and scales, 4-11 results
 constexpr uint32_t I8P_A_BYTES = I8P_BM * I8P_BK;
-constexpr uint32_t I8P_EPI = 8 * 4096;                     // of each warp: 32 rows of 128 bytes
+constexpr uint32_t I8P_EPI = 8 * 4096;                     // of each epilogue warp: 32 rows of 128 bytes
+constexpr uint32_t I8P_SCALES = (I8P_BN + I8P_BM) * 4;     // of a tile: its features', its rows'
 constexpr int I8P_STAGES = 8;                              // at most
 constexpr size_t I8P_SMEM = 227 * 1024;
 constexpr uint32_t I8P_LEADER = 0xFEFFFFFFu;               // shared::cluster address of the same offset in CTA 0
@@ -73,15 +77,19 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
   const int stages = p.stages;
-  const uint32_t stage_bytes = I8P_A_BYTES + (uint32_t)p.bn / 2 * I8P_BK, epi_smem = smem_base + stages * stage_bytes, bars = epi_smem + I8P_EPI;       // full[stages] | empty[stages] | tfull[2] | tempty[2]
+  const uint32_t stage_bytes = I8P_A_BYTES + (uint32_t)p.bn / 2 * I8P_BK, epi_smem = smem_base + stages * stage_bytes;
+  const uint32_t scale_smem = epi_smem + I8P_EPI, bars = scale_smem + 2 * I8P_SCALES;        // full[stages] | empty[stages] | tfull[2] | tempty[2] | sfull[2] | sempty[2]
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (stages + s); };
   auto tfull_bar = [&](int s) { return bars + 8u * (2 * stages + s); };
   auto tempty_bar = [&](int s) { return bars + 8u * (2 * stages + 2 + s); };
-  const uint32_t tmem_slot = bars + 8u * (2 * stages + 4);
+  auto sfull_bar = [&](int s) { return bars + 8u * (2 * stages + 4 + s); };
+  auto sempty_bar = [&](int s) { return bars + 8u * (2 * stages + 6 + s); };
+  const uint32_t tmem_slot = bars + 8u * (2 * stages + 8);
   uint8_t* const smem = smem_raw + (smem_base - tc::smem_u32(smem_raw));
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - smem_base));
   int* table = reinterpret_cast<int*>(smem + (tmem_slot + 16 - smem_base));
+  float* const scales = reinterpret_cast<float*>(smem + (scale_smem - smem_base));      // [2][features' | rows']
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank;
@@ -101,6 +109,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(tfull_bar(s), 1);
       tc::mbar_init(tempty_bar(s), 16);                     // leader's: the eight epilogue warps of both CTAs
+      tc::mbar_init(sfull_bar(s), 1);
+      tc::mbar_init(sempty_bar(s), 8);
     }
     tc::fence_barrier_init();
   }
@@ -108,9 +118,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
-  if (warp == 3) {
-    i8_list(p.work, table);
-  }
+  if (warp == 3) i8_list(p.work, table);
   tc::fence_before_sync();
   i8p_cluster_sync();                                       // barriers of both CTAs are there before the other one uses them
   tc::fence_after_sync();
@@ -160,6 +168,31 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
         i8p_commit_both(tfull_bar(as));
       }
     }
+  } else if (warp == 3) {
+    // ===================================================== scales of a tile, ahead of its epilogue
+    Int8Walk walk;
+    int it = 0;
+    for (int t = pair; t < tiles; t += n_pairs, ++it) {
+      const Int8Tile tile = walk.at(p.work, table, t);
+      const int as = it & 1, n0 = tile.col * p.bn, first = (int)rank * I8P_BM;
+      const float* const ws = p.o.ws + (size_t)tile.expert * p.o.N;
+      float fs[I8P_BN / 32], rs[I8P_BM / 32];
+#pragma unroll
+      for (int i = 0; i < I8P_BN / 32; ++i) fs[i] = n0 + lane + 32 * i < p.o.N ? ws[n0 + lane + 32 * i] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < I8P_BM / 32; ++i) {
+        const int r = first + lane + 32 * i;
+        rs[i] = r < tile.rows ? p.o.xs[tile.row0 + r] : 0.0f;
+      }
+      tc::mbar_wait(sempty_bar(as), ((it >> 1) & 1) ^ 1);
+      float* const to = scales + as * (I8P_BN + I8P_BM);
+#pragma unroll
+      for (int i = 0; i < I8P_BN / 32; ++i) to[lane + 32 * i] = fs[i];
+#pragma unroll
+      for (int i = 0; i < I8P_BM / 32; ++i) to[I8P_BN + lane + 32 * i] = rs[i];
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(sfull_bar(as));
+    }
   } else if (warp >= 4) {
     // ===================================================== results: TMEM -> registers -> shared memory -> whole lines; four warps a half of the features
     const int quarter = warp & 3, part = (warp >> 2) - 1;   // TMEM lanes [32 quarter, 32 quarter + 32)
@@ -179,9 +212,9 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
       const int n0 = tile.col * p.bn, n_end = min(n0 + p.bn, p.o.N);      // the tile's features
       const int rows = tile.rows - first;                                // how many of its 32 there are
       const size_t row0 = (size_t)tile.row0 + first;
-      const float* const ws = p.o.ws + (size_t)tile.expert * p.o.N;
-      const bool four = (((uintptr_t)(ws + n0)) & 15) == 0;              // scales of four features in one access
-      const float sx = lane < rows ? p.o.xs[row0 + lane] : 0.0f;
+      tc::mbar_wait(sfull_bar(as), (it >> 1) & 1);
+      const float* const ws = scales + as * (I8P_BN + I8P_BM);
+      const float sx = ws[I8P_BN + quarter * 32 + lane];
       tc::mbar_wait(tfull_bar(as), (it >> 1) & 1);
       tc::fence_after_sync();
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + as * I8P_BN;
@@ -204,23 +237,6 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
             uint32_t v[AT][32];
 #pragma unroll
             for (int a = 0; a < AT; ++a) tc::tmem_ld32(t_row + c0 + (h0 + a) * 32, v[a]);
-            float4 sw[AT][8];
-#pragma unroll
-            for (int a = 0; a < AT; ++a) {
-              const int col = n0 + c0 + (h0 + a) * 32;
-              if (four && col + 31 < n_end) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sw[a][j] = *reinterpret_cast<const float4*>(ws + col + 4 * j);
-              } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  sw[a][j].x = col + 4 * j < n_end ? ws[col + 4 * j] : 0.0f;
-                  sw[a][j].y = col + 4 * j + 1 < n_end ? ws[col + 4 * j + 1] : 0.0f;
-                  sw[a][j].z = col + 4 * j + 2 < n_end ? ws[col + 4 * j + 2] : 0.0f;
-                  sw[a][j].w = col + 4 * j + 3 < n_end ? ws[col + 4 * j + 3] : 0.0f;
-                }
-              }
-            }
             tc::tmem_ld_wait();
 #pragma unroll
             for (int a = 0; a < AT; ++a) {
@@ -228,10 +244,11 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
               float y[32];
 #pragma unroll
               for (int j = 0; j < 32; j += 4) {
-                y[j] = __int2float_rn((int)v[a][j]) * sx * sw[a][j / 4].x;
-                y[j + 1] = __int2float_rn((int)v[a][j + 1]) * sx * sw[a][j / 4].y;
-                y[j + 2] = __int2float_rn((int)v[a][j + 2]) * sx * sw[a][j / 4].z;
-                y[j + 3] = __int2float_rn((int)v[a][j + 3]) * sx * sw[a][j / 4].w;
+                const float4 sw = *reinterpret_cast<const float4*>(ws + c0 + h * 32 + j);
+                y[j] = __int2float_rn((int)v[a][j]) * sx * sw.x;
+                y[j + 1] = __int2float_rn((int)v[a][j + 1]) * sx * sw.y;
+                y[j + 2] = __int2float_rn((int)v[a][j + 2]) * sx * sw.z;
+                y[j + 3] = __int2float_rn((int)v[a][j + 3]) * sx * sw.w;
               }
               if constexpr (MODE == I8_RESIDUAL) {
                 if (p.o.wide) {
@@ -293,7 +310,10 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
       }
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) i8p_remote_arrive(tempty_leader + 8u * as);          // the leader's
+      if (lane == 0) {
+        i8p_remote_arrive(tempty_leader + 8u * as);         // the leader's
+        tc::mbar_arrive(sempty_bar(as));
+      }
     }
   }
 
@@ -303,7 +323,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
 }
 
-static size_t i8p_smem(int stages, int bn, int experts) { return (size_t)stages * (I8P_A_BYTES + bn / 2 * I8P_BK) + I8P_EPI + 8 * (2 * stages + 4) + 16 + 4 * i8_table_ints(experts) + 1024; }
+static size_t i8p_smem(int stages, int bn, int experts) { return (size_t)stages * (I8P_A_BYTES + bn / 2 * I8P_BK) + I8P_EPI + 2 * I8P_SCALES + 8 * (2 * stages + 8) + 16 + 4 * i8_table_ints(experts) + 1024; }
 
 using Int8PairKernel = void (*)(const CUtensorMap, const CUtensorMap, const Int8Pair);
 template <typename T>

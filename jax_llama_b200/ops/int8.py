@@ -273,7 +273,7 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
     if T:
         held, sms = w._held
         L = _lib.lib()
-        need = L.jl_int8_scratch_bytes(T, k)
+        need = L.jl_experts_int8_scratch_bytes(T, k)
         rc = L.jl_experts_int8(x.data_ptr(), TYPES[x.dtype], M, k, pitch, 0 if rows is None else rows.data_ptr(), T, offsets.data_ptr(), w.experts, *held, out.data_ptr(),
                                TYPES[out.dtype], mode, x.new_empty(need, dtype=torch.uint8).data_ptr(), need, sms, _stream())
         if rc:

@@ -475,3 +475,24 @@ def test_every_kernel_gives_a_row_the_same_bits(N, K, dtype):
         for M in (1, 30, 700):
             off = torch.tensor([0, M], dtype=torch.int32, device=DEV)
             assert torch.equal(I.expert_linear_int8(x[:M], e, off, mode=mode), full[:M])
+
+
+@pytest.mark.parametrize("counts,N", [([600, 700, 500], 1024), ([900, 0, 1100], 2050)])
+def test_gathered_rows_of_pairs(counts, N):
+    """Many rows of few tokens: every token is brought to 8 bits once and gathered; indices that are not there give zeros, rows of no expert stay."""
+    I, K_ = _ops()
+    M, K, T = 70, 520, sum(counts) + 9
+    x, w = _randn(M, K, seed=1, dtype=BF), _weight(len(counts), N, K, seed=2)
+    rows = torch.randint(0, M, (T,), device=DEV, dtype=torch.int32, generator=torch.Generator(device=DEV).manual_seed(3))
+    offsets = torch.tensor([4] + counts).cumsum(0).to(torch.int32).to(DEV)
+    bad = torch.tensor([5, 300, 617, 1500], device=DEV)
+    for mode in (K_.PLAIN, K_.SWIGLU):
+        out = torch.full((T, N // 2 if mode == K_.SWIGLU else N), 3.0, dtype=BF, device=DEV)
+        I.expert_linear_int8(x, w, offsets, rows=rows, mode=mode, out=out)
+        _expert_check(x, w, rows, offsets, T, mode, BF, out)
+        gone = rows.clone()
+        gone[bad] = torch.tensor([-1, M, -(1 << 31), (1 << 31) - 1], dtype=torch.int32, device=DEV)
+        got = I.expert_linear_int8(x, w, offsets, rows=gone, mode=mode)
+        keep = torch.ones(T, dtype=torch.bool, device=DEV)
+        keep[bad], keep[:4], keep[-5:] = False, False, False
+        assert not got[bad].any() and torch.equal(got[keep], out[keep])
