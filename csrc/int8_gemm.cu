@@ -167,25 +167,36 @@ int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       for (int tile = tile0; tile < tiles; tile += tstep, ++it) {
         const Int8Tile t = walk.at(p.work, table, tile);
         const int as = it & 1, f0 = t.col * I8S_BM + (warp & 3) * 32 + 4 * (lane & 7);
-        float sw[4];
+        float sw[4], sx[2];                                 // features'; rows' of two times 32, a lane each
         feature_scales(t.expert, f0, sw);
+        auto row_scales = [&](int c) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) sx[i] = c + 32 * i + lane < t.rows ? p.o.xs[t.row0 + c + 32 * i + lane] : 0.0f;
+        };
+        row_scales(0);
         tc::mbar_wait(tfull_bar(as), (it >> 1) & 1);
         tc::fence_after_sync();
-        const int used = (t.rows + 15) / 16 * 16;
-        for (int c0 = 0; c0 < used; c0 += 16) {
-          to_shared(t_lane + as * p.cols + c0, st + lane * 4, 128);
-          tc::fence_before_sync();
-          __syncwarp();
-          if (c0 + 16 >= used && lane == 0) tc::mbar_arrive(tempty_bar(as));      // read: the sums of the tile after next may begin
+        for (int c64 = 0; c64 < t.rows; c64 += 64) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int r = (lane >> 3) + 4 * u, row = c0 + r;
-            if (f0 >= p.o.N || row >= t.rows) continue;
-            int x[4];
-            asm volatile("ld.shared.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(st + r * 128 + (lane & 7) * 16) : "memory");
-            i8_finish4<MODE>(p.o, t.row0 + row, f0, x, p.o.xs[t.row0 + row], sw);
+          for (int q = 0; q < 4; ++q) {
+            const int c0 = c64 + 16 * q;
+            if (c0 >= t.rows) break;
+            to_shared(t_lane + as * p.cols + c0, st + lane * 4, 128);
+            tc::fence_before_sync();
+            __syncwarp();
+            if (c0 + 16 >= t.rows && lane == 0) tc::mbar_arrive(tempty_bar(as));      // read: the sums of the tile after next may begin
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int r = (lane >> 3) + 4 * u, row = c0 + r;
+              const float s = __shfl_sync(0xffffffffu, sx[q / 2], 16 * (q & 1) + r);
+              if (f0 >= p.o.N || row >= t.rows) continue;
+              int x[4];
+              asm volatile("ld.shared.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(st + r * 128 + (lane & 7) * 16) : "memory");
+              i8_finish4<MODE>(p.o, t.row0 + row, f0, x, s, sw);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (c64 + 64 < t.rows) row_scales(c64 + 64);
         }
       }
     }

@@ -149,7 +149,14 @@ def _finish_ref(y: torch.Tensor, residual: Optional[torch.Tensor], mode: int, dt
     return y.to(dtype)
 
 
-def _result(who: str, x: torch.Tensor, rows: int, n: int, mode: int, out_f32: bool, out: Optional[torch.Tensor]) -> torch.Tensor:
+def _apart(x: torch.Tensor, pitch: int, rows: int, k: int, out: torch.Tensor) -> bool:
+    """Whether out (contiguous) has no byte between the first and the last of x's rows."""
+    a, b = x.data_ptr(), out.data_ptr()
+    return rows == 0 or a + ((rows - 1) * pitch + k) * x.element_size() <= b or b + out.numel() * out.element_size() <= a
+
+
+def _result(who: str, x: torch.Tensor, pitch: int, rows: int, n: int, mode: int, out_f32: bool, out: Optional[torch.Tensor]) -> torch.Tensor:
+    """The result [rows, n] (SWIGLU: [rows, n / 2]): `out`, if that is one, or a new one."""
     if mode == SWIGLU:
         if n % 2:
             raise ValueError(f"{who}: gate and up rows are interleaved, {n} rows are no pairs")
@@ -159,8 +166,8 @@ def _result(who: str, x: torch.Tensor, rows: int, n: int, mode: int, out_f32: bo
     dtype = _F32 if out_f32 else x.dtype
     if out.dtype is not dtype or out.numel() != rows * n or not out.is_contiguous() or out.get_device() != x.get_device():
         raise ValueError(f"{who}: out is {dtype} with {rows} x {n} elements, contiguous, on {x.device} (got {out.dtype}, {tuple(out.shape)}, {out.device})")
-    if out.data_ptr() == x.data_ptr() and rows:
-        raise ValueError(f"{who}: out is x, which is read while results are written")
+    if not _apart(x, pitch, x.shape[0], x.shape[1], out):
+        raise ValueError(f"{who}: out overlaps x, which is read while results are written")
     return out
 
 
@@ -180,12 +187,14 @@ def linear_int8(x: torch.Tensor, w: Int8Weight, *, norm_w: Optional[torch.Tensor
         raise ValueError(f"{who}: x on {x.device}, weights on {w.device}")
     if norm_w is not None:
         _gain(who, norm_w, x, k)
-    out = _result(who, x, M, n, mode, out_f32, out)
+    out = _result(who, x, pitch, M, n, mode, out_f32, out)
     if residual is not None:
         if mode != RESIDUAL:
             raise ValueError(f"{who}: a residual in mode {mode}")
         if residual.dtype is not out.dtype or residual.numel() != M * n or not residual.is_contiguous() or residual.get_device() != dev:
             raise ValueError(f"{who}: residual is {out.dtype} with {M} x {n} elements, contiguous, on {x.device} (got {residual.dtype}, {tuple(residual.shape)}, {residual.device})")
+        if residual.data_ptr() != out.data_ptr() and not _apart(residual, n, M, n, out):
+            raise ValueError(f"{who}: out overlaps a residual that it is not")
     elif mode != PLAIN and mode != SWIGLU:
         raise ValueError(f"{who}: mode {mode} without a residual")
     if dev < 0:
@@ -253,7 +262,7 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
     if offsets.numel() != w.experts + 1:
         raise ValueError(f"{who}: {offsets.numel()} offsets for {w.experts} experts")
     T = M if rows is None else rows.numel()
-    out = _result(who, x, T, w.n, mode, out_f32, out)
+    out = _result(who, x, pitch, T, w.n, mode, out_f32, out)
     if dev < 0:
         flat = out.view(T, -1)
         q, s = _rows_ref(x)

@@ -140,7 +140,8 @@ def test_rows_behind_a_norm(dtype, M, K):
 # --------------------------------------------------------------------------- linear layers
 SIZES = [(1, 1, 1), (1, 8, 16), (2, 17, 3), (1, 4096, 4096), (3, 130, 127), (4, 1000, 128), (5, 6144, 512), (8, 64, 1001), (9, 100, 4096), (16, 2048, 2048), (17, 250, 640), (33, 4096, 1024),
          (64, 129, 2048), (100, 28672, 256), (128, 512, 4096), (129, 1000, 1000), (200, 4096, 4096), (256, 260, 14336), (257, 1024, 512), (333, 6144, 384), (600, 130, 2064), (1025, 640, 1111),
-         (2048, 2048, 2048), (7, 4096, 14336), (48, 1024, 8192)]
+         (2048, 2048, 2048), (7, 4096, 14336), (48, 1024, 8192), (600, 1, 64), (700, 7, 100), (1030, 2, 8), (513, 300, 1), (300, 512, 2048),
+         (512, 1024, 4096), (3, 8, 131072), (140, 20000, 256), (8, 2048, 2048), (2, 30000, 1000)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
@@ -496,3 +497,19 @@ def test_gathered_rows_of_pairs(counts, N):
         keep = torch.ones(T, dtype=torch.bool, device=DEV)
         keep[bad], keep[:4], keep[-5:] = False, False, False
         assert not got[bad].any() and torch.equal(got[keep], out[keep])
+
+
+def test_many_experts_of_many_rows():
+    I, K_ = _ops()
+    E = 300
+    counts = [(37 * e) % 401 for e in range(E)]
+    x, w = _randn(64, 32, seed=1, dtype=BF), _weight(E, 32, 32)
+    rows, offsets, T = _expert_case(counts, 64, lead=1, behind=2)
+    out = torch.full((T, 32), 3.0, dtype=BF, device=DEV)
+    I.expert_linear_int8(x, w, offsets, rows=rows, out=out)
+    q, s = O.rows(x)
+    ids = torch.repeat_interleave(torch.arange(E, device=DEV), torch.tensor(counts, device=DEV))
+    m = rows[1:T - 2].long()
+    y = torch.einsum("tk,tnk->tn", q[m], w.values.double()[ids]) * s.double()[m, None] * w.scales.double()[ids]
+    _check(out[1:T - 2], *O.bound(y, BF))
+    assert bool((out[0] == 3).all()) and bool((out[T - 2:] == 3).all())

@@ -150,8 +150,17 @@ def test_refusals_of_linear():
     with pytest.raises(ValueError):
         I.linear_int8(x, _weight(5, 16), mode=K.SWIGLU)
     square = _weight(16, 16)
-    with pytest.raises(ValueError):
-        I.linear_int8(x, square, out=x)
+    room = _randn(64 + 3 * 16)
+    for a, b in ((0, 0), (0, 16), (16, 0), (0, 47), (47, 0)):                  # results that share numbers with x, or with a residual that they are not
+        with pytest.raises(ValueError):
+            I.linear_int8(room[a:a + 48].view(3, 16), square, out=room[b:b + 48].view(3, 16))
+        if a != b:
+            with pytest.raises(ValueError):
+                I.linear_int8(x, square, mode=K.RESIDUAL, residual=room[a:a + 48].view(3, 16), out=room[b:b + 48].view(3, 16))
+    assert torch.equal(I.linear_int8(room[:48].view(3, 16), square, out=room[48:96].view(3, 16)), I.linear_int8(room[:48].view(3, 16), square))
+    r = _randn(3, 16, seed=4)
+    want = I.linear_int8(x, square, mode=K.RESIDUAL, residual=r)
+    assert torch.equal(I.linear_int8(x, square, mode=K.RESIDUAL, residual=r, out=r), want)
     with pytest.raises(ValueError):
         K.linear(x, w, force="gemm")
 
