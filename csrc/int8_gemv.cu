@@ -2,9 +2,11 @@
 //
 // A unit is 16 features; the eight warps of a CTA take 256-column pieces of K in turn, straight from memory into the registers of `mma.sync.m16n8k32.s8` (weights are its
 // 16 rows, activations its 8 columns).  The order of K within an instruction is free as long as both operands have the same: a thread takes 16 neighbouring bytes of a row
-// where the instruction's table names 4 + 4 + 4 + 4 apart, so all accesses are 16 bytes.  Two pieces, 16 KB a warp, are under way while one is multiplied, across
+// where the instruction's table names 4 + 4 + 4 + 4 apart, so all accesses are 16 bytes.  Two pieces, 8 KB a warp, are under way while one is multiplied, across
 // units; the warps' partial sums meet in shared memory, one barrier a unit, whole numbers, in any order the same.
 // Every CTA brings the activations to 8 bits itself while its first weights are under way, which saves a launch.
+// Bound by latency, then the weights: one B200, us in a chain of cold weights, 1 x 64 x 256 2.9, 1 x 64 x 4096 3.7, 1 x 2048 x 4096 4.8, 1 x 4096 x 4096 6.1 (2.6 at the memory's rate).
+// One CTA an SM, which would let the next launch's first weights in, streams too little: 1 x 28672 x 4096 22 -> 35.
 #include "int8.cuh"
 #include "jllama_b200.h"
 

@@ -6,6 +6,8 @@
 // One pass over memory: a row's 16-byte pieces stay in registers between its maximum and its values.  Rows of up to 8 x 32 pieces go eight to a CTA, a warp each; longer
 // ones have 256 threads; those longer than registers hold are read twice, an element a thread.  Rows off the 16-byte boundary are taken in pieces of the boundary all the same
 // (the two at the ends element by element); a warp then turns its values to the boundary of the result with its neighbours' bytes.
+// Bound by memory: one B200, us, 8192 x 14336 bf16 51.7 (6.8 TB/s), 32768 x 2048 29.0 (6.9), 65536 x 512 16.8 (6.0), 2048 x 4096 fp32 7.8 (5.4); off the boundary 4097 x 1001 bf16 5.7.
+// Few pieces a thread keep too little on its way: 8192 x 4096 with 2 of 256 threads 24.6, with 16 of 32 15.4.
 // Maxima are taken on the bits without their sign, as whole numbers: the order is that of the magnitudes, with infinities and NaN above all of them.
 #include <atomic>
 
