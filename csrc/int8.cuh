@@ -17,6 +17,7 @@ enum { DT_F16 = 2 };                                             // beside DT_BF
 enum { I8_PLAIN = 0, I8_RESIDUAL = 1, I8_GATED = 2 };            // result; result + residual; silu(y[2j]) y[2j+1]
 constexpr int I8_MAX_K = 131072;
 constexpr int I8_MAX_EXPERTS = 1024;
+constexpr int I8_MAX_ROWS = 1 << 30;
 
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
@@ -28,7 +29,7 @@ template <> __device__ __forceinline__ __half from_f<__half>(float v) { return _
     else { using T = __half; __VA_ARGS__; }                              \
   } while (0)
 
-// the magnitude's bits (for 16-bit types the larger of two, in the upper or lower half)
+// the magnitude's bits, and the magnitude that they are
 template <typename T> __device__ __forceinline__ uint32_t i8r_bits(T v);
 template <> __device__ __forceinline__ uint32_t i8r_bits<float>(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 template <> __device__ __forceinline__ uint32_t i8r_bits<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat16_as_ushort(v) & 0x7fffu; }
@@ -82,7 +83,7 @@ struct Int8Quotient {
 };
 
 // Ordinary rows, two elements at a time (packed fp32).  With X = 127 x and a = amax (both by 2^-8, which keeps X finite) the quotient is t0 = X * (1 / a), corrected once by what
-// it leaves: t = t0 + (X - t0 a) (1 / a).  t0 is off by a share d of a few 2^-24, the remainder is taken with one rounding, so t before its own rounding is off by d 2^-24 or so:
+// it leaves (Markstein, 1990): t = t0 + (X - t0 a) (1 / a).  t0 is off by a share d of a few 2^-24, the remainder is taken with one rounding, so t before its own rounding is off by d 2^-24 or so:
 //   * a quotient on the middle k + 1/2, which fp32 holds, comes out as that, and the sum with 1.5 * 2^23 rounds it to the even side;
 //   * rounding t does not carry it over a middle, and onto one only from less than 2^-24 t away.  With x and amax of p bits, exponents e apart, the nearest quotient beside a
 //     middle is 2^(e - p - 1) away, and 2^-24 t is at most 2^(e - 16): never for the 16-bit types (p = 8, 11).
@@ -90,7 +91,7 @@ struct Int8Quotient {
 // of 256 elements.  Settling those too took 313 us for 8192 x 14336, most of it for instructions that were not in the cache.)
 constexpr float I8R_NEAR = 0.49999f;      // (a step of fp32 below 128 is 7.6e-6)
 struct Int8Pairs {
-  uint64_t a, inv;
+  uint64_t a, inv;            // -a and 1 / a, twice
   __device__ __forceinline__ explicit Int8Pairs(float amax) {
     const float lo = amax * 0x1p-8f, r = __fdiv_rn(1.0f, lo);
     asm("mov.b64 %0, {%1, %1};" : "=l"(a) : "f"(-lo));
@@ -150,8 +151,8 @@ __device__ __forceinline__ uint32_t i8r_pack4(uint32_t a, uint32_t b, uint32_t c
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// All of an SM's shared memory for a kernel (asked for once per device)
-template <auto KERNEL>
+// Dynamic shared memory that a kernel may ask for (set once per device, to one value: calls at the same time do not lower it for one another)
+template <auto KERNEL, int BYTES = 227 * 1024>
 static cudaError_t i8_room() {
   static std::atomic<uint64_t> done{0};
   int dev = 0;
@@ -159,7 +160,7 @@ static cudaError_t i8_room() {
   if (e != cudaSuccess) return e;
   const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
   if (bit & done.load(std::memory_order_relaxed)) return cudaSuccess;
-  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }

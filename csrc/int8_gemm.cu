@@ -363,7 +363,8 @@ extern "C" JL_API size_t jl_experts_int8_scratch_bytes(int T, int K) { return va
 extern "C" JL_API int jl_linear_int8(const void* x, int dtype, int M, int K, long long ldx, const void* wq, int ldw, const float* ws, int N, const void* gain, float eps,
                                      const void* residual, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int resident, int num_sms, void* stream) {
   JL_CHECK_ARG(dtype >= DT_BF16 && dtype <= DT_F16 && out_dtype >= DT_BF16 && out_dtype <= DT_F16, "jl_linear_int8: element types %d, %d", dtype, out_dtype);
-  JL_CHECK_ARG(M >= 0 && N >= 1 && K >= 1 && K <= I8_MAX_K && (ldx >= K || M <= 1), "jl_linear_int8: M=%d N=%d K=%d (at most %d), pitch %lld", M, N, K, I8_MAX_K, ldx);
+  JL_CHECK_ARG(M >= 0 && M <= I8_MAX_ROWS && N >= 1 && N <= I8_MAX_ROWS && K >= 1 && K <= I8_MAX_K && (ldx >= K || M <= 1), "jl_linear_int8: M=%d N=%d K=%d (at most %d), pitch %lld",
+               M, N, K, I8_MAX_K, ldx);
   JL_CHECK_ARG(ldw >= K && ldw % 16 == 0 && ((uintptr_t)wq & 15) == 0, "jl_linear_int8: weights on 16-byte rows (pitch %d)", ldw);
   JL_CHECK_ARG(mode >= I8_PLAIN && mode <= I8_GATED && (mode == I8_RESIDUAL) == (residual != nullptr) && (mode != I8_GATED || N % 2 == 0),
                "jl_linear_int8: mode %d with%s residual, N=%d", mode, residual != nullptr ? "" : "out", N);
@@ -393,7 +394,7 @@ extern "C" JL_API int jl_linear_int8(const void* x, int dtype, int M, int K, lon
 extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int T, const int* offsets, int experts, const void* wq, int ldw,
                                       const float* ws, int N, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int num_sms, void* stream) {
   JL_CHECK_ARG(dtype >= DT_BF16 && dtype <= DT_F16 && out_dtype >= DT_BF16 && out_dtype <= DT_F16, "jl_experts_int8: element types %d, %d", dtype, out_dtype);
-  JL_CHECK_ARG(M >= 0 && T >= 0 && N >= 1 && K >= 1 && K <= I8_MAX_K && (ldx >= K || M <= 1) && (rows != nullptr || T <= M),
+  JL_CHECK_ARG(M >= 0 && T >= 0 && T <= I8_MAX_ROWS && N >= 1 && K >= 1 && K <= I8_MAX_K && (ldx >= K || M <= 1) && (rows != nullptr || T <= M),
                "jl_experts_int8: M=%d T=%d N=%d K=%d (at most %d), pitch %lld", M, T, N, K, I8_MAX_K, ldx);
   JL_CHECK_ARG(experts >= 1 && experts <= I8_MAX_EXPERTS && offsets != nullptr, "jl_experts_int8: %d experts (at most %d)", experts, I8_MAX_EXPERTS);
   JL_CHECK_ARG((long long)N * experts < (1ll << 31), "jl_experts_int8: %d x %d weight rows", experts, N);

@@ -14,6 +14,7 @@ namespace jl {
 
 constexpr int I8V_THREADS = 256, I8V_WARPS = 8, I8V_ROWS = 8, I8V_FEATURES = 16, I8V_PIECE = 256;
 constexpr int I8V_FUSED = 16384;
+constexpr int I8V_SMEM = 96 * 1024;      // (values and fp32 rows of that many elements: 84 KB)
 
 struct Int8Vec {
   Int8Out o;
@@ -232,7 +233,7 @@ static int vec_launch(const Int8Vec& p, size_t smem, int num_sms, cudaStream_t s
   auto kern = int8_vec_kernel<T, MODE>;
   // equal shares: as many CTAs as give each the same number of units, up to two an SM
   const int slots = 2 * num_sms, rounds = (p.units + slots - 1) / slots, grid = (p.units + rounds - 1) / rounds;
-  if (smem > 32 * 1024) JL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  JL_CUDA((i8_room<int8_vec_kernel<T, MODE>, I8V_SMEM>()));
   JL_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(I8V_THREADS), smem, stream, p));
   return JL_OK;
 }

@@ -3,14 +3,11 @@
 // Both are what 64 bits would give: s is one rounded quotient, and q is decided exactly (int8.cuh).  A row of zeros has s = 0, a row that holds an infinity or a NaN s = NaN, both
 // with q = 0: what such a row is multiplied with gives zeros or NaN.  With gains the row is normed first (RMS, fp32, no rounding in between).
 //
-// One pass over memory: a row's 16-byte pieces stay in registers between its maximum and its values.  Rows of up to 8 x 32 pieces go eight to a CTA, a warp each; longer
-// ones have 256 threads; those longer than registers hold are read twice, an element a thread.  Rows off the 16-byte boundary are taken in pieces of the boundary all the same
-// (the two at the ends element by element); a warp then turns its values to the boundary of the result with its neighbours' bytes.
+// One pass over memory: a row's 16-byte pieces stay in registers between its maximum and its values, 2 to 16 a thread; a row has a warp, 128 or 256 threads.  Rows longer than
+// registers hold are read twice, an element a thread.  Rows off the 16-byte boundary are taken in pieces of the boundary all the same (the two at the ends element by
+// element); a warp then turns its values to the boundary of the result with its neighbours' bytes.
 // Bound by memory: one B200, us, 8192 x 14336 bf16 51.7 (6.8 TB/s), 32768 x 2048 29.0 (6.9), 65536 x 512 16.8 (6.0), 2048 x 4096 fp32 7.8 (5.4); off the boundary 4097 x 1001 bf16 5.7.
-// Few pieces a thread keep too little on its way: 8192 x 4096 with 2 of 256 threads 24.6, with 16 of 32 15.4.
 // Maxima are taken on the bits without their sign, as whole numbers: the order is that of the magnitudes, with infinities and NaN above all of them.
-#include <atomic>
-
 #include "int8.cuh"
 #include "jllama_b200.h"
 
@@ -209,7 +206,8 @@ static int rows_launch(const Int8Rows& p, cudaStream_t stream) {
   const bool whole = p.K % VE == 0 && (p.ldx * (long long)sizeof(T)) % 16 == 0 && ((uintptr_t)p.x & 15) == 0 && p.ldq % VE == 0 && (uintptr_t)p.q % VE == 0 &&
                      ((uintptr_t)p.gain & 15) == 0;
   const int pieces = p.K / VE, spread = (p.K + 2 * VE - 2) / VE;      // pieces of a row: on the boundary; at most, off it
-  // few rows: their latency counts, many threads a row; many rows: bytes on their way count, many pieces a thread
+  // few rows: their latency counts, many threads a row; many rows: bytes on their way count, many pieces a thread (us with 256 threads | with one warp: 8192 x 4096 18.2 | 15.3,
+  // 8192 x 2048 13.6 | 7.6; 2000 x 4096 5.7 | 6.1)
   const bool few = p.n <= 4 * SMS;
   cudaError_t e;
   if (whole && pieces <= 2 * 32) e = rows_go<T, 32, 2, NORM>(p, stream);
@@ -243,7 +241,7 @@ using namespace jl;
 extern "C" JL_API int jl_int8_rows(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int n, const void* gain, float eps, void* q, int ldq,
                                    float* s, void* stream) {
   JL_CHECK_ARG(dtype >= DT_BF16 && dtype <= DT_F16, "jl_int8_rows: element type %d", dtype);
-  JL_CHECK_ARG(M >= 0 && n >= 0 && K >= 1 && ldq >= K && (ldx >= K || M <= 1) && (rows != nullptr || n <= M), "jl_int8_rows: %d x %d (pitch %lld) as %d rows of pitch %d", M, K, ldx, n, ldq);
+  JL_CHECK_ARG(M >= 0 && n >= 0 && n <= I8_MAX_ROWS && K >= 1 && ldq >= K && (ldx >= K || M <= 1) && (rows != nullptr || n <= M), "jl_int8_rows: %d x %d (pitch %lld) as %d rows of pitch %d", M, K, ldx, n, ldq);
   if (n == 0) return JL_OK;
   return int8_rows(x, dtype, M, K, ldx, rows, n, gain, eps, q, ldq, s, 0, (cudaStream_t)stream);
 }

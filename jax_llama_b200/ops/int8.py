@@ -21,6 +21,7 @@ from .kernels import PLAIN, RESIDUAL, SWIGLU, _here, _stream, num_sms
 TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 MAX_K = 131072                 # inputs of a layer: 127 * 127 * K stays below 2^31
 MAX_EXPERTS = 1024
+MAX_ROWS = 1 << 30
 _I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
 
 
@@ -57,6 +58,11 @@ def _take(who: str, x: torch.Tensor, K: int) -> Tuple[torch.Tensor, int, int]:
                      f"strides {x.stride()})")
 
 
+def _few(who: str, rows: int) -> None:
+    if rows > MAX_ROWS:
+        raise ValueError(f"{who}: {rows} rows (at most {MAX_ROWS})")
+
+
 def _gain(who: str, norm_w: torch.Tensor, x: torch.Tensor, K: int) -> None:
     if (norm_w.dtype is not x.dtype or norm_w.numel() != K or not norm_w.is_contiguous() or norm_w.get_device() != x.get_device()):
         raise ValueError(f"{who}: norm_w is {x.dtype} [{K}], contiguous, on {x.device} (got {norm_w.dtype}, {tuple(norm_w.shape)}, {norm_w.device})")
@@ -72,6 +78,7 @@ def quantize_rows(x: torch.Tensor, *, norm_w: Optional[torch.Tensor] = None, eps
         raise ValueError(f"{who}: x has no rows")
     K = x.shape[-1]
     x2, M, pitch = _take(who, x, K)
+    _few(who, M)
     if norm_w is not None:
         _gain(who, norm_w, x2, K)
     shape = x.shape
@@ -82,6 +89,8 @@ def quantize_rows(x: torch.Tensor, *, norm_w: Optional[torch.Tensor] = None, eps
         if q.dtype is not _I8 or s.dtype is not _F32 or q.shape != shape or s.shape != shape[:-1] or not (q.is_contiguous() and s.is_contiguous()) \
                 or q.get_device() != x.get_device() or s.get_device() != x.get_device():
             raise ValueError(f"{who}: out is int8 {tuple(shape)} and fp32 {tuple(shape[:-1])}, contiguous, on {x.device}")
+        if not (_apart(x2, pitch, M, K, q) and _apart(x2, pitch, M, K, s)):
+            raise ValueError(f"{who}: out overlaps x")
     if not x.is_cuda:
         v, sc = _rows_ref(_norm_ref(x2, norm_w, eps))
         q.view(-1, K).copy_(v)
@@ -107,8 +116,8 @@ class Int8Weight:
             raise ValueError(f"Int8Weight: values are int8 [N, K] or [E, N, K], scales fp32 of all but the last dimension, on one device (got {values.dtype} {tuple(values.shape)} on "
                              f"{values.device}, {scales.dtype} {tuple(scales.shape)} on {scales.device})")
         k = values.shape[-1]
-        if not 1 <= k <= MAX_K or values.numel() == 0:
-            raise ValueError(f"Int8Weight: 1 to {MAX_K} inputs and at least one feature (got {tuple(values.shape)})")
+        if not 1 <= k <= MAX_K or values.numel() == 0 or scales.numel() > MAX_ROWS:
+            raise ValueError(f"Int8Weight: 1 to {MAX_K} inputs, at least one feature and at most {MAX_ROWS} (got {tuple(values.shape)})")
         pitch = -(-k // 16) * 16
         if pitch != k or not values.is_contiguous() or values.data_ptr() % 16:
             room = values.new_zeros((*values.shape[:-1], pitch))
@@ -203,6 +212,7 @@ def linear_int8(x: torch.Tensor, w: Int8Weight, *, norm_w: Optional[torch.Tensor
         return out.copy_(_finish_ref(y, residual, mode, out.dtype).view(out.shape))
     _here(dev, who)
     if M:
+        _few(who, M)
         held, sms = w._held
         L = _lib.lib()
         need = L.jl_linear_int8_scratch_bytes(M, n, k)
@@ -280,6 +290,7 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
         return out
     _here(dev, who)
     if T:
+        _few(who, max(M, T))
         held, sms = w._held
         L = _lib.lib()
         need = L.jl_experts_int8_scratch_bytes(T, k)

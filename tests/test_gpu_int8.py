@@ -441,10 +441,11 @@ def test_two_streams_at_once():
         assert torch.equal(a, b)
 
 
-def test_weights_quantised_directly_before():
+@pytest.mark.parametrize("M", [1, 16, 200, 600])
+def test_weights_quantised_directly_before(M):
     """The library's own kernel writes the weights, the product follows at once."""
     I, _ = _ops()
-    x = _randn(1, 4096, seed=1, dtype=BF)
+    x = _randn(M, 4096, seed=1, dtype=BF)
     for seed in range(4):
         w16 = _randn(4096, 4096, seed=seed, dtype=BF)
         y = I.linear_int8(x, I.Int8Weight.of(w16))
@@ -513,3 +514,54 @@ def test_many_experts_of_many_rows():
     y = torch.einsum("tk,tnk->tn", q[m], w.values.double()[ids]) * s.double()[m, None] * w.scales.double()[ids]
     _check(out[1:T - 2], *O.bound(y, BF))
     assert bool((out[0] == 3).all()) and bool((out[T - 2:] == 3).all())
+
+
+def test_an_order_written_directly_before():
+    """Offsets and rows of a router's choice, at once used: they are read ahead of the wait for the activations."""
+    I, _ = _ops()
+    x, w = _randn(600, 256, seed=1, dtype=BF), _weight(16, 640, 256)
+    for M in (3, 40, 600):
+        for seed in range(4):
+            idx = _randn(M, 16, seed=seed).topk(4, -1).indices.to(torch.int32)
+            pos, rows, offsets = I.expert_order(idx, 16)
+            y = I.expert_linear_int8(x[:M], w, offsets, rows=rows)[pos.long()]
+            torch.cuda.synchronize()
+            for e in range(16):
+                at = (idx.reshape(-1) == e).nonzero()[:, 0]
+                if at.numel():
+                    one = I.Int8Weight(w.values[e], w.scales[e])
+                    assert torch.equal(y[at], I.linear_int8(x[at // 4].contiguous(), one))
+
+
+# --------------------------------------------------------------------------- places beyond 2^31
+def test_rows_beyond_2_31():
+    I, _ = _ops()
+    M, K = 140000, 16384
+    x = torch.empty(M, K, dtype=BF, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    q, s = I.quantize_rows(x)
+    at = torch.tensor([0, 131071, 131072, 139999], device=DEV)
+    _same_rows((q[at], s[at]), x[at])
+
+
+@pytest.mark.parametrize("M,N,K", [(70000, 32768, 64), (120, 20_000_000, 112)])
+def test_results_and_weights_beyond_2_31(M, N, K):
+    I, _ = _ops()
+    x = _randn(M, K, seed=1, dtype=BF)
+    w = I.Int8Weight(_values(N, K), torch.full((N,), 1e-3, device=DEV))
+    y = I.linear_int8(x, w)
+    rows, cols = torch.tensor([0, M // 2, M - 1], device=DEV), torch.tensor([0, 1, N // 2, N - 2, N - 1], device=DEV)
+    off, want = O.bound(O.products(*O.rows(x[rows]), w.values[cols], w.scales[cols]), BF)
+    _check(y[rows][:, cols], off, want)
+
+
+def test_experts_beyond_2_31():
+    I, K_ = _ops()
+    E, N, K = 40, 30000, 2048
+    x = _randn(64, K, seed=1, dtype=BF)
+    w = I.Int8Weight(_values(E, N, K), torch.full((E, N), 1e-3, device=DEV))
+    rows, offsets, T = _expert_case([3] * E, 64)
+    y = I.expert_linear_int8(x, w, offsets, rows=rows)
+    q, s = O.rows(x)
+    for e in (0, 35, 39):
+        m = rows[3 * e:3 * e + 3].long()
+        _check(y[3 * e:3 * e + 3], *O.bound(O.products(q[m], s[m], w.values[e], w.scales[e]), BF))

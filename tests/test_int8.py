@@ -126,9 +126,20 @@ def test_refusals_of_rows():
     for out in ((torch.zeros(3, 4), torch.zeros(3)), (torch.zeros(3, 4, dtype=torch.int8), torch.zeros(4)), (torch.zeros(4, 3, dtype=torch.int8).t(), torch.zeros(3))):
         with pytest.raises(ValueError):
             I.quantize_rows(x, out=out)
+    room = torch.zeros(64, dtype=torch.int8)
+    with pytest.raises(ValueError):
+        I.quantize_rows(room[:48].view(torch.float32).view(3, 4), out=(room[40:52].view(3, 4), torch.zeros(3)))
     for g in (torch.zeros(3), torch.zeros(4, dtype=torch.bfloat16), torch.zeros(8)[::2]):
         with pytest.raises(ValueError):
             I.quantize_rows(x, norm_w=g)
+
+
+def test_more_rows_than_there_may_be(monkeypatch):
+    monkeypatch.setattr(I, "MAX_ROWS", 2)
+    with pytest.raises(ValueError):
+        I.quantize_rows(torch.zeros(3, 4))
+    with pytest.raises(ValueError):
+        I.Int8Weight(torch.zeros(3, 16, dtype=torch.int8), torch.ones(3))
 
 
 def test_refusals_of_weights():
