@@ -83,7 +83,8 @@ def quantize_rows(x: torch.Tensor, *, norm_w: Optional[torch.Tensor] = None, eps
         _gain(who, norm_w, x2, K)
     shape = x.shape
     if out is None:
-        q, s = x.new_empty(shape, dtype=_I8), x.new_empty(shape[:-1], dtype=_F32)
+        q = torch.empty_like(x, dtype=_I8, memory_format=torch.contiguous_format)
+        s = x.new_empty(M, dtype=_F32) if len(shape) == 2 else x.new_empty(shape[:-1], dtype=_F32)
     else:
         q, s = out
         if q.dtype is not _I8 or s.dtype is not _F32 or q.shape != shape or s.shape != shape[:-1] or not (q.is_contiguous() and s.is_contiguous()) \
@@ -171,7 +172,7 @@ def _result(who: str, x: torch.Tensor, pitch: int, rows: int, n: int, mode: int,
             raise ValueError(f"{who}: gate and up rows are interleaved, {n} rows are no pairs")
         n //= 2
     if out is None:
-        return x.new_empty((rows, n), dtype=_F32) if out_f32 else x.new_empty((rows, n))
+        return x.new_empty(rows, n, dtype=_F32) if out_f32 else x.new_empty(rows, n)          # (a tuple costs the host 0.4 µs more)
     dtype = _F32 if out_f32 else x.dtype
     if out.dtype is not dtype or out.numel() != rows * n or not out.is_contiguous() or out.get_device() != x.get_device():
         raise ValueError(f"{who}: out is {dtype} with {rows} x {n} elements, contiguous, on {x.device} (got {out.dtype}, {tuple(out.shape)}, {out.device})")
