@@ -303,5 +303,10 @@ struct Int8Walk {
   }
 };
 __host__ __device__ constexpr int i8_table_ints(int experts) { return 2 * experts + 2; }
+// pieces of `chunk` rows, at most: every expert that has rows may have one that is not full
+inline long long i8_pieces(const Int8Work& w, int chunk) {
+  if (w.offsets == nullptr) return ((long long)w.rows + chunk - 1) / chunk;
+  return w.rows <= w.experts ? w.rows : w.experts + ((long long)w.rows - w.experts) / chunk;
+}
 
 }  // namespace jl

@@ -276,9 +276,8 @@ static int swap_launch(const void* xq, const void* wq, Int8Swap p, int ldx, int 
   const int E = p.work.experts;
   p.work.cols = (p.o.N + I8S_BM - 1) / I8S_BM;
   p.work.chunk = p.nb;
-  const bool grouped = p.work.offsets != nullptr;
   const int num_kb = (p.K + I8S_BK - 1) / I8S_BK;
-  const long long most = (long long)p.work.cols * ((p.work.rows + p.nb - 1) / p.nb + (grouped ? (E < p.work.rows ? E : p.work.rows) : 0));      // tiles, at most
+  const long long most = p.work.cols * i8_pieces(p.work, p.nb);      // tiles, at most
   JL_CHECK_ARG(most < (1ll << 30), "int8 product: %lld tiles", most);
   p.ksplit = i8s_parts(p.nb, most, num_kb, num_sms);
   const bool split = p.ksplit > 1;
@@ -414,7 +413,7 @@ extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, lo
   // rows 29.6, 25.9, 26.7, 28.0 | 40.6; 64 rows 43.6, 32.1, 29.1, 33.5 | 38.4; 128 rows 77.6, 48.1, 38.2, 41.8 | 42.9; 256 rows 145, 83, 60.4, 63.5 | 56.9); 16 wherever that
   // gives no more tiles than there are slots (8 experts of 1024 x 512, 50 rows: 7.2, 7.5, 9.2, 12.7 | 13.8).
   const int even = (T + experts - 1) / experts;
-  const long long tiles = (long long)((N + I8S_BM - 1) / I8S_BM) * ((T + 15) / 16 + (experts < T ? experts : T));
+  const long long tiles = (N + I8S_BM - 1) / I8S_BM * i8_pieces(work, 16);
   if (even > 160 && tiles > 2 * num_sms) return int8_pair(scratch, ldq, wq, ldw, o, work, K, mode, num_sms, (cudaStream_t)stream);
   return int8_swap(scratch, ldq, wq, ldw, o, work, K, tiles <= 2 * num_sms || even <= 1 ? 16 : even <= 24 ? 32 : 64, mode, num_sms, (cudaStream_t)stream);
 }

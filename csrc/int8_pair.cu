@@ -385,7 +385,7 @@ int int8_pair(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8W
   work.cols = (o.N + p.bn - 1) / p.bn;
   p.o = o; p.work = work; p.K = K;
   p.idesc = tc::idesc_s8_s32(2 * I8P_BM, p.bn);
-  const long long most = (long long)work.cols * ((work.rows + work.chunk - 1) / work.chunk + (work.offsets != nullptr ? (E < work.rows ? E : work.rows) : 0));
+  const long long most = work.cols * i8_pieces(work, work.chunk);
   JL_CHECK_ARG(most < (1ll << 30), "int8 product: %lld tiles", most);
   CUtensorMap tx, tw;
   int rc;
