@@ -7,6 +7,7 @@ Constants (activation, score function, group limits, weight scale, shared expert
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import Dict, List, Optional, Tuple
 
@@ -14,7 +15,10 @@ import numpy as np
 import torch
 
 from ..config import DenseMlpSpec, MoeMlpSpec
+from ..ops import _lib
+from ..ops import int8 as I8
 from ..ops import seq_kernels as SK
+from ..ops.kernels import SWIGLU
 from .mixers import _stack_rows
 
 
@@ -118,11 +122,14 @@ class MoeFeedForward:
     (true float32, sizes the tensor-core kernel does not take) on the exact tiled kernel, which gathers as it reads.
     The weighted sum, the shared expert and its gate meet in one combine pass.  Identity experts (router outputs beyond the
     experts with matrices) are chosen like the others; their pairs run no product and their share, weight · input, is added in the
-    combine pass."""
+    combine pass.
+
+    weights="int8": the experts' matrices are held in 8 bits and every row's activations are brought to 8 bits (ops/int8.py); pairs are ordered by expert with nothing
+    between experts, at any number of rows.  Router, shared expert and gate stay in the engine's type."""
 
     kind = "moe"
 
-    def __init__(self, spec: MoeMlpSpec, w: Dict[str, torch.Tensor]):
+    def __init__(self, spec: MoeMlpSpec, w: Dict[str, torch.Tensor], weights: str = "bf16"):
         if (spec.act not in SK.ACTIVATIONS and not spec.gated) or spec.score not in SK.SCORES:
             raise ValueError(f"unknown activation {spec.act!r} or score function {spec.score!r}")
         if spec.gated and spec.act != "glu_clamped" and spec.act not in SK.ACTIVATIONS:
@@ -132,12 +139,31 @@ class MoeFeedForward:
         self.n_route = E + spec.identity                   # router outputs: experts, then identity experts (no matrices)
         self.choice_bias = w["correction"].float().contiguous() if spec.choice_bias else None
         self.u_off = self.shared_u_off = 0
-        if spec.gated:                                                                  # [E, gate | up (padded to 8 rows), W]
+        self.up8 = self.down8 = None
+        # silu(gate) · up in the product: gate and up rows take turns
+        self.turns = spec.gated and spec.act == "silu"
+        if weights == "int8":
+            if E > I8.MAX_EXPERTS:
+                raise ValueError(f"{E} experts in 8 bits (at most {I8.MAX_EXPERTS})")
+            if not _lib.has("jl_experts_int8"):
+                raise _lib.NativeLibraryError("experts in 8 bits need the full library: python -m jax_llama_b200.ops.build")
+            if spec.gated:
+                pairs = [(w[f"e{e}.gate"], w[f"e{e}.up"]) for e in range(E)]
+                up = [torch.stack(p, 1).flatten(0, 1) if self.turns else torch.cat(p) for p in pairs]
+            else:
+                up = [w[f"e{e}.up"] for e in range(E)]
+            self.up8 = I8.Int8Weight.of(torch.stack(up))
+            del up
+            self.down8 = I8.Int8Weight.of(torch.stack([w[f"e{e}.down"] for e in range(E)]))
+            self.up = self.down = None
+            self.u_off = spec.ff if spec.gated else 0
+        elif spec.gated:                                                                  # [E, gate | up (padded to 8 rows), W]
             pairs = [_stack_rows([w[f"e{e}.gate"], w[f"e{e}.up"]]) for e in range(E)]
             self.up, self.u_off = torch.stack([p[0] for p in pairs]).contiguous(), pairs[0][1][1]
         else:
             self.up = torch.stack([w[f"e{e}.up"] for e in range(E)]).contiguous()      # [E, ff, W]
-        self.down = torch.stack([w[f"e{e}.down"] for e in range(E)]).contiguous()      # [E, W, ff]
+        if self.down8 is None:
+            self.down = torch.stack([w[f"e{e}.down"] for e in range(E)]).contiguous()  # [E, W, ff]
         self.router_bias = w["router.b"].float().contiguous() if spec.router_bias else None
         self.has_shared = spec.shared_ff > 0
         gated = self.has_shared and spec.shared_gate
@@ -168,20 +194,38 @@ class MoeFeedForward:
                 out["shared.sg"] = (1, W)
         return out
 
+    def _experts(self) -> List[torch.Tensor]:
+        """The experts' tensors, the expert in front."""
+        if self.up8 is not None:
+            return [self.up8.values, self.up8.scales, self.down8.values, self.down8.scales]
+        return [self.up, self.down]
+
     def weights(self) -> List[torch.Tensor]:
-        return [t for t in (self.up, self.down, self.w_route, self.shared_up, self.shared_down) if t is not None]
+        return [t for t in self._experts() + [self.w_route, self.shared_up, self.shared_down] if t is not None]
 
     def streamed_weights(self, rows: int) -> List[torch.Tensor]:
         """What a step of `rows` tokens reads at least: at most rows · top experts are touched."""
         s = self.spec
         frac = min(1.0, rows * s.top / s.experts)
         n = max(1, int(round(frac * s.experts)))
-        return [self.up[:n], self.down[:n]] + [t for t in (self.w_route, self.shared_up, self.shared_down) if t is not None]
+        return [t[:n] for t in self._experts()] + [t for t in (self.w_route, self.shared_up, self.shared_down) if t is not None]
 
     def run(self, h: torch.Tensor) -> torch.Tensor:
-        with SK.room_of(self):
+        # (8-bit layers take torch tensors, so nothing of theirs is cut from a layer's room)
+        with SK.room_of(self) if self.up8 is None else contextlib.nullcontext():
             parts = self._parts(h)
         return SK.moe_combine(*parts[0], **parts[1])
+
+    def _experts_int8(self, h: torch.Tensor, idx: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(fp32 rows of the experts' results, the row of every pair)."""
+        s = self.spec
+        pos, rows, offsets = I8.expert_order(idx, s.experts)
+        if self.turns:
+            t = I8.expert_linear_int8(h, self.up8, offsets, rows=rows, mode=SWIGLU)
+        else:
+            y = I8.expert_linear_int8(h, self.up8, offsets, rows=rows, out_f32=True)
+            t = _gated_act(y, self.u_off, s.ff, s.act, s.limit, h.dtype) if s.gated else SK.act_cast(y, h.dtype, self.act)
+        return I8.expert_linear_int8(t, self.down8, offsets, out_f32=True), pos
 
     def _parts(self, h: torch.Tensor) -> Tuple[tuple, dict]:
         """Everything ahead of the weighted sum: its arguments."""
@@ -191,8 +235,10 @@ class MoeFeedForward:
         ident_w = SK.empty(M, dtype=torch.float32, device=h.device) if s.identity else None
         idx, wt = SK.moe_route(z, self.n_route, s.top, s.groups, s.keep, s.group_top, self.score, s.normalise, s.scale,
                                bias=self.router_bias, choice_bias=self.choice_bias, n_real=s.experts, ident_w=ident_w)
-        n_up = self.up.shape[1]                                                    # ff, or gate | up rows of a gated expert
-        if M <= SK.MOE_PAIR_ROWS:
+        n_up = self.up.shape[1] if self.up8 is None else 0                         # ff, or gate | up rows of a gated expert
+        if self.up8 is not None:
+            y, pos = self._experts_int8(h, idx)
+        elif M <= SK.MOE_PAIR_ROWS:
             n = M * s.top
             flat = idx.view(-1)
             if s.gated:

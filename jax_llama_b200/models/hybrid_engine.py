@@ -182,8 +182,13 @@ class HybridEngine(B200Engine):
     shares_prefixes = False                      # per-layer caches of unequal shapes and recurrent states: rows are written out
 
     def __init__(self, config: Any, tensors: Dict[str, torch.Tensor], *, dtype: torch.dtype = torch.bfloat16,
-                 device: Any = "cuda", use_cuda_graph: bool = True):
-        """`tensors`: checkpoint names → tensors (any float dtype, any device); they are cast to `dtype` and moved."""
+                 device: Any = "cuda", use_cuda_graph: bool = True, expert_weights: str = "bf16"):
+        """`tensors`: checkpoint names → tensors (any float dtype, any device); they are cast to `dtype` and moved.  expert_weights="int8": the experts of the
+        mixtures are held in 8 bits with a scale per output feature (ops/int8.py): half of bfloat16's bytes, twice its rate for prompts."""
+        if expert_weights not in ("bf16", "int8"):
+            raise ValueError(f"expert_weights are 'bf16' (the engine's type) or 'int8', not {expert_weights!r}")
+        if expert_weights == "int8" and not any(l.mlp is not None and l.mlp.kind == "moe" for l in config.layers):
+            raise ValueError("expert_weights='int8': the model has no mixture of experts")
         self.config = config
         self.dtype = dtype
         SK.dtype_code(dtype)
@@ -255,7 +260,8 @@ class HybridEngine(B200Engine):
                     layer.norm2b = get(p + "norm2b")
                 fw = {k[len(p) + 4:]: get(k) for k in want if k.startswith(p + "mlp.")}
                 try:
-                    layer.ff = FEED_FORWARDS[l.mlp.kind](l.mlp, fw)
+                    more = {"weights": expert_weights} if l.mlp.kind == "moe" and expert_weights != "bf16" else {}
+                    layer.ff = FEED_FORWARDS[l.mlp.kind](l.mlp, fw, **more)
                 except ValueError as e:
                     raise ValueError(f"layer {i}: {e}") from None
             if self.side_table is not None:
