@@ -235,7 +235,7 @@ __device__ __forceinline__ void i8_finish4(const Int8Out& o, int row, int f0, co
     float r[4];
     i8_residual4(o, at, f0, r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] += r[i];
+    for (int i = 0; i < 4; ++i) y[i] = __fadd_rn(y[i], r[i]);       // never fused with the scale's product: a row's bits do not depend on the kernel
   }
   if (o.wide) {
     if (o.kind == DT_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(o.out) + at) = make_float4(y[0], y[1], y[2], y[3]);

@@ -253,22 +253,22 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
                 y[j + 2] = __int2float_rn((int)v[a][j + 2]) * sx * sw.z;
                 y[j + 3] = __int2float_rn((int)v[a][j + 3]) * sx * sw.w;
               }
-              if constexpr (MODE == I8_RESIDUAL) {
+              if constexpr (MODE == I8_RESIDUAL) {       // (__fadd_rn: see i8_finish4)
                 if (p.o.wide) {
 #pragma unroll
                   for (int j = 0; j < 32; ++j) {
                     if constexpr (sizeof(T) == 4) {
-                      y[j] += __uint_as_float(own[j]);
+                      y[j] = __fadd_rn(y[j], __uint_as_float(own[j]));
                     } else {
                       const uint32_t q = own[h * 16 + j / 2];
-                      if constexpr (std::is_same_v<T, __half>) y[j] += __half2float(__ushort_as_half((unsigned short)(j & 1 ? q >> 16 : q)));
-                      else y[j] += j & 1 ? bf16_hi(q) : bf16_lo(q);
+                      if constexpr (std::is_same_v<T, __half>) y[j] = __fadd_rn(y[j], __half2float(__ushort_as_half((unsigned short)(j & 1 ? q >> 16 : q))));
+                      else y[j] = __fadd_rn(y[j], j & 1 ? bf16_hi(q) : bf16_lo(q));
                     }
                   }
                 } else if (lane < rows) {
 #pragma unroll
                   for (int j = 0; j < 32; ++j)
-                    if (col + j < n_end) y[j] += to_f(residual[(row0 + lane) * p.o.ldo + col + j]);
+                    if (col + j < n_end) y[j] = __fadd_rn(y[j], to_f(residual[(row0 + lane) * p.o.ldo + col + j]));
                 }
               }
               if constexpr (MODE == I8_GATED) {
