@@ -21,7 +21,7 @@ namespace jl {
 constexpr int I8S_BM = 128, I8S_BK = 128, I8S_THREADS = 256;      // warp 0: TMA, warp 1: MMA, warp 2: TMEM; 4-7 (split: all): results
 constexpr uint32_t I8S_A_BYTES = I8S_BM * I8S_BK, I8S_STAGING = 16 * I8S_BM * 4;
 constexpr int I8S_PARTS = 8;                                      // of K, at most
-constexpr int I8S_HALF = 112 * 1024, I8S_WIDE = 201 * 1024;       // shared memory of a CTA of two an SM, of one
+constexpr int I8S_HALF = 112 * 1024, I8S_WIDE = 201 * 1024;       // shared memory of a CTA: of two an SM, of one
 
 struct Int8Swap {
   Int8Out o;
@@ -260,33 +260,75 @@ static size_t i8s_smem(int stages, int nb, bool split, int experts) {
   return (size_t)stages * (I8S_A_BYTES + nb * I8S_BK) + (split ? 0 : I8S_STAGING) + 8 * (2 * stages + 4) + 16 + 4 * i8_table_ints(experts) + 1024;
 }
 
-// Parts of K, a cluster's CTAs: up to eight of at least four k-blocks that fill both slots of nearly every SM; clusters find place for about 264 CTAs (48 tiles of 100 rows, K 4096: 5
-// parts 12.6 us, 6 parts 18.5; 32 tiles of 6 rows, K 14336: 2 parts 20.7, 4 15.2, 8 13.1).  Above 128 rows a CTA fills an SM: up to four, for about 128.
-static int i8s_parts(int nb, long long tiles, int num_kb, int num_sms) {
-  const int slots = nb > 128 ? num_sms - 20 : 2 * num_sms - 32;
+// Parts of K, a cluster's CTAs, at most `most` of at least four k-blocks each, for `tiles` tiles in `slots` CTAs
+static int i8s_parts(long long tiles, int num_kb, int most, int slots) {
   long long ks = slots / tiles;
-  const int most = nb > 128 ? 4 : I8S_PARTS;
   if (ks > most) ks = most;
   if (ks > num_kb / 4) ks = num_kb / 4;
   return ks > 1 ? (int)ks : 1;
 }
+// Two CTAs an SM: clusters find place for about 264 CTAs (48 tiles of 100 rows, K 4096: 5 parts 12.6 us, 6 parts 18.5; 32 tiles of 6 rows, K 14336: 2 parts 20.7, 4 15.2, 8 13.1)
+static int i8s_slots(int num_sms) { return 2 * num_sms - 32; }
+
+// How a product of M rows with one matrix is cut: pieces of rows, parts of K, and whether a CTA has an SM and its shared memory to itself.  pieces 0: the pairs' kernel.
+//
+// Up to 64 rows the weights' stream is all there is: one piece, K in up to eight parts, two CTAs an SM.  With more, a deeper ring for one CTA an SM and fewer, longer parts pay (the parts'
+// meeting takes 20 ns a row, a k-block 1.4 ns a row beside its weights); then pieces of half the rows, where that leaves K in as many parts or K is short; few features take
+// more and smaller pieces, to use the SMs at all.  us, one piece in eight or four parts -> as below: 72 x 4096 x 4096 10.4 -> 9.8; 100 x 4096 x 4096 11.8 -> 10.0; 128 x 4096 x
+// 14336 20.5 -> 18.0; 128 x 8192 x 2048 12.0 -> 10.2; 100 x 1024 x 1024 7.6 -> 6.3; 200 x 2048 x 8192 15.4 -> 13.3; 256 x 4096 x 4096 14.5 -> 13.5; 256 x 1024 x 4096 12.3 -> 9.7;
+// 256 x 6144 x 4096 16.8 -> 15.2; 512 x 1024 x 4096 14.2 -> 11.8.  One piece stays better for a long K: 256 x 4096 x 14336 23.1 and 25.6, 160 x 4096 x 4096 11.2 and 11.7; and two CTAs an SM
+// up to 80 rows over many features: 72 x 6144 x 4096 10.9 and 11.4.
+// Pairs otherwise (us here | there: 130 x 4096 x 4096 10.7 | 16.3; 512 x 4096 x 4096 17.2 | 18.3; 400 x 2048 x 2048 11.0 | 11.5; 333 x 6144 x 4096 in three pieces 16.9 | 18.4; 200 x 1024 x
+// 1024 9.3 | 6.9; 333 x 1000 x 960 9.0 | 7.3; K in one part: 256 x 28672 x 4096 45 | 32, 512 x 6144 x 4096 19.4 | 18.8).
+struct Int8Cut { int pieces, parts, wide; };
+static Int8Cut i8s_cut(int M, int N, int K, int num_sms) {
+  const int cols = (N + I8S_BM - 1) / I8S_BM, kb = (K + I8S_BK - 1) / I8S_BK, both = i8s_slots(num_sms), one = num_sms - 20;
+  const bool few = cols <= 10;
+  if (M <= 64) return {1, i8s_parts(cols, kb, I8S_PARTS, both), 0};
+  if (M <= 128) {
+    if (few) {
+      const int c = (M + 47) / 48;
+      return {c, i8s_parts((long long)cols * c, kb, 6, one), 0};
+    }
+    if (cols <= one / 2 && (M > 80 || cols <= one / 3)) return {1, i8s_parts(cols, kb, cols <= one / 6 ? 6 : 4, one), 1};
+    return {1, i8s_parts(cols, kb, I8S_PARTS, both), 0};
+  }
+  if (M > 512 || kb < 16) return {0, 0, 0};
+  if (few) {
+    const int c = (M + 111) / 112 < 4 ? (M + 111) / 112 : 4;
+    return {c, i8s_parts((long long)cols * c, kb, 6, one), 1};
+  }
+  if (M > 256) {
+    const int ks = i8s_parts(2ll * cols, kb, 4, one);
+    if (ks > 1) return {2, ks, 1};
+    if (M <= 384 && 3ll * cols > one && 3ll * cols <= num_sms) return {3, 1, 1};
+    return {0, 0, 0};
+  }
+  if (cols <= one / 6 || (kb <= 48 && M > 176)) {
+    const int ks = i8s_parts(2ll * cols, kb, 4, one);
+    if (ks > 1) return {2, ks, 1};
+    const int two = i8s_parts(2ll * cols, kb, 4, both);
+    return two > 1 ? Int8Cut{2, two, 0} : Int8Cut{0, 0, 0};
+  }
+  const int ks = i8s_parts(cols, kb, 4, one);
+  return ks > 1 ? Int8Cut{1, ks, 1} : Int8Cut{0, 0, 0};
+}
 
 template <int MODE>
-static int swap_launch(const void* xq, const void* wq, Int8Swap p, int ldx, int ldw, int num_sms, cudaStream_t stream) {
+static int swap_launch(const void* xq, const void* wq, Int8Swap p, int ldx, int ldw, bool wide, int num_sms, cudaStream_t stream) {
   const int E = p.work.experts;
   p.work.cols = (p.o.N + I8S_BM - 1) / I8S_BM;
   p.work.chunk = p.nb;
   const int num_kb = (p.K + I8S_BK - 1) / I8S_BK;
   const long long most = p.work.cols * i8_pieces(p.work, p.nb);      // tiles, at most
   JL_CHECK_ARG(most < (1ll << 30), "int8 product: %lld tiles", most);
-  p.ksplit = i8s_parts(p.nb, most, num_kb, num_sms);
   const bool split = p.ksplit > 1;
   p.cols = p.nb <= 32 ? 32 : p.nb <= 64 ? 64 : p.nb <= 128 ? 128 : 256;
   p.idesc = tc::idesc_s8_s32(I8S_BM, p.nb);
   const int stage = (int)I8S_A_BYTES + p.nb * I8S_BK, room = 4 * i8_table_ints(E) + (split ? 0 : (int)I8S_STAGING);
-  int stages = ((p.nb > 128 ? I8S_WIDE : I8S_HALF) - 2048 - room) / stage;      // (2 KB: barriers, alignment)
+  int stages = ((wide ? I8S_WIDE : I8S_HALF) - 2048 - room) / stage;      // (2 KB: barriers, alignment)
   if (stages > 10) stages = 10;
-  const int slots = p.nb <= 128 ? 2 * num_sms : num_sms;
+  const int slots = wide ? num_sms : 2 * num_sms;
   const long long blocks = split ? (num_kb + p.ksplit - 1) / p.ksplit : (most + slots - 1) / slots * num_kb;
   const int tile = split ? (p.nb * I8S_BM * 4 + stage - 1) / stage : 2;                    // a split's partial fits the ring
   if (stages > blocks) stages = (int)blocks;
@@ -331,12 +373,13 @@ int int8_vec(const void* x, int dtype, long long ldx, const void* gain, float ep
              cudaStream_t stream);
 int int8_pair(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8Work work, int K, int mode, int num_sms, cudaStream_t stream);
 
-static int int8_swap(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8Work work, int K, int nb, int mode, int num_sms, cudaStream_t stream) {
+// nb: rows of a tile; parts of K; wide: a CTA has an SM to itself (above 128 rows: always)
+static int int8_swap(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8Work work, int K, int nb, int parts, bool wide, int mode, int num_sms, cudaStream_t stream) {
   Int8Swap p{};
-  p.o = o; p.work = work; p.K = K; p.nb = nb;
-  if (mode == I8_PLAIN) return swap_launch<I8_PLAIN>(xq, wq, p, ldx, ldw, num_sms, stream);
-  if (mode == I8_RESIDUAL) return swap_launch<I8_RESIDUAL>(xq, wq, p, ldx, ldw, num_sms, stream);
-  return swap_launch<I8_GATED>(xq, wq, p, ldx, ldw, num_sms, stream);
+  p.o = o; p.work = work; p.K = K; p.nb = nb; p.ksplit = parts;
+  if (mode == I8_PLAIN) return swap_launch<I8_PLAIN>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
+  if (mode == I8_RESIDUAL) return swap_launch<I8_RESIDUAL>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
+  return swap_launch<I8_GATED>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
 }
 
 static int up16(int k) { return (k + 15) / 16 * 16; }
@@ -380,13 +423,11 @@ extern "C" JL_API int jl_linear_int8(const void* x, int dtype, int M, int K, lon
   if ((rc = int8_rows(x, dtype, M, K, ldx, nullptr, M, gain, eps, scratch, ldq, xs, resident ? 2 : 1, (cudaStream_t)stream))) return rc;
   const Int8Out o = out_of(out, residual, xs, ws, out_dtype, N, mode);
   const Int8Work work{nullptr, 1, M, 0, 0};
-  const int chunks = (M + 255) / 256, nb = ((M + chunks - 1) / chunks + 15) / 16 * 16;
-  // Up to 128 rows weights fill the MMA's rows; up to 512 where K, split over clusters, then gives every SM work and is long enough to pay for the meeting; pairs above (us,
-  // weights as rows | pairs: 130 x 4096 x 4096 10.7 | 16.9; 256 x 4096 x 4096 14.5 | 17.3; 512 x 4096 x 4096 17.2 | 18.4; 400 x 2048 x 2048 11.0 | 12.0; 200 x 1024 x 1024
-  // 9.2 | 7.2; 333 x 1000 x 960 8.9 | 7.5; no parts: 256 x 28672 x 4096 46 | 34; 333 x 6144 x 4096 21.0 | 19.3).
-  const long long tiles = (long long)((N + I8S_BM - 1) / I8S_BM) * chunks;
-  if (M <= 128 || (M <= 512 && K >= 2048 && i8s_parts(nb, tiles, 16, num_sms) > 1))
-    return int8_swap(scratch, ldq, wq, ldw, o, work, K, nb, mode, num_sms, (cudaStream_t)stream);
+  const Int8Cut cut = i8s_cut(M, N, K, num_sms);
+  if (cut.pieces > 0) {
+    const int nb = ((M + cut.pieces - 1) / cut.pieces + 15) / 16 * 16;
+    return int8_swap(scratch, ldq, wq, ldw, o, work, K, nb, cut.parts, cut.wide != 0, mode, num_sms, (cudaStream_t)stream);
+  }
   return int8_pair(scratch, ldq, wq, ldw, o, work, K, mode, num_sms, (cudaStream_t)stream);
 }
 
@@ -415,5 +456,7 @@ extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, lo
   const int even = (T + experts - 1) / experts;
   const long long tiles = (N + I8S_BM - 1) / I8S_BM * i8_pieces(work, 16);
   if (even > 160 && tiles > 2 * num_sms) return int8_pair(scratch, ldq, wq, ldw, o, work, K, mode, num_sms, (cudaStream_t)stream);
-  return int8_swap(scratch, ldq, wq, ldw, o, work, K, tiles <= 2 * num_sms || even <= 1 ? 16 : even <= 24 ? 32 : 64, mode, num_sms, (cudaStream_t)stream);
+  const int nb = tiles <= 2 * num_sms || even <= 1 ? 16 : even <= 24 ? 32 : 64;
+  const int parts = i8s_parts((N + I8S_BM - 1) / I8S_BM * i8_pieces(work, nb), (K + I8S_BK - 1) / I8S_BK, I8S_PARTS, i8s_slots(num_sms));
+  return int8_swap(scratch, ldq, wq, ldw, o, work, K, nb, parts, false, mode, num_sms, (cudaStream_t)stream);
 }

@@ -479,6 +479,20 @@ def test_every_kernel_gives_a_row_the_same_bits(N, K, dtype):
             assert torch.equal(I.expert_linear_int8(x[:M], e, off, mode=mode), full[:M])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N,K", [(200, 2500), (1000, 2056), (2100, 4100), (4096, 2048), (6200, 2064), (4500, 6400), (16380, 2080), (130, 70)])
+def test_however_a_product_is_cut(N, K, dtype):
+    """Pieces of rows and parts of K depend on the sizes; a row's results do not."""
+    I, K_ = _ops()
+    x, w, r = _randn(520, K, seed=3, dtype=dtype), _weight(N, K), _randn(520, N, seed=4, dtype=dtype)
+    plain, more = I.linear_int8(x, w), I.linear_int8(x, w, mode=K_.RESIDUAL, residual=r)
+    off, want = O.bound(O.products(*O.rows(x), w.values, w.scales), dtype)
+    _check(plain, off, want)
+    for M in (1, 2, 7, 16, 48, 64, 65, 80, 81, 97, 112, 128, 129, 144, 176, 177, 225, 256, 257, 336, 337, 384, 385, 449, 512):
+        assert torch.equal(I.linear_int8(x[:M], w), plain[:M])
+        assert torch.equal(I.linear_int8(x[:M], w, mode=K_.RESIDUAL, residual=r[:M]), more[:M])
+
+
 @pytest.mark.parametrize("counts,N", [([600, 700, 500], 1024), ([900, 0, 1100], 2050)])
 def test_gathered_rows_of_pairs(counts, N):
     """Many rows of few tokens: every token is brought to 8 bits once and gathered; indices that are not there give zeros, rows of no expert stay."""
