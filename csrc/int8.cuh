@@ -267,21 +267,29 @@ __device__ __forceinline__ void i8_list(const Int8Work& w, int* table) {
     return;
   }
   int ahead = 0;
-  for (int e0 = 0; e0 < E; e0 += 32) {
-    const int e = e0 + lane;
-    int a = 0, n = 0;
-    if (e < E) {
-      a = i8_offset(w, e);
-      n = max(i8_offset(w, e + 1) - a, 0);
+  for (int e0 = 0; e0 < E; e0 += 128) {             // four neighbours a lane: their offsets come at once
+    const int e = e0 + 4 * lane;
+    int at[5], tiles[4];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) at[i] = i8_offset(w, min(e + i, E));
+    int incl = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      tiles[i] = (max(at[i + 1] - at[i], 0) + w.chunk - 1) / w.chunk * w.cols;
+      incl += tiles[i];
     }
-    const int mine = (n + w.chunk - 1) / w.chunk * w.cols;
-    int incl = mine;
+    const int mine = incl;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
-    if (e < E) { table[e] = ahead + incl - mine; table[E + 1 + e] = a; }
+    int before = ahead + incl - mine;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (e + i < E) { table[e + i] = before; table[E + 1 + e + i] = at[i]; }
+      before += tiles[i];
+    }
     ahead += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (lane == 0) { table[E] = ahead; table[2 * E + 1] = i8_offset(w, E); }
@@ -291,7 +299,11 @@ __device__ __forceinline__ void i8_list(const Int8Work& w, int* table) {
 struct Int8Walk {
   int e = 0;
   __device__ __forceinline__ Int8Tile at(const Int8Work& w, const int* table, int t) {
-    while (t >= table[e + 1]) ++e;
+    // the last expert whose tiles begin at or ahead of t: steps that double, then halve (128 experts, one by one: 2 us)
+    int step = 1;
+    for (; e + step < w.experts && t >= table[e + step]; step *= 2) e += step;
+    for (; step > 0; step /= 2)
+      if (e + step < w.experts && t >= table[e + step]) e += step;
     const int row = table[w.experts + 1 + e], end = table[w.experts + 2 + e];
     const int pieces = (end - row + w.chunk - 1) / w.chunk, i = t - table[e];
     Int8Tile tile;
