@@ -371,6 +371,9 @@ int int8_rows(const void* x, int dtype, int M, int K, long long ldx, const int* 
 bool int8_vec_takes(int rows, int N, int K);
 int int8_vec(const void* x, int dtype, long long ldx, const void* gain, float eps, const void* wq, int ldw, Int8Out o, int rows, int K, int mode, bool early, int num_sms,
              cudaStream_t stream);
+bool int8_vec_takes_pairs(int pairs, int N, int K);
+int int8_vec_pairs(const void* x, int dtype, int M, long long ldx, const int* index, int pairs, const int* offsets, int experts, const void* wq, int ldw, Int8Out o, int K, int mode,
+                   int num_sms, cudaStream_t stream);
 int int8_pair(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8Work work, int K, int mode, int num_sms, cudaStream_t stream);
 
 // nb: rows of a tile; parts of K; wide: a CTA has an SM to itself (above 128 rows: always)
@@ -400,7 +403,7 @@ using namespace jl;
 static size_t values_bytes(int rows, int K) { return rows < 0 || K < 1 ? 0 : ((size_t)rows * up16(K) + 255) / 256 * 256 + (size_t)rows * 4; }
 extern "C" JL_API size_t jl_linear_int8_scratch_bytes(int M, int N, int K) { return int8_vec_takes(M, N, K) ? 0 : values_bytes(M, K); }
 
-extern "C" JL_API size_t jl_experts_int8_scratch_bytes(int T, int K) { return values_bytes(T, K); }
+extern "C" JL_API size_t jl_experts_int8_scratch_bytes(int T, int N, int K) { return int8_vec_takes_pairs(T, N, K) ? 0 : values_bytes(T, K); }
 
 extern "C" JL_API int jl_linear_int8(const void* x, int dtype, int M, int K, long long ldx, const void* wq, int ldw, const float* ws, int N, const void* gain, float eps,
                                      const void* residual, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int resident, int num_sms, void* stream) {
@@ -442,6 +445,10 @@ extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, lo
   JL_CHECK_ARG(mode == I8_PLAIN || (mode == I8_GATED && N % 2 == 0), "jl_experts_int8: mode %d, N=%d", mode, N);
   if (T == 0) return JL_OK;
   if (num_sms <= 0) num_sms = SMS;
+  if (int8_vec_takes_pairs(T, N, K)) {
+    const Int8Out o = out_of(out, nullptr, nullptr, ws, out_dtype, N, mode);
+    return int8_vec_pairs(x, dtype, M, M > 1 ? ldx : K, rows, T, offsets, experts, wq, ldw, o, K, mode, num_sms, (cudaStream_t)stream);
+  }
   JL_CHECK_ARG(scratch != nullptr && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= values_bytes(T, K),
                "jl_experts_int8: scratch of %zu bytes", scratch_bytes);
   const int ldq = up16(K);

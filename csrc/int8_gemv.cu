@@ -6,6 +6,7 @@
 // units; the warps' partial sums meet in shared memory, one barrier a unit, whole numbers, in any order the same.
 // Every CTA brings the activations to 8 bits itself while its first weights are under way, which saves a launch.
 // Bound by latency, then the weights: one B200, us in a chain of cold weights, 1 x 64 x 256 2.9, 1 x 64 x 4096 3.7, 1 x 2048 x 4096 4.8, 1 x 4096 x 4096 6.1 (2.6 at the memory's rate).
+// A mixture of experts: a CTA has one of up to eight rows and finds whose it is; a token's four of 32 experts of 2048 x 2048 8.6 (2.6 at the memory's rate): its weights wait for the router.
 // One CTA an SM, which would let the next launch's first weights in, streams too little: 1 x 28672 x 4096 22 -> 35.
 #include "int8.cuh"
 #include "jllama_b200.h"
@@ -25,6 +26,10 @@ struct Int8Vec {
   int rows, K, ldw, units, pieces;  // units of features; pieces of a warp
   float eps;
   int early;                        // weights may be read ahead of the wait for the kernels before
+  // the form for few rows of a mixture of experts: a CTA has one of `pairs` rows (blockIdx.y) and its expert's weights; `rows` is 1
+  const int* offsets;               // [experts + 1], as Int8Work
+  const int* index;                 // [pairs] rows of x, or nullptr: the pair's own
+  int experts, pairs, there;        // there: rows of x
 };
 
 __device__ __forceinline__ void i8v_mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -35,7 +40,7 @@ __device__ __forceinline__ void i8v_mma(int (&d)[4], uint32_t a0, uint32_t a1, u
 
 __host__ __device__ constexpr int i8v_pitch(int K) { return (K + 127) / 128 * 128 + 64; }      // rows in shared memory: two rows of 64 bytes meet all banks
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool EXPERTS>
 __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec p) {
   extern __shared__ __align__(16) uint8_t i8v_smem[];
   __shared__ int parts[2][I8V_WARPS][I8V_ROWS][I8V_FEATURES];
@@ -47,13 +52,37 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
   const int pitch = i8v_pitch(p.K), units = p.units;
   pdl_launch_dependents();
 
+  Int8Out out = p.o;
+  const int8_t* weights = p.wq;
+  const T* source = reinterpret_cast<const T*>(p.x);
+  int first = 0;                                                 // row of the result
+  bool real = true;                                              // the row is there: an index that x does not have is a row of zeros
+  if constexpr (EXPERTS) {
+    __shared__ int holder;
+    if (threadIdx.x == 0) holder = -1;
+    __syncthreads();
+    pdl_wait();
+    first = blockIdx.y;
+    const int row = p.index != nullptr ? __ldcg(p.index + first) : first;
+    const Int8Work work{p.offsets, p.experts, p.pairs, 0, 0};
+    for (int i = threadIdx.x; i < p.experts; i += I8V_THREADS)
+      if (i8_offset(work, i) <= first && first < i8_offset(work, i + 1)) holder = i;      // (one, where offsets rise)
+    __syncthreads();
+    const int e = holder;
+    if (e < 0) return;                                           // a row of no expert is left as it was
+    weights += (size_t)e * p.o.N * p.ldw;
+    out.ws += (size_t)e * p.o.N;
+    real = (unsigned)row < (unsigned)p.there;
+    if (real) source += (long long)row * p.ldx;
+  }
+
   // ---- the stream of this warp's pieces: unit after unit
   int u_load = blockIdx.x, j_load = 0;
   const int8_t *w_lo, *w_hi;                                     // rows g and g + 8 of the unit
   auto place = [&]() {
     const int f = u_load * I8V_FEATURES + g, last = p.o.N - 1;
-    w_lo = p.wq + (size_t)min(f, last) * p.ldw + 16 * t4;
-    w_hi = p.wq + (size_t)min(f + 8, last) * p.ldw + 16 * t4;
+    w_lo = weights + (size_t)min(f, last) * p.ldw + 16 * t4;
+    w_hi = weights + (size_t)min(f + 8, last) * p.ldw + 16 * t4;
   };
   auto load = [&](uint4 (&buf)[8]) {
     const int c0 = (j_load * I8V_WARPS + warp) * I8V_PIECE;
@@ -68,17 +97,17 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
   };
   place();
   uint4 buf0[8], buf1[8];
-  if (!p.early) pdl_wait();
+  if (!EXPERTS && !p.early) pdl_wait();
   load(buf0);
   load(buf1);
-  if (p.early) pdl_wait();
+  if (!EXPERTS && p.early) pdl_wait();
 
   // ---- the activations' rows in 8 bits: 8 / R' warps a row, R' = 1, 2, 4, 8
   {
     const int R = p.rows, per = R <= 1 ? 8 : R <= 2 ? 4 : R <= 4 ? 2 : 1;            // warps of a row
     const int row = warp / per, n = per * 32, i0 = threadIdx.x - row * n;
     const bool there = row < R;
-    const T* x = reinterpret_cast<const T*>(p.x) + (there ? (long long)row * p.ldx : 0);
+    const T* x = source + (there ? (long long)row * p.ldx : 0);
     const T* gain = reinterpret_cast<const T*>(p.gain);
     constexpr int VE = 16 / sizeof(T);
     // once from memory, all loads at once; what a thread keeps of the row it alone reads again
@@ -94,7 +123,7 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
       for (int i = i0 * VE; i < p.K; i += 4 * n * VE) {
         uint4 v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = i + u * n * VE < p.K ? *reinterpret_cast<const uint4*>(x + i + u * n * VE) : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < 4; ++u) v[u] = real && i + u * n * VE < p.K ? *reinterpret_cast<const uint4*>(x + i + u * n * VE) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           if (i + u * n * VE >= p.K) break;
@@ -108,7 +137,7 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
     } else if (there) {
       // element by element; a thread's places are those of its pieces
       for (int i = i0 * VE; i < p.K; i += n * VE)
-        for (int e = 0; e < VE && i + e < p.K; ++e) { raw[i + e] = x[i + e]; see(to_f(x[i + e])); }
+        for (int e = 0; e < VE && i + e < p.K; ++e) { raw[i + e] = real ? x[i + e] : T(0.0f); see(to_f(raw[i + e])); }
     }
     if (gain != nullptr) {
       sum = warp_sum(sum);
@@ -221,20 +250,20 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
         }
         float sw[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sw[i] = f0 + i < p.o.N ? p.o.ws[f0 + i] : 0.0f;
-        i8_finish4<MODE>(p.o, r, f0, sum, row_scale[r], sw);
+        for (int i = 0; i < 4; ++i) sw[i] = f0 + i < p.o.N ? out.ws[f0 + i] : 0.0f;
+        i8_finish4<MODE>(out, first + r, f0, sum, row_scale[r], sw);
       }
     }
   }
 }
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool EXPERTS = false>
 static int vec_launch(const Int8Vec& p, size_t smem, int num_sms, cudaStream_t stream) {
-  auto kern = int8_vec_kernel<T, MODE>;
+  auto kern = int8_vec_kernel<T, MODE, EXPERTS>;
   // equal shares: as many CTAs as give each the same number of units, up to two an SM
-  const int slots = 2 * num_sms, rounds = (p.units + slots - 1) / slots, grid = (p.units + rounds - 1) / rounds;
-  JL_CUDA((i8_room<int8_vec_kernel<T, MODE>, I8V_SMEM>()));
-  JL_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(I8V_THREADS), smem, stream, p));
+  const int slots = 2 * num_sms / (EXPERTS ? p.pairs : 1), rounds = (p.units + slots - 1) / slots, grid = (p.units + rounds - 1) / rounds;
+  JL_CUDA((i8_room<int8_vec_kernel<T, MODE, EXPERTS>, I8V_SMEM>()));
+  JL_CUDA(launch_pdl(kern, dim3((unsigned)grid, EXPERTS ? p.pairs : 1), dim3(I8V_THREADS), smem, stream, p));
   return JL_OK;
 }
 
@@ -245,18 +274,41 @@ bool int8_vec_takes(int rows, int N, int K) {
   return rows <= I8V_ROWS && (rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8) * (long long)K <= I8V_FUSED && (long long)N * K <= (rows <= 2 ? 1 << 25 : 1 << 23);
 }
 
-int int8_vec(const void* x, int dtype, long long ldx, const void* gain, float eps, const void* wq, int ldw, Int8Out o, int rows, int K, int mode, bool early, int num_sms,
-             cudaStream_t stream) {
+static Int8Vec vec_of(const void* x, long long ldx, const void* gain, float eps, const void* wq, int ldw, const Int8Out& o, int rows, int K, bool early) {
   Int8Vec p{};
   p.o = o;
   p.wq = (const int8_t*)wq; p.x = x; p.gain = gain; p.ldx = ldx; p.rows = rows; p.K = K; p.ldw = ldw; p.eps = eps; p.early = early;
   p.units = (o.N + I8V_FEATURES - 1) / I8V_FEATURES;
   p.pieces = (K + I8V_PIECE * I8V_WARPS - 1) / (I8V_PIECE * I8V_WARPS);
-  const size_t smem = (size_t)rows * (i8v_pitch(K) + (K + 7) / 8 * 8 * (dtype == DT_F32 ? 4 : 2));      // values, and the rows themselves
+  return p;
+}
+// values, and the rows themselves
+static size_t vec_smem(int rows, int K, int dtype) { return (size_t)rows * (i8v_pitch(K) + (K + 7) / 8 * 8 * (dtype == DT_F32 ? 4 : 2)); }
+
+int int8_vec(const void* x, int dtype, long long ldx, const void* gain, float eps, const void* wq, int ldw, Int8Out o, int rows, int K, int mode, bool early, int num_sms,
+             cudaStream_t stream) {
+  const Int8Vec p = vec_of(x, ldx, gain, eps, wq, ldw, o, rows, K, early);
+  const size_t smem = vec_smem(rows, K, dtype);
   JL_DISPATCH_INT8(dtype, {
     if (mode == I8_PLAIN) return vec_launch<T, I8_PLAIN>(p, smem, num_sms, stream);
     if (mode == I8_RESIDUAL) return vec_launch<T, I8_RESIDUAL>(p, smem, num_sms, stream);
     return vec_launch<T, I8_GATED>(p, smem, num_sms, stream);
+  });
+}
+
+// Whether `pairs` rows of a mixture of experts run here (us here | there, gated: of 32 experts of 2048 x 2048 1 pair 5.7 | 7.7, 4 8.6 | 10.0, 8 11.1 | 12.3, 16 15.6 | 13.7; of 128 of 1536 x
+// 2048 8 10.1 | 11.7; of 8 of 8192 x 4096 2 16.0 | 17.2, 4 23.2 | 21.7; 4096 x 14336 1 16.7 | 16.6).
+bool int8_vec_takes_pairs(int pairs, int N, int K) { return pairs <= I8V_ROWS && K <= I8V_FUSED && (long long)pairs * N * K <= 1 << 26; }
+
+// `pairs` rows, row index[i] of x [M, K] (or row i) with the weights of the expert whose offsets hold i
+int int8_vec_pairs(const void* x, int dtype, int M, long long ldx, const int* index, int pairs, const int* offsets, int experts, const void* wq, int ldw, Int8Out o, int K, int mode,
+                   int num_sms, cudaStream_t stream) {
+  Int8Vec p = vec_of(x, ldx, nullptr, 0.0f, wq, ldw, o, 1, K, false);
+  p.offsets = offsets; p.index = index; p.experts = experts; p.pairs = pairs; p.there = M;
+  const size_t smem = vec_smem(1, K, dtype);
+  JL_DISPATCH_INT8(dtype, {
+    if (mode == I8_PLAIN) return vec_launch<T, I8_PLAIN, true>(p, smem, num_sms, stream);
+    return vec_launch<T, I8_GATED, true>(p, smem, num_sms, stream);
   });
 }
 

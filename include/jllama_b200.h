@@ -601,10 +601,10 @@ int jl_logit_rules(const void* logits, int dtype, int B, int V, int ld, float* o
  * used.  mode 0 plain, 1 + residual (out's type and size, may be out), 2 silu(y[2j]) y[2j+1].  K <= 131072.  resident: no kernel directly before the call writes the weights.
  * jl_experts_int8: out[t], offsets[e] <= t < offsets[e + 1], of row rows[t] of x against expert e's weights wq [experts][N][ldw], ws [experts][N]; offsets [experts + 1] on
  * the device; other rows of out are left as they were.  mode 0 or 2; experts <= 1024.
- * scratch: jl_linear_int8_scratch_bytes(M, N, K) (0: none) or, for experts, jl_experts_int8_scratch_bytes(T, K) bytes of any content on a 16-byte boundary; calls that may run at the
+ * scratch: jl_linear_int8_scratch_bytes(M, N, K) or, for experts, jl_experts_int8_scratch_bytes(T, N, K) bytes (0: none) of any content on a 16-byte boundary; calls that may run at the
  * same time need one each. */
 int jl_int8_rows(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int n, const void* gain, float eps, void* q, int ldq, float* s, void* stream);
-size_t jl_experts_int8_scratch_bytes(int T, int K);
+size_t jl_experts_int8_scratch_bytes(int T, int N, int K);
 size_t jl_linear_int8_scratch_bytes(int M, int N, int K);
 int jl_linear_int8(const void* x, int dtype, int M, int K, long long ldx, const void* wq, int ldw, const float* ws, int N, const void* gain, float eps,
                    const void* residual, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int resident, int num_sms, void* stream);

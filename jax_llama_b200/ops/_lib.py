@@ -21,7 +21,7 @@ i32, f32, u64, sz, i64 = C.c_int, C.c_float, C.c_ulonglong, C.c_size_t, C.c_long
 _SIGNATURES = {
     "jl_last_error": (C.c_char_p, []),
     "jl_int8_rows": (i32, [vp, i32, i32, i32, i64, ip, i32, vp, f32, vp, i32, fp, vp]),
-    "jl_experts_int8_scratch_bytes": (sz, [i32, i32]),
+    "jl_experts_int8_scratch_bytes": (sz, [i32, i32, i32]),
     "jl_linear_int8_scratch_bytes": (sz, [i32, i32, i32]),
     "jl_linear_int8": (i32, [vp, i32, i32, i32, i64, vp, i32, fp, i32, vp, f32, vp, vp, i32, i32, vp, sz, i32, i32, vp]),
     "jl_experts_int8": (i32, [vp, i32, i32, i32, i64, ip, i32, ip, i32, vp, i32, fp, i32, vp, i32, i32, vp, sz, i32, vp]),

@@ -294,9 +294,10 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
         _few(who, max(M, T))
         held, sms = w._held
         L = _lib.lib()
-        need = L.jl_experts_int8_scratch_bytes(T, k)
+        need = L.jl_experts_int8_scratch_bytes(T, w.n, k)
+        scratch = x.new_empty(need, dtype=torch.uint8).data_ptr() if need else 0
         rc = L.jl_experts_int8(x.data_ptr(), TYPES[x.dtype], M, k, pitch, 0 if rows is None else rows.data_ptr(), T, offsets.data_ptr(), w.experts, *held, out.data_ptr(),
-                               TYPES[out.dtype], mode, x.new_empty(need, dtype=torch.uint8).data_ptr(), need, sms, _stream())
+                               TYPES[out.dtype], mode, scratch, need, sms, _stream())
         if rc:
             _lib.check(rc, "jl_experts_int8")
     return out

@@ -311,6 +311,34 @@ def test_experts(counts, N, K, dtype):
         _expert_check(x, w, rows, offsets, T, mode, dtype, out)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("E", [1, 3, 32, 300, 1024])
+@pytest.mark.parametrize("N,K", [(18, 40), (130, 1001), (256, 4096), (34, 16384)])
+def test_few_pairs(N, K, E, dtype):
+    """A token's experts and a few tokens': each row with its expert, wherever among the experts that is; some rows of none."""
+    I, K_ = _ops()
+    x, w = _randn(5, K, seed=1, dtype=dtype), _weight(E, N, K, seed=2)
+    g = torch.Generator().manual_seed(E)
+    for lead, pairs, behind in ((0, 1, 0), (1, 2, 0), (0, 4, 1), (2, 3, 3), (0, 8, 0), (0, 0, 3)):
+        T = lead + pairs + behind
+        counts = torch.bincount(torch.randint(0, E, (pairs,), generator=g), minlength=E)
+        offsets = (lead + torch.cat([torch.zeros(1, dtype=torch.long), counts.cumsum(0)])).to(torch.int32).to(DEV)
+        rows = torch.randint(0, 5, (T,), generator=g).to(torch.int32).to(DEV)
+        for mode in (K_.PLAIN, K_.SWIGLU):
+            out = torch.full((T, N // 2 if mode == K_.SWIGLU else N), 3.0, dtype=dtype, device=DEV)
+            I.expert_linear_int8(x, w, offsets, rows=rows, mode=mode, out=out)
+            _expert_check(x, w, rows, offsets, T, mode, dtype, out)
+            again = torch.zeros(T + 30, out.shape[1], dtype=dtype, device=DEV)        # with rows behind them another kernel runs: the same bits
+            I.expert_linear_int8(x, w, offsets, rows=torch.cat([rows, rows.new_zeros(30)]), mode=mode, out=again)
+            assert torch.equal(again[lead:lead + pairs], out[lead:lead + pairs])
+            none = I.expert_linear_int8(x[:0], w, offsets, rows=rows, mode=mode)[lead:lead + pairs]
+            assert not none.any()
+    strided = _randn(5, 2 * K + 1, seed=4, dtype=dtype)[:, 1:K + 1]                  # rows off any boundary
+    offsets = torch.full((E + 1,), 5, dtype=torch.int32, device=DEV)
+    offsets[0] = 0
+    _expert_check(strided, w, None, offsets, 5, K_.PLAIN, dtype, I.expert_linear_int8(strided, w, offsets))
+
+
 def test_experts_without_an_index_and_of_other_types():
     I, K_ = _ops()
     counts = [5, 0, 70, 30]
