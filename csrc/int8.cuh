@@ -196,25 +196,49 @@ __device__ __forceinline__ float2 i8_unpack(int kind, uint32_t w) {
 // silu(g) u.  The quotient is the product with an approximate reciprocal (two units in the last place): a true one branches, and values then wait for one another
 __device__ __forceinline__ float i8_gate(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
-// four neighbouring residuals (index of the first one: a multiple of four where `wide`)
-__device__ __forceinline__ void i8_residual4(const Int8Out& o, size_t at, int f0, float (&r)[4]) {
-  if (o.wide) {
-    if (o.kind == DT_F32) {
-      load4(reinterpret_cast<const float*>(o.residual) + at, r);
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(o.residual) + at);
-      const float2 a = i8_unpack(o.kind, w.x), b = i8_unpack(o.kind, w.y);
-      r[0] = a.x; r[1] = a.y; r[2] = b.x; r[3] = b.y;
-    }
-    return;
-  }
+// Four neighbouring residuals, asked for ahead of i8_finish4 (no load passes a store to what may be the same buffer) and held as they are in memory where KIND, the type, is known.
+template <int KIND>
+struct Int8Four {
+  static constexpr bool packed = KIND == DT_BF16 || KIND == DT_F16;
+  std::conditional_t<packed, uint2, float4> v;
+  __device__ __forceinline__ void load(const Int8Out& o, int row, int f0) {
+    if (f0 >= o.N) return;
+    const size_t at = (size_t)row * o.ldo + f0;
+    const int kind = KIND >= 0 ? KIND : o.kind;
+    if constexpr (packed) {
+      const uint16_t* r = reinterpret_cast<const uint16_t*>(o.residual) + at;
+      if (o.wide) { v = *reinterpret_cast<const uint2*>(r); return; }
+      uint32_t e[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = f0 + i < o.N ? i8_load(o.residual, o.kind, at + i) : 0.0f;
-}
-
-// finishes and stores features f0 .. f0 + 3 (f0 a multiple of four) of a row of the result from their sums
-template <int MODE>
-__device__ __forceinline__ void i8_finish4(const Int8Out& o, int row, int f0, const int (&acc)[4], float sx, const float (&sw)[4]) {
+      for (int i = 0; i < 4; ++i) e[i] = f0 + i < o.N ? r[i] : 0u;
+      v = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
+    } else if (o.wide && kind == DT_F32) {
+      v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(o.residual) + at);
+    } else if (o.wide) {
+      const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(o.residual) + at);
+      const float2 a = i8_unpack(kind, w.x), b = i8_unpack(kind, w.y);
+      v = make_float4(a.x, a.y, b.x, b.y);
+    } else {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = f0 + i < o.N ? i8_load(o.residual, kind, at + i) : 0.0f;
+      v = make_float4(e[0], e[1], e[2], e[3]);
+    }
+  }
+  __device__ __forceinline__ float4 floats() const {
+    if constexpr (packed) {
+      const float2 a = i8_unpack(KIND, v.x), b = i8_unpack(KIND, v.y);
+      return make_float4(a.x, a.y, b.x, b.y);
+    } else {
+      return v;
+    }
+  }
+};
+// KIND: the result's type where the kernel is one of it (what is finished runs once a launch from cold instructions: fewer are faster), or -1.
+// Finishes and stores features f0 .. f0 + 3 (f0 a multiple of four) of a row of the result from their sums
+template <int MODE, int KIND = -1>
+__device__ __forceinline__ void i8_finish4(const Int8Out& o, int row, int f0, const int (&acc)[4], float sx, const float (&sw)[4], const Int8Four<KIND>& residual) {
+  const int kind = KIND >= 0 ? KIND : o.kind;
   float y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] = __int2float_rn(acc[i]) * sx * sw[i];
@@ -222,29 +246,27 @@ __device__ __forceinline__ void i8_finish4(const Int8Out& o, int row, int f0, co
     const float a = i8_gate(y[0], y[1]), b = i8_gate(y[2], y[3]);
     const size_t at = (size_t)row * o.ldo + f0 / 2;
     if (o.wide && f0 + 3 < o.N) {
-      if (o.kind == DT_F32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(o.out) + at) = make_float2(a, b);
-      else *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(o.out) + at) = i8_pack(o.kind, a, b);
+      if (kind == DT_F32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(o.out) + at) = make_float2(a, b);
+      else *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(o.out) + at) = i8_pack(kind, a, b);
       return;
     }
-    if (f0 < o.N) i8_store(o.out, o.kind, at, a);
-    if (f0 + 2 < o.N) i8_store(o.out, o.kind, at + 1, b);
+    if (f0 < o.N) i8_store(o.out, kind, at, a);
+    if (f0 + 2 < o.N) i8_store(o.out, kind, at + 1, b);
     return;
   }
   const size_t at = (size_t)row * o.ldo + f0;
   if constexpr (MODE == I8_RESIDUAL) {
-    float r[4];
-    i8_residual4(o, at, f0, r);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = __fadd_rn(y[i], r[i]);       // never fused with the scale's product: a row's bits do not depend on the kernel
+    const float4 r = residual.floats();       // never fused with the scale's product: a row's bits do not depend on the kernel
+    y[0] = __fadd_rn(y[0], r.x); y[1] = __fadd_rn(y[1], r.y); y[2] = __fadd_rn(y[2], r.z); y[3] = __fadd_rn(y[3], r.w);
   }
   if (o.wide) {
-    if (o.kind == DT_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(o.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
-    else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(o.out) + at) = make_uint2(i8_pack(o.kind, y[0], y[1]), i8_pack(o.kind, y[2], y[3]));
+    if (kind == DT_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(o.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+    else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(o.out) + at) = make_uint2(i8_pack(kind, y[0], y[1]), i8_pack(kind, y[2], y[3]));
     return;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (f0 + i < o.N) i8_store(o.out, o.kind, at + i, y[i]);
+    if (f0 + i < o.N) i8_store(o.out, kind, at + i, y[i]);
 }
 
 // The work of a launch as a list: `chunks` pieces of at most `chunk` rows of every expert times `cols` tiles of features; a tile's pieces are neighbours, since they

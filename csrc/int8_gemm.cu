@@ -41,7 +41,7 @@ __device__ __forceinline__ int4 i8s_ld_cluster(uint32_t addr) {
   return v;
 }
 
-template <int MODE, bool SPLIT>
+template <int MODE, bool SPLIT, int KIND>
 __global__ void __launch_bounds__(I8S_THREADS, 2)
 int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Int8Swap p) {
   extern __shared__ uint8_t smem_raw[];
@@ -159,6 +159,7 @@ int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 #pragma unroll
     for (int i = 0; i < 4; ++i) sw[i] = f0 + i < p.o.N ? s[i] : 0.0f;
   };
+  constexpr int DEPTH = KIND == DT_F32 ? 1 : 2;             // how far ahead residuals are asked for: 32 registers
   if constexpr (!SPLIT) {
     // ===================================================== epilogue of a persistent CTA: warps 4-7, 16 rows at a time
     if (warp >= 4) {
@@ -176,10 +177,20 @@ int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
           for (int i = 0; i < 2; ++i) sx[i] = c + 32 * i + lane < t.rows ? p.o.xs[t.row0 + c + 32 * i + lane] : 0.0f;
         };
         row_scales(0);
+        Int8Four<KIND> r4[DEPTH + 1][4];                    // residuals of 16 rows each, asked for while those before them are finished
+        auto residuals = [&](int c, Int8Four<KIND>(&r)[4]) {
+          if constexpr (MODE == I8_RESIDUAL) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (c + (lane >> 3) + 4 * u < t.rows) r[u].load(p.o, t.row0 + c + (lane >> 3) + 4 * u, f0);
+          }
+        };
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) residuals(16 * d, r4[d + 1]);
         tc::mbar_wait(tfull_bar(as), (it >> 1) & 1);
         tc::fence_after_sync();
         for (int c64 = 0; c64 < t.rows; c64 += 64) {
-#pragma unroll
+#pragma unroll 1
           for (int q = 0; q < 4; ++q) {
             const int c0 = c64 + 16 * q;
             if (c0 >= t.rows) break;
@@ -188,13 +199,18 @@ int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
             __syncwarp();
             if (c0 + 16 >= t.rows && lane == 0) tc::mbar_arrive(tempty_bar(as));      // read: the sums of the tile after next may begin
 #pragma unroll
+            for (int d = 0; d < DEPTH; ++d)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) r4[d][u] = r4[d + 1][u];
+            residuals(c0 + 16 * DEPTH, r4[DEPTH]);
+#pragma unroll
             for (int u = 0; u < 4; ++u) {
               const int r = (lane >> 3) + 4 * u, row = c0 + r;
-              const float s = __shfl_sync(0xffffffffu, sx[q / 2], 16 * (q & 1) + r);
+              const float s = __shfl_sync(0xffffffffu, q < 2 ? sx[0] : sx[1], 16 * (q & 1) + r);
               if (f0 >= p.o.N || row >= t.rows) continue;
               int x[4];
               asm volatile("ld.shared.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(st + r * 128 + (lane & 7) * 16) : "memory");
-              i8_finish4<MODE>(p.o, t.row0 + row, f0, x, s, sw);
+              i8_finish4<MODE, KIND>(p.o, t.row0 + row, f0, x, s, sw, r4[0][u]);
             }
             __syncwarp();
           }
@@ -212,24 +228,37 @@ int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     const uint32_t put = smem_base + ((warp & 3) * 32 + lane) * 4, get = smem_base + lane * 16;
     float sw[4];
     feature_scales(t.expert, f0, sw);
-    if (tile0 < tiles) tc::mbar_wait(tfull_bar(0), 0);
-    tc::fence_after_sync();
-    // the ring is free (all MMAs done) and takes the partial
-    for (int c0 = (warp >> 2) * 16; c0 < t.rows; c0 += 32) to_shared(t_lane + c0, put + c0 * row, row);
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    auto share = [&]() {
+      if (tile0 < tiles) tc::mbar_wait(tfull_bar(0), 0);
+      tc::fence_after_sync();
+      // the ring is free (all MMAs done) and takes the partial
+      for (int c0 = (warp >> 2) * 16; c0 < t.rows; c0 += 32) to_shared(t_lane + c0, put + c0 * row, row);
+      asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    };
     const int per = (t.rows + ksplit - 1) / ksplit, t_lo = rank * per, t_hi = min(t_lo + per, t.rows);
-    // a warp takes U rows at a time, all ranks' parts of them on their way together
+    // a warp takes U rows at a time, all ranks' parts of them on their way together; the first rows' scales and residuals before the sums are there
     auto meet = [&](auto ranks, auto many) {
       constexpr int R = decltype(ranks)::value, U = decltype(many)::value;
+      float sx[DEPTH][U];
+      Int8Four<KIND> r4[DEPTH][U];
+      auto ahead = [&](int r0, int d) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (r0 + 8 * u >= t_hi) continue;
+          sx[d][u] = p.o.xs[t.row0 + r0 + 8 * u];
+          if constexpr (MODE == I8_RESIDUAL) r4[d][u].load(p.o, t.row0 + r0 + 8 * u, f0);
+        }
+      };
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) ahead(t_lo + warp + 8 * U * d, d);
+      share();
       for (int r0 = t_lo + warp; r0 < t_hi; r0 += 8 * U) {
         int4 part[U][R];
-        float sx[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int at = r0 + 8 * u;
           if (at >= t_hi) continue;
-          sx[u] = p.o.xs[t.row0 + at];
 #pragma unroll
           for (int r = 0; r < R; ++r)
             if (r < ksplit) part[u][r] = i8s_ld_cluster(i8s_mapa(get, r) + at * row);
@@ -242,8 +271,13 @@ int8_swap_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 #pragma unroll
           for (int r = 0; r < R; ++r)
             if (r < ksplit) { x[0] += part[u][r].x; x[1] += part[u][r].y; x[2] += part[u][r].z; x[3] += part[u][r].w; }
-          if (f0 < p.o.N) i8_finish4<MODE>(p.o, t.row0 + at, f0, x, sx[u], sw);
+          if (f0 < p.o.N) i8_finish4<MODE, KIND>(p.o, t.row0 + at, f0, x, sx[0][u], sw, r4[0][u]);
         }
+#pragma unroll
+        for (int d = 0; d + 1 < DEPTH; ++d)
+#pragma unroll
+          for (int u = 0; u < U; ++u) { sx[d][u] = sx[d + 1][u]; r4[d][u] = r4[d + 1][u]; }
+        ahead(r0 + 8 * U * DEPTH, DEPTH - 1);
       }
     };
     if (ksplit <= 4) meet(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
@@ -314,7 +348,7 @@ static Int8Cut i8s_cut(int M, int N, int K, int num_sms) {
   return ks > 1 ? Int8Cut{1, ks, 1} : Int8Cut{0, 0, 0};
 }
 
-template <int MODE>
+template <int MODE, int KIND>
 static int swap_launch(const void* xq, const void* wq, Int8Swap p, int ldx, int ldw, bool wide, int num_sms, cudaStream_t stream) {
   const int E = p.work.experts;
   p.work.cols = (p.o.N + I8S_BM - 1) / I8S_BM;
@@ -339,8 +373,8 @@ static int swap_launch(const void* xq, const void* wq, Int8Swap p, int ldx, int 
   if ((rc = make_tmap_2d_i8(&tw, wq, (uint64_t)p.o.N * E, p.K, ldw, I8S_BM))) return rc;
   if ((rc = make_tmap_2d_i8(&tx, xq, p.work.rows, p.K, ldx, p.nb))) return rc;
   const size_t smem = i8s_smem(stages, p.nb, split, E);
-  auto kern = split ? int8_swap_kernel<MODE, true> : int8_swap_kernel<MODE, false>;
-  JL_CUDA(split ? (i8_room<int8_swap_kernel<MODE, true>>()) : (i8_room<int8_swap_kernel<MODE, false>>()));
+  auto kern = split ? int8_swap_kernel<MODE, true, KIND> : int8_swap_kernel<MODE, false, KIND>;
+  JL_CUDA(split ? (i8_room<int8_swap_kernel<MODE, true, KIND>>()) : (i8_room<int8_swap_kernel<MODE, false, KIND>>()));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(split ? most * p.ksplit : most < slots ? most : slots));
   cfg.blockDim = dim3(I8S_THREADS);
@@ -380,9 +414,14 @@ int int8_pair(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8W
 static int int8_swap(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8Work work, int K, int nb, int parts, bool wide, int mode, int num_sms, cudaStream_t stream) {
   Int8Swap p{};
   p.o = o; p.work = work; p.K = K; p.nb = nb; p.ksplit = parts;
-  if (mode == I8_PLAIN) return swap_launch<I8_PLAIN>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
-  if (mode == I8_RESIDUAL) return swap_launch<I8_RESIDUAL>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
-  return swap_launch<I8_GATED>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
+  auto launch = [&](auto kind) {
+    constexpr int KIND = decltype(kind)::value;
+    if (mode == I8_PLAIN) return swap_launch<I8_PLAIN, KIND>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
+    if (mode == I8_RESIDUAL) return swap_launch<I8_RESIDUAL, KIND>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
+    return swap_launch<I8_GATED, KIND>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
+  };
+  if (o.kind == DT_F32) return launch(std::integral_constant<int, DT_F32>{});
+  return o.kind == DT_BF16 ? launch(std::integral_constant<int, DT_BF16>{}) : launch(std::integral_constant<int, DT_F16>{});
 }
 
 static int up16(int k) { return (k + 15) / 16 * 16; }

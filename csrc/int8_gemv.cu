@@ -251,7 +251,9 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
         float sw[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sw[i] = f0 + i < p.o.N ? out.ws[f0 + i] : 0.0f;
-        i8_finish4<MODE>(out, first + r, f0, sum, row_scale[r], sw);
+        Int8Four<-1> r4;
+        if constexpr (MODE == I8_RESIDUAL) r4.load(out, first + r, f0);
+        i8_finish4<MODE>(out, first + r, f0, sum, row_scale[r], sw, r4);
       }
     }
   }
