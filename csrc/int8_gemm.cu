@@ -7,7 +7,7 @@
 // The launch ahead is always the one that brings the activations to 8 bits, which lets this one start when the kernels before it are done (or, with resident weights, at
 // once): offsets and weights are read without waiting for it.
 // Bound by the weights' way from memory with few rows: one B200, us in a chain of cold weights, the rows' kernel included, 1 x 28672 x 4096 20.1 (5.9 TB/s), 16 x 4096 x 4096 7.8, 48 x
-// 28672 x 4096 gated 22.9 (5.3 TB/s), 64 tokens x 4 of 32 experts of 2048 x 1024 12.6 (5.4 TB/s); with more by the operands' way from L2 (24 KB for 128 x 64 x 128).
+// 28672 x 4096 gated 22.4 (5.4 TB/s), 64 tokens x 4 of 32 experts of 2048 x 1024 12.9 (5.3 TB/s); with more by the operands' way from L2 (24 KB for 128 x 64 x 128).
 // Few tiles: the CTAs of a cluster share one and take a part of K each; the partials meet in distributed shared memory, whole numbers, so their order
 // changes nothing.
 #include <type_traits>
