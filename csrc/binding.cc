@@ -91,7 +91,7 @@ struct Entry<R (*)(A...)> {
   X(jl_flash_prefill_masked) X(jl_causal_conv) X(jl_ssd_gates) X(jl_ssd_scan) X(jl_gated_groupnorm) X(jl_delta_scan)                     \
   X(jl_delta_scan_ws_floats) X(jl_delta_head_scan) X(jl_delta_head_scan_ws_floats) X(jl_weighted_sum2) X(jl_rownorm_gate)                \
   X(jl_postnorm_cast) X(jl_branch_add_cast) X(jl_attn_prep_all) X(jl_activated_scan) X(jl_mlstm_gates) X(jl_mlstm_scan)                  \
-  X(jl_mlstm_finish) X(jl_int8_rows) X(jl_experts_int8_scratch_bytes) X(jl_linear_int8_scratch_bytes) X(jl_linear_int8) X(jl_experts_int8) X(jl_moe_order)
+  X(jl_mlstm_finish) X(jl_int8_rows) X(jl_experts_int8_scratch_bytes) X(jl_linear_int8_scratch_bytes) X(jl_linear_int8) X(jl_experts_int8) X(jl_choice_int8) X(jl_moe_order)
 
 #define JL_SLOT(name) decltype(&name) slot_##name = nullptr;
 JL_ENTRIES(JL_SLOT)

@@ -406,7 +406,8 @@ bool int8_vec_takes(int rows, int N, int K);
 int int8_vec(const void* x, int dtype, long long ldx, const void* gain, float eps, const void* wq, int ldw, Int8Out o, int rows, int K, int mode, bool early, int num_sms,
              cudaStream_t stream);
 bool int8_vec_takes_pairs(int pairs, int N, int K);
-int int8_vec_pairs(const void* x, int dtype, int M, long long ldx, const int* index, int pairs, const int* offsets, int experts, const void* wq, int ldw, Int8Out o, int K, int mode,
+bool int8_vec_holds_pairs(int pairs, int K);
+int int8_vec_pairs(const void* x, int dtype, int M, long long ldx, const int* index, int pairs, const int* offsets, const int* choice, int top, int experts, const void* wq, int ldw, Int8Out o, int K, int mode,
                    int num_sms, cudaStream_t stream);
 int int8_pair(const void* xq, int ldx, const void* wq, int ldw, Int8Out o, Int8Work work, int K, int mode, int num_sms, cudaStream_t stream);
 
@@ -486,7 +487,7 @@ extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, lo
   if (num_sms <= 0) num_sms = SMS;
   if (int8_vec_takes_pairs(T, N, K)) {
     const Int8Out o = out_of(out, nullptr, nullptr, ws, out_dtype, N, mode);
-    return int8_vec_pairs(x, dtype, M, M > 1 ? ldx : K, rows, T, offsets, experts, wq, ldw, o, K, mode, num_sms, (cudaStream_t)stream);
+    return int8_vec_pairs(x, dtype, M, M > 1 ? ldx : K, rows, T, offsets, nullptr, 1, experts, wq, ldw, o, K, mode, num_sms, (cudaStream_t)stream);
   }
   JL_CHECK_ARG(scratch != nullptr && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= values_bytes(T, K),
                "jl_experts_int8: scratch of %zu bytes", scratch_bytes);
@@ -505,4 +506,18 @@ extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, lo
   const int nb = tiles <= 2 * num_sms || even <= 1 ? 16 : even <= 24 ? 32 : 64;
   const int parts = i8s_parts((N + I8S_BM - 1) / I8S_BM * i8_pieces(work, nb), (K + I8S_BK - 1) / I8S_BK, I8S_PARTS, i8s_slots(num_sms));
   return int8_swap(scratch, ldq, wq, ldw, o, work, K, nb, parts, false, mode, num_sms, (cudaStream_t)stream);
+}
+
+extern "C" JL_API int jl_choice_int8(const void* x, int dtype, int M, int K, long long ldx, const int* choice, int top, int experts, const void* wq, int ldw, const float* ws, int N,
+                                     void* out, int out_dtype, int mode, int num_sms, void* stream) {
+  JL_CHECK_ARG(dtype >= DT_BF16 && dtype <= DT_F16 && out_dtype >= DT_BF16 && out_dtype <= DT_F16, "jl_choice_int8: element types %d, %d", dtype, out_dtype);
+  JL_CHECK_ARG(M >= 0 && top >= 1 && (long long)M * top <= I8_MAX_ROWS && N >= 1 && K >= 1 && int8_vec_holds_pairs(M * top, K) && (ldx >= K || M <= 1),
+               "jl_choice_int8: M=%d top=%d N=%d K=%d, pitch %lld (at most 8 rows of 16384)", M, top, N, K, ldx);
+  JL_CHECK_ARG(experts >= 1 && experts <= I8_MAX_EXPERTS && (long long)N * experts < (1ll << 31) && choice != nullptr, "jl_choice_int8: %d experts (at most %d), %d features", experts,
+               I8_MAX_EXPERTS, N);
+  JL_CHECK_ARG(ldw >= K && ldw % 16 == 0 && ((uintptr_t)wq & 15) == 0, "jl_choice_int8: weights on 16-byte rows (pitch %d)", ldw);
+  JL_CHECK_ARG(mode == I8_PLAIN || (mode == I8_GATED && N % 2 == 0), "jl_choice_int8: mode %d, N=%d", mode, N);
+  if (M == 0) return JL_OK;
+  const Int8Out o = out_of(out, nullptr, nullptr, ws, out_dtype, N, mode);
+  return int8_vec_pairs(x, dtype, M, M > 1 ? ldx : K, nullptr, M * top, nullptr, choice, top, experts, wq, ldw, o, K, mode, num_sms > 0 ? num_sms : SMS, (cudaStream_t)stream);
 }

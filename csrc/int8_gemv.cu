@@ -29,7 +29,8 @@ struct Int8Vec {
   // the form for few rows of a mixture of experts: a CTA has one of `pairs` rows (blockIdx.y) and its expert's weights; `rows` is 1
   const int* offsets;               // [experts + 1], as Int8Work
   const int* index;                 // [pairs] rows of x, or nullptr: the pair's own
-  int experts, pairs, there;        // there: rows of x
+  const int* choice;                // [pairs] experts, in any order, instead of offsets and index: the row of x is pair / top
+  int experts, pairs, there, top;   // there: rows of x
 };
 
 __device__ __forceinline__ void i8v_mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -56,20 +57,29 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
   const int8_t* weights = p.wq;
   const T* source = reinterpret_cast<const T*>(p.x);
   int first = 0;                                                 // row of the result
-  bool real = true;                                              // the row is there: an index that x does not have is a row of zeros
+  bool real = true, nobody = false;                              // the row is there (an index that x does not have is a row of zeros); no expert's: zeros
   if constexpr (EXPERTS) {
-    __shared__ int holder;
-    if (threadIdx.x == 0) holder = -1;
-    __syncthreads();
-    pdl_wait();
     first = blockIdx.y;
-    const int row = p.index != nullptr ? __ldcg(p.index + first) : first;
-    const Int8Work work{p.offsets, p.experts, p.pairs, 0, 0};
-    for (int i = threadIdx.x; i < p.experts; i += I8V_THREADS)
-      if (i8_offset(work, i) <= first && first < i8_offset(work, i + 1)) holder = i;      // (one, where offsets rise)
-    __syncthreads();
-    const int e = holder;
-    if (e < 0) return;                                           // a row of no expert is left as it was
+    int e, row;
+    if (p.choice != nullptr) {
+      pdl_wait();
+      e = __ldcg(p.choice + first);
+      row = first / p.top;
+      nobody = (unsigned)e >= (unsigned)p.experts;
+      if (nobody) { e = 0; row = -1; }
+    } else {
+      __shared__ int holder;
+      if (threadIdx.x == 0) holder = -1;
+      __syncthreads();
+      pdl_wait();
+      row = p.index != nullptr ? __ldcg(p.index + first) : first;
+      const Int8Work work{p.offsets, p.experts, p.pairs, 0, 0};
+      for (int i = threadIdx.x; i < p.experts; i += I8V_THREADS)
+        if (i8_offset(work, i) <= first && first < i8_offset(work, i + 1)) holder = i;      // (one, where offsets rise)
+      __syncthreads();
+      e = holder;
+      if (e < 0) return;                                         // a row of no expert is left as it was
+    }
     weights += (size_t)e * p.o.N * p.ldw;
     out.ws += (size_t)e * p.o.N;
     real = (unsigned)row < (unsigned)p.there;
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
         }
         float sw[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sw[i] = f0 + i < p.o.N ? out.ws[f0 + i] : 0.0f;
+        for (int i = 0; i < 4; ++i) sw[i] = f0 + i < p.o.N && !nobody ? out.ws[f0 + i] : 0.0f;
         Int8Four<-1> r4;
         if constexpr (MODE == I8_RESIDUAL) r4.load(out, first + r, f0);
         i8_finish4<MODE>(out, first + r, f0, sum, row_scale[r], sw, r4);
@@ -298,15 +308,18 @@ int int8_vec(const void* x, int dtype, long long ldx, const void* gain, float ep
   });
 }
 
-// Whether `pairs` rows of a mixture of experts run here (us here | there, gated: of 32 experts of 2048 x 2048 1 pair 5.7 | 7.7, 4 8.6 | 10.0, 8 11.1 | 12.3, 16 15.6 | 13.7; of 128 of 1536 x
-// 2048 8 10.1 | 11.7; of 8 of 8192 x 4096 2 16.0 | 17.2, 4 23.2 | 21.7; 4096 x 14336 1 16.7 | 16.6).
-bool int8_vec_takes_pairs(int pairs, int N, int K) { return pairs <= I8V_ROWS && K <= I8V_FUSED && (long long)pairs * N * K <= 1 << 26; }
+// Whether `pairs` rows of a mixture of experts can run here
+bool int8_vec_holds_pairs(int pairs, int K) { return pairs <= I8V_ROWS && K <= I8V_FUSED; }
 
-// `pairs` rows, row index[i] of x [M, K] (or row i) with the weights of the expert whose offsets hold i
-int int8_vec_pairs(const void* x, int dtype, int M, long long ldx, const int* index, int pairs, const int* offsets, int experts, const void* wq, int ldw, Int8Out o, int K, int mode,
+// Whether they do (us here | there, gated: of 32 experts of 2048 x 2048 1 pair 5.7 | 7.7, 4 8.6 | 10.0, 8 11.1 | 12.3, 16 15.6 | 13.7; of 128 of 1536 x
+// 2048 8 10.1 | 11.7; of 8 of 8192 x 4096 2 16.0 | 17.2, 4 23.2 | 21.7; 4096 x 14336 1 16.7 | 16.6).
+bool int8_vec_takes_pairs(int pairs, int N, int K) { return int8_vec_holds_pairs(pairs, K) && (long long)pairs * N * K <= 1 << 26; }
+
+// `pairs` rows, row index[i] of x [M, K] (or row i) with the weights of the expert whose offsets hold i; or row i / top with those of expert choice[i]
+int int8_vec_pairs(const void* x, int dtype, int M, long long ldx, const int* index, int pairs, const int* offsets, const int* choice, int top, int experts, const void* wq, int ldw, Int8Out o, int K, int mode,
                    int num_sms, cudaStream_t stream) {
   Int8Vec p = vec_of(x, ldx, nullptr, 0.0f, wq, ldw, o, 1, K, false);
-  p.offsets = offsets; p.index = index; p.experts = experts; p.pairs = pairs; p.there = M;
+  p.offsets = offsets; p.index = index; p.choice = choice; p.top = top; p.experts = experts; p.pairs = pairs; p.there = M;
   const size_t smem = vec_smem(1, K, dtype);
   JL_DISPATCH_INT8(dtype, {
     if (mode == I8_PLAIN) return vec_launch<T, I8_PLAIN, true>(p, smem, num_sms, stream);

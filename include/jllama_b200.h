@@ -601,6 +601,7 @@ int jl_logit_rules(const void* logits, int dtype, int B, int V, int ld, float* o
  * used.  mode 0 plain, 1 + residual (out's type and size, may be out), 2 silu(y[2j]) y[2j+1].  K <= 131072.  resident: no kernel directly before the call writes the weights.
  * jl_experts_int8: out[t], offsets[e] <= t < offsets[e + 1], of row rows[t] of x against expert e's weights wq [experts][N][ldw], ws [experts][N]; offsets [experts + 1] on
  * the device; other rows of out are left as they were.  mode 0 or 2; experts <= 1024.
+ * jl_choice_int8: out[m top + k] of row m of x against expert choice[m top + k] (zeros where there is none), without an order: M top <= 8, K <= 16384.
  * scratch: jl_linear_int8_scratch_bytes(M, N, K) or, for experts, jl_experts_int8_scratch_bytes(T, N, K) bytes (0: none) of any content on a 16-byte boundary; calls that may run at the
  * same time need one each. */
 int jl_int8_rows(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int n, const void* gain, float eps, void* q, int ldq, float* s, void* stream);
@@ -610,6 +611,8 @@ int jl_linear_int8(const void* x, int dtype, int M, int K, long long ldx, const 
                    const void* residual, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int resident, int num_sms, void* stream);
 int jl_experts_int8(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int T, const int* offsets, int experts, const void* wq, int ldw,
                     const float* ws, int N, void* out, int out_dtype, int mode, void* scratch, size_t scratch_bytes, int num_sms, void* stream);
+int jl_choice_int8(const void* x, int dtype, int M, int K, long long ldx, const int* choice, int top, int experts, const void* wq, int ldw, const float* ws, int N,
+                   void* out, int out_dtype, int mode, int num_sms, void* stream);
 /* The M * top (token, choice) pairs ordered by expert with nothing between experts: pos [M * top]: row of each pair (-1 where idx < 0); row_src [M * top]: token of each row
  * (-1 behind the last); offsets [E + 1]: first row of every expert, and behind the last. */
 int jl_moe_order(const int* idx, int M, int top, int E, int* pos, int* row_src, int* offsets, void* stream);

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import math
-from typing import Dict, List, Optional, Tuple
+from typing import Callable, Dict, List, Optional, Tuple
 
 import numpy as np
 import torch
@@ -218,14 +218,21 @@ class MoeFeedForward:
 
     def _experts_int8(self, h: torch.Tensor, idx: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """(fp32 rows of the experts' results, the row of every pair)."""
-        s = self.spec
-        pos, rows, offsets = I8.expert_order(idx, s.experts)
-        if self.turns:
-            t = I8.expert_linear_int8(h, self.up8, offsets, rows=rows, mode=SWIGLU)
-        else:
-            y = I8.expert_linear_int8(h, self.up8, offsets, rows=rows, out_f32=True)
-            t = _gated_act(y, self.u_off, s.ff, s.act, s.limit, h.dtype) if s.gated else SK.act_cast(y, h.dtype, self.act)
+        pos, rows, offsets = I8.expert_order(idx, self.spec.experts)
+        t = self._hidden_int8(h.dtype, lambda **kw: I8.expert_linear_int8(h, self.up8, offsets, rows=rows, **kw))
         return I8.expert_linear_int8(t, self.down8, offsets, out_f32=True), pos
+
+    def _few_int8(self, h: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
+        """fp32 rows of the experts' results, one for every pair: a decoding token's, or a few tokens'."""
+        t = self._hidden_int8(h.dtype, lambda **kw: I8.choice_linear_int8(h, self.up8, idx, **kw))
+        return I8.choice_linear_int8(t, self.down8, idx.view(-1, 1), out_f32=True)
+
+    def _hidden_int8(self, dtype: torch.dtype, up: Callable[..., torch.Tensor]) -> torch.Tensor:
+        s = self.spec
+        if self.turns:
+            return up(mode=SWIGLU)
+        y = up(out_f32=True)
+        return _gated_act(y, self.u_off, s.ff, s.act, s.limit, dtype) if s.gated else SK.act_cast(y, dtype, self.act)
 
     def _parts(self, h: torch.Tensor) -> Tuple[tuple, dict]:
         """Everything ahead of the weighted sum: its arguments."""
@@ -236,7 +243,9 @@ class MoeFeedForward:
         idx, wt = SK.moe_route(z, self.n_route, s.top, s.groups, s.keep, s.group_top, self.score, s.normalise, s.scale,
                                bias=self.router_bias, choice_bias=self.choice_bias, n_real=s.experts, ident_w=ident_w)
         n_up = self.up.shape[1] if self.up8 is None else 0                         # ff, or gate | up rows of a gated expert
-        if self.up8 is not None:
+        if self.up8 is not None and idx.numel() <= I8.MAX_CHOICES and max(self.up8.k, self.down8.k) <= I8.MAX_CHOICE_K:
+            y, pos = self._few_int8(h, idx), None
+        elif self.up8 is not None:
             y, pos = self._experts_int8(h, idx)
         elif M <= SK.MOE_PAIR_ROWS:
             n = M * s.top

@@ -25,6 +25,7 @@ _SIGNATURES = {
     "jl_linear_int8_scratch_bytes": (sz, [i32, i32, i32]),
     "jl_linear_int8": (i32, [vp, i32, i32, i32, i64, vp, i32, fp, i32, vp, f32, vp, vp, i32, i32, vp, sz, i32, i32, vp]),
     "jl_experts_int8": (i32, [vp, i32, i32, i32, i64, ip, i32, ip, i32, vp, i32, fp, i32, vp, i32, i32, vp, sz, i32, vp]),
+    "jl_choice_int8": (i32, [vp, i32, i32, i32, i64, ip, i32, i32, vp, i32, fp, i32, vp, i32, i32, i32, vp]),
     "jl_version": (i32, []),
     "jl_launch_count": (u64, []),
     "jl_embed": (i32, [ip, vp, vp, i32, i32, i32, vp]),

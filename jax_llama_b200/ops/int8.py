@@ -22,6 +22,7 @@ TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 MAX_K = 131072                 # inputs of a layer: 127 * 127 * K stays below 2^31
 MAX_EXPERTS = 1024
 MAX_ROWS = 1 << 30
+MAX_CHOICES, MAX_CHOICE_K = 8, 16384          # rows and inputs of `choice_linear_int8`
 _I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
 
 
@@ -275,7 +276,7 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
     T = M if rows is None else rows.numel()
     out = _result(who, x, pitch, T, w.n, mode, out_f32, out)
     if dev < 0:
-        flat = out.view(T, -1)
+        flat = out.view(T, w.n // 2 if mode == SWIGLU else w.n)
         q, s = _rows_ref(x)
         if rows is not None:
             there = ((rows >= 0) & (rows < M))
@@ -300,4 +301,39 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
                                TYPES[out.dtype], mode, scratch, need, sms, _stream())
         if rc:
             _lib.check(rc, "jl_experts_int8")
+    return out
+
+
+def choice_linear_int8(x: torch.Tensor, w: Int8Weight, choice: torch.Tensor, *, mode: int = PLAIN, out_f32: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`expert_linear_int8` for a decoding token or a few, without an order: [M·top, N] (SWIGLU: [M·top, N / 2]), row m·top + k is row m of x [M, K] against expert
+    choice[m, k] (int32 [M, top], contiguous; zeros for a choice that is no expert's).  One launch; at most MAX_CHOICES rows of at most MAX_CHOICE_K numbers."""
+    who = "choice_linear_int8"
+    if w.__class__ is not Int8Weight or not 1 <= w.experts <= MAX_EXPERTS:
+        raise ValueError(f"{who}: w is an Int8Weight of 1 to {MAX_EXPERTS} experts")
+    if mode not in (PLAIN, SWIGLU):
+        raise ValueError(f"{who}: mode {mode}")
+    dev, k = x.get_device(), w.k
+    x, M, pitch = _take(who, x, k)
+    if dev != w.dev:
+        raise ValueError(f"{who}: x on {x.device}, weights on {w.device}")
+    if choice.dtype is not _I32 or choice.dim() != 2 or choice.shape[0] != M or choice.shape[1] < 1 or not choice.is_contiguous() or choice.get_device() != dev:
+        raise ValueError(f"{who}: choices are int32 [{M}, top], contiguous, on {x.device} (got {choice.dtype}, {tuple(choice.shape)}, {choice.device})")
+    top = choice.shape[1]
+    if M * top > MAX_CHOICES or k > MAX_CHOICE_K:
+        raise ValueError(f"{who}: {M} x {top} rows of {k} numbers (at most {MAX_CHOICES} of {MAX_CHOICE_K}; more go through expert_order)")
+    out = _result(who, x, pitch, M * top, w.n, mode, out_f32, out)
+    if dev < 0:
+        flat = out.view(M * top, w.n // 2 if mode == SWIGLU else w.n)
+        q, s = _rows_ref(x)
+        for i, e in enumerate(choice.reshape(-1).tolist()):
+            m = i // top
+            y = (q[m].double() @ w.values[e].double().t()).float() * s[m] * w.scales[e] if 0 <= e < w.experts else torch.zeros(w.n)
+            flat[i] = _finish_ref(y, None, mode, out.dtype)
+        return out
+    _here(dev, who)
+    if M:
+        held, sms = w._held
+        rc = _lib.lib().jl_choice_int8(x.data_ptr(), TYPES[x.dtype], M, k, pitch, choice.data_ptr(), top, w.experts, *held, out.data_ptr(), TYPES[out.dtype], mode, sms, _stream())
+        if rc:
+            _lib.check(rc, "jl_choice_int8")
     return out

@@ -339,6 +339,38 @@ def test_few_pairs(N, K, E, dtype):
     _expert_check(strided, w, None, offsets, 5, K_.PLAIN, dtype, I.expert_linear_int8(strided, w, offsets))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("E", [1, 3, 32, 1024])
+@pytest.mark.parametrize("N,K", [(18, 40), (130, 1001), (256, 4096), (34, 16384)])
+def test_choices_without_an_order(N, K, E, dtype):
+    I, K_ = _ops()
+    w = _weight(E, N, K, seed=2)
+    g = torch.Generator().manual_seed(E)
+    for M, top in ((1, 1), (1, 4), (2, 3), (8, 1), (1, 8), (0, 2)):
+        x = _randn(M, K + 3, seed=M, dtype=dtype)[:, :K]
+        choice = torch.randint(0, E, (M, top), generator=g).to(torch.int32)
+        if M > 1:
+            choice[1, 0] = -1 if top > 1 else E
+        choice = choice.to(DEV)
+        q, s = O.rows(x) if M else (None, None)
+        pos, rows, offsets = I.expert_order(choice, E)
+        for mode in (K_.PLAIN, K_.SWIGLU):
+            for f32 in (False, True):
+                out = I.choice_linear_int8(x, w, choice, mode=mode, out_f32=f32)
+                assert out.dtype is (F32 if f32 else dtype) and tuple(out.shape) == (M * top, N // 2 if mode == K_.SWIGLU else N)
+                for i, e in enumerate(choice.reshape(-1).tolist()):
+                    if not 0 <= e < E:
+                        assert not out[i].any()
+                        continue
+                    y = O.products(q[i // top:i // top + 1], s[i // top:i // top + 1], w.values[e], w.scales[e])
+                    off, want = O.bound_gated(y, out.dtype) if mode == K_.SWIGLU else O.bound(y, out.dtype)
+                    _check(out[i:i + 1], off, want)
+                if M:
+                    ordered = I.expert_linear_int8(x, w, offsets, rows=rows, mode=mode, out_f32=f32)      # the same bits
+                    there = pos >= 0
+                    assert torch.equal(out[there], ordered[pos[there].long()])
+
+
 def test_experts_without_an_index_and_of_other_types():
     I, K_ = _ops()
     counts = [5, 0, 70, 30]

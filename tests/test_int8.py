@@ -116,6 +116,21 @@ def test_a_layer_of_experts_together():
             assert torch.equal(got[m, c], I.linear_int8(I.linear_int8(x[m:m + 1], one[0], mode=K.SWIGLU), one[1])[0])
 
 
+def test_choices_without_an_order():
+    w, x = _weight(3, 6, 16), _randn(2, 16)
+    choice = torch.tensor([[2, 0], [-1, 1]], dtype=torch.int32)
+    pos, rows, offsets = I.expert_order(choice, 3)
+    for mode in (K.PLAIN, K.SWIGLU):
+        y = I.choice_linear_int8(x, w, choice, mode=mode)
+        z = I.expert_linear_int8(x, w, offsets, rows=rows, mode=mode)
+        assert torch.equal(y[[0, 1, 3]], z[pos[[0, 1, 3]].long()]) and not y[2].any()
+    assert I.choice_linear_int8(x[:0], w, choice[:0], out_f32=True).shape == (0, 6)
+
+
+def test_experts_without_rows():
+    assert I.expert_linear_int8(_randn(0, 16), _weight(3, 6, 16), torch.zeros(4, dtype=torch.int32), mode=K.SWIGLU).shape == (0, 3)
+
+
 # --------------------------------------------------------------------------- refusals
 def test_refusals_of_rows():
     for x in (torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, 4, dtype=torch.float64), torch.zeros(()), torch.zeros(3, 0), torch.zeros(4, 3).t(), torch.zeros(2, 3, 4).transpose(0, 1),
@@ -198,3 +213,13 @@ def test_refusals_of_the_engine():
         B200Engine(cfg, torch.zeros(1), [], torch.zeros(1), torch.zeros(1), weights="int4")
     with pytest.raises(NotImplementedError):
         B200Engine(cfg, torch.zeros(1), [], torch.zeros(1), torch.zeros(1), weights="int8", tp=2)
+
+
+def test_refusals_of_choices():
+    w, x, choice = _weight(2, 6, 16), _randn(3, 16), torch.zeros(3, 2, dtype=torch.int32)
+    bad = [dict(choice=choice.long()), dict(choice=choice[:2]), dict(choice=choice[:, 0]), dict(choice=choice[:, :0]), dict(choice=torch.zeros(2, 3, dtype=torch.int32).t()),
+           dict(choice=torch.zeros(3, 3, dtype=torch.int32)), dict(mode=K.RESIDUAL), dict(w=_weight(6, 16)), dict(w=_weight(2, 5, 16), mode=K.SWIGLU), dict(out=torch.empty(5, 6)),
+           dict(x=_randn(3, 8)), dict(w=_weight(2, 2, I.MAX_CHOICE_K + 1), x=_randn(3, I.MAX_CHOICE_K + 1))]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            I.choice_linear_int8(kw.pop("x", x), kw.pop("w", w), kw.pop("choice", choice), **kw)
