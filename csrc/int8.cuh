@@ -14,7 +14,7 @@
 namespace jl {
 
 enum { DT_F16 = 2 };                                             // beside DT_BF16 and DT_F32
-enum { I8_PLAIN = 0, I8_RESIDUAL = 1, I8_GATED = 2 };            // result; result + residual; silu(y[2j]) y[2j+1]
+enum { I8_PLAIN = 0, I8_RESIDUAL = 1, I8_GATED = 2, I8_RELU2 = 3 };      // result; result + residual; silu(y[2j]) y[2j+1]; relu(y)^2
 constexpr int I8_MAX_K = 131072;
 constexpr int I8_MAX_EXPERTS = 1024;
 constexpr int I8_MAX_ROWS = 1 << 30;
@@ -196,6 +196,12 @@ __device__ __forceinline__ float2 i8_unpack(int kind, uint32_t w) {
 // silu(g) u.  The quotient is the product with an approximate reciprocal (two units in the last place): a true one branches, and values then wait for one another
 __device__ __forceinline__ float i8_gate(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
+// relu(y)^2; a NaN stays one
+__device__ __forceinline__ float i8_relu2(float y) {
+  const float r = y <= 0.0f ? 0.0f : y;
+  return r * r;
+}
+
 // Four neighbouring residuals, asked for ahead of i8_finish4 (no load passes a store to what may be the same buffer) and held as they are in memory where KIND, the type, is known.
 template <int KIND>
 struct Int8Four {
@@ -253,6 +259,10 @@ __device__ __forceinline__ void i8_finish4(const Int8Out& o, int row, int f0, co
     if (f0 < o.N) i8_store(o.out, kind, at, a);
     if (f0 + 2 < o.N) i8_store(o.out, kind, at + 1, b);
     return;
+  }
+  if constexpr (MODE == I8_RELU2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = i8_relu2(y[i]);
   }
   const size_t at = (size_t)row * o.ldo + f0;
   if constexpr (MODE == I8_RESIDUAL) {

@@ -419,6 +419,7 @@ static int int8_swap(const void* xq, int ldx, const void* wq, int ldw, Int8Out o
     constexpr int KIND = decltype(kind)::value;
     if (mode == I8_PLAIN) return swap_launch<I8_PLAIN, KIND>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
     if (mode == I8_RESIDUAL) return swap_launch<I8_RESIDUAL, KIND>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
+    if (mode == I8_RELU2) return swap_launch<I8_RELU2, KIND>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
     return swap_launch<I8_GATED, KIND>(xq, wq, p, ldx, ldw, wide, num_sms, stream);
   };
   if (o.kind == DT_F32) return launch(std::integral_constant<int, DT_F32>{});
@@ -451,7 +452,7 @@ extern "C" JL_API int jl_linear_int8(const void* x, int dtype, int M, int K, lon
   JL_CHECK_ARG(M >= 0 && M <= I8_MAX_ROWS && N >= 1 && N <= I8_MAX_ROWS && K >= 1 && K <= I8_MAX_K && (ldx >= K || M <= 1), "jl_linear_int8: M=%d N=%d K=%d (at most %d), pitch %lld",
                M, N, K, I8_MAX_K, ldx);
   JL_CHECK_ARG(ldw >= K && ldw % 16 == 0 && ((uintptr_t)wq & 15) == 0, "jl_linear_int8: weights on 16-byte rows (pitch %d)", ldw);
-  JL_CHECK_ARG(mode >= I8_PLAIN && mode <= I8_GATED && (mode == I8_RESIDUAL) == (residual != nullptr) && (mode != I8_GATED || N % 2 == 0),
+  JL_CHECK_ARG(mode >= I8_PLAIN && mode <= I8_RELU2 && (mode == I8_RESIDUAL) == (residual != nullptr) && (mode != I8_GATED || N % 2 == 0),
                "jl_linear_int8: mode %d with%s residual, N=%d", mode, residual != nullptr ? "" : "out", N);
   if (M == 0) return JL_OK;
   if (num_sms <= 0) num_sms = SMS;
@@ -482,7 +483,7 @@ extern "C" JL_API int jl_experts_int8(const void* x, int dtype, int M, int K, lo
   JL_CHECK_ARG(experts >= 1 && experts <= I8_MAX_EXPERTS && offsets != nullptr, "jl_experts_int8: %d experts (at most %d)", experts, I8_MAX_EXPERTS);
   JL_CHECK_ARG((long long)N * experts < (1ll << 31), "jl_experts_int8: %d x %d weight rows", experts, N);
   JL_CHECK_ARG(ldw >= K && ldw % 16 == 0 && ((uintptr_t)wq & 15) == 0, "jl_experts_int8: weights on 16-byte rows (pitch %d)", ldw);
-  JL_CHECK_ARG(mode == I8_PLAIN || (mode == I8_GATED && N % 2 == 0), "jl_experts_int8: mode %d, N=%d", mode, N);
+  JL_CHECK_ARG(mode == I8_PLAIN || mode == I8_RELU2 || (mode == I8_GATED && N % 2 == 0), "jl_experts_int8: mode %d, N=%d", mode, N);
   if (T == 0) return JL_OK;
   if (num_sms <= 0) num_sms = SMS;
   if (int8_vec_takes_pairs(T, N, K)) {
@@ -516,7 +517,7 @@ extern "C" JL_API int jl_choice_int8(const void* x, int dtype, int M, int K, lon
   JL_CHECK_ARG(experts >= 1 && experts <= I8_MAX_EXPERTS && (long long)N * experts < (1ll << 31) && choice != nullptr, "jl_choice_int8: %d experts (at most %d), %d features", experts,
                I8_MAX_EXPERTS, N);
   JL_CHECK_ARG(ldw >= K && ldw % 16 == 0 && ((uintptr_t)wq & 15) == 0, "jl_choice_int8: weights on 16-byte rows (pitch %d)", ldw);
-  JL_CHECK_ARG(mode == I8_PLAIN || (mode == I8_GATED && N % 2 == 0), "jl_choice_int8: mode %d, N=%d", mode, N);
+  JL_CHECK_ARG(mode == I8_PLAIN || mode == I8_RELU2 || (mode == I8_GATED && N % 2 == 0), "jl_choice_int8: mode %d, N=%d", mode, N);
   if (M == 0) return JL_OK;
   const Int8Out o = out_of(out, nullptr, nullptr, ws, out_dtype, N, mode);
   return int8_vec_pairs(x, dtype, M, M > 1 ? ldx : K, nullptr, M * top, nullptr, choice, top, experts, wq, ldw, o, K, mode, num_sms > 0 ? num_sms : SMS, (cudaStream_t)stream);

@@ -304,6 +304,7 @@ int int8_vec(const void* x, int dtype, long long ldx, const void* gain, float ep
   JL_DISPATCH_INT8(dtype, {
     if (mode == I8_PLAIN) return vec_launch<T, I8_PLAIN>(p, smem, num_sms, stream);
     if (mode == I8_RESIDUAL) return vec_launch<T, I8_RESIDUAL>(p, smem, num_sms, stream);
+    if (mode == I8_RELU2) return vec_launch<T, I8_RELU2>(p, smem, num_sms, stream);
     return vec_launch<T, I8_GATED>(p, smem, num_sms, stream);
   });
 }
@@ -323,6 +324,7 @@ int int8_vec_pairs(const void* x, int dtype, int M, long long ldx, const int* in
   const size_t smem = vec_smem(1, K, dtype);
   JL_DISPATCH_INT8(dtype, {
     if (mode == I8_PLAIN) return vec_launch<T, I8_PLAIN, true>(p, smem, num_sms, stream);
+    if (mode == I8_RELU2) return vec_launch<T, I8_RELU2, true>(p, smem, num_sms, stream);
     return vec_launch<T, I8_GATED, true>(p, smem, num_sms, stream);
   });
 }

@@ -271,6 +271,10 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
                     if (col + j < n_end) y[j] = __fadd_rn(y[j], to_f(residual[(row0 + lane) * p.o.ldo + col + j]));
                 }
               }
+              if constexpr (MODE == I8_RELU2) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) y[j] = i8_relu2(y[j]);
+              }
               if constexpr (MODE == I8_GATED) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) y[j] = i8_gate(y[2 * j], y[2 * j + 1]);
@@ -333,6 +337,7 @@ template <typename T>
 static cudaError_t pair_kernel(int mode, Int8PairKernel* k) {
   if (mode == I8_PLAIN) { *k = int8_pair_kernel<T, I8_PLAIN>; return i8_room<int8_pair_kernel<T, I8_PLAIN>>(); }
   if (mode == I8_RESIDUAL) { *k = int8_pair_kernel<T, I8_RESIDUAL>; return i8_room<int8_pair_kernel<T, I8_RESIDUAL>>(); }
+  if (mode == I8_RELU2) { *k = int8_pair_kernel<T, I8_RELU2>; return i8_room<int8_pair_kernel<T, I8_RELU2>>(); }
   *k = int8_pair_kernel<T, I8_GATED>;
   return i8_room<int8_pair_kernel<T, I8_GATED>>();
 }

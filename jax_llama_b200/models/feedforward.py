@@ -231,6 +231,8 @@ class MoeFeedForward:
         s = self.spec
         if self.turns:
             return up(mode=SWIGLU)
+        if not s.gated and s.act == "relu2":
+            return up(mode=I8.RELU2)
         y = up(out_f32=True)
         return _gated_act(y, self.u_off, s.ff, s.act, s.limit, dtype) if s.gated else SK.act_cast(y, dtype, self.act)
 

@@ -22,6 +22,7 @@ TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 MAX_K = 131072                 # inputs of a layer: 127 * 127 * K stays below 2^31
 MAX_EXPERTS = 1024
 MAX_ROWS = 1 << 30
+RELU2 = 3                      # a mode beside `kernels`' PLAIN, RESIDUAL and SWIGLU: relu(y)²
 MAX_CHOICES, MAX_CHOICE_K = 8, 16384          # rows and inputs of `choice_linear_int8`
 _I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
 
@@ -155,6 +156,8 @@ class Int8Weight:
 def _finish_ref(y: torch.Tensor, residual: Optional[torch.Tensor], mode: int, dtype: torch.dtype) -> torch.Tensor:
     if mode == SWIGLU:
         y = F.silu(y[..., 0::2]) * y[..., 1::2]
+    elif mode == RELU2:
+        y = F.relu(y).square()
     elif mode == RESIDUAL:
         y = y + residual.view(y.shape).float()
     return y.to(dtype)
@@ -187,7 +190,7 @@ def linear_int8(x: torch.Tensor, w: Int8Weight, *, norm_w: Optional[torch.Tensor
     """`kernels.linear` with 8-bit weights: [M, N] (SWIGLU: [M, N / 2]) in x's type, or fp32, from x [..., K] (bf16, fp16 or fp32), any M >= 0 and any N.
 
     The rows of x, normed first where norm_w is given, become int8 values and a scale each (`quantize_rows`), and y[m, n] = s_m s_n Σ q_mk q_nk.  mode: PLAIN; RESIDUAL adds
-    `residual` (of the result's type and size; `out` may be it); SWIGLU gives silu(y[2j]) · y[2j + 1] of interleaved rows.  `resident`: w is a parameter that no kernel
+    `residual` (of the result's type and size; `out` may be it); SWIGLU gives silu(y[2j]) · y[2j + 1] of interleaved rows; RELU2 relu(y)².  `resident`: w is a parameter that no kernel
     directly before the call writes; it may then be read ahead of those."""
     who = "linear_int8"
     if w.__class__ is not Int8Weight or w.experts:
@@ -206,7 +209,7 @@ def linear_int8(x: torch.Tensor, w: Int8Weight, *, norm_w: Optional[torch.Tensor
             raise ValueError(f"{who}: residual is {out.dtype} with {M} x {n} elements, contiguous, on {x.device} (got {residual.dtype}, {tuple(residual.shape)}, {residual.device})")
         if residual.data_ptr() != out.data_ptr() and not _apart(residual, n, M, n, out):
             raise ValueError(f"{who}: out overlaps a residual that it is not")
-    elif mode != PLAIN and mode != SWIGLU:
+    elif mode not in (PLAIN, SWIGLU, RELU2):
         raise ValueError(f"{who}: mode {mode} without a residual")
     if dev < 0:
         q, s = _rows_ref(_norm_ref(x, norm_w, eps))
@@ -258,11 +261,11 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
 
     Row t of the result, offsets[e] <= t < offsets[e + 1] (int32 [E + 1], rising, on the device), is expert e's product with row rows[t] of x [M, K] (int32 [T]; an index
     that x does not have is a row of zeros), without `rows` with row t (T = M): [T, N] (SWIGLU: [T, N / 2]) in x's type, or fp32.  Rows in front of offsets[0] and from
-    offsets[E] on are left as they were.  `expert_order` gives rows and offsets of a router's choice.  Scales, sums and modes (PLAIN, SWIGLU) as in `linear_int8`."""
+    offsets[E] on are left as they were.  `expert_order` gives rows and offsets of a router's choice.  Scales, sums and modes (PLAIN, SWIGLU, RELU2) as in `linear_int8`."""
     who = "expert_linear_int8"
     if w.__class__ is not Int8Weight or not 1 <= w.experts <= MAX_EXPERTS:
         raise ValueError(f"{who}: w is an Int8Weight of 1 to {MAX_EXPERTS} experts")
-    if mode not in (PLAIN, SWIGLU):
+    if mode not in (PLAIN, SWIGLU, RELU2):
         raise ValueError(f"{who}: mode {mode}")
     dev, k = x.get_device(), w.k
     x, M, pitch = _take(who, x, k)
@@ -310,7 +313,7 @@ def choice_linear_int8(x: torch.Tensor, w: Int8Weight, choice: torch.Tensor, *, 
     who = "choice_linear_int8"
     if w.__class__ is not Int8Weight or not 1 <= w.experts <= MAX_EXPERTS:
         raise ValueError(f"{who}: w is an Int8Weight of 1 to {MAX_EXPERTS} experts")
-    if mode not in (PLAIN, SWIGLU):
+    if mode not in (PLAIN, SWIGLU, RELU2):
         raise ValueError(f"{who}: mode {mode}")
     dev, k = x.get_device(), w.k
     x, M, pitch = _take(who, x, k)

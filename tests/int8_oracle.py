@@ -58,3 +58,10 @@ def bound_gated(y, dtype, extra=None):
     # that is lost
     off = es * u.abs() + silu.abs() * eu + es * eu + 1.1 * U * r.abs() + 2.0 ** -126 * (g * u).abs()
     return off + half_step(dtype) * (r.abs() + off) + smallest(dtype), r
+
+
+def bound_relu2(y, dtype):
+    """relu(y)^2: y is off by three roundings, its square by twice that (and the square of it) and a rounding of its own."""
+    r = y.clamp(min=0)
+    off = (2 * 3.1 + 0.01 + 1.1) * U * r * r + smallest(torch.float32)
+    return off + half_step(dtype) * (r * r + off) + smallest(dtype), r * r

@@ -539,6 +539,24 @@ def test_every_kernel_gives_a_row_the_same_bits(N, K, dtype):
             assert torch.equal(I.expert_linear_int8(x[:M], e, off, mode=mode), full[:M])
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("M,N,K", [(1, 33, 64), (3, 2048, 512), (20, 130, 1001), (100, 4096, 2048), (300, 6144, 2080), (700, 514, 640), (9, 1, 8)])
+def test_squared_relu(M, N, K, dtype):
+    I, K_ = _ops()
+    x, w = _randn(M, K, seed=M, dtype=dtype), _weight(N, K, seed=N)
+    y = O.products(*O.rows(x), w.values, w.scales)
+    off, want = O.bound_relu2(y, dtype)
+    got = I.linear_int8(x, w, mode=I.RELU2)
+    _check(got, off, want)
+    assert torch.equal(K_.linear(x, w, mode=I.RELU2), got)
+    e = I.Int8Weight(w.values[None], w.scales[None])
+    assert torch.equal(I.expert_linear_int8(x, e, torch.tensor([0, M], dtype=torch.int32, device=DEV), mode=I.RELU2), got)
+    assert torch.equal(I.choice_linear_int8(x[:1], e, torch.zeros(1, 3, dtype=torch.int32, device=DEV), mode=I.RELU2), got[:1].expand(3, -1))
+    x[M // 2, K // 2] = float("nan")
+    got = I.linear_int8(x, w, mode=I.RELU2)
+    assert bool(got[M // 2].isnan().all()) and int(got.isnan().sum()) == N
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("N,K", [(200, 2500), (1000, 2056), (2100, 4100), (4096, 2048), (6200, 2064), (4500, 6400), (16380, 2080), (130, 70)])
 def test_however_a_product_is_cut(N, K, dtype):

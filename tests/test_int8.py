@@ -116,6 +116,16 @@ def test_a_layer_of_experts_together():
             assert torch.equal(got[m, c], I.linear_int8(I.linear_int8(x[m:m + 1], one[0], mode=K.SWIGLU), one[1])[0])
 
 
+def test_squared_relu():
+    w, x = _weight(7, 32), _randn(5, 32)
+    y = I.linear_int8(x, w)
+    assert torch.equal(I.linear_int8(x, w, mode=I.RELU2), y.clamp(min=0).square())
+    e = I.Int8Weight(w.values[None], w.scales[None])
+    assert torch.equal(I.expert_linear_int8(x, e, torch.tensor([0, 5], dtype=torch.int32), mode=I.RELU2), y.clamp(min=0).square())
+    with pytest.raises(ValueError):
+        I.linear_int8(x, w, mode=4)
+
+
 def test_choices_without_an_order():
     w, x = _weight(3, 6, 16), _randn(2, 16)
     choice = torch.tensor([[2, 0], [-1, 1]], dtype=torch.int32)
