@@ -3,7 +3,7 @@
 // Both are what 64 bits would give: s is one rounded quotient, and q is decided exactly (int8.cuh).  A row of zeros has s = 0, a row that holds an infinity or a NaN s = NaN, both
 // with q = 0: what such a row is multiplied with gives zeros or NaN.  With gains the row is normed first (RMS, fp32, no rounding in between).
 //
-// One pass over memory: a row's 16-byte pieces stay in registers between its maximum and its values, 2 to 16 a thread; a row has a warp, 128 or 256 threads.  Rows longer than
+// One pass over memory: a row's 16-byte pieces stay in registers between its maximum and its values, 2 to 16 a thread; a row has 8 threads, a warp, 128 or 256 threads.  Rows longer than
 // registers hold are read twice, an element a thread.  Rows off the 16-byte boundary are taken in pieces of the boundary all the same (the two at the ends element by
 // element); a warp then turns its values to the boundary of the result with its neighbours' bytes.
 // Bound by memory: one B200, us, 8192 x 14336 bf16 51.7 (6.8 TB/s), 32768 x 2048 29.0 (6.9), 65536 x 512 16.8 (6.0), 2048 x 4096 fp32 7.8 (5.4); off the boundary 4097 x 1001 bf16 5.7.
@@ -30,6 +30,11 @@ struct Int8Rows {
 // G threads' maximum or sum
 template <int G>
 __device__ __forceinline__ uint32_t i8r_max(uint32_t v, uint32_t* red) {
+  if constexpr (G < 32) {
+#pragma unroll
+    for (int o = G / 2; o > 0; o /= 2) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  }
   v = __reduce_max_sync(0xffffffffu, v);
   if constexpr (G == 32) return v;
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
@@ -40,6 +45,11 @@ __device__ __forceinline__ uint32_t i8r_max(uint32_t v, uint32_t* red) {
 }
 template <int G>
 __device__ __forceinline__ float i8r_sum(float v, float* red) {
+  if constexpr (G < 32) {
+#pragma unroll
+    for (int o = G / 2; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
   v = warp_sum(v);
   if constexpr (G == 32) return v;
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
@@ -60,7 +70,9 @@ __global__ void __launch_bounds__(i8r_threads(G)) int8_rows_kernel(const Int8Row
   pdl_wait();
   if (p.early == 1) pdl_launch_dependents();
   constexpr int VE = 16 / sizeof(T);
-  const int t = threadIdx.x % G, row = blockIdx.x * (i8r_threads(G) / G) + threadIdx.x / G, lane = threadIdx.x & 31;
+  const int t = threadIdx.x % G, lane = threadIdx.x & 31;
+  int row = blockIdx.x * (i8r_threads(G) / G) + threadIdx.x / G;
+  if (G < 32) row = min(row, p.n - 1);                           // (a warp has several rows and stays whole: the last one may be done twice)
   if (row >= p.n) return;                                        // (whole groups)
   const T* gain = reinterpret_cast<const T*>(p.gain);
   // first element of the row, or nullptr for a row of zeros: one that is not there
@@ -210,7 +222,8 @@ static int rows_launch(const Int8Rows& p, cudaStream_t stream) {
   // 8192 x 2048 13.6 | 7.6; 2000 x 4096 5.7 | 6.1)
   const bool few = p.n <= 4 * SMS;
   cudaError_t e;
-  if (whole && pieces <= 2 * 32) e = rows_go<T, 32, 2, NORM>(p, stream);
+  if (whole && !few && pieces <= 2 * 8) e = rows_go<T, 8, 2, NORM>(p, stream);
+  else if (whole && pieces <= 2 * 32) e = rows_go<T, 32, 2, NORM>(p, stream);
   else if (whole && few && pieces <= 2 * 256) e = rows_go<T, 256, 2, NORM>(p, stream);
   else if (whole && few && pieces <= 8 * 256) e = rows_go<T, 256, 8, NORM>(p, stream);
   else if (whole && pieces <= 8 * 32) e = rows_go<T, 32, 8, NORM>(p, stream);
