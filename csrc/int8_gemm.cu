@@ -312,8 +312,10 @@ static int i8s_slots(int num_sms) { return 2 * num_sms - 32; }
 // 14336 20.5 -> 18.0; 128 x 8192 x 2048 12.0 -> 10.2; 100 x 1024 x 1024 7.6 -> 6.3; 200 x 2048 x 8192 15.4 -> 13.3; 256 x 4096 x 4096 14.5 -> 13.5; 256 x 1024 x 4096 12.3 -> 9.7;
 // 256 x 6144 x 4096 16.8 -> 15.2; 512 x 1024 x 4096 14.2 -> 11.8.  One piece stays better for a long K: 256 x 4096 x 14336 23.1 and 25.6, 160 x 4096 x 4096 11.2 and 11.7; and two CTAs an SM
 // up to 80 rows over many features: 72 x 6144 x 4096 10.9 and 11.4.
-// Pairs otherwise (us here | there: 130 x 4096 x 4096 10.7 | 16.3; 512 x 4096 x 4096 17.2 | 18.3; 400 x 2048 x 2048 11.0 | 11.5; 333 x 6144 x 4096 in three pieces 16.9 | 18.4; 200 x 1024 x
-// 1024 9.3 | 6.9; 333 x 1000 x 960 9.0 | 7.3; K in one part: 256 x 28672 x 4096 45 | 32, 512 x 6144 x 4096 19.4 | 18.8).
+// Beyond 256 rows pieces of 128 as long as each can have an SM, whatever their number (us here | in pairs: 600 x 1024 x 4096 13.4 | 17.4; 1024 x 2048 x 4096 18.8 | 21.4; 4096 x 128 x
+// 8192 24.3 | 38.7; 333 x 6144 x 4096 16.4 | 18.9; 500 x 4608 x 4096 17.7 | 18.7; 8192 x 128 x 2048 16.0 | 17.4).
+// Pairs otherwise (130 x 4096 x 4096 10.7 | 16.3; 512 x 4096 x 4096 17.2 | 18.3; K short: 200 x 1024 x 1024 9.3 | 6.9; 333 x 1000 x 960 9.0 | 7.3; many tiles: 256 x 28672 x 4096
+// 45 | 32, 512 x 6144 x 4096 19.4 | 18.8).
 struct Int8Cut { int pieces, parts, wide; };
 static Int8Cut i8s_cut(int M, int N, int K, int num_sms) {
   const int cols = (N + I8S_BM - 1) / I8S_BM, kb = (K + I8S_BK - 1) / I8S_BK, both = i8s_slots(num_sms), one = num_sms - 20;
@@ -327,7 +329,9 @@ static Int8Cut i8s_cut(int M, int N, int K, int num_sms) {
     if (cols <= one / 2 && (M > 80 || cols <= one / 3)) return {1, i8s_parts(cols, kb, cols <= one / 6 ? 6 : 4, one), 1};
     return {1, i8s_parts(cols, kb, I8S_PARTS, both), 0};
   }
-  if (M > 512 || kb < 16) return {0, 0, 0};
+  if (kb < 16) return {0, 0, 0};
+  const long long tiles = (long long)cols * ((M + 127) / 128);      // of 128 x 128
+  if (M > 512) return tiles <= num_sms ? Int8Cut{(M + 127) / 128, i8s_parts(tiles, kb, 4, one), 1} : Int8Cut{0, 0, 0};
   if (few) {
     const int c = (M + 111) / 112 < 4 ? (M + 111) / 112 : 4;
     return {c, i8s_parts((long long)cols * c, kb, 6, one), 1};
@@ -335,8 +339,7 @@ static Int8Cut i8s_cut(int M, int N, int K, int num_sms) {
   if (M > 256) {
     const int ks = i8s_parts(2ll * cols, kb, 4, one);
     if (ks > 1) return {2, ks, 1};
-    if (M <= 384 && 3ll * cols > one && 3ll * cols <= num_sms) return {3, 1, 1};
-    return {0, 0, 0};
+    return tiles <= num_sms ? Int8Cut{(M + 127) / 128, 1, 1} : Int8Cut{0, 0, 0};
   }
   if (cols <= one / 6 || (kb <= 48 && M > 176)) {
     const int ks = i8s_parts(2ll * cols, kb, 4, one);

@@ -53,6 +53,27 @@ def test_rows(dtype, M, K):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("M,K", [(593, 8), (1001, 64), (2003, 128), (700, 16), (601, 104), (5000, 24), (602, 40)])
+def test_many_short_rows(dtype, M, K):
+    I, _ = _ops()
+    x = _randn(M, K, seed=K, dtype=dtype, scale=3.0)
+    x[5], x[77, K // 2], x[78, 0], x[-1, -1] = 0, float("nan"), float("-inf"), float("inf")
+    x[6] *= 1e-30 if dtype is not HF else 1e-6
+    q, s = I.quantize_rows(x)
+    fine = torch.isfinite(x).all(1)
+    _same_rows((q[fine], s[fine]), x[fine])
+    assert not q[~fine].any() and bool(s[~fine].isnan().all())
+    g = _randn(K, seed=1, dtype=dtype)
+    a, b = I.quantize_rows(x[fine], norm_w=g)
+    xd = x[fine].double()
+    h = xd / (xd.pow(2).mean(-1, keepdim=True) + 1e-5).sqrt() * g.double()
+    amax = h.abs().amax(-1, keepdim=True)
+    t = torch.where(amax > 0, 127.0 * h / amax, torch.zeros_like(h))
+    near = (t - t.floor() - 0.5).abs() < 127.0 * 8 * O.U
+    assert bool(((a.double() - t.round()).abs() <= near).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
 @pytest.mark.parametrize("K", [64, 333, 4096])
 def test_rows_on_the_middle_of_two_values(dtype, K):
     """Quotients on and next to k + 1/2: amax 127 and 254, elements on halves and one step of the type beside them."""
@@ -569,6 +590,43 @@ def test_however_a_product_is_cut(N, K, dtype):
     for M in (1, 2, 7, 16, 48, 64, 65, 80, 81, 97, 112, 128, 129, 144, 176, 177, 225, 256, 257, 336, 337, 384, 385, 449, 512):
         assert torch.equal(I.linear_int8(x[:M], w), plain[:M])
         assert torch.equal(I.linear_int8(x[:M], w, mode=K_.RESIDUAL, residual=r[:M]), more[:M])
+
+
+@pytest.mark.parametrize("N,K", [(100, 4096), (163, 11374), (1000, 2056), (2048, 2048), (4608, 2100)])
+def test_many_rows_of_few_features(N, K):
+    I, K_ = _ops()
+    x, w, r = _randn(1500, K, seed=3, dtype=BF), _weight(N, K), _randn(1500, N, seed=4, dtype=BF)
+    off, want = O.bound(O.products(*O.rows(x), w.values, w.scales), BF, residual=r)
+    for M in (513, 700, 1500):
+        got = I.linear_int8(x[:M], w, mode=K_.RESIDUAL, residual=r[:M])
+        _check(got, off[:M], want[:M])
+        assert torch.equal(got, torch.cat([I.linear_int8(x[i:min(i + 60, M)], w, mode=K_.RESIDUAL, residual=r[i:min(i + 60, M)]) for i in range(0, M, 60)]))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("M,N,K", [(700, 1001, 200), (1030, 2502, 72), (601, 1034, 1000), (300, 35, 256), (1000, 4, 64), (530, 259, 130)])
+def test_results_off_the_boundary(M, N, K, dtype):
+    """Rows of results and residuals that begin anywhere: odd ones, and those on four bytes."""
+    I, K_ = _ops()
+    x, w, r = _randn(M, K, seed=3, dtype=dtype), _weight(N, K), _randn(M, N, seed=4, dtype=dtype)
+    y = O.products(*O.rows(x), w.values, w.scales)
+    room = torch.full((M * N + 9,), 3.0, dtype=dtype, device=DEV)
+    for shift in (1, 2):
+        out = room[shift:shift + M * N].view(M, N)
+        off, want = O.bound(y, dtype, residual=r)
+        I.linear_int8(x, w, mode=K_.RESIDUAL, residual=r, out=out)
+        _check(out, off, want)
+        out.copy_(r)
+        I.linear_int8(x, w, mode=K_.RESIDUAL, residual=out, out=out)                  # in place
+        _check(out, off, want)
+        off, want = O.bound(y, dtype)
+        I.linear_int8(x, w, out=out)
+        _check(out, off, want)
+        assert bool((room[:shift] == 3).all()) and bool((room[shift + M * N:] == 3).all())
+        room.fill_(3.0)
+    if N % 2 == 0:
+        off, want = O.bound_gated(y, dtype)
+        _check(I.linear_int8(x, w, mode=K_.SWIGLU), off, want)
 
 
 @pytest.mark.parametrize("counts,N", [([600, 700, 500], 1024), ([900, 0, 1100], 2050)])
