@@ -6,7 +6,8 @@
 // One pass over memory: a row's 16-byte pieces stay in registers between its maximum and its values, 2 to 16 a thread; a row has 8 threads, a warp, 128 or 256 threads.  Rows longer than
 // registers hold are read twice, an element a thread.  Rows off the 16-byte boundary are taken in pieces of the boundary all the same (the two at the ends element by
 // element); a warp then turns its values to the boundary of the result with its neighbours' bytes.
-// Bound by memory: one B200, us, 8192 x 14336 bf16 51.7 (6.8 TB/s), 32768 x 2048 29.0 (6.9), 65536 x 512 16.8 (6.0), 2048 x 4096 fp32 7.8 (5.4); off the boundary 4097 x 1001 bf16 5.7.
+// Bound by memory: one B200, us, 8192 x 14336 bf16 51.7 (6.8 TB/s), 32768 x 2048 29.0 (6.9), 65536 x 512 16.8 (6.0), 2048 x 4096 fp32 7.8 (5.4); with many short rows 65536 x 128 5.6
+// (4.5; a warp a row 13.7); off the boundary about twice the time: 4097 x 1001 bf16 5.7, 6753 x 11331 66, 61737 x 45 8.8 (a warp a row 28).
 // Maxima are taken on the bits without their sign, as whole numbers: the order is that of the magnitudes, with infinities and NaN above all of them.
 #include "int8.cuh"
 #include "jllama_b200.h"
@@ -147,15 +148,16 @@ __global__ void __launch_bounds__(i8r_threads(G)) int8_rows_kernel(const Int8Row
       int8_t* q = p.q + (size_t)row * p.ldq;
       for (int i = p.K + t; i < p.ldq; i += G) q[i] = 0;
       if (t == 0) p.s[row] = quotient.scale();
-      if (!quotient.ordinary()) {                                // zeros, tiny numbers, no numbers: element by element, again from memory
+      const bool ordinary = quotient.ordinary();
+      if (!ordinary) {                                           // zeros, tiny numbers, no numbers: element by element, again from memory
 #pragma unroll 1
         for (int i = t; i < p.K; i += G) q[i] = (int8_t)(quotient(x == nullptr ? 0.0f : element(to_f(x[i]), NORM ? to_f(gain[i]) : 0.0f)) & 0xffu);
-        return;
+        if (!(EDGE && G < 32)) return;                           // (a warp's rows turn their values together)
       }
       const Int8Pairs pairs(amax);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        if ((EDGE ? t - lane : t) + v * G >= pieces) break;        // (EDGE: whole warps)
+        if (EDGE && G < 32 ? v * G >= (p.K + 2 * VE - 2) / VE : (EDGE ? t - lane : t) + v * G >= pieces) break;        // (EDGE: whole warps)
         float f[VE], g[VE] = {};
         i8r_unpack<T>(w[v], f);
         gains(v, g);
@@ -173,10 +175,11 @@ __global__ void __launch_bounds__(i8r_threads(G)) int8_rows_kernel(const Int8Row
           // the word of the result that holds this piece's first byte: `turn_by` bytes of the piece before it, then this one's.  Whole words are stored by the lane whose
           // piece begins in them, the bytes of others one by one.
           const int turn_by = (int)((uintptr_t)(q + c) % VE);
-          const Word before = __shfl_up_sync(0xffffffffu, mine, 1);
-          const bool there = t + v * G < pieces;
-          const bool full = there && (lane > 0 || turn_by == 0) && c - turn_by >= 0 && c - turn_by + VE <= p.K;
-          const bool next = __shfl_down_sync(0xffffffffu, full, 1) && lane < 31;
+          constexpr int W = G < 32 ? G : 32;
+          const Word before = __shfl_up_sync(0xffffffffu, mine, 1, W);
+          const bool there = t + v * G < pieces && (G >= 32 || ordinary);
+          const bool full = there && (lane % W > 0 || turn_by == 0) && c - turn_by >= 0 && c - turn_by + VE <= p.K;
+          const bool next = __shfl_down_sync(0xffffffffu, full, 1, W) && lane % W < W - 1;
           if (full) *reinterpret_cast<Word*>(q + c - turn_by) = turn_by == 0 ? mine : (Word)(mine << (8 * turn_by)) | (Word)(before >> (8 * (VE - turn_by)));
           if (there && (!full || (!next && turn_by > 0))) {
 #pragma unroll
@@ -212,6 +215,13 @@ static cudaError_t rows_go(const Int8Rows& p, cudaStream_t stream) {
   return launch_pdl(int8_rows_kernel<T, G, NV, NORM, EDGE>, dim3((unsigned)((p.n + PER - 1) / PER)), dim3(i8r_threads(G)), 0, stream, p);
 }
 
+// off the boundary, sixteen pieces a thread (with gains as well that is more than registers hold: not called).  us, before -> so: 32768 x 2047 79 -> 65, 1431 x 26683 81 -> 37
+template <typename T, int G, bool NORM>
+static cudaError_t rows_edge(const Int8Rows& p, cudaStream_t stream) {
+  if constexpr (NORM) return cudaErrorInvalidValue;
+  else return rows_go<T, G, 16, false, true>(p, stream);
+}
+
 template <typename T, bool NORM>
 static int rows_launch(const Int8Rows& p, cudaStream_t stream) {
   constexpr int VE = 16 / sizeof(T);
@@ -231,11 +241,14 @@ static int rows_launch(const Int8Rows& p, cudaStream_t stream) {
   else if (whole && pieces <= 8 * 128) e = rows_go<T, 128, 8, NORM>(p, stream);
   else if (whole && pieces <= 16 * 128) e = rows_go<T, 128, 16, NORM>(p, stream);
   else if (whole && pieces <= 16 * 256) e = rows_go<T, 256, 16, NORM>(p, stream);
+  else if (!few && spread <= 2 * 8) e = rows_go<T, 8, 2, NORM, true>(p, stream);
   else if (spread <= 2 * 32) e = rows_go<T, 32, 2, NORM, true>(p, stream);
   else if (few && spread <= 2 * 256) e = rows_go<T, 256, 2, NORM, true>(p, stream);
   else if (spread <= 8 * 32) e = rows_go<T, 32, 8, NORM, true>(p, stream);
+  else if (!NORM && !few && spread <= 16 * 32) e = rows_edge<T, 32, NORM>(p, stream);
   else if (spread <= 8 * 128) e = rows_go<T, 128, 8, NORM, true>(p, stream);
   else if (spread <= 16 * 128) e = rows_go<T, 128, 16, NORM, true>(p, stream);
+  else if (!NORM && spread <= 16 * 256) e = rows_edge<T, 256, NORM>(p, stream);
   else e = rows_go<T, 256, 0, NORM>(p, stream);
   JL_CUDA(e);
   return JL_OK;
