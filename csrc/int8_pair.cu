@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t i8p_pack(float a, float b) {
 }
 
 // `rows` rows of up to 128 bytes, `cols` elements of them, between a warp's buffer (chunks of 16 bytes turned by the row) and rows of memory on any boundary: neighbouring lanes
-// have neighbouring words.  (A row a lane, element by element: 6975 x 26652 x 72 gated 196 us, 2924 x 11962 x 112 + residual 152.)
+// have neighbouring words.  (2924 x 11962 x 112 + residual 71 us; a row a lane, element by element, 152.)
 template <typename Word, bool OUT, typename T>
 __device__ __forceinline__ void i8p_words(uint8_t* buffer, T* memory, int pitch, int rows, int cols, int lane) {
   constexpr int FLY = OUT ? 8 : 32;                                                   // rows under way at once
