@@ -221,9 +221,10 @@ def linear_int8(x: torch.Tensor, w: Int8Weight, *, norm_w: Optional[torch.Tensor
         held, sms = w._held
         L = _lib.lib()
         need = L.jl_linear_int8_scratch_bytes(M, n, k)
-        scratch = x.new_empty(need, dtype=torch.uint8).data_ptr() if need else 0
+        # (held until both launches are issued: another thread of this stream would be given what is let go of here, and the library runs without the interpreter's lock)
+        room = x.new_empty(need, dtype=torch.uint8) if need else None
         rc = L.jl_linear_int8(x.data_ptr(), TYPES[x.dtype], M, k, pitch, *held, 0 if norm_w is None else norm_w.data_ptr(), eps, 0 if residual is None else residual.data_ptr(),
-                              out.data_ptr(), TYPES[out.dtype], mode, scratch, need, resident, sms, _stream())
+                              out.data_ptr(), TYPES[out.dtype], mode, 0 if room is None else room.data_ptr(), need, resident, sms, _stream())
         if rc:
             _lib.check(rc, "jl_linear_int8")
     return out
@@ -299,9 +300,9 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
         held, sms = w._held
         L = _lib.lib()
         need = L.jl_experts_int8_scratch_bytes(T, w.n, k)
-        scratch = x.new_empty(need, dtype=torch.uint8).data_ptr() if need else 0
+        room = x.new_empty(need, dtype=torch.uint8) if need else None                # (held, as in linear_int8)
         rc = L.jl_experts_int8(x.data_ptr(), TYPES[x.dtype], M, k, pitch, 0 if rows is None else rows.data_ptr(), T, offsets.data_ptr(), w.experts, *held, out.data_ptr(),
-                               TYPES[out.dtype], mode, scratch, need, sms, _stream())
+                               TYPES[out.dtype], mode, 0 if room is None else room.data_ptr(), need, sms, _stream())
         if rc:
             _lib.check(rc, "jl_experts_int8")
     return out

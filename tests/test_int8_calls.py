@@ -1,0 +1,81 @@
+"""How the functions of 8-bit layers call the library: on the CPU, with a stand-in for its entry points."""
+import weakref
+
+import pytest
+import torch
+
+from jax_llama_b200.ops import int8 as I
+
+
+class OnGpu(torch.Tensor):
+    """A tensor of the CPU that says it is on cuda:0, and remembers the workspaces that were made from it."""
+
+    made = []
+
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+    def new_empty(self, *args, **kw):
+        t = super().new_empty(*args, **kw)
+        if t.dtype is torch.uint8:
+            OnGpu.made.append(weakref.ref(t))
+        return t
+
+
+class Library:
+    """Entry points that look at their arguments and launch nothing."""
+
+    def __init__(self):
+        self.calls = []
+
+    def jl_linear_int8_scratch_bytes(self, M, N, K):
+        return 1024
+
+    def jl_experts_int8_scratch_bytes(self, T, N, K):
+        return 2048
+
+    def _called(self, name, args):
+        held = [t() for t in OnGpu.made]
+        assert len(held) == 1 and held[0] is not None, f"{name}: its workspace is gone"
+        assert held[0].data_ptr() in args and held[0].numel() in args
+        self.calls.append((name, args))
+        return 0
+
+    def jl_linear_int8(self, *args):
+        return self._called("linear", args)
+
+    def jl_experts_int8(self, *args):
+        return self._called("experts", args)
+
+
+@pytest.fixture
+def library(monkeypatch):
+    lib = Library()
+    OnGpu.made = []
+    monkeypatch.setattr(I._lib, "lib", lambda: lib)
+    monkeypatch.setattr(I, "_here", lambda dev, who: None)
+    monkeypatch.setattr(I, "_stream", lambda: 0)
+    return lib
+
+
+def on_gpu(t):
+    return t.as_subclass(OnGpu)
+
+
+def weight(*shape):
+    w = I.Int8Weight(torch.ones(shape, dtype=torch.int8), torch.ones(shape[:-1]))
+    w.dev = 0
+    return w
+
+
+def test_the_workspace_of_a_layer_lives_until_the_call_is_over(library):
+    I.linear_int8(on_gpu(torch.randn(300, 64)), weight(32, 64))
+    assert [n for n, _ in library.calls] == ["linear"]
+
+
+def test_the_workspace_of_experts_lives_until_the_call_is_over(library):
+    x = on_gpu(torch.randn(30, 64))
+    I.expert_linear_int8(x, weight(2, 32, 64), on_gpu(torch.tensor([0, 10, 30], dtype=torch.int32)))
+    assert [n for n, _ in library.calls] == ["experts"]
