@@ -147,6 +147,24 @@ __device__ __forceinline__ void i8r_piece(const Int8Pairs& pairs, float amax, co
     }
   }
 }
+// The sum of squares of a row that is normed first has one order, whatever kernel takes the row, so that its values and scale do not depend on the rows beside it.  The squares of a
+// 16-byte piece, one that begins at a column that is a multiple of its elements, are added in turn; pieces I8R_PIECES apart are added in rising order; of the I8R_PIECES sums the upper half is added
+// to the lower one, half by half.  A piece that is not there adds a zero and changes nothing.  The upper bits of a piece's number are those of a thread's own pieces (t + v G), then the warp's, then the lane's.
+constexpr int I8R_PIECES = 4096;
+// leaves FIRST, FIRST + STEP, .. below N joined so
+template <int FIRST, int STEP, int N, typename F>
+__device__ __forceinline__ float i8r_join(const F& leaf) {
+  if constexpr (STEP == N) return leaf(std::integral_constant<int, FIRST>{});
+  else return __fadd_rn(i8r_join<FIRST, 2 * STEP, N>(leaf), i8r_join<FIRST + STEP, 2 * STEP, N>(leaf));
+}
+template <int VE>
+__device__ __forceinline__ float i8r_squares(const float (&f)[VE]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) s = fmaf(f[e], f[e], s);
+  return s;
+}
+
 __device__ __forceinline__ uint32_t i8r_pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }

@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
   __shared__ int parts[2][I8V_WARPS][I8V_ROWS][I8V_FEATURES];
   __shared__ float row_scale[I8V_ROWS];
   __shared__ uint32_t red[I8V_WARPS];
-  __shared__ float red_f[I8V_WARPS];
+  __shared__ float red_f[I8V_THREADS];
   int8_t* const xs = reinterpret_cast<int8_t*>(i8v_smem);                                 // [rows][pitch]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int pitch = i8v_pitch(p.K), units = p.units;
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
 
   // ---- the activations' rows in 8 bits: 8 / R' warps a row, R' = 1, 2, 4, 8
   {
-    const int R = p.rows, per = R <= 1 ? 8 : R <= 2 ? 4 : R <= 4 ? 2 : 1;            // warps of a row
+    const int R = EXPERTS ? 1 : p.rows, per = R <= 1 ? 8 : R <= 2 ? 4 : R <= 4 ? 2 : 1;            // warps of a row
     const int row = warp / per, n = per * 32, i0 = threadIdx.x - row * n;
     const bool there = row < R;
     const T* x = source + (there ? (long long)row * p.ldx : 0);
@@ -124,11 +124,7 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
     T* const raw = reinterpret_cast<T*>(i8v_smem + (size_t)R * pitch) + (size_t)row * ((p.K + VE - 1) / VE * VE);
     const bool whole = p.K % VE == 0 && (p.ldx * (long long)sizeof(T)) % 16 == 0 && (((uintptr_t)p.x | (uintptr_t)p.gain) & 15) == 0;
     uint32_t m = 0;
-    float sum = 0.0f, norm = 1.0f;
-    auto see = [&](float f) {
-      m = max(m, i8r_bits(f));
-      sum = fmaf(f, f, sum);
-    };
+    float norm = 1.0f;
     if (there && whole) {
       for (int i = i0 * VE; i < p.K; i += 4 * n * VE) {
         uint4 v[4];
@@ -141,31 +137,48 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
           float f[VE];
           i8r_unpack<T>(v[u], f);
 #pragma unroll
-          for (int e = 0; e < VE; ++e) see(f[e]);
+          for (int e = 0; e < VE; ++e) m = max(m, i8r_bits(f[e]));
         }
       }
     } else if (there) {
       // element by element; a thread's places are those of its pieces
       for (int i = i0 * VE; i < p.K; i += n * VE)
-        for (int e = 0; e < VE && i + e < p.K; ++e) { raw[i + e] = real ? x[i + e] : T(0.0f); see(to_f(raw[i + e])); }
+        for (int e = 0; e < VE && i + e < p.K; ++e) { raw[i + e] = real ? x[i + e] : T(0.0f); m = max(m, i8r_bits(to_f(raw[i + e]))); }
     }
-    if (gain != nullptr) {
-      sum = warp_sum(sum);
-      if (lane == 0) red_f[warp] = sum;
-      __syncthreads();
-      sum = 0.0f;
-      for (int i = 0; i < per; ++i) sum += red_f[row * per + i];
-      norm = 1.0f / sqrtf(sum / (float)p.K + p.eps);
-    }
-    // the piece at i, normed; columns behind K are zeros
-    auto piece = [&](int i, float (&f)[VE]) {
+    // the piece at i; columns behind K are zeros
+    auto held = [&](int i, float (&f)[VE]) {
       if (whole) {
         i8r_unpack<T>(*reinterpret_cast<const uint4*>(raw + i), f);
       } else {
 #pragma unroll
         for (int e = 0; e < VE; ++e) f[e] = i + e < p.K ? to_f(raw[i + e]) : 0.0f;
       }
-      if (gain == nullptr) return;
+    };
+    if (!EXPERTS && gain != nullptr) {
+      // the sum of squares in the order of i8r_join: a thread has at most 16 pieces (I8V_FUSED), four times four; the first and third four meet, the second and fourth
+      float first[4] = {}, second[4] = {};
+      bool odd = false;
+      for (int i = i0 * VE; there && i < p.K; i += 4 * n * VE, odd = !odd) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (i + u * n * VE >= p.K) break;
+          float f[VE];
+          held(i + u * n * VE, f);
+          const float s = i8r_squares(f);
+          first[u] = __fadd_rn(first[u], odd ? 0.0f : s);
+          second[u] = __fadd_rn(second[u], odd ? s : 0.0f);
+        }
+      }
+      red_f[threadIdx.x] = __fadd_rn(__fadd_rn(__fadd_rn(first[0], second[0]), __fadd_rn(first[2], second[2])), __fadd_rn(__fadd_rn(first[1], second[1]), __fadd_rn(first[3], second[3])));
+      __syncthreads();
+      const float* mine = red_f + row * n + lane;
+      const float sum = warp_sum(i8r_join<0, 1, I8V_WARPS>([&](auto w) { return decltype(w)::value < per ? mine[32 * decltype(w)::value] : 0.0f; }));
+      norm = 1.0f / sqrtf(sum / (float)p.K + p.eps);
+    }
+    // .. normed
+    auto piece = [&](int i, float (&f)[VE]) {
+      held(i, f);
+      if (EXPERTS || gain == nullptr) return;
       float w[VE];
       if (whole) {
         i8r_unpack<T>(*reinterpret_cast<const uint4*>(gain + i), w);
@@ -176,7 +189,7 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
 #pragma unroll
       for (int e = 0; e < VE; ++e) f[e] = f[e] * norm * w[e];
     };
-    if (gain != nullptr) {
+    if (!EXPERTS && gain != nullptr) {
       m = 0;
       if (there) {
         for (int i = i0 * VE; i < p.K; i += n * VE) {
@@ -208,7 +221,7 @@ __global__ void __launch_bounds__(I8V_THREADS, 2) int8_vec_kernel(const Int8Vec 
           for (int e = 0; e < VE; ++e) q[i + e] = (int8_t)(quotient(f[e]) & 0xffu);
           continue;
         }
-        if (gain == nullptr) i8r_piece<T, true>(pairs, amax, f, b);
+        if (EXPERTS || gain == nullptr) i8r_piece<T, true>(pairs, amax, f, b);
         else i8r_piece<T, false>(pairs, amax, f, b);
         if constexpr (VE == 8) *reinterpret_cast<uint2*>(q + i) = make_uint2(i8r_pack4(b[0], b[1], b[2], b[3]), i8r_pack4(b[4], b[5], b[6], b[7]));
         else *reinterpret_cast<uint32_t*>(q + i) = i8r_pack4(b[0], b[1], b[2], b[3]);
