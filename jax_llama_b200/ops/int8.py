@@ -286,7 +286,7 @@ def expert_linear_int8(x: torch.Tensor, w: Int8Weight, offsets: torch.Tensor, *,
             there = ((rows >= 0) & (rows < M))
             at = rows.long().clamp(0, max(M - 1, 0))
             q = q[at] * there[:, None] if M else q.new_zeros((T, w.k))
-            s = s[at] * there if M else s.new_zeros(T)
+            s = s[at].masked_fill(~there, 0.0) if M else s.new_zeros(T)              # (a product would keep the NaN of the row that stands in)
         ends = [min(max(int(v), 0), T) for v in offsets.tolist()]
         for e in range(w.experts):
             a, b = ends[e], ends[e + 1]

@@ -79,3 +79,13 @@ def test_the_workspace_of_experts_lives_until_the_call_is_over(library):
     x = on_gpu(torch.randn(30, 64))
     I.expert_linear_int8(x, weight(2, 32, 64), on_gpu(torch.tensor([0, 10, 30], dtype=torch.int32)))
     assert [n for n, _ in library.calls] == ["experts"]
+
+
+def test_a_row_that_is_not_there_is_zeros_beside_rows_that_are_no_numbers():
+    """An index that x does not have, where the rows that x does have hold NaN or infinities."""
+    w = I.Int8Weight(torch.ones(2, 6, 16, dtype=torch.int8), torch.ones(2, 6))
+    x = torch.full((3, 16), float("nan"))
+    x[1] = 2.0
+    x[2, 5] = float("inf")
+    y = I.expert_linear_int8(x, w, torch.tensor([0, 3, 5], dtype=torch.int32), rows=torch.tensor([-1, 1, 3, 99, 0], dtype=torch.int32))
+    assert not y[[0, 2, 3]].any() and torch.isfinite(y[1]).all() and torch.isnan(y[4]).all()
