@@ -18,6 +18,7 @@ enum { I8_PLAIN = 0, I8_RESIDUAL = 1, I8_GATED = 2, I8_RELU2 = 3 };      // resu
 constexpr int I8_MAX_K = 131072;
 constexpr int I8_MAX_EXPERTS = 1024;
 constexpr int I8_MAX_ROWS = 1 << 30;
+constexpr int I8_MAX_COLUMNS = 1 << 30;      // of rows alone; columns and a block's threads behind them stay whole numbers of 32 bits
 
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }

@@ -335,7 +335,7 @@ using namespace jl;
 extern "C" JL_API int jl_int8_rows(const void* x, int dtype, int M, int K, long long ldx, const int* rows, int n, const void* gain, float eps, void* q, int ldq,
                                    float* s, void* stream) {
   JL_CHECK_ARG(dtype >= DT_BF16 && dtype <= DT_F16, "jl_int8_rows: element type %d", dtype);
-  JL_CHECK_ARG(M >= 0 && n >= 0 && n <= I8_MAX_ROWS && K >= 1 && ldq >= K && (ldx >= K || M <= 1) && (rows != nullptr || n <= M), "jl_int8_rows: %d x %d (pitch %lld) as %d rows of pitch %d", M, K, ldx, n, ldq);
+  JL_CHECK_ARG(M >= 0 && n >= 0 && n <= I8_MAX_ROWS && K >= 1 && K <= I8_MAX_COLUMNS && ldq >= K && ldq <= I8_MAX_COLUMNS + 16 && (ldx >= K || M <= 1) && (rows != nullptr || n <= M), "jl_int8_rows: %d x %d (pitch %lld) as %d rows of pitch %d", M, K, ldx, n, ldq);
   if (n == 0) return JL_OK;
   return int8_rows(x, dtype, M, K, ldx, rows, n, gain, eps, q, ldq, s, 0, (cudaStream_t)stream);
 }

@@ -596,7 +596,7 @@ int jl_logit_rules(const void* logits, int dtype, int B, int V, int ld, float* o
  * give them; a row of zeros has s = 0, one with an infinity or a NaN s = NaN and q = 0.  Element types 0 bf16, 1 fp32, 2 fp16.
  *
  * jl_int8_rows: n rows of x [M, K] (row pitch ldx): row rows[i] (NULL: row i; one that x does not have: zeros), normed first where gain [K] (x's type) is given; q with row
- * pitch ldq, columns behind K zero.
+ * pitch ldq, columns behind K zero; K <= 2^30.
  * jl_linear_int8: out [M, N] (gated: [M, N / 2]) = sx sw (qx qw^T) of the rows of x [M, K] and weights wq [N, ldw] / ws [N]; ldw a multiple of 16, the columns behind K not
  * used.  mode 0 plain, 1 + residual (out's type and size, may be out), 2 silu(y[2j]) y[2j+1], 3 relu(y)^2.  K <= 131072.  resident: no kernel directly before the call writes the weights.
  * jl_experts_int8: out[t], offsets[e] <= t < offsets[e + 1], of row rows[t] of x against expert e's weights wq [experts][N][ldw], ws [experts][N]; offsets [experts + 1] on

@@ -22,6 +22,7 @@ TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 MAX_K = 131072                 # inputs of a layer: 127 * 127 * K stays below 2^31
 MAX_EXPERTS = 1024
 MAX_ROWS = 1 << 30
+MAX_COLUMNS = 1 << 30          # of `quantize_rows`
 RELU2 = 3                      # a mode beside `kernels`' PLAIN, RESIDUAL and SWIGLU: relu(y)²
 MAX_CHOICES, MAX_CHOICE_K = 8, 16384          # rows and inputs of `choice_linear_int8`
 _I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
@@ -73,7 +74,7 @@ def _gain(who: str, norm_w: torch.Tensor, x: torch.Tensor, K: int) -> None:
 def quantize_rows(x: torch.Tensor, *, norm_w: Optional[torch.Tensor] = None, eps: float = 1e-5,
                   out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(values int8 [..., K], scales fp32 [...]) of the rows of x [..., K] (bf16, fp16 or fp32; two dimensions: any row pitch).  Both are what 64 bits would give: the
-    scale is amax / 127 rounded once, a value is the whole number nearest to 127 x / amax.  A row of zeros has scale 0; a row that holds an infinity or a NaN has scale
+    scale is amax / 127 rounded once, a value is the whole number nearest to 127 x / amax.  At most MAX_ROWS rows of MAX_COLUMNS.  A row of zeros has scale 0; a row that holds an infinity or a NaN has scale
     NaN and values 0, so that what it is multiplied with is NaN.  With norm_w the rows are normed first (RMS, fp32, no rounding in between)."""
     who = "quantize_rows"
     if x.dim() < 1:
@@ -81,6 +82,8 @@ def quantize_rows(x: torch.Tensor, *, norm_w: Optional[torch.Tensor] = None, eps
     K = x.shape[-1]
     x2, M, pitch = _take(who, x, K)
     _few(who, M)
+    if K > MAX_COLUMNS:
+        raise ValueError(f"{who}: rows of {K} numbers (at most {MAX_COLUMNS})")
     if norm_w is not None:
         _gain(who, norm_w, x2, K)
     shape = x.shape

@@ -89,3 +89,14 @@ def test_a_row_that_is_not_there_is_zeros_beside_rows_that_are_no_numbers():
     x[2, 5] = float("inf")
     y = I.expert_linear_int8(x, w, torch.tensor([0, 3, 5], dtype=torch.int32), rows=torch.tensor([-1, 1, 3, 99, 0], dtype=torch.int32))
     assert not y[[0, 2, 3]].any() and torch.isfinite(y[1]).all() and torch.isnan(y[4]).all()
+
+
+def test_rows_longer_than_they_may_be(monkeypatch):
+    """A number of columns beyond 32 bits would reach the library cut short."""
+    from jax_llama_b200.ops import _lib
+    assert I.MAX_COLUMNS == 1 << 30
+    monkeypatch.setattr(I, "MAX_COLUMNS", 7)
+    with pytest.raises(ValueError, match="rows of 8 numbers"):
+        I.quantize_rows(torch.zeros(3, 8))
+    K = (1 << 30) + 8                                           # (refused by the library ahead of any use of the device)
+    assert _lib.lib().jl_int8_rows(0, 0, 1, K, K, 0, 1, 0, 1e-5, 0, K, 0, 0) != 0
