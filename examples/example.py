@@ -37,7 +37,11 @@ def load(ckpt_dir: str, tokenizer_path: str, is_llama3: bool, device: str = "aut
             model_kwargs.update(tp=world, rank=rank)
         else:
             params, config = convert_llama_weights(ckpt_dir, tokenizer, max_seq_len=max_seq_len, dtype=torch.bfloat16)
-        params = tree_to(params, device=dev, dtype=torch.bfloat16)
+        if model_kwargs.get("weights", "bf16") == "int8":      # layer by layer to the GPU, which never holds the model in bf16
+            from jax_llama_b200.models.engine import B200Engine
+            params = {"engine": B200Engine.from_tree(config, params, device=dev, **model_kwargs)}
+        else:
+            params = tree_to(params, device=dev, dtype=torch.bfloat16)
     else:
         if world > 1:
             raise SystemExit("multi-process runs need one CUDA device per rank")

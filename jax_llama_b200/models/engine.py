@@ -20,7 +20,7 @@ from __future__ import annotations
 import logging
 import os
 import weakref
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Any, Dict, List, Optional, Tuple
 
 import torch
@@ -80,6 +80,23 @@ class LayerWeights:
     w13: torch.Tensor
     w2: torch.Tensor
 
+    MATRICES = ("wqkv", "wo", "w13", "w2")
+
+    def in_8_bits(self) -> "LayerWeights":
+        """The layer with its matrices in 8 bits (those that are so already are kept); this one stays as it is."""
+        return replace(self, **{n: _in_8_bits(getattr(self, n)) for n in self.MATRICES})
+
+
+def _in_8_bits(w: Any) -> Int8Weight:
+    return w if isinstance(w, Int8Weight) else Int8Weight.of(w)
+
+
+def _check_weights(weights: str, tp: int) -> None:
+    if weights not in ("bf16", "int8"):
+        raise ValueError(f"weights are 'bf16' or 'int8', not {weights!r}")
+    if weights == "int8" and int(tp) > 1:
+        raise NotImplementedError("weights='int8' runs on one GPU (tp = 1)")
+
 
 def interleave_rows(w1: torch.Tensor, w3: torch.Tensor) -> torch.Tensor:
     """[F, H], [F, H] → [2F, H] with row 2j = w1[j], row 2j+1 = w3[j]."""
@@ -130,11 +147,10 @@ class B200Engine:
 
         weights="int8": the layers and the head are held in 8 bits with a scale per output feature, and every token's activations are brought to 8 bits in front
         of each product (ops/int8.py): half the bytes in memory and per decoded token, twice the tensor-core rate for prompts.  One GPU (tp = 1); decoding runs the
-        per-op step (the whole-step kernel streams bf16)."""
-        if weights not in ("bf16", "int8"):
-            raise ValueError(f"weights are 'bf16' or 'int8', not {weights!r}")
-        if weights == "int8" and int(tp) > 1:
-            raise NotImplementedError("weights='int8' runs on one GPU (tp = 1)")
+        per-op step (the whole-step kernel streams bf16).  `layers` are left as they are; some or all may be in 8 bits already (`LayerWeights.in_8_bits`)."""
+        _check_weights(weights, tp)
+        if weights == "bf16" and any(isinstance(w, Int8Weight) for w in [lm_head] + [getattr(l, n) for l in layers for n in LayerWeights.MATRICES]):
+            raise ValueError("weights='bf16' with layers in 8 bits")
         self.config = config
         self.weights = weights
         self.tp, self.rank = int(tp), int(rank)
@@ -150,13 +166,10 @@ class B200Engine:
             raise ValueError("B200Engine needs CUDA tensors")
         _lib.lib()                                      # fail here, loudly, if the native library is absent
         self.embedding = embedding
-        self.layers = layers
         self.final_norm = final_norm
         if weights == "int8":
-            lm_head = Int8Weight.of(lm_head)
-            for l in layers:
-                for name in ("wqkv", "wo", "w13", "w2"):
-                    setattr(l, name, Int8Weight.of(getattr(l, name)))          # (one matrix at a time: its bf16 form is dropped)
+            lm_head, layers = _in_8_bits(lm_head), [l.in_8_bits() for l in layers]
+        self.layers = layers
         self.lm_head = lm_head
         self.use_cuda_graph = use_cuda_graph
         self.nh = config.num_attention_heads // self.tp          # local (per-rank) head counts
@@ -248,20 +261,25 @@ class B200Engine:
 
     # ------------------------------------------------------------------ construction
     @classmethod
-    def from_tree(cls, config: LLaMAConfig, params: Tree, **kw: Any) -> "B200Engine":
-        """Repack a canonical (``[in, out]``) tree that already lives on a CUDA device."""
+    def from_tree(cls, config: LLaMAConfig, params: Tree, *, device: Any = None, **kw: Any) -> "B200Engine":
+        """Repack a canonical (``[in, out]``) tree that lives on a CUDA device, or anywhere with `device`: it goes there layer by layer.  With weights="int8" a layer's bf16 form is dropped before the
+        next layer is built: a tree in host memory needs no more of the GPU than its 8-bit form, the embedding table and one layer (or the head)."""
+        int8 = kw.get("weights", "bf16") == "int8"
+        _check_weights(kw.get("weights", "bf16"), kw.get("tp", 1))
         t = params["transformer"]
-        bf = lambda x: x.to(torch.bfloat16)          # noqa: E731
+        bf = lambda x: x.to(device=device, dtype=torch.bfloat16)          # noqa: E731
         layers = []
         for i in range(config.num_hidden_layers):
             l = t["h"][str(i)]
             a, f = l["attention"], l["feed_forward"]
             wqkv = torch.cat([bf(a["wq"]["kernel"]).t(), bf(a["wk"]["kernel"]).t(), bf(a["wv"]["kernel"]).t()], 0)
-            layers.append(LayerWeights(
+            layer = LayerWeights(
                 attn_norm=bf(l["attention_norm"]["kernel"]).contiguous(), wqkv=wqkv.contiguous(),
                 wo=bf(a["wo"]["kernel"]).t().contiguous(), ffn_norm=bf(l["ffn_norm"]["kernel"]).contiguous(),
                 w13=interleave_rows(bf(f["w1"]["kernel"]).t(), bf(f["w3"]["kernel"]).t()),
-                w2=bf(f["w2"]["kernel"]).t().contiguous()))
+                w2=bf(f["w2"]["kernel"]).t().contiguous())
+            layers.append(layer.in_8_bits() if int8 else layer)
+            del layer, wqkv
         emb = bf(t["wte"]["embedding"]).contiguous()
         tp = int(kw.get("tp", 1))
         head = emb if config.tie_word_embeddings else bf(params["lm_head"]["kernel"]).t().contiguous()
@@ -282,6 +300,8 @@ class B200Engine:
         engine built with the same seed are the same model: `bench.py` uses that for its pre-run `tp_check`."""
         dev = torch.device(device)
         tp, rank = int(kw.get("tp", 1)), int(kw.get("rank", 0))
+        int8 = kw.get("weights", "bf16") == "int8"
+        _check_weights(kw.get("weights", "bf16"), tp)
         g = torch.Generator(device=dev).manual_seed(seed * 1000)
         std = config.initializer_range
         h, F, V = config.hidden_size, config.intermediate_size, config.vocab_size
@@ -307,7 +327,9 @@ class B200Engine:
             wo = cols(full(h, NH * hd), nh * hd)
             w13 = rows(full(2 * F, h), 2 * f)                  # (w1_j, w3_j) rows interleaved: a slice of 2f rows is f pairs
             w2 = cols(full(h, F), f)
-            layers.append(LayerWeights(ones(), wqkv_r, wo, ones(), w13, w2))
+            layer = LayerWeights(ones(), wqkv_r, wo, ones(), w13, w2)
+            layers.append(layer.in_8_bits() if int8 else layer)          # (a layer in bf16 at a time)
+            del layer, wqkv_r, wo, w13, w2
         ge = torch.Generator(device=dev).manual_seed(seed * 1000 + 999)      # same table on every rank
         emb = (torch.randn(V, h, generator=ge, device=dev, dtype=torch.float32) * std).to(torch.bfloat16)
         head = emb if (config.tie_word_embeddings and tp == 1) else rows(full(V, h), v)
