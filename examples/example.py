@@ -25,9 +25,11 @@ from jax_llama_b200.parallel.comm import init_distributed  # noqa: E402
 def load(ckpt_dir: str, tokenizer_path: str, is_llama3: bool, device: str = "auto", max_seq_len: int = 2048,
          **model_kwargs) -> LLaMA:
     """Checkpoint → ready-to-generate `LLaMA` (mirrors jax_example.load: mesh (1, n_devices) over 'dp','mp')."""
+    use_cuda = torch.cuda.is_available() and device != "cpu"
+    if model_kwargs.get("weights", "bf16") != "bf16" and not use_cuda:
+        raise SystemExit(f"weights={model_kwargs['weights']!r} needs a CUDA device")
     rank, world, local = init_distributed()
     tokenizer = LLaMA3Tokenizer(tokenizer_path) if is_llama3 else LLaMA2Tokenizer(tokenizer_path)
-    use_cuda = torch.cuda.is_available() and device != "cpu"
     mesh = Mesh({"dp": 1, "mp": world})
     if use_cuda:
         dev = torch.device("cuda", local)

@@ -82,7 +82,9 @@ class LLaMAPreTrainedModel:
         self.input_shape = input_shape
         self._params: Optional[Tree] = None
         self._engines: Dict[int, Tuple[Any, Any, Any]] = {}      # id(tree) → (weakref(leaf), version stamp, engine)
-        self.runtime_kwargs = kwargs            # tp / max_batch / kernel toggles, forwarded to the engine
+        self.runtime_kwargs = kwargs            # tp / max_batch / kernel toggles / weights, forwarded to the engine
+        if kwargs.get("weights", "bf16") not in ("bf16", "int8"):
+            raise ValueError(f"weights are 'bf16' or 'int8', not {kwargs['weights']!r}")
         if _do_init:
             self._params = self.init_weights(seed, input_shape, device=device)
 
@@ -116,6 +118,9 @@ class LLaMAPreTrainedModel:
         (``B200Engine.random_init`` in the benchmarks)."""
         pre = params.get("engine") if isinstance(params, dict) else None
         if pre is not None and not isinstance(pre, (dict, torch.Tensor)):
+            wanted, held = self.runtime_kwargs.get("weights"), getattr(pre, "weights", None)
+            if None not in (wanted, held) and wanted != held:
+                raise ValueError(f"a model with weights={wanted!r} on an engine with weights={held!r}")
             return pre
         leaves = list(_flatten(params).values())
         stamp = (len(leaves), tuple(int(t._version) for t in leaves))
@@ -130,11 +135,18 @@ class LLaMAPreTrainedModel:
         self._engines[key] = (weakref.ref(leaves[0]), stamp, eng)
         return eng
 
-    def _use_engine(self, params: Tree, output_attentions: bool, output_hidden_states: bool) -> bool:
-        if _tree_device(params).type != "cuda":
+    def _use_engine(self, params: Tree, output_attentions: bool = False, output_hidden_states: bool = False) -> bool:
+        """Whether the B200 engine answers, or the reference backend: that has the full weights only, so a model of 8-bit weights does not go there."""
+        int8 = self.runtime_kwargs.get("weights") == "int8"
+        dev = _tree_device(params)
+        if dev.type != "cuda":
+            if int8:
+                raise ValueError(f"weights='int8' is of the B200 engine: move the parameters to a CUDA device (they are on {dev})")
             return False
         if output_attentions or output_hidden_states:
             # flash kernels never materialise [B, nh, Q, K]; introspection requests take the unfused path
+            if int8:
+                raise NotImplementedError("output_attentions and output_hidden_states are of the full weights: a model with weights='int8' has none")
             return False
         return True
 
@@ -142,7 +154,7 @@ class LLaMAPreTrainedModel:
     def init_cache(self, batch_size: int, max_length: int, params: Optional[Tree] = None) -> KVCache:
         """Allocate an empty KV cache directly (no throw-away model init as in model.py:459-476)."""
         params = params if params is not None else self._params
-        if params is not None and _tree_device(params).type == "cuda":
+        if params is not None and self._use_engine(params):
             return self._engine_for(params).new_cache(batch_size, max_length)
         dtype = next(iter(_flatten(params).values())).dtype if params is not None else self.dtype
         dev = _tree_device(params) if params is not None else "cpu"
@@ -302,7 +314,7 @@ class LLaMAForCausalLM(LLaMAPreTrainedModel):
         if attention_mask is not None:
             attention_mask = torch.as_tensor(attention_mask).to(dev)
 
-        if dev.type == "cuda":
+        if self._use_engine(params):
             seqs = self._engine_for(params).generate(
                 input_ids, attention_mask, max_length=max_length, do_sample=do_sample,
                 temperature=temperature, top_k=top_k, top_p=top_p, pad_token_id=pad,
