@@ -184,7 +184,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, *, norm_w: Optional[torch.Tensor] =
     TMA-ring GEMV, which falls back when the activations do not fit next to its ring), otherwise the tcgen05
     GEMM (swap-AB up to M = 128, and to 256 with few features).  `force` ∈ {"gemv_tma", "gemv", "gemm"} pins the kernel.  Up to 128
     rows w is a parameter: it is read ahead of this library's kernels directly before the call, which must not write it.
-    An `int8.Int8Weight` for w makes it a layer in 8-bit integers (`int8.linear_int8`, with the same contract; no `force`)."""
+    An `int8.Int8Weight` for w makes it a layer in 8-bit integers (`int8.linear_int8`; no `force`): that is a parameter, read ahead, at any number of rows
+    (`linear_int8` with `resident=False` is for weights that are written directly before)."""
     if not isinstance(w, torch.Tensor):
         from .int8 import linear_int8
         if force is not None:

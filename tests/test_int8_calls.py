@@ -100,3 +100,16 @@ def test_rows_longer_than_they_may_be(monkeypatch):
         I.quantize_rows(torch.zeros(3, 8))
     K = (1 << 30) + 8                                           # (refused by the library ahead of any use of the device)
     assert _lib.lib().jl_int8_rows(0, 0, 1, K, K, 0, 1, 0, 1e-5, 0, K, 0, 0) != 0
+
+
+@pytest.mark.parametrize("M", [2, 128, 200, 3000])
+def test_weights_through_the_framework_are_parameters_at_any_number_of_rows(library, M):
+    """kernels.linear says that weights in 8 bits may be read ahead; linear_int8 reads them in turn unless it is told."""
+    from jax_llama_b200.ops import kernels as K
+    w = weight(32, 64)
+    x = on_gpu(torch.randn(M, 64))
+    assert "at any number of rows" in " ".join(K.linear.__doc__.split())
+    for call, resident in ((lambda: K.linear(x, w), True), (lambda: I.linear_int8(x, w), False)):
+        OnGpu.made = []
+        call()
+        assert library.calls[-1][1][-3] is resident
