@@ -212,7 +212,8 @@ __device__ __forceinline__ float2 i8_unpack(int kind, uint32_t w) {
   if (kind == DT_BF16) return make_float2(bf16_lo(w), bf16_hi(w));
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
-// silu(g) u.  The quotient is the product with an approximate reciprocal (two units in the last place): a true one branches, and values then wait for one another
+// silu(g) u.  The quotient is the product with an approximate reciprocal (two units in the last place): a true one branches, and values then wait for one another.  From
+// 1 + exp(-g) = 2^126 on the reciprocal is 0 and so is the result, where g e^g u is of less than 2^-119 |u|
 __device__ __forceinline__ float i8_gate(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
 // relu(y)^2; a NaN stays one

@@ -598,7 +598,7 @@ int jl_logit_rules(const void* logits, int dtype, int B, int V, int ld, float* o
  * jl_int8_rows: n rows of x [M, K] (row pitch ldx): row rows[i] (NULL: row i; one that x does not have: zeros), normed first where gain [K] (x's type) is given; q with row
  * pitch ldq, columns behind K zero; K <= 2^30.
  * jl_linear_int8: out [M, N] (gated: [M, N / 2]) = sx sw (qx qw^T) of the rows of x [M, K] and weights wq [N, ldw] / ws [N]; ldw a multiple of 16, the columns behind K not
- * used.  mode 0 plain, 1 + residual (out's type and size, may be out), 2 silu(y[2j]) y[2j+1], 3 relu(y)^2.  K <= 131072.  resident: no kernel directly before the call writes the weights.
+ * used.  mode 0 plain, 1 + residual (out's type and size, may be out), 2 silu(y[2j]) y[2j+1] (silu(y) is 0 from exp(-y) = 2^126 on), 3 relu(y)^2.  K <= 131072.  resident: no kernel directly before the call writes the weights.
  * jl_experts_int8: out[t], offsets[e] <= t < offsets[e + 1], of row rows[t] of x against expert e's weights wq [experts][N][ldw], ws [experts][N]; offsets [experts + 1] on
  * the device; other rows of out are left as they were.  mode 0, 2 or 3; experts <= 1024.
  * jl_choice_int8: out[m top + k] of row m of x against expert choice[m top + k] (zeros where there is none), without an order: M top <= 8, K <= 16384.
@@ -614,7 +614,7 @@ int jl_experts_int8(const void* x, int dtype, int M, int K, long long ldx, const
 int jl_choice_int8(const void* x, int dtype, int M, int K, long long ldx, const int* choice, int top, int experts, const void* wq, int ldw, const float* ws, int N,
                    void* out, int out_dtype, int mode, int num_sms, void* stream);
 /* The M * top (token, choice) pairs ordered by expert with nothing between experts: pos [M * top]: row of each pair (-1 where idx < 0); row_src [M * top]: token of each row
- * (-1 behind the last); offsets [E + 1]: first row of every expert, and behind the last. */
+ * (-1 behind the last); offsets [E + 1]: first row of every expert, and behind the last.  An expert's pairs are in any order among themselves. */
 int jl_moe_order(const int* idx, int M, int top, int E, int* pos, int* row_src, int* offsets, void* stream);
 
 #ifdef __cplusplus

@@ -193,7 +193,8 @@ def linear_int8(x: torch.Tensor, w: Int8Weight, *, norm_w: Optional[torch.Tensor
     """`kernels.linear` with 8-bit weights: [M, N] (SWIGLU: [M, N / 2]) in x's type, or fp32, from x [..., K] (bf16, fp16 or fp32), any M >= 0 and any N.
 
     The rows of x, normed first where norm_w is given, become int8 values and a scale each (`quantize_rows`), and y[m, n] = s_m s_n Σ q_mk q_nk.  mode: PLAIN; RESIDUAL adds
-    `residual` (of the result's type and size; `out` may be it); SWIGLU gives silu(y[2j]) · y[2j + 1] of interleaved rows; RELU2 relu(y)².  `resident`: w is a parameter that no kernel
+    `residual` (of the result's type and size; `out` may be it); SWIGLU gives silu(y[2j]) · y[2j + 1] of interleaved rows, where silu(y) is 0 from exp(-y) = 2^126 on (y below -87.3: it is less than 2^-119
+    there); RELU2 relu(y)².  `resident`: w is a parameter that no kernel
     directly before the call writes; it may then be read ahead of those."""
     who = "linear_int8"
     if w.__class__ is not Int8Weight or w.experts:
@@ -236,7 +237,7 @@ def linear_int8(x: torch.Tensor, w: Int8Weight, *, norm_w: Optional[torch.Tensor
 def expert_order(idx: torch.Tensor, E: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(pos int32 [M·top], rows int32 [M·top], offsets int32 [E + 1]) of the pairs idx int32 [M, top] ordered by expert, with nothing between experts: the row of
     every pair (-1 for a choice that is no expert's), the token of every row (-1 behind the last), the first row of every expert and, last, how many rows there are.
-    What `expert_linear_int8` takes."""
+    What `expert_linear_int8` takes.  An expert's pairs are in any order among themselves, on CUDA another one from call to call: `pos` is where each went."""
     who = "expert_order"
     if idx.dtype is not torch.int32 or idx.dim() != 2 or idx.shape[1] < 1 or not idx.is_contiguous() or E < 1:
         raise ValueError(f"{who}: choices are int32 [M, top], contiguous, at least one a token, of at least one expert (got {idx.dtype}, {tuple(idx.shape)}, {E} experts)")
