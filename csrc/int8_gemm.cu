@@ -313,9 +313,8 @@ static int i8s_slots(int num_sms) { return 2 * num_sms - 32; }
 // 256 x 6144 x 4096 16.8 -> 15.2; 512 x 1024 x 4096 14.2 -> 11.8.  One piece stays better for a long K: 256 x 4096 x 14336 23.1 and 25.6, 160 x 4096 x 4096 11.2 and 11.7; and two CTAs an SM
 // up to 80 rows over many features: 72 x 6144 x 4096 10.9 and 11.4.
 // Beyond 256 rows pieces of 128 as long as each can have an SM, whatever their number (us here | in pairs: 600 x 1024 x 4096 13.4 | 17.4; 1024 x 2048 x 4096 18.8 | 21.4; 4096 x 128 x
-// 8192 24.3 | 38.7; 333 x 6144 x 4096 16.4 | 18.9; 500 x 4608 x 4096 17.7 | 18.7; 8192 x 128 x 2048 16.0 | 17.4).
-// Pairs otherwise (130 x 4096 x 4096 10.7 | 16.3; 512 x 4096 x 4096 17.2 | 18.3; K short: 200 x 1024 x 1024 9.3 | 6.9; 333 x 1000 x 960 9.0 | 7.3; many tiles: 256 x 28672 x 4096
-// 45 | 32, 512 x 6144 x 4096 19.4 | 18.8).
+// 8192 24.3 | 38.7; 333 x 6144 x 4096 16.4 | 18.9; 500 x 4608 x 4096 17.7 | 18.7; 8192 x 128 x 2048 16.0 | 17.4; in fewer pieces, K in parts, 130 x 4096 x 4096 10.7 | 16.3, 512 x 4096 x 4096 17.2 | 18.3).
+// Pairs otherwise: K short (200 x 1024 x 1024 9.3 | 6.9, 333 x 1000 x 960 9.0 | 7.3) or many tiles (256 x 28672 x 4096 45 | 32, 512 x 6144 x 4096 19.4 | 18.8).
 struct Int8Cut { int pieces, parts, wide; };
 static Int8Cut i8s_cut(int M, int N, int K, int num_sms) {
   const int cols = (N + I8S_BM - 1) / I8S_BM, kb = (K + I8S_BK - 1) / I8S_BK, both = i8s_slots(num_sms), one = num_sms - 20;

@@ -5,8 +5,9 @@
 // where the instruction's table names 4 + 4 + 4 + 4 apart, so all accesses are 16 bytes.  Two pieces, 8 KB a warp, are under way while one is multiplied, across
 // units; the warps' partial sums meet in shared memory, one barrier a unit, whole numbers, in any order the same.
 // Every CTA brings the activations to 8 bits itself while its first weights are under way, which saves a launch.
-// Bound by latency, then the weights: one B200, us in a chain of cold weights, 1 x 64 x 256 2.9, 1 x 64 x 4096 3.7, 1 x 2048 x 4096 gated 4.5, 1 x 4096 x 4096 5.7 (2.6 at the memory's rate).
-// A mixture of experts: a CTA has one of up to eight rows and finds whose it is; a token's four of 32 experts of 2048 x 2048 8.6 (2.6 at the memory's rate): its weights wait for the router.
+// Bound by latency, then the weights: one B200, us in a chain of cold weights, 1 x 64 x 256 2.5, 1 x 64 x 4096 3.0, 1 x 2048 x 4096 gated 3.9, 1 x 4096 x 4096 5.3 (2.6 at the memory's rate); behind a
+// norm a pass over the row more, 1 x 64 x 4096 4.4, 1 x 6144 x 4096 8.5 (3.8), 8 x 2048 x 2048 9.95 (5.4 without).
+// A mixture of experts: a CTA has one of up to eight rows and finds whose it is; a token's four of 32 experts of 2048 x 2048 7.7, by choice 7.2 (2.6 at the memory's rate): its weights wait for the router.
 // One CTA an SM, which would let the next launch's first weights in, streams too little: 1 x 28672 x 4096 22 -> 35.
 #include "int8.cuh"
 #include "jllama_b200.h"

@@ -6,10 +6,11 @@
 // memory, so that a warp's stores are whole lines.
 // Bound by the products and, in seconds of them, the power cap: one B200, us, 2048 x 9216 x 4096 60 (54 without loads, 47 without products), 8192 x 28672 x 4096 gated 718 (2680 TOP/s at
 // 1.45 GHz); with few k-blocks by the epilogue: 8192 x 2048 x 128 13.9 (18.5 with scales from memory in the epilogue), gated 8192 x 4096 x 128 27 (32; 36 with a true quotient per
-// gate).  Rings of 3, 4, 5 stages: 2048 x 9216 x 4096 69, 62, 59; six gave nothing more.
+// gate; issue slots 43 %, tensor pipe 6 %: eight warps, each one chain from
+// accumulator to store).  Rings of 3, 4, 5 stages: 2048 x 9216 x 4096 69, 62, 59; six gave nothing more.
 // One matrix, or one per expert (rows ordered by expert, at any row): what a tile holds of the next expert's rows is computed and not stored.  (Rows of
 // several experts held once and gathered by the loads, `tile::gather4`: 8192 tokens x 4 of 32 experts of 2048 x 2048 410 us, with the rows written out by the kernel that
-// brings them to 8 bits 145.)
+// brings them to 8 bits 144.)
 #include <atomic>
 
 #include "int8.cuh"
