@@ -113,7 +113,8 @@ def quantize_rows(x: torch.Tensor, *, norm_w: Optional[torch.Tensor] = None, eps
 # --------------------------------------------------------------------------- weights
 class Int8Weight:
     """Weights [N, K], or [E, N, K] of E experts, as int8 values and fp32 scales [N] / [E, N].  Rows lie on 16-byte boundaries (a copy is made where K is not a multiple
-    of 16).  A SWIGLU layer's rows are interleaved: row 2j is the gate of result j, row 2j + 1 its up part (`models.engine.interleave_rows`)."""
+    of 16).  A SWIGLU layer's rows are interleaved: row 2j is the gate of result j, row 2j + 1 its up part (`models.engine.interleave_rows`).  Calls use the addresses of
+    values and scales: new numbers are written into those, and no field is assigned."""
 
     __slots__ = ("values", "scales", "experts", "n", "k", "pitch", "device", "dev", "_held")
 
@@ -135,6 +136,15 @@ class Int8Weight:
         self.device, self.dev = values.device, values.get_device()
         # what a call hands to the library: (values, row pitch, scales, features), and the SMs there are (asked once: a layer is called for every token)
         self._held = (values.data_ptr(), pitch, self.scales.data_ptr(), self.n), num_sms(self.device) if self.dev >= 0 else 0
+
+    def __setattr__(self, name: str, value: object) -> None:
+        if hasattr(self, "_held"):
+            raise AttributeError(f"Int8Weight: {name} is not assigned once it is laid out (write into its values and scales, or make another one)")
+        object.__setattr__(self, name, value)
+
+    def __reduce__(self) -> tuple:
+        """Copied and pickled as values and scales: the copy is laid out where its own are."""
+        return Int8Weight, (self.values, self.scales)
 
     @classmethod
     def of(cls, w: torch.Tensor) -> "Int8Weight":

@@ -1,4 +1,6 @@
 """How the functions of 8-bit layers call the library: on the CPU, with a stand-in for its entry points."""
+import copy
+import io
 import weakref
 
 import pytest
@@ -66,7 +68,7 @@ def on_gpu(t):
 
 def weight(*shape):
     w = I.Int8Weight(torch.ones(shape, dtype=torch.int8), torch.ones(shape[:-1]))
-    w.dev = 0
+    object.__setattr__(w, "dev", 0)
     return w
 
 
@@ -113,3 +115,26 @@ def test_weights_through_the_framework_are_parameters_at_any_number_of_rows(libr
         OnGpu.made = []
         call()
         assert library.calls[-1][1][-3] is resident
+
+
+@pytest.mark.parametrize("shape", [(4, 16), (3, 6, 20)])
+def test_copies_of_weights_have_their_own_addresses(shape):
+    """What a call hands to the library are addresses: those of a copy, or of weights that were stored and loaded, are not the first one's."""
+    w = I.Int8Weight.of(torch.randn(shape))
+    room = io.BytesIO()
+    torch.save(w, room)
+    room.seek(0)
+    for other in (copy.deepcopy(w), torch.load(room, weights_only=False)):
+        assert torch.equal(other.values, w.values) and torch.equal(other.scales, w.scales) and (other.n, other.k, other.pitch, other.experts) == (w.n, w.k, w.pitch, w.experts)
+        assert other.values.data_ptr() != w.values.data_ptr()
+        assert other._held[0] == (other.values.data_ptr(), other.pitch, other.scales.data_ptr(), other.n)
+        assert other.values.stride(-2) == other.pitch and other.values.data_ptr() % 16 == 0
+
+
+def test_fields_of_weights_are_not_assigned():
+    w = I.Int8Weight.of(torch.randn(4, 16))
+    for name in ("values", "scales", "k", "_held"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, getattr(w, name))
+    w.values.zero_()                                            # (written into, they are what calls read)
+    assert not I.linear_int8(torch.randn(2, 16), w).any()
