@@ -75,7 +75,8 @@ def quantize_rows(x: torch.Tensor, *, norm_w: Optional[torch.Tensor] = None, eps
                   out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(values int8 [..., K], scales fp32 [...]) of the rows of x [..., K] (bf16, fp16 or fp32; two dimensions: any row pitch).  Both are what 64 bits would give: the
     scale is amax / 127 rounded once, a value is the whole number nearest to 127 x / amax.  At most MAX_ROWS rows of MAX_COLUMNS.  A row of zeros has scale 0; a row that holds an infinity or a NaN has scale
-    NaN and values 0, so that what it is multiplied with is NaN.  With norm_w the rows are normed first (RMS, fp32, no rounding in between)."""
+    NaN and values 0, so that what it is multiplied with is NaN.  With norm_w the rows are normed first (RMS, fp32, no rounding in between), on CUDA with the
+    same bits beside any rows; of what fp32 leaves, a value whose quotient is next to a middle may be the neighbour of the one of 64 bits."""
     who = "quantize_rows"
     if x.dim() < 1:
         raise ValueError(f"{who}: x has no rows")
