@@ -215,6 +215,7 @@ __global__ void __launch_bounds__(i8r_threads(G)) int8_rows_kernel(const Int8Row
     static_assert(16 * G == I8R_PIECES, "the order of the sum");
     const int pieces = (p.K + VE - 1) / VE;
     auto at = [&](const T* v, int c, int off) {
+      if (v == nullptr) return make_uint4(0, 0, 0, 0);               // (a row that is not there)
       if (off == 0 || c < off || c - off + 2 * VE > p.K) return i8r_load(v, c, off == 0 ? p.K : 0, p.K);
       return i8r_turn<T>(*reinterpret_cast<const uint4*>(v + c - off), *reinterpret_cast<const uint4*>(v + c - off + VE), off);
     };

@@ -100,3 +100,25 @@ def test_rows_that_hold_nothing_or_no_numbers(K):
     x[0], x[1, K // 2], x[2, K - 1] = 0, float("nan"), float("inf")
     q, s = I.quantize_rows(x, norm_w=g)
     assert s[0] == 0 and torch.isnan(s[1:3]).all() and not q[:3].any() and torch.isfinite(s[3:]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("K", [40, 1001, 8192, 20001, 40000])
+@pytest.mark.parametrize("n", [9, 700])
+def test_chosen_rows_behind_a_norm(dtype, K, n):
+    """The library's own entry point takes an index with gains: rows in any order, and zeros for those that are not there."""
+    from jax_llama_b200.ops import _lib
+    I, _ = _ops()
+    x, g = _randn(9, K, seed=K, dtype=dtype), _randn(K, seed=1, dtype=dtype)
+    index = torch.randint(-2, 12, (n,), generator=torch.Generator().manual_seed(K)).to(torch.int32)
+    index[:3] = torch.tensor([-1, 9, 4])
+    q, s = torch.full((n, K), 5, dtype=torch.int8, device=DEV), torch.full((n,), 5.0, device=DEV)
+    rows = index.to(DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _lib.lib().jl_int8_rows(x.data_ptr(), I.TYPES[dtype], 9, K, K, rows.data_ptr(), n, g.data_ptr(), 1e-5, q.data_ptr(), K, s.data_ptr(), stream) == 0
+    p, r = I.quantize_rows(x, norm_w=g)
+    there = (index >= 0) & (index < 9)
+    at = index[there].long().to(DEV)
+    there = there.to(DEV)
+    assert torch.equal(q[there], p[at]) and torch.equal(s[there], r[at])
+    assert not q[~there].any() and not s[~there].any()
