@@ -161,7 +161,8 @@ def test_the_engine(name, B, S, monkeypatch):
         else:
             q, s, near = rows_behind_a_norm(x0, norm, eps)
             y = O.products(q, s, wq, ws)
-            extra = (near @ wq.abs().t()) * s[:, None] * ws.double() + 19 * U * y.abs()
+            # (a value that is the neighbour counts with the scale as it came out, and is rounded with the rest: 19 + 4 of U more)
+            extra = (near @ wq.abs().t()) * s[:, None] * ws.double() * (1 + 23 * U) + 19 * U * y.abs()
         bound = O.bound_gated(y, dtype, extra=extra) if gated else O.bound(y, dtype, residual=None if residual is None else residual.view(y.shape), extra=extra)
         within(out.view(bound[1].shape), *bound)
         return out
